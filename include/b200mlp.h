@@ -377,6 +377,30 @@ int b2_site_report(const b2_handle* h, int* tensor_core_sites, int* cuda_core_si
  * tensor-core GEMMs of its steps. (GEMMs of B2_PREC_FP32 count in `total` only, on whichever unit they run.) */
 int b2_launch_counts(const b2_handle* h, long long* total, long long* tensor_core);
 
+/* ---- Operators around the layers of a language model: token input, loss over a vocabulary, weight update.
+ * The reference has no counterpart (its inputs are dense, its loss is quadratic, its update is SGD). They need no
+ * handle: all matrices are caller-owned DEVICE memory of the calling thread's current device, row-major with a leading
+ * dimension in ELEMENTS, of dtype B2_DTYPE_F32 or B2_DTYPE_BF16 throughout a call; `stream` is a cudaStream_t (NULL =
+ * default stream), on which a call queues its work and returns without waiting, allocating or synchronising, so that it
+ * may be captured. A workspace is caller-owned device memory of at least the size that the operator's *_workspace()
+ * function gives, on a 256-byte boundary, whose contents nothing keeps between calls; calls that may overlap on the GPU
+ * need one each. Errors are returned as everywhere, with the text in b2_last_error(NULL); a bad argument is
+ * refused before anything is queued. Outputs may not overlap inputs, except where a matrix is said to be updated.
+ * Tokens and targets are 32- or 64-bit integers (token_bytes 4 or 8) in device memory; one outside [0, vocab) is
+ * padding: an embedding row of zeros, no gradient, no loss. */
+
+/* out[i] = scale * table[tokens[i]], n rows of `width` elements. Any leading dimension and alignment of whole elements;
+ * fastest where rows are whole 16-byte pieces. */
+int b2_embed(const void* tokens, int token_bytes, size_t n, const void* table, int dtype, size_t vocab, size_t width,
+             size_t ld_table, float scale, void* out, size_t ld_out, void* stream);
+/* Its gradient: dtable[v] = scale * sum of dout[i] over the i with tokens[i] = v, for all v in [0, vocab) (rows of tokens
+ * that do not occur are written as zeros). Sums run in fp32 over tokens sorted by (token, position), and equal inputs
+ * give equal bits. */
+int b2_embed_grad_workspace(size_t n, size_t vocab, size_t width, size_t* bytes);
+int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dout, int dtype, size_t ld_dout,
+                  size_t vocab, size_t width, float scale, void* dtable, size_t ld_dtable, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -35,7 +35,8 @@ class Config(C.Structure):
 
 
 # every symbol include/b200mlp.h declares: name -> (restype, argtypes)
-_H = C.c_void_p
+_H = _vp = C.c_void_p
+_sz = C.c_size_t
 SYMBOLS = {
     "b2_config_default": (C.c_int, [C.POINTER(Config)]),
     "b2_version": (C.c_char_p, []),
@@ -90,6 +91,9 @@ SYMBOLS = {
     "b2_write_trace": (C.c_int, [_H, C.c_char_p]),
     "b2_site_report": (C.c_int, [_H, C.POINTER(C.c_int), C.POINTER(C.c_int), C.c_char_p, C.c_size_t]),
     "b2_launch_counts": (C.c_int, [_H, C.POINTER(C.c_longlong), C.POINTER(C.c_longlong)]),
+    "b2_embed": (C.c_int, [_vp, C.c_int, _sz, _vp, C.c_int, _sz, _sz, _sz, C.c_float, _vp, _sz, _vp]),
+    "b2_embed_grad_workspace": (C.c_int, [_sz, _sz, _sz, C.POINTER(_sz)]),
+    "b2_embed_grad": (C.c_int, [_vp, C.c_int, _sz, _vp, C.c_int, _sz, _sz, _sz, C.c_float, _vp, _sz, _vp, _sz, _vp]),
 }
 
 _lib = None

@@ -13,6 +13,7 @@ import glob
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -51,13 +52,12 @@ def build_cuda(force=False, verbose=False, ptxas_info=False):
         glob.glob(os.path.join(ROOT, "include", "*.h"))
     if not force and not _stale(LIB, deps):
         return LIB
-    objs = []
-    for s in srcs:
-        o = s[:-3] + ".o"
-        if force or _stale(o, deps):
-            cmd = [NVCC] + NVCC_FLAGS + (["-Xptxas", "-v"] if ptxas_info else []) + ["-c", s, "-o", o]
-            _run(cmd, verbose or ptxas_info)
-        objs.append(o)
+    headers = [d for d in deps if d not in srcs]
+    objs = [s[:-3] + ".o" for s in srcs]
+    cmds = [[NVCC] + NVCC_FLAGS + (["-Xptxas", "-v"] if ptxas_info else []) + ["-c", s, "-o", o]
+            for s, o in zip(srcs, objs) if force or _stale(o, [s] + headers)]
+    with ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+        list(pool.map(lambda c: _run(c, verbose or ptxas_info), cmds))
     _run([NVCC, "-shared", "-o", LIB] + objs + ["-ldl", "-ccbin", CXX], verbose)
     return LIB
 

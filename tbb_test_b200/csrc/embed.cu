@@ -1,0 +1,564 @@
+// Rows of a table by token number, scaled, and the table's gradient:
+//
+//   out[i]   = scale * table[t_i]                     (zeros where t_i is outside [0, vocab))
+//   dtable[v] = scale * sum over i with t_i = v of dout[i]
+//
+// Both are bound by HBM: the forward pass reads and writes n rows, the gradient reads n rows and writes vocab rows.
+//
+// The gradient sorts (token, position) pairs and adds each token's rows in the order of their positions, in fp32, so
+// that its bits do not depend on the order in which blocks run; no float is added by an atomic. The sorted list is cut
+// into chunks of equal length, one group of threads per chunk and slice of columns, so that a token that makes up
+// a tenth of a batch takes no longer than many rare ones. A run of one token inside a chunk is finished there. One that
+// crosses chunk borders leaves a partial sum per chunk, and a second kernel adds these in order. The rows of tokens that do
+// not occur are zeroed by blocks of the first kernel, which look the token up in the sorted list.
+#include "lm.cuh"
+
+namespace b2 {
+namespace {
+
+constexpr int EMBED_THREADS = 256;
+
+template <typename T, int VB, int U>
+__global__ void __launch_bounds__(EMBED_THREADS) embed_kernel(const void* __restrict__ tokens, int wide, size_t n,
+                                                              const char* __restrict__ table, unsigned int vocab,
+                                                              int vecs, size_t ld_table, float scale,
+                                                              char* __restrict__ out, size_t ld_out, int tpr_log2) {
+  typedef Elems<T, VB> E;
+  typedef typename E::raw raw;
+  const int col0 = threadIdx.x & ((1 << tpr_log2) - 1), sub = threadIdx.x >> tpr_log2;
+  const int group = EMBED_THREADS >> tpr_log2;
+  const size_t row0 = (size_t)blockIdx.x * group * U + sub;
+  unsigned int t[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const size_t r = row0 + (size_t)u * group;
+    t[u] = r < n ? token_at(tokens, wide, r, vocab) : vocab;
+  }
+  for (int c = col0; c < vecs; c += 1 << tpr_log2) {
+    raw v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {  // U loads in flight
+      memset(&v[u], 0, sizeof(raw));
+      if (t[u] < vocab) v[u] = __ldg(reinterpret_cast<const raw*>(table + t[u] * ld_table) + c);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const size_t r = row0 + (size_t)u * group;
+      if (r >= n) continue;
+      float f[E::N];
+      E::get(v[u], f);
+#pragma unroll
+      for (int i = 0; i < E::N; ++i) f[i] = t[u] < vocab ? f[i] * scale : 0.f;
+      reinterpret_cast<raw*>(out + r * ld_out)[c] = E::put(f);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ sorting (token, position)
+
+// Short lists: an element's place is the number of elements that sort before it. Every block holds all keys in shared
+// memory and each warp counts for four elements at once.
+constexpr int RANK_MOST = 8192;
+constexpr int RANK_THREADS = 256, RANK_PER_WARP = 4;
+__global__ void __launch_bounds__(RANK_THREADS) rank_sort_kernel(const void* __restrict__ tokens, int wide, int n,
+                                                                 unsigned int vocab, unsigned int* __restrict__ keys,
+                                                                 unsigned int* __restrict__ pos) {
+  extern __shared__ unsigned int key_s[];
+  for (int i = threadIdx.x; i < n; i += RANK_THREADS) key_s[i] = token_at(tokens, wide, i, vocab);
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  const int i0 = (blockIdx.x * (RANK_THREADS / 32) + (threadIdx.x >> 5)) * RANK_PER_WARP;
+  unsigned int key[RANK_PER_WARP], before[RANK_PER_WARP];
+#pragma unroll
+  for (int u = 0; u < RANK_PER_WARP; ++u) {
+    key[u] = i0 + u < n ? key_s[i0 + u] : 0u;
+    before[u] = 0;
+  }
+  for (int j = lane; j < n; j += 32) {
+    const unsigned int k = key_s[j];
+#pragma unroll
+    for (int u = 0; u < RANK_PER_WARP; ++u) before[u] += k < key[u] + (j < i0 + u ? 1u : 0u);  // equal keys: by position
+  }
+#pragma unroll
+  for (int u = 0; u < RANK_PER_WARP; ++u) {
+    const unsigned int r = __reduce_add_sync(0xFFFFFFFFu, before[u]);
+    if (lane == 0 && i0 + u < n) {
+      keys[r] = key[u];
+      pos[r] = i0 + u;
+    }
+  }
+}
+
+// Longer ones: a stable radix sort, lowest digit first, of at most RADIX_TILES tiles of consecutive elements, so that a
+// block finds its digits' first places by reading all tiles' counts itself instead of after a third launch per digit.
+constexpr int RADIX_THREADS = 512, RADIX_WARPS = RADIX_THREADS / 32, RADIX_ROUNDS = 8;
+constexpr int RADIX_STEP = RADIX_THREADS * RADIX_ROUNDS;  // elements a block places at a time
+constexpr int RADIX_TILES = 64, RADIX_MOST_BITS = 10;
+
+struct RadixPass {
+  const void* tokens;  // first pass: keys come from here and positions are their index
+  int wide;
+  unsigned int vocab;
+  const unsigned int *keys, *pos;
+  unsigned int *keys_out, *pos_out;
+  unsigned int* counts;  // tiles x bins
+  unsigned int n, tile;  // elements, elements per tile (a multiple of RADIX_STEP)
+  int tiles, shift, bits;
+};
+__device__ __forceinline__ unsigned int radix_key(const RadixPass& p, unsigned int i) {
+  return p.tokens ? token_at(p.tokens, p.wide, i, p.vocab) : p.keys[i];
+}
+
+__global__ void __launch_bounds__(RADIX_THREADS) radix_count_kernel(const RadixPass p) {
+  __shared__ unsigned int count[1 << RADIX_MOST_BITS];
+  const int bins = 1 << p.bits;
+  for (int b = threadIdx.x; b < bins; b += RADIX_THREADS) count[b] = 0;
+  __syncthreads();
+  const unsigned int begin = blockIdx.x * p.tile, end = min(p.n, begin + p.tile);
+  for (unsigned int i = begin + threadIdx.x; i < end; i += RADIX_THREADS)
+    atomicAdd(&count[(radix_key(p, i) >> p.shift) & (bins - 1)], 1u);
+  __syncthreads();
+  for (int b = threadIdx.x; b < bins; b += RADIX_THREADS) p.counts[(size_t)blockIdx.x * bins + b] = count[b];
+}
+
+__global__ void __launch_bounds__(RADIX_THREADS) radix_place_kernel(const RadixPass p) {
+  __shared__ unsigned int next[1 << RADIX_MOST_BITS];  // where this tile's next element of a digit goes
+  __shared__ unsigned short seen[RADIX_WARPS][1 << RADIX_MOST_BITS];
+  __shared__ unsigned int warp_sum[RADIX_WARPS];
+  const int bins = 1 << p.bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // exclusive sum over digits of all tiles' counts, plus the counts of the tiles before this one
+  unsigned int running = 0;
+  for (int b0 = 0; b0 < bins; b0 += RADIX_THREADS) {
+    const int b = b0 + threadIdx.x;
+    unsigned int total = 0, before = 0;
+    if (b < bins)
+      for (int t = 0; t < p.tiles; ++t) {
+        const unsigned int c = p.counts[(size_t)t * bins + b];
+        total += c;
+        before += t < (int)blockIdx.x ? c : 0u;
+      }
+    unsigned int scan = total;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const unsigned int up = __shfl_up_sync(0xFFFFFFFFu, scan, d);
+      if (lane >= d) scan += up;
+    }
+    if (lane == 31) warp_sum[warp] = scan;
+    __syncthreads();
+    unsigned int base = running, all = 0;
+    for (int w = 0; w < RADIX_WARPS; ++w) {
+      base += w < warp ? warp_sum[w] : 0u;
+      all += warp_sum[w];
+    }
+    if (b < bins) next[b] = base + scan - total + before;
+    running += all;
+    __syncthreads();
+  }
+  const unsigned int begin = blockIdx.x * p.tile, end = min(p.n, begin + p.tile);
+  for (unsigned int step = begin; step < end; step += RADIX_STEP) {
+    for (int i = threadIdx.x; i < RADIX_WARPS * bins; i += RADIX_THREADS) seen[i >> p.bits][i & (bins - 1)] = 0;
+    __syncthreads();
+    // a warp places 256 consecutive elements, 32 at a time: equal digits of a round keep the order of the lanes
+    unsigned int key[RADIX_ROUNDS], pos[RADIX_ROUNDS], place[RADIX_ROUNDS];
+    const unsigned int first = step + warp * 32 * RADIX_ROUNDS + lane;
+#pragma unroll
+    for (int r = 0; r < RADIX_ROUNDS; ++r) {
+      const unsigned int i = first + r * 32;
+      key[r] = i < end ? radix_key(p, i) : 0u;
+      pos[r] = i < end ? (p.tokens ? i : p.pos[i]) : 0u;
+    }
+#pragma unroll
+    for (int r = 0; r < RADIX_ROUNDS; ++r) {
+      const bool in = first + r * 32 < end;
+      const unsigned int digit = (key[r] >> p.shift) & (bins - 1);
+      const unsigned int same = __match_any_sync(0xFFFFFFFFu, in ? digit : 0xFFFFFFFFu);
+      const unsigned int old = in ? seen[warp][digit] : 0u;
+      place[r] = old + __popc(same & ((1u << lane) - 1));
+      __syncwarp();
+      if (in && lane == __ffs(same) - 1) seen[warp][digit] = (unsigned short)(old + __popc(same));
+      __syncwarp();
+    }
+    __syncthreads();
+    unsigned int moved[(1 << RADIX_MOST_BITS) / RADIX_THREADS];
+#pragma unroll
+    for (int k = 0; k < (1 << RADIX_MOST_BITS) / RADIX_THREADS; ++k) {
+      const int b = k * RADIX_THREADS + threadIdx.x;
+      moved[k] = 0;
+      if (b < bins)
+        for (int w = 0; w < RADIX_WARPS; ++w) {
+          const unsigned int c = seen[w][b];
+          seen[w][b] = (unsigned short)moved[k];
+          moved[k] += c;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < RADIX_ROUNDS; ++r)
+      if (first + r * 32 < end) {
+        const unsigned int digit = (key[r] >> p.shift) & (bins - 1);
+        const unsigned int to = next[digit] + seen[warp][digit] + place[r];
+        p.keys_out[to] = key[r];
+        p.pos_out[to] = pos[r];
+      }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < (1 << RADIX_MOST_BITS) / RADIX_THREADS; ++k) {
+      const int b = k * RADIX_THREADS + threadIdx.x;
+      if (b < bins) next[b] += moved[k];
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------ sums of runs
+
+struct RunSum {
+  const unsigned int *keys, *pos;  // sorted; positions without a token carry key = vocab and stand last
+  unsigned int n, vocab, chunk;    // chunk: sorted elements per chunk
+  unsigned int chunks;
+  const char* dout;
+  size_t ld_dout;  // bytes
+  char* dtable;
+  size_t ld_dtable;
+  float *head, *tail;  // chunks x pitch partial sums: of the run that came from the chunk before, and of the one that goes on
+  size_t pitch;        // floats per partial row
+  float scale;
+  int vecs, slices, tpr_log2;
+  unsigned int sum_blocks;
+};
+
+// First index whose key is >= `key`.
+__device__ __forceinline__ unsigned int lower_bound(const unsigned int* keys, unsigned int n, unsigned int key) {
+  unsigned int lo = 0, hi = n;
+  while (lo < hi) {
+    const unsigned int mid = (lo + hi) >> 1;
+    if (__ldg(keys + mid) < key) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+constexpr int RUN_THREADS = 128, RUN_AHEAD = 8;
+template <typename T, int VB>
+__global__ void __launch_bounds__(RUN_THREADS) run_sum_kernel(const RunSum p) {
+  typedef Elems<T, VB> E;
+  typedef typename E::raw raw;
+  if (blockIdx.x >= p.sum_blocks) {  // rows of tokens that do not occur
+    const int lane = threadIdx.x & 31;
+    const unsigned int v0 = (blockIdx.x - p.sum_blocks) * RUN_THREADS + (threadIdx.x & ~31u);
+    const unsigned int v = v0 + lane;
+    bool absent = false;
+    if (v < p.vocab) {
+      const unsigned int at = lower_bound(p.keys, p.n, v);
+      absent = at == p.n || __ldg(p.keys + at) != v;
+    }
+    unsigned int rows = __ballot_sync(0xFFFFFFFFu, absent);
+    raw zero;
+    memset(&zero, 0, sizeof zero);
+    for (; rows; rows &= rows - 1) {
+      raw* row = reinterpret_cast<raw*>(p.dtable + (size_t)(v0 + __ffs(rows) - 1) * p.ld_dtable);
+      for (int c = lane; c < p.vecs; c += 32) row[c] = zero;
+    }
+    return;
+  }
+  const int tpr = 1 << p.tpr_log2;
+  const unsigned int unit = blockIdx.x * (RUN_THREADS >> p.tpr_log2) + (threadIdx.x >> p.tpr_log2);
+  const unsigned int chunk = unit / p.slices;
+  const int col = (int)(unit - chunk * p.slices) * tpr + (threadIdx.x & (tpr - 1));
+  if (chunk >= p.chunks || col >= p.vecs) return;
+  const unsigned int begin = chunk * p.chunk, end = min(p.n, begin + p.chunk);
+  unsigned int cur = __ldg(p.keys + begin);
+  bool from_before = begin > 0 && __ldg(p.keys + begin - 1) == cur;
+  float acc[E::N];
+#pragma unroll
+  for (int j = 0; j < E::N; ++j) acc[j] = 0.f;
+  auto finish = [&](bool goes_on) {
+    if (from_before || goes_on) {
+      float* to = (from_before ? p.head : p.tail) + (size_t)chunk * p.pitch + (size_t)col * E::N;
+#pragma unroll
+      for (int j = 0; j < E::N; ++j) to[j] = acc[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < E::N; ++j) acc[j] *= p.scale;
+      reinterpret_cast<raw*>(p.dtable + (size_t)cur * p.ld_dtable)[col] = E::put(acc);
+    }
+  };
+  for (unsigned int i = begin; i < end && cur < p.vocab; i += RUN_AHEAD) {
+    unsigned int key[RUN_AHEAD];
+    raw v[RUN_AHEAD];
+#pragma unroll
+    for (int u = 0; u < RUN_AHEAD; ++u) {
+      key[u] = i + u < end ? __ldg(p.keys + i + u) : p.vocab;
+      memset(&v[u], 0, sizeof(raw));
+      if (key[u] < p.vocab) v[u] = __ldg(reinterpret_cast<const raw*>(p.dout + (size_t)__ldg(p.pos + i + u) * p.ld_dout) + col);
+    }
+#pragma unroll
+    for (int u = 0; u < RUN_AHEAD; ++u) {
+      if (key[u] != cur) {
+        if (i + u < end) {
+          finish(false);
+          cur = key[u];
+          from_before = false;
+#pragma unroll
+          for (int j = 0; j < E::N; ++j) acc[j] = 0.f;
+        }
+        if (key[u] >= p.vocab) break;
+      }
+      float f[E::N];
+      E::get(v[u], f);
+#pragma unroll
+      for (int j = 0; j < E::N; ++j) acc[j] += f[j];
+    }
+  }
+  if (cur < p.vocab) finish(end < p.n && __ldg(p.keys + end) == cur);
+}
+
+// Runs that cross chunk borders: the chunk a run begins in adds its tail and the heads of the chunks behind it,
+// JOIN_PARTS contiguous shares of them side by side, which are then added in order.
+constexpr int JOIN_PARTS = 8;
+template <typename T>
+__global__ void __launch_bounds__(32 * JOIN_PARTS) run_join_kernel(const RunSum p, int width) {
+  __shared__ float part[JOIN_PARTS][32];
+  const unsigned int chunk = blockIdx.x;
+  const unsigned int begin = chunk * p.chunk, end = begin + p.chunk;
+  if (end >= p.n) return;
+  const unsigned int key = __ldg(p.keys + end);
+  if (key >= p.vocab || __ldg(p.keys + end - 1) != key) return;                                    // nothing goes on
+  if (begin > 0 && __ldg(p.keys + begin) == key && __ldg(p.keys + begin - 1) == key) return;  // it began earlier
+  const unsigned int last = (lower_bound(p.keys, p.n, key + 1) - 1) / p.chunk;
+  const unsigned int count = last - chunk + 1;
+  const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
+  const unsigned int from = (unsigned int)((size_t)count * share / JOIN_PARTS), to = (unsigned int)((size_t)count * (share + 1) / JOIN_PARTS);
+  for (int c0 = blockIdx.y * 32; c0 < width; c0 += gridDim.y * 32) {
+    const int c = c0 + lane;
+    float sum = 0.f;
+    if (c < width)
+#pragma unroll 8
+      for (unsigned int k = from; k < to; ++k) sum += (k == 0 ? p.tail : p.head)[(size_t)(chunk + k) * p.pitch + c];
+    part[share][lane] = sum;
+    __syncthreads();
+    if (share == 0 && c < width) {
+      for (int s = 1; s < JOIN_PARTS; ++s) sum += part[s][lane];
+      reinterpret_cast<T*>(p.dtable + (size_t)key * p.ld_dtable)[c] = (T)(sum * p.scale);
+    }
+    __syncthreads();
+  }
+}
+
+int log2_ceil(size_t v) {
+  int b = 0;
+  while (((size_t)1 << b) < v) ++b;
+  return b;
+}
+
+struct GradPlan {
+  int passes, bits, tiles;
+  unsigned int tile, chunk, chunks;
+  size_t pitch;
+};
+GradPlan grad_plan(size_t n, size_t vocab, size_t width) {
+  GradPlan g{};
+  if (n > RANK_MOST) {
+    const int bits = log2_ceil(vocab + 1);
+    g.passes = (bits + RADIX_MOST_BITS - 1) / RADIX_MOST_BITS;
+    g.bits = (bits + g.passes - 1) / g.passes;
+    const size_t steps = (n + RADIX_STEP - 1) / RADIX_STEP;
+    g.tile = (unsigned int)((steps + RADIX_TILES - 1) / RADIX_TILES * RADIX_STEP);
+    g.tiles = (int)((n + g.tile - 1) / g.tile);
+  }
+  // about eight groups per SM where there are enough elements, and no less than eight elements in a row
+  g.chunk = 8;
+  while (g.chunk < 512 && n / g.chunk > 148 * 8) g.chunk *= 2;
+  g.chunks = (unsigned int)((n + g.chunk - 1) / g.chunk);
+  g.pitch = (width + 3) / 4 * 4;
+  return g;
+}
+struct GradSpace {
+  unsigned int *keys[2], *pos[2], *counts;
+  float *head, *tail;
+};
+size_t grad_space(const GradPlan& g, size_t n, void* base, GradSpace* s) {
+  Carver c(base);
+  const int buffers = g.passes ? 2 : 1;
+  for (int i = 0; i < buffers; ++i) {
+    s->keys[i] = c.take<unsigned int>(n);
+    s->pos[i] = c.take<unsigned int>(n);
+  }
+  s->counts = c.take<unsigned int>(g.passes ? (size_t)g.tiles << g.bits : 0);
+  s->head = c.take<float>(g.chunks * g.pitch);
+  s->tail = c.take<float>(g.chunks * g.pitch);
+  return c.used;
+}
+
+int check_table(const char* who, size_t n, int token_bytes, int dtype, size_t vocab, size_t width, size_t ld_rows,
+                size_t ld_table) {
+  if (token_bytes != 4 && token_bytes != 8) return call_error(B2_ERR_INVALID, "%s: token_bytes is 4 or 8, not %d", who, token_bytes);
+  if (!dtype_ok(dtype)) return call_error(B2_ERR_INVALID, "%s: dtype %d", who, dtype);
+  if (width < 1 || width > 0x7FFFFFFFu / 4) return call_error(B2_ERR_INVALID, "%s: width %zu", who, width);
+  if (vocab < 1 || vocab >= 0x7FFFFFFFu) return call_error(B2_ERR_INVALID, "%s: vocab %zu", who, vocab);
+  if (n >= 0x7FFFFFFFu) return call_error(B2_ERR_INVALID, "%s: %zu tokens", who, n);
+  if (ld_rows < width || ld_table < width) return call_error(B2_ERR_INVALID, "%s: leading dimension smaller than the width", who);
+  return B2_OK;
+}
+
+template <typename T, int VB>
+cudaError_t embed_launch(const void* tokens, int wide, size_t n, const void* table, size_t vocab, size_t width,
+                         size_t ld_table, float scale, void* out, size_t ld_out, int sms, cudaStream_t s) {
+  const int vecs = (int)(width * sizeof(T) / VB);
+  int tpr = log2_ceil(vecs);
+  if (tpr > 8) tpr = 8;
+  const size_t group = EMBED_THREADS >> tpr;
+  // four rows per thread keep enough loads in flight; with few rows one, which spreads them over more SMs
+  const bool many = n > group * 4 * (size_t)sms * 4;
+  const size_t rows = group * (many ? 4 : 1);
+  const size_t lt = ld_table * sizeof(T), lo = ld_out * sizeof(T);
+  const unsigned int grid = (unsigned int)((n + rows - 1) / rows);
+  if (many)
+    embed_kernel<T, VB, 4><<<grid, EMBED_THREADS, 0, s>>>(tokens, wide, n, (const char*)table, (unsigned int)vocab, vecs, lt, scale, (char*)out, lo, tpr);
+  else
+    embed_kernel<T, VB, 1><<<grid, EMBED_THREADS, 0, s>>>(tokens, wide, n, (const char*)table, (unsigned int)vocab, vecs, lt, scale, (char*)out, lo, tpr);
+  return cudaGetLastError();
+}
+
+template <typename T, int VB>
+cudaError_t run_launch(RunSum p, size_t width, cudaStream_t s) {
+  p.vecs = (int)(width * sizeof(T) / VB);
+  p.tpr_log2 = log2_ceil(p.vecs);
+  if (p.tpr_log2 > 7) p.tpr_log2 = 7;
+  p.slices = (p.vecs + (1 << p.tpr_log2) - 1) >> p.tpr_log2;
+  const size_t units = (size_t)p.chunks * p.slices, per_block = RUN_THREADS >> p.tpr_log2;
+  p.sum_blocks = (unsigned int)((units + per_block - 1) / per_block);
+  const unsigned int fill = (p.vocab + RUN_THREADS - 1) / RUN_THREADS;
+  run_sum_kernel<T, VB><<<p.sum_blocks + fill, RUN_THREADS, 0, s>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace b2
+
+using namespace b2;
+
+extern "C" {
+
+int b2_embed(const void* tokens, int token_bytes, size_t n, const void* table, int dtype, size_t vocab, size_t width,
+             size_t ld_table, float scale, void* out, size_t ld_out, void* stream) {
+  int rc = check_table("b2_embed", n, token_bytes, dtype, vocab, width, ld_out, ld_table);
+  if (rc != B2_OK) return rc;
+  if (n == 0) return B2_OK;
+  if (!tokens || !table || !out) return call_error(B2_ERR_INVALID, "b2_embed: null pointer");
+  int sms;
+  if ((rc = lm_device(&sms)) != B2_OK) return rc;
+  const size_t e = dtype_bytes(dtype);
+  if ((reinterpret_cast<size_t>(table) | reinterpret_cast<size_t>(out)) % e || reinterpret_cast<size_t>(tokens) % token_bytes)
+    return call_error(B2_ERR_INVALID, "b2_embed: a pointer is not aligned to its elements");
+  const int vb = vector_bytes(e, reinterpret_cast<size_t>(table) | reinterpret_cast<size_t>(out) | width * e | ld_table * e | ld_out * e);
+  const int wide = token_bytes == 8;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t err;
+#define B2_EMBED(T, VB) err = embed_launch<T, VB>(tokens, wide, n, table, vocab, width, ld_table, scale, out, ld_out, sms, s)
+  if (dtype == B2_DTYPE_BF16) {
+    if (vb == 16) B2_EMBED(__nv_bfloat16, 16);
+    else if (vb == 8) B2_EMBED(__nv_bfloat16, 8);
+    else if (vb == 4) B2_EMBED(__nv_bfloat16, 4);
+    else B2_EMBED(__nv_bfloat16, 2);
+  } else {
+    if (vb == 16) B2_EMBED(float, 16);
+    else if (vb == 8) B2_EMBED(float, 8);
+    else B2_EMBED(float, 4);
+  }
+#undef B2_EMBED
+  return launch_error(err, "b2_embed");
+}
+
+int b2_embed_grad_workspace(size_t n, size_t vocab, size_t width, size_t* bytes) {
+  int rc = check_table("b2_embed_grad_workspace", n, 4, B2_DTYPE_F32, vocab, width, width, width);
+  if (rc != B2_OK) return rc;
+  if (!bytes) return call_error(B2_ERR_INVALID, "b2_embed_grad_workspace: null pointer");
+  GradSpace s;
+  *bytes = grad_space(grad_plan(n, vocab, width), n, nullptr, &s);
+  return B2_OK;
+}
+
+int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dout, int dtype, size_t ld_dout,
+                  size_t vocab, size_t width, float scale, void* dtable, size_t ld_dtable, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+  int rc = check_table("b2_embed_grad", n, token_bytes, dtype, vocab, width, ld_dout, ld_dtable);
+  if (rc != B2_OK) return rc;
+  if (!dtable || (n && (!tokens || !dout || !workspace))) return call_error(B2_ERR_INVALID, "b2_embed_grad: null pointer");
+  const size_t e = dtype_bytes(dtype);
+  if ((reinterpret_cast<size_t>(dout) | reinterpret_cast<size_t>(dtable)) % e || reinterpret_cast<size_t>(tokens) % token_bytes)
+    return call_error(B2_ERR_INVALID, "b2_embed_grad: a pointer is not aligned to its elements");
+  if (reinterpret_cast<size_t>(workspace) % 256) return call_error(B2_ERR_INVALID, "b2_embed_grad: the workspace is not on a 256-byte boundary");
+  const GradPlan g = grad_plan(n, vocab, width);
+  GradSpace w;
+  const size_t need = grad_space(g, n, workspace, &w);
+  if (n && workspace_bytes < need) return call_error(B2_ERR_INVALID, "b2_embed_grad: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  int sms;
+  if ((rc = lm_device(&sms)) != B2_OK) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (n == 0)
+    return launch_error(cudaMemset2DAsync(dtable, ld_dtable * e, 0, width * e, vocab, s), "b2_embed_grad");
+  const int wide = token_bytes == 8;
+  int sorted = 0;
+  if (g.passes == 0) {
+    const int per_block = RANK_THREADS / 32 * RANK_PER_WARP;
+    rank_sort_kernel<<<(unsigned int)((n + per_block - 1) / per_block), RANK_THREADS, n * 4, s>>>(tokens, wide, (int)n, (unsigned int)vocab, w.keys[0], w.pos[0]);
+  } else {
+    RadixPass p{};
+    p.wide = wide;
+    p.vocab = (unsigned int)vocab;
+    p.counts = w.counts;
+    p.n = (unsigned int)n;
+    p.tile = g.tile;
+    p.tiles = g.tiles;
+    p.bits = g.bits;
+    for (int i = 0; i < g.passes; ++i) {
+      p.tokens = i == 0 ? tokens : nullptr;
+      p.keys = w.keys[sorted];
+      p.pos = w.pos[sorted];
+      if (i > 0) sorted ^= 1;
+      p.keys_out = w.keys[sorted];
+      p.pos_out = w.pos[sorted];
+      p.shift = i * g.bits;
+      radix_count_kernel<<<g.tiles, RADIX_THREADS, 0, s>>>(p);
+      radix_place_kernel<<<g.tiles, RADIX_THREADS, 0, s>>>(p);
+    }
+  }
+  cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return launch_error(err, "b2_embed_grad");
+  RunSum r{};
+  r.keys = w.keys[sorted];
+  r.pos = w.pos[sorted];
+  r.n = (unsigned int)n;
+  r.vocab = (unsigned int)vocab;
+  r.chunk = g.chunk;
+  r.chunks = g.chunks;
+  r.dout = static_cast<const char*>(dout);
+  r.ld_dout = ld_dout * e;
+  r.dtable = static_cast<char*>(dtable);
+  r.ld_dtable = ld_dtable * e;
+  r.head = w.head;
+  r.tail = w.tail;
+  r.pitch = g.pitch;
+  r.scale = scale;
+  const int vb = vector_bytes(e, reinterpret_cast<size_t>(dout) | reinterpret_cast<size_t>(dtable) | width * e | r.ld_dout | r.ld_dtable);
+  if (dtype == B2_DTYPE_BF16)
+    err = vb == 16  ? run_launch<__nv_bfloat16, 16>(r, width, s)
+          : vb == 8 ? run_launch<__nv_bfloat16, 8>(r, width, s)
+          : vb == 4 ? run_launch<__nv_bfloat16, 4>(r, width, s)
+                    : run_launch<__nv_bfloat16, 2>(r, width, s);
+  else
+    err = vb == 16 ? run_launch<float, 16>(r, width, s) : vb == 8 ? run_launch<float, 8>(r, width, s) : run_launch<float, 4>(r, width, s);
+  if (err == cudaSuccess && g.chunks > 1) {
+    // most blocks find that no run begins in their chunk and goes on: a few thousand of them at most
+    unsigned int slices = (unsigned int)((width + 31) / 32);
+    while (slices > 1 && (size_t)slices * g.chunks > 4096) slices /= 2;
+    const dim3 grid(g.chunks, slices);
+    if (dtype == B2_DTYPE_BF16) run_join_kernel<__nv_bfloat16><<<grid, 32 * JOIN_PARTS, 0, s>>>(r, (int)width);
+    else run_join_kernel<float><<<grid, 32 * JOIN_PARTS, 0, s>>>(r, (int)width);
+    err = cudaGetLastError();
+  }
+  return launch_error(err, "b2_embed_grad");
+}
+
+}  // extern "C"

@@ -34,6 +34,7 @@
 #include "download_plan.h"
 #include "step_choice.h"
 #include "common.cuh"
+#include "lm.cuh"
 #include "nccl_dyn.h"
 
 using namespace b2;
@@ -1230,6 +1231,29 @@ int dev_alloc(b2_handle* h, T** p, size_t bytes) {
 }
 
 }  // namespace
+
+int b2::call_error(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  try {
+    g_tls_error = buf;
+  } catch (...) {  // no memory for the text: the code alone goes back
+  }
+  return code;
+}
+
+int b2::lm_device(int* sms) {
+  int dev = 0, major = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return call_error(B2_ERR_CUDA, "no usable CUDA device: %s (there is no CPU path)", cudaGetErrorString(e));
+  if (major != 10) return call_error(B2_ERR_UNSUPPORTED, "device %d has compute capability %d.x; the kernels are built for sm_100a", dev, major);
+  return B2_OK;
+}
 
 extern "C" {
 

@@ -1,0 +1,78 @@
+// What the operators around a language model's layers share (embed.cu, xent.cu, muon.cu): error texts, element
+// vectors, and workspaces cut into pieces.
+#pragma once
+
+#include <stddef.h>
+
+#include "../../include/b200mlp.h"
+#include "common.cuh"
+
+namespace b2 {
+
+// Records the text b2_last_error(NULL) returns on this thread and gives back `code` (engine.cu).
+int call_error(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+
+// B2_OK where the calling thread's device can run this library's kernels; *sms = its multiprocessors.
+int lm_device(int* sms);
+
+namespace {
+
+inline int launch_error(cudaError_t e, const char* what) {
+  return e == cudaSuccess ? B2_OK : call_error(B2_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+inline size_t dtype_bytes(int dtype) { return dtype == B2_DTYPE_BF16 ? 2 : 4; }
+inline bool dtype_ok(int dtype) { return dtype == B2_DTYPE_F32 || dtype == B2_DTYPE_BF16; }
+
+// Pieces of a caller's workspace, each on a 256-byte boundary. With a null base it only adds up sizes.
+struct Carver {
+  char* base;
+  size_t used;
+  explicit Carver(void* p) : base(static_cast<char*>(p)), used(0) {}
+  template <typename T>
+  T* take(size_t count) {
+    T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
+    used += (count * sizeof(T) + 255) / 256 * 256;
+    return p;
+  }
+};
+
+// The widest vector (16, 8 or 4 bytes, or one element) that divides every one of the given addresses and byte counts.
+inline int vector_bytes(size_t elem, size_t bits) {
+  for (int v = 16; v > (int)elem; v >>= 1)
+    if (bits % v == 0) return v;
+  return (int)elem;
+}
+
+template <int BYTES> struct Raw;
+template <> struct Raw<16> { typedef uint4 type; };
+template <> struct Raw<8> { typedef uint2 type; };
+template <> struct Raw<4> { typedef unsigned int type; };
+template <> struct Raw<2> { typedef unsigned short type; };
+
+// BYTES bytes of elements of type T as floats, and back (rounded to nearest).
+template <typename T, int BYTES>
+struct Elems {
+  static constexpr int N = BYTES / (int)sizeof(T);
+  typedef typename Raw<BYTES>::type raw;
+  static __device__ __forceinline__ void get(const raw& r, float (&f)[N]) {
+    const T* t = reinterpret_cast<const T*>(&r);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = (float)t[i];
+  }
+  static __device__ __forceinline__ raw put(const float (&f)[N]) {
+    raw r;
+    T* t = reinterpret_cast<T*>(&r);
+#pragma unroll
+    for (int i = 0; i < N; ++i) t[i] = (T)f[i];
+    return r;
+  }
+};
+
+// Token number i of a list of 32- or 64-bit ones; anything outside [0, vocab) becomes vocab.
+__device__ __forceinline__ unsigned int token_at(const void* tokens, int wide, size_t i, unsigned int vocab) {
+  const long long t = wide ? __ldg(static_cast<const long long*>(tokens) + i) : (long long)__ldg(static_cast<const int*>(tokens) + i);
+  return t >= 0 && t < (long long)vocab ? (unsigned int)t : vocab;
+}
+
+}  // namespace
+}  // namespace b2

@@ -401,6 +401,28 @@ int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dou
                   size_t vocab, size_t width, float scale, void* dtable, size_t ld_dtable, void* workspace,
                   size_t workspace_bytes, void* stream);
 
+/* Softmax cross entropy behind a linear layer as wide as a vocabulary: x = h w' (h rows x width, w vocab x width),
+ *   row_loss[i] = log(sum over v of exp(x[i][v])) - x[i][targets[i]]        fp32, always written
+ *   dh = gradient of scale * sum(row_loss) with respect to h, dw the same with respect to w
+ * dh and dw are of `dtype` and are written, not added to; NULL leaves one (or both: losses only) out. Rows whose target
+ * is padding have loss 0 and a zero row of dh, take no part in dw whatever they hold, and cost next to nothing. The
+ * logits are computed in pieces of the vocabulary, with gradients twice, and never kept. Types: bf16 matrices
+ * are multiplied as they are with fp32 sums, the logits' gradients rounded to bf16 once; fp32 matrices, and the
+ * logits' gradients between them, at 22 bits of every element down to 2^-27 of the largest (1 for the latter) and to
+ * 2^-50 of the largest below that. Equal inputs give equal bits. Limits: rows and vocab at most 2^24,
+ * width at most 2^20. Fastest where w begins on a 16-byte boundary and ldw is a multiple of 8 (bf16); otherwise, and in fp32,
+ * a copy of w goes to the workspace, which is why its size depends on `w` and `ldw`. `grads` is 1 where the call will
+ * ask for dh or dw. For 1 / global batch as `scale` the gradients are this rank's share, as everywhere in this library. */
+int b2_xent_workspace(size_t rows, size_t width, size_t vocab, int dtype, int grads, const void* w, size_t ldw,
+                      size_t* bytes);
+int b2_xent(size_t rows, size_t width, size_t vocab, int dtype, const void* h, size_t ldh, const void* w, size_t ldw,
+            const void* targets, int token_bytes, float scale, float* row_loss, void* dh, size_t ld_dh, void* dw,
+            size_t ld_dw, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Waits for `stream` and returns B2_ERR_TIMEOUT if a bounded wait inside one of this section's tensor-core kernels on
+ * the current device gave up since the last call (their results are then not valid), B2_OK otherwise. */
+int b2_lm_sync(void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -94,6 +94,10 @@ SYMBOLS = {
     "b2_embed": (C.c_int, [_vp, C.c_int, _sz, _vp, C.c_int, _sz, _sz, _sz, C.c_float, _vp, _sz, _vp]),
     "b2_embed_grad_workspace": (C.c_int, [_sz, _sz, _sz, C.POINTER(_sz)]),
     "b2_embed_grad": (C.c_int, [_vp, C.c_int, _sz, _vp, C.c_int, _sz, _sz, _sz, C.c_float, _vp, _sz, _vp, _sz, _vp]),
+    "b2_xent_workspace": (C.c_int, [_sz, _sz, _sz, C.c_int, C.c_int, _vp, _sz, C.POINTER(_sz)]),
+    "b2_xent": (C.c_int, [_sz, _sz, _sz, C.c_int, _vp, _sz, _vp, _sz, _vp, C.c_int, C.c_float, _vp, _vp, _sz, _vp, _sz,
+                          _vp, _sz, _vp]),
+    "b2_lm_sync": (C.c_int, [_vp]),
 }
 
 _lib = None

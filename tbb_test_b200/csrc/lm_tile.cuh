@@ -1,0 +1,389 @@
+// Tiles of matrix products for the operators around a language model's layers (xent.cu, muon.cu): a persistent kernel of
+// CTA pairs on the tensor cores whose operator Op says which tiles there are and what happens to their elements.
+//
+// A pair (a cluster of two CTAs on neighbouring SMs) computes 256 x BN of C = A B' with tcgen05.mma.cta_group::2: CTA r holds
+// rows [128 r, 128 r + 128) of A's slab and the r-th half of B's, the leader issues every MMA, and each CTA's tensor
+// memory receives its own 128 rows. Operands are 16-bit, either with K contiguous or with M/N contiguous, and come by TMA in
+// slabs of 64 k. Two accumulators take turns, so that one tile's elements are worked on while the next is summed.
+//
+// Two forms:
+//   plain   bf16 operands, BN = 256, six stages of 32 KB
+//   split   every operand is a pair of fp16 matrices x = hi + 2^-11 lo, 22 bits together; hi hi' goes to one
+//           accumulator, hi lo' + lo hi' to another behind it (lo lo' is 2^-22 of the product and left out). BN = 128, four
+//           stages of 48 KB. Three MMAs at the full fp16 rate give what three tf32 MMAs give at half of it, provided the
+//           caller scales its matrices into fp16's range; with lo as large as hi, 22 bits are kept down to magnitudes of
+//           2^-13 and what lies below is held to 2^-36. The tensor core truncates when it adds to an
+//           accumulator (about 2e-8 of the sum each time, and always towards zero), so a sum is handed over every
+//           SPLIT_SUM k-blocks and added up in fp32 registers, rounded to nearest.
+//
+// Warps: 0 loads, 1 allocates tensor memory and (in the leader) issues, 2 to 9 work on elements: the warps of a lane quarter
+// share its columns by halves.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "lm.cuh"
+#include "tcgen05.cuh"
+
+namespace b2 {
+namespace {
+
+constexpr int TILE_M = 256, TILE_K = 64;
+constexpr int TILE_EPI_WARPS = 8;
+constexpr int TILE_THREADS = 64 + 32 * TILE_EPI_WARPS;
+constexpr int STAGE_PITCH = 33;  // floats: conflict-free by rows and by columns
+constexpr int STAGE_WORDS = 32 * STAGE_PITCH;
+constexpr int SPLIT_SUM = 16;  // k-blocks per hand-over
+constexpr float LO_UP = 2048.f;  // lo = 2^11 (x - hi)
+constexpr uint32_t ACC_COLS = 256;  // tensor-memory columns of an accumulator stage
+constexpr int TILE_MAX_STAGES = 6;
+
+// A wait that gave up leaves its role's number here; b2_lm_sync reports and clears it.
+__device__ unsigned int tile_status;
+
+template <bool SPLIT>
+struct TileForm {
+  static constexpr int BN = SPLIT ? 128 : 256;
+  static constexpr int STAGES = SPLIT ? 4 : 6;
+  static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128;
+  static constexpr uint32_t STAGE_BYTES = (A_BYTES + B_BYTES) * (SPLIT ? 2 : 1);
+  static constexpr size_t SMEM = 1024 + STAGES * STAGE_BYTES + TILE_EPI_WARPS * STAGE_WORDS * 4;
+};
+
+struct TileMaps {
+  CUtensorMap a, a_lo, b, b_lo;
+};
+struct TileLayout {
+  int a_form, b_form;  // SlabForm
+  uint32_t a_lbo, a_kstep, b_lbo, b_kstep;
+  uint32_t idesc;
+};
+// One tile: rows and columns of C from m0, n0 on; where its slabs lie in A and B along M/N and along K.
+struct Tile {
+  int m0, n0;
+  int a_mn, b_mn, a_k, b_k;
+  int kblocks;
+  int z;  // matrix of a batch
+};
+
+// Op: struct Params; static constexpr bool SPLIT; Op(const Params&); int tiles(); Tile tile(int t);
+//     and in the element warps: void begin(const Tile&, int row, int half); void chunk(const Tile&, int row0, int col0,
+//     float (&v)[32], float* stage, int lane) for 32 columns of rows row0 + lane; void end(const Tile&, int row, int half).
+template <class Op>
+__global__ void __launch_bounds__(TILE_THREADS, 1) tile_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ TileLayout L,
+                                                               const __grid_constant__ typename Op::Params params) {
+  constexpr bool SPLIT = Op::SPLIT;
+  typedef TileForm<SPLIT> F;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full_bar[TILE_MAX_STAGES];
+  __shared__ __align__(8) uint64_t empty_bar[TILE_MAX_STAGES];
+  __shared__ __align__(8) uint64_t acc_full_bar[2];
+  __shared__ __align__(8) uint64_t acc_empty_bar[2];
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int abort_s;
+
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  volatile int* abort_flag = &abort_s;
+
+  if (threadIdx.x == 0) {
+    abort_s = 0;
+    for (int s = 0; s < F::STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&acc_full_bar[a], 1);
+      mbar_init(&acc_empty_bar[a], 2 * TILE_EPI_WARPS);  // the element warps of both CTAs
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.b) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_base_s;
+  Op op(params);
+  const int tiles = op.tiles();
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint32_t full0 = map_to_cta(smem_u32(full_bar), 0), empty0 = smem_u32(empty_bar), ring0 = smem_u32(smem);
+      for (int t = pair; t < tiles && ok; t += num_pairs) {
+        const Tile tile = op.tile(t);
+        const int am = tile.a_mn + (int)rank * 128, bn = tile.b_mn + (int)rank * (F::BN / 2);
+        for (int kb = 0; kb < tile.kblocks; ++kb) {
+          if (!mbar_wait(empty0 + 8u * stage, phase ^ 1, abort_flag, &tile_status, 1u)) { ok = false; break; }
+          const uint32_t s0 = ring0 + (uint32_t)stage * F::STAGE_BYTES;
+          if (rank == 0) mbar_expect_tx(smem_u32(full_bar) + 8u * stage, 2 * F::STAGE_BYTES);  // both CTAs' bytes
+          const uint32_t full = full0 + 8u * stage;
+          const int ka = tile.a_k + kb * TILE_K, kbb = tile.b_k + kb * TILE_K;
+          load_slab<true>(&maps.a, full, s0, L.a_form, ka, am, 2, TILE_K * 128, 6);
+          const uint32_t sb = s0 + F::A_BYTES * (SPLIT ? 2 : 1);
+          load_slab<true>(&maps.b, full, sb, L.b_form, kbb, bn, F::BN / 128, TILE_K * 128, 6);
+          if (SPLIT) {
+            load_slab<true>(&maps.a_lo, full, s0 + F::A_BYTES, L.a_form, ka, am, 2, TILE_K * 128, 6);
+            load_slab<true>(&maps.b_lo, full, sb + F::B_BYTES, L.b_form, kbb, bn, F::BN / 128, TILE_K * 128, 6);
+          }
+          if (++stage == F::STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok) {  // copies in flight get a bounded time to land before the CTA retires
+        const unsigned long long t0 = globaltimer();
+        while (globaltimer() - t0 < 2000000ull) __nanosleep(1000);
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0 && elect_one()) {
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      const uint64_t a_tmpl = make_smem_desc(smem_u32(smem), L.a_lbo, 1024, 2);
+      const uint64_t b_tmpl = make_smem_desc(smem_u32(smem) + F::A_BYTES * (SPLIT ? 2 : 1), L.b_lbo, 1024, 2);
+      const uint32_t a_step = L.a_kstep >> 4, b_step = L.b_kstep >> 4, idesc = L.idesc;
+      const uint32_t full0 = smem_u32(full_bar), empty0 = smem_u32(empty_bar), acc_full0 = smem_u32(acc_full_bar);
+      for (int t = pair; t < tiles && ok; t += num_pairs) {
+        const int kblocks = op.tile(t).kblocks;
+        for (int kb = 0; kb < kblocks; ++kb) {
+          const bool first = kb == 0 || (SPLIT && kb % SPLIT_SUM == 0);
+          if (first) {
+            if (!mbar_wait(&acc_empty_bar[acc], acc_phase ^ 1, abort_flag, &tile_status, 2u)) { ok = false; break; }
+            tc_fence_after();
+          }
+          if (!mbar_wait(full0 + 8u * stage, phase, abort_flag, &tile_status, 3u)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t d = tmem_base + (uint32_t)acc * ACC_COLS;
+          const uint32_t off = ((uint32_t)stage * F::STAGE_BYTES) >> 4;
+#pragma unroll
+          for (int ks = 0; ks < TILE_K / 16; ++ks) {
+            const uint64_t ad = a_tmpl + off + (uint64_t)(ks * a_step), bd = b_tmpl + off + (uint64_t)(ks * b_step);
+            const uint32_t go = first && ks == 0 ? 0u : 1u;
+            mma_issue<false, true>(d, ad, bd, idesc, go);
+            if (SPLIT) {
+              mma_issue<false, true>(d + F::BN, ad, bd + (F::B_BYTES >> 4), idesc, go);
+              mma_issue<false, true>(d + F::BN, ad + (F::A_BYTES >> 4), bd, idesc, 1u);
+            }
+          }
+          tc_commit_pair(empty0 + 8u * stage);
+          if (++stage == F::STAGES) { stage = 0; phase ^= 1; }
+          if (kb + 1 == kblocks || (SPLIT && (kb + 1) % SPLIT_SUM == 0)) {
+            tc_commit_pair(acc_full0 + 8u * acc);
+            acc ^= 1;
+            if (acc == 0) acc_phase ^= 1;
+          }
+        }
+      }
+    }
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    constexpr int COLS = F::BN / 2;  // columns of this warp
+    float* stage = reinterpret_cast<float*>(smem + F::STAGES * F::STAGE_BYTES) + (warp - 2) * STAGE_WORDS;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int t = pair; t < tiles && ok; t += num_pairs) {
+      const Tile tile = op.tile(t);
+      const int row0 = tile.m0 + (int)rank * 128 + q * 32, c0 = half * COLS;
+      const uint32_t lanes = (uint32_t)(q * 32) << 16;
+      if (SPLIT) {
+        float sum[COLS];
+        for (int kb = 0; kb < tile.kblocks; kb += SPLIT_SUM) {
+          if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_flag, &tile_status, 4u)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t from = tmem_base + lanes + (uint32_t)acc * ACC_COLS + (uint32_t)c0;
+#pragma unroll
+          for (int c = 0; c < COLS; c += 32) {
+            uint32_t r[32], x[32];
+            tmem_ld32(from + c, r);
+            tmem_ld32(from + F::BN + c, x);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float v = fmaf(__uint_as_float(x[j]), 1.f / LO_UP, __uint_as_float(r[j]));
+              sum[c + j] = kb == 0 ? v : sum[c + j] + v;
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_leader(map_to_cta(smem_u32(&acc_empty_bar[acc]), 0));
+          acc ^= 1;
+          if (acc == 0) acc_phase ^= 1;
+        }
+        if (!ok) break;
+        op.begin(tile, row0 + lane, half);
+#pragma unroll
+        for (int c = 0; c < COLS; c += 32) {
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = sum[c + j];
+          op.chunk(tile, row0, tile.n0 + c0 + c, v, stage, lane);
+        }
+        op.end(tile, row0 + lane, half);
+      } else {
+        op.begin(tile, row0 + lane, half);
+        if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_flag, &tile_status, 4u)) break;
+        tc_fence_after();
+        const uint32_t from = tmem_base + lanes + (uint32_t)acc * ACC_COLS + (uint32_t)c0;
+#pragma unroll 1
+        for (int c = 0; c < COLS; c += 32) {
+          uint32_t r[32];
+          tmem_ld32(from + c, r);
+          if (c + 32 == COLS) {  // all read: the next tile may be summed here
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_leader(map_to_cta(smem_u32(&acc_empty_bar[acc]), 0));
+          }
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+          op.chunk(tile, row0, tile.n0 + c0 + c, v, stage, lane);
+        }
+        op.end(tile, row0 + lane, half);
+        acc ^= 1;
+        if (acc == 0) acc_phase ^= 1;
+      }
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+  }
+}
+
+__device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
+  hi = __float2half_rn(v);
+  lo = __float2half_rn((v - __half2float(hi)) * LO_UP);
+}
+
+// The chunk through shared memory, so that a warp's accesses to global memory cover whole rows: f(row, col, v) gets four
+// neighbouring columns of a row, eight lanes per row, four rows at a time.
+template <class Fn>
+__device__ __forceinline__ void by_rows(int row0, int col0, const float (&v)[32], float* stage, int lane, Fn f) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) stage[lane * STAGE_PITCH + j] = v[j];
+  __syncwarp();
+  const int c = (lane & 7) * 4;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = 4 * i + (lane >> 3);
+    const float* s = stage + r * STAGE_PITCH + c;
+    const float4 x = make_float4(s[0], s[1], s[2], s[3]);
+    f(row0 + r, col0 + c, x);
+  }
+  __syncwarp();
+}
+// The same chunk transposed: f(col, row, v) gets four neighbouring rows of a column. Behind by_rows, before the next chunk.
+template <class Fn>
+__device__ __forceinline__ void by_columns(int row0, int col0, const float (&v)[32], float* stage, int lane, Fn f) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) stage[lane * STAGE_PITCH + j] = v[j];
+  __syncwarp();
+  const int r = (lane & 7) * 4;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int c = 4 * i + (lane >> 3);
+    const float* s = stage + r * STAGE_PITCH + c;
+    const float4 x = make_float4(s[0], s[STAGE_PITCH], s[2 * STAGE_PITCH], s[3 * STAGE_PITCH]);
+    f(col0 + c, row0 + r, x);
+  }
+  __syncwarp();
+}
+
+// ------------------------------------------------------------------ host side
+
+// An operand in device memory: `mn` rows (or, with mn_contiguous, columns) by k elements of 16 bits, ld between rows.
+struct TileOperand {
+  const void *hi, *lo;
+  long long mn, k, ld;
+  bool mn_contiguous;
+};
+
+inline bool tile_maps(const TileOperand& a, const TileOperand& b, bool split, bool bf16, TileMaps* maps, TileLayout* L) {
+  const int bn = split ? 128 : 256;
+  auto one = [](const TileOperand& o, const void* p, int rows, int* form, CUtensorMap* m) {
+    if (!o.mn_contiguous) {
+      *form = SLAB_K;
+      return make_map(m, p, 2, o.k, o.mn, o.ld, TILE_K, rows, 0);
+    }
+    if (o.mn % 64 == 0 && make_map_columns(m, p, 2, o.mn, o.k, o.ld, TILE_K, rows / 64, 0)) {
+      *form = SLAB_MN3;
+      return true;
+    }
+    *form = SLAB_MN2;
+    return make_map(m, p, 2, o.mn, o.k, o.ld, 64, TILE_K, 0);
+  };
+  bool ok = one(a, a.hi, 128, &L->a_form, &maps->a) && one(b, b.hi, bn / 2, &L->b_form, &maps->b);
+  if (split) {
+    ok = ok && one(a, a.lo, 128, &L->a_form, &maps->a_lo) && one(b, b.lo, bn / 2, &L->b_form, &maps->b_lo);
+  } else {
+    maps->a_lo = maps->a;
+    maps->b_lo = maps->b;
+  }
+  L->a_lbo = a.mn_contiguous ? TILE_K * 128 : 16;
+  L->b_lbo = b.mn_contiguous ? TILE_K * 128 : 16;
+  L->a_kstep = a.mn_contiguous ? 16 * 128 : 32;
+  L->b_kstep = b.mn_contiguous ? 16 * 128 : 32;
+  const uint32_t fmt = bf16 ? 1u : 0u;  // bf16 : f16
+  L->idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a.mn_contiguous << 15) | ((uint32_t)b.mn_contiguous << 16) |
+             ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(TILE_M >> 4) << 24);
+  return ok;
+}
+
+// most_tiles: an upper bound on the tiles that the kernel will find.
+template <class Op>
+int tile_launch(const char* who, const TileOperand& a, const TileOperand& b, const typename Op::Params& p, bool bf16, long long most_tiles,
+                int sms, cudaStream_t s) {
+  if (most_tiles <= 0) return B2_OK;
+  TileMaps maps;
+  TileLayout L;
+  if (!tile_maps(a, b, Op::SPLIT, bf16, &maps, &L)) return call_error(B2_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", who);
+  const size_t smem = TileForm<Op::SPLIT>::SMEM;
+  cudaError_t e = cudaFuncSetAttribute(tile_kernel<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return launch_error(e, who);
+  const int pairs = sms / 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * (unsigned int)(most_tiles < pairs ? most_tiles : pairs));
+  cfg.blockDim = dim3(TILE_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, tile_kernel<Op>, maps, L, p);
+  return launch_error(e, who);
+}
+
+// What a wait that gave up left in this file's status word, which is cleared; the stream is waited for.
+inline cudaError_t tile_status_take(unsigned int* code, cudaStream_t s) {
+  const unsigned int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(code, tile_status, sizeof *code, 0, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e == cudaSuccess && *code) {
+    e = cudaMemcpyToSymbolAsync(tile_status, &zero, sizeof zero, 0, cudaMemcpyHostToDevice, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  }
+  return e;
+}
+
+}  // namespace
+}  // namespace b2

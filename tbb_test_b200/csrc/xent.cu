@@ -1,0 +1,671 @@
+// Softmax cross entropy behind a linear layer as wide as a vocabulary, with its gradients, without keeping the logits:
+//
+//   x_iv = h_i . w_v      l_i = log sum_v exp(x_iv) - x_i,t_i      d_iv = scale (exp(x_iv) / sum_u exp(x_iu) - [v = t_i])
+//   dh_i = sum_v d_iv w_v      dw_v = sum_i d_iv h_i
+//
+// Work: 2 R V F operations for the losses and 6 R V F with gradients; 8 R V F in this form, because the logits are
+// computed a second time when their row's maximum and sum are known, instead of R x V of them being kept.
+// It is bound by the tensor cores (tile kernels of lm_tile.cuh) unless R is small, when reading w is what it takes.
+//
+//   1. Rows without a target are left out: the others' numbers are listed in order, their h copied one after another.
+//      So such a row costs nothing, and nothing in it (a NaN, say) reaches dw.
+//   2. Logits, 256 x 256 at a time; each row's maximum and sum over a tile's half go to a list.
+//   3. The lists give each row's maximum and sum, and the loss.
+//   4. Per piece of the vocabulary: logits again, d to a buffer of R x piece; dh += d w; dw of the piece = d' h.
+//
+// Precision: bf16 matrices are multiplied as they are, with fp32 sums; d is rounded to bf16 once, which is a
+// relative 2^-9 at most of each product of the gradients, as much as the gradients' own rounding. fp32 matrices are
+// split into fp16 pairs behind a power of two that brings the largest element to 2^14: 22 bits of an element down to 2^-27 of
+// the largest, and nothing finer than 2^-50 of it; d the same, with 1 for the largest. Maxima, sums and the losses are fp32.
+#include <type_traits>
+
+#include "lm_tile.cuh"
+
+namespace b2 {
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int D_EXP = 14;  // fp32 matrices: d is kept as 2^14 (p - [v = t])
+
+struct Meta {
+  unsigned int rows;  // with a target
+  unsigned int max_h, max_w;  // bits of the largest magnitude (fp32 matrices)
+};
+
+__device__ __forceinline__ float ex2(float x) {  // 2^x, two units in the last place
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Power of two that brings a matrix whose largest magnitude has these bits below 2^15: its exponent. 0 for zeros and
+// for what is not finite.
+__device__ __forceinline__ int up_exp(unsigned int max_bits) {
+  const int e = (int)(max_bits >> 23) - 127;
+  if (max_bits == 0 || e == 128) return 0;
+  return min(14 - e, 100);
+}
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
+// ------------------------------------------------------------------ rows with a target
+
+constexpr int LIST_THREADS = 1024, LIST_EACH = 8;
+__global__ void __launch_bounds__(LIST_THREADS) list_rows_kernel(const void* __restrict__ targets, int wide, int rows,
+                                                                 unsigned int vocab, Meta* meta, int* __restrict__ row_of,
+                                                                 int* __restrict__ slot_of, int* __restrict__ target,
+                                                                 float* __restrict__ row_loss) {
+  __shared__ unsigned int warp_sum[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned int base = 0;
+  for (int r0 = 0; r0 < rows; r0 += LIST_THREADS * LIST_EACH) {
+    const int first = r0 + threadIdx.x * LIST_EACH;
+    unsigned int t[LIST_EACH], mine = 0;
+#pragma unroll
+    for (int k = 0; k < LIST_EACH; ++k) {
+      t[k] = first + k < rows ? token_at(targets, wide, first + k, vocab) : vocab;
+      mine += t[k] < vocab;
+    }
+    unsigned int scan = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const unsigned int up = __shfl_up_sync(0xFFFFFFFFu, scan, d);
+      if (lane >= d) scan += up;
+    }
+    if (lane == 31) warp_sum[warp] = scan;
+    __syncthreads();
+    unsigned int before = 0, all = 0;
+    for (int w = 0; w < 32; ++w) {
+      before += w < warp ? warp_sum[w] : 0u;
+      all += warp_sum[w];
+    }
+    unsigned int at = base + before + scan - mine;
+#pragma unroll
+    for (int k = 0; k < LIST_EACH; ++k) {
+      if (first + k >= rows) break;
+      if (t[k] < vocab) {
+        row_of[at] = first + k;
+        target[at] = (int)t[k];
+        slot_of[first + k] = (int)at++;
+      } else {
+        slot_of[first + k] = -1;
+        row_loss[first + k] = 0.f;
+      }
+    }
+    base += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *meta = Meta{base, 0u, 0u};
+}
+
+__device__ __forceinline__ int row_blocks(unsigned int rows) { return max(1, (int)((rows + TILE_M - 1) / TILE_M)); }
+
+// Largest magnitudes of the listed rows of h (blocks below split_at) and of w.
+__global__ void __launch_bounds__(256) max_kernel(const float* __restrict__ h, size_t ldh, const int* __restrict__ row_of,
+                                                  const float* __restrict__ w, size_t ldw, int vocab, int width,
+                                                  int split_at, Meta* meta) {
+  const bool of_h = (int)blockIdx.x < split_at;
+  const int block = of_h ? blockIdx.x : blockIdx.x - split_at, blocks = of_h ? split_at : gridDim.x - split_at;
+  const int rows = of_h ? (int)meta->rows : vocab;
+  unsigned int most = 0;
+  for (int r = block; r < rows; r += blocks) {
+    const float* x = of_h ? h + (size_t)row_of[r] * ldh : w + (size_t)r * ldw;
+    for (int c = threadIdx.x; c < width; c += 256) most = max(most, __float_as_uint(x[c]) & 0x7FFFFFFFu);
+  }
+  most = __reduce_max_sync(0xFFFFFFFFu, most);
+  if ((threadIdx.x & 31) == 0 && most) atomicMax(of_h ? &meta->max_h : &meta->max_w, most);  // order does not matter
+}
+
+// Rows one after another, zeros behind `width` up to `pitch` and in the rows that fill up a block of 256. GATHER: the listed
+// rows of h; else all rows of w.
+template <typename T, bool GATHER>
+__global__ void __launch_bounds__(256) copy_rows_kernel(const T* __restrict__ x, size_t ld, const int* __restrict__ row_of,
+                                                        int all_rows, int width, int pitch, const Meta* __restrict__ meta,
+                                                        uint16_t* __restrict__ hi, uint16_t* __restrict__ lo) {
+  constexpr bool SPLIT = sizeof(T) == 4;
+  const int have = GATHER ? (int)meta->rows : all_rows;
+  const int rows = GATHER ? row_blocks(have) * TILE_M : all_rows;
+  const float up = SPLIT ? pow2(up_exp(GATHER ? meta->max_h : meta->max_w)) : 1.f;
+  const bool vec = ld % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+    const bool in = r < have;
+    const T* src = in ? x + (size_t)(GATHER ? row_of[r] : r) * ld : x;
+    for (int c = threadIdx.x * 8; c < pitch; c += 256 * 8) {
+      T v[8];
+      if (in && vec && c + 8 <= width) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+          reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(src + c) + i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = in && c + i < width ? src[c + i] : (T)0.f;
+      }
+      if (SPLIT) {
+        __half a[8], b[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) split_half((float)v[i] * up, a[i], b[i]);
+        *reinterpret_cast<uint4*>(hi + (size_t)r * pitch + c) = *reinterpret_cast<const uint4*>(a);
+        *reinterpret_cast<uint4*>(lo + (size_t)r * pitch + c) = *reinterpret_cast<const uint4*>(b);
+      } else {
+        *reinterpret_cast<uint4*>(hi + (size_t)r * pitch + c) = *reinterpret_cast<const uint4*>(v);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ logits
+
+struct LogitParams {
+  const Meta* meta;
+  int vocab, v_begin, v_count;  // this call's piece of the vocabulary
+  int kblocks;
+  long long row_pitch;  // rows of the lists: parts are [tile half][row]
+  const int* target;
+  float2* parts;        // maximum (times log2 e) and sum of 2^(x - maximum)
+  float* target_logit;  // times log2 e
+  const float2* row_stat;  // maximum and 1 / sum of whole rows
+  uint16_t *d_hi, *d_lo;
+  long long ld_d;
+  float scale;
+};
+
+template <bool SPLIT_>
+struct LogitTiles {
+  static constexpr bool SPLIT = SPLIT_;
+  static constexpr int BN = TileForm<SPLIT_>::BN;
+  const LogitParams& p;
+  int rows, m_blocks, n_blocks, band;
+  float unit;  // accumulators times this are logits times log2 e
+  __device__ explicit LogitTiles(const LogitParams& q) : p(q) {
+    rows = (int)p.meta->rows;
+    m_blocks = row_blocks(rows);
+    n_blocks = (p.v_count + BN - 1) / BN;
+    // all row blocks of a column block one after another, as long as the copy of h they read stays in the L2 cache
+    band = m_blocks <= 64 ? m_blocks : 16;
+    unit = SPLIT ? LOG2E * pow2(-up_exp(p.meta->max_h)) * pow2(-up_exp(p.meta->max_w)) : LOG2E;
+  }
+  __device__ int tiles() const { return m_blocks * n_blocks; }
+  __device__ Tile tile(int t) const {
+    const int b = t / (band * n_blocks), in = t - b * band * n_blocks;
+    const int tall = min(band, m_blocks - b * band);
+    Tile r;
+    r.m0 = (b * band + in % tall) * TILE_M;
+    r.n0 = in / tall * BN;
+    r.a_mn = r.m0;
+    r.b_mn = p.v_begin + r.n0;
+    r.a_k = r.b_k = 0;
+    r.kblocks = p.kblocks;
+    r.z = 0;
+    return r;
+  }
+};
+
+// Maximum and sum of exponentials of a row over the columns of one warp, and the target's logit.
+template <bool SPLIT_>
+struct StatOp : LogitTiles<SPLIT_> {
+  typedef LogitParams Params;
+  using LogitTiles<SPLIT_>::p;
+  float top, sum;
+  int target;
+  __device__ explicit StatOp(const LogitParams& q) : LogitTiles<SPLIT_>(q) {}
+  __device__ __forceinline__ void begin(const Tile&, int row, int) {
+    top = -INFINITY;
+    sum = 0.f;
+    target = row < this->rows ? __ldg(p.target + row) : -1;
+  }
+  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[32], float*, int lane) {
+    if (col0 >= p.vocab) return;
+    if (col0 + 32 > p.vocab) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (col0 + j >= p.vocab) v[j] = -INFINITY;
+    }
+    float most = v[0];
+#pragma unroll
+    for (int j = 1; j < 32; ++j) most = fmaxf(most, v[j]);
+    const float now = fmaxf(top, most * this->unit);
+    const float base = now == -INFINITY ? 0.f : now;  // nothing but -inf so far: their exponentials are 0
+    float s[4] = {sum * ex2(top - base), 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 32; ++j) s[j & 3] += ex2(fmaf(v[j], this->unit, -base));
+    sum = (s[0] + s[1]) + (s[2] + s[3]);
+    top = now;
+    const int at = target - col0;
+    if (at >= 0 && at < 32) {
+      float x = v[0];
+#pragma unroll
+      for (int j = 1; j < 32; ++j) x = j == at ? v[j] : x;
+      p.target_logit[row0 + lane] = x * this->unit;
+    }
+  }
+  __device__ __forceinline__ void end(const Tile& t, int row, int half) {
+    if (row < this->rows) p.parts[(long long)(t.n0 / LogitTiles<SPLIT_>::BN * 2 + half) * p.row_pitch + row] = make_float2(top, sum);
+  }
+};
+
+// d of a piece, zeros in rows and columns that fill up tiles.
+template <bool SPLIT_>
+struct GradOp : LogitTiles<SPLIT_> {
+  typedef LogitParams Params;
+  using LogitTiles<SPLIT_>::p;
+  float top, inv;
+  int target;
+  bool in;
+  __device__ explicit GradOp(const LogitParams& q) : LogitTiles<SPLIT_>(q) {}
+  __device__ __forceinline__ void begin(const Tile&, int row, int) {
+    in = row < this->rows;
+    const float2 st = in ? __ldg(p.row_stat + row) : make_float2(0.f, 0.f);
+    top = st.x;
+    inv = st.y;
+    target = in ? __ldg(p.target + row) - p.v_begin : -1;
+  }
+  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[32], float* stage, int lane) {
+    const float to = SPLIT_ ? (float)(1 << D_EXP) : p.scale;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      float d = ex2(fmaf(v[j], this->unit, -top)) * inv;
+      if (col0 + j == target) d -= 1.f;
+      v[j] = in && col0 + j < p.v_count ? d * to : 0.f;
+    }
+    by_rows(row0, col0, v, stage, lane, [&](int r, int c, const float4& x) {
+      const long long at = (long long)r * p.ld_d + c;
+      if (SPLIT_) {
+        const float f[4] = {x.x, x.y, x.z, x.w};
+        __half a[4], b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split_half(f[i], a[i], b[i]);
+        *reinterpret_cast<uint2*>(p.d_hi + at) = *reinterpret_cast<const uint2*>(a);
+        *reinterpret_cast<uint2*>(p.d_lo + at) = *reinterpret_cast<const uint2*>(b);
+      } else {
+        *reinterpret_cast<uint2*>(p.d_hi + at) = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
+      }
+    });
+  }
+  __device__ __forceinline__ void end(const Tile&, int, int) {}
+};
+
+// Whole rows' maximum and sum from the lists, and the losses. Eight warps share 32 rows' lists.
+__global__ void __launch_bounds__(256) join_rows_kernel(const float2* __restrict__ parts, long long row_pitch, int count,
+                                                        const Meta* __restrict__ meta, const float* __restrict__ target_logit,
+                                                        const int* __restrict__ row_of, float2* __restrict__ row_stat,
+                                                        float* __restrict__ row_loss) {
+  __shared__ float2 part[8][32];
+  const int lane = threadIdx.x & 31, share = threadIdx.x >> 5, rows = (int)meta->rows;
+  const int row = blockIdx.x * 32 + lane;
+  if ((int)blockIdx.x * 32 >= rows) return;
+  float top = -INFINITY, sum = 0.f;
+  auto add = [&](float2 x) {
+    const float now = fmaxf(top, x.x);
+    const float base = now == -INFINITY ? 0.f : now;
+    sum = sum * ex2(top - base) + x.y * ex2(x.x - base);
+    top = now;
+  };
+  if (row < rows)
+#pragma unroll 4
+    for (int k = share; k < count; k += 8) add(__ldg(parts + (long long)k * row_pitch + row));
+  part[share][lane] = make_float2(top, sum);
+  __syncthreads();
+  if (share || row >= rows) return;
+  for (int k = 1; k < 8; ++k) add(part[k][lane]);
+  row_stat[row] = make_float2(top, 1.f / sum);
+  row_loss[row_of[row]] = ((top - target_logit[row]) + log2f(sum)) * LN2;
+}
+
+// ------------------------------------------------------------------ gradients
+
+struct ProductParams {
+  const Meta* meta;
+  int v_begin, v_count;
+  int width;
+  float scale;
+  // dh: fp32 sums over the pieces
+  float* acc;
+  long long ld_acc;
+  int first;  // first piece: written, not added to
+  // dw
+  void* dw;
+  long long ld_dw;
+  int out_bf16, vec;  // vec: rows begin on whole groups of four elements
+};
+
+// dh (listed rows) += d w over a piece.
+template <bool SPLIT_>
+struct HiddenOp {
+  typedef ProductParams Params;
+  static constexpr bool SPLIT = SPLIT_;
+  static constexpr int BN = TileForm<SPLIT_>::BN;
+  const ProductParams& p;
+  int m_blocks, n_blocks;
+  float unit;
+  __device__ explicit HiddenOp(const ProductParams& q) : p(q) {
+    m_blocks = row_blocks(p.meta->rows);
+    n_blocks = (p.width + BN - 1) / BN;
+    unit = SPLIT ? p.scale * pow2(-D_EXP) * pow2(-up_exp(p.meta->max_w)) : 1.f;
+  }
+  __device__ int tiles() const { return m_blocks * n_blocks; }
+  __device__ Tile tile(int t) const {
+    Tile r;
+    r.m0 = t / n_blocks * TILE_M;
+    r.n0 = t % n_blocks * BN;
+    r.a_mn = r.m0;
+    r.b_mn = r.n0;
+    r.a_k = 0;
+    r.b_k = p.v_begin;
+    r.kblocks = (p.v_count + TILE_K - 1) / TILE_K;
+    r.z = 0;
+    return r;
+  }
+  __device__ __forceinline__ void begin(const Tile&, int, int) {}
+  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[32], float* stage, int lane) {
+    by_rows(row0, col0, v, stage, lane, [&](int r, int c, const float4& x) {
+      if (c >= p.width) return;
+      float4* to = reinterpret_cast<float4*>(p.acc + (long long)r * p.ld_acc + c);
+      float4 a = p.first ? make_float4(0.f, 0.f, 0.f, 0.f) : *to;
+      a.x = fmaf(x.x, unit, a.x);
+      a.y = fmaf(x.y, unit, a.y);
+      a.z = fmaf(x.z, unit, a.z);
+      a.w = fmaf(x.w, unit, a.w);
+      *to = a;
+    });
+  }
+  __device__ __forceinline__ void end(const Tile&, int, int) {}
+};
+
+// dw of a piece = d' h.
+template <bool SPLIT_>
+struct WeightOp {
+  typedef ProductParams Params;
+  static constexpr bool SPLIT = SPLIT_;
+  static constexpr int BN = TileForm<SPLIT_>::BN;
+  const ProductParams& p;
+  int m_blocks, n_blocks, kblocks;
+  float unit;
+  __device__ explicit WeightOp(const ProductParams& q) : p(q) {
+    m_blocks = (p.v_count + TILE_M - 1) / TILE_M;
+    n_blocks = (p.width + BN - 1) / BN;
+    kblocks = max(1, (int)((p.meta->rows + TILE_K - 1) / TILE_K));  // without rows: zeros, as they are stored
+    unit = SPLIT ? p.scale * pow2(-D_EXP) * pow2(-up_exp(p.meta->max_h)) : 1.f;
+  }
+  __device__ int tiles() const { return m_blocks * n_blocks; }
+  __device__ Tile tile(int t) const {
+    Tile r;
+    r.m0 = t / n_blocks * TILE_M;
+    r.n0 = t % n_blocks * BN;
+    r.a_mn = r.m0;
+    r.b_mn = r.n0;
+    r.a_k = r.b_k = 0;
+    r.kblocks = kblocks;
+    r.z = 0;
+    return r;
+  }
+  __device__ __forceinline__ void begin(const Tile&, int, int) {}
+  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[32], float* stage, int lane) {
+    by_rows(row0, col0, v, stage, lane, [&](int r, int c, const float4& x) {
+      if (r >= p.v_count || c >= p.width) return;
+      const long long at = (long long)(p.v_begin + r) * p.ld_dw + c;
+      const float f[4] = {x.x * unit, x.y * unit, x.z * unit, x.w * unit};
+      if (p.out_bf16) {
+        __nv_bfloat16* to = static_cast<__nv_bfloat16*>(p.dw) + at;
+        if (p.vec && c + 4 <= p.width) {
+          *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (c + i < p.width) to[i] = __float2bfloat16_rn(f[i]);
+        }
+      } else {
+        float* to = static_cast<float*>(p.dw) + at;
+        if (p.vec && c + 4 <= p.width) {
+          *reinterpret_cast<float4*>(to) = make_float4(f[0], f[1], f[2], f[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (c + i < p.width) to[i] = f[i];
+        }
+      }
+    });
+  }
+  __device__ __forceinline__ void end(const Tile&, int, int) {}
+};
+
+// dh in the caller's order and type, zeros for rows without a target.
+template <typename T>
+__global__ void __launch_bounds__(256) spread_rows_kernel(const float* __restrict__ acc, long long ld_acc,
+                                                          const int* __restrict__ slot_of, int rows, int width, int vec,
+                                                          T* __restrict__ dh, size_t ld) {
+  for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+    const int slot = slot_of[r];
+    T* to = dh + (size_t)r * ld;
+    for (int c = threadIdx.x * 4; c < width; c += 256 * 4) {
+      const float4 x = slot >= 0 ? *reinterpret_cast<const float4*>(acc + slot * ld_acc + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float f[4] = {x.x, x.y, x.z, x.w};
+      if (vec && c + 4 <= width) {
+        typedef Elems<T, 4 * (int)sizeof(T)> E;
+        *reinterpret_cast<typename E::raw*>(to + c) = E::put(f);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (c + i < width) to[c + i] = (T)f[i];
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host side
+
+struct Sizes {
+  long long rows_up, pitch;  // rows of the copy of h (whole blocks), elements per row of the copies
+  long long parts;           // lists per row
+  long long piece;           // columns of d
+  bool split, copy_w;
+};
+Sizes sizes_of(size_t rows, size_t width, size_t vocab, int dtype, int grads, const void* w, size_t ldw) {
+  Sizes z;
+  z.split = dtype == B2_DTYPE_F32;
+  // TMA reads rows that begin on 16-byte boundaries
+  z.copy_w = z.split || reinterpret_cast<uintptr_t>(w) % 16 != 0 || ldw % 8 != 0;
+  z.rows_up = (long long)(rows + TILE_M - 1) / TILE_M * TILE_M;
+  z.pitch = (long long)(width + 63) / 64 * 64;
+  const int bn = z.split ? 128 : 256;
+  z.parts = 2 * (((long long)vocab + bn - 1) / bn);
+  z.piece = 0;
+  if (grads) {
+    // A piece of d should be in the L2 cache when the two products read it, and its 256-wide column blocks should go evenly
+    // over 74 pairs: 37 of them do for any number of row blocks.
+    const long long all = ((long long)vocab + 255) / 256 * 256, unit = 37 * 256;
+    long long fit = (160ll << 20) / (z.rows_up * (z.split ? 4 : 2));
+    if (fit >= unit) fit = fit / unit * unit;
+    else fit = fit / 256 * 256;
+    if (fit < 1024) fit = 1024;
+    z.piece = all < fit ? all : fit;
+  }
+  return z;
+}
+struct Space {
+  Meta* meta;
+  int *row_of, *slot_of, *target;
+  float* target_logit;
+  float2 *row_stat, *parts;
+  uint16_t *h_hi, *h_lo, *w_hi, *w_lo, *d_hi, *d_lo;
+  float* acc;
+};
+size_t space_of(const Sizes& z, size_t rows, size_t vocab, int grads, void* base, Space* s) {
+  Carver c(base);
+  const size_t lo = z.split ? 1 : 0;
+  s->meta = c.take<Meta>(1);
+  s->row_of = c.take<int>(z.rows_up);
+  s->slot_of = c.take<int>(rows);
+  s->target = c.take<int>(z.rows_up);
+  s->target_logit = c.take<float>(z.rows_up);
+  s->row_stat = c.take<float2>(z.rows_up);
+  s->parts = c.take<float2>(z.parts * z.rows_up);
+  s->h_hi = c.take<uint16_t>(z.rows_up * z.pitch);
+  s->h_lo = c.take<uint16_t>(lo * z.rows_up * z.pitch);
+  s->w_hi = c.take<uint16_t>(z.copy_w ? vocab * z.pitch : 0);
+  s->w_lo = c.take<uint16_t>(lo * vocab * z.pitch);
+  s->d_hi = c.take<uint16_t>(z.rows_up * z.piece);
+  s->d_lo = c.take<uint16_t>(lo * z.rows_up * z.piece);
+  s->acc = c.take<float>(grads ? z.rows_up * z.pitch : 0);
+  return c.used;
+}
+
+struct XentCall {
+  size_t rows, width, vocab;
+  int dtype;
+  const void* h;
+  size_t ldh;
+  const void* w;
+  size_t ldw;
+  const void* targets;
+  int wide;
+  float scale;
+  float* row_loss;
+  void* dh;
+  size_t ld_dh;
+  void* dw;
+  size_t ld_dw;
+};
+
+template <bool SPLIT>
+int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStream_t st) {
+  typedef typename std::conditional<SPLIT, float, __nv_bfloat16>::type T;
+  constexpr int BN = TileForm<SPLIT>::BN;
+  const int rows = (int)c.rows, width = (int)c.width, vocab = (int)c.vocab, pitch = (int)z.pitch;
+  const T *h = static_cast<const T*>(c.h), *w = static_cast<const T*>(c.w);
+  list_rows_kernel<<<1, LIST_THREADS, 0, st>>>(c.targets, c.wide, rows, (unsigned int)vocab, s.meta, s.row_of, s.slot_of, s.target,
+                                               c.row_loss);
+  auto blocks = [&](long long n) { return (unsigned int)(n < 8ll * sms ? n : 8ll * sms); };
+  if (SPLIT) {
+    const int of_h = (int)blocks(rows);
+    max_kernel<<<of_h + blocks(vocab), 256, 0, st>>>((const float*)c.h, c.ldh, s.row_of, (const float*)c.w, c.ldw, vocab, width, of_h, s.meta);
+  }
+  copy_rows_kernel<T, true><<<blocks(z.rows_up), 256, 0, st>>>(h, c.ldh, s.row_of, 0, width, pitch, s.meta, s.h_hi, s.h_lo);
+  if (z.copy_w)
+    copy_rows_kernel<T, false><<<blocks(vocab), 256, 0, st>>>(w, c.ldw, nullptr, vocab, width, pitch, s.meta, s.w_hi, s.w_lo);
+  int rc = launch_error(cudaGetLastError(), "b2_xent");
+  if (rc != B2_OK) return rc;
+
+  const TileOperand h_k{s.h_hi, s.h_lo, z.rows_up, pitch, pitch, false}, h_mn{s.h_hi, s.h_lo, pitch, z.rows_up, pitch, true};
+  const void* w_hi = z.copy_w ? (const void*)s.w_hi : c.w;
+  const long long w_width = z.copy_w ? pitch : width, w_ld = z.copy_w ? pitch : (long long)c.ldw;
+  const TileOperand w_k{w_hi, s.w_lo, vocab, w_width, w_ld, false}, w_mn{w_hi, s.w_lo, w_width, vocab, w_ld, true};
+  const long long m_blocks = z.rows_up / TILE_M;
+  LogitParams lp{};
+  lp.meta = s.meta;
+  lp.vocab = vocab;
+  lp.v_count = vocab;
+  lp.kblocks = (width + TILE_K - 1) / TILE_K;
+  lp.row_pitch = z.rows_up;
+  lp.target = s.target;
+  lp.parts = s.parts;
+  lp.target_logit = s.target_logit;
+  lp.row_stat = s.row_stat;
+  lp.d_hi = s.d_hi;
+  lp.d_lo = s.d_lo;
+  lp.ld_d = z.piece;
+  lp.scale = c.scale;
+  rc = tile_launch<StatOp<SPLIT>>("b2_xent", h_k, w_k, lp, !SPLIT, m_blocks * ((vocab + BN - 1) / BN), sms, st);
+  if (rc != B2_OK) return rc;
+  join_rows_kernel<<<(rows + 31) / 32, 256, 0, st>>>(s.parts, z.rows_up, (int)z.parts, s.meta, s.target_logit, s.row_of, s.row_stat,
+                                                     c.row_loss);
+  rc = launch_error(cudaGetLastError(), "b2_xent");
+  if (rc != B2_OK || (!c.dh && !c.dw)) return rc;
+
+  ProductParams pp{};
+  pp.meta = s.meta;
+  pp.width = width;
+  pp.scale = c.scale;
+  pp.acc = s.acc;
+  pp.ld_acc = pitch;
+  pp.dw = c.dw;
+  pp.ld_dw = (long long)c.ld_dw;
+  pp.out_bf16 = !SPLIT;
+  pp.vec = c.ld_dw % 4 == 0 && reinterpret_cast<uintptr_t>(c.dw) % (4 * sizeof(T)) == 0;
+  const TileOperand d_k{s.d_hi, s.d_lo, z.rows_up, z.piece, z.piece, false}, d_mn{s.d_hi, s.d_lo, z.piece, z.rows_up, z.piece, true};
+  const long long w_blocks = (width + BN - 1) / BN;
+  for (int v0 = 0; v0 < vocab; v0 += (int)z.piece) {
+    const int count = vocab - v0 < z.piece ? vocab - v0 : (int)z.piece;
+    lp.v_begin = pp.v_begin = v0;
+    lp.v_count = pp.v_count = count;
+    pp.first = v0 == 0;
+    // d's columns are written in blocks of 256, whatever the tile
+    rc = tile_launch<GradOp<SPLIT>>("b2_xent", h_k, w_k, lp, !SPLIT, m_blocks * ((count + BN - 1) / BN), sms, st);
+    if (rc == B2_OK && c.dh) rc = tile_launch<HiddenOp<SPLIT>>("b2_xent", d_k, w_mn, pp, !SPLIT, m_blocks * w_blocks, sms, st);
+    if (rc == B2_OK && c.dw)
+      rc = tile_launch<WeightOp<SPLIT>>("b2_xent", d_mn, h_mn, pp, !SPLIT, (count + TILE_M - 1) / TILE_M * w_blocks, sms, st);
+    if (rc != B2_OK) return rc;
+  }
+  if (c.dh) {
+    const int vec = c.ld_dh % 4 == 0 && reinterpret_cast<uintptr_t>(c.dh) % (4 * sizeof(T)) == 0;
+    spread_rows_kernel<T><<<blocks(rows), 256, 0, st>>>(s.acc, pitch, s.slot_of, rows, width, vec, static_cast<T*>(c.dh), c.ld_dh);
+    rc = launch_error(cudaGetLastError(), "b2_xent");
+  }
+  return rc;
+}
+
+int check_sizes(const char* who, size_t rows, size_t width, size_t vocab, int dtype) {
+  if (!dtype_ok(dtype)) return call_error(B2_ERR_INVALID, "%s: dtype %d", who, dtype);
+  if (rows > (1u << 24)) return call_error(B2_ERR_INVALID, "%s: %zu rows, at most %u", who, rows, 1u << 24);
+  if (width < 1 || width > (1u << 20)) return call_error(B2_ERR_INVALID, "%s: width %zu", who, width);
+  if (vocab < 1 || vocab > (1u << 24)) return call_error(B2_ERR_INVALID, "%s: vocab %zu", who, vocab);
+  return B2_OK;
+}
+
+}  // namespace
+
+cudaError_t xent_status_take(unsigned int* code, cudaStream_t s) { return tile_status_take(code, s); }
+
+}  // namespace b2
+
+using namespace b2;
+
+extern "C" {
+
+int b2_xent_workspace(size_t rows, size_t width, size_t vocab, int dtype, int grads, const void* w, size_t ldw, size_t* bytes) {
+  int rc = check_sizes("b2_xent_workspace", rows, width, vocab, dtype);
+  if (rc != B2_OK) return rc;
+  if (!bytes) return call_error(B2_ERR_INVALID, "b2_xent_workspace: null pointer");
+  Space s;
+  *bytes = rows ? space_of(sizes_of(rows, width, vocab, dtype, grads, w, ldw), rows, vocab, grads, nullptr, &s) : 0;
+  return B2_OK;
+}
+
+int b2_xent(size_t rows, size_t width, size_t vocab, int dtype, const void* h, size_t ldh, const void* w, size_t ldw,
+            const void* targets, int token_bytes, float scale, float* row_loss, void* dh, size_t ld_dh, void* dw,
+            size_t ld_dw, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_sizes("b2_xent", rows, width, vocab, dtype);
+  if (rc != B2_OK) return rc;
+  if (token_bytes != 4 && token_bytes != 8) return call_error(B2_ERR_INVALID, "b2_xent: token_bytes is 4 or 8, not %d", token_bytes);
+  if (!w || (rows && (!h || !targets || !row_loss || !workspace))) return call_error(B2_ERR_INVALID, "b2_xent: null pointer");
+  if (ldh < width || ldw < width || (dh && ld_dh < width) || (dw && ld_dw < width))
+    return call_error(B2_ERR_INVALID, "b2_xent: leading dimension smaller than the width");
+  const size_t e = dtype_bytes(dtype);
+  if ((reinterpret_cast<size_t>(h) | reinterpret_cast<size_t>(w) | reinterpret_cast<size_t>(dh) | reinterpret_cast<size_t>(dw)) % e ||
+      reinterpret_cast<size_t>(targets) % token_bytes || reinterpret_cast<size_t>(row_loss) % 4)
+    return call_error(B2_ERR_INVALID, "b2_xent: a pointer is not aligned to its elements");
+  if (reinterpret_cast<size_t>(workspace) % 256) return call_error(B2_ERR_INVALID, "b2_xent: the workspace is not on a 256-byte boundary");
+  const int grads = dh || dw;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  Sizes z{};
+  Space s;
+  if (rows) {
+    z = sizes_of(rows, width, vocab, dtype, grads, w, ldw);
+    const size_t need = space_of(z, rows, vocab, grads, workspace, &s);
+    if (workspace_bytes < need) return call_error(B2_ERR_INVALID, "b2_xent: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  }
+  int sms;
+  if ((rc = lm_device(&sms)) != B2_OK) return rc;
+  if (rows == 0) return dw ? launch_error(cudaMemset2DAsync(dw, ld_dw * e, 0, width * e, vocab, st), "b2_xent") : B2_OK;
+  const XentCall c{rows, width, vocab, dtype, h, ldh, w, ldw, targets, token_bytes == 8, scale, row_loss, dh, ld_dh, dw, ld_dw};
+  return z.split ? xent_run<true>(c, z, s, sms, st) : xent_run<false>(c, z, s, sms, st);
+}
+
+int b2_lm_sync(void* stream) {
+  int sms, rc = lm_device(&sms);
+  if (rc != B2_OK) return rc;
+  unsigned int code = 0;
+  const cudaError_t e = xent_status_take(&code, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return launch_error(e, "b2_lm_sync");
+  if (code) return call_error(B2_ERR_TIMEOUT, "a tile kernel gave up waiting on a pipeline barrier (role %u)", code);
+  return B2_OK;
+}
+
+}  // extern "C"

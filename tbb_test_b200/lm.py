@@ -1,6 +1,8 @@
 """Operators around the layers of a language model, on torch tensors of one GPU.
 
   embed, embed_grad   rows of a table by token number, and the table's gradient
+  xent                softmax cross entropy behind a linear layer as wide as a vocabulary, with its gradients
+  sync                waits for the current stream and raises if a kernel's bounded wait gave up
 
 Thin wrappers over the C ABI (include/b200mlp.h, "Operators around the layers of a language model"): they
 check shapes, types and devices, allocate what is returned, and queue the work on the current torch stream without waiting
@@ -88,3 +90,41 @@ def embed_grad(tokens, dout, vocab, scale=1.0, out=None):
         _ck(K.lib().b2_embed_grad(t.data_ptr(), size, n, p, _DTYPES[dout.dtype], ld, vocab, width, scale, po, ldo,
                                   ws.data_ptr(), ws.numel(), _stream(dout.device)))
     return out
+
+
+def xent(h, w, targets, scale=1.0, grad=True, dh=None, dw=None):
+    """Losses of `h @ w.T` against `targets`, one float32 per row (0 for padding); with `grad` also the gradients of
+    `scale * losses.sum()` with respect to h and w: (losses, dh, dw). `dh` and `dw` may be given to be written to. The logits
+    are never kept (see b2_xent in include/b200mlp.h)."""
+    ph, ldh = _matrix("h", h)
+    rows, width = h.shape
+    device, dtype = h.device, h.dtype
+    pw, ldw = _matrix("w", w, dtype, (w.shape[0], width) if w.dim() == 2 else None, device)
+    vocab = w.shape[0]
+    t, size = _tokens("targets", targets, device)
+    if t.numel() != rows:
+        raise ValueError(f"targets: {t.numel()} for {rows} rows")
+    if not grad and (dh is not None or dw is not None):
+        raise ValueError("dh and dw go with grad=True")
+    loss = torch.empty(rows, dtype=torch.float32, device=device)
+    pdh = pdw = None
+    lddh = lddw = 0
+    if grad:
+        dh = torch.empty(rows, width, dtype=dtype, device=device) if dh is None else dh
+        dw = torch.empty(vocab, width, dtype=dtype, device=device) if dw is None else dw
+        pdh, lddh = _matrix("dh", dh, dtype, (rows, width), device)
+        pdw, lddw = _matrix("dw", dw, dtype, (vocab, width), device)
+    need = C.c_size_t()
+    _ck(K.lib().b2_xent_workspace(rows, width, vocab, _DTYPES[dtype], int(grad), pw, ldw, C.byref(need)))
+    with torch.cuda.device(device):
+        ws = _workspace(need.value, device)
+        _ck(K.lib().b2_xent(rows, width, vocab, _DTYPES[dtype], ph, ldh, pw, ldw, t.data_ptr(), size, scale,
+                            loss.data_ptr(), pdh, lddh, pdw, lddw, ws.data_ptr(), ws.numel(), _stream(device)))
+    return (loss, dh, dw) if grad else loss
+
+
+def sync(device=None):
+    """Waits for the current stream of `device`; K.B2Error with code ERR_TIMEOUT if a bounded wait of a kernel gave up."""
+    device = torch.device("cuda" if device is None else device)
+    with torch.cuda.device(device):
+        _ck(K.lib().b2_lm_sync(_stream(device)))

@@ -419,6 +419,29 @@ int b2_xent(size_t rows, size_t width, size_t vocab, int dtype, const void* h, s
             const void* targets, int token_bytes, float scale, float* row_loss, void* dh, size_t ld_dh, void* dw,
             size_t ld_dw, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Momentum and an orthogonalised update of `count` matrices of one shape (what replaces SGD on the weights of hidden layers):
+ *   m = momentum * m + g       u = g + momentum * m (nesterov) or m       x = u / (|u| + eps)   (Frobenius norm)
+ *   steps times: a = x x', x = (3.4445 I - 4.7750 a + 2.0315 a a) x        (for tall matrices a = x' x, x = x (...))
+ *   w = (1 - lr * weight_decay) * w - lr * scale * x
+ * w[i] and momentum[i] (rows x cols, fp32) are updated in place; copy (or NULL) lists bf16 matrices that receive the new
+ * weights too, as the operands of B2_PREC_BF16 GEMMs; grad[i] is of grad_dtype. The lists themselves are host arrays of
+ * device pointers, read during the call; the matrices of a call may not overlap one another. Products are of fp16 pairs,
+ * 22 bits, with fp32 sums, since rounding errors grow 3.4 times a step; a matrix of zeros stays as it is but for the decay.
+ * Equal inputs give equal bits. */
+typedef struct {
+  float lr, momentum, weight_decay;
+  float scale;  /* of the update: 1, or what the caller's rule makes of the shape, such as 0.2 * sqrt(max(rows, cols)) */
+  float eps;
+  int nesterov;
+  int steps;
+} b2_muon_options;
+/* lr 0.02, momentum 0.95, weight_decay 0, scale 1, eps 1e-7, nesterov 1, steps 5 */
+int b2_muon_options_default(b2_muon_options* options);
+int b2_muon_workspace(int count, int rows, int cols, size_t* bytes);
+int b2_muon(int count, int rows, int cols, int grad_dtype, float* const* w, size_t ld_w, void* const* copy,
+            size_t ld_copy, float* const* momentum, size_t ld_m, const void* const* grad, size_t ld_g,
+            const b2_muon_options* options, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Waits for `stream` and returns B2_ERR_TIMEOUT if a bounded wait inside one of this section's tensor-core kernels on
  * the current device gave up since the last call (their results are then not valid), B2_OK otherwise. */
 int b2_lm_sync(void* stream);

@@ -34,6 +34,11 @@ class Config(C.Structure):
     ]
 
 
+class MuonOptions(C.Structure):
+    _fields_ = [("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float), ("scale", C.c_float),
+                ("eps", C.c_float), ("nesterov", C.c_int), ("steps", C.c_int)]
+
+
 # every symbol include/b200mlp.h declares: name -> (restype, argtypes)
 _H = _vp = C.c_void_p
 _sz = C.c_size_t
@@ -97,6 +102,10 @@ SYMBOLS = {
     "b2_xent_workspace": (C.c_int, [_sz, _sz, _sz, C.c_int, C.c_int, _vp, _sz, C.POINTER(_sz)]),
     "b2_xent": (C.c_int, [_sz, _sz, _sz, C.c_int, _vp, _sz, _vp, _sz, _vp, C.c_int, C.c_float, _vp, _vp, _sz, _vp, _sz,
                           _vp, _sz, _vp]),
+    "b2_muon_options_default": (C.c_int, [C.POINTER(MuonOptions)]),
+    "b2_muon_workspace": (C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(_sz)]),
+    "b2_muon": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(_vp), _sz, C.POINTER(_vp), _sz, C.POINTER(_vp), _sz,
+                          C.POINTER(_vp), _sz, C.POINTER(MuonOptions), _vp, _sz, _vp]),
     "b2_lm_sync": (C.c_int, [_vp]),
 }
 

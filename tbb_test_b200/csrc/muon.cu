@@ -1,0 +1,489 @@
+// Momentum and an orthogonalised update of matrices, by Newton-Schulz products:
+//
+//   m = mu m + g        u = g + mu m (Nesterov) or m        x = u / (|u|_F + eps)
+//   `steps` times:  a = x x'   x = (A I + B a + C a a) x          with A, B, C = 3.4445, -4.7750, 2.0315
+//   w = (1 - lr decay) w - lr scale x
+//
+// The polynomial A s + B s^3 + C s^5 takes every singular value s of x to between 0.7 and 1.2 in five steps, so that the
+// update is x's nearest matrix with equal singular values, roughly. Small singular values grow by A each step, and with
+// them every rounding error of the products before: 485 times in five steps. That is why products are of fp16 pairs
+// (22 bits, lm_tile.cuh) and not of bf16: x is at most 1 in norm and a, B a + C a a stay below 4, so fixed powers of two
+// bring them into fp16's range.
+//
+// With r the smaller and c the larger side of a matrix a step has 2 r^2 c operations for a, 2 r^3 for a a and 2 r^2 c for the
+// new x, all on the tensor cores. a and a a are symmetric: only tiles on and above the diagonal are computed, which stores
+// each tile twice. The smaller side is m for wide matrices and n for tall ones; tall ones are not transposed, as the
+// tile kernel reads operands along either side. A I is added to the middle factor, whose tiles it only touches on the
+// diagonal, so that x is read once per step. The last step's tiles update w as they are finished.
+//
+// Matrices of a call have one shape and go side by side, so that small ones fill the GPU together. Sides are rounded up to
+// 128 with zeros, which stay zeros.
+#include "lm_tile.cuh"
+
+namespace b2 {
+namespace {
+
+constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
+// powers of two on x (norm at most 1.3), a (1.6) and the middle factor (3.5): below fp16's 65504 with room
+constexpr float X_UP = 8192.f, A_UP = 16384.f, P_UP = 8192.f;
+constexpr int MUON_GROUP = 16;   // matrices per launch at most
+constexpr int NORM_PARTS = 256;  // partial sums of a matrix's squares
+
+struct MatrixList {
+  float* w[MUON_GROUP];
+  __nv_bfloat16* copy[MUON_GROUP];
+  float* m[MUON_GROUP];
+  const void* g[MUON_GROUP];
+};
+struct Elementwise {
+  MatrixList list;
+  int rows, cols;
+  long long ld_m, ld_g;
+  int rows_up, cols_up;
+  float mu, eps;
+  int nesterov;
+  double* parts;  // matrices x NORM_PARTS
+  __half *x_hi, *x_lo;
+};
+
+template <typename G>
+__device__ __forceinline__ float update_of(float g, float m, const Elementwise& p) {
+  return p.nesterov ? fmaf(p.mu, m, g) : m;
+}
+
+// m = mu m + g, and the sum of u's squares: each block has its own place for it, so that the sum has one order.
+template <typename G>
+__global__ void __launch_bounds__(256) momentum_kernel(const __grid_constant__ Elementwise p) {
+  __shared__ double part[8];
+  float* m = p.list.m[blockIdx.y];
+  const G* g = static_cast<const G*>(p.list.g[blockIdx.y]);
+  double sum = 0.0;
+  for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    float* mr = m + (long long)r * p.ld_m;
+    const G* gr = g + (long long)r * p.ld_g;
+    for (int c = threadIdx.x; c < p.cols; c += 256) {
+      const float gv = (float)gr[c], mv = fmaf(p.mu, mr[c], gv);
+      mr[c] = mv;
+      const float u = update_of<G>(gv, mv, p);
+      sum += (double)u * u;
+    }
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < 8; ++k) sum += part[k];
+    p.parts[blockIdx.y * NORM_PARTS + blockIdx.x] = sum;
+  }
+}
+
+// x = u / (|u| + eps) as a pair, zeros in the rows and columns that fill up.
+template <typename G>
+__global__ void __launch_bounds__(256) normalise_kernel(const __grid_constant__ Elementwise p, int parts) {
+  __shared__ double part[8];
+  double sum = (int)threadIdx.x < parts ? p.parts[blockIdx.y * NORM_PARTS + threadIdx.x] : 0.0;
+#pragma unroll
+  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  sum = 0.0;
+  for (int k = 0; k < 8; ++k) sum += part[k];
+  const float by = (float)(1.0 / (sqrt(sum) + (double)p.eps));
+  const float* m = p.list.m[blockIdx.y];
+  const G* g = static_cast<const G*>(p.list.g[blockIdx.y]);
+  const size_t base = (size_t)blockIdx.y * p.rows_up * p.cols_up;
+  for (int r = blockIdx.x; r < p.rows_up; r += gridDim.x) {
+    for (int c = threadIdx.x * 4; c < p.cols_up; c += 256 * 4) {
+      __half hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = 0.f;
+        if (r < p.rows && c + i < p.cols)
+          x = update_of<G>(p.nesterov ? (float)g[(long long)r * p.ld_g + c + i] : 0.f, m[(long long)r * p.ld_m + c + i], p) * by;
+        split_half(x * X_UP, hi[i], lo[i]);
+      }
+      const size_t at = base + (size_t)r * p.cols_up + c;
+      *reinterpret_cast<uint2*>(p.x_hi + at) = *reinterpret_cast<const uint2*>(hi);
+      *reinterpret_cast<uint2*>(p.x_lo + at) = *reinterpret_cast<const uint2*>(lo);
+    }
+  }
+}
+
+__device__ __forceinline__ void store_pair(__half* hi, __half* lo, long long at, const float4& x) {
+  const float f[4] = {x.x, x.y, x.z, x.w};
+  __half a[4], b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) split_half(f[i], a[i], b[i]);
+  *reinterpret_cast<uint2*>(hi + at) = *reinterpret_cast<const uint2*>(a);
+  *reinterpret_cast<uint2*>(lo + at) = *reinterpret_cast<const uint2*>(b);
+}
+__device__ __forceinline__ float4 load_pair(const __half* hi, const __half* lo, long long at) {
+  const uint2 a = *reinterpret_cast<const uint2*>(hi + at), b = *reinterpret_cast<const uint2*>(lo + at);
+  const __half2 *ah = reinterpret_cast<const __half2*>(&a), *bh = reinterpret_cast<const __half2*>(&b);
+  const float2 a0 = __half22float2(ah[0]), a1 = __half22float2(ah[1]), b0 = __half22float2(bh[0]), b1 = __half22float2(bh[1]);
+  return make_float4(fmaf(b0.x, 1.f / LO_UP, a0.x), fmaf(b0.y, 1.f / LO_UP, a0.y), fmaf(b1.x, 1.f / LO_UP, a1.x), fmaf(b1.y, 1.f / LO_UP, a1.y));
+}
+
+// ------------------------------------------------------------------ products
+
+// Symmetric results, side x side per matrix: a = x x' (middle 0), or A I + B a + C a a from a a (middle 1).
+struct SymmetricParams {
+  int side, count, kblocks;
+  long long a_step, b_step;  // rows (or k) between matrices in the operands
+  int steps_k;               // 1: matrices lie behind one another along k
+  const __half *a_hi, *a_lo;
+  __half *to_hi, *to_lo;
+};
+template <bool MIDDLE>
+struct SymmetricOp {
+  typedef SymmetricParams Params;
+  static constexpr bool SPLIT = true;
+  const SymmetricParams& p;
+  int m_blocks, n_blocks, per;
+  __device__ explicit SymmetricOp(const SymmetricParams& q) : p(q) {
+    m_blocks = (p.side + TILE_M - 1) / TILE_M;
+    n_blocks = p.side / 128;
+    per = m_blocks * n_blocks - m_blocks * (m_blocks - 1);  // row block i has column blocks 2 i and up
+  }
+  __device__ int tiles() const { return per * p.count; }
+  __device__ Tile tile(int t) const {
+    Tile r;
+    r.z = t / per;
+    int in = t - r.z * per, i = 0;
+    while (in >= n_blocks - 2 * i) in -= n_blocks - 2 * i++;
+    r.m0 = i * TILE_M;
+    r.n0 = (2 * i + in) * 128;
+    const int off = r.z * (int)p.a_step;
+    r.a_mn = r.m0 + (p.steps_k ? 0 : off);
+    r.b_mn = r.n0 + (p.steps_k ? 0 : off);
+    r.a_k = r.b_k = p.steps_k ? off : 0;
+    r.kblocks = p.kblocks;
+    return r;
+  }
+  __device__ __forceinline__ void begin(const Tile&, int, int) {}
+  __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[32], float* stage, int lane) {
+    const long long base = (long long)t.z * p.side * p.side;
+    if (row0 >= p.side) return;  // uniform: sides are multiples of 128
+    const float unit = MIDDLE ? P_UP * NS_C / (A_UP * A_UP) : A_UP / (X_UP * X_UP);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] *= unit;
+    by_rows(row0, col0, v, stage, lane, [&](int r, int c, float4 x) {
+      const long long at = base + (long long)r * p.side + c;
+      if (MIDDLE) {
+        const float4 a = load_pair(p.a_hi, p.a_lo, at);
+        constexpr float b = P_UP * NS_B / A_UP;
+        x = make_float4(fmaf(b, a.x, x.x), fmaf(b, a.y, x.y), fmaf(b, a.z, x.z), fmaf(b, a.w, x.w));
+        if (r == c) x.x += NS_A * P_UP;
+        if (r == c + 1) x.y += NS_A * P_UP;
+        if (r == c + 2) x.z += NS_A * P_UP;
+        if (r == c + 3) x.w += NS_A * P_UP;
+      }
+      store_pair(p.to_hi, p.to_lo, at, x);
+    });
+    if (t.n0 < t.m0 + TILE_M) return;  // on the diagonal both halves are computed
+    by_columns(row0, col0, v, stage, lane, [&](int r, int c, float4 x) {  // r: a column of the tile, c: a row
+      const long long at = base + (long long)r * p.side + c;
+      if (MIDDLE) {
+        constexpr float b = P_UP * NS_B / A_UP;
+        // a at the transposed place, the same value as a there: it is stored twice with the same bits
+        const float4 a = load_pair(p.a_hi, p.a_lo, at);
+        x = make_float4(fmaf(b, a.x, x.x), fmaf(b, a.y, x.y), fmaf(b, a.z, x.z), fmaf(b, a.w, x.w));
+      }
+      store_pair(p.to_hi, p.to_lo, at, x);
+    });
+  }
+  __device__ __forceinline__ void end(const Tile&, int, int) {}
+};
+
+// The new x: middle factor times x (wide) or x times middle factor (tall); the last one updates w instead.
+struct NextParams {
+  MatrixList list;
+  int rows, cols, rows_up, cols_up, count, kblocks, wide;
+  __half *to_hi, *to_lo;
+  long long ld_w, ld_copy;
+  float keep, step;  // w = keep w - step x
+  int vec_w, vec_copy;
+};
+template <bool LAST>
+struct NextOp {
+  typedef NextParams Params;
+  static constexpr bool SPLIT = true;
+  const NextParams& p;
+  int m_blocks, n_blocks;
+  __device__ explicit NextOp(const NextParams& q) : p(q) {
+    m_blocks = (p.rows_up + TILE_M - 1) / TILE_M;
+    n_blocks = p.cols_up / 128;
+  }
+  __device__ int tiles() const { return m_blocks * n_blocks * p.count; }
+  __device__ Tile tile(int t) const {
+    Tile r;
+    const int per = m_blocks * n_blocks;
+    r.z = t / per;
+    const int in = t - r.z * per;
+    // bands of eight row blocks: what the pairs work on at a time is about square
+    const int b = in / (8 * n_blocks), at = in - b * 8 * n_blocks, tall = min(8, m_blocks - 8 * b);
+    r.m0 = (8 * b + at % tall) * TILE_M;
+    r.n0 = at / tall * 128;
+    r.a_mn = r.m0 + r.z * p.rows_up;
+    r.a_k = 0;
+    r.b_mn = r.n0 + (p.wide ? 0 : r.z * p.cols_up);
+    r.b_k = p.wide ? r.z * p.rows_up : 0;
+    r.kblocks = p.kblocks;
+    return r;
+  }
+  __device__ __forceinline__ void begin(const Tile&, int, int) {}
+  __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[32], float* stage, int lane) {
+    if (row0 >= p.rows_up) return;
+    const float unit = LAST ? p.step / (X_UP * P_UP) : 1.f / P_UP;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] *= unit;
+    if (!LAST) {
+      const long long base = (long long)t.z * p.rows_up * p.cols_up;
+      by_rows(row0, col0, v, stage, lane,
+              [&](int r, int c, const float4& x) { store_pair(p.to_hi, p.to_lo, base + (long long)r * p.cols_up + c, x); });
+      return;
+    }
+    float* w = p.list.w[t.z];
+    __nv_bfloat16* copy = p.list.copy[t.z];
+    by_rows(row0, col0, v, stage, lane, [&](int r, int c, const float4& x) {
+      if (r >= p.rows || c >= p.cols) return;
+      float* to = w + (long long)r * p.ld_w + c;
+      float f[4] = {x.x, x.y, x.z, x.w};
+      const bool whole = c + 4 <= p.cols;
+      if (p.vec_w && whole) {
+        const float4 old = *reinterpret_cast<const float4*>(to);
+        f[0] = fmaf(p.keep, old.x, -f[0]);
+        f[1] = fmaf(p.keep, old.y, -f[1]);
+        f[2] = fmaf(p.keep, old.z, -f[2]);
+        f[3] = fmaf(p.keep, old.w, -f[3]);
+        *reinterpret_cast<float4*>(to) = make_float4(f[0], f[1], f[2], f[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (c + i < p.cols) {
+            f[i] = fmaf(p.keep, to[i], -f[i]);
+            to[i] = f[i];
+          }
+      }
+      if (!copy) return;
+      __nv_bfloat16* out = copy + (long long)r * p.ld_copy + c;
+      if (p.vec_copy && whole) {
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (c + i < p.cols) out[i] = __float2bfloat16_rn(f[i]);
+      }
+    });
+  }
+  __device__ __forceinline__ void end(const Tile&, int, int) {}
+};
+
+// ------------------------------------------------------------------ host side
+
+struct MuonSizes {
+  int rows_up, cols_up, side, group;
+};
+MuonSizes muon_sizes(int count, int rows, int cols) {
+  MuonSizes z;
+  z.rows_up = (rows + 127) / 128 * 128;
+  z.cols_up = (cols + 127) / 128 * 128;
+  z.side = rows <= cols ? z.rows_up : z.cols_up;
+  // as many side by side as give every pair of SMs several tiles of the smallest product
+  const long long blocks = z.side / 128, per = (blocks * blocks / 2 + blocks) / 2 + 1;
+  long long group = (4 * 74 + per - 1) / per;
+  if (group > MUON_GROUP) group = MUON_GROUP;
+  z.group = count < group ? count : (int)group;
+  return z;
+}
+struct MuonSpace {
+  double* parts;
+  __half *x_hi[2], *x_lo[2], *a_hi, *a_lo, *p_hi, *p_lo;
+};
+size_t muon_space(const MuonSizes& z, void* base, MuonSpace* s) {
+  Carver c(base);
+  const size_t x = (size_t)z.group * z.rows_up * z.cols_up, a = (size_t)z.group * z.side * z.side;
+  s->parts = c.take<double>((size_t)z.group * NORM_PARTS);
+  for (int i = 0; i < 2; ++i) {
+    s->x_hi[i] = c.take<__half>(x);
+    s->x_lo[i] = c.take<__half>(x);
+  }
+  s->a_hi = c.take<__half>(a);
+  s->a_lo = c.take<__half>(a);
+  s->p_hi = c.take<__half>(a);
+  s->p_lo = c.take<__half>(a);
+  return c.used;
+}
+
+int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_dtype, size_t ld_w, size_t ld_copy, size_t ld_m,
+               size_t ld_g, const b2_muon_options& o, const MuonSizes& z, const MuonSpace& s, int sms, cudaStream_t st) {
+  const char* who = "b2_muon";
+  Elementwise e{};
+  e.list = list;
+  e.rows = rows;
+  e.cols = cols;
+  e.ld_m = (long long)ld_m;
+  e.ld_g = (long long)ld_g;
+  e.rows_up = z.rows_up;
+  e.cols_up = z.cols_up;
+  e.mu = o.momentum;
+  e.eps = o.eps;
+  e.nesterov = o.nesterov;
+  e.parts = s.parts;
+  e.x_hi = s.x_hi[0];
+  e.x_lo = s.x_lo[0];
+  int parts = (8 * sms + count - 1) / count;
+  if (parts > NORM_PARTS) parts = NORM_PARTS;
+  if (parts > rows) parts = rows;
+  const dim3 grid(parts, count), grid2((unsigned int)(z.rows_up < 8 * sms ? z.rows_up : 8 * sms), count);
+  if (grad_dtype == B2_DTYPE_BF16) {
+    momentum_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(e);
+    normalise_kernel<__nv_bfloat16><<<grid2, 256, 0, st>>>(e, parts);
+  } else {
+    momentum_kernel<float><<<grid, 256, 0, st>>>(e);
+    normalise_kernel<float><<<grid2, 256, 0, st>>>(e, parts);
+  }
+  int rc = launch_error(cudaGetLastError(), who);
+  const bool wide = rows <= cols;
+  const long long x_rows = (long long)z.rows_up * count, a_rows = (long long)z.side * count;
+  const long long half_tiles = [&] {
+    const long long m = (z.side + TILE_M - 1) / TILE_M, n = z.side / 128;
+    return (m * n - m * (m - 1)) * count;
+  }();
+  const TileOperand a_op{s.a_hi, s.a_lo, a_rows, z.side, z.side, false}, p_op{s.p_hi, s.p_lo, a_rows, z.side, z.side, false};
+  int at = 0;
+  for (int k = 0; k < o.steps && rc == B2_OK; ++k, at ^= 1) {
+    const TileOperand x_k{s.x_hi[at], s.x_lo[at], x_rows, z.cols_up, z.cols_up, false};
+    const TileOperand x_mn{s.x_hi[at], s.x_lo[at], z.cols_up, x_rows, z.cols_up, true};
+    SymmetricParams q{};
+    q.side = z.side;
+    q.count = count;
+    q.kblocks = (wide ? z.cols_up : z.rows_up) / TILE_K;
+    q.a_step = z.rows_up;
+    q.steps_k = !wide;
+    q.to_hi = s.a_hi;
+    q.to_lo = s.a_lo;
+    rc = tile_launch<SymmetricOp<false>>(who, wide ? x_k : x_mn, wide ? x_k : x_mn, q, false, half_tiles, sms, st);
+    if (rc != B2_OK) return rc;
+    q.kblocks = z.side / TILE_K;
+    q.a_step = z.side;
+    q.steps_k = 0;
+    q.a_hi = s.a_hi;
+    q.a_lo = s.a_lo;
+    q.to_hi = s.p_hi;
+    q.to_lo = s.p_lo;
+    rc = tile_launch<SymmetricOp<true>>(who, a_op, a_op, q, false, half_tiles, sms, st);
+    if (rc != B2_OK) return rc;
+    NextParams n{};
+    n.list = list;
+    n.rows = rows;
+    n.cols = cols;
+    n.rows_up = z.rows_up;
+    n.cols_up = z.cols_up;
+    n.count = count;
+    n.kblocks = z.side / TILE_K;
+    n.wide = wide;
+    n.to_hi = s.x_hi[at ^ 1];
+    n.to_lo = s.x_lo[at ^ 1];
+    n.ld_w = (long long)ld_w;
+    n.ld_copy = (long long)ld_copy;
+    n.keep = (float)(1.0 - (double)o.lr * o.weight_decay);
+    n.step = (float)((double)o.lr * o.scale);
+    n.vec_w = ld_w % 4 == 0;
+    n.vec_copy = ld_copy % 4 == 0;
+    for (int i = 0; i < count; ++i) {
+      if (reinterpret_cast<uintptr_t>(list.w[i]) % 16) n.vec_w = 0;
+      if (reinterpret_cast<uintptr_t>(list.copy[i]) % 8) n.vec_copy = 0;
+    }
+    const long long tiles = (long long)((z.rows_up + TILE_M - 1) / TILE_M) * (z.cols_up / 128) * count;
+    const TileOperand &ao = wide ? p_op : x_k, &bo = wide ? x_mn : p_op;
+    rc = k + 1 == o.steps ? tile_launch<NextOp<true>>(who, ao, bo, n, false, tiles, sms, st)
+                          : tile_launch<NextOp<false>>(who, ao, bo, n, false, tiles, sms, st);
+  }
+  return rc;
+}
+
+int check_muon(const char* who, int count, int rows, int cols) {
+  if (count < 0 || rows < 1 || cols < 1 || rows > 65536 || cols > 65536)
+    return call_error(B2_ERR_INVALID, "%s: %d matrices of %d x %d (sides of 1 to 65536)", who, count, rows, cols);
+  return B2_OK;
+}
+
+}  // namespace
+
+cudaError_t muon_status_take(unsigned int* code, cudaStream_t s) { return tile_status_take(code, s); }
+
+}  // namespace b2
+
+using namespace b2;
+
+extern "C" {
+
+int b2_muon_options_default(b2_muon_options* o) {
+  if (!o) return call_error(B2_ERR_INVALID, "b2_muon_options_default: null pointer");
+  *o = b2_muon_options{0.02f, 0.95f, 0.f, 1.f, 1e-7f, 1, 5};
+  return B2_OK;
+}
+
+int b2_muon_workspace(int count, int rows, int cols, size_t* bytes) {
+  int rc = check_muon("b2_muon_workspace", count, rows, cols);
+  if (rc != B2_OK) return rc;
+  if (!bytes) return call_error(B2_ERR_INVALID, "b2_muon_workspace: null pointer");
+  MuonSpace s;
+  *bytes = muon_space(muon_sizes(count, rows, cols), nullptr, &s);
+  return B2_OK;
+}
+
+int b2_muon(int count, int rows, int cols, int grad_dtype, float* const* w, size_t ld_w, void* const* copy, size_t ld_copy,
+            float* const* momentum, size_t ld_m, const void* const* grad, size_t ld_g, const b2_muon_options* options,
+            void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "b2_muon";
+  int rc = check_muon(who, count, rows, cols);
+  if (rc != B2_OK) return rc;
+  if (!dtype_ok(grad_dtype)) return call_error(B2_ERR_INVALID, "%s: dtype %d", who, grad_dtype);
+  if (!options || (count && (!w || !momentum || !grad || !workspace))) return call_error(B2_ERR_INVALID, "%s: null pointer", who);
+  const size_t c = (size_t)cols;
+  if (ld_w < c || ld_m < c || ld_g < c || (copy && ld_copy < c)) return call_error(B2_ERR_INVALID, "%s: leading dimension smaller than the width", who);
+  if (options->steps < 1 || options->steps > 100) return call_error(B2_ERR_INVALID, "%s: %d steps (1 to 100)", who, options->steps);
+  if (!(options->eps >= 0.f)) return call_error(B2_ERR_INVALID, "%s: eps is negative or not a number", who);
+  for (int i = 0; i < count; ++i) {
+    if (!w[i] || !momentum[i] || !grad[i] || (copy && !copy[i])) return call_error(B2_ERR_INVALID, "%s: null pointer of matrix %d", who, i);
+    if ((reinterpret_cast<uintptr_t>(w[i]) | reinterpret_cast<uintptr_t>(momentum[i])) % 4 ||
+        reinterpret_cast<uintptr_t>(grad[i]) % dtype_bytes(grad_dtype) || (copy && reinterpret_cast<uintptr_t>(copy[i]) % 2))
+      return call_error(B2_ERR_INVALID, "%s: a pointer of matrix %d is not aligned to its elements", who, i);
+  }
+  if (reinterpret_cast<size_t>(workspace) % 256) return call_error(B2_ERR_INVALID, "%s: the workspace is not on a 256-byte boundary", who);
+  if (count == 0) return B2_OK;
+  const MuonSizes z = muon_sizes(count, rows, cols);
+  MuonSpace s;
+  const size_t need = muon_space(z, workspace, &s);
+  if (workspace_bytes < need) return call_error(B2_ERR_INVALID, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, need);
+  int sms;
+  if ((rc = lm_device(&sms)) != B2_OK) return rc;
+  for (int i = 0; i < count && rc == B2_OK; i += z.group) {
+    const int n = count - i < z.group ? count - i : z.group;
+    MatrixList list{};
+    for (int k = 0; k < n; ++k) {
+      list.w[k] = w[i + k];
+      list.copy[k] = copy ? static_cast<__nv_bfloat16*>(copy[i + k]) : nullptr;
+      list.m[k] = momentum[i + k];
+      list.g[k] = grad[i + k];
+    }
+    rc = muon_group(list, n, rows, cols, grad_dtype, ld_w, ld_copy, ld_m, ld_g, *options, z, s, sms, static_cast<cudaStream_t>(stream));
+  }
+  return rc;
+}
+
+int b2_lm_sync(void* stream) {
+  int sms, rc = lm_device(&sms);
+  if (rc != B2_OK) return rc;
+  unsigned int a = 0, b = 0;
+  cudaError_t e = xent_status_take(&a, static_cast<cudaStream_t>(stream));
+  if (e == cudaSuccess) e = muon_status_take(&b, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return launch_error(e, "b2_lm_sync");
+  if (a || b) return call_error(B2_ERR_TIMEOUT, "a tile kernel gave up waiting on a pipeline barrier (role %u)", a ? a : b);
+  return B2_OK;
+}
+
+}  // extern "C"

@@ -658,14 +658,4 @@ int b2_xent(size_t rows, size_t width, size_t vocab, int dtype, const void* h, s
   return z.split ? xent_run<true>(c, z, s, sms, st) : xent_run<false>(c, z, s, sms, st);
 }
 
-int b2_lm_sync(void* stream) {
-  int sms, rc = lm_device(&sms);
-  if (rc != B2_OK) return rc;
-  unsigned int code = 0;
-  const cudaError_t e = xent_status_take(&code, static_cast<cudaStream_t>(stream));
-  if (e != cudaSuccess) return launch_error(e, "b2_lm_sync");
-  if (code) return call_error(B2_ERR_TIMEOUT, "a tile kernel gave up waiting on a pipeline barrier (role %u)", code);
-  return B2_OK;
-}
-
 }  // extern "C"

@@ -2,6 +2,7 @@
 
   embed, embed_grad   rows of a table by token number, and the table's gradient
   xent                softmax cross entropy behind a linear layer as wide as a vocabulary, with its gradients
+  muon                momentum and an orthogonalised update of weight matrices
   sync                waits for the current stream and raises if a kernel's bounded wait gave up
 
 Thin wrappers over the C ABI (include/b200mlp.h, "Operators around the layers of a language model"): they
@@ -121,6 +122,41 @@ def xent(h, w, targets, scale=1.0, grad=True, dh=None, dw=None):
         _ck(K.lib().b2_xent(rows, width, vocab, _DTYPES[dtype], ph, ldh, pw, ldw, t.data_ptr(), size, scale,
                             loss.data_ptr(), pdh, lddh, pdw, lddw, ws.data_ptr(), ws.numel(), _stream(device)))
     return (loss, dh, dw) if grad else loss
+
+
+def _matrices(name, x, dtype, shape, device):
+    """(list of addresses, leading dimension) of equally shaped matrices: a three-dimensional tensor or a sequence of matrices."""
+    xs = list(x.unbind(0)) if isinstance(x, torch.Tensor) and x.dim() == 3 else list(x)
+    got = [_matrix(f"{name}[{i}]", y, dtype, shape, device) for i, y in enumerate(xs)]
+    if len({ld for _, ld in got}) > 1:
+        raise ValueError(f"{name}: the matrices' rows lie at different distances")
+    return [p for p, _ in got], got[0][1] if got else 1
+
+
+def muon(w, momentum_buffer, grad, *, lr, momentum=0.95, nesterov=True, weight_decay=0.0, scale=1.0, eps=1e-7, steps=5, copy=None):
+    """Updates the matrices `w` and their momenta in place (see b2_muon in include/b200mlp.h): sequences of matrices of one
+    shape, or three-dimensional tensors of them. w and momentum_buffer are float32, grad float32 or bfloat16; `copy`, bfloat16,
+    receives the new weights too."""
+    ws = list(w.unbind(0)) if isinstance(w, torch.Tensor) and w.dim() == 3 else list(w)
+    if not ws:
+        raise ValueError("w: no matrices")
+    shape, device = ws[0].shape, ws[0].device
+    gs = list(grad.unbind(0)) if isinstance(grad, torch.Tensor) and grad.dim() == 3 else list(grad)
+    pw, ldw = _matrices("w", ws, torch.float32, shape, device)
+    pm, ldm = _matrices("momentum_buffer", momentum_buffer, torch.float32, shape, device)
+    pg, ldg = _matrices("grad", gs, gs[0].dtype if gs else None, shape, device)
+    pc, ldc = _matrices("copy", copy, torch.bfloat16, shape, device) if copy is not None else (None, 0)
+    if not len(pw) == len(pm) == len(pg) == (len(pc) if pc is not None else len(pw)):
+        raise ValueError("w, momentum_buffer, grad and copy list different numbers of matrices")
+    n = len(pw)
+    arr = lambda ps: None if ps is None else (C.c_void_p * n)(*ps)  # noqa: E731
+    o = K.MuonOptions(lr, momentum, weight_decay, scale, eps, int(nesterov), steps)
+    need = C.c_size_t()
+    _ck(K.lib().b2_muon_workspace(n, shape[0], shape[1], C.byref(need)))
+    with torch.cuda.device(device):
+        ws_ = _workspace(need.value, device)
+        _ck(K.lib().b2_muon(n, shape[0], shape[1], _DTYPES[gs[0].dtype], arr(pw), ldw, arr(pc), ldc, arr(pm), ldm, arr(pg), ldg,
+                            C.byref(o), ws_.data_ptr(), ws_.numel(), _stream(device)))
 
 
 def sync(device=None):

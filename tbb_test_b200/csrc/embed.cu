@@ -64,6 +64,7 @@ __global__ void __launch_bounds__(RANK_THREADS) rank_sort_kernel(const void* __r
                                                                  unsigned int vocab, unsigned int* __restrict__ keys,
                                                                  unsigned int* __restrict__ pos) {
   extern __shared__ unsigned int key_s[];
+  let_next_start();
   for (int i = threadIdx.x; i < n; i += RANK_THREADS) key_s[i] = token_at(tokens, wide, i, vocab);
   __syncthreads();
   const int lane = threadIdx.x & 31;
@@ -91,9 +92,11 @@ __global__ void __launch_bounds__(RANK_THREADS) rank_sort_kernel(const void* __r
 
 // Longer ones: a stable radix sort, lowest digit first, of at most RADIX_TILES tiles of consecutive elements, so that a
 // block finds its digits' first places by reading all tiles' counts itself instead of after a third launch per digit.
-constexpr int RADIX_THREADS = 512, RADIX_WARPS = RADIX_THREADS / 32, RADIX_ROUNDS = 8;
-constexpr int RADIX_STEP = RADIX_THREADS * RADIX_ROUNDS;  // elements a block places at a time
+// A block places RADIX_THREADS * ROUNDS elements at a time: 2 rounds where that gives 64 tiles of few steps, 8 for long lists,
+// whose steps then cost less each.
+constexpr int RADIX_THREADS = 512, RADIX_WARPS = RADIX_THREADS / 32;
 constexpr int RADIX_TILES = 64, RADIX_MOST_BITS = 10;
+constexpr int radix_rounds(size_t n) { return n <= (1u << 18) ? 2 : 8; }
 
 struct RadixPass {
   const void* tokens;  // first pass: keys come from here and positions are their index
@@ -102,7 +105,7 @@ struct RadixPass {
   const unsigned int *keys, *pos;
   unsigned int *keys_out, *pos_out;
   unsigned int* counts;  // tiles x bins
-  unsigned int n, tile;  // elements, elements per tile (a multiple of RADIX_STEP)
+  unsigned int n, tile;  // elements, elements per tile (a multiple of a block's step)
   int tiles, shift, bits;
 };
 __device__ __forceinline__ unsigned int radix_key(const RadixPass& p, unsigned int i) {
@@ -114,6 +117,8 @@ __global__ void __launch_bounds__(RADIX_THREADS) radix_count_kernel(const RadixP
   const int bins = 1 << p.bits;
   for (int b = threadIdx.x; b < bins; b += RADIX_THREADS) count[b] = 0;
   __syncthreads();
+  after_previous();
+  let_next_start();
   const unsigned int begin = blockIdx.x * p.tile, end = min(p.n, begin + p.tile);
   for (unsigned int i = begin + threadIdx.x; i < end; i += RADIX_THREADS)
     atomicAdd(&count[(radix_key(p, i) >> p.shift) & (bins - 1)], 1u);
@@ -121,17 +126,22 @@ __global__ void __launch_bounds__(RADIX_THREADS) radix_count_kernel(const RadixP
   for (int b = threadIdx.x; b < bins; b += RADIX_THREADS) p.counts[(size_t)blockIdx.x * bins + b] = count[b];
 }
 
+template <int RADIX_ROUNDS>
 __global__ void __launch_bounds__(RADIX_THREADS) radix_place_kernel(const RadixPass p) {
+  constexpr int RADIX_STEP = RADIX_THREADS * RADIX_ROUNDS;
   __shared__ unsigned int next[1 << RADIX_MOST_BITS];  // where this tile's next element of a digit goes
   __shared__ unsigned short seen[RADIX_WARPS][1 << RADIX_MOST_BITS];
   __shared__ unsigned int warp_sum[RADIX_WARPS];
   const int bins = 1 << p.bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  after_previous();
+  let_next_start();
   // exclusive sum over digits of all tiles' counts, plus the counts of the tiles before this one
   unsigned int running = 0;
   for (int b0 = 0; b0 < bins; b0 += RADIX_THREADS) {
     const int b = b0 + threadIdx.x;
     unsigned int total = 0, before = 0;
     if (b < bins)
+#pragma unroll 16
       for (int t = 0; t < p.tiles; ++t) {
         const unsigned int c = p.counts[(size_t)t * bins + b];
         total += c;
@@ -158,7 +168,7 @@ __global__ void __launch_bounds__(RADIX_THREADS) radix_place_kernel(const RadixP
   for (unsigned int step = begin; step < end; step += RADIX_STEP) {
     for (int i = threadIdx.x; i < RADIX_WARPS * bins; i += RADIX_THREADS) seen[i >> p.bits][i & (bins - 1)] = 0;
     __syncthreads();
-    // a warp places 256 consecutive elements, 32 at a time: equal digits of a round keep the order of the lanes
+    // a warp places its share of consecutive elements 32 at a time: equal digits of a round keep the order of the lanes
     unsigned int key[RADIX_ROUNDS], pos[RADIX_ROUNDS], place[RADIX_ROUNDS];
     const unsigned int first = step + warp * 32 * RADIX_ROUNDS + lane;
 #pragma unroll
@@ -239,16 +249,19 @@ __device__ __forceinline__ unsigned int lower_bound(const unsigned int* keys, un
 }
 
 constexpr int RUN_THREADS = 128, RUN_AHEAD = 8;
+constexpr int FILL_ROWS = 8;  // rows that a warp looks up and zeroes
 template <typename T, int VB>
 __global__ void __launch_bounds__(RUN_THREADS) run_sum_kernel(const RunSum p) {
   typedef Elems<T, VB> E;
   typedef typename E::raw raw;
+  const int lane = threadIdx.x & 31;
+  after_previous();
+  let_next_start();
   if (blockIdx.x >= p.sum_blocks) {  // rows of tokens that do not occur
-    const int lane = threadIdx.x & 31;
-    const unsigned int v0 = (blockIdx.x - p.sum_blocks) * RUN_THREADS + (threadIdx.x & ~31u);
+    const unsigned int v0 = ((blockIdx.x - p.sum_blocks) * (RUN_THREADS / 32) + (threadIdx.x >> 5)) * FILL_ROWS;
     const unsigned int v = v0 + lane;
     bool absent = false;
-    if (v < p.vocab) {
+    if (lane < FILL_ROWS && v < p.vocab) {
       const unsigned int at = lower_bound(p.keys, p.n, v);
       absent = at == p.n || __ldg(p.keys + at) != v;
     }
@@ -261,18 +274,21 @@ __global__ void __launch_bounds__(RUN_THREADS) run_sum_kernel(const RunSum p) {
     }
     return;
   }
-  const int tpr = 1 << p.tpr_log2;
+  // A unit is a chunk and a slice of columns, worked on by 2^tpr_log2 >= 8 threads. Keys and positions of the next `span` elements
+  // come with one load by the unit's threads and are handed round by shuffles.
+  const int tpr = 1 << p.tpr_log2, span = min(tpr, 32), in_span = lane & (span - 1);
   const unsigned int unit = blockIdx.x * (RUN_THREADS >> p.tpr_log2) + (threadIdx.x >> p.tpr_log2);
   const unsigned int chunk = unit / p.slices;
   const int col = (int)(unit - chunk * p.slices) * tpr + (threadIdx.x & (tpr - 1));
-  if (chunk >= p.chunks || col >= p.vecs) return;
-  const unsigned int begin = chunk * p.chunk, end = min(p.n, begin + p.chunk);
-  unsigned int cur = __ldg(p.keys + begin);
-  bool from_before = begin > 0 && __ldg(p.keys + begin - 1) == cur;
+  const unsigned int begin = chunk * p.chunk, end = chunk < p.chunks ? min(p.n, begin + p.chunk) : begin;
+  const bool works = col < p.vecs;
+  unsigned int cur = begin < end ? __ldg(p.keys + begin) : p.vocab;
+  bool from_before = begin > 0 && begin < end && __ldg(p.keys + begin - 1) == cur;
   float acc[E::N];
 #pragma unroll
   for (int j = 0; j < E::N; ++j) acc[j] = 0.f;
   auto finish = [&](bool goes_on) {
+    if (!works) return;
     if (from_before || goes_on) {
       float* to = (from_before ? p.head : p.tail) + (size_t)chunk * p.pitch + (size_t)col * E::N;
 #pragma unroll
@@ -283,31 +299,39 @@ __global__ void __launch_bounds__(RUN_THREADS) run_sum_kernel(const RunSum p) {
       reinterpret_cast<raw*>(p.dtable + (size_t)cur * p.ld_dtable)[col] = E::put(acc);
     }
   };
-  for (unsigned int i = begin; i < end && cur < p.vocab; i += RUN_AHEAD) {
-    unsigned int key[RUN_AHEAD];
-    raw v[RUN_AHEAD];
+  unsigned int next_key = p.vocab, next_pos = 0;
+  auto fetch = [&](unsigned int i) {
+    next_key = i < end ? __ldg(p.keys + i) : p.vocab;
+    next_pos = i < end ? __ldg(p.pos + i) : 0u;
+  };
+  fetch(begin + in_span);
+  for (unsigned int i = 0; i < p.chunk; i += span) {
+    const unsigned int span_key = next_key, span_pos = next_pos;
+    fetch(begin + i + span + in_span);
+    for (int k0 = 0; k0 < span; k0 += RUN_AHEAD) {
+      unsigned int key[RUN_AHEAD];
+      raw v[RUN_AHEAD];
 #pragma unroll
-    for (int u = 0; u < RUN_AHEAD; ++u) {
-      key[u] = i + u < end ? __ldg(p.keys + i + u) : p.vocab;
-      memset(&v[u], 0, sizeof(raw));
-      if (key[u] < p.vocab) v[u] = __ldg(reinterpret_cast<const raw*>(p.dout + (size_t)__ldg(p.pos + i + u) * p.ld_dout) + col);
-    }
+      for (int u = 0; u < RUN_AHEAD; ++u) {
+        key[u] = __shfl_sync(0xFFFFFFFFu, span_key, k0 + u, span);
+        const unsigned int pos = __shfl_sync(0xFFFFFFFFu, span_pos, k0 + u, span);
+        memset(&v[u], 0, sizeof(raw));
+        if (works && key[u] < p.vocab) v[u] = __ldg(reinterpret_cast<const raw*>(p.dout + (size_t)pos * p.ld_dout) + col);
+      }
 #pragma unroll
-    for (int u = 0; u < RUN_AHEAD; ++u) {
-      if (key[u] != cur) {
-        if (i + u < end) {
-          finish(false);
+      for (int u = 0; u < RUN_AHEAD; ++u) {
+        if (key[u] != cur && begin + i + k0 + u < end) {
+          if (cur < p.vocab) finish(false);
           cur = key[u];
           from_before = false;
 #pragma unroll
           for (int j = 0; j < E::N; ++j) acc[j] = 0.f;
         }
-        if (key[u] >= p.vocab) break;
-      }
-      float f[E::N];
-      E::get(v[u], f);
+        float f[E::N];
+        E::get(v[u], f);  // zeros behind the last element and in place of padding
 #pragma unroll
-      for (int j = 0; j < E::N; ++j) acc[j] += f[j];
+        for (int j = 0; j < E::N; ++j) acc[j] += f[j];
+      }
     }
   }
   if (cur < p.vocab) finish(end < p.n && __ldg(p.keys + end) == cur);
@@ -318,28 +342,46 @@ __global__ void __launch_bounds__(RUN_THREADS) run_sum_kernel(const RunSum p) {
 constexpr int JOIN_PARTS = 8;
 template <typename T>
 __global__ void __launch_bounds__(32 * JOIN_PARTS) run_join_kernel(const RunSum p, int width) {
-  __shared__ float part[JOIN_PARTS][32];
+  __shared__ float4 part[JOIN_PARTS][32];
   const unsigned int chunk = blockIdx.x;
   const unsigned int begin = chunk * p.chunk, end = begin + p.chunk;
+  const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
+  after_previous();
+  let_next_start();
   if (end >= p.n) return;
   const unsigned int key = __ldg(p.keys + end);
   if (key >= p.vocab || __ldg(p.keys + end - 1) != key) return;                                    // nothing goes on
   if (begin > 0 && __ldg(p.keys + begin) == key && __ldg(p.keys + begin - 1) == key) return;  // it began earlier
-  const unsigned int last = (lower_bound(p.keys, p.n, key + 1) - 1) / p.chunk;
+  // the run's last chunk: chunks whose first element has the key
+  unsigned int last = chunk;
+  for (;;) {
+    const size_t at = (size_t)(last + 1 + lane) * p.chunk;
+    const unsigned int same = __ballot_sync(0xFFFFFFFFu, at < p.n && __ldg(p.keys + at) == key);
+    last += same == 0xFFFFFFFFu ? 32 : __ffs(~same) - 1;
+    if (same != 0xFFFFFFFFu) break;
+  }
   const unsigned int count = last - chunk + 1;
-  const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
   const unsigned int from = (unsigned int)((size_t)count * share / JOIN_PARTS), to = (unsigned int)((size_t)count * (share + 1) / JOIN_PARTS);
-  for (int c0 = blockIdx.y * 32; c0 < width; c0 += gridDim.y * 32) {
-    const int c = c0 + lane;
-    float sum = 0.f;
+  for (int c0 = blockIdx.y * 128; c0 < width; c0 += gridDim.y * 128) {
+    const int c = c0 + lane * 4;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     if (c < width)
 #pragma unroll 8
-      for (unsigned int k = from; k < to; ++k) sum += (k == 0 ? p.tail : p.head)[(size_t)(chunk + k) * p.pitch + c];
+      for (unsigned int k = from; k < to; ++k) {
+        const float4 x = *reinterpret_cast<const float4*>((k == 0 ? p.tail : p.head) + (size_t)(chunk + k) * p.pitch + c);
+        sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+      }
     part[share][lane] = sum;
     __syncthreads();
     if (share == 0 && c < width) {
-      for (int s = 1; s < JOIN_PARTS; ++s) sum += part[s][lane];
-      reinterpret_cast<T*>(p.dtable + (size_t)key * p.ld_dtable)[c] = (T)(sum * p.scale);
+      for (int s = 1; s < JOIN_PARTS; ++s) {
+        const float4 x = part[s][lane];
+        sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+      }
+      const float f[4] = {sum.x, sum.y, sum.z, sum.w};
+      T* row = reinterpret_cast<T*>(p.dtable + (size_t)key * p.ld_dtable) + c;
+      for (int i = 0; i < 4; ++i)
+        if (c + i < width) row[i] = (T)(f[i] * p.scale);
     }
     __syncthreads();
   }
@@ -362,8 +404,8 @@ GradPlan grad_plan(size_t n, size_t vocab, size_t width) {
     const int bits = log2_ceil(vocab + 1);
     g.passes = (bits + RADIX_MOST_BITS - 1) / RADIX_MOST_BITS;
     g.bits = (bits + g.passes - 1) / g.passes;
-    const size_t steps = (n + RADIX_STEP - 1) / RADIX_STEP;
-    g.tile = (unsigned int)((steps + RADIX_TILES - 1) / RADIX_TILES * RADIX_STEP);
+    const size_t step = (size_t)RADIX_THREADS * radix_rounds(n), steps = (n + step - 1) / step;
+    g.tile = (unsigned int)((steps + RADIX_TILES - 1) / RADIX_TILES * step);
     g.tiles = (int)((n + g.tile - 1) / g.tile);
   }
   // about eight groups per SM where there are enough elements, and no less than eight elements in a row
@@ -421,16 +463,22 @@ cudaError_t embed_launch(const void* tokens, int wide, size_t n, const void* tab
 }
 
 template <typename T, int VB>
-cudaError_t run_launch(RunSum p, size_t width, cudaStream_t s) {
+void run_launch(RunSum p, size_t width, Chain& chain) {
   p.vecs = (int)(width * sizeof(T) / VB);
   p.tpr_log2 = log2_ceil(p.vecs);
   if (p.tpr_log2 > 7) p.tpr_log2 = 7;
+  if (p.tpr_log2 < 3) p.tpr_log2 = 3;
   p.slices = (p.vecs + (1 << p.tpr_log2) - 1) >> p.tpr_log2;
   const size_t units = (size_t)p.chunks * p.slices, per_block = RUN_THREADS >> p.tpr_log2;
   p.sum_blocks = (unsigned int)((units + per_block - 1) / per_block);
-  const unsigned int fill = (p.vocab + RUN_THREADS - 1) / RUN_THREADS;
-  run_sum_kernel<T, VB><<<p.sum_blocks + fill, RUN_THREADS, 0, s>>>(p);
-  return cudaGetLastError();
+  const unsigned int per_fill = RUN_THREADS / 32 * FILL_ROWS, fill = (p.vocab + per_fill - 1) / per_fill;
+  chain.launch(run_sum_kernel<T, VB>, dim3(p.sum_blocks + fill), RUN_THREADS, 0, 0, p);
+  if (p.chunks > 1) {
+    // most blocks find that no run begins in their chunk and goes on: a few thousand of them at most
+    unsigned int slices = (unsigned int)((width + 127) / 128);
+    while (slices > 1 && (size_t)slices * p.chunks > 8192) slices /= 2;
+    chain.launch(run_join_kernel<T>, dim3(p.chunks, slices), 32 * JOIN_PARTS, 0, 0, p, (int)width);
+  }
 }
 
 }  // namespace
@@ -499,10 +547,12 @@ int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dou
   if (n == 0)
     return launch_error(cudaMemset2DAsync(dtable, ld_dtable * e, 0, width * e, vocab, s), "b2_embed_grad");
   const int wide = token_bytes == 8;
+  Chain chain(s);
   int sorted = 0;
   if (g.passes == 0) {
     const int per_block = RANK_THREADS / 32 * RANK_PER_WARP;
-    rank_sort_kernel<<<(unsigned int)((n + per_block - 1) / per_block), RANK_THREADS, n * 4, s>>>(tokens, wide, (int)n, (unsigned int)vocab, w.keys[0], w.pos[0]);
+    chain.launch(rank_sort_kernel, dim3((unsigned int)((n + per_block - 1) / per_block)), RANK_THREADS, n * 4, 0, tokens, wide, (int)n,
+                 (unsigned int)vocab, w.keys[0], w.pos[0]);
   } else {
     RadixPass p{};
     p.wide = wide;
@@ -520,12 +570,11 @@ int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dou
       p.keys_out = w.keys[sorted];
       p.pos_out = w.pos[sorted];
       p.shift = i * g.bits;
-      radix_count_kernel<<<g.tiles, RADIX_THREADS, 0, s>>>(p);
-      radix_place_kernel<<<g.tiles, RADIX_THREADS, 0, s>>>(p);
+      chain.launch(radix_count_kernel, dim3(g.tiles), RADIX_THREADS, 0, 0, p);
+      if (radix_rounds(n) == 2) chain.launch(radix_place_kernel<2>, dim3(g.tiles), RADIX_THREADS, 0, 0, p);
+      else chain.launch(radix_place_kernel<8>, dim3(g.tiles), RADIX_THREADS, 0, 0, p);
     }
   }
-  cudaError_t err = cudaGetLastError();
-  if (err != cudaSuccess) return launch_error(err, "b2_embed_grad");
   RunSum r{};
   r.keys = w.keys[sorted];
   r.pos = w.pos[sorted];
@@ -542,23 +591,17 @@ int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dou
   r.pitch = g.pitch;
   r.scale = scale;
   const int vb = vector_bytes(e, reinterpret_cast<size_t>(dout) | reinterpret_cast<size_t>(dtable) | width * e | r.ld_dout | r.ld_dtable);
-  if (dtype == B2_DTYPE_BF16)
-    err = vb == 16  ? run_launch<__nv_bfloat16, 16>(r, width, s)
-          : vb == 8 ? run_launch<__nv_bfloat16, 8>(r, width, s)
-          : vb == 4 ? run_launch<__nv_bfloat16, 4>(r, width, s)
-                    : run_launch<__nv_bfloat16, 2>(r, width, s);
-  else
-    err = vb == 16 ? run_launch<float, 16>(r, width, s) : vb == 8 ? run_launch<float, 8>(r, width, s) : run_launch<float, 4>(r, width, s);
-  if (err == cudaSuccess && g.chunks > 1) {
-    // most blocks find that no run begins in their chunk and goes on: a few thousand of them at most
-    unsigned int slices = (unsigned int)((width + 31) / 32);
-    while (slices > 1 && (size_t)slices * g.chunks > 4096) slices /= 2;
-    const dim3 grid(g.chunks, slices);
-    if (dtype == B2_DTYPE_BF16) run_join_kernel<__nv_bfloat16><<<grid, 32 * JOIN_PARTS, 0, s>>>(r, (int)width);
-    else run_join_kernel<float><<<grid, 32 * JOIN_PARTS, 0, s>>>(r, (int)width);
-    err = cudaGetLastError();
+  if (dtype == B2_DTYPE_BF16) {
+    if (vb == 16) run_launch<__nv_bfloat16, 16>(r, width, chain);
+    else if (vb == 8) run_launch<__nv_bfloat16, 8>(r, width, chain);
+    else if (vb == 4) run_launch<__nv_bfloat16, 4>(r, width, chain);
+    else run_launch<__nv_bfloat16, 2>(r, width, chain);
+  } else {
+    if (vb == 16) run_launch<float, 16>(r, width, chain);
+    else if (vb == 8) run_launch<float, 8>(r, width, chain);
+    else run_launch<float, 4>(r, width, chain);
   }
-  return launch_error(err, "b2_embed_grad");
+  return launch_error(chain.err, "b2_embed_grad");
 }
 
 }  // extern "C"

@@ -40,6 +40,48 @@ struct Carver {
   }
 };
 
+// The kernels of a call follow one another by programmatic dependent launch: a kernel may be set up while the one before it
+// ends, and waits in after_previous() until that one's results are there. `first` kernels of a call are launched in the
+// ordinary way, behind whatever the caller's stream holds. Every kernel calls both functions before it reads or writes anything
+// that another kernel of the call touches.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+struct Chain {
+  cudaStream_t stream;
+  bool first;
+  cudaError_t err;
+  explicit Chain(cudaStream_t s) : stream(s), first(true), err(cudaSuccess) {}
+  // cluster: CTAs per cluster, 0 for none
+  template <typename... P, typename... A>
+  void launch(void (*kernel)(P...), dim3 grid, unsigned int threads, size_t smem, int cluster, A&&... args) {
+    if (err != cudaSuccess) return;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (cluster) {
+      attr[n].id = cudaLaunchAttributeClusterDimension;
+      attr[n].val.clusterDim.x = cluster;
+      attr[n].val.clusterDim.y = 1;
+      attr[n].val.clusterDim.z = 1;
+      ++n;
+    }
+    if (!first) {
+      attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[n].val.programmaticStreamSerializationAllowed = 1;
+      ++n;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    err = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    first = false;
+  }
+};
+
 // The widest vector (16, 8 or 4 bytes, or one element) that divides every one of the given addresses and byte counts.
 inline int vector_bytes(size_t elem, size_t bits) {
   for (int v = 16; v > (int)elem; v >>= 1)

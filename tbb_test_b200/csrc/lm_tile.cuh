@@ -31,8 +31,7 @@ namespace {
 constexpr int TILE_M = 256, TILE_K = 64;
 constexpr int TILE_EPI_WARPS = 8;
 constexpr int TILE_THREADS = 64 + 32 * TILE_EPI_WARPS;
-constexpr int STAGE_PITCH = 33;  // floats: conflict-free by rows and by columns
-constexpr int STAGE_WORDS = 32 * STAGE_PITCH;
+constexpr int STAGE_BYTES = 32 * 128;  // a warp's buffer for 32 rows of 128 bytes
 constexpr int SPLIT_SUM = 16;  // k-blocks per hand-over
 constexpr float LO_UP = 2048.f;  // lo = 2^11 (x - hi)
 constexpr uint32_t ACC_COLS = 256;  // tensor-memory columns of an accumulator stage
@@ -46,12 +45,13 @@ struct TileForm {
   static constexpr int BN = SPLIT ? 128 : 256;
   static constexpr int STAGES = SPLIT ? 4 : 6;
   static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128;
-  static constexpr uint32_t STAGE_BYTES = (A_BYTES + B_BYTES) * (SPLIT ? 2 : 1);
-  static constexpr size_t SMEM = 1024 + STAGES * STAGE_BYTES + TILE_EPI_WARPS * STAGE_WORDS * 4;
+  static constexpr uint32_t SLABS = (A_BYTES + B_BYTES) * (SPLIT ? 2 : 1);  // of a stage
+  static constexpr size_t SMEM = 1024 + STAGES * SLABS + TILE_EPI_WARPS * STAGE_BYTES;
 };
 
 struct TileMaps {
   CUtensorMap a, a_lo, b, b_lo;
+  CUtensorMap c;  // of a result that leaves by TMA stores, where the operator has one
 };
 struct TileLayout {
   int a_form, b_form;  // SlabForm
@@ -62,13 +62,14 @@ struct TileLayout {
 struct Tile {
   int m0, n0;
   int a_mn, b_mn, a_k, b_k;
-  int kblocks;
-  int z;  // matrix of a batch
+  int kblocks;  // 0: nothing to sum, the elements are zeros
+  int z;        // the operator's own
 };
 
-// Op: struct Params; static constexpr bool SPLIT; Op(const Params&); int tiles(); Tile tile(int t);
+// Op: struct Params; static constexpr bool SPLIT; Op(const Params&, const TileMaps&); int tiles(); Tile tile(int t);
 //     and in the element warps: void begin(const Tile&, int row, int half); void chunk(const Tile&, int row0, int col0,
-//     float (&v)[32], float* stage, int lane) for 32 columns of rows row0 + lane; void end(const Tile&, int row, int half).
+//     float (&v)[32], uint8_t* stage, int lane) for 32 columns of rows row0 + lane; void end(const Tile&, int row, int half);
+//     static constexpr bool STORES: it issues TMA stores from `stage`.
 template <class Op>
 __global__ void __launch_bounds__(TILE_THREADS, 1) tile_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ TileLayout L,
                                                                const __grid_constant__ typename Op::Params params) {
@@ -112,7 +113,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) tile_kernel(const __grid_cons
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_s;
-  Op op(params);
+  after_previous();
+  let_next_start();
+  Op op(params, maps);
   const int tiles = op.tiles();
 
   if (warp == 0) {
@@ -126,8 +129,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) tile_kernel(const __grid_cons
         const int am = tile.a_mn + (int)rank * 128, bn = tile.b_mn + (int)rank * (F::BN / 2);
         for (int kb = 0; kb < tile.kblocks; ++kb) {
           if (!mbar_wait(empty0 + 8u * stage, phase ^ 1, abort_flag, &tile_status, 1u)) { ok = false; break; }
-          const uint32_t s0 = ring0 + (uint32_t)stage * F::STAGE_BYTES;
-          if (rank == 0) mbar_expect_tx(smem_u32(full_bar) + 8u * stage, 2 * F::STAGE_BYTES);  // both CTAs' bytes
+          const uint32_t s0 = ring0 + (uint32_t)stage * F::SLABS;
+          if (rank == 0) mbar_expect_tx(smem_u32(full_bar) + 8u * stage, 2 * F::SLABS);  // both CTAs' bytes
           const uint32_t full = full0 + 8u * stage;
           const int ka = tile.a_k + kb * TILE_K, kbb = tile.b_k + kb * TILE_K;
           load_slab<true>(&maps.a, full, s0, L.a_form, ka, am, 2, TILE_K * 128, 6);
@@ -165,7 +168,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) tile_kernel(const __grid_cons
           if (!mbar_wait(full0 + 8u * stage, phase, abort_flag, &tile_status, 3u)) { ok = false; break; }
           tc_fence_after();
           const uint32_t d = tmem_base + (uint32_t)acc * ACC_COLS;
-          const uint32_t off = ((uint32_t)stage * F::STAGE_BYTES) >> 4;
+          const uint32_t off = ((uint32_t)stage * F::SLABS) >> 4;
 #pragma unroll
           for (int ks = 0; ks < TILE_K / 16; ++ks) {
             const uint64_t ad = a_tmpl + off + (uint64_t)(ks * a_step), bd = b_tmpl + off + (uint64_t)(ks * b_step);
@@ -189,7 +192,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) tile_kernel(const __grid_cons
   } else {
     const int q = warp & 3, half = (warp - 2) >> 2;
     constexpr int COLS = F::BN / 2;  // columns of this warp
-    float* stage = reinterpret_cast<float*>(smem + F::STAGES * F::STAGE_BYTES) + (warp - 2) * STAGE_WORDS;
+    uint8_t* stage = smem + F::STAGES * F::SLABS + (warp - 2) * STAGE_BYTES;
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
@@ -199,6 +202,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) tile_kernel(const __grid_cons
       const uint32_t lanes = (uint32_t)(q * 32) << 16;
       if (SPLIT) {
         float sum[COLS];
+        if (tile.kblocks == 0) {
+#pragma unroll
+          for (int c = 0; c < COLS; ++c) sum[c] = 0.f;
+        }
         for (int kb = 0; kb < tile.kblocks; kb += SPLIT_SUM) {
           if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_flag, &tile_status, 4u)) { ok = false; break; }
           tc_fence_after();
@@ -232,14 +239,22 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) tile_kernel(const __grid_cons
         op.end(tile, row0 + lane, half);
       } else {
         op.begin(tile, row0 + lane, half);
-        if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_flag, &tile_status, 4u)) break;
-        tc_fence_after();
+        const bool summed = tile.kblocks > 0;
+        if (summed) {
+          if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_flag, &tile_status, 4u)) break;
+          tc_fence_after();
+        }
         const uint32_t from = tmem_base + lanes + (uint32_t)acc * ACC_COLS + (uint32_t)c0;
 #pragma unroll 1
         for (int c = 0; c < COLS; c += 32) {
           uint32_t r[32];
-          tmem_ld32(from + c, r);
-          if (c + 32 == COLS) {  // all read: the next tile may be summed here
+          if (summed) {
+            tmem_ld32(from + c, r);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = 0u;
+          }
+          if (summed && c + 32 == COLS) {  // all read: the next tile may be summed here
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_leader(map_to_cta(smem_u32(&acc_empty_bar[acc]), 0));
@@ -250,10 +265,13 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) tile_kernel(const __grid_cons
           op.chunk(tile, row0, tile.n0 + c0 + c, v, stage, lane);
         }
         op.end(tile, row0 + lane, half);
-        acc ^= 1;
-        if (acc == 0) acc_phase ^= 1;
+        if (summed) {
+          acc ^= 1;
+          if (acc == 0) acc_phase ^= 1;
+        }
       }
     }
+    if (Op::STORES && lane == 0) bulk_wait_all();  // the buffers must outlive the stores that read them
   }
 
   __syncwarp();
@@ -271,38 +289,82 @@ __device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
   lo = __float2half_rn((v - __half2float(hi)) * LO_UP);
 }
 
-// The chunk through shared memory, so that a warp's accesses to global memory cover whole rows: f(row, col, v) gets four
-// neighbouring columns of a row, eight lanes per row, four rows at a time.
-template <class Fn>
-__device__ __forceinline__ void by_rows(int row0, int col0, const float (&v)[32], float* stage, int lane, Fn f) {
+__device__ __forceinline__ void store_pair(__half* hi, __half* lo, long long at, const float4& x) {
+  const float f[4] = {x.x, x.y, x.z, x.w};
+  __half a[4], b[4];
 #pragma unroll
-  for (int j = 0; j < 32; ++j) stage[lane * STAGE_PITCH + j] = v[j];
-  __syncwarp();
+  for (int i = 0; i < 4; ++i) split_half(f[i], a[i], b[i]);
+  *reinterpret_cast<uint2*>(hi + at) = *reinterpret_cast<const uint2*>(a);
+  *reinterpret_cast<uint2*>(lo + at) = *reinterpret_cast<const uint2*>(b);
+}
+__device__ __forceinline__ float4 load_pair(const __half* hi, const __half* lo, long long at) {
+  const uint2 a = *reinterpret_cast<const uint2*>(hi + at), b = *reinterpret_cast<const uint2*>(lo + at);
+  const __half2 *ah = reinterpret_cast<const __half2*>(&a), *bh = reinterpret_cast<const __half2*>(&b);
+  const float2 a0 = __half22float2(ah[0]), a1 = __half22float2(ah[1]), b0 = __half22float2(bh[0]), b1 = __half22float2(bh[1]);
+  return make_float4(fmaf(b0.x, 1.f / LO_UP, a0.x), fmaf(b0.y, 1.f / LO_UP, a0.y), fmaf(b1.x, 1.f / LO_UP, a1.x), fmaf(b1.y, 1.f / LO_UP, a1.y));
+}
+
+// The chunk through shared memory, so that a warp's accesses to global memory cover whole rows: f(row, col, v, old) gets
+// four neighbouring columns of a row, eight lanes per row, four rows at a time, and what load(row, col) read for it before.
+// 16-byte piece j of row r lies at slot j ^ (r & 7): no conflicts either way.
+template <class Load, class Fn>
+__device__ __forceinline__ void by_rows(int row0, int col0, const float (&v)[32], uint8_t* stage, int lane, Load load, Fn f) {
   const int c = (lane & 7) * 4;
+  decltype(load(0, 0)) old[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) old[i] = load(row0 + 4 * i + (lane >> 3), col0 + c);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<float4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  __syncwarp();
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = 4 * i + (lane >> 3);
-    const float* s = stage + r * STAGE_PITCH + c;
-    const float4 x = make_float4(s[0], s[1], s[2], s[3]);
-    f(row0 + r, col0 + c, x);
+    f(row0 + r, col0 + c, *reinterpret_cast<const float4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), old[i]);
   }
   __syncwarp();
 }
-// The same chunk transposed: f(col, row, v) gets four neighbouring rows of a column. Behind by_rows, before the next chunk.
-template <class Fn>
-__device__ __forceinline__ void by_columns(int row0, int col0, const float (&v)[32], float* stage, int lane, Fn f) {
-#pragma unroll
-  for (int j = 0; j < 32; ++j) stage[lane * STAGE_PITCH + j] = v[j];
-  __syncwarp();
+struct Nothing {};
+struct LoadNothing {
+  __device__ __forceinline__ Nothing operator()(int, int) const { return Nothing{}; }
+};
+// The same chunk transposed: f(col, row, v, old) gets four neighbouring rows of a column.
+template <class Load, class Fn>
+__device__ __forceinline__ void by_columns(int row0, int col0, const float (&v)[32], uint8_t* stage, int lane, Load load, Fn f) {
   const int r = (lane & 7) * 4;
+  decltype(load(0, 0)) old[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) old[i] = load(col0 + 4 * i + (lane >> 3), row0 + r);
+#pragma unroll
+  for (int j = 0; j < 32; ++j) *reinterpret_cast<float*>(stage + j * 128 + lane * 4) = v[j];
+  __syncwarp();
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int c = 4 * i + (lane >> 3);
-    const float* s = stage + r * STAGE_PITCH + c;
-    const float4 x = make_float4(s[0], s[STAGE_PITCH], s[2 * STAGE_PITCH], s[3 * STAGE_PITCH]);
-    f(col0 + c, row0 + r, x);
+    f(col0 + c, row0 + r, *reinterpret_cast<const float4*>(stage + c * 128 + r * 4), old[i]);
   }
   __syncwarp();
+}
+// 32 columns of 16-bit elements into columns 32 * part and up of a buffer of 64, in the swizzle that TMA stores undo; with
+// the second part the buffer leaves for column col, row row of the map's matrix. The first part waits until the store
+// before has read the buffer.
+__device__ __forceinline__ void store_half_words(const CUtensorMap* map, const uint32_t (&w)[16], int part, int row, int col, uint8_t* stage,
+                                                 int lane) {
+  if (part == 0) {
+    if (lane == 0) bulk_wait_read<0>();
+    __syncwarp();
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<uint4*>(stage + lane * 128 + (((part * 4 + j) ^ (lane & 7)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+  if (part == 1) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(map, stage, col, row);
+      bulk_commit();
+    }
+  }
 }
 
 // ------------------------------------------------------------------ host side
@@ -345,32 +407,30 @@ inline bool tile_maps(const TileOperand& a, const TileOperand& b, bool split, bo
   return ok;
 }
 
+// A row-major matrix of 16-bit elements that store_half_words writes to.
+struct TileResult {
+  void* p;
+  long long rows, cols, ld;
+};
+
 // most_tiles: an upper bound on the tiles that the kernel will find.
 template <class Op>
-int tile_launch(const char* who, const TileOperand& a, const TileOperand& b, const typename Op::Params& p, bool bf16, long long most_tiles,
-                int sms, cudaStream_t s) {
+int tile_launch(const char* who, const TileOperand& a, const TileOperand& b, const TileResult* c, const typename Op::Params& p, bool bf16,
+                long long most_tiles, int sms, Chain& chain) {
   if (most_tiles <= 0) return B2_OK;
   TileMaps maps;
   TileLayout L;
-  if (!tile_maps(a, b, Op::SPLIT, bf16, &maps, &L)) return call_error(B2_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", who);
+  bool ok = tile_maps(a, b, Op::SPLIT, bf16, &maps, &L);
+  if (c) ok = ok && make_map(&maps.c, c->p, 2, c->cols, c->rows, c->ld, 64, 32, 0);
+  else maps.c = maps.a;
+  if (!ok) return call_error(B2_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", who);
   const size_t smem = TileForm<Op::SPLIT>::SMEM;
   cudaError_t e = cudaFuncSetAttribute(tile_kernel<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return launch_error(e, who);
   const int pairs = sms / 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * (unsigned int)(most_tiles < pairs ? most_tiles : pairs));
-  cfg.blockDim = dim3(TILE_THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, tile_kernel<Op>, maps, L, p);
-  return launch_error(e, who);
+  const unsigned int grid = 2 * (unsigned int)(most_tiles < pairs ? most_tiles : pairs);
+  chain.launch(tile_kernel<Op>, dim3(grid), TILE_THREADS, smem, 2, maps, L, p);
+  return launch_error(chain.err, who);
 }
 
 // What a wait that gave up left in this file's status word, which is cleared; the stream is waited for.

@@ -46,26 +46,52 @@ struct Elementwise {
   __half *x_hi, *x_lo;
 };
 
-template <typename G>
 __device__ __forceinline__ float update_of(float g, float m, const Elementwise& p) {
   return p.nesterov ? fmaf(p.mu, m, g) : m;
 }
 
-// m = mu m + g, and the sum of u's squares: each block has its own place for it, so that the sum has one order.
-template <typename G>
+// m = mu m + g, and the sum of u's squares: each block has its own place for it, so that the sum has one order. VEC: rows
+// are whole groups of four elements on 16-byte (g: 8-byte) boundaries.
+template <typename G, bool VEC>
 __global__ void __launch_bounds__(256) momentum_kernel(const __grid_constant__ Elementwise p) {
   __shared__ double part[8];
   float* m = p.list.m[blockIdx.y];
   const G* g = static_cast<const G*>(p.list.g[blockIdx.y]);
+  let_next_start();
   double sum = 0.0;
-  for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
-    float* mr = m + (long long)r * p.ld_m;
-    const G* gr = g + (long long)r * p.ld_g;
-    for (int c = threadIdx.x; c < p.cols; c += 256) {
-      const float gv = (float)gr[c], mv = fmaf(p.mu, mr[c], gv);
-      mr[c] = mv;
-      const float u = update_of<G>(gv, mv, p);
-      sum += (double)u * u;
+  constexpr int E = VEC ? 4 : 1, AHEAD = 4;
+  const int per_row = p.cols / E;
+  const long long all = (long long)p.rows * per_row, stride = (long long)gridDim.x * 256;
+  for (long long i0 = (long long)blockIdx.x * 256 + threadIdx.x; i0 < all; i0 += stride * AHEAD) {
+    typedef Elems<float, 4 * E> M;
+    typedef Elems<G, (int)sizeof(G) * E> V;
+    typename M::raw mr[AHEAD];
+    typename V::raw gr[AHEAD];
+    float* to[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const long long i = i0 + u * stride;
+      to[u] = nullptr;
+      if (i < all) {
+        const int r = (int)(i / per_row), c = (int)(i - (long long)r * per_row) * E;
+        to[u] = m + (long long)r * p.ld_m + c;
+        mr[u] = *reinterpret_cast<const typename M::raw*>(to[u]);
+        gr[u] = __ldg(reinterpret_cast<const typename V::raw*>(g + (long long)r * p.ld_g + c));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      if (!to[u]) continue;
+      float mv[E], gv[E];
+      M::get(mr[u], mv);
+      V::get(gr[u], gv);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        mv[e] = fmaf(p.mu, mv[e], gv[e]);
+        const double x = update_of(gv[e], mv[e], p);
+        sum = fma(x, x, sum);
+      }
+      *reinterpret_cast<typename M::raw*>(to[u]) = M::put(mv);
     }
   }
 #pragma unroll
@@ -79,9 +105,11 @@ __global__ void __launch_bounds__(256) momentum_kernel(const __grid_constant__ E
 }
 
 // x = u / (|u| + eps) as a pair, zeros in the rows and columns that fill up.
-template <typename G>
+template <typename G, bool VEC>
 __global__ void __launch_bounds__(256) normalise_kernel(const __grid_constant__ Elementwise p, int parts) {
   __shared__ double part[8];
+  after_previous();
+  let_next_start();
   double sum = (int)threadIdx.x < parts ? p.parts[blockIdx.y * NORM_PARTS + threadIdx.x] : 0.0;
 #pragma unroll
   for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
@@ -93,36 +121,35 @@ __global__ void __launch_bounds__(256) normalise_kernel(const __grid_constant__ 
   const float* m = p.list.m[blockIdx.y];
   const G* g = static_cast<const G*>(p.list.g[blockIdx.y]);
   const size_t base = (size_t)blockIdx.y * p.rows_up * p.cols_up;
-  for (int r = blockIdx.x; r < p.rows_up; r += gridDim.x) {
-    for (int c = threadIdx.x * 4; c < p.cols_up; c += 256 * 4) {
-      __half hi[4], lo[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x = 0.f;
-        if (r < p.rows && c + i < p.cols)
-          x = update_of<G>(p.nesterov ? (float)g[(long long)r * p.ld_g + c + i] : 0.f, m[(long long)r * p.ld_m + c + i], p) * by;
-        split_half(x * X_UP, hi[i], lo[i]);
+  const int per_row = p.cols_up / 4;
+  const long long all = (long long)p.rows_up * per_row, stride = (long long)gridDim.x * 256;
+#pragma unroll 4
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += stride) {
+    const int r = (int)(i / per_row), c = (int)(i - (long long)r * per_row) * 4;
+    const float* mr = m + (long long)r * p.ld_m + c;
+    const G* gr = g + (long long)r * p.ld_g + c;
+    float mv[4] = {0.f, 0.f, 0.f, 0.f}, gv[4] = {0.f, 0.f, 0.f, 0.f};
+    if (VEC) {
+      if (r < p.rows && c < p.cols) {
+        Elems<float, 16>::get(*reinterpret_cast<const uint4*>(mr), mv);
+        typedef Elems<G, 4 * (int)sizeof(G)> V;
+        if (p.nesterov) V::get(__ldg(reinterpret_cast<const typename V::raw*>(gr)), gv);
       }
-      const size_t at = base + (size_t)r * p.cols_up + c;
-      *reinterpret_cast<uint2*>(p.x_hi + at) = *reinterpret_cast<const uint2*>(hi);
-      *reinterpret_cast<uint2*>(p.x_lo + at) = *reinterpret_cast<const uint2*>(lo);
-    }
-  }
-}
-
-__device__ __forceinline__ void store_pair(__half* hi, __half* lo, long long at, const float4& x) {
-  const float f[4] = {x.x, x.y, x.z, x.w};
-  __half a[4], b[4];
+    } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) split_half(f[i], a[i], b[i]);
-  *reinterpret_cast<uint2*>(hi + at) = *reinterpret_cast<const uint2*>(a);
-  *reinterpret_cast<uint2*>(lo + at) = *reinterpret_cast<const uint2*>(b);
-}
-__device__ __forceinline__ float4 load_pair(const __half* hi, const __half* lo, long long at) {
-  const uint2 a = *reinterpret_cast<const uint2*>(hi + at), b = *reinterpret_cast<const uint2*>(lo + at);
-  const __half2 *ah = reinterpret_cast<const __half2*>(&a), *bh = reinterpret_cast<const __half2*>(&b);
-  const float2 a0 = __half22float2(ah[0]), a1 = __half22float2(ah[1]), b0 = __half22float2(bh[0]), b1 = __half22float2(bh[1]);
-  return make_float4(fmaf(b0.x, 1.f / LO_UP, a0.x), fmaf(b0.y, 1.f / LO_UP, a0.y), fmaf(b1.x, 1.f / LO_UP, a1.x), fmaf(b1.y, 1.f / LO_UP, a1.y));
+      for (int e = 0; e < 4; ++e)
+        if (r < p.rows && c + e < p.cols) {
+          mv[e] = mr[e];
+          if (p.nesterov) gv[e] = (float)gr[e];
+        }
+    }
+    __half hi[4], lo[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split_half(update_of(gv[e], mv[e], p) * by * X_UP, hi[e], lo[e]);
+    const size_t at = base + (size_t)r * p.cols_up + c;
+    *reinterpret_cast<uint2*>(p.x_hi + at) = *reinterpret_cast<const uint2*>(hi);
+    *reinterpret_cast<uint2*>(p.x_lo + at) = *reinterpret_cast<const uint2*>(lo);
+  }
 }
 
 // ------------------------------------------------------------------ products
@@ -138,10 +165,10 @@ struct SymmetricParams {
 template <bool MIDDLE>
 struct SymmetricOp {
   typedef SymmetricParams Params;
-  static constexpr bool SPLIT = true;
+  static constexpr bool SPLIT = true, STORES = false;
   const SymmetricParams& p;
   int m_blocks, n_blocks, per;
-  __device__ explicit SymmetricOp(const SymmetricParams& q) : p(q) {
+  __device__ explicit SymmetricOp(const SymmetricParams& q, const TileMaps&) : p(q) {
     m_blocks = (p.side + TILE_M - 1) / TILE_M;
     n_blocks = p.side / 128;
     per = m_blocks * n_blocks - m_blocks * (m_blocks - 1);  // row block i has column blocks 2 i and up
@@ -162,36 +189,31 @@ struct SymmetricOp {
     return r;
   }
   __device__ __forceinline__ void begin(const Tile&, int, int) {}
-  __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[32], float* stage, int lane) {
+  __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[32], uint8_t* stage, int lane) {
     const long long base = (long long)t.z * p.side * p.side;
     if (row0 >= p.side) return;  // uniform: sides are multiples of 128
     const float unit = MIDDLE ? P_UP * NS_C / (A_UP * A_UP) : A_UP / (X_UP * X_UP);
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] *= unit;
-    by_rows(row0, col0, v, stage, lane, [&](int r, int c, float4 x) {
-      const long long at = base + (long long)r * p.side + c;
-      if (MIDDLE) {
-        const float4 a = load_pair(p.a_hi, p.a_lo, at);
-        constexpr float b = P_UP * NS_B / A_UP;
-        x = make_float4(fmaf(b, a.x, x.x), fmaf(b, a.y, x.y), fmaf(b, a.z, x.z), fmaf(b, a.w, x.w));
+    if constexpr (MIDDLE) {
+      constexpr float b = P_UP * NS_B / A_UP;
+      auto load = [&](int r, int c) { return load_pair(p.a_hi, p.a_lo, base + (long long)r * p.side + c); };
+      auto store = [&](int r, int c, const float4& y, const float4& a) {
+        float4 x = make_float4(fmaf(b, a.x, y.x), fmaf(b, a.y, y.y), fmaf(b, a.z, y.z), fmaf(b, a.w, y.w));
         if (r == c) x.x += NS_A * P_UP;
         if (r == c + 1) x.y += NS_A * P_UP;
         if (r == c + 2) x.z += NS_A * P_UP;
         if (r == c + 3) x.w += NS_A * P_UP;
-      }
-      store_pair(p.to_hi, p.to_lo, at, x);
-    });
-    if (t.n0 < t.m0 + TILE_M) return;  // on the diagonal both halves are computed
-    by_columns(row0, col0, v, stage, lane, [&](int r, int c, float4 x) {  // r: a column of the tile, c: a row
-      const long long at = base + (long long)r * p.side + c;
-      if (MIDDLE) {
-        constexpr float b = P_UP * NS_B / A_UP;
-        // a at the transposed place, the same value as a there: it is stored twice with the same bits
-        const float4 a = load_pair(p.a_hi, p.a_lo, at);
-        x = make_float4(fmaf(b, a.x, x.x), fmaf(b, a.y, x.y), fmaf(b, a.z, x.z), fmaf(b, a.w, x.w));
-      }
-      store_pair(p.to_hi, p.to_lo, at, x);
-    });
+        store_pair(p.to_hi, p.to_lo, base + (long long)r * p.side + c, x);
+      };
+      by_rows(row0, col0, v, stage, lane, load, store);
+      // on the diagonal both halves are computed; elsewhere a at the transposed place, which holds the same bits
+      if (t.n0 >= t.m0 + TILE_M) by_columns(row0, col0, v, stage, lane, load, store);
+    } else {
+      auto store = [&](int r, int c, const float4& x, Nothing) { store_pair(p.to_hi, p.to_lo, base + (long long)r * p.side + c, x); };
+      by_rows(row0, col0, v, stage, lane, LoadNothing(), store);
+      if (t.n0 >= t.m0 + TILE_M) by_columns(row0, col0, v, stage, lane, LoadNothing(), store);
+    }
   }
   __device__ __forceinline__ void end(const Tile&, int, int) {}
 };
@@ -208,10 +230,10 @@ struct NextParams {
 template <bool LAST>
 struct NextOp {
   typedef NextParams Params;
-  static constexpr bool SPLIT = true;
+  static constexpr bool SPLIT = true, STORES = false;
   const NextParams& p;
   int m_blocks, n_blocks;
-  __device__ explicit NextOp(const NextParams& q) : p(q) {
+  __device__ explicit NextOp(const NextParams& q, const TileMaps&) : p(q) {
     m_blocks = (p.rows_up + TILE_M - 1) / TILE_M;
     n_blocks = p.cols_up / 128;
   }
@@ -233,38 +255,46 @@ struct NextOp {
     return r;
   }
   __device__ __forceinline__ void begin(const Tile&, int, int) {}
-  __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[32], float* stage, int lane) {
+  __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[32], uint8_t* stage, int lane) {
     if (row0 >= p.rows_up) return;
     const float unit = LAST ? p.step / (X_UP * P_UP) : 1.f / P_UP;
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] *= unit;
     if (!LAST) {
       const long long base = (long long)t.z * p.rows_up * p.cols_up;
-      by_rows(row0, col0, v, stage, lane,
-              [&](int r, int c, const float4& x) { store_pair(p.to_hi, p.to_lo, base + (long long)r * p.cols_up + c, x); });
+      by_rows(row0, col0, v, stage, lane, LoadNothing(), [&](int r, int c, const float4& x, Nothing) {
+        store_pair(p.to_hi, p.to_lo, base + (long long)r * p.cols_up + c, x);
+      });
       return;
     }
     float* w = p.list.w[t.z];
     __nv_bfloat16* copy = p.list.copy[t.z];
-    by_rows(row0, col0, v, stage, lane, [&](int r, int c, const float4& x) {
+    auto load = [&](int r, int c) {
+      float4 old = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < p.rows && c < p.cols) {
+        const float* from = w + (long long)r * p.ld_w + c;
+        if (p.vec_w && c + 4 <= p.cols) {
+          old = *reinterpret_cast<const float4*>(from);
+        } else {
+          old.x = from[0];
+          if (c + 1 < p.cols) old.y = from[1];
+          if (c + 2 < p.cols) old.z = from[2];
+          if (c + 3 < p.cols) old.w = from[3];
+        }
+      }
+      return old;
+    };
+    by_rows(row0, col0, v, stage, lane, load, [&](int r, int c, const float4& x, const float4& old) {
       if (r >= p.rows || c >= p.cols) return;
+      const float f[4] = {fmaf(p.keep, old.x, -x.x), fmaf(p.keep, old.y, -x.y), fmaf(p.keep, old.z, -x.z), fmaf(p.keep, old.w, -x.w)};
       float* to = w + (long long)r * p.ld_w + c;
-      float f[4] = {x.x, x.y, x.z, x.w};
       const bool whole = c + 4 <= p.cols;
       if (p.vec_w && whole) {
-        const float4 old = *reinterpret_cast<const float4*>(to);
-        f[0] = fmaf(p.keep, old.x, -f[0]);
-        f[1] = fmaf(p.keep, old.y, -f[1]);
-        f[2] = fmaf(p.keep, old.z, -f[2]);
-        f[3] = fmaf(p.keep, old.w, -f[3]);
         *reinterpret_cast<float4*>(to) = make_float4(f[0], f[1], f[2], f[3]);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (c + i < p.cols) {
-            f[i] = fmaf(p.keep, to[i], -f[i]);
-            to[i] = f[i];
-          }
+          if (c + i < p.cols) to[i] = f[i];
       }
       if (!copy) return;
       __nv_bfloat16* out = copy + (long long)r * p.ld_copy + c;
@@ -333,18 +363,29 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
   e.parts = s.parts;
   e.x_hi = s.x_hi[0];
   e.x_lo = s.x_lo[0];
-  int parts = (8 * sms + count - 1) / count;
-  if (parts > NORM_PARTS) parts = NORM_PARTS;
-  if (parts > rows) parts = rows;
-  const dim3 grid(parts, count), grid2((unsigned int)(z.rows_up < 8 * sms ? z.rows_up : 8 * sms), count);
+  bool vec = cols % 4 == 0 && ld_m % 4 == 0 && ld_g % 4 == 0;
+  for (int i = 0; i < count; ++i)
+    if (reinterpret_cast<uintptr_t>(list.m[i]) % 16 || reinterpret_cast<uintptr_t>(list.g[i]) % (4 * dtype_bytes(grad_dtype))) vec = false;
+  auto blocks = [&](long long threads, int most) {  // of a matrix: eight per SM over all of them
+    long long n = (threads + 255) / 256, fair = (8 * sms + count - 1) / count;
+    if (n > fair) n = fair;
+    return (int)(n > most ? most : n);
+  };
+  const int parts = blocks((long long)rows * cols / (vec ? 16 : 4) + 1, NORM_PARTS);
+  const dim3 grid(parts, count), grid2(blocks((long long)z.rows_up * z.cols_up / 8, 1 << 20), count);
+  Chain chain(st);
+  auto start = [&](auto momentum, auto normalise) {
+    chain.launch(momentum, grid, 256, 0, 0, e);
+    chain.launch(normalise, grid2, 256, 0, 0, e, parts);
+  };
   if (grad_dtype == B2_DTYPE_BF16) {
-    momentum_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(e);
-    normalise_kernel<__nv_bfloat16><<<grid2, 256, 0, st>>>(e, parts);
+    if (vec) start(momentum_kernel<__nv_bfloat16, true>, normalise_kernel<__nv_bfloat16, true>);
+    else start(momentum_kernel<__nv_bfloat16, false>, normalise_kernel<__nv_bfloat16, false>);
   } else {
-    momentum_kernel<float><<<grid, 256, 0, st>>>(e);
-    normalise_kernel<float><<<grid2, 256, 0, st>>>(e, parts);
+    if (vec) start(momentum_kernel<float, true>, normalise_kernel<float, true>);
+    else start(momentum_kernel<float, false>, normalise_kernel<float, false>);
   }
-  int rc = launch_error(cudaGetLastError(), who);
+  int rc = launch_error(chain.err, who);
   const bool wide = rows <= cols;
   const long long x_rows = (long long)z.rows_up * count, a_rows = (long long)z.side * count;
   const long long half_tiles = [&] {
@@ -364,7 +405,7 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
     q.steps_k = !wide;
     q.to_hi = s.a_hi;
     q.to_lo = s.a_lo;
-    rc = tile_launch<SymmetricOp<false>>(who, wide ? x_k : x_mn, wide ? x_k : x_mn, q, false, half_tiles, sms, st);
+    rc = tile_launch<SymmetricOp<false>>(who, wide ? x_k : x_mn, wide ? x_k : x_mn, nullptr, q, false, half_tiles, sms, chain);
     if (rc != B2_OK) return rc;
     q.kblocks = z.side / TILE_K;
     q.a_step = z.side;
@@ -373,7 +414,7 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
     q.a_lo = s.a_lo;
     q.to_hi = s.p_hi;
     q.to_lo = s.p_lo;
-    rc = tile_launch<SymmetricOp<true>>(who, a_op, a_op, q, false, half_tiles, sms, st);
+    rc = tile_launch<SymmetricOp<true>>(who, a_op, a_op, nullptr, q, false, half_tiles, sms, chain);
     if (rc != B2_OK) return rc;
     NextParams n{};
     n.list = list;
@@ -398,8 +439,8 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
     }
     const long long tiles = (long long)((z.rows_up + TILE_M - 1) / TILE_M) * (z.cols_up / 128) * count;
     const TileOperand &ao = wide ? p_op : x_k, &bo = wide ? x_mn : p_op;
-    rc = k + 1 == o.steps ? tile_launch<NextOp<true>>(who, ao, bo, n, false, tiles, sms, st)
-                          : tile_launch<NextOp<false>>(who, ao, bo, n, false, tiles, sms, st);
+    rc = k + 1 == o.steps ? tile_launch<NextOp<true>>(who, ao, bo, nullptr, n, false, tiles, sms, chain)
+                          : tile_launch<NextOp<false>>(who, ao, bo, nullptr, n, false, tiles, sms, chain);
   }
   return rc;
 }

@@ -48,52 +48,44 @@ __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) <
 
 // ------------------------------------------------------------------ rows with a target
 
-constexpr int LIST_THREADS = 1024, LIST_EACH = 8;
-__global__ void __launch_bounds__(LIST_THREADS) list_rows_kernel(const void* __restrict__ targets, int wide, int rows,
+// Each block lists its own share of the rows, behind the rows that it counts in the shares before.
+constexpr int LIST_THREADS = 1024, LIST_BLOCKS = 32;
+__global__ void __launch_bounds__(LIST_THREADS) list_rows_kernel(const void* __restrict__ targets, int wide, int rows, int share,
                                                                  unsigned int vocab, Meta* meta, int* __restrict__ row_of,
                                                                  int* __restrict__ slot_of, int* __restrict__ target,
                                                                  float* __restrict__ row_loss) {
   __shared__ unsigned int warp_sum[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned int base = 0;
-  for (int r0 = 0; r0 < rows; r0 += LIST_THREADS * LIST_EACH) {
-    const int first = r0 + threadIdx.x * LIST_EACH;
-    unsigned int t[LIST_EACH], mine = 0;
-#pragma unroll
-    for (int k = 0; k < LIST_EACH; ++k) {
-      t[k] = first + k < rows ? token_at(targets, wide, first + k, vocab) : vocab;
-      mine += t[k] < vocab;
-    }
-    unsigned int scan = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const unsigned int up = __shfl_up_sync(0xFFFFFFFFu, scan, d);
-      if (lane >= d) scan += up;
-    }
-    if (lane == 31) warp_sum[warp] = scan;
+  let_next_start();
+  const int begin = blockIdx.x * share, end = min(rows, begin + share);
+  auto block_sum = [&](unsigned int mine) {  // over all threads; the warps' sums stay in warp_sum
+    const unsigned int sum = __reduce_add_sync(0xFFFFFFFFu, mine);
     __syncthreads();
-    unsigned int before = 0, all = 0;
-    for (int w = 0; w < 32; ++w) {
-      before += w < warp ? warp_sum[w] : 0u;
-      all += warp_sum[w];
-    }
-    unsigned int at = base + before + scan - mine;
-#pragma unroll
-    for (int k = 0; k < LIST_EACH; ++k) {
-      if (first + k >= rows) break;
-      if (t[k] < vocab) {
-        row_of[at] = first + k;
-        target[at] = (int)t[k];
-        slot_of[first + k] = (int)at++;
-      } else {
-        slot_of[first + k] = -1;
-        row_loss[first + k] = 0.f;
-      }
+    if (lane == 0) warp_sum[warp] = sum;
+    __syncthreads();
+    return __reduce_add_sync(0xFFFFFFFFu, warp_sum[lane]);
+  };
+  unsigned int before = 0;
+#pragma unroll 4
+  for (int r = threadIdx.x; r < begin; r += LIST_THREADS) before += token_at(targets, wide, r, vocab) < vocab;
+  unsigned int base = block_sum(before);
+  for (int r0 = begin; r0 < end; r0 += LIST_THREADS) {
+    const int r = r0 + threadIdx.x;
+    const unsigned int t = r < end ? token_at(targets, wide, r, vocab) : vocab;
+    const unsigned int have = __ballot_sync(0xFFFFFFFFu, t < vocab);
+    const unsigned int all = block_sum(t < vocab ? 1u : 0u);
+    const unsigned int at = base + __reduce_add_sync(0xFFFFFFFFu, lane < warp ? warp_sum[lane] : 0u) + __popc(have & ((1u << lane) - 1));
+    if (t < vocab) {
+      row_of[at] = r;
+      target[at] = (int)t;
+      slot_of[r] = (int)at;
+    } else if (r < end) {
+      slot_of[r] = -1;
+      row_loss[r] = 0.f;
     }
     base += all;
-    __syncthreads();
   }
-  if (threadIdx.x == 0) *meta = Meta{base, 0u, 0u};
+  if (end == rows && threadIdx.x == 0) *meta = Meta{base, 0u, 0u};
 }
 
 __device__ __forceinline__ int row_blocks(unsigned int rows) { return max(1, (int)((rows + TILE_M - 1) / TILE_M)); }
@@ -102,13 +94,16 @@ __device__ __forceinline__ int row_blocks(unsigned int rows) { return max(1, (in
 __global__ void __launch_bounds__(256) max_kernel(const float* __restrict__ h, size_t ldh, const int* __restrict__ row_of,
                                                   const float* __restrict__ w, size_t ldw, int vocab, int width,
                                                   int split_at, Meta* meta) {
+  after_previous();
+  let_next_start();
   const bool of_h = (int)blockIdx.x < split_at;
   const int block = of_h ? blockIdx.x : blockIdx.x - split_at, blocks = of_h ? split_at : gridDim.x - split_at;
   const int rows = of_h ? (int)meta->rows : vocab;
   unsigned int most = 0;
   for (int r = block; r < rows; r += blocks) {
     const float* x = of_h ? h + (size_t)row_of[r] * ldh : w + (size_t)r * ldw;
-    for (int c = threadIdx.x; c < width; c += 256) most = max(most, __float_as_uint(x[c]) & 0x7FFFFFFFu);
+#pragma unroll 4
+    for (int c = threadIdx.x; c < width; c += 256) most = max(most, __float_as_uint(__ldg(x + c)) & 0x7FFFFFFFu);
   }
   most = __reduce_max_sync(0xFFFFFFFFu, most);
   if ((threadIdx.x & 31) == 0 && most) atomicMax(of_h ? &meta->max_h : &meta->max_w, most);  // order does not matter
@@ -121,6 +116,8 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(const T* __restrict__ x,
                                                         int all_rows, int width, int pitch, const Meta* __restrict__ meta,
                                                         uint16_t* __restrict__ hi, uint16_t* __restrict__ lo) {
   constexpr bool SPLIT = sizeof(T) == 4;
+  after_previous();
+  let_next_start();
   const int have = GATHER ? (int)meta->rows : all_rows;
   const int rows = GATHER ? row_blocks(have) * TILE_M : all_rows;
   const float up = SPLIT ? pow2(up_exp(GATHER ? meta->max_h : meta->max_w)) : 1.f;
@@ -174,7 +171,7 @@ struct LogitTiles {
   const LogitParams& p;
   int rows, m_blocks, n_blocks, band;
   float unit;  // accumulators times this are logits times log2 e
-  __device__ explicit LogitTiles(const LogitParams& q) : p(q) {
+  __device__ explicit LogitTiles(const LogitParams& q, const TileMaps&) : p(q) {
     rows = (int)p.meta->rows;
     m_blocks = row_blocks(rows);
     n_blocks = (p.v_count + BN - 1) / BN;
@@ -202,16 +199,17 @@ struct LogitTiles {
 template <bool SPLIT_>
 struct StatOp : LogitTiles<SPLIT_> {
   typedef LogitParams Params;
+  static constexpr bool STORES = false;
   using LogitTiles<SPLIT_>::p;
   float top, sum;
   int target;
-  __device__ explicit StatOp(const LogitParams& q) : LogitTiles<SPLIT_>(q) {}
+  __device__ explicit StatOp(const LogitParams& q, const TileMaps& m) : LogitTiles<SPLIT_>(q, m) {}
   __device__ __forceinline__ void begin(const Tile&, int row, int) {
     top = -INFINITY;
     sum = 0.f;
     target = row < this->rows ? __ldg(p.target + row) : -1;
   }
-  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[32], float*, int lane) {
+  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[32], uint8_t*, int lane) {
     if (col0 >= p.vocab) return;
     if (col0 + 32 > p.vocab) {
 #pragma unroll
@@ -241,43 +239,51 @@ struct StatOp : LogitTiles<SPLIT_> {
   }
 };
 
-// d of a piece, zeros in rows and columns that fill up tiles.
+// d of a piece, zeros in rows and columns that fill up tiles. What an element takes here bounds the kernel when width is small
+// (1024 and less: 8 us per tile before stores went by TMA and the target's column was a branch of its own, 5.8 us
+// of products), so it is one FMA, one exponential, one product and half a conversion.
 template <bool SPLIT_>
 struct GradOp : LogitTiles<SPLIT_> {
   typedef LogitParams Params;
+  static constexpr bool STORES = !SPLIT_;
   using LogitTiles<SPLIT_>::p;
-  float top, inv;
+  const CUtensorMap* map;
+  float top, by, to;
   int target;
   bool in;
-  __device__ explicit GradOp(const LogitParams& q) : LogitTiles<SPLIT_>(q) {}
+  __device__ explicit GradOp(const LogitParams& q, const TileMaps& m) : LogitTiles<SPLIT_>(q, m), map(&m.c) {
+    to = SPLIT_ ? (float)(1 << D_EXP) : p.scale;
+  }
   __device__ __forceinline__ void begin(const Tile&, int row, int) {
     in = row < this->rows;
     const float2 st = in ? __ldg(p.row_stat + row) : make_float2(0.f, 0.f);
     top = st.x;
-    inv = st.y;
+    by = st.y * to;
     target = in ? __ldg(p.target + row) - p.v_begin : -1;
   }
-  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[32], float* stage, int lane) {
-    const float to = SPLIT_ ? (float)(1 << D_EXP) : p.scale;
+  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[32], uint8_t* stage, int lane) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      float d = ex2(fmaf(v[j], this->unit, -top)) * inv;
-      if (col0 + j == target) d -= 1.f;
-      v[j] = in && col0 + j < p.v_count ? d * to : 0.f;
+    for (int j = 0; j < 32; ++j) v[j] = ex2(fmaf(v[j], this->unit, -top)) * by;
+    const int at = target - col0;
+    if (at >= 0 && at < 32) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] -= j == at ? to : 0.f;
     }
-    by_rows(row0, col0, v, stage, lane, [&](int r, int c, const float4& x) {
-      const long long at = (long long)r * p.ld_d + c;
-      if (SPLIT_) {
-        const float f[4] = {x.x, x.y, x.z, x.w};
-        __half a[4], b[4];
+    if (!in || col0 + 32 > p.v_count) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) split_half(f[i], a[i], b[i]);
-        *reinterpret_cast<uint2*>(p.d_hi + at) = *reinterpret_cast<const uint2*>(a);
-        *reinterpret_cast<uint2*>(p.d_lo + at) = *reinterpret_cast<const uint2*>(b);
-      } else {
-        *reinterpret_cast<uint2*>(p.d_hi + at) = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
-      }
-    });
+      for (int j = 0; j < 32; ++j)
+        if (!in || col0 + j >= p.v_count) v[j] = 0.f;
+    }
+    if constexpr (SPLIT_) {
+      by_rows(row0, col0, v, stage, lane, LoadNothing(), [&](int r, int c, const float4& x, Nothing) {
+        store_pair(reinterpret_cast<__half*>(p.d_hi), reinterpret_cast<__half*>(p.d_lo), (long long)r * p.ld_d + c, x);
+      });
+    } else {
+      uint32_t w[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+      store_half_words(map, w, col0 >> 5 & 1, row0, col0 & ~63, stage, lane);
+    }
   }
   __device__ __forceinline__ void end(const Tile&, int, int) {}
 };
@@ -288,6 +294,8 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const float2* __restrict
                                                         const int* __restrict__ row_of, float2* __restrict__ row_stat,
                                                         float* __restrict__ row_loss) {
   __shared__ float2 part[8][32];
+  after_previous();
+  let_next_start();
   const int lane = threadIdx.x & 31, share = threadIdx.x >> 5, rows = (int)meta->rows;
   const int row = blockIdx.x * 32 + lane;
   if ((int)blockIdx.x * 32 >= rows) return;
@@ -298,9 +306,23 @@ __global__ void __launch_bounds__(256) join_rows_kernel(const float2* __restrict
     sum = sum * ex2(top - base) + x.y * ex2(x.x - base);
     top = now;
   };
-  if (row < rows)
-#pragma unroll 4
-    for (int k = share; k < count; k += 8) add(__ldg(parts + (long long)k * row_pitch + row));
+  if (row < rows) {
+    int k = share;
+    for (; k + 56 < count; k += 64) {  // eight of this warp's at a time, on one maximum
+      float2 x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = __ldg(parts + (long long)(k + 8 * u) * row_pitch + row);
+      float now = top;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) now = fmaxf(now, x[u].x);
+      const float base = now == -INFINITY ? 0.f : now;
+      sum *= ex2(top - base);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) sum = fmaf(x[u].y, ex2(x[u].x - base), sum);
+      top = now;
+    }
+    for (; k < count; k += 8) add(__ldg(parts + (long long)k * row_pitch + row));
+  }
   part[share][lane] = make_float2(top, sum);
   __syncthreads();
   if (share || row >= rows) return;
@@ -317,54 +339,109 @@ struct ProductParams {
   int width;
   float scale;
   // dh: fp32 sums over the pieces
-  float* acc;
+  float *acc, *slots;
   long long ld_acc;
-  int first;  // first piece: written, not added to
+  int pairs, full_kblocks;  // full_kblocks: of a whole piece
+  int first;                // first piece: written, not added to
   // dw
   void* dw;
   long long ld_dw;
   int out_bf16, vec;  // vec: rows begin on whole groups of four elements
 };
 
+// How the tiles of dh go over the pairs. There are few of them and their sums are long, so whole tiles alone would leave many
+// pairs idle in the last round (232 tiles on 74 pairs: 4 rounds for 3.1). Whole tiles fill complete rounds, all pairs in step so
+// that they share their slabs in the L2 cache; the k range of the `rest` tiles behind them is cut into `shares` equal parts,
+// one per pair, which may cover the end of one tile and the beginning of the next. A part's sum goes to a slot of its
+// pair, and spread_rows_kernel adds a tile's parts in order. Which part is whose does not depend on the piece, so the slots
+// are added to from piece to piece.
+struct HiddenSplit {
+  int m_blocks, n_blocks, whole, rest, shares;
+  __device__ HiddenSplit(const ProductParams& p, unsigned int rows, int bn) {
+    m_blocks = row_blocks(rows);
+    n_blocks = (p.width + bn - 1) / bn;
+    const int tiles = m_blocks * n_blocks;
+    whole = tiles / p.pairs * p.pairs;
+    rest = tiles - whole;
+    // no part shorter than eight k-blocks, where there is a choice
+    shares = (int)min((long long)p.pairs, max((long long)rest, (long long)rest * p.full_kblocks / 8));
+  }
+  // Part j (0, 1) of share s: tile, and its range of k in 1 / shares of a tile. False: there is none.
+  __device__ bool part(int s, int j, int& tile, int& from, int& to) const {
+    const int begin = s * rest, end = begin + rest;  // in 1 / shares of a tile
+    tile = begin / shares + j;
+    from = max(begin - tile * shares, 0);
+    to = min(end - tile * shares, shares);
+    return to > from;
+  }
+};
+
 // dh (listed rows) += d w over a piece.
 template <bool SPLIT_>
 struct HiddenOp {
   typedef ProductParams Params;
-  static constexpr bool SPLIT = SPLIT_;
+  static constexpr bool SPLIT = SPLIT_, STORES = false;
   static constexpr int BN = TileForm<SPLIT_>::BN;
   const ProductParams& p;
-  int m_blocks, n_blocks;
+  HiddenSplit split;
+  int kblocks;
   float unit;
-  __device__ explicit HiddenOp(const ProductParams& q) : p(q) {
-    m_blocks = row_blocks(p.meta->rows);
-    n_blocks = (p.width + BN - 1) / BN;
+  float* to;
+  long long ld;
+  __device__ explicit HiddenOp(const ProductParams& q, const TileMaps&) : p(q), split(q, q.meta->rows, BN) {
+    kblocks = (p.v_count + TILE_K - 1) / TILE_K;
     unit = SPLIT ? p.scale * pow2(-D_EXP) * pow2(-up_exp(p.meta->max_w)) : 1.f;
   }
-  __device__ int tiles() const { return m_blocks * n_blocks; }
+  __device__ int tiles() const { return split.whole + 2 * p.pairs; }
   __device__ Tile tile(int t) const {
     Tile r;
-    r.m0 = t / n_blocks * TILE_M;
-    r.n0 = t % n_blocks * BN;
+    int at = t, from = 0, kb = kblocks;
+    r.z = -1;  // straight to acc
+    if (t >= split.whole) {
+      const int j = (t - split.whole) / p.pairs, s = t - split.whole - j * p.pairs;
+      int a, b;
+      if (s >= split.shares || !split.part(s, j, at, a, b)) {
+        r.z = -2;  // nothing
+        r.m0 = r.n0 = r.a_mn = r.b_mn = r.a_k = r.b_k = r.kblocks = 0;
+        return r;
+      }
+      at += split.whole;
+      from = (int)((long long)kblocks * a / split.shares);
+      kb = (int)((long long)kblocks * b / split.shares) - from;
+      if (a > 0 || b < split.shares) r.z = 2 * s + (a > 0 ? 0 : 1);
+    }
+    r.m0 = at / split.n_blocks * TILE_M;
+    r.n0 = at % split.n_blocks * BN;
     r.a_mn = r.m0;
     r.b_mn = r.n0;
-    r.a_k = 0;
-    r.b_k = p.v_begin;
-    r.kblocks = (p.v_count + TILE_K - 1) / TILE_K;
-    r.z = 0;
+    r.a_k = from * TILE_K;
+    r.b_k = p.v_begin + from * TILE_K;
+    r.kblocks = kb;
     return r;
   }
-  __device__ __forceinline__ void begin(const Tile&, int, int) {}
-  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[32], float* stage, int lane) {
-    by_rows(row0, col0, v, stage, lane, [&](int r, int c, const float4& x) {
-      if (c >= p.width) return;
-      float4* to = reinterpret_cast<float4*>(p.acc + (long long)r * p.ld_acc + c);
-      float4 a = p.first ? make_float4(0.f, 0.f, 0.f, 0.f) : *to;
-      a.x = fmaf(x.x, unit, a.x);
-      a.y = fmaf(x.y, unit, a.y);
-      a.z = fmaf(x.z, unit, a.z);
-      a.w = fmaf(x.w, unit, a.w);
-      *to = a;
-    });
+  __device__ __forceinline__ void begin(const Tile& t, int, int) {
+    if (t.z >= 0) {
+      ld = BN;
+      to = p.slots + (long long)t.z * TILE_M * BN - (t.m0 * ld + t.n0);
+    } else {
+      ld = p.ld_acc;
+      to = p.acc;
+    }
+  }
+  __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[32], uint8_t* stage, int lane) {
+    if (t.z == -2 || col0 >= p.width) return;
+    if (p.first)
+      by_rows(row0, col0, v, stage, lane, LoadNothing(), [&](int r, int c, const float4& x, Nothing) {
+        if (c < p.width) *reinterpret_cast<float4*>(to + r * ld + c) = make_float4(x.x * unit, x.y * unit, x.z * unit, x.w * unit);
+      });
+    else
+      by_rows(row0, col0, v, stage, lane,
+              [&](int r, int c) { return c < p.width ? *reinterpret_cast<const float4*>(to + r * ld + c) : make_float4(0.f, 0.f, 0.f, 0.f); },
+              [&](int r, int c, const float4& x, const float4& a) {
+                if (c < p.width)
+                  *reinterpret_cast<float4*>(to + r * ld + c) =
+                      make_float4(fmaf(x.x, unit, a.x), fmaf(x.y, unit, a.y), fmaf(x.z, unit, a.z), fmaf(x.w, unit, a.w));
+              });
   }
   __device__ __forceinline__ void end(const Tile&, int, int) {}
 };
@@ -373,12 +450,12 @@ struct HiddenOp {
 template <bool SPLIT_>
 struct WeightOp {
   typedef ProductParams Params;
-  static constexpr bool SPLIT = SPLIT_;
+  static constexpr bool SPLIT = SPLIT_, STORES = false;
   static constexpr int BN = TileForm<SPLIT_>::BN;
   const ProductParams& p;
   int m_blocks, n_blocks, kblocks;
   float unit;
-  __device__ explicit WeightOp(const ProductParams& q) : p(q) {
+  __device__ explicit WeightOp(const ProductParams& q, const TileMaps&) : p(q) {
     m_blocks = (p.v_count + TILE_M - 1) / TILE_M;
     n_blocks = (p.width + BN - 1) / BN;
     kblocks = max(1, (int)((p.meta->rows + TILE_K - 1) / TILE_K));  // without rows: zeros, as they are stored
@@ -397,8 +474,8 @@ struct WeightOp {
     return r;
   }
   __device__ __forceinline__ void begin(const Tile&, int, int) {}
-  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[32], float* stage, int lane) {
-    by_rows(row0, col0, v, stage, lane, [&](int r, int c, const float4& x) {
+  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[32], uint8_t* stage, int lane) {
+    by_rows(row0, col0, v, stage, lane, LoadNothing(), [&](int r, int c, const float4& x, Nothing) {
       if (r >= p.v_count || c >= p.width) return;
       const long long at = (long long)(p.v_begin + r) * p.ld_dw + c;
       const float f[4] = {x.x * unit, x.y * unit, x.z * unit, x.w * unit};
@@ -428,14 +505,32 @@ struct WeightOp {
 
 // dh in the caller's order and type, zeros for rows without a target.
 template <typename T>
-__global__ void __launch_bounds__(256) spread_rows_kernel(const float* __restrict__ acc, long long ld_acc,
-                                                          const int* __restrict__ slot_of, int rows, int width, int vec,
+__global__ void __launch_bounds__(256) spread_rows_kernel(const ProductParams p, const int* __restrict__ slot_of, int rows, int vec,
                                                           T* __restrict__ dh, size_t ld) {
+  constexpr int BN = TileForm<sizeof(T) == 4>::BN;
+  after_previous();
+  let_next_start();
+  const HiddenSplit split(p, p.meta->rows, BN);
+  const int width = p.width;
   for (int r = blockIdx.x; r < rows; r += gridDim.x) {
     const int slot = slot_of[r];
     T* to = dh + (size_t)r * ld;
     for (int c = threadIdx.x * 4; c < width; c += 256 * 4) {
-      const float4 x = slot >= 0 ? *reinterpret_cast<const float4*>(acc + slot * ld_acc + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (slot >= 0) {
+        const int t = slot / TILE_M * split.n_blocks + c / BN - split.whole;
+        // the shares that a tile behind the whole ones lies in; one alone means that it was not cut
+        const int s0 = t < 0 ? 0 : t * split.shares / split.rest, s1 = t < 0 ? 0 : ((t + 1) * split.shares - 1) / split.rest;
+        if (s0 == s1) {
+          x = *reinterpret_cast<const float4*>(p.acc + slot * p.ld_acc + c);
+        } else {
+          for (int s = s0; s <= s1; ++s) {
+            const int z = 2 * s + (s * split.rest > t * split.shares ? 0 : 1);  // not from the tile's beginning on: HiddenOp's a > 0
+            const float4 y = *reinterpret_cast<const float4*>(p.slots + ((long long)z * TILE_M + slot % TILE_M) * BN + c % BN);
+            x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+          }
+        }
+      }
       const float f[4] = {x.x, x.y, x.z, x.w};
       if (vec && c + 4 <= width) {
         typedef Elems<T, 4 * (int)sizeof(T)> E;
@@ -485,8 +580,9 @@ struct Space {
   float* target_logit;
   float2 *row_stat, *parts;
   uint16_t *h_hi, *h_lo, *w_hi, *w_lo, *d_hi, *d_lo;
-  float* acc;
+  float *acc, *slots;
 };
+constexpr int MOST_PAIRS = 74;  // 148 SMs
 size_t space_of(const Sizes& z, size_t rows, size_t vocab, int grads, void* base, Space* s) {
   Carver c(base);
   const size_t lo = z.split ? 1 : 0;
@@ -504,6 +600,7 @@ size_t space_of(const Sizes& z, size_t rows, size_t vocab, int grads, void* base
   s->d_hi = c.take<uint16_t>(z.rows_up * z.piece);
   s->d_lo = c.take<uint16_t>(lo * z.rows_up * z.piece);
   s->acc = c.take<float>(grads ? z.rows_up * z.pitch : 0);
+  s->slots = c.take<float>(grads ? 2ll * MOST_PAIRS * TILE_M * (z.split ? 128 : 256) : 0);
   return c.used;
 }
 
@@ -530,17 +627,22 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
   constexpr int BN = TileForm<SPLIT>::BN;
   const int rows = (int)c.rows, width = (int)c.width, vocab = (int)c.vocab, pitch = (int)z.pitch;
   const T *h = static_cast<const T*>(c.h), *w = static_cast<const T*>(c.w);
-  list_rows_kernel<<<1, LIST_THREADS, 0, st>>>(c.targets, c.wide, rows, (unsigned int)vocab, s.meta, s.row_of, s.slot_of, s.target,
-                                               c.row_loss);
+  Chain chain(st);
   auto blocks = [&](long long n) { return (unsigned int)(n < 8ll * sms ? n : 8ll * sms); };
+  int share = (rows + LIST_BLOCKS - 1) / LIST_BLOCKS;
+  share = (share + LIST_THREADS - 1) / LIST_THREADS * LIST_THREADS;
+  chain.launch(list_rows_kernel, dim3((rows + share - 1) / share), LIST_THREADS, 0, 0, c.targets, c.wide, rows, share, (unsigned int)vocab,
+               s.meta, s.row_of, s.slot_of, s.target, c.row_loss);
   if (SPLIT) {
     const int of_h = (int)blocks(rows);
-    max_kernel<<<of_h + blocks(vocab), 256, 0, st>>>((const float*)c.h, c.ldh, s.row_of, (const float*)c.w, c.ldw, vocab, width, of_h, s.meta);
+    chain.launch(max_kernel, dim3(of_h + blocks(vocab)), 256, 0, 0, (const float*)c.h, c.ldh, s.row_of, (const float*)c.w, c.ldw, vocab, width,
+                 of_h, s.meta);
   }
-  copy_rows_kernel<T, true><<<blocks(z.rows_up), 256, 0, st>>>(h, c.ldh, s.row_of, 0, width, pitch, s.meta, s.h_hi, s.h_lo);
+  chain.launch(copy_rows_kernel<T, true>, dim3(blocks(z.rows_up)), 256, 0, 0, h, c.ldh, s.row_of, 0, width, pitch, s.meta, s.h_hi, s.h_lo);
   if (z.copy_w)
-    copy_rows_kernel<T, false><<<blocks(vocab), 256, 0, st>>>(w, c.ldw, nullptr, vocab, width, pitch, s.meta, s.w_hi, s.w_lo);
-  int rc = launch_error(cudaGetLastError(), "b2_xent");
+    chain.launch(copy_rows_kernel<T, false>, dim3(blocks(vocab)), 256, 0, 0, w, c.ldw, (const int*)nullptr, vocab, width, pitch, s.meta,
+                 s.w_hi, s.w_lo);
+  int rc = launch_error(chain.err, "b2_xent");
   if (rc != B2_OK) return rc;
 
   const TileOperand h_k{s.h_hi, s.h_lo, z.rows_up, pitch, pitch, false}, h_mn{s.h_hi, s.h_lo, pitch, z.rows_up, pitch, true};
@@ -562,11 +664,11 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
   lp.d_lo = s.d_lo;
   lp.ld_d = z.piece;
   lp.scale = c.scale;
-  rc = tile_launch<StatOp<SPLIT>>("b2_xent", h_k, w_k, lp, !SPLIT, m_blocks * ((vocab + BN - 1) / BN), sms, st);
+  rc = tile_launch<StatOp<SPLIT>>("b2_xent", h_k, w_k, nullptr, lp, !SPLIT, m_blocks * ((vocab + BN - 1) / BN), sms, chain);
   if (rc != B2_OK) return rc;
-  join_rows_kernel<<<(rows + 31) / 32, 256, 0, st>>>(s.parts, z.rows_up, (int)z.parts, s.meta, s.target_logit, s.row_of, s.row_stat,
-                                                     c.row_loss);
-  rc = launch_error(cudaGetLastError(), "b2_xent");
+  chain.launch(join_rows_kernel, dim3((rows + 31) / 32), 256, 0, 0, s.parts, z.rows_up, (int)z.parts, s.meta, s.target_logit, s.row_of, s.row_stat,
+               c.row_loss);
+  rc = launch_error(chain.err, "b2_xent");
   if (rc != B2_OK || (!c.dh && !c.dw)) return rc;
 
   ProductParams pp{};
@@ -574,29 +676,32 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
   pp.width = width;
   pp.scale = c.scale;
   pp.acc = s.acc;
+  pp.slots = s.slots;
+  pp.pairs = sms / 2 < MOST_PAIRS ? sms / 2 : MOST_PAIRS;
+  pp.full_kblocks = (int)(z.piece / TILE_K);
   pp.ld_acc = pitch;
   pp.dw = c.dw;
   pp.ld_dw = (long long)c.ld_dw;
   pp.out_bf16 = !SPLIT;
   pp.vec = c.ld_dw % 4 == 0 && reinterpret_cast<uintptr_t>(c.dw) % (4 * sizeof(T)) == 0;
   const TileOperand d_k{s.d_hi, s.d_lo, z.rows_up, z.piece, z.piece, false}, d_mn{s.d_hi, s.d_lo, z.piece, z.rows_up, z.piece, true};
+  const TileResult d_out{s.d_hi, z.rows_up, z.piece, z.piece};
   const long long w_blocks = (width + BN - 1) / BN;
   for (int v0 = 0; v0 < vocab; v0 += (int)z.piece) {
     const int count = vocab - v0 < z.piece ? vocab - v0 : (int)z.piece;
     lp.v_begin = pp.v_begin = v0;
     lp.v_count = pp.v_count = count;
     pp.first = v0 == 0;
-    // d's columns are written in blocks of 256, whatever the tile
-    rc = tile_launch<GradOp<SPLIT>>("b2_xent", h_k, w_k, lp, !SPLIT, m_blocks * ((count + BN - 1) / BN), sms, st);
-    if (rc == B2_OK && c.dh) rc = tile_launch<HiddenOp<SPLIT>>("b2_xent", d_k, w_mn, pp, !SPLIT, m_blocks * w_blocks, sms, st);
+    rc = tile_launch<GradOp<SPLIT>>("b2_xent", h_k, w_k, SPLIT ? nullptr : &d_out, lp, !SPLIT, m_blocks * ((count + BN - 1) / BN), sms, chain);
+    if (rc == B2_OK && c.dh) rc = tile_launch<HiddenOp<SPLIT>>("b2_xent", d_k, w_mn, nullptr, pp, !SPLIT, pp.pairs, sms, chain);
     if (rc == B2_OK && c.dw)
-      rc = tile_launch<WeightOp<SPLIT>>("b2_xent", d_mn, h_mn, pp, !SPLIT, (count + TILE_M - 1) / TILE_M * w_blocks, sms, st);
+      rc = tile_launch<WeightOp<SPLIT>>("b2_xent", d_mn, h_mn, nullptr, pp, !SPLIT, (count + TILE_M - 1) / TILE_M * w_blocks, sms, chain);
     if (rc != B2_OK) return rc;
   }
   if (c.dh) {
     const int vec = c.ld_dh % 4 == 0 && reinterpret_cast<uintptr_t>(c.dh) % (4 * sizeof(T)) == 0;
-    spread_rows_kernel<T><<<blocks(rows), 256, 0, st>>>(s.acc, pitch, s.slot_of, rows, width, vec, static_cast<T*>(c.dh), c.ld_dh);
-    rc = launch_error(cudaGetLastError(), "b2_xent");
+    chain.launch(spread_rows_kernel<T>, dim3(blocks(rows)), 256, 0, 0, pp, s.slot_of, rows, vec, static_cast<T*>(c.dh), c.ld_dh);
+    rc = launch_error(chain.err, "b2_xent");
   }
   return rc;
 }

@@ -32,13 +32,17 @@ def _matrix(name, x, dtype=None, shape=None, device=None):
         raise ValueError(f"{name}: on {x.device}, wanted on {device if device is not None else 'a CUDA device'}")
     if x.dtype not in _DTYPES or (dtype is not None and x.dtype != dtype):
         raise ValueError(f"{name}: {x.dtype}, wanted {dtype if dtype is not None else 'float32 or bfloat16'}")
-    if shape is not None and tuple(x.shape) != tuple(shape):
-        raise ValueError(f"{name}: shape {tuple(x.shape)}, wanted {tuple(shape)}")
-    if x.shape[1] > 1 and x.stride(1) != 1:
+    rows, cols = x.shape
+    if shape is not None and (rows, cols) != tuple(shape):
+        raise ValueError(f"{name}: shape {(rows, cols)}, wanted {tuple(shape)}")
+    between, along = x.stride()
+    if cols > 1 and along != 1:
         raise ValueError(f"{name}: rows need unit stride")
-    if x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+    if rows <= 1:
+        between = cols
+    elif between < cols:
         raise ValueError(f"{name}: rows overlap")
-    return x.data_ptr(), max(x.stride(0), x.shape[1]) if x.shape[0] > 1 else x.shape[1]
+    return x.data_ptr(), between
 
 
 def _tokens(name, t, device):
@@ -46,8 +50,9 @@ def _tokens(name, t, device):
         raise ValueError(f"{name}: an int32 or int64 tensor is wanted")
     if t.device != device:
         raise ValueError(f"{name}: on {t.device}, wanted on {device}")
-    t = t.reshape(-1).contiguous()
-    return t, t.element_size()
+    if t.dim() != 1 or not t.is_contiguous():
+        t = t.reshape(-1).contiguous()
+    return t, 8 if t.dtype == torch.int64 else 4
 
 
 def _workspace(size, device):
@@ -55,8 +60,21 @@ def _workspace(size, device):
     return torch.empty(max(int(size), 1), dtype=torch.uint8, device=device)
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+class _on:
+    """The device of a call made the current one, where it is not already; gives the address of its current stream."""
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.index != self.before:
+            torch.cuda.set_device(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *a):
+        if self.index != self.before:
+            torch.cuda.set_device(self.before)
 
 
 def embed(tokens, table, scale=1.0, out=None):
@@ -68,9 +86,9 @@ def embed(tokens, table, scale=1.0, out=None):
     if out is None:
         out = torch.empty(n, width, dtype=table.dtype, device=table.device)
     po, ldo = _matrix("out", out, table.dtype, (n, width), table.device)
-    with torch.cuda.device(table.device):
+    with _on(table.device) as stream:
         _ck(K.lib().b2_embed(t.data_ptr(), size, n, p, _DTYPES[table.dtype], vocab, width, ld, scale, po, ldo,
-                             _stream(table.device)))
+                             stream))
     return out
 
 
@@ -86,10 +104,10 @@ def embed_grad(tokens, dout, vocab, scale=1.0, out=None):
     po, ldo = _matrix("out", out, dout.dtype, (vocab, width), dout.device)
     need = C.c_size_t()
     _ck(K.lib().b2_embed_grad_workspace(n, vocab, width, C.byref(need)))
-    with torch.cuda.device(dout.device):
+    with _on(dout.device) as stream:
         ws = _workspace(need.value, dout.device)
         _ck(K.lib().b2_embed_grad(t.data_ptr(), size, n, p, _DTYPES[dout.dtype], ld, vocab, width, scale, po, ldo,
-                                  ws.data_ptr(), ws.numel(), _stream(dout.device)))
+                                  ws.data_ptr(), ws.numel(), stream))
     return out
 
 
@@ -117,10 +135,10 @@ def xent(h, w, targets, scale=1.0, grad=True, dh=None, dw=None):
         pdw, lddw = _matrix("dw", dw, dtype, (vocab, width), device)
     need = C.c_size_t()
     _ck(K.lib().b2_xent_workspace(rows, width, vocab, _DTYPES[dtype], int(grad), pw, ldw, C.byref(need)))
-    with torch.cuda.device(device):
+    with _on(device) as stream:
         ws = _workspace(need.value, device)
         _ck(K.lib().b2_xent(rows, width, vocab, _DTYPES[dtype], ph, ldh, pw, ldw, t.data_ptr(), size, scale,
-                            loss.data_ptr(), pdh, lddh, pdw, lddw, ws.data_ptr(), ws.numel(), _stream(device)))
+                            loss.data_ptr(), pdh, lddh, pdw, lddw, ws.data_ptr(), ws.numel(), stream))
     return (loss, dh, dw) if grad else loss
 
 
@@ -153,14 +171,14 @@ def muon(w, momentum_buffer, grad, *, lr, momentum=0.95, nesterov=True, weight_d
     o = K.MuonOptions(lr, momentum, weight_decay, scale, eps, int(nesterov), steps)
     need = C.c_size_t()
     _ck(K.lib().b2_muon_workspace(n, shape[0], shape[1], C.byref(need)))
-    with torch.cuda.device(device):
+    with _on(device) as stream:
         ws_ = _workspace(need.value, device)
         _ck(K.lib().b2_muon(n, shape[0], shape[1], _DTYPES[gs[0].dtype], arr(pw), ldw, arr(pc), ldc, arr(pm), ldm, arr(pg), ldg,
-                            C.byref(o), ws_.data_ptr(), ws_.numel(), _stream(device)))
+                            C.byref(o), ws_.data_ptr(), ws_.numel(), stream))
 
 
 def sync(device=None):
     """Waits for the current stream of `device`; K.B2Error with code ERR_TIMEOUT if a bounded wait of a kernel gave up."""
-    device = torch.device("cuda" if device is None else device)
-    with torch.cuda.device(device):
-        _ck(K.lib().b2_lm_sync(_stream(device)))
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    with _on(device) as stream:
+        _ck(K.lib().b2_lm_sync(stream))

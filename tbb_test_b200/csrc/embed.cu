@@ -10,7 +10,7 @@
 // into chunks of equal length, one group of threads per chunk and slice of columns, so that a token that makes up
 // a tenth of a batch takes no longer than many rare ones. A run of one token inside a chunk is finished there. One that
 // crosses chunk borders leaves a partial sum per chunk, and a second kernel adds these in order. The rows of tokens that do
-// not occur are zeroed by blocks of the first kernel, which look the token up in the sorted list.
+// not occur are zeroed meanwhile.
 #include "lm.cuh"
 
 namespace b2 {
@@ -62,9 +62,10 @@ constexpr int RANK_MOST = 8192;
 constexpr int RANK_THREADS = 256, RANK_PER_WARP = 4;
 __global__ void __launch_bounds__(RANK_THREADS) rank_sort_kernel(const void* __restrict__ tokens, int wide, int n,
                                                                  unsigned int vocab, unsigned int* __restrict__ keys,
-                                                                 unsigned int* __restrict__ pos) {
+                                                                 unsigned int* __restrict__ pos, unsigned int* joins) {
   extern __shared__ unsigned int key_s[];
   let_next_start();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *joins = 0;
   for (int i = threadIdx.x; i < n; i += RANK_THREADS) key_s[i] = token_at(tokens, wide, i, vocab);
   __syncthreads();
   const int lane = threadIdx.x & 31;
@@ -104,7 +105,9 @@ struct RadixPass {
   unsigned int vocab;
   const unsigned int *keys, *pos;
   unsigned int *keys_out, *pos_out;
-  unsigned int* counts;  // tiles x bins
+  unsigned int* counts;       // tiles x bins
+  unsigned char* present;     // first pass: set for every token that occurs
+  unsigned int* next_counts;  // the same of the next digit, counted where this one's elements go; zeroed by the first kernel
   unsigned int n, tile;  // elements, elements per tile (a multiple of a block's step)
   int tiles, shift, bits;
 };
@@ -112,13 +115,18 @@ __device__ __forceinline__ unsigned int radix_key(const RadixPass& p, unsigned i
   return p.tokens ? token_at(p.tokens, p.wide, i, p.vocab) : p.keys[i];
 }
 
-__global__ void __launch_bounds__(RADIX_THREADS) radix_count_kernel(const RadixPass p) {
+// Counts of the first digit, and zeros for what the kernels behind it count and mark.
+__global__ void __launch_bounds__(RADIX_THREADS) radix_count_kernel(const RadixPass p, unsigned int* other_counts, int others,
+                                                                    unsigned char* present, unsigned int* joins) {
   __shared__ unsigned int count[1 << RADIX_MOST_BITS];
   const int bins = 1 << p.bits;
-  for (int b = threadIdx.x; b < bins; b += RADIX_THREADS) count[b] = 0;
-  __syncthreads();
-  after_previous();
   let_next_start();
+  for (int b = threadIdx.x; b < bins; b += RADIX_THREADS) count[b] = 0;
+  for (int b = blockIdx.x * RADIX_THREADS + threadIdx.x; b < others; b += gridDim.x * RADIX_THREADS) other_counts[b] = 0;
+  for (size_t v = ((size_t)blockIdx.x * RADIX_THREADS + threadIdx.x) * 16; v < p.vocab; v += (size_t)gridDim.x * RADIX_THREADS * 16)
+    *reinterpret_cast<uint4*>(present + v) = make_uint4(0, 0, 0, 0);  // the array is whole 16-byte pieces
+  if (blockIdx.x == 0 && threadIdx.x == 0) *joins = 0;
+  __syncthreads();
   const unsigned int begin = blockIdx.x * p.tile, end = min(p.n, begin + p.tile);
   for (unsigned int i = begin + threadIdx.x; i < end; i += RADIX_THREADS)
     atomicAdd(&count[(radix_key(p, i) >> p.shift) & (bins - 1)], 1u);
@@ -141,7 +149,7 @@ __global__ void __launch_bounds__(RADIX_THREADS) radix_place_kernel(const RadixP
     const int b = b0 + threadIdx.x;
     unsigned int total = 0, before = 0;
     if (b < bins)
-#pragma unroll 16
+#pragma unroll 32
       for (int t = 0; t < p.tiles; ++t) {
         const unsigned int c = p.counts[(size_t)t * bins + b];
         total += c;
@@ -209,6 +217,9 @@ __global__ void __launch_bounds__(RADIX_THREADS) radix_place_kernel(const RadixP
         const unsigned int to = next[digit] + seen[warp][digit] + place[r];
         p.keys_out[to] = key[r];
         p.pos_out[to] = pos[r];
+        if (p.present && key[r] < p.vocab) p.present[key[r]] = 1;
+        if (p.next_counts)  // whole numbers: the order of the additions does not matter
+          atomicAdd(p.next_counts + ((size_t)(to / p.tile) << p.bits) + ((key[r] >> (p.shift + p.bits)) & (bins - 1)), 1u);
       }
     __syncthreads();
 #pragma unroll
@@ -232,9 +243,12 @@ struct RunSum {
   size_t ld_dtable;
   float *head, *tail;  // chunks x pitch partial sums: of the run that came from the chunk before, and of the one that goes on
   size_t pitch;        // floats per partial row
+  unsigned int* joins;  // how many runs go on behind the chunk they begin in
+  uint2* join_runs;     // their chunks and tokens, in any order
   float scale;
   int vecs, slices, tpr_log2;
-  unsigned int sum_blocks;
+  const unsigned char* present;  // by token, or null: looked up in the sorted list
+  unsigned int fill_blocks;      // of the second kernel
 };
 
 // First index whose key is >= `key`.
@@ -249,7 +263,6 @@ __device__ __forceinline__ unsigned int lower_bound(const unsigned int* keys, un
 }
 
 constexpr int RUN_THREADS = 128, RUN_AHEAD = 8;
-constexpr int FILL_ROWS = 8;  // rows that a warp looks up and zeroes
 template <typename T, int VB>
 __global__ void __launch_bounds__(RUN_THREADS) run_sum_kernel(const RunSum p) {
   typedef Elems<T, VB> E;
@@ -257,23 +270,6 @@ __global__ void __launch_bounds__(RUN_THREADS) run_sum_kernel(const RunSum p) {
   const int lane = threadIdx.x & 31;
   after_previous();
   let_next_start();
-  if (blockIdx.x >= p.sum_blocks) {  // rows of tokens that do not occur
-    const unsigned int v0 = ((blockIdx.x - p.sum_blocks) * (RUN_THREADS / 32) + (threadIdx.x >> 5)) * FILL_ROWS;
-    const unsigned int v = v0 + lane;
-    bool absent = false;
-    if (lane < FILL_ROWS && v < p.vocab) {
-      const unsigned int at = lower_bound(p.keys, p.n, v);
-      absent = at == p.n || __ldg(p.keys + at) != v;
-    }
-    unsigned int rows = __ballot_sync(0xFFFFFFFFu, absent);
-    raw zero;
-    memset(&zero, 0, sizeof zero);
-    for (; rows; rows &= rows - 1) {
-      raw* row = reinterpret_cast<raw*>(p.dtable + (size_t)(v0 + __ffs(rows) - 1) * p.ld_dtable);
-      for (int c = lane; c < p.vecs; c += 32) row[c] = zero;
-    }
-    return;
-  }
   // A unit is a chunk and a slice of columns, worked on by 2^tpr_log2 >= 8 threads. Keys and positions of the next `span` elements
   // come with one load by the unit's threads and are handed round by shuffles.
   const int tpr = 1 << p.tpr_log2, span = min(tpr, 32), in_span = lane & (span - 1);
@@ -293,6 +289,7 @@ __global__ void __launch_bounds__(RUN_THREADS) run_sum_kernel(const RunSum p) {
       float* to = (from_before ? p.head : p.tail) + (size_t)chunk * p.pitch + (size_t)col * E::N;
 #pragma unroll
       for (int j = 0; j < E::N; ++j) to[j] = acc[j];
+      if (goes_on && !from_before && col == 0) p.join_runs[atomicAdd(p.joins, 1u)] = make_uint2(chunk, cur);
     } else {
 #pragma unroll
       for (int j = 0; j < E::N; ++j) acc[j] *= p.scale;
@@ -337,33 +334,55 @@ __global__ void __launch_bounds__(RUN_THREADS) run_sum_kernel(const RunSum p) {
   if (cur < p.vocab) finish(end < p.n && __ldg(p.keys + end) == cur);
 }
 
-// Runs that cross chunk borders: the chunk a run begins in adds its tail and the heads of the chunks behind it,
-// JOIN_PARTS contiguous shares of them side by side, which are then added in order.
-constexpr int JOIN_PARTS = 8;
-template <typename T>
-__global__ void __launch_bounds__(32 * JOIN_PARTS) run_join_kernel(const RunSum p, int width) {
+// Runs that cross chunk borders: the tail of the chunk a run begins in and the heads of the chunks behind it, JOIN_PARTS
+// contiguous shares of them side by side, which are then added in order. A block takes 128 columns of a run at a time. The blocks
+// before these zero the rows of tokens that do not occur, which needs no sums and so does not wait for the kernel before: that
+// one has waited for the sorted list before this one starts.
+constexpr int JOIN_PARTS = 4, JOIN_THREADS = 32 * JOIN_PARTS;
+constexpr int FILL_ROWS = 8;  // rows that a warp looks up and zeroes
+template <typename T, int VB>
+__global__ void __launch_bounds__(JOIN_THREADS) run_join_kernel(const RunSum p, int width) {
   __shared__ float4 part[JOIN_PARTS][32];
-  const unsigned int chunk = blockIdx.x;
-  const unsigned int begin = chunk * p.chunk, end = begin + p.chunk;
   const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
-  after_previous();
   let_next_start();
-  if (end >= p.n) return;
-  const unsigned int key = __ldg(p.keys + end);
-  if (key >= p.vocab || __ldg(p.keys + end - 1) != key) return;                                    // nothing goes on
-  if (begin > 0 && __ldg(p.keys + begin) == key && __ldg(p.keys + begin - 1) == key) return;  // it began earlier
-  // the run's last chunk: chunks whose first element has the key
-  unsigned int last = chunk;
-  for (;;) {
-    const size_t at = (size_t)(last + 1 + lane) * p.chunk;
-    const unsigned int same = __ballot_sync(0xFFFFFFFFu, at < p.n && __ldg(p.keys + at) == key);
-    last += same == 0xFFFFFFFFu ? 32 : __ffs(~same) - 1;
-    if (same != 0xFFFFFFFFu) break;
+  if (blockIdx.x < p.fill_blocks) {
+    typedef typename Raw<VB>::type raw;
+    const unsigned int v0 = (blockIdx.x * JOIN_PARTS + share) * FILL_ROWS, v = v0 + lane;
+    bool absent = false;
+    if (lane < FILL_ROWS && v < p.vocab) {
+      if (p.present) {
+        absent = !p.present[v];
+      } else {
+        const unsigned int at = lower_bound(p.keys, p.n, v);
+        absent = at == p.n || __ldg(p.keys + at) != v;
+      }
+    }
+    unsigned int rows = __ballot_sync(0xFFFFFFFFu, absent);
+    raw zero;
+    memset(&zero, 0, sizeof zero);
+    for (; rows; rows &= rows - 1) {
+      raw* row = reinterpret_cast<raw*>(p.dtable + (size_t)(v0 + __ffs(rows) - 1) * p.ld_dtable);
+      for (int c = lane; c < p.vecs; c += 32) row[c] = zero;
+    }
+    return;
   }
-  const unsigned int count = last - chunk + 1;
-  const unsigned int from = (unsigned int)((size_t)count * share / JOIN_PARTS), to = (unsigned int)((size_t)count * (share + 1) / JOIN_PARTS);
-  for (int c0 = blockIdx.y * 128; c0 < width; c0 += gridDim.y * 128) {
-    const int c = c0 + lane * 4;
+  after_previous();
+  const unsigned int slices = (width + 127) / 128;
+  const size_t items = (size_t)*p.joins * slices;
+  for (size_t item = blockIdx.x - p.fill_blocks; item < items; item += gridDim.x - p.fill_blocks) {
+    const uint2 run = p.join_runs[item / slices];
+    const unsigned int chunk = run.x, key = run.y;
+    // the run's last chunk: chunks whose first element has the key
+    unsigned int last = chunk;
+    for (;;) {
+      const size_t at = (size_t)(last + 1 + lane) * p.chunk;
+      const unsigned int same = __ballot_sync(0xFFFFFFFFu, at < p.n && __ldg(p.keys + at) == key);
+      last += same == 0xFFFFFFFFu ? 32 : __ffs(~same) - 1;
+      if (same != 0xFFFFFFFFu) break;
+    }
+    const unsigned int count = last - chunk + 1;
+    const unsigned int from = (unsigned int)((size_t)count * share / JOIN_PARTS), to = (unsigned int)((size_t)count * (share + 1) / JOIN_PARTS);
+    const int c = (int)(item % slices) * 128 + lane * 4;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     if (c < width)
 #pragma unroll 8
@@ -416,17 +435,22 @@ GradPlan grad_plan(size_t n, size_t vocab, size_t width) {
   return g;
 }
 struct GradSpace {
-  unsigned int *keys[2], *pos[2], *counts;
+  unsigned int *keys[2], *pos[2], *counts, *joins;
+  unsigned char* present;
+  uint2* join_runs;
   float *head, *tail;
 };
-size_t grad_space(const GradPlan& g, size_t n, void* base, GradSpace* s) {
+size_t grad_space(const GradPlan& g, size_t n, size_t vocab, void* base, GradSpace* s) {
   Carver c(base);
   const int buffers = g.passes ? 2 : 1;
   for (int i = 0; i < buffers; ++i) {
     s->keys[i] = c.take<unsigned int>(n);
     s->pos[i] = c.take<unsigned int>(n);
   }
-  s->counts = c.take<unsigned int>(g.passes ? (size_t)g.tiles << g.bits : 0);
+  s->counts = c.take<unsigned int>(((size_t)g.passes * g.tiles) << g.bits);
+  s->present = c.take<unsigned char>(g.passes ? vocab : 0);
+  s->joins = c.take<unsigned int>(1);
+  s->join_runs = c.take<uint2>(g.chunks);
   s->head = c.take<float>(g.chunks * g.pitch);
   s->tail = c.take<float>(g.chunks * g.pitch);
   return c.used;
@@ -470,15 +494,12 @@ void run_launch(RunSum p, size_t width, Chain& chain) {
   if (p.tpr_log2 < 3) p.tpr_log2 = 3;
   p.slices = (p.vecs + (1 << p.tpr_log2) - 1) >> p.tpr_log2;
   const size_t units = (size_t)p.chunks * p.slices, per_block = RUN_THREADS >> p.tpr_log2;
-  p.sum_blocks = (unsigned int)((units + per_block - 1) / per_block);
-  const unsigned int per_fill = RUN_THREADS / 32 * FILL_ROWS, fill = (p.vocab + per_fill - 1) / per_fill;
-  chain.launch(run_sum_kernel<T, VB>, dim3(p.sum_blocks + fill), RUN_THREADS, 0, 0, p);
-  if (p.chunks > 1) {
-    // most blocks find that no run begins in their chunk and goes on: a few thousand of them at most
-    unsigned int slices = (unsigned int)((width + 127) / 128);
-    while (slices > 1 && (size_t)slices * p.chunks > 8192) slices /= 2;
-    chain.launch(run_join_kernel<T>, dim3(p.chunks, slices), 32 * JOIN_PARTS, 0, 0, p, (int)width);
-  }
+  chain.launch(run_sum_kernel<T, VB>, dim3((unsigned int)((units + per_block - 1) / per_block)), RUN_THREADS, 0, 0, p);
+  const size_t most = (size_t)(p.chunks - 1) * ((width + 127) / 128);
+  const unsigned int per_fill = JOIN_PARTS * FILL_ROWS;
+  p.fill_blocks = (p.vocab + per_fill - 1) / per_fill;
+  const unsigned int join_blocks = (unsigned int)(most < 148 * 16 ? most : 148 * 16);
+  chain.launch(run_join_kernel<T, VB>, dim3(p.fill_blocks + join_blocks), JOIN_THREADS, 0, 0, p, (int)width);
 }
 
 }  // namespace
@@ -523,7 +544,7 @@ int b2_embed_grad_workspace(size_t n, size_t vocab, size_t width, size_t* bytes)
   if (rc != B2_OK) return rc;
   if (!bytes) return call_error(B2_ERR_INVALID, "b2_embed_grad_workspace: null pointer");
   GradSpace s;
-  *bytes = grad_space(grad_plan(n, vocab, width), n, nullptr, &s);
+  *bytes = grad_space(grad_plan(n, vocab, width), n, vocab, nullptr, &s);
   return B2_OK;
 }
 
@@ -539,7 +560,7 @@ int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dou
   if (reinterpret_cast<size_t>(workspace) % 256) return call_error(B2_ERR_INVALID, "b2_embed_grad: the workspace is not on a 256-byte boundary");
   const GradPlan g = grad_plan(n, vocab, width);
   GradSpace w;
-  const size_t need = grad_space(g, n, workspace, &w);
+  const size_t need = grad_space(g, n, vocab, workspace, &w);
   if (n && workspace_bytes < need) return call_error(B2_ERR_INVALID, "b2_embed_grad: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   int sms;
   if ((rc = lm_device(&sms)) != B2_OK) return rc;
@@ -552,12 +573,11 @@ int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dou
   if (g.passes == 0) {
     const int per_block = RANK_THREADS / 32 * RANK_PER_WARP;
     chain.launch(rank_sort_kernel, dim3((unsigned int)((n + per_block - 1) / per_block)), RANK_THREADS, n * 4, 0, tokens, wide, (int)n,
-                 (unsigned int)vocab, w.keys[0], w.pos[0]);
+                 (unsigned int)vocab, w.keys[0], w.pos[0], w.joins);
   } else {
     RadixPass p{};
     p.wide = wide;
     p.vocab = (unsigned int)vocab;
-    p.counts = w.counts;
     p.n = (unsigned int)n;
     p.tile = g.tile;
     p.tiles = g.tiles;
@@ -570,7 +590,13 @@ int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dou
       p.keys_out = w.keys[sorted];
       p.pos_out = w.pos[sorted];
       p.shift = i * g.bits;
-      chain.launch(radix_count_kernel, dim3(g.tiles), RADIX_THREADS, 0, 0, p);
+      const size_t bins = (size_t)g.tiles << g.bits;
+      p.counts = w.counts + i * bins;
+      p.present = i == 0 ? w.present : nullptr;
+      p.next_counts = i + 1 < g.passes ? p.counts + bins : nullptr;
+      if (i == 0)
+        chain.launch(radix_count_kernel, dim3(g.tiles), RADIX_THREADS, 0, 0, p, p.counts + bins, (int)((g.passes - 1) * bins), w.present,
+                     w.joins);
       if (radix_rounds(n) == 2) chain.launch(radix_place_kernel<2>, dim3(g.tiles), RADIX_THREADS, 0, 0, p);
       else chain.launch(radix_place_kernel<8>, dim3(g.tiles), RADIX_THREADS, 0, 0, p);
     }
@@ -589,6 +615,9 @@ int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dou
   r.head = w.head;
   r.tail = w.tail;
   r.pitch = g.pitch;
+  r.joins = w.joins;
+  r.join_runs = w.join_runs;
+  r.present = g.passes ? w.present : nullptr;
   r.scale = scale;
   const int vb = vector_bytes(e, reinterpret_cast<size_t>(dout) | reinterpret_cast<size_t>(dtable) | width * e | r.ld_dout | r.ld_dtable);
   if (dtype == B2_DTYPE_BF16) {

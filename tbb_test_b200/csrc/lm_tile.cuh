@@ -16,8 +16,8 @@
 //           accumulator (about 2e-8 of the sum each time, and always towards zero), so a sum is handed over every
 //           SPLIT_SUM k-blocks and added up in fp32 registers, rounded to nearest.
 //
-// Warps: 0 loads, 1 allocates tensor memory and (in the leader) issues, 2 to 9 work on elements: the warps of a lane quarter
-// share its columns by halves.
+// Warps: 0 loads, 1 allocates tensor memory and (in the leader) issues, the others work on elements: those of a lane quarter share
+// its columns. There are 8 of them in the plain form and 16 in the split one, where small matrices wait for nothing else as long.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -29,9 +29,6 @@ namespace b2 {
 namespace {
 
 constexpr int TILE_M = 256, TILE_K = 64;
-constexpr int TILE_EPI_WARPS = 8;
-constexpr int TILE_THREADS = 64 + 32 * TILE_EPI_WARPS;
-constexpr int STAGE_BYTES = 32 * 128;  // a warp's buffer for 32 rows of 128 bytes
 constexpr int SPLIT_SUM = 16;  // k-blocks per hand-over
 constexpr float LO_UP = 2048.f;  // lo = 2^11 (x - hi)
 constexpr uint32_t ACC_COLS = 256;  // tensor-memory columns of an accumulator stage
@@ -46,7 +43,14 @@ struct TileForm {
   static constexpr int STAGES = SPLIT ? 4 : 6;
   static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128;
   static constexpr uint32_t SLABS = (A_BYTES + B_BYTES) * (SPLIT ? 2 : 1);  // of a stage
-  static constexpr size_t SMEM = 1024 + STAGES * SLABS + TILE_EPI_WARPS * STAGE_BYTES;
+  static constexpr int WARPS = SPLIT ? 16 : 8;   // on elements
+  static constexpr int PARTS = WARPS / 4;        // warps that share a row's columns
+  static constexpr int COLS = BN / PARTS;        // columns of a warp
+  static constexpr int CHUNK = SPLIT ? 16 : 32;  // columns that it works on at a time
+  static constexpr int STAGE = 32 * CHUNK * 4;   // bytes of its buffer for that
+  static constexpr int THREADS = 64 + 32 * WARPS;
+  static constexpr int BOUND = SPLIT ? 640 : THREADS;  // registers are handed out as if 18 warps were 20
+  static constexpr size_t SMEM = 1024 + STAGES * SLABS + WARPS * STAGE;
 };
 
 struct TileMaps {
@@ -67,11 +71,12 @@ struct Tile {
 };
 
 // Op: struct Params; static constexpr bool SPLIT; Op(const Params&, const TileMaps&); int tiles(); Tile tile(int t);
-//     and in the element warps: void begin(const Tile&, int row, int half); void chunk(const Tile&, int row0, int col0,
-//     float (&v)[32], uint8_t* stage, int lane) for 32 columns of rows row0 + lane; void end(const Tile&, int row, int half);
+//     and in the element warps: void begin(const Tile&, int row, int col, int lane) before the sums are there, for the warp's
+//     first row and column; void chunk(const Tile&, int row0, int col0, float (&v)[CHUNK], uint8_t* stage, int lane) for CHUNK columns of
+//     rows row0 + lane; void end(const Tile&, int row, int part) for the thread's row and its warp's part of the columns;
 //     static constexpr bool STORES: it issues TMA stores from `stage`.
 template <class Op>
-__global__ void __launch_bounds__(TILE_THREADS, 1) tile_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ TileLayout L,
+__global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ TileLayout L,
                                                                const __grid_constant__ typename Op::Params params) {
   constexpr bool SPLIT = Op::SPLIT;
   typedef TileForm<SPLIT> F;
@@ -97,7 +102,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) tile_kernel(const __grid_cons
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full_bar[a], 1);
-      mbar_init(&acc_empty_bar[a], 2 * TILE_EPI_WARPS);  // the element warps of both CTAs
+      mbar_init(&acc_empty_bar[a], 2 * F::WARPS);  // the element warps of both CTAs
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a) : "memory");
@@ -190,36 +195,34 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) tile_kernel(const __grid_cons
       }
     }
   } else {
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    constexpr int COLS = F::BN / 2;  // columns of this warp
-    uint8_t* stage = smem + F::STAGES * F::SLABS + (warp - 2) * STAGE_BYTES;
+    const int q = warp & 3, part = (warp - 2) >> 2;
+    constexpr int CHUNK = F::CHUNK;
+    uint8_t* stage = smem + F::STAGES * F::SLABS + (warp - 2) * F::STAGE;
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
     for (int t = pair; t < tiles && ok; t += num_pairs) {
       const Tile tile = op.tile(t);
-      const int row0 = tile.m0 + (int)rank * 128 + q * 32, c0 = half * COLS;
-      const uint32_t lanes = (uint32_t)(q * 32) << 16;
-      if (SPLIT) {
-        float sum[COLS];
+      const int row0 = tile.m0 + (int)rank * 128 + q * 32, col0 = tile.n0 + part * F::COLS;
+      const uint32_t place = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(part * F::COLS);
+      op.begin(tile, row0, col0, lane);
+      if constexpr (SPLIT) {
+        float sum[F::COLS];
         if (tile.kblocks == 0) {
 #pragma unroll
-          for (int c = 0; c < COLS; ++c) sum[c] = 0.f;
+          for (int c = 0; c < F::COLS; ++c) sum[c] = 0.f;
         }
         for (int kb = 0; kb < tile.kblocks; kb += SPLIT_SUM) {
           if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_flag, &tile_status, 4u)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t from = tmem_base + lanes + (uint32_t)acc * ACC_COLS + (uint32_t)c0;
+          const uint32_t from = place + (uint32_t)acc * ACC_COLS;
+          uint32_t r[32], x[32];
+          tmem_ld32(from, r);
+          tmem_ld32(from + F::BN, x);
 #pragma unroll
-          for (int c = 0; c < COLS; c += 32) {
-            uint32_t r[32], x[32];
-            tmem_ld32(from + c, r);
-            tmem_ld32(from + F::BN + c, x);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float v = fmaf(__uint_as_float(x[j]), 1.f / LO_UP, __uint_as_float(r[j]));
-              sum[c + j] = kb == 0 ? v : sum[c + j] + v;
-            }
+          for (int j = 0; j < 32; ++j) {
+            const float v = fmaf(__uint_as_float(x[j]), 1.f / LO_UP, __uint_as_float(r[j]));
+            sum[j] = kb == 0 ? v : sum[j] + v;
           }
           tc_fence_before();
           __syncwarp();
@@ -228,25 +231,23 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) tile_kernel(const __grid_cons
           if (acc == 0) acc_phase ^= 1;
         }
         if (!ok) break;
-        op.begin(tile, row0 + lane, half);
 #pragma unroll
-        for (int c = 0; c < COLS; c += 32) {
-          float v[32];
+        for (int c = 0; c < F::COLS; c += CHUNK) {
+          float v[CHUNK];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = sum[c + j];
-          op.chunk(tile, row0, tile.n0 + c0 + c, v, stage, lane);
+          for (int j = 0; j < CHUNK; ++j) v[j] = sum[c + j];
+          op.chunk(tile, row0, col0 + c, v, stage, lane);
         }
-        op.end(tile, row0 + lane, half);
+        op.end(tile, row0 + lane, part);
       } else {
-        op.begin(tile, row0 + lane, half);
         const bool summed = tile.kblocks > 0;
         if (summed) {
           if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_flag, &tile_status, 4u)) break;
           tc_fence_after();
         }
-        const uint32_t from = tmem_base + lanes + (uint32_t)acc * ACC_COLS + (uint32_t)c0;
+        const uint32_t from = place + (uint32_t)acc * ACC_COLS;
 #pragma unroll 1
-        for (int c = 0; c < COLS; c += 32) {
+        for (int c = 0; c < F::COLS; c += CHUNK) {
           uint32_t r[32];
           if (summed) {
             tmem_ld32(from + c, r);
@@ -254,17 +255,17 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) tile_kernel(const __grid_cons
 #pragma unroll
             for (int j = 0; j < 32; ++j) r[j] = 0u;
           }
-          if (summed && c + 32 == COLS) {  // all read: the next tile may be summed here
+          if (summed && c + CHUNK == F::COLS) {  // all read: the next tile may be summed here
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_leader(map_to_cta(smem_u32(&acc_empty_bar[acc]), 0));
           }
-          float v[32];
+          float v[CHUNK];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-          op.chunk(tile, row0, tile.n0 + c0 + c, v, stage, lane);
+          for (int j = 0; j < CHUNK; ++j) v[j] = __uint_as_float(r[j]);
+          op.chunk(tile, row0, col0 + c, v, stage, lane);
         }
-        op.end(tile, row0 + lane, half);
+        op.end(tile, row0 + lane, part);
         if (summed) {
           acc ^= 1;
           if (acc == 0) acc_phase ^= 1;
@@ -290,58 +291,67 @@ __device__ __forceinline__ void split_half(float v, __half& hi, __half& lo) {
 }
 
 __device__ __forceinline__ void store_pair(__half* hi, __half* lo, long long at, const float4& x) {
-  const float f[4] = {x.x, x.y, x.z, x.w};
-  __half a[4], b[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) split_half(f[i], a[i], b[i]);
-  *reinterpret_cast<uint2*>(hi + at) = *reinterpret_cast<const uint2*>(a);
-  *reinterpret_cast<uint2*>(lo + at) = *reinterpret_cast<const uint2*>(b);
+  const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);  // two at a time
+  const float2 f = __half22float2(a), g = __half22float2(b);
+  const __half2 c = __floats2half2_rn((x.x - f.x) * LO_UP, (x.y - f.y) * LO_UP), d = __floats2half2_rn((x.z - g.x) * LO_UP, (x.w - g.y) * LO_UP);
+  *reinterpret_cast<uint2*>(hi + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  *reinterpret_cast<uint2*>(lo + at) = make_uint2(*reinterpret_cast<const uint32_t*>(&c), *reinterpret_cast<const uint32_t*>(&d));
 }
-__device__ __forceinline__ float4 load_pair(const __half* hi, const __half* lo, long long at) {
-  const uint2 a = *reinterpret_cast<const uint2*>(hi + at), b = *reinterpret_cast<const uint2*>(lo + at);
-  const __half2 *ah = reinterpret_cast<const __half2*>(&a), *bh = reinterpret_cast<const __half2*>(&b);
-  const float2 a0 = __half22float2(ah[0]), a1 = __half22float2(ah[1]), b0 = __half22float2(bh[0]), b1 = __half22float2(bh[1]);
+struct Pair4 {  // four neighbouring elements as they lie in memory
+  uint2 hi, lo;
+};
+__device__ __forceinline__ Pair4 load_pair(const __half* hi, const __half* lo, long long at) {
+  return Pair4{*reinterpret_cast<const uint2*>(hi + at), *reinterpret_cast<const uint2*>(lo + at)};
+}
+__device__ __forceinline__ float4 pair_value(const Pair4& p) {
+  const __half2 *a = reinterpret_cast<const __half2*>(&p.hi), *b = reinterpret_cast<const __half2*>(&p.lo);
+  const float2 a0 = __half22float2(a[0]), a1 = __half22float2(a[1]), b0 = __half22float2(b[0]), b1 = __half22float2(b[1]);
   return make_float4(fmaf(b0.x, 1.f / LO_UP, a0.x), fmaf(b0.y, 1.f / LO_UP, a0.y), fmaf(b1.x, 1.f / LO_UP, a1.x), fmaf(b1.y, 1.f / LO_UP, a1.y));
 }
 
-// The chunk through shared memory, so that a warp's accesses to global memory cover whole rows: f(row, col, v, old) gets
-// four neighbouring columns of a row, eight lanes per row, four rows at a time, and what load(row, col) read for it before.
-// 16-byte piece j of row r lies at slot j ^ (r & 7): no conflicts either way.
-template <class Load, class Fn>
-__device__ __forceinline__ void by_rows(int row0, int col0, const float (&v)[32], uint8_t* stage, int lane, Load load, Fn f) {
-  const int c = (lane & 7) * 4;
-  decltype(load(0, 0)) old[8];
+// A chunk of W columns through shared memory, so that a warp's accesses to global memory cover whole rows: W / 4 lanes take four
+// neighbouring columns of a row each. Quad i of a lane is row quad_row<W>(i, lane), columns quad_col<W>(lane) and up, of the chunk; f(i,
+// row, col, v) gets it. 16-byte pieces are swizzled so that there are no conflicts either way.
+template <int W>
+__device__ __forceinline__ int quad_row(int i, int lane) { return i * (128 / W) + lane / (W / 4); }
+template <int W>
+__device__ __forceinline__ int quad_col(int lane) { return lane % (W / 4) * 4; }
+template <int W>
+__device__ __forceinline__ int quad_slot(int row, int piece) { return row * W * 4 + ((piece ^ (W == 32 ? row & 7 : row >> 1 & 3)) << 4); }
+template <int W, class Fn>
+__device__ __forceinline__ void by_rows(int row0, int col0, const float (&v)[W], uint8_t* stage, int lane, Fn f) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) old[i] = load(row0 + 4 * i + (lane >> 3), col0 + c);
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    *reinterpret_cast<float4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  for (int j = 0; j < W / 4; ++j)
+    *reinterpret_cast<float4*>(stage + quad_slot<W>(lane, j)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
   __syncwarp();
+  const int c = quad_col<W>(lane);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = 4 * i + (lane >> 3);
-    f(row0 + r, col0 + c, *reinterpret_cast<const float4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4)), old[i]);
+  for (int i = 0; i < W / 4; ++i) {
+    const int r = quad_row<W>(i, lane);
+    f(i, row0 + r, col0 + c, *reinterpret_cast<const float4*>(stage + quad_slot<W>(r, c / 4)));
   }
   __syncwarp();
 }
-struct Nothing {};
-struct LoadNothing {
-  __device__ __forceinline__ Nothing operator()(int, int) const { return Nothing{}; }
-};
-// The same chunk transposed: f(col, row, v, old) gets four neighbouring rows of a column.
-template <class Load, class Fn>
-__device__ __forceinline__ void by_columns(int row0, int col0, const float (&v)[32], uint8_t* stage, int lane, Load load, Fn f) {
-  const int r = (lane & 7) * 4;
-  decltype(load(0, 0)) old[8];
+// Quads as by_rows hands them out, transposed: f(col, row, v) gets four neighbouring rows of a column. Rows of a column lie
+// at r ^ 8 (c / 4), for 16 columns.
+template <class Fn>
+__device__ __forceinline__ void by_columns(int row0, int col0, const float4 (&x)[4], uint8_t* stage, int lane, Fn f) {
+  float* t = reinterpret_cast<float*>(stage);
+  const int c0 = quad_col<16>(lane), turn = (c0 >> 2) * 8;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) old[i] = load(col0 + 4 * i + (lane >> 3), row0 + r);
-#pragma unroll
-  for (int j = 0; j < 32; ++j) *reinterpret_cast<float*>(stage + j * 128 + lane * 4) = v[j];
+  for (int i = 0; i < 4; ++i) {
+    const int r = quad_row<16>(i, lane) ^ turn;
+    t[c0 * 32 + r] = x[i].x;
+    t[(c0 + 1) * 32 + r] = x[i].y;
+    t[(c0 + 2) * 32 + r] = x[i].z;
+    t[(c0 + 3) * 32 + r] = x[i].w;
+  }
   __syncwarp();
+  const int r = (lane & 7) * 4;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
     const int c = 4 * i + (lane >> 3);
-    f(col0 + c, row0 + r, *reinterpret_cast<const float4*>(stage + c * 128 + r * 4), old[i]);
+    f(col0 + c, row0 + r, *reinterpret_cast<const float4*>(t + c * 32 + (r ^ (i * 8))));
   }
   __syncwarp();
 }
@@ -429,7 +439,7 @@ int tile_launch(const char* who, const TileOperand& a, const TileOperand& b, con
   if (e != cudaSuccess) return launch_error(e, who);
   const int pairs = sms / 2;
   const unsigned int grid = 2 * (unsigned int)(most_tiles < pairs ? most_tiles : pairs);
-  chain.launch(tile_kernel<Op>, dim3(grid), TILE_THREADS, smem, 2, maps, L, p);
+  chain.launch(tile_kernel<Op>, dim3(grid), TileForm<Op::SPLIT>::THREADS, smem, 2, maps, L, p);
   return launch_error(chain.err, who);
 }
 

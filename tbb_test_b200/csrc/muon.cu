@@ -188,32 +188,36 @@ struct SymmetricOp {
     r.kblocks = p.kblocks;
     return r;
   }
-  __device__ __forceinline__ void begin(const Tile&, int, int) {}
-  __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[32], uint8_t* stage, int lane) {
-    const long long base = (long long)t.z * p.side * p.side;
-    if (row0 >= p.side) return;  // uniform: sides are multiples of 128
-    const float unit = MIDDLE ? P_UP * NS_C / (A_UP * A_UP) : A_UP / (X_UP * X_UP);
+  // a is loaded while the products are summed: it is what a small matrix's middle factor would wait for otherwise (5.6 against 2.7 us
+  // for the elements of a tile)
+  Pair4 a[8];
+  __device__ __forceinline__ void begin(const Tile& t, int row0, int col0, int lane) {
+    if (!MIDDLE || row0 >= p.side) return;
+    const __half *hi = p.a_hi + (long long)t.z * p.side * p.side, *lo = p.a_lo + (long long)t.z * p.side * p.side;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] *= unit;
-    if constexpr (MIDDLE) {
-      constexpr float b = P_UP * NS_B / A_UP;
-      auto load = [&](int r, int c) { return load_pair(p.a_hi, p.a_lo, base + (long long)r * p.side + c); };
-      auto store = [&](int r, int c, const float4& y, const float4& a) {
-        float4 x = make_float4(fmaf(b, a.x, y.x), fmaf(b, a.y, y.y), fmaf(b, a.z, y.z), fmaf(b, a.w, y.w));
-        if (r == c) x.x += NS_A * P_UP;
-        if (r == c + 1) x.y += NS_A * P_UP;
-        if (r == c + 2) x.z += NS_A * P_UP;
-        if (r == c + 3) x.w += NS_A * P_UP;
-        store_pair(p.to_hi, p.to_lo, base + (long long)r * p.side + c, x);
-      };
-      by_rows(row0, col0, v, stage, lane, load, store);
-      // on the diagonal both halves are computed; elsewhere a at the transposed place, which holds the same bits
-      if (t.n0 >= t.m0 + TILE_M) by_columns(row0, col0, v, stage, lane, load, store);
-    } else {
-      auto store = [&](int r, int c, const float4& x, Nothing) { store_pair(p.to_hi, p.to_lo, base + (long long)r * p.side + c, x); };
-      by_rows(row0, col0, v, stage, lane, LoadNothing(), store);
-      if (t.n0 >= t.m0 + TILE_M) by_columns(row0, col0, v, stage, lane, LoadNothing(), store);
-    }
+    for (int i = 0; i < 8; ++i)
+      a[i] = load_pair(hi, lo, (long long)(row0 + quad_row<16>(i & 3, lane)) * p.side + col0 + (i >> 2) * 16 + quad_col<16>(lane));
+  }
+  __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[16], uint8_t* stage, int lane) {
+    if (row0 >= p.side) return;  // uniform: sides are multiples of 128
+    const long long base = (long long)t.z * p.side * p.side;
+    constexpr float unit = MIDDLE ? P_UP * NS_C / (A_UP * A_UP) : A_UP / (X_UP * X_UP), b = P_UP * NS_B / A_UP;
+    const bool second = (col0 - t.n0) & 16;  // of the warp's two chunks
+    float4 x[4];
+    by_rows(row0, col0, v, stage, lane, [&](int i, int r, int c, const float4& y) {
+      x[i] = make_float4(y.x * unit, y.y * unit, y.z * unit, y.w * unit);
+      if (MIDDLE) {
+        const float4 old = pair_value(second ? a[4 + i] : a[i]);
+        x[i] = make_float4(fmaf(b, old.x, x[i].x), fmaf(b, old.y, x[i].y), fmaf(b, old.z, x[i].z), fmaf(b, old.w, x[i].w));
+        if (r == c) x[i].x += NS_A * P_UP;
+        if (r == c + 1) x[i].y += NS_A * P_UP;
+        if (r == c + 2) x[i].z += NS_A * P_UP;
+        if (r == c + 3) x[i].w += NS_A * P_UP;
+      }
+      store_pair(p.to_hi, p.to_lo, base + (long long)r * p.side + c, x[i]);
+    });
+    if (t.n0 >= t.m0 + TILE_M)  // on the diagonal both halves are computed
+      by_columns(row0, col0, x, stage, lane, [&](int r, int c, const float4& y) { store_pair(p.to_hi, p.to_lo, base + (long long)r * p.side + c, y); });
   }
   __device__ __forceinline__ void end(const Tile&, int, int) {}
 };
@@ -254,47 +258,52 @@ struct NextOp {
     r.kblocks = p.kblocks;
     return r;
   }
-  __device__ __forceinline__ void begin(const Tile&, int, int) {}
-  __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[32], uint8_t* stage, int lane) {
-    if (row0 >= p.rows_up) return;
-    const float unit = LAST ? p.step / (X_UP * P_UP) : 1.f / P_UP;
+  float4 old[8];  // of w, loaded while the last step's products are summed
+  __device__ __forceinline__ void begin(const Tile& t, int row0, int col0, int lane) {
+    if (!LAST) return;
+    const float* w = p.list.w[t.z];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] *= unit;
+    for (int i = 0; i < 8; ++i) {
+      const int r = row0 + quad_row<16>(i & 3, lane), c = col0 + (i >> 2) * 16 + quad_col<16>(lane);
+      old[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r >= p.rows || c >= p.cols) continue;
+      const float* from = w + (long long)r * p.ld_w + c;
+      if (p.vec_w && c + 4 <= p.cols) {
+        old[i] = *reinterpret_cast<const float4*>(from);
+      } else {
+        old[i].x = from[0];
+        if (c + 1 < p.cols) old[i].y = from[1];
+        if (c + 2 < p.cols) old[i].z = from[2];
+        if (c + 3 < p.cols) old[i].w = from[3];
+      }
+    }
+  }
+  __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[16], uint8_t* stage, int lane) {
+    if (row0 >= p.rows_up) return;
     if (!LAST) {
       const long long base = (long long)t.z * p.rows_up * p.cols_up;
-      by_rows(row0, col0, v, stage, lane, LoadNothing(), [&](int r, int c, const float4& x, Nothing) {
-        store_pair(p.to_hi, p.to_lo, base + (long long)r * p.cols_up + c, x);
+      constexpr float unit = 1.f / P_UP;
+      by_rows(row0, col0, v, stage, lane, [&](int, int r, int c, const float4& x) {
+        store_pair(p.to_hi, p.to_lo, base + (long long)r * p.cols_up + c, make_float4(x.x * unit, x.y * unit, x.z * unit, x.w * unit));
       });
       return;
     }
+    const float unit = p.step / (X_UP * P_UP);
+    const bool second = (col0 - t.n0) & 16;  // of the warp's two chunks
     float* w = p.list.w[t.z];
     __nv_bfloat16* copy = p.list.copy[t.z];
-    auto load = [&](int r, int c) {
-      float4 old = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r < p.rows && c < p.cols) {
-        const float* from = w + (long long)r * p.ld_w + c;
-        if (p.vec_w && c + 4 <= p.cols) {
-          old = *reinterpret_cast<const float4*>(from);
-        } else {
-          old.x = from[0];
-          if (c + 1 < p.cols) old.y = from[1];
-          if (c + 2 < p.cols) old.z = from[2];
-          if (c + 3 < p.cols) old.w = from[3];
-        }
-      }
-      return old;
-    };
-    by_rows(row0, col0, v, stage, lane, load, [&](int r, int c, const float4& x, const float4& old) {
+    by_rows(row0, col0, v, stage, lane, [&](int i, int r, int c, const float4& x) {
       if (r >= p.rows || c >= p.cols) return;
-      const float f[4] = {fmaf(p.keep, old.x, -x.x), fmaf(p.keep, old.y, -x.y), fmaf(p.keep, old.z, -x.z), fmaf(p.keep, old.w, -x.w)};
+      const float4 o = second ? old[4 + i] : old[i];
+      const float f[4] = {fmaf(p.keep, o.x, -x.x * unit), fmaf(p.keep, o.y, -x.y * unit), fmaf(p.keep, o.z, -x.z * unit), fmaf(p.keep, o.w, -x.w * unit)};
       float* to = w + (long long)r * p.ld_w + c;
       const bool whole = c + 4 <= p.cols;
       if (p.vec_w && whole) {
         *reinterpret_cast<float4*>(to) = make_float4(f[0], f[1], f[2], f[3]);
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (c + i < p.cols) to[i] = f[i];
+        for (int k = 0; k < 4; ++k)
+          if (c + k < p.cols) to[k] = f[k];
       }
       if (!copy) return;
       __nv_bfloat16* out = copy + (long long)r * p.ld_copy + c;
@@ -302,8 +311,8 @@ struct NextOp {
         *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]));
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (c + i < p.cols) out[i] = __float2bfloat16_rn(f[i]);
+        for (int k = 0; k < 4; ++k)
+          if (c + k < p.cols) out[k] = __float2bfloat16_rn(f[k]);
       }
     });
   }

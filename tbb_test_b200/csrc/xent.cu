@@ -99,11 +99,22 @@ __global__ void __launch_bounds__(256) max_kernel(const float* __restrict__ h, s
   const bool of_h = (int)blockIdx.x < split_at;
   const int block = of_h ? blockIdx.x : blockIdx.x - split_at, blocks = of_h ? split_at : gridDim.x - split_at;
   const int rows = of_h ? (int)meta->rows : vocab;
+  const float* x = of_h ? h : w;
+  const size_t ld = of_h ? ldh : ldw;
+  const bool vec = width % 4 == 0 && ld % 4 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  const int per_row = vec ? width / 4 : width;
+  const long long all = (long long)rows * per_row, stride = (long long)blocks * 256;
   unsigned int most = 0;
-  for (int r = block; r < rows; r += blocks) {
-    const float* x = of_h ? h + (size_t)row_of[r] * ldh : w + (size_t)r * ldw;
 #pragma unroll 4
-    for (int c = threadIdx.x; c < width; c += 256) most = max(most, __float_as_uint(__ldg(x + c)) & 0x7FFFFFFFu);
+  for (long long i = (long long)block * 256 + threadIdx.x; i < all; i += stride) {
+    const int r = (int)(i / per_row), c = (int)(i - (long long)r * per_row);
+    const float* row = x + (size_t)(of_h ? __ldg(row_of + r) : r) * ld;
+    if (vec) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(row) + c);
+      most = max(most, max(max(v.x & 0x7FFFFFFFu, v.y & 0x7FFFFFFFu), max(v.z & 0x7FFFFFFFu, v.w & 0x7FFFFFFFu)));
+    } else {
+      most = max(most, __float_as_uint(__ldg(row + c)) & 0x7FFFFFFFu);
+    }
   }
   most = __reduce_max_sync(0xFFFFFFFFu, most);
   if ((threadIdx.x & 31) == 0 && most) atomicMax(of_h ? &meta->max_h : &meta->max_w, most);  // order does not matter
@@ -122,10 +133,14 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(const T* __restrict__ x,
   const int rows = GATHER ? row_blocks(have) * TILE_M : all_rows;
   const float up = SPLIT ? pow2(up_exp(GATHER ? meta->max_h : meta->max_w)) : 1.f;
   const bool vec = ld % (16 / sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
-  for (int r = blockIdx.x; r < rows; r += gridDim.x) {
-    const bool in = r < have;
-    const T* src = in ? x + (size_t)(GATHER ? row_of[r] : r) * ld : x;
-    for (int c = threadIdx.x * 8; c < pitch; c += 256 * 8) {
+  const int per_row = pitch / 8;
+  const long long all = (long long)rows * per_row;
+  {
+#pragma unroll 2
+    for (long long k = (long long)blockIdx.x * 256 + threadIdx.x; k < all; k += (long long)gridDim.x * 256) {
+      const int r = (int)(k / per_row), c = (int)(k - (long long)r * per_row) * 8;
+      const bool in = r < have;
+      const T* src = in ? x + (size_t)(GATHER ? __ldg(row_of + r) : r) * ld : x;
       T v[8];
       if (in && vec && c + 8 <= width) {
 #pragma unroll
@@ -154,7 +169,7 @@ struct LogitParams {
   const Meta* meta;
   int vocab, v_begin, v_count;  // this call's piece of the vocabulary
   int kblocks;
-  long long row_pitch;  // rows of the lists: parts are [tile half][row]
+  long long row_pitch;  // rows of the lists: parts are [warp of a tile's row][row]
   const int* target;
   float2* parts;        // maximum (times log2 e) and sum of 2^(x - maximum)
   float* target_logit;  // times log2 e
@@ -167,7 +182,7 @@ struct LogitParams {
 template <bool SPLIT_>
 struct LogitTiles {
   static constexpr bool SPLIT = SPLIT_;
-  static constexpr int BN = TileForm<SPLIT_>::BN;
+  static constexpr int BN = TileForm<SPLIT_>::BN, W = TileForm<SPLIT_>::CHUNK;
   const LogitParams& p;
   int rows, m_blocks, n_blocks, band;
   float unit;  // accumulators times this are logits times log2 e
@@ -204,38 +219,40 @@ struct StatOp : LogitTiles<SPLIT_> {
   float top, sum;
   int target;
   __device__ explicit StatOp(const LogitParams& q, const TileMaps& m) : LogitTiles<SPLIT_>(q, m) {}
-  __device__ __forceinline__ void begin(const Tile&, int row, int) {
+  __device__ __forceinline__ void begin(const Tile&, int row0, int, int lane) {
     top = -INFINITY;
     sum = 0.f;
-    target = row < this->rows ? __ldg(p.target + row) : -1;
+    target = row0 + lane < this->rows ? __ldg(p.target + row0 + lane) : -1;
   }
-  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[32], uint8_t*, int lane) {
+  static constexpr int W = LogitTiles<SPLIT_>::W;
+  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[W], uint8_t*, int lane) {
     if (col0 >= p.vocab) return;
-    if (col0 + 32 > p.vocab) {
+    if (col0 + W > p.vocab) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
+      for (int j = 0; j < W; ++j)
         if (col0 + j >= p.vocab) v[j] = -INFINITY;
     }
     float most = v[0];
 #pragma unroll
-    for (int j = 1; j < 32; ++j) most = fmaxf(most, v[j]);
+    for (int j = 1; j < W; ++j) most = fmaxf(most, v[j]);
     const float now = fmaxf(top, most * this->unit);
     const float base = now == -INFINITY ? 0.f : now;  // nothing but -inf so far: their exponentials are 0
     float s[4] = {sum * ex2(top - base), 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < 32; ++j) s[j & 3] += ex2(fmaf(v[j], this->unit, -base));
+    for (int j = 0; j < W; ++j) s[j & 3] += ex2(fmaf(v[j], this->unit, -base));
     sum = (s[0] + s[1]) + (s[2] + s[3]);
     top = now;
     const int at = target - col0;
-    if (at >= 0 && at < 32) {
+    if (at >= 0 && at < W) {
       float x = v[0];
 #pragma unroll
-      for (int j = 1; j < 32; ++j) x = j == at ? v[j] : x;
+      for (int j = 1; j < W; ++j) x = j == at ? v[j] : x;
       p.target_logit[row0 + lane] = x * this->unit;
     }
   }
-  __device__ __forceinline__ void end(const Tile& t, int row, int half) {
-    if (row < this->rows) p.parts[(long long)(t.n0 / LogitTiles<SPLIT_>::BN * 2 + half) * p.row_pitch + row] = make_float2(top, sum);
+  __device__ __forceinline__ void end(const Tile& t, int row, int part) {
+    typedef TileForm<SPLIT_> F;
+    if (row < this->rows) p.parts[(long long)(t.n0 / F::BN * F::PARTS + part) * p.row_pitch + row] = make_float2(top, sum);
   }
 };
 
@@ -254,28 +271,30 @@ struct GradOp : LogitTiles<SPLIT_> {
   __device__ explicit GradOp(const LogitParams& q, const TileMaps& m) : LogitTiles<SPLIT_>(q, m), map(&m.c) {
     to = SPLIT_ ? (float)(1 << D_EXP) : p.scale;
   }
-  __device__ __forceinline__ void begin(const Tile&, int row, int) {
+  __device__ __forceinline__ void begin(const Tile&, int row0, int, int lane) {
+    const int row = row0 + lane;
     in = row < this->rows;
     const float2 st = in ? __ldg(p.row_stat + row) : make_float2(0.f, 0.f);
     top = st.x;
     by = st.y * to;
     target = in ? __ldg(p.target + row) - p.v_begin : -1;
   }
-  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[32], uint8_t* stage, int lane) {
+  static constexpr int W = LogitTiles<SPLIT_>::W;
+  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[W], uint8_t* stage, int lane) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = ex2(fmaf(v[j], this->unit, -top)) * by;
+    for (int j = 0; j < W; ++j) v[j] = ex2(fmaf(v[j], this->unit, -top)) * by;
     const int at = target - col0;
-    if (at >= 0 && at < 32) {
+    if (at >= 0 && at < W) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] -= j == at ? to : 0.f;
+      for (int j = 0; j < W; ++j) v[j] -= j == at ? to : 0.f;
     }
-    if (!in || col0 + 32 > p.v_count) {
+    if (!in || col0 + W > p.v_count) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
+      for (int j = 0; j < W; ++j)
         if (!in || col0 + j >= p.v_count) v[j] = 0.f;
     }
     if constexpr (SPLIT_) {
-      by_rows(row0, col0, v, stage, lane, LoadNothing(), [&](int r, int c, const float4& x, Nothing) {
+      by_rows(row0, col0, v, stage, lane, [&](int, int r, int c, const float4& x) {
         store_pair(reinterpret_cast<__half*>(p.d_hi), reinterpret_cast<__half*>(p.d_lo), (long long)r * p.ld_d + c, x);
       });
     } else {
@@ -419,7 +438,7 @@ struct HiddenOp {
     r.kblocks = kb;
     return r;
   }
-  __device__ __forceinline__ void begin(const Tile& t, int, int) {
+  __device__ __forceinline__ void begin(const Tile& t, int, int, int) {
     if (t.z >= 0) {
       ld = BN;
       to = p.slots + (long long)t.z * TILE_M * BN - (t.m0 * ld + t.n0);
@@ -428,20 +447,21 @@ struct HiddenOp {
       to = p.acc;
     }
   }
-  __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[32], uint8_t* stage, int lane) {
+  static constexpr int W = TileForm<SPLIT_>::CHUNK;
+  __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[W], uint8_t* stage, int lane) {
     if (t.z == -2 || col0 >= p.width) return;
-    if (p.first)
-      by_rows(row0, col0, v, stage, lane, LoadNothing(), [&](int r, int c, const float4& x, Nothing) {
-        if (c < p.width) *reinterpret_cast<float4*>(to + r * ld + c) = make_float4(x.x * unit, x.y * unit, x.z * unit, x.w * unit);
-      });
-    else
-      by_rows(row0, col0, v, stage, lane,
-              [&](int r, int c) { return c < p.width ? *reinterpret_cast<const float4*>(to + r * ld + c) : make_float4(0.f, 0.f, 0.f, 0.f); },
-              [&](int r, int c, const float4& x, const float4& a) {
-                if (c < p.width)
-                  *reinterpret_cast<float4*>(to + r * ld + c) =
-                      make_float4(fmaf(x.x, unit, a.x), fmaf(x.y, unit, a.y), fmaf(x.z, unit, a.z), fmaf(x.w, unit, a.w));
-              });
+    float4 old[W / 4];
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i) {
+      const int c = col0 + quad_col<W>(lane);
+      old[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (!p.first && c < p.width) old[i] = *reinterpret_cast<const float4*>(to + (row0 + quad_row<W>(i, lane)) * ld + c);
+    }
+    by_rows(row0, col0, v, stage, lane, [&](int i, int r, int c, const float4& x) {
+      if (c < p.width)
+        *reinterpret_cast<float4*>(to + r * ld + c) =
+            make_float4(fmaf(x.x, unit, old[i].x), fmaf(x.y, unit, old[i].y), fmaf(x.z, unit, old[i].z), fmaf(x.w, unit, old[i].w));
+    });
   }
   __device__ __forceinline__ void end(const Tile&, int, int) {}
 };
@@ -473,9 +493,10 @@ struct WeightOp {
     r.z = 0;
     return r;
   }
-  __device__ __forceinline__ void begin(const Tile&, int, int) {}
-  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[32], uint8_t* stage, int lane) {
-    by_rows(row0, col0, v, stage, lane, LoadNothing(), [&](int r, int c, const float4& x, Nothing) {
+  __device__ __forceinline__ void begin(const Tile&, int, int, int) {}
+  static constexpr int W = TileForm<SPLIT_>::CHUNK;
+  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[W], uint8_t* stage, int lane) {
+    by_rows(row0, col0, v, stage, lane, [&](int, int r, int c, const float4& x) {
       if (r >= p.v_count || c >= p.width) return;
       const long long at = (long long)(p.v_begin + r) * p.ld_dw + c;
       const float f[4] = {x.x * unit, x.y * unit, x.z * unit, x.w * unit};
@@ -559,8 +580,8 @@ Sizes sizes_of(size_t rows, size_t width, size_t vocab, int dtype, int grads, co
   z.copy_w = z.split || reinterpret_cast<uintptr_t>(w) % 16 != 0 || ldw % 8 != 0;
   z.rows_up = (long long)(rows + TILE_M - 1) / TILE_M * TILE_M;
   z.pitch = (long long)(width + 63) / 64 * 64;
-  const int bn = z.split ? 128 : 256;
-  z.parts = 2 * (((long long)vocab + bn - 1) / bn);
+  const int bn = z.split ? TileForm<true>::BN : TileForm<false>::BN, shares = z.split ? TileForm<true>::PARTS : TileForm<false>::PARTS;
+  z.parts = shares * (((long long)vocab + bn - 1) / bn);
   z.piece = 0;
   if (grads) {
     // A piece of d should be in the L2 cache when the two products read it, and its 256-wide column blocks should go evenly

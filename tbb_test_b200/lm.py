@@ -11,6 +11,7 @@ for it. Matrices are float32 or bfloat16, all of one call alike, with unit strid
 rows. Tokens are int32 or int64; one outside [0, vocab) is padding. There is no CPU path.
 """
 import ctypes as C
+import functools
 
 import torch
 
@@ -55,9 +56,17 @@ def _tokens(name, t, device):
     return t, 8 if t.dtype == torch.int64 else 4
 
 
-def _workspace(size, device):
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(entry, *sizes):
+    """What b2_<entry>_workspace says for these sizes."""
+    need = C.c_size_t()
+    _ck(getattr(K.lib(), f"b2_{entry}_workspace")(*sizes, C.byref(need)))
+    return max(need.value, 1)
+
+
+def _workspace(device, entry, *sizes):
     """Device memory from torch's allocator, which hands it out again only behind this stream's work."""
-    return torch.empty(max(int(size), 1), dtype=torch.uint8, device=device)
+    return torch.empty(_workspace_bytes(entry, *sizes), dtype=torch.uint8, device=device)
 
 
 class _on:
@@ -102,10 +111,8 @@ def embed_grad(tokens, dout, vocab, scale=1.0, out=None):
     if out is None:
         out = torch.empty(vocab, width, dtype=dout.dtype, device=dout.device)
     po, ldo = _matrix("out", out, dout.dtype, (vocab, width), dout.device)
-    need = C.c_size_t()
-    _ck(K.lib().b2_embed_grad_workspace(n, vocab, width, C.byref(need)))
     with _on(dout.device) as stream:
-        ws = _workspace(need.value, dout.device)
+        ws = _workspace(dout.device, "embed_grad", n, vocab, width)
         _ck(K.lib().b2_embed_grad(t.data_ptr(), size, n, p, _DTYPES[dout.dtype], ld, vocab, width, scale, po, ldo,
                                   ws.data_ptr(), ws.numel(), stream))
     return out
@@ -133,10 +140,9 @@ def xent(h, w, targets, scale=1.0, grad=True, dh=None, dw=None):
         dw = torch.empty(vocab, width, dtype=dtype, device=device) if dw is None else dw
         pdh, lddh = _matrix("dh", dh, dtype, (rows, width), device)
         pdw, lddw = _matrix("dw", dw, dtype, (vocab, width), device)
-    need = C.c_size_t()
-    _ck(K.lib().b2_xent_workspace(rows, width, vocab, _DTYPES[dtype], int(grad), pw, ldw, C.byref(need)))
     with _on(device) as stream:
-        ws = _workspace(need.value, device)
+        # the size goes by the alignment of w and its rows
+        ws = _workspace(device, "xent", rows, width, vocab, _DTYPES[dtype], int(grad), pw % 256 or None, ldw)
         _ck(K.lib().b2_xent(rows, width, vocab, _DTYPES[dtype], ph, ldh, pw, ldw, t.data_ptr(), size, scale,
                             loss.data_ptr(), pdh, lddh, pdw, lddw, ws.data_ptr(), ws.numel(), stream))
     return (loss, dh, dw) if grad else loss
@@ -169,10 +175,8 @@ def muon(w, momentum_buffer, grad, *, lr, momentum=0.95, nesterov=True, weight_d
     n = len(pw)
     arr = lambda ps: None if ps is None else (C.c_void_p * n)(*ps)  # noqa: E731
     o = K.MuonOptions(lr, momentum, weight_decay, scale, eps, int(nesterov), steps)
-    need = C.c_size_t()
-    _ck(K.lib().b2_muon_workspace(n, shape[0], shape[1], C.byref(need)))
     with _on(device) as stream:
-        ws_ = _workspace(need.value, device)
+        ws_ = _workspace(device, "muon", n, shape[0], shape[1])
         _ck(K.lib().b2_muon(n, shape[0], shape[1], _DTYPES[gs[0].dtype], arr(pw), ldw, arr(pc), ldc, arr(pm), ldm, arr(pg), ldg,
                             C.byref(o), ws_.data_ptr(), ws_.numel(), stream))
 

@@ -14,10 +14,11 @@
 //           caller scales its matrices into fp16's range; with lo as large as hi, 22 bits are kept down to magnitudes of
 //           2^-13 and what lies below is held to 2^-36. The tensor core truncates when it adds to an
 //           accumulator (about 2e-8 of the sum each time, and always towards zero), so a sum is handed over every
-//           SPLIT_SUM k-blocks and added up in fp32 registers, rounded to nearest.
+//           Op::SUM k-blocks and added up in fp32 registers, rounded to nearest.
 //
 // Warps: 0 loads, 1 allocates tensor memory and (in the leader) issues, the others work on elements: those of a lane quarter share
-// its columns. There are 8 of them in the plain form and 16 in the split one, where small matrices wait for nothing else as long.
+// its columns. There are 16 of them in the split form, where small matrices wait for nothing else as long (256 x 256: 154 -> 144 us
+// per update), and 8 in the plain one, which the power limit binds (with 16 and five stages 8192 x 2048 x 65536 took 6.2 ms for 6.0).
 #pragma once
 
 #include <cuda_fp16.h>
@@ -29,7 +30,6 @@ namespace b2 {
 namespace {
 
 constexpr int TILE_M = 256, TILE_K = 64;
-constexpr int SPLIT_SUM = 16;  // k-blocks per hand-over
 constexpr float LO_UP = 2048.f;  // lo = 2^11 (x - hi)
 constexpr uint32_t ACC_COLS = 256;  // tensor-memory columns of an accumulator stage
 constexpr int TILE_MAX_STAGES = 6;
@@ -74,7 +74,7 @@ struct Tile {
 //     and in the element warps: void begin(const Tile&, int row, int col, int lane) before the sums are there, for the warp's
 //     first row and column; void chunk(const Tile&, int row0, int col0, float (&v)[CHUNK], uint8_t* stage, int lane) for CHUNK columns of
 //     rows row0 + lane; void end(const Tile&, int row, int part) for the thread's row and its warp's part of the columns;
-//     static constexpr bool STORES: it issues TMA stores from `stage`.
+//     static constexpr bool STORES: it issues TMA stores from `stage`; static constexpr int SUM: k-blocks per hand-over (split form).
 template <class Op>
 __global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ TileLayout L,
                                                                const __grid_constant__ typename Op::Params params) {
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(con
       for (int t = pair; t < tiles && ok; t += num_pairs) {
         const int kblocks = op.tile(t).kblocks;
         for (int kb = 0; kb < kblocks; ++kb) {
-          const bool first = kb == 0 || (SPLIT && kb % SPLIT_SUM == 0);
+          const bool first = kb == 0 || (SPLIT && kb % Op::SUM == 0);
           if (first) {
             if (!mbar_wait(&acc_empty_bar[acc], acc_phase ^ 1, abort_flag, &tile_status, 2u)) { ok = false; break; }
             tc_fence_after();
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(con
           }
           tc_commit_pair(empty0 + 8u * stage);
           if (++stage == F::STAGES) { stage = 0; phase ^= 1; }
-          if (kb + 1 == kblocks || (SPLIT && (kb + 1) % SPLIT_SUM == 0)) {
+          if (kb + 1 == kblocks || (SPLIT && (kb + 1) % Op::SUM == 0)) {
             tc_commit_pair(acc_full0 + 8u * acc);
             acc ^= 1;
             if (acc == 0) acc_phase ^= 1;
@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(con
 #pragma unroll
           for (int c = 0; c < F::COLS; ++c) sum[c] = 0.f;
         }
-        for (int kb = 0; kb < tile.kblocks; kb += SPLIT_SUM) {
+        for (int kb = 0; kb < tile.kblocks; kb += Op::SUM) {
           if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_flag, &tile_status, 4u)) { ok = false; break; }
           tc_fence_after();
           const uint32_t from = place + (uint32_t)acc * ACC_COLS;

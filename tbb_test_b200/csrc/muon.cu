@@ -26,6 +26,8 @@ namespace {
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 // powers of two on x (norm at most 1.3), a (1.6) and the middle factor (3.5): below fp16's 65504 with room
 constexpr float X_UP = 8192.f, A_UP = 16384.f, P_UP = 8192.f;
+// k-blocks per hand-over of sums: 16 leaves 3e-6 of x, 8 would halve that and take 3 % longer (8 matrices of 4096 x 4096)
+constexpr int MUON_SUM = 16;
 constexpr int MUON_GROUP = 16;   // matrices per launch at most
 constexpr int NORM_PARTS = 256;  // partial sums of a matrix's squares
 
@@ -166,6 +168,7 @@ template <bool MIDDLE>
 struct SymmetricOp {
   typedef SymmetricParams Params;
   static constexpr bool SPLIT = true, STORES = false;
+  static constexpr int SUM = MUON_SUM;
   const SymmetricParams& p;
   int m_blocks, n_blocks, per;
   __device__ explicit SymmetricOp(const SymmetricParams& q, const TileMaps&) : p(q) {
@@ -235,6 +238,7 @@ template <bool LAST>
 struct NextOp {
   typedef NextParams Params;
   static constexpr bool SPLIT = true, STORES = false;
+  static constexpr int SUM = MUON_SUM;
   const NextParams& p;
   int m_blocks, n_blocks;
   __device__ explicit NextOp(const NextParams& q, const TileMaps&) : p(q) {

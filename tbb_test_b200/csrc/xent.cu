@@ -25,6 +25,8 @@ namespace b2 {
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+// k-blocks per hand-over of the split form's sums: with 16 dw of 1024 rows is 1.1e-6 off (relative), with 8 0.8e-6, in the same time
+constexpr int XENT_SUM = 8;
 constexpr int D_EXP = 14;  // fp32 matrices: d is kept as 2^14 (p - [v = t])
 
 struct Meta {
@@ -182,7 +184,7 @@ struct LogitParams {
 template <bool SPLIT_>
 struct LogitTiles {
   static constexpr bool SPLIT = SPLIT_;
-  static constexpr int BN = TileForm<SPLIT_>::BN, W = TileForm<SPLIT_>::CHUNK;
+  static constexpr int SUM = XENT_SUM, BN = TileForm<SPLIT_>::BN, W = TileForm<SPLIT_>::CHUNK;
   const LogitParams& p;
   int rows, m_blocks, n_blocks, band;
   float unit;  // accumulators times this are logits times log2 e
@@ -366,6 +368,7 @@ struct ProductParams {
   void* dw;
   long long ld_dw;
   int out_bf16, vec;  // vec: rows begin on whole groups of four elements
+  int by_tma;         // rows are whole 16-byte pieces, which is how TMA clips
 };
 
 // How the tiles of dh go over the pairs. There are few of them and their sums are long, so whole tiles alone would leave many
@@ -400,7 +403,7 @@ template <bool SPLIT_>
 struct HiddenOp {
   typedef ProductParams Params;
   static constexpr bool SPLIT = SPLIT_, STORES = false;
-  static constexpr int BN = TileForm<SPLIT_>::BN;
+  static constexpr int SUM = XENT_SUM, BN = TileForm<SPLIT_>::BN;
   const ProductParams& p;
   HiddenSplit split;
   int kblocks;
@@ -470,12 +473,13 @@ struct HiddenOp {
 template <bool SPLIT_>
 struct WeightOp {
   typedef ProductParams Params;
-  static constexpr bool SPLIT = SPLIT_, STORES = false;
-  static constexpr int BN = TileForm<SPLIT_>::BN;
+  static constexpr bool SPLIT = SPLIT_, STORES = !SPLIT_;
+  static constexpr int SUM = XENT_SUM, BN = TileForm<SPLIT_>::BN;
   const ProductParams& p;
+  const CUtensorMap* map;
   int m_blocks, n_blocks, kblocks;
   float unit;
-  __device__ explicit WeightOp(const ProductParams& q, const TileMaps&) : p(q) {
+  __device__ explicit WeightOp(const ProductParams& q, const TileMaps& m) : p(q), map(&m.c) {
     m_blocks = (p.v_count + TILE_M - 1) / TILE_M;
     n_blocks = (p.width + BN - 1) / BN;
     kblocks = max(1, (int)((p.meta->rows + TILE_K - 1) / TILE_K));  // without rows: zeros, as they are stored
@@ -496,6 +500,15 @@ struct WeightOp {
   __device__ __forceinline__ void begin(const Tile&, int, int, int) {}
   static constexpr int W = TileForm<SPLIT_>::CHUNK;
   __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[W], uint8_t* stage, int lane) {
+    if constexpr (!SPLIT_) {
+      if (p.by_tma) {  // pieces are whole 256-row tiles but for the last one, whose rows the map ends with
+        uint32_t w[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+        store_half_words(map, w, col0 >> 5 & 1, p.v_begin + row0, col0 & ~63, stage, lane);
+        return;
+      }
+    }
     by_rows(row0, col0, v, stage, lane, [&](int, int r, int c, const float4& x) {
       if (r >= p.v_count || c >= p.width) return;
       const long long at = (long long)(p.v_begin + r) * p.ld_dw + c;
@@ -706,6 +719,8 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
   pp.out_bf16 = !SPLIT;
   pp.vec = c.ld_dw % 4 == 0 && reinterpret_cast<uintptr_t>(c.dw) % (4 * sizeof(T)) == 0;
   const TileOperand d_k{s.d_hi, s.d_lo, z.rows_up, z.piece, z.piece, false}, d_mn{s.d_hi, s.d_lo, z.piece, z.rows_up, z.piece, true};
+  pp.by_tma = !SPLIT && reinterpret_cast<uintptr_t>(c.dw) % 16 == 0 && c.ld_dw % 8 == 0 && width % 8 == 0;
+  const TileResult dw_out{c.dw, vocab, width, (long long)c.ld_dw};
   const TileResult d_out{s.d_hi, z.rows_up, z.piece, z.piece};
   const long long w_blocks = (width + BN - 1) / BN;
   for (int v0 = 0; v0 < vocab; v0 += (int)z.piece) {
@@ -716,7 +731,7 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
     rc = tile_launch<GradOp<SPLIT>>("b2_xent", h_k, w_k, SPLIT ? nullptr : &d_out, lp, !SPLIT, m_blocks * ((count + BN - 1) / BN), sms, chain);
     if (rc == B2_OK && c.dh) rc = tile_launch<HiddenOp<SPLIT>>("b2_xent", d_k, w_mn, nullptr, pp, !SPLIT, pp.pairs, sms, chain);
     if (rc == B2_OK && c.dw)
-      rc = tile_launch<WeightOp<SPLIT>>("b2_xent", d_mn, h_mn, nullptr, pp, !SPLIT, (count + TILE_M - 1) / TILE_M * w_blocks, sms, chain);
+      rc = tile_launch<WeightOp<SPLIT>>("b2_xent", d_mn, h_mn, pp.by_tma ? &dw_out : nullptr, pp, !SPLIT, (count + TILE_M - 1) / TILE_M * w_blocks, sms, chain);
     if (rc != B2_OK) return rc;
   }
   if (c.dh) {

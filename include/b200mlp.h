@@ -409,8 +409,8 @@ int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dou
  * logits are computed in pieces of the vocabulary, with gradients twice, and never kept. Types: bf16 matrices
  * are multiplied as they are with fp32 sums, the logits' gradients rounded to bf16 once; fp32 matrices, and the
  * logits' gradients between them, at 22 bits of every element down to 2^-27 of the largest (1 for the latter) and to
- * 2^-50 of the largest below that. Equal inputs give equal bits. Limits: rows and vocab at most 2^24,
- * width at most 2^20. Fastest where w begins on a 16-byte boundary and ldw is a multiple of 8 (bf16); otherwise, and in fp32,
+ * 2^-50 of the largest below that. Equal inputs give equal bits. Limits: rows and vocab at most 2^24
+ * each and 2^44 together, width at most 2^20. Fastest where w begins on a 16-byte boundary and ldw is a multiple of 8 (bf16); otherwise, and in fp32,
  * a copy of w goes to the workspace, which is why its size depends on `w` and `ldw`. `grads` is 1 where the call will
  * ask for dh or dw. For 1 / global batch as `scale` the gradients are this rank's share, as everywhere in this library. */
 int b2_xent_workspace(size_t rows, size_t width, size_t vocab, int dtype, int grads, const void* w, size_t ldw,

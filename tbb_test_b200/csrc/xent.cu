@@ -39,12 +39,13 @@ __device__ __forceinline__ float ex2(float x) {  // 2^x, two units in the last p
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Power of two that brings a matrix whose largest magnitude has these bits below 2^15: its exponent. 0 for zeros and
-// for what is not finite.
+// Power of two that brings a matrix whose largest finite magnitude has these bits below 2^15: its exponent, 0 for zeros.
 __device__ __forceinline__ int up_exp(unsigned int max_bits) {
-  const int e = (int)(max_bits >> 23) - 127;
-  if (max_bits == 0 || e == 128) return 0;
-  return min(14 - e, 100);
+  return max_bits == 0 ? 0 : min(14 - ((int)(max_bits >> 23) - 127), 100);
+}
+__device__ __forceinline__ unsigned int finite_bits(unsigned int v) {  // of the magnitude; what is not finite stays so under any scale
+  v &= 0x7FFFFFFFu;
+  return v < 0x7F800000u ? v : 0u;
 }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
@@ -92,7 +93,7 @@ __global__ void __launch_bounds__(LIST_THREADS) list_rows_kernel(const void* __r
 
 __device__ __forceinline__ int row_blocks(unsigned int rows) { return max(1, (int)((rows + TILE_M - 1) / TILE_M)); }
 
-// Largest magnitudes of the listed rows of h (blocks below split_at) and of w.
+// Largest finite magnitudes of the listed rows of h (blocks below split_at) and of w.
 __global__ void __launch_bounds__(256) max_kernel(const float* __restrict__ h, size_t ldh, const int* __restrict__ row_of,
                                                   const float* __restrict__ w, size_t ldw, int vocab, int width,
                                                   int split_at, Meta* meta) {
@@ -113,9 +114,9 @@ __global__ void __launch_bounds__(256) max_kernel(const float* __restrict__ h, s
     const float* row = x + (size_t)(of_h ? __ldg(row_of + r) : r) * ld;
     if (vec) {
       const uint4 v = __ldg(reinterpret_cast<const uint4*>(row) + c);
-      most = max(most, max(max(v.x & 0x7FFFFFFFu, v.y & 0x7FFFFFFFu), max(v.z & 0x7FFFFFFFu, v.w & 0x7FFFFFFFu)));
+      most = max(most, max(max(finite_bits(v.x), finite_bits(v.y)), max(finite_bits(v.z), finite_bits(v.w))));
     } else {
-      most = max(most, __float_as_uint(__ldg(row + c)) & 0x7FFFFFFFu);
+      most = max(most, finite_bits(__float_as_uint(__ldg(row + c))));
     }
   }
   most = __reduce_max_sync(0xFFFFFFFFu, most);
@@ -747,6 +748,7 @@ int check_sizes(const char* who, size_t rows, size_t width, size_t vocab, int dt
   if (rows > (1u << 24)) return call_error(B2_ERR_INVALID, "%s: %zu rows, at most %u", who, rows, 1u << 24);
   if (width < 1 || width > (1u << 20)) return call_error(B2_ERR_INVALID, "%s: width %zu", who, width);
   if (vocab < 1 || vocab > (1u << 24)) return call_error(B2_ERR_INVALID, "%s: vocab %zu", who, vocab);
+  if (rows * vocab > (1ull << 44)) return call_error(B2_ERR_INVALID, "%s: %zu rows x %zu columns of logits, at most 2^44", who, rows, vocab);
   return B2_OK;
 }
 

@@ -132,6 +132,25 @@ def test_on_another_stream_and_without_tokens(lm):
 
 
 @pytest.mark.gpu
+def test_in_a_graph(lm):
+    table = _rows(500, 64, "bf16", 1)
+    t = _tokens(20000, 500, "zipf", 1)
+    y = lm.embed(t, table)
+    want = lm.embed_grad(t, y, 500)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = lm.embed(t, table)
+        got = lm.embed_grad(t, out, 500)
+    out.zero_()
+    got.zero_()
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, y) and torch.equal(got, want)
+
+
+@pytest.mark.gpu
 def test_wrapper_refuses(lm):
     table = torch.zeros(8, 16, device="cuda")
     t = torch.zeros(4, dtype=torch.int64, device="cuda")

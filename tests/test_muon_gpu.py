@@ -97,6 +97,32 @@ def test_steps_and_low_rank(lm, steps):
 
 
 @pytest.mark.gpu
+def test_even_steps_and_an_update_after_an_update(lm):
+    """The buffers end on the other side, and a second call begins from what the first left."""
+    w, m, g = _make(2, 333, 200, torch.bfloat16)
+    for steps in (2, 4):
+        before = (w.clone(), m.clone(), g)
+        lm.muon(w, m, g, steps=steps, **OPTIONS)
+        _check(before, (w, m, None), dict(OPTIONS, nesterov=True, steps=steps))
+
+
+@pytest.mark.gpu
+def test_in_a_graph(lm):
+    w, m, g = _make(2, 200, 130, torch.float32)
+    w1, m1 = w.clone(), m.clone()
+    for _ in range(2):
+        lm.muon(w1, m1, g, **OPTIONS)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lm.muon(w, m, g, **OPTIONS)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(w, w1) and torch.equal(m, m1)
+
+
+@pytest.mark.gpu
 def test_singular_values_come_near_one(lm):
     g = torch.Generator(device="cuda").manual_seed(3)
     u, v = (torch.linalg.qr(torch.randn(n, 200, device="cuda", generator=g).double())[0] for n in (300, 200))

@@ -142,6 +142,20 @@ def test_large_and_infinite_logits(lm, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("size", [1.0, 1e20])
+def test_infinity_stays_in_its_row_fp32(lm, size):
+    """One infinite element of h must not set the scale that the other rows are split with."""
+    h, w, t = _case(50, 40, 300, "fp32", padding=0.0)
+    h, w = h * size, w / size
+    clean = lm.xent(h, w, t)
+    h[7, 3] = float("inf")
+    loss, dh, _ = lm.xent(h, w, t)
+    rest = torch.arange(50, device="cuda") != 7
+    assert bool(torch.isnan(loss[7])) and torch.equal(loss[rest], clean[0][rest])
+    assert torch.equal(dh[rest], clean[1][rest])
+
+
+@pytest.mark.gpu
 def test_small_and_large_magnitudes_fp32(lm):
     """The split of fp32 matrices follows their largest element."""
     for a, b in ((1e-20, 1e20), (1e15, 1e-15), (1e-30, 1.0)):
@@ -227,7 +241,7 @@ def test_c_entry_refuses_before_any_device_work(native):
     def xent(**kw):
         return lib.b2_xent(*{**good, **kw}.values())
 
-    for kw in (dict(rows=(1 << 24) + 1), dict(width=0), dict(width=(1 << 20) + 1), dict(vocab=0), dict(vocab=1 << 25), dict(dtype=3),
+    for kw in (dict(rows=(1 << 24) + 1), dict(width=0), dict(width=(1 << 20) + 1), dict(vocab=0), dict(vocab=1 << 25), dict(rows=1 << 23, vocab=1 << 22), dict(dtype=3),
                dict(h=None), dict(w=None), dict(t=None), dict(loss=None), dict(ws=None), dict(ldh=7), dict(ldw=7), dict(lddh=7),
                dict(lddw=7), dict(size=1), dict(ws=C.c_void_p(128)), dict(ws_bytes=100), dict(h=C.c_void_p(258)),
                dict(t=C.c_void_p(260)), dict(dw=C.c_void_p(257))):

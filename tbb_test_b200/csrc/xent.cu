@@ -1,7 +1,7 @@
 // Softmax cross entropy behind a linear layer as wide as a vocabulary, with its gradients, without keeping the logits:
 //
-//   x_iv = h_i . w_v      l_i = log sum_v exp(x_iv) - x_i,t_i      d_iv = scale (exp(x_iv) / sum_u exp(x_iu) - [v = t_i])
-//   dh_i = sum_v d_iv w_v      dw_v = sum_i d_iv h_i
+//   x_iv = h_i . w_v      l_i = log sum_v exp(x_iv) - x_i,t_i      d_iv = exp(x_iv) / sum_u exp(x_iu) - [v = t_i]
+//   dh_i = scale sum_v d_iv w_v      dw_v = scale sum_i d_iv h_i
 //
 // Work: 2 R V F operations for the losses and 6 R V F with gradients; 8 R V F in this form, because the logits are
 // computed a second time when their row's maximum and sum are known, instead of R x V of them being kept.
@@ -13,8 +13,8 @@
 //   3. The lists give each row's maximum and sum, and the loss.
 //   4. Per piece of the vocabulary: logits again, d to a buffer of R x piece; dh += d w; dw of the piece = d' h.
 //
-// Precision: bf16 matrices are multiplied as they are, with fp32 sums; d is rounded to bf16 once, which is a
-// relative 2^-9 at most of each product of the gradients, as much as the gradients' own rounding. fp32 matrices are
+// Precision: bf16 matrices are multiplied as they are, with fp32 sums; d is rounded to bf16 once, as the
+// gradients are in the end. fp32 matrices are
 // split into fp16 pairs behind a power of two that brings the largest element to 2^14: 22 bits of an element down to 2^-27 of
 // the largest, and nothing finer than 2^-50 of it; d the same, with 1 for the largest. Maxima, sums and the losses are fp32.
 #include <type_traits>
@@ -179,7 +179,6 @@ struct LogitParams {
   const float2* row_stat;  // maximum and 1 / sum of whole rows
   uint16_t *d_hi, *d_lo;
   long long ld_d;
-  float scale;
 };
 
 template <bool SPLIT_>
@@ -272,7 +271,7 @@ struct GradOp : LogitTiles<SPLIT_> {
   int target;
   bool in;
   __device__ explicit GradOp(const LogitParams& q, const TileMaps& m) : LogitTiles<SPLIT_>(q, m), map(&m.c) {
-    to = SPLIT_ ? (float)(1 << D_EXP) : p.scale;
+    to = SPLIT_ ? (float)(1 << D_EXP) : 1.f;  // the caller's scale comes behind the products: -1 at an unlikely target is exact
   }
   __device__ __forceinline__ void begin(const Tile&, int row0, int, int lane) {
     const int row = row0 + lane;
@@ -413,7 +412,7 @@ struct HiddenOp {
   long long ld;
   __device__ explicit HiddenOp(const ProductParams& q, const TileMaps&) : p(q), split(q, q.meta->rows, BN) {
     kblocks = (p.v_count + TILE_K - 1) / TILE_K;
-    unit = SPLIT ? p.scale * pow2(-D_EXP) * pow2(-up_exp(p.meta->max_w)) : 1.f;
+    unit = SPLIT ? p.scale * pow2(-D_EXP) * pow2(-up_exp(p.meta->max_w)) : p.scale;
   }
   __device__ int tiles() const { return split.whole + 2 * p.pairs; }
   __device__ Tile tile(int t) const {
@@ -484,7 +483,7 @@ struct WeightOp {
     m_blocks = (p.v_count + TILE_M - 1) / TILE_M;
     n_blocks = (p.width + BN - 1) / BN;
     kblocks = max(1, (int)((p.meta->rows + TILE_K - 1) / TILE_K));  // without rows: zeros, as they are stored
-    unit = SPLIT ? p.scale * pow2(-D_EXP) * pow2(-up_exp(p.meta->max_h)) : 1.f;
+    unit = SPLIT ? p.scale * pow2(-D_EXP) * pow2(-up_exp(p.meta->max_h)) : p.scale;
   }
   __device__ int tiles() const { return m_blocks * n_blocks; }
   __device__ Tile tile(int t) const {
@@ -505,7 +504,7 @@ struct WeightOp {
       if (p.by_tma) {  // pieces are whole 256-row tiles but for the last one, whose rows the map ends with
         uint32_t w[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+        for (int j = 0; j < 16; ++j) w[j] = pack_bf16(v[2 * j] * unit, v[2 * j + 1] * unit);
         store_half_words(map, w, col0 >> 5 & 1, p.v_begin + row0, col0 & ~63, stage, lane);
         return;
       }
@@ -698,7 +697,6 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
   lp.d_hi = s.d_hi;
   lp.d_lo = s.d_lo;
   lp.ld_d = z.piece;
-  lp.scale = c.scale;
   rc = tile_launch<StatOp<SPLIT>>("b2_xent", h_k, w_k, nullptr, lp, !SPLIT, m_blocks * ((vocab + BN - 1) / BN), sms, chain);
   if (rc != B2_OK) return rc;
   chain.launch(join_rows_kernel, dim3((rows + 31) / 32), 256, 0, 0, s.parts, z.rows_up, (int)z.parts, s.meta, s.target_logit, s.row_of, s.row_stat,

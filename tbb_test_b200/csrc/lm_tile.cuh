@@ -70,11 +70,26 @@ struct Tile {
   int z;        // the operator's own
 };
 
+// Adds 16 finished columns of this lane's row to `sum`.
+__device__ __forceinline__ void tile_add16(uint32_t from, float* sum) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(from)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < 16; ++j) sum[j] += __uint_as_float(r[j]);
+}
+
 // Op: struct Params; static constexpr bool SPLIT; Op(const Params&, const TileMaps&); int tiles(); Tile tile(int t);
 //     and in the element warps: void begin(const Tile&, int row, int col, int lane) before the sums are there, for the warp's
 //     first row and column; void chunk(const Tile&, int row0, int col0, float (&v)[CHUNK], uint8_t* stage, int lane) for CHUNK columns of
 //     rows row0 + lane; void end(const Tile&, int row, int part) for the thread's row and its warp's part of the columns;
-//     static constexpr bool STORES: it issues TMA stores from `stage`; static constexpr int SUM: k-blocks per hand-over (split form).
+//     static constexpr bool STORES: it issues TMA stores from `stage`; static constexpr bool LONG: sums are handed over every SUM
+//     (static constexpr int) k-blocks, which the split form always does; chunks have 16 columns then.
 template <class Op>
 __global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ TileLayout L,
                                                                const __grid_constant__ typename Op::Params params) {
@@ -165,7 +180,7 @@ __global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(con
       for (int t = pair; t < tiles && ok; t += num_pairs) {
         const int kblocks = op.tile(t).kblocks;
         for (int kb = 0; kb < kblocks; ++kb) {
-          const bool first = kb == 0 || (SPLIT && kb % Op::SUM == 0);
+          const bool first = kb == 0 || (Op::LONG && kb % Op::SUM == 0);
           if (first) {
             if (!mbar_wait(&acc_empty_bar[acc], acc_phase ^ 1, abort_flag, &tile_status, 2u)) { ok = false; break; }
             tc_fence_after();
@@ -186,7 +201,7 @@ __global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(con
           }
           tc_commit_pair(empty0 + 8u * stage);
           if (++stage == F::STAGES) { stage = 0; phase ^= 1; }
-          if (kb + 1 == kblocks || (SPLIT && (kb + 1) % Op::SUM == 0)) {
+          if (kb + 1 == kblocks || (Op::LONG && (kb + 1) % Op::SUM == 0)) {
             tc_commit_pair(acc_full0 + 8u * acc);
             acc ^= 1;
             if (acc == 0) acc_phase ^= 1;
@@ -238,6 +253,41 @@ __global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(con
           for (int j = 0; j < CHUNK; ++j) v[j] = sum[c + j];
           op.chunk(tile, row0, col0 + c, v, stage, lane);
         }
+        op.end(tile, row0 + lane, part);
+      } else if constexpr (Op::LONG) {
+        // sums of SUM k-blocks at a time are added up in registers; the last ones go straight on, 16 columns at a time
+        float sum[F::COLS];
+#pragma unroll
+        for (int c = 0; c < F::COLS; ++c) sum[c] = 0.f;
+        for (int kb = 0; kb < tile.kblocks; kb += Op::SUM) {
+          if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_flag, &tile_status, 4u)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t from = place + (uint32_t)acc * ACC_COLS;
+          if (kb + Op::SUM < tile.kblocks) {
+#pragma unroll
+            for (int c = 0; c < F::COLS; c += 16) tile_add16(from + c, sum + c);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_leader(map_to_cta(smem_u32(&acc_empty_bar[acc]), 0));
+          } else {
+#pragma unroll
+            for (int c = 0; c < F::COLS; c += 16) {
+              tile_add16(from + c, sum + c);
+              if (c + 16 == F::COLS) {  // all read: the next tile may be summed here
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_leader(map_to_cta(smem_u32(&acc_empty_bar[acc]), 0));
+              }
+              float v[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[j] = sum[c + j];
+              op.chunk(tile, row0, col0 + c, v, stage, lane);
+            }
+          }
+          acc ^= 1;
+          if (acc == 0) acc_phase ^= 1;
+        }
+        if (!ok) break;
         op.end(tile, row0 + lane, part);
       } else {
         const bool summed = tile.kblocks > 0;

@@ -167,7 +167,7 @@ struct SymmetricParams {
 template <bool MIDDLE>
 struct SymmetricOp {
   typedef SymmetricParams Params;
-  static constexpr bool SPLIT = true, STORES = false;
+  static constexpr bool SPLIT = true, STORES = false, LONG = true;
   static constexpr int SUM = MUON_SUM;
   const SymmetricParams& p;
   int m_blocks, n_blocks, per;
@@ -237,7 +237,7 @@ struct NextParams {
 template <bool LAST>
 struct NextOp {
   typedef NextParams Params;
-  static constexpr bool SPLIT = true, STORES = false;
+  static constexpr bool SPLIT = true, STORES = false, LONG = true;
   static constexpr int SUM = MUON_SUM;
   const NextParams& p;
   int m_blocks, n_blocks;

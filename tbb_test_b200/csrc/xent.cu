@@ -212,10 +212,14 @@ struct LogitTiles {
   }
 };
 
-// Maximum and sum of exponentials of a row over the columns of one warp, and the target's logit.
-template <bool SPLIT_>
+// Maximum and sum of exponentials of a row over the columns of one warp, and the target's logit. LONG: for more than 16 k-blocks,
+// whose sums the tensor core would leave too small (bf16, width 2048: losses 1.0e-6 off, with sums of 16 added in fp32 0.5e-6, in the
+// same time).
+template <bool SPLIT_, bool LONG_>
 struct StatOp : LogitTiles<SPLIT_> {
   typedef LogitParams Params;
+  static constexpr bool LONG = SPLIT_ || LONG_;
+  static constexpr int SUM = SPLIT_ ? XENT_SUM : 16;
   static constexpr bool STORES = false;
   using LogitTiles<SPLIT_>::p;
   float top, sum;
@@ -226,7 +230,7 @@ struct StatOp : LogitTiles<SPLIT_> {
     sum = 0.f;
     target = row0 + lane < this->rows ? __ldg(p.target + row0 + lane) : -1;
   }
-  static constexpr int W = LogitTiles<SPLIT_>::W;
+  static constexpr int W = LONG ? 16 : LogitTiles<SPLIT_>::W;
   __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[W], uint8_t*, int lane) {
     if (col0 >= p.vocab) return;
     if (col0 + W > p.vocab) {
@@ -264,6 +268,7 @@ struct StatOp : LogitTiles<SPLIT_> {
 template <bool SPLIT_>
 struct GradOp : LogitTiles<SPLIT_> {
   typedef LogitParams Params;
+  static constexpr bool LONG = SPLIT_;
   static constexpr bool STORES = !SPLIT_;
   using LogitTiles<SPLIT_>::p;
   const CUtensorMap* map;
@@ -403,6 +408,7 @@ template <bool SPLIT_>
 struct HiddenOp {
   typedef ProductParams Params;
   static constexpr bool SPLIT = SPLIT_, STORES = false;
+  static constexpr bool LONG = SPLIT_;
   static constexpr int SUM = XENT_SUM, BN = TileForm<SPLIT_>::BN;
   const ProductParams& p;
   HiddenSplit split;
@@ -474,6 +480,7 @@ template <bool SPLIT_>
 struct WeightOp {
   typedef ProductParams Params;
   static constexpr bool SPLIT = SPLIT_, STORES = !SPLIT_;
+  static constexpr bool LONG = SPLIT_;
   static constexpr int SUM = XENT_SUM, BN = TileForm<SPLIT_>::BN;
   const ProductParams& p;
   const CUtensorMap* map;
@@ -697,7 +704,10 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
   lp.d_hi = s.d_hi;
   lp.d_lo = s.d_lo;
   lp.ld_d = z.piece;
-  rc = tile_launch<StatOp<SPLIT>>("b2_xent", h_k, w_k, nullptr, lp, !SPLIT, m_blocks * ((vocab + BN - 1) / BN), sms, chain);
+  const long long stat_tiles = m_blocks * ((vocab + BN - 1) / BN);
+  rc = !SPLIT && lp.kblocks > StatOp<false, true>::SUM
+           ? tile_launch<StatOp<SPLIT, !SPLIT>>("b2_xent", h_k, w_k, nullptr, lp, !SPLIT, stat_tiles, sms, chain)
+           : tile_launch<StatOp<SPLIT, false>>("b2_xent", h_k, w_k, nullptr, lp, !SPLIT, stat_tiles, sms, chain);
   if (rc != B2_OK) return rc;
   chain.launch(join_rows_kernel, dim3((rows + 31) / 32), 256, 0, 0, s.parts, z.rows_up, (int)z.parts, s.meta, s.target_logit, s.row_of, s.row_stat,
                c.row_loss);

@@ -99,6 +99,52 @@ constexpr int RADIX_THREADS = 512, RADIX_WARPS = RADIX_THREADS / 32;
 constexpr int RADIX_TILES = 64, RADIX_MOST_BITS = 10;
 constexpr int radix_rounds(size_t n) { return n <= (1u << 18) ? 2 : 8; }
 
+// First index whose key is >= `key`.
+__device__ __forceinline__ unsigned int lower_bound(const unsigned int* keys, unsigned int n, unsigned int key) {
+  unsigned int lo = 0, hi = n;
+  while (lo < hi) {
+    const unsigned int mid = (lo + hi) >> 1;
+    if (__ldg(keys + mid) < key) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Rows of the gradient whose token does not occur: zeros. A warp takes FILL_ROWS of them.
+constexpr int FILL_ROWS = 8;
+struct Fill {
+  const unsigned char* present;  // by token, or null: looked up in the sorted keys
+  const unsigned int* keys;
+  unsigned int n, vocab;
+  char* dtable;
+  size_t ld;  // bytes
+  int vb, vecs;
+};
+__device__ __forceinline__ void fill_rows(const Fill& p, unsigned int warp, int lane) {
+  const unsigned int v0 = warp * FILL_ROWS, v = v0 + lane;
+  bool absent = false;
+  if (lane < FILL_ROWS && v < p.vocab) {
+    if (p.present) {
+      absent = !p.present[v];
+    } else {
+      const unsigned int at = lower_bound(p.keys, p.n, v);
+      absent = at == p.n || __ldg(p.keys + at) != v;
+    }
+  }
+  for (unsigned int rows = __ballot_sync(0xFFFFFFFFu, absent); rows; rows &= rows - 1) {
+    char* row = p.dtable + (size_t)(v0 + __ffs(rows) - 1) * p.ld;
+    if (p.vb == 16) {
+      for (int c = lane; c < p.vecs; c += 32) reinterpret_cast<uint4*>(row)[c] = make_uint4(0, 0, 0, 0);
+    } else if (p.vb == 8) {
+      for (int c = lane; c < p.vecs; c += 32) reinterpret_cast<uint2*>(row)[c] = make_uint2(0, 0);
+    } else if (p.vb == 4) {
+      for (int c = lane; c < p.vecs; c += 32) reinterpret_cast<unsigned int*>(row)[c] = 0;
+    } else {
+      for (int c = lane; c < p.vecs; c += 32) reinterpret_cast<unsigned short*>(row)[c] = 0;
+    }
+  }
+}
+
 struct RadixPass {
   const void* tokens;  // first pass: keys come from here and positions are their index
   int wide;
@@ -134,8 +180,9 @@ __global__ void __launch_bounds__(RADIX_THREADS) radix_count_kernel(const RadixP
   for (int b = threadIdx.x; b < bins; b += RADIX_THREADS) p.counts[(size_t)blockIdx.x * bins + b] = count[b];
 }
 
+// Blocks behind the tiles' zero rows meanwhile (last pass; the sort keeps 64 SMs busy at most).
 template <int RADIX_ROUNDS>
-__global__ void __launch_bounds__(RADIX_THREADS) radix_place_kernel(const RadixPass p) {
+__global__ void __launch_bounds__(RADIX_THREADS) radix_place_kernel(const RadixPass p, const Fill fill) {
   constexpr int RADIX_STEP = RADIX_THREADS * RADIX_ROUNDS;
   __shared__ unsigned int next[1 << RADIX_MOST_BITS];  // where this tile's next element of a digit goes
   __shared__ unsigned short seen[RADIX_WARPS][1 << RADIX_MOST_BITS];
@@ -143,6 +190,10 @@ __global__ void __launch_bounds__(RADIX_THREADS) radix_place_kernel(const RadixP
   const int bins = 1 << p.bits, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   after_previous();
   let_next_start();
+  if (blockIdx.x >= p.tiles) {
+    fill_rows(fill, (blockIdx.x - p.tiles) * RADIX_WARPS + warp, lane);
+    return;
+  }
   // exclusive sum over digits of all tiles' counts, plus the counts of the tiles before this one
   unsigned int running = 0;
   for (int b0 = 0; b0 < bins; b0 += RADIX_THREADS) {
@@ -247,20 +298,8 @@ struct RunSum {
   uint2* join_runs;     // their chunks and tokens, in any order
   float scale;
   int vecs, slices, tpr_log2;
-  const unsigned char* present;  // by token, or null: looked up in the sorted list
-  unsigned int fill_blocks;      // of the second kernel
+  unsigned int fill_blocks;  // of the second kernel
 };
-
-// First index whose key is >= `key`.
-__device__ __forceinline__ unsigned int lower_bound(const unsigned int* keys, unsigned int n, unsigned int key) {
-  unsigned int lo = 0, hi = n;
-  while (lo < hi) {
-    const unsigned int mid = (lo + hi) >> 1;
-    if (__ldg(keys + mid) < key) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
-}
 
 constexpr int RUN_THREADS = 128, RUN_AHEAD = 8;
 template <typename T, int VB>
@@ -334,36 +373,122 @@ __global__ void __launch_bounds__(RUN_THREADS) run_sum_kernel(const RunSum p) {
   if (cur < p.vocab) finish(end < p.n && __ldg(p.keys + end) == cur);
 }
 
+// The same for rows of 32 and more 16-byte pieces, which go through shared memory: a thread copies its own piece of the next 16 rows
+// there without holding registers for them and refills a place when it has added it; seven blocks keep up to 220 KB in flight per SM.
+// Where runs begin comes as a mask per 32 elements, so that a row takes about 25 instructions per warp and not 74, which is
+// what bounded this kernel (65536 rows of 2 KB: 50 us and DRAM 43 % busy with eight rows ahead in registers, 39 us
+// this way, while 92 MB of zero rows go from L2 to DRAM).
+constexpr int SPAN = 32, RING = 16, RING_GROUP = 4, RING_GROUPS = RING / RING_GROUP;
+template <typename T>
+__global__ void __launch_bounds__(RUN_THREADS) run_sum_ring_kernel(const RunSum p) {
+  typedef Elems<T, 16> E;
+  extern __shared__ uint4 ring_s[];  // place k of this thread at k * RUN_THREADS
+  uint4* ring = ring_s + threadIdx.x;
+  const int lane = threadIdx.x & 31, tpr = 1 << p.tpr_log2;  // 32 and more: a warp is of one unit
+  after_previous();
+  let_next_start();
+  const unsigned int unit = blockIdx.x * (RUN_THREADS >> p.tpr_log2) + (threadIdx.x >> p.tpr_log2);
+  const unsigned int chunk = unit / p.slices;
+  const int col = (int)(unit - chunk * p.slices) * tpr + (threadIdx.x & (tpr - 1));
+  if (chunk >= p.chunks) return;
+  const unsigned int begin = chunk * p.chunk, end = min(p.n, begin + p.chunk);
+  const bool works = col < p.vecs;
+  const char* from = p.dout + (size_t)col * 16;
+  unsigned int cur = __ldg(p.keys + begin);
+  bool from_before = begin > 0 && __ldg(p.keys + begin - 1) == cur;
+  float acc[E::N];
+#pragma unroll
+  for (int j = 0; j < E::N; ++j) acc[j] = 0.f;
+  auto finish = [&](bool goes_on) {
+    if (!works) return;
+    if (from_before || goes_on) {
+      float4* to = reinterpret_cast<float4*>((from_before ? p.head : p.tail) + (size_t)chunk * p.pitch + (size_t)col * E::N);
+#pragma unroll
+      for (int j = 0; j < E::N / 4; ++j) to[j] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+      if (goes_on && !from_before && col == 0) p.join_runs[atomicAdd(p.joins, 1u)] = make_uint2(chunk, cur);
+    } else {
+#pragma unroll
+      for (int j = 0; j < E::N; ++j) acc[j] *= p.scale;
+      reinterpret_cast<uint4*>(p.dtable + (size_t)cur * p.ld_dtable)[col] = E::put(acc);
+    }
+  };
+  // Keys and positions of 32 elements, one per lane; behind the last element key = vocab. Three spans of them: the one that is added,
+  // the one whose rows are copied meanwhile, and the one whose keys are on their way.
+  unsigned int key[3], pos[3];
+  auto fetch = [&](unsigned int i, unsigned int& k, unsigned int& at) {
+    k = i < end ? __ldg(p.keys + i) : p.vocab;
+    at = i < end ? __ldg(p.pos + i) : 0u;
+  };
+  auto count = [&](unsigned int k) { return __popc(__ballot_sync(0xFFFFFFFFu, k < p.vocab)); };  // they stand first
+  auto copy_group = [&](int g, unsigned int at, int have) {  // group g of a span
+#pragma unroll
+    for (int u = 0; u < RING_GROUP; ++u) {
+      const int e = g * RING_GROUP + u;
+      const unsigned int row = __shfl_sync(0xFFFFFFFFu, at, e);
+      if (works && e < have)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned int)__cvta_generic_to_shared(ring + e % RING * RUN_THREADS)),
+                     "l"(from + (size_t)row * p.ld_dout)
+                     : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  fetch(begin + lane, key[0], pos[0]);
+  fetch(begin + SPAN + lane, key[1], pos[1]);
+  int have = count(key[0]);
+#pragma unroll
+  for (int g = 0; g < RING_GROUPS; ++g) copy_group(g, pos[0], have);
+  unsigned int before = cur;  // the key in front of the span
+  for (unsigned int i = begin; i < end && have > 0; i += SPAN) {
+    fetch(i + 2 * SPAN + lane, key[2], pos[2]);
+    // bit e: a run begins at element e of the span
+    const unsigned int up = __shfl_up_sync(0xFFFFFFFFu, key[0], 1);
+    const unsigned int starts = __ballot_sync(0xFFFFFFFFu, key[0] != (lane ? up : before));
+    before = __shfl_sync(0xFFFFFFFFu, key[0], 31);
+    const int next_have = count(key[1]);
+#pragma unroll 1
+    for (int g = 0; g < SPAN / RING_GROUP; ++g) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(RING_GROUPS - 1) : "memory");
+#pragma unroll
+      for (int u = 0; u < RING_GROUP; ++u) {
+        const int e = g * RING_GROUP + u;
+        if (e >= have) break;
+        if (starts >> e & 1) {
+          finish(false);
+          cur = __shfl_sync(0xFFFFFFFFu, key[0], e);
+          from_before = false;
+#pragma unroll
+          for (int j = 0; j < E::N; ++j) acc[j] = 0.f;
+        }
+        float f[E::N];
+        E::get(ring[e % RING * RUN_THREADS], f);
+#pragma unroll
+        for (int j = 0; j < E::N; ++j) acc[j] += f[j];
+      }
+      const bool same = g + RING_GROUPS < SPAN / RING_GROUP;  // the group that takes the places just read
+      copy_group((g + RING_GROUPS) % (SPAN / RING_GROUP), same ? pos[0] : pos[1], same ? have : next_have);
+    }
+    have = next_have;
+    key[0] = key[1];
+    pos[0] = pos[1];
+    key[1] = key[2];
+    pos[1] = pos[2];
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (cur < p.vocab) finish(end < p.n && __ldg(p.keys + end) == cur);
+}
+
 // Runs that cross chunk borders: the tail of the chunk a run begins in and the heads of the chunks behind it, JOIN_PARTS
-// contiguous shares of them side by side, which are then added in order. A block takes 128 columns of a run at a time. The blocks
-// before these zero the rows of tokens that do not occur, which needs no sums and so does not wait for the kernel before: that
-// one has waited for the sorted list before this one starts.
+// contiguous shares of them side by side, which are then added in order. A block takes 128 columns of a run at a time. Short
+// lists, whose sort has no room for it, leave zeroing rows to the blocks before these; it needs no sums, so these blocks do not
+// wait for the kernel before, which has waited for the sorted list before this one starts.
 constexpr int JOIN_PARTS = 4, JOIN_THREADS = 32 * JOIN_PARTS;
-constexpr int FILL_ROWS = 8;  // rows that a warp looks up and zeroes
-template <typename T, int VB>
-__global__ void __launch_bounds__(JOIN_THREADS) run_join_kernel(const RunSum p, int width) {
+template <typename T>
+__global__ void __launch_bounds__(JOIN_THREADS) run_join_kernel(const RunSum p, const Fill fill, int width) {
   __shared__ float4 part[JOIN_PARTS][32];
   const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
   let_next_start();
   if (blockIdx.x < p.fill_blocks) {
-    typedef typename Raw<VB>::type raw;
-    const unsigned int v0 = (blockIdx.x * JOIN_PARTS + share) * FILL_ROWS, v = v0 + lane;
-    bool absent = false;
-    if (lane < FILL_ROWS && v < p.vocab) {
-      if (p.present) {
-        absent = !p.present[v];
-      } else {
-        const unsigned int at = lower_bound(p.keys, p.n, v);
-        absent = at == p.n || __ldg(p.keys + at) != v;
-      }
-    }
-    unsigned int rows = __ballot_sync(0xFFFFFFFFu, absent);
-    raw zero;
-    memset(&zero, 0, sizeof zero);
-    for (; rows; rows &= rows - 1) {
-      raw* row = reinterpret_cast<raw*>(p.dtable + (size_t)(v0 + __ffs(rows) - 1) * p.ld_dtable);
-      for (int c = lane; c < p.vecs; c += 32) row[c] = zero;
-    }
+    fill_rows(fill, blockIdx.x * JOIN_PARTS + share, lane);
     return;
   }
   after_previous();
@@ -487,19 +612,27 @@ cudaError_t embed_launch(const void* tokens, int wide, size_t n, const void* tab
 }
 
 template <typename T, int VB>
-void run_launch(RunSum p, size_t width, Chain& chain) {
+void run_launch(RunSum p, const Fill& fill, bool filled, size_t width, Chain& chain) {
   p.vecs = (int)(width * sizeof(T) / VB);
   p.tpr_log2 = log2_ceil(p.vecs);
   if (p.tpr_log2 > 7) p.tpr_log2 = 7;
   if (p.tpr_log2 < 3) p.tpr_log2 = 3;
   p.slices = (p.vecs + (1 << p.tpr_log2) - 1) >> p.tpr_log2;
   const size_t units = (size_t)p.chunks * p.slices, per_block = RUN_THREADS >> p.tpr_log2;
-  chain.launch(run_sum_kernel<T, VB>, dim3((unsigned int)((units + per_block - 1) / per_block)), RUN_THREADS, 0, 0, p);
+  const dim3 grid((unsigned int)((units + per_block - 1) / per_block));
+  if (VB == 16 && p.tpr_log2 >= 5) {
+    const size_t smem = (size_t)RING * RUN_THREADS * 16;
+    if (chain.err == cudaSuccess)
+      chain.err = cudaFuncSetAttribute(run_sum_ring_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    chain.launch(run_sum_ring_kernel<T>, grid, RUN_THREADS, smem, 0, p);
+  } else {
+    chain.launch(run_sum_kernel<T, VB>, grid, RUN_THREADS, 0, 0, p);
+  }
   const size_t most = (size_t)(p.chunks - 1) * ((width + 127) / 128);
   const unsigned int per_fill = JOIN_PARTS * FILL_ROWS;
-  p.fill_blocks = (p.vocab + per_fill - 1) / per_fill;
+  p.fill_blocks = filled ? 0 : (p.vocab + per_fill - 1) / per_fill;
   const unsigned int join_blocks = (unsigned int)(most < 148 * 16 ? most : 148 * 16);
-  chain.launch(run_join_kernel<T, VB>, dim3(p.fill_blocks + join_blocks), JOIN_THREADS, 0, 0, p, (int)width);
+  if (p.fill_blocks + join_blocks) chain.launch(run_join_kernel<T>, dim3(p.fill_blocks + join_blocks), JOIN_THREADS, 0, 0, p, fill, (int)width);
 }
 
 }  // namespace
@@ -569,6 +702,8 @@ int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dou
     return launch_error(cudaMemset2DAsync(dtable, ld_dtable * e, 0, width * e, vocab, s), "b2_embed_grad");
   const int wide = token_bytes == 8;
   Chain chain(s);
+  const int vb = vector_bytes(e, reinterpret_cast<size_t>(dout) | reinterpret_cast<size_t>(dtable) | width * e | ld_dout * e | ld_dtable * e);
+  Fill fill{g.passes ? w.present : nullptr, nullptr, (unsigned int)n, (unsigned int)vocab, static_cast<char*>(dtable), ld_dtable * e, vb, (int)(width * e / vb)};
   int sorted = 0;
   if (g.passes == 0) {
     const int per_block = RANK_THREADS / 32 * RANK_PER_WARP;
@@ -597,8 +732,11 @@ int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dou
       if (i == 0)
         chain.launch(radix_count_kernel, dim3(g.tiles), RADIX_THREADS, 0, 0, p, p.counts + bins, (int)((g.passes - 1) * bins), w.present,
                      w.joins);
-      if (radix_rounds(n) == 2) chain.launch(radix_place_kernel<2>, dim3(g.tiles), RADIX_THREADS, 0, 0, p);
-      else chain.launch(radix_place_kernel<8>, dim3(g.tiles), RADIX_THREADS, 0, 0, p);
+      // the first pass marks the tokens that occur, so that the last of several can zero the other rows
+      const unsigned int per_fill = RADIX_WARPS * FILL_ROWS;
+      const dim3 grid(g.tiles + (i > 0 && i + 1 == g.passes ? (unsigned int)((vocab + per_fill - 1) / per_fill) : 0));
+      if (radix_rounds(n) == 2) chain.launch(radix_place_kernel<2>, grid, RADIX_THREADS, 0, 0, p, fill);
+      else chain.launch(radix_place_kernel<8>, grid, RADIX_THREADS, 0, 0, p, fill);
     }
   }
   RunSum r{};
@@ -617,18 +755,18 @@ int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dou
   r.pitch = g.pitch;
   r.joins = w.joins;
   r.join_runs = w.join_runs;
-  r.present = g.passes ? w.present : nullptr;
+  fill.keys = r.keys;
+  const bool filled = g.passes > 1;
   r.scale = scale;
-  const int vb = vector_bytes(e, reinterpret_cast<size_t>(dout) | reinterpret_cast<size_t>(dtable) | width * e | r.ld_dout | r.ld_dtable);
   if (dtype == B2_DTYPE_BF16) {
-    if (vb == 16) run_launch<__nv_bfloat16, 16>(r, width, chain);
-    else if (vb == 8) run_launch<__nv_bfloat16, 8>(r, width, chain);
-    else if (vb == 4) run_launch<__nv_bfloat16, 4>(r, width, chain);
-    else run_launch<__nv_bfloat16, 2>(r, width, chain);
+    if (vb == 16) run_launch<__nv_bfloat16, 16>(r, fill, filled, width, chain);
+    else if (vb == 8) run_launch<__nv_bfloat16, 8>(r, fill, filled, width, chain);
+    else if (vb == 4) run_launch<__nv_bfloat16, 4>(r, fill, filled, width, chain);
+    else run_launch<__nv_bfloat16, 2>(r, fill, filled, width, chain);
   } else {
-    if (vb == 16) run_launch<float, 16>(r, width, chain);
-    else if (vb == 8) run_launch<float, 8>(r, width, chain);
-    else run_launch<float, 4>(r, width, chain);
+    if (vb == 16) run_launch<float, 16>(r, fill, filled, width, chain);
+    else if (vb == 8) run_launch<float, 8>(r, fill, filled, width, chain);
+    else run_launch<float, 4>(r, fill, filled, width, chain);
   }
   return launch_error(chain.err, "b2_embed_grad");
 }

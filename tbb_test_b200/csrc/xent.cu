@@ -378,29 +378,42 @@ struct ProductParams {
 
 // How the tiles of dh go over the pairs. There are few of them and their sums are long, so whole tiles alone would leave many
 // pairs idle in the last round (232 tiles on 74 pairs: 4 rounds for 3.1). Whole tiles fill complete rounds, all pairs in step so
-// that they share their slabs in the L2 cache; the k range of the `rest` tiles behind them is cut into `shares` equal parts,
-// one per pair, which may cover the end of one tile and the beginning of the next. A part's sum goes to a slot of its
-// pair, and spread_rows_kernel adds a tile's parts in order. Which part is whose does not depend on the piece, so the slots
-// are added to from piece to piece.
+// that they share their slabs in the L2 cache; the k range of the `rest` tiles behind them is cut into equal parts, one per
+// pair, which may cover the end of one tile and the beginning of the next. A part's sum goes to a slot of its pair, and
+// spread_rows_kernel adds a tile's parts in order. Which part is whose does not depend on the piece, so the slots are added to
+// from piece to piece.
+// Where the rest is whole rows of tiles, `side` pairs go through the k range of a row of tiles side by side, so that they read the
+// same slab of d at the same time (28 tiles, 4 in a row, 296 k-blocks, twice: 450 -> 435 us
+// for the whole call).
 struct HiddenSplit {
-  int m_blocks, n_blocks, whole, rest, shares;
+  int m_blocks, n_blocks, whole, side, rest, shares;  // rest and shares count rows of `side` tiles and of pairs
   __device__ HiddenSplit(const ProductParams& p, unsigned int rows, int bn) {
     m_blocks = row_blocks(rows);
     n_blocks = (p.width + bn - 1) / bn;
     const int tiles = m_blocks * n_blocks;
     whole = tiles / p.pairs * p.pairs;
-    rest = tiles - whole;
+    side = whole == 0 && n_blocks <= 8 ? n_blocks : 1;
+    rest = (tiles - whole) / side;
     // no part shorter than eight k-blocks, where there is a choice
-    shares = (int)min((long long)p.pairs, max((long long)rest, (long long)rest * p.full_kblocks / 8));
+    shares = (int)min((long long)(p.pairs / side), max((long long)rest, (long long)rest * p.full_kblocks / 8));
   }
-  // Part j (0, 1) of share s: tile, and its range of k in 1 / shares of a tile. False: there is none.
+  // Part j (0, 1) of pair s: tile behind the whole ones, and its range of k in 1 / shares of a tile. False: there is none.
   __device__ bool part(int s, int j, int& tile, int& from, int& to) const {
-    const int begin = s * rest, end = begin + rest;  // in 1 / shares of a tile
-    tile = begin / shares + j;
-    from = max(begin - tile * shares, 0);
-    to = min(end - tile * shares, shares);
+    const int begin = s / side * rest, end = begin + rest;  // in 1 / shares of a row of tiles
+    if (s / side >= shares) return false;
+    const int row = begin / shares + j;
+    tile = row * side + s % side;
+    from = max(begin - row * shares, 0);
+    to = min(end - row * shares, shares);
     return to > from;
   }
+  // How many parts tile t has, and the slot of the n-th, where there are more than one.
+  __device__ int parts(int t) const { return t < 0 ? 1 : ((t / side + 1) * shares - 1) / rest - t / side * shares / rest + 1; }
+  __device__ int slot(int t, int n) const {
+    const int share = t / side * shares / rest + n;
+    return slot_of(share * side + t % side, share * rest > t / side * shares);
+  }
+  __device__ static int slot_of(int s, bool begun_before) { return 2 * s + (begun_before ? 0 : 1); }
 };
 
 // dh (listed rows) += d w over a piece.
@@ -428,7 +441,7 @@ struct HiddenOp {
     if (t >= split.whole) {
       const int j = (t - split.whole) / p.pairs, s = t - split.whole - j * p.pairs;
       int a, b;
-      if (s >= split.shares || !split.part(s, j, at, a, b)) {
+      if (!split.part(s, j, at, a, b)) {
         r.z = -2;  // nothing
         r.m0 = r.n0 = r.a_mn = r.b_mn = r.a_k = r.b_k = r.kblocks = 0;
         return r;
@@ -436,7 +449,7 @@ struct HiddenOp {
       at += split.whole;
       from = (int)((long long)kblocks * a / split.shares);
       kb = (int)((long long)kblocks * b / split.shares) - from;
-      if (a > 0 || b < split.shares) r.z = 2 * s + (a > 0 ? 0 : 1);
+      if (a > 0 || b < split.shares) r.z = HiddenSplit::slot_of(s, a > 0);
     }
     r.m0 = at / split.n_blocks * TILE_M;
     r.n0 = at % split.n_blocks * BN;
@@ -560,14 +573,12 @@ __global__ void __launch_bounds__(256) spread_rows_kernel(const ProductParams p,
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
       if (slot >= 0) {
         const int t = slot / TILE_M * split.n_blocks + c / BN - split.whole;
-        // the shares that a tile behind the whole ones lies in; one alone means that it was not cut
-        const int s0 = t < 0 ? 0 : t * split.shares / split.rest, s1 = t < 0 ? 0 : ((t + 1) * split.shares - 1) / split.rest;
-        if (s0 == s1) {
+        const int parts = split.parts(t);
+        if (parts == 1) {
           x = *reinterpret_cast<const float4*>(p.acc + slot * p.ld_acc + c);
         } else {
-          for (int s = s0; s <= s1; ++s) {
-            const int z = 2 * s + (s * split.rest > t * split.shares ? 0 : 1);  // not from the tile's beginning on: HiddenOp's a > 0
-            const float4 y = *reinterpret_cast<const float4*>(p.slots + ((long long)z * TILE_M + slot % TILE_M) * BN + c % BN);
+          for (int n = 0; n < parts; ++n) {
+            const float4 y = *reinterpret_cast<const float4*>(p.slots + ((long long)split.slot(t, n) * TILE_M + slot % TILE_M) * BN + c % BN);
             x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
           }
         }

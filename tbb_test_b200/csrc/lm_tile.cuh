@@ -23,6 +23,8 @@
 
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "lm.cuh"
 #include "tcgen05.cuh"
 
@@ -485,7 +487,13 @@ int tile_launch(const char* who, const TileOperand& a, const TileOperand& b, con
   else maps.c = maps.a;
   if (!ok) return call_error(B2_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", who);
   const size_t smem = TileForm<Op::SPLIT>::SMEM;
-  cudaError_t e = cudaFuncSetAttribute(tile_kernel<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<unsigned long long> raised{0};  // the kernel's shared-memory limit: one bit per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !(raised.load() >> dev & 1))) {
+    e = cudaFuncSetAttribute(tile_kernel<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess && dev < 64) raised.fetch_or(1ull << dev);
+  }
   if (e != cudaSuccess) return launch_error(e, who);
   const int pairs = sms / 2;
   const unsigned int grid = 2 * (unsigned int)(most_tiles < pairs ? most_tiles : pairs);

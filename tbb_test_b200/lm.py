@@ -46,6 +46,14 @@ def _matrix(name, x, dtype=None, shape=None, device=None):
     return x.data_ptr(), between
 
 
+def _result(name, x, rows, cols, dtype, device):
+    """(tensor, address, leading dimension) of a result: the given one, checked, or a new one."""
+    if x is None:
+        x = torch.empty(rows, cols, dtype=dtype, device=device)
+        return x, x.data_ptr(), cols
+    return (x, *_matrix(name, x, dtype, (rows, cols), device))
+
+
 def _tokens(name, t, device):
     if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name}: an int32 or int64 tensor is wanted")
@@ -72,6 +80,8 @@ def _workspace(device, entry, *sizes):
 class _on:
     """The device of a call made the current one, where it is not already; gives the address of its current stream."""
 
+    __slots__ = ("index", "before")
+
     def __init__(self, device):
         self.index = device.index
 
@@ -90,14 +100,12 @@ def embed(tokens, table, scale=1.0, out=None):
     """`scale * table[tokens]`: one row per token in the order of `tokens.reshape(-1)`; zeros for padding."""
     p, ld = _matrix("table", table)
     vocab, width = table.shape
-    t, size = _tokens("tokens", tokens, table.device)
+    device = table.device
+    t, size = _tokens("tokens", tokens, device)
     n = t.numel()
-    if out is None:
-        out = torch.empty(n, width, dtype=table.dtype, device=table.device)
-    po, ldo = _matrix("out", out, table.dtype, (n, width), table.device)
-    with _on(table.device) as stream:
-        _ck(K.lib().b2_embed(t.data_ptr(), size, n, p, _DTYPES[table.dtype], vocab, width, ld, scale, po, ldo,
-                             stream))
+    out, po, ldo = _result("out", out, n, width, table.dtype, device)
+    with _on(device) as stream:
+        _ck(K.lib().b2_embed(t.data_ptr(), size, n, p, _DTYPES[table.dtype], vocab, width, ld, scale, po, ldo, stream))
     return out
 
 
@@ -105,14 +113,13 @@ def embed_grad(tokens, dout, vocab, scale=1.0, out=None):
     """Gradient of `embed` with respect to the table, vocab x width, from the gradient `dout` of its output."""
     p, ld = _matrix("dout", dout)
     n, width = dout.shape
-    t, size = _tokens("tokens", tokens, dout.device)
+    device = dout.device
+    t, size = _tokens("tokens", tokens, device)
     if t.numel() != n:
         raise ValueError(f"dout: {n} rows for {t.numel()} tokens")
-    if out is None:
-        out = torch.empty(vocab, width, dtype=dout.dtype, device=dout.device)
-    po, ldo = _matrix("out", out, dout.dtype, (vocab, width), dout.device)
-    with _on(dout.device) as stream:
-        ws = _workspace(dout.device, "embed_grad", n, vocab, width)
+    out, po, ldo = _result("out", out, vocab, width, dout.dtype, device)
+    with _on(device) as stream:
+        ws = _workspace(device, "embed_grad", n, vocab, width)
         _ck(K.lib().b2_embed_grad(t.data_ptr(), size, n, p, _DTYPES[dout.dtype], ld, vocab, width, scale, po, ldo,
                                   ws.data_ptr(), ws.numel(), stream))
     return out
@@ -136,10 +143,8 @@ def xent(h, w, targets, scale=1.0, grad=True, dh=None, dw=None):
     pdh = pdw = None
     lddh = lddw = 0
     if grad:
-        dh = torch.empty(rows, width, dtype=dtype, device=device) if dh is None else dh
-        dw = torch.empty(vocab, width, dtype=dtype, device=device) if dw is None else dw
-        pdh, lddh = _matrix("dh", dh, dtype, (rows, width), device)
-        pdw, lddw = _matrix("dw", dw, dtype, (vocab, width), device)
+        dh, pdh, lddh = _result("dh", dh, rows, width, dtype, device)
+        dw, pdw, lddw = _result("dw", dw, vocab, width, dtype, device)
     with _on(device) as stream:
         # the size goes by the alignment of w and its rows
         ws = _workspace(device, "xent", rows, width, vocab, _DTYPES[dtype], int(grad), pw % 256 or None, ldw)

@@ -17,7 +17,7 @@
 // diagonal, so that x is read once per step. The last step's tiles update w as they are finished.
 //
 // Matrices of a call have one shape and go side by side, so that small ones fill the GPU together. Sides are rounded up to
-// 128 with zeros, which stay zeros.
+// 64, a k-block, with zeros, which stay zeros.
 #include "lm_tile.cuh"
 
 namespace b2 {
@@ -173,7 +173,7 @@ struct SymmetricOp {
   int m_blocks, n_blocks, per;
   __device__ explicit SymmetricOp(const SymmetricParams& q, const TileMaps&) : p(q) {
     m_blocks = (p.side + TILE_M - 1) / TILE_M;
-    n_blocks = p.side / 128;
+    n_blocks = (p.side + 127) / 128;
     per = m_blocks * n_blocks - m_blocks * (m_blocks - 1);  // row block i has column blocks 2 i and up
   }
   __device__ int tiles() const { return per * p.count; }
@@ -195,14 +195,14 @@ struct SymmetricOp {
   // for the elements of a tile)
   Pair4 a[8];
   __device__ __forceinline__ void begin(const Tile& t, int row0, int col0, int lane) {
-    if (!MIDDLE || row0 >= p.side) return;
+    if (!MIDDLE || row0 >= p.side || col0 >= p.side) return;
     const __half *hi = p.a_hi + (long long)t.z * p.side * p.side, *lo = p.a_lo + (long long)t.z * p.side * p.side;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       a[i] = load_pair(hi, lo, (long long)(row0 + quad_row<16>(i & 3, lane)) * p.side + col0 + (i >> 2) * 16 + quad_col<16>(lane));
   }
   __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[16], uint8_t* stage, int lane) {
-    if (row0 >= p.side) return;  // uniform: sides are multiples of 128
+    if (row0 >= p.side || col0 >= p.side) return;  // uniform: sides are multiples of 64
     const long long base = (long long)t.z * p.side * p.side;
     constexpr float unit = MIDDLE ? P_UP * NS_C / (A_UP * A_UP) : A_UP / (X_UP * X_UP), b = P_UP * NS_B / A_UP;
     const bool second = (col0 - t.n0) & 16;  // of the warp's two chunks
@@ -243,7 +243,7 @@ struct NextOp {
   int m_blocks, n_blocks;
   __device__ explicit NextOp(const NextParams& q, const TileMaps&) : p(q) {
     m_blocks = (p.rows_up + TILE_M - 1) / TILE_M;
-    n_blocks = p.cols_up / 128;
+    n_blocks = (p.cols_up + 127) / 128;
   }
   __device__ int tiles() const { return m_blocks * n_blocks * p.count; }
   __device__ Tile tile(int t) const {
@@ -283,7 +283,7 @@ struct NextOp {
     }
   }
   __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[16], uint8_t* stage, int lane) {
-    if (row0 >= p.rows_up) return;
+    if (row0 >= p.rows_up || col0 >= p.cols_up) return;
     if (!LAST) {
       const long long base = (long long)t.z * p.rows_up * p.cols_up;
       constexpr float unit = 1.f / P_UP;
@@ -330,11 +330,11 @@ struct MuonSizes {
 };
 MuonSizes muon_sizes(int count, int rows, int cols) {
   MuonSizes z;
-  z.rows_up = (rows + 127) / 128 * 128;
-  z.cols_up = (cols + 127) / 128 * 128;
+  z.rows_up = (rows + TILE_K - 1) / TILE_K * TILE_K;
+  z.cols_up = (cols + TILE_K - 1) / TILE_K * TILE_K;
   z.side = rows <= cols ? z.rows_up : z.cols_up;
   // as many side by side as give every pair of SMs several tiles of the smallest product
-  const long long blocks = z.side / 128, per = (blocks * blocks / 2 + blocks) / 2 + 1;
+  const long long blocks = (z.side + 127) / 128, per = (blocks * blocks / 2 + blocks) / 2 + 1;
   long long group = (4 * 74 + per - 1) / per;
   if (group > MUON_GROUP) group = MUON_GROUP;
   z.group = count < group ? count : (int)group;
@@ -402,7 +402,7 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
   const bool wide = rows <= cols;
   const long long x_rows = (long long)z.rows_up * count, a_rows = (long long)z.side * count;
   const long long half_tiles = [&] {
-    const long long m = (z.side + TILE_M - 1) / TILE_M, n = z.side / 128;
+    const long long m = (z.side + TILE_M - 1) / TILE_M, n = (z.side + 127) / 128;
     return (m * n - m * (m - 1)) * count;
   }();
   const TileOperand a_op{s.a_hi, s.a_lo, a_rows, z.side, z.side, false}, p_op{s.p_hi, s.p_lo, a_rows, z.side, z.side, false};
@@ -450,7 +450,7 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
       if (reinterpret_cast<uintptr_t>(list.w[i]) % 16) n.vec_w = 0;
       if (reinterpret_cast<uintptr_t>(list.copy[i]) % 8) n.vec_copy = 0;
     }
-    const long long tiles = (long long)((z.rows_up + TILE_M - 1) / TILE_M) * (z.cols_up / 128) * count;
+    const long long tiles = (long long)((z.rows_up + TILE_M - 1) / TILE_M) * ((z.cols_up + 127) / 128) * count;
     const TileOperand &ao = wide ? p_op : x_k, &bo = wide ? x_mn : p_op;
     rc = k + 1 == o.steps ? tile_launch<NextOp<true>>(who, ao, bo, nullptr, n, false, tiles, sms, chain)
                           : tile_launch<NextOp<false>>(who, ao, bo, nullptr, n, false, tiles, sms, chain);

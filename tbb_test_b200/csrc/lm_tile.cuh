@@ -16,9 +16,14 @@
 //           accumulator (about 2e-8 of the sum each time, and always towards zero), so a sum is handed over every
 //           Op::SUM k-blocks and added up in fp32 registers, rounded to nearest.
 //
+// Where there are fewer tiles than SMs, single CTAs (ONE) with tcgen05.mma.cta_group::1 and tiles of a quarter of the size take less
+// time: more SMs have work, and a call's products, which wait for one another, start and end sooner without a cluster (15 products of 256 x
+// 256 x 256: 144 -> 99 us; of 1024 x 1024 x 1024 249 -> 184). With more tiles pairs do, which read half of B's slab each: 1536 x 1536 in
+// two rounds of single CTAs 393 us, in one of pairs 324.
+//
 // Warps: 0 loads, 1 allocates tensor memory and (in the leader) issues, the others work on elements: those of a lane quarter share
-// its columns. There are 16 of them in the split form, where small matrices wait for nothing else as long (256 x 256: 154 -> 144 us
-// per update), and 8 in the plain one, which the power limit binds (with 16 and five stages 8192 x 2048 x 65536 took 6.2 ms for 6.0).
+// its columns. There are 16 of them in the split form, where small matrices wait for nothing else as long (256 x 256 in pairs: 154 ->
+// 144 us), and 8 in the plain one, which the power limit binds (with 16 and five stages 8192 x 2048 x 65536 took 6.2 ms for 6.0).
 #pragma once
 
 #include <cuda_fp16.h>
@@ -39,11 +44,16 @@ constexpr int TILE_MAX_STAGES = 6;
 // A wait that gave up leaves its role's number here; b2_lm_sync reports and clears it.
 __device__ unsigned int tile_status;
 
-template <bool SPLIT>
+template <bool SPLIT_, bool ONE_ = false>
 struct TileForm {
-  static constexpr int BN = SPLIT ? 128 : 256;
+  static constexpr bool SPLIT = SPLIT_, ONE = ONE_;
+  static_assert(SPLIT || !ONE, "single CTAs are for the split form");
+  static constexpr int CTAS = ONE ? 1 : 2;       // that share a tile
+  static constexpr int M = CTAS * 128;
+  static constexpr int BN = !SPLIT ? 256 : ONE ? 64 : 128;
+  static constexpr int B_ROWS = BN / CTAS;       // of B's slab, in a CTA
   static constexpr int STAGES = SPLIT ? 4 : 6;
-  static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = BN / 2 * 128;
+  static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = B_ROWS * 128;
   static constexpr uint32_t SLABS = (A_BYTES + B_BYTES) * (SPLIT ? 2 : 1);  // of a stage
   static constexpr int WARPS = SPLIT ? 16 : 8;   // on elements
   static constexpr int PARTS = WARPS / 4;        // warps that share a row's columns
@@ -72,9 +82,9 @@ struct Tile {
   int z;        // the operator's own
 };
 
-// Adds 16 finished columns of this lane's row to `sum`.
-__device__ __forceinline__ void tile_add16(uint32_t from, float* sum) {
-  uint32_t r[16];
+// Finished columns of this lane's row.
+__device__ __forceinline__ void tile_read(uint32_t from, uint32_t (&r)[32]) { tmem_ld32(from, r); }
+__device__ __forceinline__ void tile_read(uint32_t from, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
@@ -82,21 +92,48 @@ __device__ __forceinline__ void tile_add16(uint32_t from, float* sum) {
       : "r"(from)
       : "memory");
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tile_add16(uint32_t from, float* sum) {
+  uint32_t r[16];
+  tile_read(from, r);
 #pragma unroll
   for (int j = 0; j < 16; ++j) sum[j] += __uint_as_float(r[j]);
 }
+template <bool PAIR>
+__device__ __forceinline__ void tile_commit(uint32_t bar) {
+  if (PAIR) tc_commit_pair(bar);
+  else tc_commit(bar);
+}
+// All 512 columns of tensor memory, by one whole warp (of each CTA of a pair).
+template <bool PAIR>
+__device__ __forceinline__ void tmem_take(uint32_t* base) {
+#define B2_TAKE(GROUP)                                                                                                             \
+  asm volatile("tcgen05.alloc." GROUP ".sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(base)), "r"(512u) : "memory"); \
+  asm volatile("tcgen05.relinquish_alloc_permit." GROUP ".sync.aligned;" ::: "memory")
+  if (PAIR) {
+    B2_TAKE("cta_group::2");
+  } else {
+    B2_TAKE("cta_group::1");
+  }
+#undef B2_TAKE
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_give(uint32_t base) {
+  if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(512u) : "memory");
+  else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(512u) : "memory");
+}
 
-// Op: struct Params; static constexpr bool SPLIT; Op(const Params&, const TileMaps&); int tiles(); Tile tile(int t);
+// Op: struct Params; typedef TileForm<...> Form; Op(const Params&, const TileMaps&); int tiles(); Tile tile(int t);
 //     and in the element warps: void begin(const Tile&, int row, int col, int lane) before the sums are there, for the warp's
 //     first row and column; void chunk(const Tile&, int row0, int col0, float (&v)[CHUNK], uint8_t* stage, int lane) for CHUNK columns of
 //     rows row0 + lane; void end(const Tile&, int row, int part) for the thread's row and its warp's part of the columns;
 //     static constexpr bool STORES: it issues TMA stores from `stage`; static constexpr bool LONG: sums are handed over every SUM
 //     (static constexpr int) k-blocks, which the split form always does; chunks have 16 columns then.
 template <class Op>
-__global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ TileLayout L,
-                                                               const __grid_constant__ typename Op::Params params) {
-  constexpr bool SPLIT = Op::SPLIT;
-  typedef TileForm<SPLIT> F;
+__global__ void __launch_bounds__(Op::Form::BOUND, 1) tile_kernel(const __grid_constant__ TileMaps maps, const __grid_constant__ TileLayout L,
+                                                                const __grid_constant__ typename Op::Params params) {
+  typedef typename Op::Form F;
+  constexpr bool SPLIT = F::SPLIT, PAIR = !F::ONE;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[TILE_MAX_STAGES];
   __shared__ __align__(8) uint64_t empty_bar[TILE_MAX_STAGES];
@@ -107,8 +144,8 @@ __global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(con
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_ctarank();
-  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0u;
+  const int first_tile = blockIdx.x / F::CTAS, every = gridDim.x / F::CTAS;
   volatile int* abort_flag = &abort_s;
 
   if (threadIdx.x == 0) {
@@ -119,20 +156,18 @@ __global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(con
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full_bar[a], 1);
-      mbar_init(&acc_empty_bar[a], 2 * F::WARPS);  // the element warps of both CTAs
+      mbar_init(&acc_empty_bar[a], F::CTAS * F::WARPS);  // the element warps of all
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.a) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.b) : "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(512u)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    tmem_take<PAIR>(&tmem_base_s);
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();
+  if (PAIR) cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_s;
   after_previous();
@@ -146,21 +181,21 @@ __global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(con
       uint32_t phase = 0;
       bool ok = true;
       const uint32_t full0 = map_to_cta(smem_u32(full_bar), 0), empty0 = smem_u32(empty_bar), ring0 = smem_u32(smem);
-      for (int t = pair; t < tiles && ok; t += num_pairs) {
+      for (int t = first_tile; t < tiles && ok; t += every) {
         const Tile tile = op.tile(t);
-        const int am = tile.a_mn + (int)rank * 128, bn = tile.b_mn + (int)rank * (F::BN / 2);
+        const int am = tile.a_mn + (int)rank * 128, bn = tile.b_mn + (int)rank * F::B_ROWS;
         for (int kb = 0; kb < tile.kblocks; ++kb) {
           if (!mbar_wait(empty0 + 8u * stage, phase ^ 1, abort_flag, &tile_status, 1u)) { ok = false; break; }
           const uint32_t s0 = ring0 + (uint32_t)stage * F::SLABS;
-          if (rank == 0) mbar_expect_tx(smem_u32(full_bar) + 8u * stage, 2 * F::SLABS);  // both CTAs' bytes
+          if (rank == 0) mbar_expect_tx(smem_u32(full_bar) + 8u * stage, F::CTAS * F::SLABS);  // both CTAs' bytes
           const uint32_t full = full0 + 8u * stage;
           const int ka = tile.a_k + kb * TILE_K, kbb = tile.b_k + kb * TILE_K;
-          load_slab<true>(&maps.a, full, s0, L.a_form, ka, am, 2, TILE_K * 128, 6);
+          load_slab<PAIR>(&maps.a, full, s0, L.a_form, ka, am, 2, TILE_K * 128, 6);
           const uint32_t sb = s0 + F::A_BYTES * (SPLIT ? 2 : 1);
-          load_slab<true>(&maps.b, full, sb, L.b_form, kbb, bn, F::BN / 128, TILE_K * 128, 6);
+          load_slab<PAIR>(&maps.b, full, sb, L.b_form, kbb, bn, F::B_ROWS / 64, TILE_K * 128, 6);
           if (SPLIT) {
-            load_slab<true>(&maps.a_lo, full, s0 + F::A_BYTES, L.a_form, ka, am, 2, TILE_K * 128, 6);
-            load_slab<true>(&maps.b_lo, full, sb + F::B_BYTES, L.b_form, kbb, bn, F::BN / 128, TILE_K * 128, 6);
+            load_slab<PAIR>(&maps.a_lo, full, s0 + F::A_BYTES, L.a_form, ka, am, 2, TILE_K * 128, 6);
+            load_slab<PAIR>(&maps.b_lo, full, sb + F::B_BYTES, L.b_form, kbb, bn, F::B_ROWS / 64, TILE_K * 128, 6);
           }
           if (++stage == F::STAGES) { stage = 0; phase ^= 1; }
         }
@@ -179,7 +214,7 @@ __global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(con
       const uint64_t b_tmpl = make_smem_desc(smem_u32(smem) + F::A_BYTES * (SPLIT ? 2 : 1), L.b_lbo, 1024, 2);
       const uint32_t a_step = L.a_kstep >> 4, b_step = L.b_kstep >> 4, idesc = L.idesc;
       const uint32_t full0 = smem_u32(full_bar), empty0 = smem_u32(empty_bar), acc_full0 = smem_u32(acc_full_bar);
-      for (int t = pair; t < tiles && ok; t += num_pairs) {
+      for (int t = first_tile; t < tiles && ok; t += every) {
         const int kblocks = op.tile(t).kblocks;
         for (int kb = 0; kb < kblocks; ++kb) {
           const bool first = kb == 0 || (Op::LONG && kb % Op::SUM == 0);
@@ -195,16 +230,16 @@ __global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(con
           for (int ks = 0; ks < TILE_K / 16; ++ks) {
             const uint64_t ad = a_tmpl + off + (uint64_t)(ks * a_step), bd = b_tmpl + off + (uint64_t)(ks * b_step);
             const uint32_t go = first && ks == 0 ? 0u : 1u;
-            mma_issue<false, true>(d, ad, bd, idesc, go);
+            mma_issue<false, PAIR>(d, ad, bd, idesc, go);
             if (SPLIT) {
-              mma_issue<false, true>(d + F::BN, ad, bd + (F::B_BYTES >> 4), idesc, go);
-              mma_issue<false, true>(d + F::BN, ad + (F::A_BYTES >> 4), bd, idesc, 1u);
+              mma_issue<false, PAIR>(d + F::BN, ad, bd + (F::B_BYTES >> 4), idesc, go);
+              mma_issue<false, PAIR>(d + F::BN, ad + (F::A_BYTES >> 4), bd, idesc, 1u);
             }
           }
-          tc_commit_pair(empty0 + 8u * stage);
+          tile_commit<PAIR>(empty0 + 8u * stage);
           if (++stage == F::STAGES) { stage = 0; phase ^= 1; }
           if (kb + 1 == kblocks || (Op::LONG && (kb + 1) % Op::SUM == 0)) {
-            tc_commit_pair(acc_full0 + 8u * acc);
+            tile_commit<PAIR>(acc_full0 + 8u * acc);
             acc ^= 1;
             if (acc == 0) acc_phase ^= 1;
           }
@@ -218,7 +253,7 @@ __global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(con
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    for (int t = pair; t < tiles && ok; t += num_pairs) {
+    for (int t = first_tile; t < tiles && ok; t += every) {
       const Tile tile = op.tile(t);
       const int row0 = tile.m0 + (int)rank * 128 + q * 32, col0 = tile.n0 + part * F::COLS;
       const uint32_t place = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(part * F::COLS);
@@ -233,11 +268,11 @@ __global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(con
           if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_flag, &tile_status, 4u)) { ok = false; break; }
           tc_fence_after();
           const uint32_t from = place + (uint32_t)acc * ACC_COLS;
-          uint32_t r[32], x[32];
-          tmem_ld32(from, r);
-          tmem_ld32(from + F::BN, x);
+          uint32_t r[F::COLS], x[F::COLS];
+          tile_read(from, r);
+          tile_read(from + F::BN, x);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
+          for (int j = 0; j < F::COLS; ++j) {
             const float v = fmaf(__uint_as_float(x[j]), 1.f / LO_UP, __uint_as_float(r[j]));
             sum[j] = kb == 0 ? v : sum[j] + v;
           }
@@ -330,10 +365,10 @@ __global__ void __launch_bounds__(TileForm<Op::SPLIT>::BOUND, 1) tile_kernel(con
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();
+  if (PAIR) cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+    tmem_give<PAIR>(tmem_base);
   }
 }
 
@@ -438,8 +473,8 @@ struct TileOperand {
   bool mn_contiguous;
 };
 
-inline bool tile_maps(const TileOperand& a, const TileOperand& b, bool split, bool bf16, TileMaps* maps, TileLayout* L) {
-  const int bn = split ? 128 : 256;
+template <class F>
+bool tile_maps(const TileOperand& a, const TileOperand& b, bool bf16, TileMaps* maps, TileLayout* L) {
   auto one = [](const TileOperand& o, const void* p, int rows, int* form, CUtensorMap* m) {
     if (!o.mn_contiguous) {
       *form = SLAB_K;
@@ -452,9 +487,9 @@ inline bool tile_maps(const TileOperand& a, const TileOperand& b, bool split, bo
     *form = SLAB_MN2;
     return make_map(m, p, 2, o.mn, o.k, o.ld, 64, TILE_K, 0);
   };
-  bool ok = one(a, a.hi, 128, &L->a_form, &maps->a) && one(b, b.hi, bn / 2, &L->b_form, &maps->b);
-  if (split) {
-    ok = ok && one(a, a.lo, 128, &L->a_form, &maps->a_lo) && one(b, b.lo, bn / 2, &L->b_form, &maps->b_lo);
+  bool ok = one(a, a.hi, 128, &L->a_form, &maps->a) && one(b, b.hi, F::B_ROWS, &L->b_form, &maps->b);
+  if (F::SPLIT) {
+    ok = ok && one(a, a.lo, 128, &L->a_form, &maps->a_lo) && one(b, b.lo, F::B_ROWS, &L->b_form, &maps->b_lo);
   } else {
     maps->a_lo = maps->a;
     maps->b_lo = maps->b;
@@ -465,7 +500,7 @@ inline bool tile_maps(const TileOperand& a, const TileOperand& b, bool split, bo
   L->b_kstep = b.mn_contiguous ? 16 * 128 : 32;
   const uint32_t fmt = bf16 ? 1u : 0u;  // bf16 : f16
   L->idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a.mn_contiguous << 15) | ((uint32_t)b.mn_contiguous << 16) |
-             ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(TILE_M >> 4) << 24);
+             ((uint32_t)(F::BN >> 3) << 17) | ((uint32_t)(F::M >> 4) << 24);
   return ok;
 }
 
@@ -479,14 +514,15 @@ struct TileResult {
 template <class Op>
 int tile_launch(const char* who, const TileOperand& a, const TileOperand& b, const TileResult* c, const typename Op::Params& p, bool bf16,
                 long long most_tiles, int sms, Chain& chain) {
+  typedef typename Op::Form F;
   if (most_tiles <= 0) return B2_OK;
   TileMaps maps;
   TileLayout L;
-  bool ok = tile_maps(a, b, Op::SPLIT, bf16, &maps, &L);
+  bool ok = tile_maps<F>(a, b, bf16, &maps, &L);
   if (c) ok = ok && make_map(&maps.c, c->p, 2, c->cols, c->rows, c->ld, 64, 32, 0);
   else maps.c = maps.a;
   if (!ok) return call_error(B2_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", who);
-  const size_t smem = TileForm<Op::SPLIT>::SMEM;
+  const size_t smem = F::SMEM;
   static std::atomic<unsigned long long> raised{0};  // the kernel's shared-memory limit: one bit per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -495,9 +531,9 @@ int tile_launch(const char* who, const TileOperand& a, const TileOperand& b, con
     if (e == cudaSuccess && dev < 64) raised.fetch_or(1ull << dev);
   }
   if (e != cudaSuccess) return launch_error(e, who);
-  const int pairs = sms / 2;
-  const unsigned int grid = 2 * (unsigned int)(most_tiles < pairs ? most_tiles : pairs);
-  chain.launch(tile_kernel<Op>, dim3(grid), TileForm<Op::SPLIT>::THREADS, smem, 2, maps, L, p);
+  const int most = sms / F::CTAS;
+  const unsigned int grid = F::CTAS * (unsigned int)(most_tiles < most ? most_tiles : most);
+  chain.launch(tile_kernel<Op>, dim3(grid), F::THREADS, smem, F::ONE ? 0 : 2, maps, L, p);
   return launch_error(chain.err, who);
 }
 

@@ -164,16 +164,17 @@ struct SymmetricParams {
   const __half *a_hi, *a_lo;
   __half *to_hi, *to_lo;
 };
-template <bool MIDDLE>
+template <bool MIDDLE, bool ONE>
 struct SymmetricOp {
   typedef SymmetricParams Params;
-  static constexpr bool SPLIT = true, STORES = false, LONG = true;
+  typedef TileForm<true, ONE> Form;
+  static constexpr bool STORES = false, LONG = true;
   static constexpr int SUM = MUON_SUM;
   const SymmetricParams& p;
   int m_blocks, n_blocks, per;
   __device__ explicit SymmetricOp(const SymmetricParams& q, const TileMaps&) : p(q) {
-    m_blocks = (p.side + TILE_M - 1) / TILE_M;
-    n_blocks = (p.side + 127) / 128;
+    m_blocks = (p.side + Form::M - 1) / Form::M;
+    n_blocks = (p.side + Form::BN - 1) / Form::BN;
     per = m_blocks * n_blocks - m_blocks * (m_blocks - 1);  // row block i has column blocks 2 i and up
   }
   __device__ int tiles() const { return per * p.count; }
@@ -182,8 +183,8 @@ struct SymmetricOp {
     r.z = t / per;
     int in = t - r.z * per, i = 0;
     while (in >= n_blocks - 2 * i) in -= n_blocks - 2 * i++;
-    r.m0 = i * TILE_M;
-    r.n0 = (2 * i + in) * 128;
+    r.m0 = i * Form::M;
+    r.n0 = (2 * i + in) * Form::BN;
     const int off = r.z * (int)p.a_step;
     r.a_mn = r.m0 + (p.steps_k ? 0 : off);
     r.b_mn = r.n0 + (p.steps_k ? 0 : off);
@@ -193,24 +194,25 @@ struct SymmetricOp {
   }
   // a is loaded while the products are summed: it is what a small matrix's middle factor would wait for otherwise (5.6 against 2.7 us
   // for the elements of a tile)
-  Pair4 a[8];
+  static constexpr int QUADS = Form::COLS / 4;
+  Pair4 a[QUADS];
   __device__ __forceinline__ void begin(const Tile& t, int row0, int col0, int lane) {
     if (!MIDDLE || row0 >= p.side || col0 >= p.side) return;
     const __half *hi = p.a_hi + (long long)t.z * p.side * p.side, *lo = p.a_lo + (long long)t.z * p.side * p.side;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < QUADS; ++i)
       a[i] = load_pair(hi, lo, (long long)(row0 + quad_row<16>(i & 3, lane)) * p.side + col0 + (i >> 2) * 16 + quad_col<16>(lane));
   }
   __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[16], uint8_t* stage, int lane) {
     if (row0 >= p.side || col0 >= p.side) return;  // uniform: sides are multiples of 64
     const long long base = (long long)t.z * p.side * p.side;
     constexpr float unit = MIDDLE ? P_UP * NS_C / (A_UP * A_UP) : A_UP / (X_UP * X_UP), b = P_UP * NS_B / A_UP;
-    const bool second = (col0 - t.n0) & 16;  // of the warp's two chunks
+    const bool second = QUADS > 4 && (col0 - t.n0) & 16;  // of the warp's two chunks
     float4 x[4];
     by_rows(row0, col0, v, stage, lane, [&](int i, int r, int c, const float4& y) {
       x[i] = make_float4(y.x * unit, y.y * unit, y.z * unit, y.w * unit);
       if (MIDDLE) {
-        const float4 old = pair_value(second ? a[4 + i] : a[i]);
+        const float4 old = pair_value(second ? a[QUADS - 4 + i] : a[i]);
         x[i] = make_float4(fmaf(b, old.x, x[i].x), fmaf(b, old.y, x[i].y), fmaf(b, old.z, x[i].z), fmaf(b, old.w, x[i].w));
         if (r == c) x[i].x += NS_A * P_UP;
         if (r == c + 1) x[i].y += NS_A * P_UP;
@@ -219,7 +221,7 @@ struct SymmetricOp {
       }
       store_pair(p.to_hi, p.to_lo, base + (long long)r * p.side + c, x[i]);
     });
-    if (t.n0 >= t.m0 + TILE_M)  // on the diagonal both halves are computed
+    if (t.n0 >= t.m0 + Form::M)  // on the diagonal both halves are computed
       by_columns(row0, col0, x, stage, lane, [&](int r, int c, const float4& y) { store_pair(p.to_hi, p.to_lo, base + (long long)r * p.side + c, y); });
   }
   __device__ __forceinline__ void end(const Tile&, int, int) {}
@@ -234,16 +236,17 @@ struct NextParams {
   float keep, step;  // w = keep w - step x
   int vec_w, vec_copy;
 };
-template <bool LAST>
+template <bool LAST, bool ONE>
 struct NextOp {
   typedef NextParams Params;
-  static constexpr bool SPLIT = true, STORES = false, LONG = true;
+  typedef TileForm<true, ONE> Form;
+  static constexpr bool STORES = false, LONG = true;
   static constexpr int SUM = MUON_SUM;
   const NextParams& p;
   int m_blocks, n_blocks;
   __device__ explicit NextOp(const NextParams& q, const TileMaps&) : p(q) {
-    m_blocks = (p.rows_up + TILE_M - 1) / TILE_M;
-    n_blocks = (p.cols_up + 127) / 128;
+    m_blocks = (p.rows_up + Form::M - 1) / Form::M;
+    n_blocks = (p.cols_up + Form::BN - 1) / Form::BN;
   }
   __device__ int tiles() const { return m_blocks * n_blocks * p.count; }
   __device__ Tile tile(int t) const {
@@ -253,8 +256,8 @@ struct NextOp {
     const int in = t - r.z * per;
     // bands of eight row blocks: what the pairs work on at a time is about square
     const int b = in / (8 * n_blocks), at = in - b * 8 * n_blocks, tall = min(8, m_blocks - 8 * b);
-    r.m0 = (8 * b + at % tall) * TILE_M;
-    r.n0 = at / tall * 128;
+    r.m0 = (8 * b + at % tall) * Form::M;
+    r.n0 = at / tall * Form::BN;
     r.a_mn = r.m0 + r.z * p.rows_up;
     r.a_k = 0;
     r.b_mn = r.n0 + (p.wide ? 0 : r.z * p.cols_up);
@@ -262,12 +265,13 @@ struct NextOp {
     r.kblocks = p.kblocks;
     return r;
   }
-  float4 old[8];  // of w, loaded while the last step's products are summed
+  static constexpr int QUADS = Form::COLS / 4;
+  float4 old[QUADS];  // of w, loaded while the last step's products are summed
   __device__ __forceinline__ void begin(const Tile& t, int row0, int col0, int lane) {
     if (!LAST) return;
     const float* w = p.list.w[t.z];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < QUADS; ++i) {
       const int r = row0 + quad_row<16>(i & 3, lane), c = col0 + (i >> 2) * 16 + quad_col<16>(lane);
       old[i] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r >= p.rows || c >= p.cols) continue;
@@ -293,12 +297,12 @@ struct NextOp {
       return;
     }
     const float unit = p.step / (X_UP * P_UP);
-    const bool second = (col0 - t.n0) & 16;  // of the warp's two chunks
+    const bool second = QUADS > 4 && (col0 - t.n0) & 16;  // of the warp's two chunks
     float* w = p.list.w[t.z];
     __nv_bfloat16* copy = p.list.copy[t.z];
     by_rows(row0, col0, v, stage, lane, [&](int i, int r, int c, const float4& x) {
       if (r >= p.rows || c >= p.cols) return;
-      const float4 o = second ? old[4 + i] : old[i];
+      const float4 o = second ? old[QUADS - 4 + i] : old[i];
       const float f[4] = {fmaf(p.keep, o.x, -x.x * unit), fmaf(p.keep, o.y, -x.y * unit), fmaf(p.keep, o.z, -x.z * unit), fmaf(p.keep, o.w, -x.w * unit)};
       float* to = w + (long long)r * p.ld_w + c;
       const bool whole = c + 4 <= p.cols;
@@ -401,10 +405,14 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
   int rc = launch_error(chain.err, who);
   const bool wide = rows <= cols;
   const long long x_rows = (long long)z.rows_up * count, a_rows = (long long)z.side * count;
-  const long long half_tiles = [&] {
-    const long long m = (z.side + TILE_M - 1) / TILE_M, n = (z.side + 127) / 128;
+  // Tiles of a symmetric and of a full product, in tiles of bm rows; single CTAs where each has one at most.
+  auto symmetric = [&](int bm) {
+    const long long m = (z.side + bm - 1) / bm, n = (z.side + bm / 2 - 1) / (bm / 2);
     return (m * n - m * (m - 1)) * count;
-  }();
+  };
+  auto full = [&](int bm) { return (long long)((z.rows_up + bm - 1) / bm) * ((z.cols_up + bm / 2 - 1) / (bm / 2)) * count; };
+  const bool half_one = symmetric(128) <= sms, full_one = full(128) <= sms;
+  const long long half_tiles = symmetric(half_one ? 128 : 256), tiles = full(full_one ? 128 : 256);
   const TileOperand a_op{s.a_hi, s.a_lo, a_rows, z.side, z.side, false}, p_op{s.p_hi, s.p_lo, a_rows, z.side, z.side, false};
   int at = 0;
   for (int k = 0; k < o.steps && rc == B2_OK; ++k, at ^= 1) {
@@ -418,7 +426,8 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
     q.steps_k = !wide;
     q.to_hi = s.a_hi;
     q.to_lo = s.a_lo;
-    rc = tile_launch<SymmetricOp<false>>(who, wide ? x_k : x_mn, wide ? x_k : x_mn, nullptr, q, false, half_tiles, sms, chain);
+    const TileOperand& x = wide ? x_k : x_mn;
+    rc = (half_one ? tile_launch<SymmetricOp<false, true>> : tile_launch<SymmetricOp<false, false>>)(who, x, x, nullptr, q, false, half_tiles, sms, chain);
     if (rc != B2_OK) return rc;
     q.kblocks = z.side / TILE_K;
     q.a_step = z.side;
@@ -427,7 +436,7 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
     q.a_lo = s.a_lo;
     q.to_hi = s.p_hi;
     q.to_lo = s.p_lo;
-    rc = tile_launch<SymmetricOp<true>>(who, a_op, a_op, nullptr, q, false, half_tiles, sms, chain);
+    rc = (half_one ? tile_launch<SymmetricOp<true, true>> : tile_launch<SymmetricOp<true, false>>)(who, a_op, a_op, nullptr, q, false, half_tiles, sms, chain);
     if (rc != B2_OK) return rc;
     NextParams n{};
     n.list = list;
@@ -450,10 +459,10 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
       if (reinterpret_cast<uintptr_t>(list.w[i]) % 16) n.vec_w = 0;
       if (reinterpret_cast<uintptr_t>(list.copy[i]) % 8) n.vec_copy = 0;
     }
-    const long long tiles = (long long)((z.rows_up + TILE_M - 1) / TILE_M) * ((z.cols_up + 127) / 128) * count;
     const TileOperand &ao = wide ? p_op : x_k, &bo = wide ? x_mn : p_op;
-    rc = k + 1 == o.steps ? tile_launch<NextOp<true>>(who, ao, bo, nullptr, n, false, tiles, sms, chain)
-                          : tile_launch<NextOp<false>>(who, ao, bo, nullptr, n, false, tiles, sms, chain);
+    auto next = k + 1 < o.steps ? (full_one ? tile_launch<NextOp<false, true>> : tile_launch<NextOp<false, false>>)
+                                : (full_one ? tile_launch<NextOp<true, true>> : tile_launch<NextOp<true, false>>);
+    rc = next(who, ao, bo, nullptr, n, false, tiles, sms, chain);
   }
   return rc;
 }

@@ -183,6 +183,7 @@ struct LogitParams {
 
 template <bool SPLIT_>
 struct LogitTiles {
+  typedef TileForm<SPLIT_> Form;
   static constexpr bool SPLIT = SPLIT_;
   static constexpr int SUM = XENT_SUM, BN = TileForm<SPLIT_>::BN, W = TileForm<SPLIT_>::CHUNK;
   const LogitParams& p;
@@ -420,6 +421,7 @@ struct HiddenSplit {
 template <bool SPLIT_>
 struct HiddenOp {
   typedef ProductParams Params;
+  typedef TileForm<SPLIT_> Form;
   static constexpr bool SPLIT = SPLIT_, STORES = false;
   static constexpr bool LONG = SPLIT_;
   static constexpr int SUM = XENT_SUM, BN = TileForm<SPLIT_>::BN;
@@ -492,6 +494,7 @@ struct HiddenOp {
 template <bool SPLIT_>
 struct WeightOp {
   typedef ProductParams Params;
+  typedef TileForm<SPLIT_> Form;
   static constexpr bool SPLIT = SPLIT_, STORES = !SPLIT_;
   static constexpr bool LONG = SPLIT_;
   static constexpr int SUM = XENT_SUM, BN = TileForm<SPLIT_>::BN;

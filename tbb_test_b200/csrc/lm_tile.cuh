@@ -19,7 +19,7 @@
 // Where there are fewer tiles than SMs, single CTAs (ONE) with tcgen05.mma.cta_group::1 and tiles of a quarter of the size take less
 // time: more SMs have work, and a call's products, which wait for one another, start and end sooner without a cluster (15 products of 256 x
 // 256 x 256: 144 -> 99 us; of 1024 x 1024 x 1024 249 -> 184). With more tiles pairs do, which read half of B's slab each: 1536 x 1536 in
-// two rounds of single CTAs 393 us, in one of pairs 324.
+// two rounds of single CTAs 393 us, in one of pairs 324. The plain form's single CTAs take 128 x 128.
 //
 // Warps: 0 loads, 1 allocates tensor memory and (in the leader) issues, the others work on elements: those of a lane quarter share
 // its columns. There are 16 of them in the split form, where small matrices wait for nothing else as long (256 x 256 in pairs: 154 ->
@@ -47,10 +47,9 @@ __device__ unsigned int tile_status;
 template <bool SPLIT_, bool ONE_ = false>
 struct TileForm {
   static constexpr bool SPLIT = SPLIT_, ONE = ONE_;
-  static_assert(SPLIT || !ONE, "single CTAs are for the split form");
   static constexpr int CTAS = ONE ? 1 : 2;       // that share a tile
   static constexpr int M = CTAS * 128;
-  static constexpr int BN = !SPLIT ? 256 : ONE ? 64 : 128;
+  static constexpr int BN = (SPLIT ? 64 : 128) * CTAS;
   static constexpr int B_ROWS = BN / CTAS;       // of B's slab, in a CTA
   static constexpr int STAGES = SPLIT ? 4 : 6;
   static constexpr uint32_t A_BYTES = 128 * 128, B_BYTES = B_ROWS * 128;

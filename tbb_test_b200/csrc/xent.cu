@@ -181,17 +181,17 @@ struct LogitParams {
   long long ld_d;
 };
 
-template <bool SPLIT_>
+template <class F>
 struct LogitTiles {
-  typedef TileForm<SPLIT_> Form;
-  static constexpr bool SPLIT = SPLIT_;
-  static constexpr int SUM = XENT_SUM, BN = TileForm<SPLIT_>::BN, W = TileForm<SPLIT_>::CHUNK;
+  typedef F Form;
+  static constexpr bool SPLIT = F::SPLIT;
+  static constexpr int SUM = XENT_SUM, BN = F::BN, W = F::CHUNK;
   const LogitParams& p;
   int rows, m_blocks, n_blocks, band;
   float unit;  // accumulators times this are logits times log2 e
   __device__ explicit LogitTiles(const LogitParams& q, const TileMaps&) : p(q) {
     rows = (int)p.meta->rows;
-    m_blocks = row_blocks(rows);
+    m_blocks = max(1, (rows + F::M - 1) / F::M);
     n_blocks = (p.v_count + BN - 1) / BN;
     // all row blocks of a column block one after another, as long as the copy of h they read stays in the L2 cache
     band = m_blocks <= 64 ? m_blocks : 16;
@@ -202,7 +202,7 @@ struct LogitTiles {
     const int b = t / (band * n_blocks), in = t - b * band * n_blocks;
     const int tall = min(band, m_blocks - b * band);
     Tile r;
-    r.m0 = (b * band + in % tall) * TILE_M;
+    r.m0 = (b * band + in % tall) * F::M;
     r.n0 = in / tall * BN;
     r.a_mn = r.m0;
     r.b_mn = p.v_begin + r.n0;
@@ -216,22 +216,22 @@ struct LogitTiles {
 // Maximum and sum of exponentials of a row over the columns of one warp, and the target's logit. LONG: for more than 16 k-blocks,
 // whose sums the tensor core would leave too small (bf16, width 2048: losses 1.0e-6 off, with sums of 16 added in fp32 0.5e-6, in the
 // same time).
-template <bool SPLIT_, bool LONG_>
-struct StatOp : LogitTiles<SPLIT_> {
+template <class F, bool LONG_>
+struct StatOp : LogitTiles<F> {
   typedef LogitParams Params;
-  static constexpr bool LONG = SPLIT_ || LONG_;
-  static constexpr int SUM = SPLIT_ ? XENT_SUM : 16;
+  static constexpr bool LONG = F::SPLIT || LONG_;
+  static constexpr int SUM = F::SPLIT ? XENT_SUM : 16;
   static constexpr bool STORES = false;
-  using LogitTiles<SPLIT_>::p;
+  using LogitTiles<F>::p;
   float top, sum;
   int target;
-  __device__ explicit StatOp(const LogitParams& q, const TileMaps& m) : LogitTiles<SPLIT_>(q, m) {}
+  __device__ explicit StatOp(const LogitParams& q, const TileMaps& m) : LogitTiles<F>(q, m) {}
   __device__ __forceinline__ void begin(const Tile&, int row0, int, int lane) {
     top = -INFINITY;
     sum = 0.f;
     target = row0 + lane < this->rows ? __ldg(p.target + row0 + lane) : -1;
   }
-  static constexpr int W = LONG ? 16 : LogitTiles<SPLIT_>::W;
+  static constexpr int W = LONG ? 16 : LogitTiles<F>::W;
   __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[W], uint8_t*, int lane) {
     if (col0 >= p.vocab) return;
     if (col0 + W > p.vocab) {
@@ -258,7 +258,6 @@ struct StatOp : LogitTiles<SPLIT_> {
     }
   }
   __device__ __forceinline__ void end(const Tile& t, int row, int part) {
-    typedef TileForm<SPLIT_> F;
     if (row < this->rows) p.parts[(long long)(t.n0 / F::BN * F::PARTS + part) * p.row_pitch + row] = make_float2(top, sum);
   }
 };
@@ -266,18 +265,18 @@ struct StatOp : LogitTiles<SPLIT_> {
 // d of a piece, zeros in rows and columns that fill up tiles. What an element takes here bounds the kernel when width is small
 // (1024 and less: 8 us per tile before stores went by TMA and the target's column was a branch of its own, 5.8 us
 // of products), so it is one FMA, one exponential, one product and half a conversion.
-template <bool SPLIT_>
-struct GradOp : LogitTiles<SPLIT_> {
+template <class F>
+struct GradOp : LogitTiles<F> {
   typedef LogitParams Params;
-  static constexpr bool LONG = SPLIT_;
-  static constexpr bool STORES = !SPLIT_;
-  using LogitTiles<SPLIT_>::p;
+  static constexpr bool LONG = F::SPLIT;
+  static constexpr bool STORES = !F::SPLIT;
+  using LogitTiles<F>::p;
   const CUtensorMap* map;
   float top, by, to;
   int target;
   bool in;
-  __device__ explicit GradOp(const LogitParams& q, const TileMaps& m) : LogitTiles<SPLIT_>(q, m), map(&m.c) {
-    to = SPLIT_ ? (float)(1 << D_EXP) : 1.f;  // the caller's scale comes behind the products: -1 at an unlikely target is exact
+  __device__ explicit GradOp(const LogitParams& q, const TileMaps& m) : LogitTiles<F>(q, m), map(&m.c) {
+    to = F::SPLIT ? (float)(1 << D_EXP) : 1.f;  // the caller's scale comes behind the products: -1 at an unlikely target is exact
   }
   __device__ __forceinline__ void begin(const Tile&, int row0, int, int lane) {
     const int row = row0 + lane;
@@ -287,7 +286,7 @@ struct GradOp : LogitTiles<SPLIT_> {
     by = st.y * to;
     target = in ? __ldg(p.target + row) - p.v_begin : -1;
   }
-  static constexpr int W = LogitTiles<SPLIT_>::W;
+  static constexpr int W = LogitTiles<F>::W;
   __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[W], uint8_t* stage, int lane) {
 #pragma unroll
     for (int j = 0; j < W; ++j) v[j] = ex2(fmaf(v[j], this->unit, -top)) * by;
@@ -301,7 +300,7 @@ struct GradOp : LogitTiles<SPLIT_> {
       for (int j = 0; j < W; ++j)
         if (!in || col0 + j >= p.v_count) v[j] = 0.f;
     }
-    if constexpr (SPLIT_) {
+    if constexpr (F::SPLIT) {
       by_rows(row0, col0, v, stage, lane, [&](int, int r, int c, const float4& x) {
         store_pair(reinterpret_cast<__half*>(p.d_hi), reinterpret_cast<__half*>(p.d_lo), (long long)r * p.ld_d + c, x);
       });
@@ -491,19 +490,19 @@ struct HiddenOp {
 };
 
 // dw of a piece = d' h.
-template <bool SPLIT_>
+template <class F>
 struct WeightOp {
   typedef ProductParams Params;
-  typedef TileForm<SPLIT_> Form;
-  static constexpr bool SPLIT = SPLIT_, STORES = !SPLIT_;
-  static constexpr bool LONG = SPLIT_;
-  static constexpr int SUM = XENT_SUM, BN = TileForm<SPLIT_>::BN;
+  typedef F Form;
+  static constexpr bool SPLIT = F::SPLIT, STORES = !SPLIT;
+  static constexpr bool LONG = SPLIT;
+  static constexpr int SUM = XENT_SUM, BN = F::BN;
   const ProductParams& p;
   const CUtensorMap* map;
   int m_blocks, n_blocks, kblocks;
   float unit;
   __device__ explicit WeightOp(const ProductParams& q, const TileMaps& m) : p(q), map(&m.c) {
-    m_blocks = (p.v_count + TILE_M - 1) / TILE_M;
+    m_blocks = (p.v_count + F::M - 1) / F::M;
     n_blocks = (p.width + BN - 1) / BN;
     kblocks = max(1, (int)((p.meta->rows + TILE_K - 1) / TILE_K));  // without rows: zeros, as they are stored
     unit = SPLIT ? p.scale * pow2(-D_EXP) * pow2(-up_exp(p.meta->max_h)) : p.scale;
@@ -511,7 +510,7 @@ struct WeightOp {
   __device__ int tiles() const { return m_blocks * n_blocks; }
   __device__ Tile tile(int t) const {
     Tile r;
-    r.m0 = t / n_blocks * TILE_M;
+    r.m0 = t / n_blocks * F::M;
     r.n0 = t % n_blocks * BN;
     r.a_mn = r.m0;
     r.b_mn = r.n0;
@@ -521,9 +520,9 @@ struct WeightOp {
     return r;
   }
   __device__ __forceinline__ void begin(const Tile&, int, int, int) {}
-  static constexpr int W = TileForm<SPLIT_>::CHUNK;
+  static constexpr int W = F::CHUNK;
   __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[W], uint8_t* stage, int lane) {
-    if constexpr (!SPLIT_) {
+    if constexpr (!SPLIT) {
       if (p.by_tma) {  // pieces are whole 256-row tiles but for the last one, whose rows the map ends with
         uint32_t w[16];
 #pragma unroll
@@ -606,7 +605,18 @@ struct Sizes {
   long long parts;           // lists per row
   long long piece;           // columns of d
   bool split, copy_w;
+  bool one;                  // logits by single CTAs
 };
+constexpr int MOST_PAIRS = 74;  // 148 SMs
+template <class F>
+long long tiles_of(long long m, long long n) { return (m + F::M - 1) / F::M * ((n + F::BN - 1) / F::BN); }
+template <class F>
+void logit_sizes(Sizes* z, size_t rows, size_t vocab) {  // F: single CTAs, which take over when each has one tile at most
+  typedef TileForm<F::SPLIT> Pairs;
+  z->one = tiles_of<F>(rows, vocab) <= 2 * MOST_PAIRS;
+  const int bn = z->one ? F::BN : Pairs::BN;
+  z->parts = F::PARTS * (((long long)vocab + bn - 1) / bn);
+}
 Sizes sizes_of(size_t rows, size_t width, size_t vocab, int dtype, int grads, const void* w, size_t ldw) {
   Sizes z;
   z.split = dtype == B2_DTYPE_F32;
@@ -614,8 +624,8 @@ Sizes sizes_of(size_t rows, size_t width, size_t vocab, int dtype, int grads, co
   z.copy_w = z.split || reinterpret_cast<uintptr_t>(w) % 16 != 0 || ldw % 8 != 0;
   z.rows_up = (long long)(rows + TILE_M - 1) / TILE_M * TILE_M;
   z.pitch = (long long)(width + 63) / 64 * 64;
-  const int bn = z.split ? TileForm<true>::BN : TileForm<false>::BN, shares = z.split ? TileForm<true>::PARTS : TileForm<false>::PARTS;
-  z.parts = shares * (((long long)vocab + bn - 1) / bn);
+  if (z.split) logit_sizes<TileForm<true, true>>(&z, rows, vocab);
+  else logit_sizes<TileForm<false, true>>(&z, rows, vocab);
   z.piece = 0;
   if (grads) {
     // A piece of d should be in the L2 cache when the two products read it, and its 256-wide column blocks should go evenly
@@ -637,7 +647,6 @@ struct Space {
   uint16_t *h_hi, *h_lo, *w_hi, *w_lo, *d_hi, *d_lo;
   float *acc, *slots;
 };
-constexpr int MOST_PAIRS = 74;  // 148 SMs
 size_t space_of(const Sizes& z, size_t rows, size_t vocab, int grads, void* base, Space* s) {
   Carver c(base);
   const size_t lo = z.split ? 1 : 0;
@@ -679,7 +688,9 @@ struct XentCall {
 template <bool SPLIT>
 int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStream_t st) {
   typedef typename std::conditional<SPLIT, float, __nv_bfloat16>::type T;
-  constexpr int BN = TileForm<SPLIT>::BN;
+  typedef TileForm<SPLIT> Pairs;
+  typedef TileForm<SPLIT, true> One;
+  const char* who = "b2_xent";
   const int rows = (int)c.rows, width = (int)c.width, vocab = (int)c.vocab, pitch = (int)z.pitch;
   const T *h = static_cast<const T*>(c.h), *w = static_cast<const T*>(c.w);
   Chain chain(st);
@@ -697,14 +708,13 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
   if (z.copy_w)
     chain.launch(copy_rows_kernel<T, false>, dim3(blocks(vocab)), 256, 0, 0, w, c.ldw, (const int*)nullptr, vocab, width, pitch, s.meta,
                  s.w_hi, s.w_lo);
-  int rc = launch_error(chain.err, "b2_xent");
+  int rc = launch_error(chain.err, who);
   if (rc != B2_OK) return rc;
 
   const TileOperand h_k{s.h_hi, s.h_lo, z.rows_up, pitch, pitch, false}, h_mn{s.h_hi, s.h_lo, pitch, z.rows_up, pitch, true};
   const void* w_hi = z.copy_w ? (const void*)s.w_hi : c.w;
   const long long w_width = z.copy_w ? pitch : width, w_ld = z.copy_w ? pitch : (long long)c.ldw;
   const TileOperand w_k{w_hi, s.w_lo, vocab, w_width, w_ld, false}, w_mn{w_hi, s.w_lo, w_width, vocab, w_ld, true};
-  const long long m_blocks = z.rows_up / TILE_M;
   LogitParams lp{};
   lp.meta = s.meta;
   lp.vocab = vocab;
@@ -718,14 +728,14 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
   lp.d_hi = s.d_hi;
   lp.d_lo = s.d_lo;
   lp.ld_d = z.piece;
-  const long long stat_tiles = m_blocks * ((vocab + BN - 1) / BN);
-  rc = !SPLIT && lp.kblocks > StatOp<false, true>::SUM
-           ? tile_launch<StatOp<SPLIT, !SPLIT>>("b2_xent", h_k, w_k, nullptr, lp, !SPLIT, stat_tiles, sms, chain)
-           : tile_launch<StatOp<SPLIT, false>>("b2_xent", h_k, w_k, nullptr, lp, !SPLIT, stat_tiles, sms, chain);
+  const bool sums = !SPLIT && lp.kblocks > StatOp<Pairs, true>::SUM;
+  auto stat = z.one ? (sums ? tile_launch<StatOp<One, !SPLIT>> : tile_launch<StatOp<One, false>>)
+                    : (sums ? tile_launch<StatOp<Pairs, !SPLIT>> : tile_launch<StatOp<Pairs, false>>);
+  rc = stat(who, h_k, w_k, nullptr, lp, !SPLIT, z.one ? tiles_of<One>(rows, vocab) : tiles_of<Pairs>(rows, vocab), sms, chain);
   if (rc != B2_OK) return rc;
   chain.launch(join_rows_kernel, dim3((rows + 31) / 32), 256, 0, 0, s.parts, z.rows_up, (int)z.parts, s.meta, s.target_logit, s.row_of, s.row_stat,
                c.row_loss);
-  rc = launch_error(chain.err, "b2_xent");
+  rc = launch_error(chain.err, who);
   if (rc != B2_OK || (!c.dh && !c.dw)) return rc;
 
   ProductParams pp{};
@@ -745,22 +755,25 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
   pp.by_tma = !SPLIT && reinterpret_cast<uintptr_t>(c.dw) % 16 == 0 && c.ld_dw % 8 == 0 && width % 8 == 0;
   const TileResult dw_out{c.dw, vocab, width, (long long)c.ld_dw};
   const TileResult d_out{s.d_hi, z.rows_up, z.piece, z.piece};
-  const long long w_blocks = (width + BN - 1) / BN;
   for (int v0 = 0; v0 < vocab; v0 += (int)z.piece) {
     const int count = vocab - v0 < z.piece ? vocab - v0 : (int)z.piece;
     lp.v_begin = pp.v_begin = v0;
     lp.v_count = pp.v_count = count;
     pp.first = v0 == 0;
-    rc = tile_launch<GradOp<SPLIT>>("b2_xent", h_k, w_k, SPLIT ? nullptr : &d_out, lp, !SPLIT, m_blocks * ((count + BN - 1) / BN), sms, chain);
-    if (rc == B2_OK && c.dh) rc = tile_launch<HiddenOp<SPLIT>>("b2_xent", d_k, w_mn, nullptr, pp, !SPLIT, pp.pairs, sms, chain);
-    if (rc == B2_OK && c.dw)
-      rc = tile_launch<WeightOp<SPLIT>>("b2_xent", d_mn, h_mn, pp.by_tma ? &dw_out : nullptr, pp, !SPLIT, (count + TILE_M - 1) / TILE_M * w_blocks, sms, chain);
+    rc = (z.one ? tile_launch<GradOp<One>> : tile_launch<GradOp<Pairs>>)(who, h_k, w_k, SPLIT ? nullptr : &d_out, lp, !SPLIT,
+                                                                         z.one ? tiles_of<One>(rows, count) : tiles_of<Pairs>(rows, count), sms, chain);
+    if (rc == B2_OK && c.dh) rc = tile_launch<HiddenOp<SPLIT>>(who, d_k, w_mn, nullptr, pp, !SPLIT, pp.pairs, sms, chain);
+    if (rc == B2_OK && c.dw) {
+      const bool one = tiles_of<One>(count, width) <= sms;
+      rc = (one ? tile_launch<WeightOp<One>> : tile_launch<WeightOp<Pairs>>)(who, d_mn, h_mn, pp.by_tma ? &dw_out : nullptr, pp, !SPLIT,
+                                                                             one ? tiles_of<One>(count, width) : tiles_of<Pairs>(count, width), sms, chain);
+    }
     if (rc != B2_OK) return rc;
   }
   if (c.dh) {
     const int vec = c.ld_dh % 4 == 0 && reinterpret_cast<uintptr_t>(c.dh) % (4 * sizeof(T)) == 0;
     chain.launch(spread_rows_kernel<T>, dim3(blocks(rows)), 256, 0, 0, pp, s.slot_of, rows, vec, static_cast<T*>(c.dh), c.ld_dh);
-    rc = launch_error(chain.err, "b2_xent");
+    rc = launch_error(chain.err, who);
   }
   return rc;
 }

@@ -1,17 +1,18 @@
-// Softmax cross entropy behind a linear layer as wide as a vocabulary, with its gradients, without keeping the logits:
+// Softmax cross entropy behind a linear layer as wide as a vocabulary, with its gradients, without keeping more than 512 MB of logits:
 //
 //   x_iv = h_i . w_v      l_i = log sum_v exp(x_iv) - x_i,t_i      d_iv = exp(x_iv) / sum_u exp(x_iu) - [v = t_i]
 //   dh_i = scale sum_v d_iv w_v      dw_v = scale sum_i d_iv h_i
 //
-// Work: 2 R V F operations for the losses and 6 R V F with gradients; 8 R V F in this form, because the logits are
-// computed a second time when their row's maximum and sum are known, instead of R x V of them being kept.
+// Work: 2 R V F operations for the losses and 6 R V F with gradients; 8 R V F in this form where the logits are
+// computed a second time when their row's maximum and sum are known, instead of R x V of them being kept (keeps_logits).
 // It is bound by the tensor cores (tile kernels of lm_tile.cuh) unless R is small, when reading w is what it takes.
 //
 //   1. Rows without a target are left out: the others' numbers are listed in order, their h copied one after another.
 //      So such a row costs nothing, and nothing in it (a NaN, say) reaches dw.
 //   2. Logits, 256 x 256 at a time; each row's maximum and sum over a tile's half go to a list.
 //   3. The lists give each row's maximum and sum, and the loss.
-//   4. Per piece of the vocabulary: logits again, d to a buffer of R x piece; dh += d w; dw of the piece = d' h.
+//   4. Per piece of the vocabulary: d from logits that are kept or computed again to a buffer of R x piece; dh += d w; dw of the
+//      piece = d' h.
 //
 // Precision: bf16 matrices are multiplied as they are, with fp32 sums; d is rounded to bf16 once, as the
 // gradients are in the end. fp32 matrices are
@@ -179,6 +180,8 @@ struct LogitParams {
   const float2* row_stat;  // maximum and 1 / sum of whole rows
   uint16_t *d_hi, *d_lo;
   long long ld_d;
+  float* x;  // logits as they are summed, where they are kept
+  long long ld_x;
 };
 
 template <class F>
@@ -216,7 +219,7 @@ struct LogitTiles {
 // Maximum and sum of exponentials of a row over the columns of one warp, and the target's logit. LONG: for more than 16 k-blocks,
 // whose sums the tensor core would leave too small (bf16, width 2048: losses 1.0e-6 off, with sums of 16 added in fp32 0.5e-6, in the
 // same time).
-template <class F, bool LONG_>
+template <class F, bool LONG_, bool KEEP>
 struct StatOp : LogitTiles<F> {
   typedef LogitParams Params;
   static constexpr bool LONG = F::SPLIT || LONG_;
@@ -232,8 +235,12 @@ struct StatOp : LogitTiles<F> {
     target = row0 + lane < this->rows ? __ldg(p.target + row0 + lane) : -1;
   }
   static constexpr int W = LONG ? 16 : LogitTiles<F>::W;
-  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[W], uint8_t*, int lane) {
+  __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[W], uint8_t* stage, int lane) {
     if (col0 >= p.vocab) return;
+    if (KEEP)
+      by_rows(row0, col0, v, stage, lane, [&](int, int r, int c, const float4& x) {
+        if (r < this->rows && c < p.vocab) *reinterpret_cast<float4*>(p.x + r * p.ld_x + c) = x;
+      });
     if (col0 + W > p.vocab) {
 #pragma unroll
       for (int j = 0; j < W; ++j)
@@ -313,6 +320,48 @@ struct GradOp : LogitTiles<F> {
   }
   __device__ __forceinline__ void end(const Tile&, int, int) {}
 };
+
+// The same d from kept logits, eight neighbouring elements per thread, zeros up to whole k-blocks of the products that read it.
+template <bool SPLIT>
+__global__ void __launch_bounds__(256) kept_kernel(const LogitParams p) {
+  after_previous();
+  let_next_start();
+  const Meta meta = *p.meta;
+  const unsigned int rows = meta.rows, rows_up = max(1u, (rows + TILE_K - 1) / TILE_K) * TILE_K;
+  const unsigned int per_row = (unsigned int)((p.v_count + TILE_K - 1) / TILE_K * (TILE_K / 8)), all = rows_up * per_row;
+  const float unit = SPLIT ? LOG2E * pow2(-up_exp(meta.max_h)) * pow2(-up_exp(meta.max_w)) : LOG2E, to = SPLIT ? (float)(1 << D_EXP) : 1.f;
+#pragma unroll 2
+  for (unsigned int i = blockIdx.x * 256 + threadIdx.x; i < all; i += gridDim.x * 256) {
+    const unsigned int r = i / per_row;
+    const int c = (int)(i - r * per_row) * 8;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (r < rows) {
+      const float* from = p.x + r * p.ld_x + p.v_begin + c;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (c + 4 * j < p.v_count) *reinterpret_cast<float4*>(v + 4 * j) = *reinterpret_cast<const float4*>(from + 4 * j);
+      const float2 st = __ldg(p.row_stat + r);
+      const int target = __ldg(p.target + r) - p.v_begin - c;
+      const float by = st.y * to;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = ex2(fmaf(v[j], unit, -st.x)) * by;
+        v[j] -= j == target ? to : 0.f;
+        if (c + j >= p.v_count) v[j] = 0.f;
+      }
+    }
+    const long long at = r * p.ld_d + c;
+    if (SPLIT) {
+      __half hi[8], lo[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) split_half(v[j], hi[j], lo[j]);
+      *reinterpret_cast<uint4*>(p.d_hi + at) = *reinterpret_cast<const uint4*>(hi);
+      *reinterpret_cast<uint4*>(p.d_lo + at) = *reinterpret_cast<const uint4*>(lo);
+    } else {
+      *reinterpret_cast<uint4*>(p.d_hi + at) = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+    }
+  }
+}
 
 // Whole rows' maximum and sum from the lists, and the losses. Eight warps share 32 rows' lists.
 __global__ void __launch_bounds__(256) join_rows_kernel(const float2* __restrict__ parts, long long row_pitch, int count,
@@ -606,6 +655,8 @@ struct Sizes {
   long long piece;           // columns of d
   bool split, copy_w;
   bool one;                  // logits by single CTAs
+  bool keep;                 // logits are kept for d
+  long long ld_x;
 };
 constexpr int MOST_PAIRS = 74;  // 148 SMs
 template <class F>
@@ -617,6 +668,13 @@ void logit_sizes(Sizes* z, size_t rows, size_t vocab) {  // F: single CTAs, whic
   const int bn = z->one ? F::BN : Pairs::BN;
   z->parts = F::PARTS * (((long long)vocab + bn - 1) / bn);
 }
+// Logits that are kept cost their bytes twice, others 2 F operations each again. What stays in the L2 cache is kept (1024 x 512 x 8192 in
+// fp32 140 -> 125 us, 16 x 2048 x 65536 in bf16 251 -> 217); beyond it the operations cost more with three MMAs or great widths (2048 x
+// 1024 x 32768 in fp32 1 550 -> 1 340 us, 1024 x 4096 x 32768 in bf16 923 -> 800) and less with small ones (bf16: 2048 x 512 x 32768 241 -> 303,
+// 2048 x 768 x 32768 387 -> 415, 2048 x 1024 x 32768 474 -> 480). 8192 x 2048 x 65536 would gain 4 % and take 2 GB.
+bool keeps_logits(long long bytes, size_t width, bool split) {
+  return bytes <= 64ll << 20 || (bytes <= 512ll << 20 && width >= (split ? 256 : 2048));
+}
 Sizes sizes_of(size_t rows, size_t width, size_t vocab, int dtype, int grads, const void* w, size_t ldw) {
   Sizes z;
   z.split = dtype == B2_DTYPE_F32;
@@ -627,6 +685,8 @@ Sizes sizes_of(size_t rows, size_t width, size_t vocab, int dtype, int grads, co
   if (z.split) logit_sizes<TileForm<true, true>>(&z, rows, vocab);
   else logit_sizes<TileForm<false, true>>(&z, rows, vocab);
   z.piece = 0;
+  z.ld_x = ((long long)vocab + 3) / 4 * 4;
+  z.keep = grads && keeps_logits((long long)rows * z.ld_x * 4, width, z.split);
   if (grads) {
     // A piece of d should be in the L2 cache when the two products read it, and its 256-wide column blocks should go evenly
     // over 74 pairs: 37 of them do for any number of row blocks.
@@ -645,7 +705,7 @@ struct Space {
   float* target_logit;
   float2 *row_stat, *parts;
   uint16_t *h_hi, *h_lo, *w_hi, *w_lo, *d_hi, *d_lo;
-  float *acc, *slots;
+  float *acc, *slots, *x;
 };
 size_t space_of(const Sizes& z, size_t rows, size_t vocab, int grads, void* base, Space* s) {
   Carver c(base);
@@ -665,6 +725,7 @@ size_t space_of(const Sizes& z, size_t rows, size_t vocab, int grads, void* base
   s->d_lo = c.take<uint16_t>(lo * z.rows_up * z.piece);
   s->acc = c.take<float>(grads ? z.rows_up * z.pitch : 0);
   s->slots = c.take<float>(grads ? 2ll * MOST_PAIRS * TILE_M * (z.split ? 128 : 256) : 0);
+  s->x = c.take<float>(z.keep ? rows * z.ld_x : 0);
   return c.used;
 }
 
@@ -728,9 +789,17 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
   lp.d_hi = s.d_hi;
   lp.d_lo = s.d_lo;
   lp.ld_d = z.piece;
-  const bool sums = !SPLIT && lp.kblocks > StatOp<Pairs, true>::SUM;
-  auto stat = z.one ? (sums ? tile_launch<StatOp<One, !SPLIT>> : tile_launch<StatOp<One, false>>)
-                    : (sums ? tile_launch<StatOp<Pairs, !SPLIT>> : tile_launch<StatOp<Pairs, false>>);
+  lp.x = s.x;
+  lp.ld_x = z.ld_x;
+  const bool sums = !SPLIT && lp.kblocks > StatOp<Pairs, true, false>::SUM;
+  auto stat_of = [&](auto form, auto keep) {
+    typedef decltype(form) F;
+    constexpr bool KEEP = decltype(keep)::value;
+    return sums ? tile_launch<StatOp<F, !SPLIT, KEEP>> : tile_launch<StatOp<F, false, KEEP>>;
+  };
+  const std::true_type yes;
+  const std::false_type no;
+  auto stat = z.one ? (z.keep ? stat_of(One(), yes) : stat_of(One(), no)) : (z.keep ? stat_of(Pairs(), yes) : stat_of(Pairs(), no));
   rc = stat(who, h_k, w_k, nullptr, lp, !SPLIT, z.one ? tiles_of<One>(rows, vocab) : tiles_of<Pairs>(rows, vocab), sms, chain);
   if (rc != B2_OK) return rc;
   chain.launch(join_rows_kernel, dim3((rows + 31) / 32), 256, 0, 0, s.parts, z.rows_up, (int)z.parts, s.meta, s.target_logit, s.row_of, s.row_stat,
@@ -760,8 +829,13 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
     lp.v_begin = pp.v_begin = v0;
     lp.v_count = pp.v_count = count;
     pp.first = v0 == 0;
-    rc = (z.one ? tile_launch<GradOp<One>> : tile_launch<GradOp<Pairs>>)(who, h_k, w_k, SPLIT ? nullptr : &d_out, lp, !SPLIT,
-                                                                         z.one ? tiles_of<One>(rows, count) : tiles_of<Pairs>(rows, count), sms, chain);
+    if (z.keep) {
+      const long long r = (rows + TILE_K - 1) / TILE_K * TILE_K, n = (count + TILE_K - 1) / TILE_K * TILE_K;
+      chain.launch(kept_kernel<SPLIT>, dim3(blocks((r * n / 8 + 255) / 256)), 256, 0, 0, lp);
+      rc = launch_error(chain.err, who);
+    } else {
+      rc = tile_launch<GradOp<Pairs>>(who, h_k, w_k, SPLIT ? nullptr : &d_out, lp, !SPLIT, tiles_of<Pairs>(rows, count), sms, chain);
+    }
     if (rc == B2_OK && c.dh) rc = tile_launch<HiddenOp<SPLIT>>(who, d_k, w_mn, nullptr, pp, !SPLIT, pp.pairs, sms, chain);
     if (rc == B2_OK && c.dw) {
       const bool one = tiles_of<One>(count, width) <= sms;

@@ -127,8 +127,8 @@ def embed_grad(tokens, dout, vocab, scale=1.0, out=None):
 
 def xent(h, w, targets, scale=1.0, grad=True, dh=None, dw=None):
     """Losses of `h @ w.T` against `targets`, one float32 per row (0 for padding); with `grad` also the gradients of
-    `scale * losses.sum()` with respect to h and w: (losses, dh, dw). `dh` and `dw` may be given to be written to. The logits
-    are never kept (see b2_xent in include/b200mlp.h)."""
+    `scale * losses.sum()` with respect to h and w: (losses, dh, dw). `dh` and `dw` may be given to be written to. No more
+    than 512 MB of logits are held (see b2_xent in include/b200mlp.h)."""
     ph, ldh = _matrix("h", h)
     rows, width = h.shape
     device, dtype = h.device, h.dtype

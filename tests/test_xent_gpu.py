@@ -109,6 +109,17 @@ def test_several_pieces(lm, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,rows,width,vocab", [
+    ("bf16", 40, 32, 400001), ("fp32", 40, 32, 200001),  # few rows: logits are kept, d goes in pieces
+    ("bf16", 600, 2048, 30001), ("fp32", 300, 264, 60002),  # kept although they are more than the L2 cache should hold
+    ("bf16", 3000, 200, 6001), ("fp32", 3000, 200, 6003)])  # too many: computed a second time
+def test_logits_kept_or_computed_again(lm, dtype, rows, width, vocab):
+    h, w, t = _case(rows, width, vocab, dtype)
+    _check(h, w, t, 1.0, lm.xent(h, w, t), dtype)
+    lm.sync()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_rows_without_a_target(lm, dtype):
     """They cost nothing and nothing of them gets out, not even NaN; a call of such rows alone gives zeros."""

@@ -109,6 +109,17 @@ def test_several_pieces(lm, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows,width,vocab", [(1200, 72, 90), (32768, 8, 5), (32769, 24, 70), (70001, 40, 33)])
+def test_many_rows(lm, dtype, rows, width, vocab):
+    """More rows than blocks that list them, and than every block counts by itself."""
+    h, w, t = _case(rows, width, vocab, dtype)
+    t[: rows // 3] = -100
+    _check(h, w, t, 1.0, lm.xent(h, w, t), dtype)
+    lm.sync()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,rows,width,vocab", [
     ("bf16", 40, 32, 400001), ("fp32", 40, 32, 200001),  # few rows: logits are kept, d goes in pieces
     ("bf16", 600, 2048, 30001), ("fp32", 300, 264, 60002),  # kept although they are more than the L2 cache should hold

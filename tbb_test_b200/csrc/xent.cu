@@ -775,10 +775,11 @@ Sizes sizes_of(size_t rows, size_t width, size_t vocab, int dtype, int grads, co
   z.ld_x = ((long long)vocab + 3) / 4 * 4;
   z.keep = grads && keeps_logits((long long)rows * z.ld_x * 4, width, z.split);
   if (grads) {
-    // A piece of d should be in the L2 cache when the two products read it, and its 256-wide column blocks should go evenly
-    // over 74 pairs: 37 of them do for any number of row blocks.
+    // Few pieces: each has three kernels to fill and drain, which costs more than reading d from HBM (8192 x 2048 x 65536 with pieces of 160
+    // MB 6.05 ms, 320 MB 5.94, 640 MB 5.86, 80 MB 6.5; 2048 x 1024 x 65536 948, 906 and 832 us). The 256-wide column blocks of a piece should go
+    // evenly over 74 pairs: 37 of them do for any number of row blocks.
     const long long all = ((long long)vocab + 255) / 256 * 256, unit = 37 * 256;
-    long long fit = (160ll << 20) / (z.rows_up * (z.split ? 4 : 2));
+    long long fit = (640ll << 20) / (z.rows_up * (z.split ? 4 : 2));
     if (fit >= unit) fit = fit / unit * unit;
     else fit = fit / 256 * 256;
     if (fit < 1024) fit = 1024;

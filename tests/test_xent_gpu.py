@@ -102,7 +102,7 @@ def test_losses_and_gradients(lm, dtype, rows, width, vocab, ldh, ldw, offset):
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_several_pieces(lm, dtype):
     """More rows x vocabulary than one piece of the logits' gradients holds."""
-    rows, vocab = (6000, 30001) if dtype == "bf16" else (3000, 30001)
+    rows, vocab = (12000, 30001) if dtype == "bf16" else (6000, 30001)
     h, w, t = _case(rows, 64, vocab, dtype)
     _check(h, w, t, 1.0, lm.xent(h, w, t), dtype)
     lm.sync()
@@ -121,7 +121,7 @@ def test_many_rows(lm, dtype, rows, width, vocab):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,rows,width,vocab", [
-    ("bf16", 40, 32, 400001), ("fp32", 40, 32, 200001),  # few rows: logits are kept, d goes in pieces
+    ("bf16", 10, 8, 1400001), ("fp32", 20, 8, 700001),  # few rows: logits are kept, d goes in pieces
     ("bf16", 600, 2048, 30001), ("fp32", 300, 264, 60002),  # kept although they are more than the L2 cache should hold
     ("bf16", 3000, 200, 6001), ("fp32", 3000, 200, 6003)])  # too many: computed a second time
 def test_logits_kept_or_computed_again(lm, dtype, rows, width, vocab):

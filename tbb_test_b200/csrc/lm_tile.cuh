@@ -16,7 +16,7 @@
 //           accumulator (about 2e-8 of the sum each time, and always towards zero), so a sum is handed over every
 //           Op::SUM k-blocks and added up in fp32 registers, rounded to nearest.
 //
-// Where there are fewer tiles than SMs, single CTAs (ONE) with tcgen05.mma.cta_group::1 and tiles of a quarter of the size take less
+// Where there are no more tiles than SMs, single CTAs (ONE) with tcgen05.mma.cta_group::1 and tiles of a quarter of the size take less
 // time: more SMs have work, and a call's products, which wait for one another, start and end sooner without a cluster (15 products of 256 x
 // 256 x 256: 144 -> 99 us; of 1024 x 1024 x 1024 249 -> 184). With more tiles pairs do, which read half of B's slab each: 1536 x 1536 in
 // two rounds of single CTAs 393 us, in one of pairs 324. The plain form's single CTAs take 128 x 128.
@@ -229,6 +229,13 @@ __global__ void __launch_bounds__(Op::Form::BOUND, 1) tile_kernel(const __grid_c
           for (int ks = 0; ks < TILE_K / 16; ++ks) {
             const uint64_t ad = a_tmpl + off + (uint64_t)(ks * a_step), bd = b_tmpl + off + (uint64_t)(ks * b_step);
             const uint32_t go = first && ks == 0 ? 0u : 1u;
+            if (SPLIT && !PAIR) {
+              // B's halves lie behind one another, as their results do: one MMA of twice the columns reads hi once for both. Shared memory is
+              // what bounds these tiles (1024 x 1024: 185 -> 164 us per update). In a pair each CTA has half of either.
+              mma_issue<false, PAIR>(d, ad, bd, idesc + ((uint32_t)(F::BN >> 3) << 17), go);
+              mma_issue<false, PAIR>(d + F::BN, ad + (F::A_BYTES >> 4), bd, idesc, 1u);
+              continue;
+            }
             mma_issue<false, PAIR>(d, ad, bd, idesc, go);
             if (SPLIT) {
               mma_issue<false, PAIR>(d + F::BN, ad, bd + (F::B_BYTES >> 4), idesc, go);

@@ -405,14 +405,20 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
   int rc = launch_error(chain.err, who);
   const bool wide = rows <= cols;
   const long long x_rows = (long long)z.rows_up * count, a_rows = (long long)z.side * count;
-  // Tiles of a symmetric and of a full product, in tiles of bm rows; single CTAs where each has one at most.
+  // Tiles of a symmetric and of a full product, in tiles of bm rows. Single CTAs or pairs: what shared memory takes to be filled and read for a
+  // k-block (832 and 960 clocks), times the rounds of tiles, and 3 us for a launch of clusters.
   auto symmetric = [&](int bm) {
     const long long m = (z.side + bm - 1) / bm, n = (z.side + bm / 2 - 1) / (bm / 2);
     return (m * n - m * (m - 1)) * count;
   };
   auto full = [&](int bm) { return (long long)((z.rows_up + bm - 1) / bm) * ((z.cols_up + bm / 2 - 1) / (bm / 2)) * count; };
-  const bool half_one = symmetric(128) <= sms, full_one = full(128) <= sms;
-  const long long half_tiles = symmetric(half_one ? 128 : 256), tiles = full(full_one ? 128 : 256);
+  auto one_is_less = [&](long long one, long long pairs, int kblocks) {
+    return (one + sms - 1) / sms * 832 * kblocks <= (pairs + sms / 2 - 1) / (sms / 2) * 960 * kblocks + 6000;
+  };
+  const int k_a = (wide ? z.cols_up : z.rows_up) / TILE_K, k_b = z.side / TILE_K;
+  const bool a_one = one_is_less(symmetric(128), symmetric(256), k_a), p_one = one_is_less(symmetric(128), symmetric(256), k_b),
+             full_one = one_is_less(full(128), full(256), k_b);
+  const long long a_tiles = symmetric(a_one ? 128 : 256), p_tiles = symmetric(p_one ? 128 : 256), tiles = full(full_one ? 128 : 256);
   const TileOperand a_op{s.a_hi, s.a_lo, a_rows, z.side, z.side, false}, p_op{s.p_hi, s.p_lo, a_rows, z.side, z.side, false};
   int at = 0;
   for (int k = 0; k < o.steps && rc == B2_OK; ++k, at ^= 1) {
@@ -421,22 +427,22 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
     SymmetricParams q{};
     q.side = z.side;
     q.count = count;
-    q.kblocks = (wide ? z.cols_up : z.rows_up) / TILE_K;
+    q.kblocks = k_a;
     q.a_step = z.rows_up;
     q.steps_k = !wide;
     q.to_hi = s.a_hi;
     q.to_lo = s.a_lo;
     const TileOperand& x = wide ? x_k : x_mn;
-    rc = (half_one ? tile_launch<SymmetricOp<false, true>> : tile_launch<SymmetricOp<false, false>>)(who, x, x, nullptr, q, false, half_tiles, sms, chain);
+    rc = (a_one ? tile_launch<SymmetricOp<false, true>> : tile_launch<SymmetricOp<false, false>>)(who, x, x, nullptr, q, false, a_tiles, sms, chain);
     if (rc != B2_OK) return rc;
-    q.kblocks = z.side / TILE_K;
+    q.kblocks = k_b;
     q.a_step = z.side;
     q.steps_k = 0;
     q.a_hi = s.a_hi;
     q.a_lo = s.a_lo;
     q.to_hi = s.p_hi;
     q.to_lo = s.p_lo;
-    rc = (half_one ? tile_launch<SymmetricOp<true, true>> : tile_launch<SymmetricOp<true, false>>)(who, a_op, a_op, nullptr, q, false, half_tiles, sms, chain);
+    rc = (p_one ? tile_launch<SymmetricOp<true, true>> : tile_launch<SymmetricOp<true, false>>)(who, a_op, a_op, nullptr, q, false, p_tiles, sms, chain);
     if (rc != B2_OK) return rc;
     NextParams n{};
     n.list = list;
@@ -445,7 +451,7 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
     n.rows_up = z.rows_up;
     n.cols_up = z.cols_up;
     n.count = count;
-    n.kblocks = z.side / TILE_K;
+    n.kblocks = k_b;
     n.wide = wide;
     n.to_hi = s.x_hi[at ^ 1];
     n.to_lo = s.x_lo[at ^ 1];

@@ -156,6 +156,8 @@ __global__ void __launch_bounds__(256) normalise_kernel(const __grid_constant__ 
 
 // ------------------------------------------------------------------ products
 
+constexpr float A_UNIT = A_UP / (X_UP * X_UP);  // of sums of x x'
+
 // Symmetric results, side x side per matrix: a = x x' (middle 0), or A I + B a + C a a from a a (middle 1).
 struct SymmetricParams {
   int side, count, kblocks;
@@ -163,11 +165,15 @@ struct SymmetricParams {
   int steps_k;               // 1: matrices lie behind one another along k
   const __half *a_hi, *a_lo;
   __half *to_hi, *to_lo;
+  int parts;     // PARTS: of the k range
+  float* sums;   // matrices x parts x side x side
 };
-template <bool MIDDLE, bool ONE>
+enum Symmetric { WHOLE, MIDDLE_FACTOR, PARTS };
+template <Symmetric KIND, bool ONE>
 struct SymmetricOp {
   typedef SymmetricParams Params;
   typedef TileForm<true, ONE> Form;
+  static constexpr bool MIDDLE = KIND == MIDDLE_FACTOR;
   static constexpr bool STORES = false, LONG = true;
   static constexpr int SUM = MUON_SUM;
   const SymmetricParams& p;
@@ -177,19 +183,24 @@ struct SymmetricOp {
     n_blocks = (p.side + Form::BN - 1) / Form::BN;
     per = m_blocks * n_blocks - m_blocks * (m_blocks - 1);  // row block i has column blocks 2 i and up
   }
-  __device__ int tiles() const { return per * p.count; }
+  __device__ int tiles() const { return per * p.count * (KIND == PARTS ? p.parts : 1); }
   __device__ Tile tile(int t) const {
     Tile r;
-    r.z = t / per;
+    r.z = t / per;  // PARTS: a part of a matrix
     int in = t - r.z * per, i = 0;
     while (in >= n_blocks - 2 * i) in -= n_blocks - 2 * i++;
     r.m0 = i * Form::M;
     r.n0 = (2 * i + in) * Form::BN;
-    const int off = r.z * (int)p.a_step;
+    const int matrix = KIND == PARTS ? r.z / p.parts : r.z, off = matrix * (int)p.a_step;
     r.a_mn = r.m0 + (p.steps_k ? 0 : off);
     r.b_mn = r.n0 + (p.steps_k ? 0 : off);
     r.a_k = r.b_k = p.steps_k ? off : 0;
     r.kblocks = p.kblocks;
+    if (KIND == PARTS) {
+      const int part = r.z - matrix * p.parts, from = p.kblocks * part / p.parts;
+      r.a_k = r.b_k += from * TILE_K;
+      r.kblocks = p.kblocks * (part + 1) / p.parts - from;
+    }
     return r;
   }
   // a is loaded while the products are summed: it is what a small matrix's middle factor would wait for otherwise (5.6 against 2.7 us
@@ -206,7 +217,11 @@ struct SymmetricOp {
   __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[16], uint8_t* stage, int lane) {
     if (row0 >= p.side || col0 >= p.side) return;  // uniform: sides are multiples of 64
     const long long base = (long long)t.z * p.side * p.side;
-    constexpr float unit = MIDDLE ? P_UP * NS_C / (A_UP * A_UP) : A_UP / (X_UP * X_UP), b = P_UP * NS_B / A_UP;
+    if constexpr (KIND == PARTS) {
+      by_rows(row0, col0, v, stage, lane, [&](int, int r, int c, const float4& y) { *reinterpret_cast<float4*>(p.sums + base + (long long)r * p.side + c) = y; });
+      return;
+    }
+    constexpr float unit = MIDDLE ? P_UP * NS_C / (A_UP * A_UP) : A_UNIT, b = P_UP * NS_B / A_UP;
     const bool second = QUADS > 4 && (col0 - t.n0) & 16;  // of the warp's two chunks
     float4 x[4];
     by_rows(row0, col0, v, stage, lane, [&](int i, int r, int c, const float4& y) {
@@ -226,6 +241,35 @@ struct SymmetricOp {
   }
   __device__ __forceinline__ void end(const Tile&, int, int) {}
 };
+
+// a from its parts on and above the diagonal, in order, 32 x 32 elements per block; the block on the other side of the diagonal gets
+// them transposed.
+__global__ void __launch_bounds__(256) join_parts_kernel(const float* __restrict__ sums, int parts, int side, __half* __restrict__ hi, __half* __restrict__ lo) {
+  __shared__ float turned[32][33];
+  after_previous();
+  let_next_start();
+  const int n = side / 32, z = blockIdx.y;
+  int in = blockIdx.x, i = 0;
+  while (in >= n - i) in -= n - i++;
+  const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 4, j = i + in;
+  const long long all = (long long)side * side;
+  const float* from = sums + z * parts * all + (long long)(i * 32 + r) * side + j * 32 + c;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int k = 0; k < parts; ++k) {
+    const float4 y = *reinterpret_cast<const float4*>(from + k * all);
+    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+  }
+  x = make_float4(x.x * A_UNIT, x.y * A_UNIT, x.z * A_UNIT, x.w * A_UNIT);
+  store_pair(hi, lo, z * all + (long long)(i * 32 + r) * side + j * 32 + c, x);
+  if (i == j) return;  // computed on both sides of the diagonal
+  turned[c][r] = x.x;
+  turned[c + 1][r] = x.y;
+  turned[c + 2][r] = x.z;
+  turned[c + 3][r] = x.w;
+  __syncthreads();
+  store_pair(hi, lo, z * all + (long long)(j * 32 + r) * side + i * 32 + c, make_float4(turned[r][c], turned[r][c + 1], turned[r][c + 2], turned[r][c + 3]));
+}
 
 // The new x: middle factor times x (wide) or x times middle factor (tall); the last one updates w instead.
 struct NextParams {
@@ -331,7 +375,29 @@ struct NextOp {
 
 struct MuonSizes {
   int rows_up, cols_up, side, group;
+  int most_parts;  // of a, over all matrices of a group
 };
+constexpr int MOST_SMS = 148;
+long long symmetric_tiles(int side, int bm) {
+  const long long m = (side + bm - 1) / bm, n = (side + bm / 2 - 1) / (bm / 2);
+  return m * n - m * (m - 1);
+}
+// A product x x' of few tiles and a long k range goes in parts, as many as there are SMs for and of four k-blocks at least. In clocks: 832 per
+// k-block, 4500 for the kernel that joins them, 1 per 250 elements of every part. 4000 x 256 189 -> 123 us per update, 512 x 8192 370 -> 236,
+// 64 x 2048 115 -> 86; 1024 x 1024 stays whole (164 us, 172 in two parts).
+int parts_of(int count, int side, int kblocks, int sms) {
+  long long most = sms / (symmetric_tiles(side, 128) * count);
+  if (most > kblocks / 4) most = kblocks / 4;
+  long long parts = 1, least = 832ll * kblocks - 4500;
+  for (int n = 2; n <= most; ++n) {
+    const long long clocks = 832ll * ((kblocks + n - 1) / n) + (long long)n * count * side * side / 250;
+    if (clocks < least) {
+      least = clocks;
+      parts = n;
+    }
+  }
+  return (int)parts;
+}
 MuonSizes muon_sizes(int count, int rows, int cols) {
   MuonSizes z;
   z.rows_up = (rows + TILE_K - 1) / TILE_K * TILE_K;
@@ -342,10 +408,17 @@ MuonSizes muon_sizes(int count, int rows, int cols) {
   long long group = (4 * 74 + per - 1) / per;
   if (group > MUON_GROUP) group = MUON_GROUP;
   z.group = count < group ? count : (int)group;
+  const int long_side = rows <= cols ? z.cols_up : z.rows_up;
+  z.most_parts = 0;
+  for (int n = 1; n <= z.group; ++n) {
+    const int parts = parts_of(n, z.side, long_side / TILE_K, MOST_SMS);
+    if (parts > 1 && parts * n > z.most_parts) z.most_parts = parts * n;
+  }
   return z;
 }
 struct MuonSpace {
   double* parts;
+  float* sums;
   __half *x_hi[2], *x_lo[2], *a_hi, *a_lo, *p_hi, *p_lo;
 };
 size_t muon_space(const MuonSizes& z, void* base, MuonSpace* s) {
@@ -360,6 +433,7 @@ size_t muon_space(const MuonSizes& z, void* base, MuonSpace* s) {
   s->a_lo = c.take<__half>(a);
   s->p_hi = c.take<__half>(a);
   s->p_lo = c.take<__half>(a);
+  s->sums = c.take<float>((size_t)z.most_parts * z.side * z.side);
   return c.used;
 }
 
@@ -407,10 +481,7 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
   const long long x_rows = (long long)z.rows_up * count, a_rows = (long long)z.side * count;
   // Tiles of a symmetric and of a full product, in tiles of bm rows. Single CTAs or pairs: what shared memory takes to be filled and read for a
   // k-block (832 and 960 clocks), times the rounds of tiles, and 3 us for a launch of clusters.
-  auto symmetric = [&](int bm) {
-    const long long m = (z.side + bm - 1) / bm, n = (z.side + bm / 2 - 1) / (bm / 2);
-    return (m * n - m * (m - 1)) * count;
-  };
+  auto symmetric = [&](int bm) { return symmetric_tiles(z.side, bm) * count; };
   auto full = [&](int bm) { return (long long)((z.rows_up + bm - 1) / bm) * ((z.cols_up + bm / 2 - 1) / (bm / 2)) * count; };
   auto one_is_less = [&](long long one, long long pairs, int kblocks) {
     return (one + sms - 1) / sms * 832 * kblocks <= (pairs + sms / 2 - 1) / (sms / 2) * 960 * kblocks + 6000;
@@ -418,6 +489,7 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
   const int k_a = (wide ? z.cols_up : z.rows_up) / TILE_K, k_b = z.side / TILE_K;
   const bool a_one = one_is_less(symmetric(128), symmetric(256), k_a), p_one = one_is_less(symmetric(128), symmetric(256), k_b),
              full_one = one_is_less(full(128), full(256), k_b);
+  const int a_parts = parts_of(count, z.side, k_a, sms < MOST_SMS ? sms : MOST_SMS);
   const long long a_tiles = symmetric(a_one ? 128 : 256), p_tiles = symmetric(p_one ? 128 : 256), tiles = full(full_one ? 128 : 256);
   const TileOperand a_op{s.a_hi, s.a_lo, a_rows, z.side, z.side, false}, p_op{s.p_hi, s.p_lo, a_rows, z.side, z.side, false};
   int at = 0;
@@ -433,7 +505,16 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
     q.to_hi = s.a_hi;
     q.to_lo = s.a_lo;
     const TileOperand& x = wide ? x_k : x_mn;
-    rc = (a_one ? tile_launch<SymmetricOp<false, true>> : tile_launch<SymmetricOp<false, false>>)(who, x, x, nullptr, q, false, a_tiles, sms, chain);
+    if (a_parts > 1) {
+      q.parts = a_parts;
+      q.sums = s.sums;
+      rc = tile_launch<SymmetricOp<PARTS, true>>(who, x, x, nullptr, q, false, symmetric(128) * a_parts, sms, chain);
+      const int n = z.side / 32;
+      chain.launch(join_parts_kernel, dim3(n * (n + 1) / 2, count), 256, 0, 0, s.sums, a_parts, z.side, s.a_hi, s.a_lo);
+      if (rc == B2_OK) rc = launch_error(chain.err, who);
+    } else {
+      rc = (a_one ? tile_launch<SymmetricOp<WHOLE, true>> : tile_launch<SymmetricOp<WHOLE, false>>)(who, x, x, nullptr, q, false, a_tiles, sms, chain);
+    }
     if (rc != B2_OK) return rc;
     q.kblocks = k_b;
     q.a_step = z.side;
@@ -442,7 +523,7 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
     q.a_lo = s.a_lo;
     q.to_hi = s.p_hi;
     q.to_lo = s.p_lo;
-    rc = (p_one ? tile_launch<SymmetricOp<true, true>> : tile_launch<SymmetricOp<true, false>>)(who, a_op, a_op, nullptr, q, false, p_tiles, sms, chain);
+    rc = (p_one ? tile_launch<SymmetricOp<MIDDLE_FACTOR, true>> : tile_launch<SymmetricOp<MIDDLE_FACTOR, false>>)(who, a_op, a_op, nullptr, q, false, p_tiles, sms, chain);
     if (rc != B2_OK) return rc;
     NextParams n{};
     n.list = list;

@@ -88,6 +88,18 @@ def test_update(lm, count, rows, cols, ld, offset, dtype, nesterov):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("count,rows,cols", [(1, 64, 2050), (2, 2047, 70), (1, 515, 2100), (3, 300, 5000), (17, 40, 2000), (1, 2100, 1000), (8, 520, 500),
+                                             (2, 1000, 1030), (5, 900, 950)])
+def test_forms_of_products(lm, count, rows, cols):
+    """Long sums in parts, single CTAs in one and two rounds, pairs."""
+    w, m, g = _make(count, rows, cols, torch.float32)
+    before = (w.clone(), m.clone(), g)
+    lm.muon(w, m, g, **OPTIONS)
+    lm.sync()
+    _check(before, (w, m, None), dict(OPTIONS, nesterov=True))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("steps", [1, 3, 7])
 def test_steps_and_low_rank(lm, steps):
     w, m, g = _make(2, 200, 333, torch.float32, low_rank=True)

@@ -510,6 +510,13 @@ bool tile_maps(const TileOperand& a, const TileOperand& b, bool bf16, TileMaps* 
   return ok;
 }
 
+// Whether single CTAs take less time than pairs: what shared memory takes to be filled and read for a k-block of a tile, times k-blocks and
+// rounds of tiles, and 3 us for a launch of clusters, all in clocks.
+template <bool SPLIT>
+bool single_ctas(long long rounds_one, long long kblocks_one, long long rounds_pairs, long long kblocks_pairs) {
+  return rounds_one * kblocks_one * (SPLIT ? 832 : 512) <= rounds_pairs * kblocks_pairs * (SPLIT ? 960 : 512) + 6000;
+}
+
 // A row-major matrix of 16-bit elements that store_half_words writes to.
 struct TileResult {
   void* p;

@@ -479,12 +479,11 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
   int rc = launch_error(chain.err, who);
   const bool wide = rows <= cols;
   const long long x_rows = (long long)z.rows_up * count, a_rows = (long long)z.side * count;
-  // Tiles of a symmetric and of a full product, in tiles of bm rows. Single CTAs or pairs: what shared memory takes to be filled and read for a
-  // k-block (832 and 960 clocks), times the rounds of tiles, and 3 us for a launch of clusters.
+  // Tiles of a symmetric and of a full product, in tiles of bm rows
   auto symmetric = [&](int bm) { return symmetric_tiles(z.side, bm) * count; };
   auto full = [&](int bm) { return (long long)((z.rows_up + bm - 1) / bm) * ((z.cols_up + bm / 2 - 1) / (bm / 2)) * count; };
   auto one_is_less = [&](long long one, long long pairs, int kblocks) {
-    return (one + sms - 1) / sms * 832 * kblocks <= (pairs + sms / 2 - 1) / (sms / 2) * 960 * kblocks + 6000;
+    return single_ctas<true>((one + sms - 1) / sms, kblocks, (pairs + sms / 2 - 1) / (sms / 2), kblocks);
   };
   const int k_a = (wide ? z.cols_up : z.rows_up) / TILE_K, k_b = z.side / TILE_K;
   const bool a_one = one_is_less(symmetric(128), symmetric(256), k_a), p_one = one_is_less(symmetric(128), symmetric(256), k_b),

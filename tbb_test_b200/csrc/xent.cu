@@ -83,8 +83,13 @@ __device__ __forceinline__ unsigned int block_max(unsigned int mine, unsigned in
   __syncthreads();
   return __reduce_max_sync(0xFFFFFFFFu, lane < FRONT_THREADS / 32 ? warp_max[lane] : 0u);
 }
-// Threads of a row of n pieces: a power of two up to a warp, as a shift.
-__device__ __forceinline__ int row_shift(int n) { return n >= 32 ? 5 : 31 - __clz(max(n, 1)); }
+// Threads of a row of n pieces, as a shift: the power of two below, up to the whole block.
+__host__ __device__ __forceinline__ int row_shift(int n) {
+  int shift = 0;
+  while (shift < 9 && 2 << shift <= n) ++shift;
+  return shift;
+}
+static_assert(FRONT_THREADS == 1 << 9, "a whole block");
 
 // Rows first + k of a copy, for a block's share of the k below n: row of(k) of x, zeros behind `width` up to `pitch`, or zeros alone where
 // of(k) is negative.
@@ -252,7 +257,6 @@ __global__ void __launch_bounds__(FRONT_THREADS) pairs_kernel(const __grid_const
   }
 }
 
-__device__ __forceinline__ int row_blocks(unsigned int rows) { return max(1, (int)((rows + TILE_M - 1) / TILE_M)); }
 
 // ------------------------------------------------------------------ logits
 
@@ -267,8 +271,9 @@ struct LogitParams {
   const float2* row_stat;  // maximum and 1 / sum of whole rows
   uint16_t *d_hi, *d_lo;
   long long ld_d;
-  float* x;  // logits as they are summed, where they are kept
+  float* x;  // logits as they are summed, where they are kept: parts x all_rows x ld_x
   long long ld_x;
+  int x_parts, all_rows;
 };
 
 template <class F>
@@ -301,6 +306,32 @@ struct LogitTiles {
     r.z = 0;
     return r;
   }
+};
+
+// Few tiles: their sums as they are, in parts of the k range where there are more SMs than tiles.
+template <class F>
+struct PlainOp : LogitTiles<F> {
+  typedef LogitParams Params;
+  static constexpr bool LONG = true, STORES = false;
+  static constexpr int SUM = F::SPLIT ? XENT_SUM : 16, W = 16;
+  using LogitTiles<F>::p;
+  __device__ explicit PlainOp(const LogitParams& q, const TileMaps& m) : LogitTiles<F>(q, m) {}
+  __device__ int tiles() const { return LogitTiles<F>::tiles() * p.x_parts; }
+  __device__ Tile tile(int t) const {
+    const int whole = LogitTiles<F>::tiles(), part = t / whole, from = p.kblocks * part / p.x_parts;
+    Tile r = LogitTiles<F>::tile(t - part * whole);
+    r.a_k = r.b_k = from * TILE_K;
+    r.kblocks = p.kblocks * (part + 1) / p.x_parts - from;
+    r.z = part;
+    return r;
+  }
+  __device__ __forceinline__ void begin(const Tile&, int, int, int) {}
+  __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[W], uint8_t* stage, int lane) {
+    by_rows(row0, col0, v, stage, lane, [&](int, int r, int c, const float4& x) {
+      if (r < this->rows && c < p.vocab) *reinterpret_cast<float4*>(p.x + ((long long)t.z * p.all_rows + r) * p.ld_x + c) = x;
+    });
+  }
+  __device__ __forceinline__ void end(const Tile&, int, int) {}
 };
 
 // Maximum and sum of exponentials of a row over the columns of one warp, and the target's logit. LONG: for more than 16 k-blocks,
@@ -450,6 +481,89 @@ __global__ void __launch_bounds__(256) kept_kernel(const LogitParams p) {
   }
 }
 
+// Loss of a row, and its d, from the parts of its logits: a block has a row, its threads four neighbouring columns at a time, and
+// keeps it in registers. d has zeros up to whole k-blocks, as above.
+constexpr int ROW_THREADS = 512, ROW_QUADS = 10;
+template <bool SPLIT>
+__global__ void __launch_bounds__(ROW_THREADS) row_kernel(const LogitParams p, const int* __restrict__ row_of, float* __restrict__ row_loss, int grads) {
+  __shared__ float across[ROW_THREADS / 32];
+  after_previous();
+  let_next_start();
+  const int lane = threadIdx.x & 31, r = blockIdx.x, at = threadIdx.x * 4;
+  const Meta meta = *p.meta;
+  const int rows = (int)meta.rows, whole = whole_rows(rows);
+  if (r >= whole) return;
+  const float unit = SPLIT ? LOG2E * pow2(-up_exp(meta.max_h)) * pow2(-up_exp(meta.max_w)) : LOG2E, to = SPLIT ? (float)(1 << D_EXP) : 1.f;
+  const long long stride = (long long)p.all_rows * p.ld_x;
+  const float* from = p.x + r * p.ld_x;
+  auto over_all = [&](float v, auto join) {  // threads
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v = join(v, __shfl_xor_sync(0xFFFFFFFFu, v, d));
+    __syncthreads();
+    if (lane == 0) across[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = across[lane & 15];
+#pragma unroll
+    for (int d = 8; d; d >>= 1) v = join(v, __shfl_xor_sync(0xFFFFFFFFu, v, d));
+    return v;
+  };
+  static_assert(ROW_THREADS == 512, "16 warps");
+  float x[ROW_QUADS][4];
+  float top = -INFINITY, sum = 0.f, by = 0.f;
+  int target = -1;
+  if (r < rows) {
+#pragma unroll
+    for (int i = 0; i < ROW_QUADS; ++i) {
+      const int c = at + i * ROW_THREADS * 4;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[i][j] = 0.f;
+      if (c >= p.vocab) continue;
+#pragma unroll 4
+      for (int k = 0; k < p.x_parts; ++k) {
+        const float4 y = *reinterpret_cast<const float4*>(from + k * stride + c);
+        x[i][0] += y.x; x[i][1] += y.y; x[i][2] += y.z; x[i][3] += y.w;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (c + j >= p.vocab) x[i][j] = -INFINITY;
+        top = fmaxf(top, x[i][j]);
+      }
+    }
+    top = over_all(top, [](float a, float b) { return fmaxf(a, b); }) * unit;
+    const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int i = 0; i < ROW_QUADS; ++i) {
+      if (at + i * ROW_THREADS * 4 >= p.vocab) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[i][j] = ex2(fmaf(x[i][j], unit, -base));
+        sum += x[i][j];
+      }
+    }
+    sum = over_all(sum, [](float a, float b) { return a + b; });
+    by = to / sum;
+    target = __ldg(p.target + r);
+    if (at == 0) {
+      float own = 0.f;
+      for (int k = 0; k < p.x_parts; ++k) own += from[k * stride + target];
+      row_loss[row_of[r]] = ((top - own * unit) + log2f(sum)) * LN2;
+    }
+  }
+  if (!grads) return;
+  const int cols = (p.vocab + TILE_K - 1) / TILE_K * TILE_K;
+#pragma unroll
+  for (int i = 0; i < ROW_QUADS; ++i) {
+    const int c = at + i * ROW_THREADS * 4;
+    if (c >= cols) continue;
+    float d[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) d[j] = r < rows && c + j < p.vocab ? x[i][j] * by - (c + j == target ? to : 0.f) : 0.f;
+    const long long to_at = r * p.ld_d + c;
+    if (SPLIT) store_pair(reinterpret_cast<__half*>(p.d_hi), reinterpret_cast<__half*>(p.d_lo), to_at, make_float4(d[0], d[1], d[2], d[3]));
+    else *reinterpret_cast<uint2*>(p.d_hi + to_at) = make_uint2(pack_bf16(d[0], d[1]), pack_bf16(d[2], d[3]));
+  }
+}
+
 // Whole rows' maximum and sum from the lists, and the losses. A block has 32 rows: its warps share their lists first, and then each
 // joins one row's 32 shares.
 __global__ void __launch_bounds__(1024) join_rows_kernel(const float2* __restrict__ parts, long long row_pitch, int count,
@@ -503,7 +617,7 @@ struct ProductParams {
   // dh: fp32 sums over the pieces
   float *acc, *slots;
   long long ld_acc;
-  int pairs, full_kblocks;  // full_kblocks: of a whole piece
+  int pairs, full_kblocks;  // pairs of CTAs, or single ones; full_kblocks: of a whole piece
   int first;                // first piece: written, not added to
   // dw
   void* dw;
@@ -523,8 +637,8 @@ struct ProductParams {
 // for the whole call).
 struct HiddenSplit {
   int m_blocks, n_blocks, whole, side, rest, shares;  // rest and shares count rows of `side` tiles and of pairs
-  __device__ HiddenSplit(const ProductParams& p, unsigned int rows, int bn) {
-    m_blocks = row_blocks(rows);
+  __device__ HiddenSplit(const ProductParams& p, unsigned int rows, int bm, int bn) {
+    m_blocks = max(1, (int)((rows + bm - 1) / bm));
     n_blocks = (p.width + bn - 1) / bn;
     const int tiles = m_blocks * n_blocks;
     whole = tiles / p.pairs * p.pairs;
@@ -553,20 +667,20 @@ struct HiddenSplit {
 };
 
 // dh (listed rows) += d w over a piece.
-template <bool SPLIT_>
+template <class F>
 struct HiddenOp {
   typedef ProductParams Params;
-  typedef TileForm<SPLIT_> Form;
-  static constexpr bool SPLIT = SPLIT_, STORES = false;
-  static constexpr bool LONG = SPLIT_;
-  static constexpr int SUM = XENT_SUM, BN = TileForm<SPLIT_>::BN;
+  typedef F Form;
+  static constexpr bool SPLIT = F::SPLIT, STORES = false;
+  static constexpr bool LONG = SPLIT;
+  static constexpr int SUM = XENT_SUM, BN = F::BN;
   const ProductParams& p;
   HiddenSplit split;
   int kblocks;
   float unit;
   float* to;
   long long ld;
-  __device__ explicit HiddenOp(const ProductParams& q, const TileMaps&) : p(q), split(q, q.meta->rows, BN) {
+  __device__ explicit HiddenOp(const ProductParams& q, const TileMaps&) : p(q), split(q, q.meta->rows, F::M, BN) {
     kblocks = (p.v_count + TILE_K - 1) / TILE_K;
     unit = SPLIT ? p.scale * pow2(-D_EXP) * pow2(-up_exp(p.meta->max_w)) : p.scale;
   }
@@ -588,7 +702,7 @@ struct HiddenOp {
       kb = (int)((long long)kblocks * b / split.shares) - from;
       if (a > 0 || b < split.shares) r.z = HiddenSplit::slot_of(s, a > 0);
     }
-    r.m0 = at / split.n_blocks * TILE_M;
+    r.m0 = at / split.n_blocks * F::M;
     r.n0 = at % split.n_blocks * BN;
     r.a_mn = r.m0;
     r.b_mn = r.n0;
@@ -600,13 +714,13 @@ struct HiddenOp {
   __device__ __forceinline__ void begin(const Tile& t, int, int, int) {
     if (t.z >= 0) {
       ld = BN;
-      to = p.slots + (long long)t.z * TILE_M * BN - (t.m0 * ld + t.n0);
+      to = p.slots + (long long)t.z * F::M * BN - (t.m0 * ld + t.n0);
     } else {
       ld = p.ld_acc;
       to = p.acc;
     }
   }
-  static constexpr int W = TileForm<SPLIT_>::CHUNK;
+  static constexpr int W = F::CHUNK;
   __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[W], uint8_t* stage, int lane) {
     if (t.z == -2 || col0 >= p.width) return;
     float4 old[W / 4];
@@ -696,13 +810,13 @@ struct WeightOp {
 };
 
 // dh in the caller's order and type, zeros for rows without a target.
-template <typename T>
+template <typename T, class F>
 __global__ void __launch_bounds__(256) spread_rows_kernel(const ProductParams p, const int* __restrict__ slot_of, int rows, int vec,
                                                           T* __restrict__ dh, size_t ld) {
-  constexpr int BN = TileForm<sizeof(T) == 4>::BN;
+  constexpr int BN = F::BN;
   after_previous();
   let_next_start();
-  const HiddenSplit split(p, p.meta->rows, BN);
+  const HiddenSplit split(p, p.meta->rows, F::M, BN);
   const int width = p.width;
   for (int r = blockIdx.x; r < rows; r += gridDim.x) {
     const int slot = slot_of[r];
@@ -710,13 +824,13 @@ __global__ void __launch_bounds__(256) spread_rows_kernel(const ProductParams p,
     for (int c = threadIdx.x * 4; c < width; c += 256 * 4) {
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
       if (slot >= 0) {
-        const int t = slot / TILE_M * split.n_blocks + c / BN - split.whole;
+        const int t = slot / F::M * split.n_blocks + c / BN - split.whole;
         const int parts = split.parts(t);
         if (parts == 1) {
           x = *reinterpret_cast<const float4*>(p.acc + slot * p.ld_acc + c);
         } else {
           for (int n = 0; n < parts; ++n) {
-            const float4 y = *reinterpret_cast<const float4*>(p.slots + ((long long)split.slot(t, n) * TILE_M + slot % TILE_M) * BN + c % BN);
+            const float4 y = *reinterpret_cast<const float4*>(p.slots + ((long long)split.slot(t, n) * F::M + slot % F::M) * BN + c % BN);
             x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
           }
         }
@@ -741,19 +855,28 @@ struct Sizes {
   long long parts;           // lists per row
   long long piece;           // columns of d
   bool split, copy_w;
-  bool one;                  // logits by single CTAs
-  bool keep;                 // logits are kept for d
+  bool one;                  // few tiles of logits: single CTAs
+  bool by_rows;              // and few rows: PlainOp and row_kernel
+  int x_parts;               // parts of their k range
+  bool keep;                 // logits are kept
   long long ld_x;
 };
 constexpr int MOST_PAIRS = 74;  // 148 SMs
 template <class F>
 long long tiles_of(long long m, long long n) { return (m + F::M - 1) / F::M * ((n + F::BN - 1) / F::BN); }
+// Single CTAs take over when each has one tile at most. Where they would leave SMs idle through a long k range, it goes in parts, and
+// row_kernel takes its time for each of a few rows (with gradients 1 x 3972 x 806 in fp32 84 -> 74 us, 75 x 1152 x 2411 in bf16 43 -> 38).
 template <class F>
-void logit_sizes(Sizes* z, size_t rows, size_t vocab) {  // F: single CTAs, which take over when each has one tile at most
+void logit_sizes(Sizes* z, size_t rows, size_t width, size_t vocab) {  // F: single CTAs
   typedef TileForm<F::SPLIT> Pairs;
-  z->one = tiles_of<F>(rows, vocab) <= 2 * MOST_PAIRS;
+  const long long tiles = tiles_of<F>(rows, vocab), kblocks = (long long)(width + TILE_K - 1) / TILE_K;
+  z->one = tiles <= 2 * MOST_PAIRS;
+  long long parts = z->one ? 2 * MOST_PAIRS / tiles : 1;
+  if (parts > kblocks / 4) parts = kblocks / 4;
+  z->by_rows = parts > 1 && kblocks - kblocks / parts >= 8 && rows <= 4 * MOST_PAIRS && vocab <= ROW_QUADS * 4 * ROW_THREADS;
+  z->x_parts = z->by_rows ? (int)parts : 1;
   const int bn = z->one ? F::BN : Pairs::BN;
-  z->parts = F::PARTS * (((long long)vocab + bn - 1) / bn);
+  z->parts = z->by_rows ? 0 : F::PARTS * (((long long)vocab + bn - 1) / bn);
 }
 // Logits that are kept cost their bytes twice, others 2 F operations each again. What stays in the L2 cache is kept (1024 x 512 x 8192 in
 // fp32 140 -> 125 us, 16 x 2048 x 65536 in bf16 251 -> 217); beyond it the operations cost more with three MMAs or great widths (2048 x
@@ -769,11 +892,11 @@ Sizes sizes_of(size_t rows, size_t width, size_t vocab, int dtype, int grads, co
   z.copy_w = z.split || reinterpret_cast<uintptr_t>(w) % 16 != 0 || ldw % 8 != 0;
   z.rows_up = (long long)(rows + TILE_M - 1) / TILE_M * TILE_M;
   z.pitch = (long long)(width + 63) / 64 * 64;
-  if (z.split) logit_sizes<TileForm<true, true>>(&z, rows, vocab);
-  else logit_sizes<TileForm<false, true>>(&z, rows, vocab);
+  if (z.split) logit_sizes<TileForm<true, true>>(&z, rows, width, vocab);
+  else logit_sizes<TileForm<false, true>>(&z, rows, width, vocab);
   z.piece = 0;
   z.ld_x = ((long long)vocab + 3) / 4 * 4;
-  z.keep = grads && keeps_logits((long long)rows * z.ld_x * 4, width, z.split);
+  z.keep = z.by_rows || (grads && keeps_logits((long long)rows * z.ld_x * 4, width, z.split));
   if (grads) {
     // Few pieces: each has three kernels to fill and drain, which costs more than reading d from HBM (8192 x 2048 x 65536 with pieces of 160
     // MB 6.05 ms, 320 MB 5.94, 640 MB 5.86, 80 MB 6.5; 2048 x 1024 x 65536 948, 906 and 832 us). The 256-wide column blocks of a piece should go
@@ -817,7 +940,7 @@ size_t space_of(const Sizes& z, size_t rows, size_t vocab, int grads, void* base
   s->d_lo = c.take<uint16_t>(lo * z.rows_up * z.piece);
   s->acc = c.take<float>(grads ? z.rows_up * z.pitch : 0);
   s->slots = c.take<float>(grads ? 2ll * MOST_PAIRS * TILE_M * (z.split ? 128 : 256) : 0);
-  s->x = c.take<float>(z.keep ? rows * z.ld_x : 0);
+  s->x = c.take<float>(z.keep ? z.x_parts * rows * z.ld_x : 0);
   return c.used;
 }
 
@@ -876,14 +999,15 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
   f.share = (rows + FRONT_BLOCKS - 1) / FRONT_BLOCKS;
   if (f.share < 4) f.share = 4;
   f.blocks_h = (rows + f.share - 1) / f.share;
-  f.blocks_w = z.copy_w ? some((vocab + 15) / 16, 2 * FRONT_BLOCKS) : 0;
+  const int at_once = FRONT_THREADS >> row_shift(pitch / 8);
+  f.blocks_w = z.copy_w ? some((vocab + at_once - 1) / at_once, 2 * FRONT_BLOCKS) : 0;
   if (rows > COUNT_ROWS) {
     chain.launch(count_kernel, dim3(f.blocks_h), FRONT_THREADS, 0, 0, f, s.counts);
     f.counts = s.counts;
   }
   chain.launch(front_kernel<T>, dim3(f.blocks_h + f.blocks_w), FRONT_THREADS, 0, 0, f);
   if (SPLIT) {
-    const int on_h = some((z.rows_up + 15) / 16, FRONT_BLOCKS);
+    const int on_h = some((z.rows_up + at_once - 1) / at_once, FRONT_BLOCKS);
     chain.launch(pairs_kernel, dim3(on_h + f.blocks_w), FRONT_THREADS, 0, 0, f, on_h, f.blocks_w);
   }
   int rc = launch_error(chain.err, who);
@@ -908,21 +1032,30 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
   lp.ld_d = z.piece;
   lp.x = s.x;
   lp.ld_x = z.ld_x;
-  const bool sums = !SPLIT && lp.kblocks > StatOp<Pairs, true, false>::SUM;
-  auto stat_of = [&](auto form, auto keep) {
-    typedef decltype(form) F;
-    constexpr bool KEEP = decltype(keep)::value;
-    return sums ? tile_launch<StatOp<F, !SPLIT, KEEP>> : tile_launch<StatOp<F, false, KEEP>>;
-  };
-  const std::true_type yes;
-  const std::false_type no;
-  auto stat = z.one ? (z.keep ? stat_of(One(), yes) : stat_of(One(), no)) : (z.keep ? stat_of(Pairs(), yes) : stat_of(Pairs(), no));
-  rc = stat(who, h_k, w_k, nullptr, lp, !SPLIT, z.one ? tiles_of<One>(rows, vocab) : tiles_of<Pairs>(rows, vocab), sms, chain);
-  if (rc != B2_OK) return rc;
-  chain.launch(join_rows_kernel, dim3((rows + 31) / 32), 1024, 0, 0, s.parts, z.rows_up, (int)z.parts, s.meta, s.target_logit, s.row_of, s.row_stat,
-               c.row_loss);
+  lp.x_parts = z.x_parts;
+  lp.all_rows = rows;
+  const int grads = c.dh || c.dw;
+  if (z.by_rows) {
+    rc = tile_launch<PlainOp<One>>(who, h_k, w_k, nullptr, lp, !SPLIT, tiles_of<One>(rows, vocab) * z.x_parts, sms, chain);
+    if (rc != B2_OK) return rc;
+    chain.launch(row_kernel<SPLIT>, dim3((rows + TILE_K - 1) / TILE_K * TILE_K), ROW_THREADS, 0, 0, lp, s.row_of, c.row_loss, grads);
+  } else {
+    const bool sums = !SPLIT && lp.kblocks > StatOp<Pairs, true, false>::SUM;
+    auto stat_of = [&](auto form, auto keep) {
+      typedef decltype(form) F;
+      constexpr bool KEEP = decltype(keep)::value;
+      return sums ? tile_launch<StatOp<F, !SPLIT, KEEP>> : tile_launch<StatOp<F, false, KEEP>>;
+    };
+    const std::true_type yes;
+    const std::false_type no;
+    auto stat = z.one ? (z.keep ? stat_of(One(), yes) : stat_of(One(), no)) : (z.keep ? stat_of(Pairs(), yes) : stat_of(Pairs(), no));
+    rc = stat(who, h_k, w_k, nullptr, lp, !SPLIT, z.one ? tiles_of<One>(rows, vocab) : tiles_of<Pairs>(rows, vocab), sms, chain);
+    if (rc != B2_OK) return rc;
+    chain.launch(join_rows_kernel, dim3((rows + 31) / 32), 1024, 0, 0, s.parts, z.rows_up, (int)z.parts, s.meta, s.target_logit, s.row_of, s.row_stat,
+                 c.row_loss);
+  }
   rc = launch_error(chain.err, who);
-  if (rc != B2_OK || (!c.dh && !c.dw)) return rc;
+  if (rc != B2_OK || !grads) return rc;
 
   ProductParams pp{};
   pp.meta = s.meta;
@@ -930,7 +1063,15 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
   pp.scale = c.scale;
   pp.acc = s.acc;
   pp.slots = s.slots;
-  pp.pairs = sms / 2 < MOST_PAIRS ? sms / 2 : MOST_PAIRS;
+  // dh's k range is shared out evenly over CTAs or pairs, in parts of eight k-blocks at least
+  const long long dh_one = tiles_of<One>(rows, width), dh_pairs = tiles_of<Pairs>(rows, width), dh_k = ((vocab < z.piece ? vocab : z.piece) + TILE_K - 1) / TILE_K;
+  const int pairs = sms / 2 < MOST_PAIRS ? sms / 2 : MOST_PAIRS;
+  auto share_of = [&](long long tiles, int over) {
+    const long long k = (tiles * dh_k + over - 1) / over, least = dh_k < 8 ? dh_k : 8;
+    return k > least ? k : least;
+  };
+  const bool h_one = single_ctas<SPLIT>(1, share_of(dh_one, 2 * pairs), 1, share_of(dh_pairs, pairs));
+  pp.pairs = h_one ? 2 * pairs : pairs;
   pp.full_kblocks = (int)(z.piece / TILE_K);
   pp.ld_acc = pitch;
   pp.dw = c.dw;
@@ -946,16 +1087,18 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
     lp.v_begin = pp.v_begin = v0;
     lp.v_count = pp.v_count = count;
     pp.first = v0 == 0;
-    if (z.keep) {
+    if (z.by_rows) {  // d is there
+    } else if (z.keep) {
       const long long r = (rows + TILE_K - 1) / TILE_K * TILE_K, n = (count + TILE_K - 1) / TILE_K * TILE_K;
       chain.launch(kept_kernel<SPLIT>, dim3(blocks((r * n / 8 + 255) / 256)), 256, 0, 0, lp);
       rc = launch_error(chain.err, who);
     } else {
       rc = tile_launch<GradOp<Pairs>>(who, h_k, w_k, SPLIT ? nullptr : &d_out, lp, !SPLIT, tiles_of<Pairs>(rows, count), sms, chain);
     }
-    if (rc == B2_OK && c.dh) rc = tile_launch<HiddenOp<SPLIT>>(who, d_k, w_mn, nullptr, pp, !SPLIT, pp.pairs, sms, chain);
+    if (rc == B2_OK && c.dh) rc = (h_one ? tile_launch<HiddenOp<One>> : tile_launch<HiddenOp<Pairs>>)(who, d_k, w_mn, nullptr, pp, !SPLIT, pp.pairs, sms, chain);
     if (rc == B2_OK && c.dw) {
-      const bool one = tiles_of<One>(count, width) <= sms;
+      const long long k = (rows + TILE_K - 1) / TILE_K;
+      const bool one = single_ctas<SPLIT>((tiles_of<One>(count, width) + sms - 1) / sms, k, (tiles_of<Pairs>(count, width) + pairs - 1) / pairs, k);
       rc = (one ? tile_launch<WeightOp<One>> : tile_launch<WeightOp<Pairs>>)(who, d_mn, h_mn, pp.by_tma ? &dw_out : nullptr, pp, !SPLIT,
                                                                              one ? tiles_of<One>(count, width) : tiles_of<Pairs>(count, width), sms, chain);
     }
@@ -963,7 +1106,7 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
   }
   if (c.dh) {
     const int vec = c.ld_dh % 4 == 0 && reinterpret_cast<uintptr_t>(c.dh) % (4 * sizeof(T)) == 0;
-    chain.launch(spread_rows_kernel<T>, dim3(blocks(rows)), 256, 0, 0, pp, s.slot_of, rows, vec, static_cast<T*>(c.dh), c.ld_dh);
+    chain.launch(h_one ? spread_rows_kernel<T, One> : spread_rows_kernel<T, Pairs>, dim3(blocks(rows)), 256, 0, 0, pp, s.slot_of, rows, vec, static_cast<T*>(c.dh), c.ld_dh);
     rc = launch_error(chain.err, who);
   }
   return rc;

@@ -120,6 +120,21 @@ def test_many_rows(lm, dtype, rows, width, vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows,width,vocab", [(1, 3973, 806), (23, 2000, 9472), (290, 1100, 130), (297, 1100, 130), (64, 1500, 1), (130, 2049, 4099), (1100, 900, 1200)])
+def test_few_tiles(lm, dtype, rows, width, vocab):
+    """Long sums in parts and whole, with gradients and without."""
+    h, w, t = _case(rows, width, vocab, dtype)
+    got = lm.xent(h, w, t)
+    _check(h, w, t, 1.0, got, dtype)
+    assert torch.equal(lm.xent(h, w, t, grad=False), got[0])
+    t[:] = -100
+    loss, dh, dw = lm.xent(h, w, t)
+    assert not loss.any() and not dh.any() and not dw.any()
+    lm.sync()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,rows,width,vocab", [
     ("bf16", 10, 8, 1400001), ("fp32", 20, 8, 700001),  # few rows: logits are kept, d goes in pieces
     ("bf16", 600, 2048, 30001), ("fp32", 300, 264, 60002),  # kept although they are more than the L2 cache should hold

@@ -176,7 +176,19 @@ __global__ void __launch_bounds__(FRONT_THREADS) front_kernel(const __grid_const
     const int block = blockIdx.x - p.blocks_h;
     auto same = [](int k) { return k; };
     if constexpr (SPLIT) {
-      const unsigned int most = block_max(max_rows(w, p.ldw, p.vocab, block, p.blocks_w, p.width, same), warp_sum);
+      unsigned int most = 0;
+      if (p.ldw == p.width && reinterpret_cast<uintptr_t>(w) % 16 == 0) {  // rows without gaps: one list of elements, whatever the width
+        const long long all = (long long)p.vocab * p.width, step = (long long)p.blocks_w * FRONT_THREADS;
+#pragma unroll 4
+        for (long long i = (long long)block * FRONT_THREADS + threadIdx.x; i < all / 4; i += step) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(w) + i);
+          most = max(most, max(max(finite_bits(v.x), finite_bits(v.y)), max(finite_bits(v.z), finite_bits(v.w))));
+        }
+        if (block == 0 && threadIdx.x < (all & 3)) most = max(most, finite_bits(__float_as_uint(__ldg(w + (all & ~3ll) + threadIdx.x))));
+      } else {
+        most = max_rows(w, p.ldw, p.vocab, block, p.blocks_w, p.width, same);
+      }
+      most = block_max(most, warp_sum);
       if (threadIdx.x == 0) p.most[blockIdx.x] = most;
     } else {
       copy_rows(w, p.ldw, p.vocab, block, p.blocks_w, p.width, p.pitch, 1.f, p.w_hi, p.w_lo, 0, same);
@@ -265,6 +277,7 @@ struct LogitParams {
   int vocab, v_begin, v_count;  // this call's piece of the vocabulary
   int kblocks;
   long long row_pitch;  // rows of the lists: parts are [warp of a tile's row][row]
+  int run;              // all tiles have the same rows: a warp goes on with its maximum and sum, and parts are [warp][row]
   const int* target;
   float2* parts;        // maximum (times log2 e) and sum of 2^(x - maximum)
   float* target_logit;  // times log2 e
@@ -347,14 +360,18 @@ struct StatOp : LogitTiles<F> {
   float top, sum;
   int target;
   __device__ explicit StatOp(const LogitParams& q, const TileMaps& m) : LogitTiles<F>(q, m) {}
+  bool begun = false;
   __device__ __forceinline__ void begin(const Tile&, int row0, int, int lane) {
-    top = -INFINITY;
-    sum = 0.f;
+    if (!begun) {
+      top = -INFINITY;
+      sum = 0.f;
+    }
+    begun = p.run;
     target = row0 + lane < this->rows ? __ldg(p.target + row0 + lane) : -1;
   }
   static constexpr int W = LONG ? 16 : LogitTiles<F>::W;
   __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[W], uint8_t* stage, int lane) {
-    if (col0 >= p.vocab) return;
+    if (col0 >= p.vocab || row0 >= this->rows) return;
     if (KEEP)
       by_rows(row0, col0, v, stage, lane, [&](int, int r, int c, const float4& x) {
         if (r < this->rows && c < p.vocab) *reinterpret_cast<float4*>(p.x + r * p.ld_x + c) = x;
@@ -383,7 +400,8 @@ struct StatOp : LogitTiles<F> {
     }
   }
   __device__ __forceinline__ void end(const Tile& t, int row, int part) {
-    if (row < this->rows) p.parts[(long long)(t.n0 / F::BN * F::PARTS + part) * p.row_pitch + row] = make_float2(top, sum);
+    const int list = p.run ? blockIdx.x / F::CTAS : t.n0 / F::BN;
+    if (row < this->rows) p.parts[(long long)(list * F::PARTS + part) * p.row_pitch + row] = make_float2(top, sum);
   }
 };
 
@@ -864,19 +882,26 @@ struct Sizes {
 constexpr int MOST_PAIRS = 74;  // 148 SMs
 template <class F>
 long long tiles_of(long long m, long long n) { return (m + F::M - 1) / F::M * ((n + F::BN - 1) / F::BN); }
-// Single CTAs take over when each has one tile at most. Where they would leave SMs idle through a long k range, it goes in parts, and
-// row_kernel takes its time for each of a few rows (with gradients 1 x 3972 x 806 in fp32 84 -> 74 us, 75 x 1152 x 2411 in bf16 43 -> 38).
+// Where single CTAs would leave SMs idle through a long k range, it goes in parts, and row_kernel takes its time for each of a few rows
+// (with gradients 1 x 3972 x 806 in fp32 84 -> 74 us, 75 x 1152 x 2411 in bf16 43 -> 38).
+template <class F>
+int lists_of(size_t rows, size_t vocab, int sms, int* run) {  // per row: for one block of rows (*run) a list per warp, else per tile and warp
+  const long long tiles = ((long long)vocab + F::BN - 1) / F::BN, most = sms / F::CTAS;
+  *run = rows <= F::M;
+  return (int)(F::PARTS * (*run && tiles > most ? most : tiles));
+}
 template <class F>
 void logit_sizes(Sizes* z, size_t rows, size_t width, size_t vocab) {  // F: single CTAs
   typedef TileForm<F::SPLIT> Pairs;
-  const long long tiles = tiles_of<F>(rows, vocab), kblocks = (long long)(width + TILE_K - 1) / TILE_K;
-  z->one = tiles <= 2 * MOST_PAIRS;
-  long long parts = z->one ? 2 * MOST_PAIRS / tiles : 1;
+  const int sms = 2 * MOST_PAIRS;
+  const long long one = tiles_of<F>(rows, vocab), pairs = tiles_of<Pairs>(rows, vocab), kblocks = (long long)(width + TILE_K - 1) / TILE_K;
+  z->one = single_ctas<F::SPLIT>((one + sms - 1) / sms, kblocks, (pairs + MOST_PAIRS - 1) / MOST_PAIRS, kblocks);
+  long long parts = z->one ? sms / one : 1;
   if (parts > kblocks / 4) parts = kblocks / 4;
   z->by_rows = parts > 1 && kblocks - kblocks / parts >= 8 && rows <= 4 * MOST_PAIRS && vocab <= ROW_QUADS * 4 * ROW_THREADS;
   z->x_parts = z->by_rows ? (int)parts : 1;
-  const int bn = z->one ? F::BN : Pairs::BN;
-  z->parts = z->by_rows ? 0 : F::PARTS * (((long long)vocab + bn - 1) / bn);
+  int run;
+  z->parts = z->by_rows ? 0 : z->one ? lists_of<F>(rows, vocab, sms, &run) : lists_of<Pairs>(rows, vocab, sms, &run);
 }
 // Logits that are kept cost their bytes twice, others 2 F operations each again. What stays in the L2 cache is kept (1024 x 512 x 8192 in
 // fp32 140 -> 125 us, 16 x 2048 x 65536 in bf16 251 -> 217); beyond it the operations cost more with three MMAs or great widths (2048 x
@@ -1048,10 +1073,11 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
     };
     const std::true_type yes;
     const std::false_type no;
+    const int lists = z.one ? lists_of<One>(rows, vocab, sms, &lp.run) : lists_of<Pairs>(rows, vocab, sms, &lp.run);
     auto stat = z.one ? (z.keep ? stat_of(One(), yes) : stat_of(One(), no)) : (z.keep ? stat_of(Pairs(), yes) : stat_of(Pairs(), no));
     rc = stat(who, h_k, w_k, nullptr, lp, !SPLIT, z.one ? tiles_of<One>(rows, vocab) : tiles_of<Pairs>(rows, vocab), sms, chain);
     if (rc != B2_OK) return rc;
-    chain.launch(join_rows_kernel, dim3((rows + 31) / 32), 1024, 0, 0, s.parts, z.rows_up, (int)z.parts, s.meta, s.target_logit, s.row_of, s.row_stat,
+    chain.launch(join_rows_kernel, dim3((rows + 31) / 32), 1024, 0, 0, s.parts, z.rows_up, lists, s.meta, s.target_logit, s.row_of, s.row_stat,
                  c.row_loss);
   }
   rc = launch_error(chain.err, who);

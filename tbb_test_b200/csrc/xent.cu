@@ -7,12 +7,13 @@
 // computed a second time when their row's maximum and sum are known, instead of R x V of them being kept (keeps_logits).
 // It is bound by the tensor cores (tile kernels of lm_tile.cuh) unless R is small, when reading w is what it takes.
 //
-//   1. Rows without a target are left out: the others' numbers are listed in order, their h copied one after another.
-//      So such a row costs nothing, and nothing in it (a NaN, say) reaches dw.
-//   2. Logits, 256 x 256 at a time; each row's maximum and sum over a tile's half go to a list.
+//   1. Rows without a target are left out: the others' numbers are listed in order, their h copied one after another (fp32: as pairs,
+//      and w too). So such a row costs nothing, and nothing in it (a NaN, say) reaches dw.
+//   2. Logits, a tile at a time; each row's maximum and sum over a warp's columns go to a list.
 //   3. The lists give each row's maximum and sum, and the loss.
 //   4. Per piece of the vocabulary: d from logits that are kept or computed again to a buffer of R x piece; dh += d w; dw of the
 //      piece = d' h.
+// A few rows with few tiles of long sums: the logits go out in parts of the k range, and 3 and d are one kernel with a block per row.
 //
 // Precision: bf16 matrices are multiplied as they are, with fp32 sums; d is rounded to bf16 once, as the
 // gradients are in the end. fp32 matrices are

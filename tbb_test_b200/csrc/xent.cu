@@ -1192,6 +1192,7 @@ int b2_xent(size_t rows, size_t width, size_t vocab, int dtype, const void* h, s
   }
   int sms;
   if ((rc = lm_device(&sms)) != B2_OK) return rc;
+  if (sms > 2 * MOST_PAIRS) sms = 2 * MOST_PAIRS;  // what the workspace is made for
   if (rows == 0) return dw ? launch_error(cudaMemset2DAsync(dw, ld_dw * e, 0, width * e, vocab, st), "b2_xent") : B2_OK;
   const XentCall c{rows, width, vocab, dtype, h, ldh, w, ldw, targets, token_bytes == 8, scale, row_loss, dh, ld_dh, dw, ld_dw};
   return z.split ? xent_run<true>(c, z, s, sms, st) : xent_run<false>(c, z, s, sms, st);

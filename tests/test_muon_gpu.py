@@ -100,6 +100,26 @@ def test_forms_of_products(lm, count, rows, cols):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("count,rows,cols", [(1, 64, 2050), (3, 300, 500), (2, 1030, 70), (2, 1500, 1600)])
+def test_what_the_workspace_held_does_not_matter(lm, count, rows, cols):
+    import ctypes as ct
+    from tbb_test_b200 import _capi as K
+    w, m, g = _make(count, rows, cols, torch.float32)
+    need, options, out = ct.c_size_t(), K.MuonOptions(), []
+    assert K.lib().b2_muon_workspace(count, rows, cols, ct.byref(need)) == 0
+    K.lib().b2_muon_options_default(ct.byref(options))
+    for fill in (0, 255):
+        space = torch.full((need.value,), fill, dtype=torch.uint8, device="cuda")
+        w2, m2 = w.clone(), m.clone()
+        lists = [(ct.c_void_p * count)(*[x.data_ptr() for x in xs]) for xs in (w2, m2, g)]
+        assert K.lib().b2_muon(count, rows, cols, 0, lists[0], cols, None, 0, lists[1], cols, lists[2], cols, ct.byref(options), space.data_ptr(), need.value,
+                               torch.cuda.current_stream().cuda_stream) == 0
+        lm.sync()
+        out.append((w2, m2))
+    assert all(bool(torch.isfinite(x).all()) and torch.equal(x, y) for x, y in zip(*out))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("steps", [1, 3, 7])
 def test_steps_and_low_rank(lm, steps):
     w, m, g = _make(2, 200, 333, torch.float32, low_rank=True)

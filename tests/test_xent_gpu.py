@@ -147,6 +147,27 @@ def test_logits_kept_or_computed_again(lm, dtype, rows, width, vocab):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows,width,vocab", [(1, 8, 300), (5, 1500, 700), (70, 200, 1000), (300, 100, 3001), (300, 64, 40000), (3000, 200, 6003)])
+def test_what_the_workspace_held_does_not_matter(lm, dtype, rows, width, vocab):
+    """NaN everywhere, in every type, against zeros: equal bits."""
+    import ctypes as ct
+    from tbb_test_b200 import _capi as K
+    h, w, t = _case(rows, width, vocab, dtype)
+    kind, out = 1 if dtype == "bf16" else 0, []
+    need = ct.c_size_t()
+    assert K.lib().b2_xent_workspace(rows, width, vocab, kind, 1, w.data_ptr(), width, ct.byref(need)) == 0
+    for fill in (0, 255):
+        space = torch.full((need.value,), fill, dtype=torch.uint8, device="cuda")
+        loss, dh, dw = torch.zeros(rows, device="cuda"), torch.zeros_like(h), torch.zeros_like(w)
+        assert K.lib().b2_xent(rows, width, vocab, kind, h.data_ptr(), width, w.data_ptr(), width, t.data_ptr(), 8, 1.0, loss.data_ptr(), dh.data_ptr(),
+                               width, dw.data_ptr(), width, space.data_ptr(), need.value, torch.cuda.current_stream().cuda_stream) == 0
+        lm.sync()
+        out.append((loss, dh, dw))
+    assert all(bool(torch.isfinite(x).all()) and torch.equal(x, y) for x, y in zip(*out))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_rows_without_a_target(lm, dtype):
     """They cost nothing and nothing of them gets out, not even NaN; a call of such rows alone gives zeros."""
     h, w, t = _case(500, 96, 700, dtype, padding=0.0)

@@ -278,7 +278,6 @@ struct LogitParams {
   int vocab, v_begin, v_count;  // this call's piece of the vocabulary
   int kblocks;
   long long row_pitch;  // rows of the lists: parts are [warp of a tile's row][row]
-  int run;              // all tiles have the same rows: a warp goes on with its maximum and sum, and parts are [warp][row]
   const int* target;
   float2* parts;        // maximum (times log2 e) and sum of 2^(x - maximum)
   float* target_logit;  // times log2 e
@@ -350,8 +349,8 @@ struct PlainOp : LogitTiles<F> {
 
 // Maximum and sum of exponentials of a row over the columns of one warp, and the target's logit. LONG: for more than 16 k-blocks,
 // whose sums the tensor core would leave too small (bf16, width 2048: losses 1.0e-6 off, with sums of 16 added in fp32 0.5e-6, in the
-// same time).
-template <class F, bool LONG_, bool KEEP>
+// same time). RUN: all tiles have the same rows, so a warp goes on with its maximum and sum, and lists are [warp][row].
+template <class F, bool LONG_, bool KEEP, bool RUN>
 struct StatOp : LogitTiles<F> {
   typedef LogitParams Params;
   static constexpr bool LONG = F::SPLIT || LONG_;
@@ -363,11 +362,11 @@ struct StatOp : LogitTiles<F> {
   __device__ explicit StatOp(const LogitParams& q, const TileMaps& m) : LogitTiles<F>(q, m) {}
   bool begun = false;
   __device__ __forceinline__ void begin(const Tile&, int row0, int, int lane) {
-    if (!begun) {
+    if (!RUN || !begun) {
       top = -INFINITY;
       sum = 0.f;
     }
-    begun = p.run;
+    begun = true;
     target = row0 + lane < this->rows ? __ldg(p.target + row0 + lane) : -1;
   }
   static constexpr int W = LONG ? 16 : LogitTiles<F>::W;
@@ -401,7 +400,7 @@ struct StatOp : LogitTiles<F> {
     }
   }
   __device__ __forceinline__ void end(const Tile& t, int row, int part) {
-    const int list = p.run ? blockIdx.x / F::CTAS : t.n0 / F::BN;
+    const int list = RUN ? blockIdx.x / F::CTAS : t.n0 / F::BN;
     if (row < this->rows) p.parts[(long long)(list * F::PARTS + part) * p.row_pitch + row] = make_float2(top, sum);
   }
 };
@@ -1066,16 +1065,19 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
     if (rc != B2_OK) return rc;
     chain.launch(row_kernel<SPLIT>, dim3((rows + TILE_K - 1) / TILE_K * TILE_K), ROW_THREADS, 0, 0, lp, s.row_of, c.row_loss, grads);
   } else {
-    const bool sums = !SPLIT && lp.kblocks > StatOp<Pairs, true, false>::SUM;
-    auto stat_of = [&](auto form, auto keep) {
-      typedef decltype(form) F;
-      constexpr bool KEEP = decltype(keep)::value;
-      return sums ? tile_launch<StatOp<F, !SPLIT, KEEP>> : tile_launch<StatOp<F, false, KEEP>>;
-    };
+    const bool sums = !SPLIT && lp.kblocks > StatOp<Pairs, true, false, false>::SUM;
+    int run;
+    const int lists = z.one ? lists_of<One>(rows, vocab, sms, &run) : lists_of<Pairs>(rows, vocab, sms, &run);
     const std::true_type yes;
     const std::false_type no;
-    const int lists = z.one ? lists_of<One>(rows, vocab, sms, &lp.run) : lists_of<Pairs>(rows, vocab, sms, &lp.run);
-    auto stat = z.one ? (z.keep ? stat_of(One(), yes) : stat_of(One(), no)) : (z.keep ? stat_of(Pairs(), yes) : stat_of(Pairs(), no));
+    auto by_run = [&](auto form, auto keep, auto goes_on) {
+      typedef decltype(form) F;
+      constexpr bool KEEP = decltype(keep)::value, RUN = decltype(goes_on)::value;
+      return sums ? tile_launch<StatOp<F, !SPLIT, KEEP, RUN>> : tile_launch<StatOp<F, false, KEEP, RUN>>;
+    };
+    auto by_keep = [&](auto form, auto keep) { return run ? by_run(form, keep, yes) : by_run(form, keep, no); };
+    auto stat_of = [&](auto form) { return z.keep ? by_keep(form, yes) : by_keep(form, no); };
+    auto stat = z.one ? stat_of(One()) : stat_of(Pairs());
     rc = stat(who, h_k, w_k, nullptr, lp, !SPLIT, z.one ? tiles_of<One>(rows, vocab) : tiles_of<Pairs>(rows, vocab), sms, chain);
     if (rc != B2_OK) return rc;
     chain.launch(join_rows_kernel, dim3((rows + 31) / 32), 1024, 0, 0, s.parts, z.rows_up, lists, s.meta, s.target_logit, s.row_of, s.row_stat,

@@ -479,8 +479,8 @@ __global__ void __launch_bounds__(RUN_THREADS) run_sum_ring_kernel(const RunSum 
 
 // Runs that cross chunk borders: the tail of the chunk a run begins in and the heads of the chunks behind it, JOIN_PARTS
 // contiguous shares of them side by side, which are then added in order. A block takes 128 columns of a run at a time. Short
-// lists, whose sort has no room for it, leave zeroing rows to the blocks before these; it needs no sums, so these blocks do not
-// wait for the kernel before, which has waited for the sorted list before this one starts.
+// lists, whose sort has no room for it, leave zeroing rows to the blocks before these; it needs no sums, so these blocks
+// wait for the kernel before only when they are done: it has waited for the sorted list before this one starts.
 constexpr int JOIN_PARTS = 4, JOIN_THREADS = 32 * JOIN_PARTS;
 template <typename T>
 __global__ void __launch_bounds__(JOIN_THREADS) run_join_kernel(const RunSum p, const Fill fill, int width) {
@@ -489,6 +489,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) run_join_kernel(const RunSum p, 
   let_next_start();
   if (blockIdx.x < p.fill_blocks) {
     fill_rows(fill, blockIdx.x * JOIN_PARTS + share, lane);
+    after_previous();  // up to eight tokens have no runs to join: then these blocks' end is the call's, and has to be behind the sums
     return;
   }
   after_previous();

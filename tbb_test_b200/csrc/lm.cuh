@@ -42,8 +42,9 @@ struct Carver {
 
 // The kernels of a call follow one another by programmatic dependent launch: a kernel may be set up while the one before it
 // ends, and waits in after_previous() until that one's results are there. `first` kernels of a call are launched in the
-// ordinary way, behind whatever the caller's stream holds. Every kernel calls both functions before it reads or writes anything
-// that another kernel of the call touches.
+// ordinary way, behind whatever the caller's stream holds. Every kernel but the first calls after_previous() in all its blocks before it
+// reads or writes anything that the kernel before writes or reads, and in any case before a block ends: only then is the end of a
+// kernel, which the next one and whatever follows the call wait for, behind the ends of all kernels before it.
 __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

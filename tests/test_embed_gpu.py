@@ -151,6 +151,46 @@ def test_in_a_graph(lm):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("n", range(1, 10))
+def test_few_tokens_end_behind_their_sums(lm, n, graph):
+    """Up to eight tokens are one chunk, whose runs nothing joins. What follows on the stream finds whole sums, and may write over the
+    gradient's input and the workspace."""
+    import ctypes as C
+    from tbb_test_b200 import _capi as K
+    vocab, width = 40, 8192
+    t = _tokens(n, vocab, "any", n)
+    dout = _rows(n, width, "fp32", n)
+    want = torch.zeros(vocab, width, device="cuda", dtype=torch.float64).index_add_(0, t, dout.double())
+    size = torch.zeros(vocab, width, device="cuda", dtype=torch.float64).index_add_(0, t, dout.double().abs())
+    kept, out, need = dout.clone(), torch.empty(vocab, width, device="cuda"), C.c_size_t()
+    assert K.lib().b2_embed_grad_workspace(n, vocab, width, C.byref(need)) == K.OK
+    space, got = torch.empty(need.value, dtype=torch.uint8, device="cuda"), torch.empty_like(out)
+
+    def call():
+        dout.copy_(kept)
+        assert K.lib().b2_embed_grad(t.data_ptr(), 8, n, dout.data_ptr(), 0, width, vocab, width, 1.0, out.data_ptr(), width, space.data_ptr(),
+                                     space.numel(), torch.cuda.current_stream().cuda_stream) == K.OK
+        got.copy_(out)
+        dout.fill_(float("nan"))
+        space.fill_(255)
+        out.fill_(float("nan"))
+
+    call()
+    torch.cuda.synchronize()
+    run = call
+    if graph:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call()
+        run = g.replay
+    for _ in range(20):
+        got.zero_()
+        run()
+        assert bool(((got.double() - want).abs() <= size * (n + 1) * 2.0 ** -24 + want.abs() * EPS["fp32"] * 1.01).all())
+
+
+@pytest.mark.gpu
 def test_wrapper_refuses(lm):
     table = torch.zeros(8, 16, device="cuda")
     t = torch.zeros(4, dtype=torch.int64, device="cuda")

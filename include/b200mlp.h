@@ -444,7 +444,9 @@ int b2_muon(int count, int rows, int cols, int grad_dtype, float* const* w, size
             const b2_muon_options* options, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Waits for `stream` and returns B2_ERR_TIMEOUT if a bounded wait inside one of this section's tensor-core kernels on
- * the current device gave up since the last call (their results are then not valid), B2_OK otherwise. */
+ * the current device gave up since the last b2_lm_sync of the same stream (at its first: since the library was loaded), B2_OK otherwise.
+ * The kernels cannot tell whose call it was, so every stream is told, once each: after B2_ERR_TIMEOUT no result since that
+ * stream's last B2_OK is to be relied on, and a caller on another stream still learns of it. */
 int b2_lm_sync(void* stream);
 
 #ifdef __cplusplus

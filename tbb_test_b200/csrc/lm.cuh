@@ -15,9 +15,8 @@ int call_error(int code, const char* fmt, ...) __attribute__((format(printf, 2, 
 // B2_OK where the calling thread's device can run this library's kernels; *sms = its multiprocessors.
 int lm_device(int* sms);
 
-// The status words of the tile kernels of xent.cu and muon.cu (lm_tile.cuh): waits for the stream, reads and clears.
-cudaError_t xent_status_take(unsigned int* code, cudaStream_t s);
-cudaError_t muon_status_take(unsigned int* code, cudaStream_t s);
+// The report of xent.cu's tile kernels (lm_tile.cuh): CTAs in which a wait gave up, and the first one's role. Waits for the stream.
+cudaError_t xent_waits_given_up(unsigned int* count, unsigned int* role, cudaStream_t s);
 
 namespace {
 

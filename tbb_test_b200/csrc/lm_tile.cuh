@@ -41,8 +41,11 @@ constexpr float LO_UP = 2048.f;  // lo = 2^11 (x - hi)
 constexpr uint32_t ACC_COLS = 256;  // tensor-memory columns of an accumulator stage
 constexpr int TILE_MAX_STAGES = 6;
 
-// A wait that gave up leaves its role's number here; b2_lm_sync reports and clears it.
-__device__ unsigned int tile_status;
+// CTAs in which a wait gave up, and the number of the role that was first to; never cleared (b2_lm_sync reports what is new).
+struct TileReport {
+  unsigned int count, role;
+};
+__device__ TileReport tile_report;
 
 template <bool SPLIT_, bool ONE_ = false>
 struct TileForm {
@@ -184,7 +187,7 @@ __global__ void __launch_bounds__(Op::Form::BOUND, 1) tile_kernel(const __grid_c
         const Tile tile = op.tile(t);
         const int am = tile.a_mn + (int)rank * 128, bn = tile.b_mn + (int)rank * F::B_ROWS;
         for (int kb = 0; kb < tile.kblocks; ++kb) {
-          if (!mbar_wait(empty0 + 8u * stage, phase ^ 1, abort_flag, &tile_status, 1u)) { ok = false; break; }
+          if (!mbar_wait(empty0 + 8u * stage, phase ^ 1, abort_flag, &tile_report.role, 1u)) { ok = false; break; }
           const uint32_t s0 = ring0 + (uint32_t)stage * F::SLABS;
           if (rank == 0) mbar_expect_tx(smem_u32(full_bar) + 8u * stage, F::CTAS * F::SLABS);  // both CTAs' bytes
           const uint32_t full = full0 + 8u * stage;
@@ -218,10 +221,10 @@ __global__ void __launch_bounds__(Op::Form::BOUND, 1) tile_kernel(const __grid_c
         for (int kb = 0; kb < kblocks; ++kb) {
           const bool first = kb == 0 || (Op::LONG && kb % Op::SUM == 0);
           if (first) {
-            if (!mbar_wait(&acc_empty_bar[acc], acc_phase ^ 1, abort_flag, &tile_status, 2u)) { ok = false; break; }
+            if (!mbar_wait(&acc_empty_bar[acc], acc_phase ^ 1, abort_flag, &tile_report.role, 2u)) { ok = false; break; }
             tc_fence_after();
           }
-          if (!mbar_wait(full0 + 8u * stage, phase, abort_flag, &tile_status, 3u)) { ok = false; break; }
+          if (!mbar_wait(full0 + 8u * stage, phase, abort_flag, &tile_report.role, 3u)) { ok = false; break; }
           tc_fence_after();
           const uint32_t d = tmem_base + (uint32_t)acc * ACC_COLS;
           const uint32_t off = ((uint32_t)stage * F::SLABS) >> 4;
@@ -271,7 +274,7 @@ __global__ void __launch_bounds__(Op::Form::BOUND, 1) tile_kernel(const __grid_c
           for (int c = 0; c < F::COLS; ++c) sum[c] = 0.f;
         }
         for (int kb = 0; kb < tile.kblocks; kb += Op::SUM) {
-          if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_flag, &tile_status, 4u)) { ok = false; break; }
+          if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_flag, &tile_report.role, 4u)) { ok = false; break; }
           tc_fence_after();
           const uint32_t from = place + (uint32_t)acc * ACC_COLS;
           uint32_t r[F::COLS], x[F::COLS];
@@ -303,7 +306,7 @@ __global__ void __launch_bounds__(Op::Form::BOUND, 1) tile_kernel(const __grid_c
 #pragma unroll
         for (int c = 0; c < F::COLS; ++c) sum[c] = 0.f;
         for (int kb = 0; kb < tile.kblocks; kb += Op::SUM) {
-          if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_flag, &tile_status, 4u)) { ok = false; break; }
+          if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_flag, &tile_report.role, 4u)) { ok = false; break; }
           tc_fence_after();
           const uint32_t from = place + (uint32_t)acc * ACC_COLS;
           if (kb + Op::SUM < tile.kblocks) {
@@ -335,7 +338,7 @@ __global__ void __launch_bounds__(Op::Form::BOUND, 1) tile_kernel(const __grid_c
       } else {
         const bool summed = tile.kblocks > 0;
         if (summed) {
-          if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_flag, &tile_status, 4u)) break;
+          if (!mbar_wait(&acc_full_bar[acc], acc_phase, abort_flag, &tile_report.role, 4u)) break;
           tc_fence_after();
         }
         const uint32_t from = place + (uint32_t)acc * ACC_COLS;
@@ -371,6 +374,7 @@ __global__ void __launch_bounds__(Op::Form::BOUND, 1) tile_kernel(const __grid_c
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if (abort_s && threadIdx.x == 0) atomicAdd(&tile_report.count, 1u);
   if (PAIR) cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();
@@ -550,16 +554,10 @@ int tile_launch(const char* who, const TileOperand& a, const TileOperand& b, con
   return launch_error(chain.err, who);
 }
 
-// What a wait that gave up left in this file's status word, which is cleared; the stream is waited for.
-inline cudaError_t tile_status_take(unsigned int* code, cudaStream_t s) {
-  const unsigned int zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbolAsync(code, tile_status, sizeof *code, 0, cudaMemcpyDeviceToHost, s);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-  if (e == cudaSuccess && *code) {
-    e = cudaMemcpyToSymbolAsync(tile_status, &zero, sizeof zero, 0, cudaMemcpyHostToDevice, s);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-  }
-  return e;
+// This file's report, behind the stream's work, which is waited for.
+inline cudaError_t tile_report_read(TileReport* r, cudaStream_t s) {
+  cudaError_t e = cudaMemcpyFromSymbolAsync(r, tile_report, sizeof *r, 0, cudaMemcpyDeviceToHost, s);
+  return e == cudaSuccess ? cudaStreamSynchronize(s) : e;
 }
 
 }  // namespace

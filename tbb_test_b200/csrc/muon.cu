@@ -19,6 +19,7 @@
 // Matrices of a call have one shape and go side by side, so that small ones fill the GPU together. Sides are rounded up to
 // 64, a k-block, with zeros, which stay zeros.
 #include "lm_tile.cuh"
+#include "wait_reports.h"
 
 namespace b2 {
 namespace {
@@ -561,8 +562,6 @@ int check_muon(const char* who, int count, int rows, int cols) {
 
 }  // namespace
 
-cudaError_t muon_status_take(unsigned int* code, cudaStream_t s) { return tile_status_take(code, s); }
-
 }  // namespace b2
 
 using namespace b2;
@@ -625,13 +624,25 @@ int b2_muon(int count, int rows, int cols, int grad_dtype, float* const* w, size
 }
 
 int b2_lm_sync(void* stream) {
-  int sms, rc = lm_device(&sms);
+  static WaitReports reports;
+  int sms, dev = 0, rc = lm_device(&sms);
   if (rc != B2_OK) return rc;
-  unsigned int a = 0, b = 0;
-  cudaError_t e = xent_status_take(&a, static_cast<cudaStream_t>(stream));
-  if (e == cudaSuccess) e = muon_status_take(&b, static_cast<cudaStream_t>(stream));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  unsigned int xent = 0, role = 0;
+  unsigned long long id = 0;  // of a stream that is gone no other one gets it, unlike its address
+  TileReport own{};
+  cudaError_t e = xent_waits_given_up(&xent, &role, st);
+  if (e == cudaSuccess) e = tile_report_read(&own, st);
+  if (e == cudaSuccess) e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaStreamGetId(st, &id);
   if (e != cudaSuccess) return launch_error(e, "b2_lm_sync");
-  if (a || b) return call_error(B2_ERR_TIMEOUT, "a tile kernel gave up waiting on a pipeline barrier (role %u)", a ? a : b);
+  bool news = true;
+  try {
+    news = reports.news(dev, id, xent + own.count);
+  } catch (...) {  // no memory to note what was told: it is told again
+    news = xent + own.count != 0;
+  }
+  if (news) return call_error(B2_ERR_TIMEOUT, "a tile kernel gave up waiting on a pipeline barrier (role %u)", role ? role : own.role);
   return B2_OK;
 }
 

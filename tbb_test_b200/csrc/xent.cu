@@ -1152,7 +1152,13 @@ int check_sizes(const char* who, size_t rows, size_t width, size_t vocab, int dt
 
 }  // namespace
 
-cudaError_t xent_status_take(unsigned int* code, cudaStream_t s) { return tile_status_take(code, s); }
+cudaError_t xent_waits_given_up(unsigned int* count, unsigned int* role, cudaStream_t s) {
+  TileReport r{};
+  const cudaError_t e = tile_report_read(&r, s);
+  *count = r.count;
+  *role = r.role;
+  return e;
+}
 
 }  // namespace b2
 

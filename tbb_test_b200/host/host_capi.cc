@@ -11,6 +11,7 @@
 #include "../csrc/simt_tile.h"
 #include "../csrc/step_choice.h"
 #include "../csrc/tile_choice.h"
+#include "../csrc/wait_reports.h"
 #include "HyperCubeAllReduce.h"
 #include "b2_rng.h"
 #include "TwistedHyperCube.h"
@@ -164,6 +165,12 @@ void b2h_downloads(int n, const size_t* width, const size_t* rows, int cores, si
 
 // Tile of the CUDA-core GEMM for small fp32 grids (csrc/simt_tile.h), 0 where the general kernel serves.
 int b2h_f32_tile(int m, int n, int whole_pieces) { return b2::f32_tile(m, n, whole_pieces != 0, 148); }
+
+// What streams that ask one after the other are told of waits that gave up (csrc/wait_reports.h): 0 or 1 each.
+void b2h_wait_reports(int n, const int* device, const unsigned long long* stream, const unsigned int* count, int* out) {
+  b2::WaitReports reports;
+  for (int i = 0; i < n; ++i) out[i] = reports.news(device[i], stream[i], count[i]);
+}
 
 void b2h_ring_info(int nsock, int sid, int task, int* out3) {
   nsockets = nsock;

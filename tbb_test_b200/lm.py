@@ -187,7 +187,8 @@ def muon(w, momentum_buffer, grad, *, lr, momentum=0.95, nesterov=True, weight_d
 
 
 def sync(device=None):
-    """Waits for the current stream of `device`; K.B2Error with code ERR_TIMEOUT if a bounded wait of a kernel gave up."""
+    """Waits for the current stream of `device`; K.B2Error with code ERR_TIMEOUT if a bounded wait of a kernel on the device gave up
+    since this stream last asked (see b2_lm_sync in include/b200mlp.h)."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     with _on(device) as stream:
         _ck(K.lib().b2_lm_sync(stream))

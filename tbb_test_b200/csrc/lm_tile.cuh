@@ -202,10 +202,6 @@ __global__ void __launch_bounds__(Op::Form::BOUND, 1) tile_kernel(const __grid_c
           if (++stage == F::STAGES) { stage = 0; phase ^= 1; }
         }
       }
-      if (!ok) {  // copies in flight get a bounded time to land before the CTA retires
-        const unsigned long long t0 = globaltimer();
-        while (globaltimer() - t0 < 2000000ull) __nanosleep(1000);
-      }
     }
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
@@ -374,7 +370,14 @@ __global__ void __launch_bounds__(Op::Form::BOUND, 1) tile_kernel(const __grid_c
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (abort_s && threadIdx.x == 0) atomicAdd(&tile_report.count, 1u);
+  if (abort_s) {  // whichever role gave up: copies and MMAs in flight get a bounded time to end before their memory is given back
+    if (threadIdx.x == 0) {
+      atomicAdd(&tile_report.count, 1u);
+      const unsigned long long t0 = globaltimer();
+      while (globaltimer() - t0 < 2000000ull) __nanosleep(1000);
+    }
+    __syncthreads();
+  }
   if (PAIR) cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();

@@ -410,7 +410,8 @@ int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dou
  * makes computing them dearer), and larger ones are computed a second time in pieces of the vocabulary. Types: bf16 matrices
  * are multiplied as they are with fp32 sums, the logits' gradients rounded to bf16 once; fp32 matrices, and the
  * logits' gradients between them, at 22 bits of every element down to 2^-27 of the largest (1 for the latter) and to
- * 2^-50 of the largest below that. Equal inputs give equal bits. Limits: rows and vocab at most 2^24
+ * 2^-50 of the largest below that; a logit with an infinite element of w or h in it is infinite or NaN by the definition, and one of
+ * -inf a probability of 0, in either type. Equal inputs give equal bits. Limits: rows and vocab at most 2^24
  * each and 2^44 together, width at most 2^20. Fastest where w begins on a 16-byte boundary and ldw is a multiple of 8 (bf16); otherwise, and in fp32,
  * a copy of w goes to the workspace, which is why its size depends on `w` and `ldw`. `grads` is 1 where the call will
  * ask for dh or dw. For 1 / global batch as `scale` the gradients are this rank's share, as everywhere in this library. */

@@ -278,7 +278,9 @@ __global__ void __launch_bounds__(Op::Form::BOUND, 1) tile_kernel(const __grid_c
           tile_read(from + F::BN, x);
 #pragma unroll
           for (int j = 0; j < F::COLS; ++j) {
-            const float v = fmaf(__uint_as_float(x[j]), 1.f / LO_UP, __uint_as_float(r[j]));
+            const float main = __uint_as_float(r[j]);
+            // an infinite element's low half is not a number: the high halves alone say what its sums are
+            const float v = fabsf(main) < INFINITY ? fmaf(__uint_as_float(x[j]), 1.f / LO_UP, main) : main;
             sum[j] = kb == 0 ? v : sum[j] + v;
           }
           tc_fence_before();

@@ -18,7 +18,8 @@
 // Precision: bf16 matrices are multiplied as they are, with fp32 sums; d is rounded to bf16 once, as the
 // gradients are in the end. fp32 matrices are
 // split into fp16 pairs behind a power of two that brings the largest element to 2^14: 22 bits of an element down to 2^-27 of
-// the largest, and nothing finer than 2^-50 of it; d the same, with 1 for the largest. Maxima, sums and the losses are fp32.
+// the largest, and nothing finer than 2^-50 of it; d the same, with 1 for the largest. Infinite elements take no part in that: their
+// logits are infinite by the signs, or NaN, as in bf16. Maxima, sums and the losses are fp32.
 #include <type_traits>
 
 #include "lm_tile.cuh"
@@ -92,6 +93,15 @@ __host__ __device__ __forceinline__ int row_shift(int n) {
 }
 static_assert(FRONT_THREADS == 1 << 9, "a whole block");
 
+// An element as a pair, behind the scale. One that is too small for the high half gets the smallest number there, of its sign, and the rest in
+// the low one, whose steps are the same as they would be otherwise: times an infinity it is then not 0, which would make it NaN.
+__device__ __forceinline__ void split_scaled(float v, float up, __half& hi, __half& lo) {
+  const float x = v * up;
+  hi = __float2half_rn(x);
+  if (__half2float(hi) == 0.f && v != 0.f) hi = __ushort_as_half(v < 0.f ? 0x8001 : 0x0001);
+  lo = __float2half_rn((x - __half2float(hi)) * LO_UP);
+}
+
 // Rows first + k of a copy, for a block's share of the k below n: row of(k) of x, zeros behind `width` up to `pitch`, or zeros alone where
 // of(k) is negative.
 template <typename T, class Of>
@@ -117,7 +127,7 @@ __device__ __forceinline__ void copy_rows(const T* __restrict__ x, long long ld,
       if (SPLIT) {
         __half a[8], b[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) split_half((float)v[i] * up, a[i], b[i]);
+        for (int i = 0; i < 8; ++i) split_scaled((float)v[i], up, a[i], b[i]);
         *reinterpret_cast<uint4*>(hi + to + c) = *reinterpret_cast<const uint4*>(a);
         *reinterpret_cast<uint4*>(lo + to + c) = *reinterpret_cast<const uint4*>(b);
       } else {

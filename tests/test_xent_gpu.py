@@ -214,6 +214,56 @@ def test_infinity_stays_in_its_row_fp32(lm, size):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows,width,vocab", [(64, 32, 900), (5, 1500, 700), (300, 64, 40000), (3000, 200, 6003), (2, 2056, 5000)])
+def test_infinite_weights(lm, dtype, rows, width, vocab):
+    """A logit of -inf is a probability of 0, and only the columns of dh that its weight's infinity stands in are NaN (0 times infinity)."""
+    h, w, t = _case(rows, width, vocab, dtype, padding=0.0)
+    a, b = 3, width - 2
+    h[:, a], h[:, b] = 1.0, -0.5
+    h[-1, a] = 1e-20  # far below what the pair of fp16 matrices holds beside the others, but not 0
+    out = torch.tensor([7, vocab // 2, vocab - 1], device="cuda")
+    t[(t[:, None] == out).any(1)] = 8
+    for v, c, x in zip(out.tolist(), (a, b, a), (float("-inf"), float("inf"), float("-inf"))):
+        w[v, c] = x
+    got = lm.xent(h, w, t, scale=0.5)
+    lm.sync()
+    assert torch.equal(lm.xent(h, w, t, grad=False), got[0])
+    # what a vocabulary without those words gives
+    keep = torch.ones(vocab, dtype=torch.bool, device="cuda")
+    keep[out] = False
+    place = torch.cumsum(keep, 0) - 1
+    loss, dh, dw = got
+    assert bool(torch.isnan(dh[:, [a, b]]).all()) and not dw[out].any()
+    rest = torch.ones(width, dtype=torch.bool, device="cuda")
+    rest[[a, b]] = False
+    some = dh.clone()
+    x = h.double() @ w[keep].double().T
+    d = torch.softmax(x, 1)
+    d[torch.arange(rows, device="cuda"), place[t]] -= 1.0
+    some[:, ~rest] = (0.5 * d @ w[keep].double())[:, ~rest].to(dh.dtype)
+    _check(h, w[keep], place[t], 0.5, (loss, some, dw[keep]), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_infinite_weights_by_sign(lm, dtype):
+    """+inf in a row's logits, and 0 times infinity, make its loss NaN; the target's -inf makes it +inf."""
+    h, w, t = _case(40, 64, 500, dtype, padding=0.0)
+    t[:] = 3
+    t[5] = 11
+    w[11, 9] = float("-inf")
+    h[:, 9] = 0.25
+    h[1, 9], h[2, 9], h[3, 9] = -0.25, 0.0, -1e-20
+    loss = lm.xent(h, w, t, grad=False)
+    bad = torch.zeros(40, dtype=torch.bool, device="cuda")
+    bad[1:4] = True
+    assert bool(torch.isnan(loss[bad]).all()) and float(loss[5]) == float("inf")
+    bad[5] = True
+    assert bool(torch.isfinite(loss[~bad]).all())
+
+
+@pytest.mark.gpu
 def test_small_and_large_magnitudes_fp32(lm):
     """The split of fp32 matrices follows their largest element."""
     for a, b in ((1e-20, 1e20), (1e15, 1e-15), (1e-30, 1.0)):

@@ -457,23 +457,24 @@ __device__ __forceinline__ void by_columns(int row0, int col0, const float4 (&x)
   }
   __syncwarp();
 }
-// 32 columns of 16-bit elements into columns 32 * part and up of a buffer of 64, in the swizzle that TMA stores undo; with
-// the second part the buffer leaves for column col, row row of the map's matrix. The first part waits until the store
-// before has read the buffer.
-__device__ __forceinline__ void store_half_words(const CUtensorMap* map, const uint32_t (&w)[16], int part, int row, int col, uint8_t* stage,
-                                                 int lane) {
+// 2 N columns (16 or 32) of 16-bit elements, from column `col` of the map's matrix on, into their place in a buffer of 64 columns, in
+// the swizzle that TMA stores undo; with the last ones the buffer leaves. The first ones wait until the store before has
+// read the buffer.
+template <int N>
+__device__ __forceinline__ void store_half_words(const CUtensorMap* map, const uint32_t (&w)[N], int row, int col, uint8_t* stage, int lane) {
+  const int part = (col & 63) / (2 * N);
   if (part == 0) {
     if (lane == 0) bulk_wait_read<0>();
     __syncwarp();
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    *reinterpret_cast<uint4*>(stage + lane * 128 + (((part * 4 + j) ^ (lane & 7)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-  if (part == 1) {
+  for (int j = 0; j < N / 4; ++j)
+    *reinterpret_cast<uint4*>(stage + lane * 128 + (((part * (N / 4) + j) ^ (lane & 7)) << 4)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+  if (part == 32 / N - 1) {
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
-      tma_store_2d(map, stage, col, row);
+      tma_store_2d(map, stage, col & ~63, row);
       bulk_commit();
     }
   }

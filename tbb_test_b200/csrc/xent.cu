@@ -417,11 +417,14 @@ struct StatOp : LogitTiles<F> {
 
 // d of a piece, zeros in rows and columns that fill up tiles. What an element takes here bounds the kernel when width is small
 // (1024 and less: 8 us per tile before stores went by TMA and the target's column was a branch of its own, 5.8 us
-// of products), so it is one FMA, one exponential, one product and half a conversion.
-template <class F>
+// of products), so it is one FMA, one exponential, one product and half a conversion. Sums are handed over as in StatOp, so that the
+// logits are the same bits: where one pass truncates more than the other, a row's p do not add up to 1, and p - 1 of a target that is
+// nearly certain is wrong by as much (width 2000, logits of 65: off by as much as itself at p = 1 - 1e-4).
+template <class F, bool LONG_>
 struct GradOp : LogitTiles<F> {
   typedef LogitParams Params;
-  static constexpr bool LONG = F::SPLIT;
+  static constexpr bool LONG = F::SPLIT || LONG_;
+  static constexpr int SUM = StatOp<F, LONG_, false, false>::SUM;
   static constexpr bool STORES = !F::SPLIT;
   using LogitTiles<F>::p;
   const CUtensorMap* map;
@@ -439,7 +442,7 @@ struct GradOp : LogitTiles<F> {
     by = st.y * to;
     target = in ? __ldg(p.target + row) - p.v_begin : -1;
   }
-  static constexpr int W = LogitTiles<F>::W;
+  static constexpr int W = LONG ? 16 : LogitTiles<F>::W;
   __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[W], uint8_t* stage, int lane) {
 #pragma unroll
     for (int j = 0; j < W; ++j) v[j] = ex2(fmaf(v[j], this->unit, -top)) * by;
@@ -458,10 +461,10 @@ struct GradOp : LogitTiles<F> {
         store_pair(reinterpret_cast<__half*>(p.d_hi), reinterpret_cast<__half*>(p.d_lo), (long long)r * p.ld_d + c, x);
       });
     } else {
-      uint32_t w[16];
+      uint32_t w[W / 2];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
-      store_half_words(map, w, col0 >> 5 & 1, row0, col0 & ~63, stage, lane);
+      for (int j = 0; j < W / 2; ++j) w[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+      store_half_words(map, w, row0, col0, stage, lane);
     }
   }
   __device__ __forceinline__ void end(const Tile&, int, int) {}
@@ -805,7 +808,7 @@ struct WeightOp {
         uint32_t w[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) w[j] = pack_bf16(v[2 * j] * unit, v[2 * j + 1] * unit);
-        store_half_words(map, w, col0 >> 5 & 1, p.v_begin + row0, col0 & ~63, stage, lane);
+        store_half_words(map, w, p.v_begin + row0, col0, stage, lane);
         return;
       }
     }
@@ -1070,12 +1073,12 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
   lp.x_parts = z.x_parts;
   lp.all_rows = rows;
   const int grads = c.dh || c.dw;
+  const bool sums = !SPLIT && lp.kblocks > StatOp<Pairs, true, false, false>::SUM;
   if (z.by_rows) {
     rc = tile_launch<PlainOp<One>>(who, h_k, w_k, nullptr, lp, !SPLIT, tiles_of<One>(rows, vocab) * z.x_parts, sms, chain);
     if (rc != B2_OK) return rc;
     chain.launch(row_kernel<SPLIT>, dim3((rows + TILE_K - 1) / TILE_K * TILE_K), ROW_THREADS, 0, 0, lp, s.row_of, c.row_loss, grads);
   } else {
-    const bool sums = !SPLIT && lp.kblocks > StatOp<Pairs, true, false, false>::SUM;
     int run;
     const int lists = z.one ? lists_of<One>(rows, vocab, sms, &run) : lists_of<Pairs>(rows, vocab, sms, &run);
     const std::true_type yes;
@@ -1132,7 +1135,7 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
       chain.launch(kept_kernel<SPLIT>, dim3(blocks((r * n / 8 + 255) / 256)), 256, 0, 0, lp);
       rc = launch_error(chain.err, who);
     } else {
-      rc = tile_launch<GradOp<Pairs>>(who, h_k, w_k, SPLIT ? nullptr : &d_out, lp, !SPLIT, tiles_of<Pairs>(rows, count), sms, chain);
+      rc = (sums ? tile_launch<GradOp<Pairs, !SPLIT>> : tile_launch<GradOp<Pairs, false>>)(who, h_k, w_k, SPLIT ? nullptr : &d_out, lp, !SPLIT, tiles_of<Pairs>(rows, count), sms, chain);
     }
     if (rc == B2_OK && c.dh) rc = (h_one ? tile_launch<HiddenOp<One>> : tile_launch<HiddenOp<Pairs>>)(who, d_k, w_mn, nullptr, pp, !SPLIT, pp.pairs, sms, chain);
     if (rc == B2_OK && c.dw) {

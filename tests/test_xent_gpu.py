@@ -264,6 +264,32 @@ def test_infinite_weights_by_sign(lm, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,width,vocab", [(300, 2000, 60002), (2100, 4096, 65536), (300, 2048, 1000), (300, 1024, 60002)])
+def test_nearly_certain_targets(lm, rows, width, vocab):
+    """Logits of 65 whose target has a probability of about 1 - 1e-4, kept and computed again: dh relative to its own rows. The logits of a row
+    come from one and the same sums in both passes, so p adds up to 1 and d is off by its share of two things only: its rounding to bf16, and
+    what the sums of 16 k-blocks (64 additions of the tensor core, each at 2^-23 of the magnitudes) and their join are off."""
+    g = torch.Generator(device="cuda").manual_seed(width)
+    common = torch.randn(width, device="cuda", generator=g)
+    common *= 3.0 / torch.linalg.norm(common)
+    own = torch.randn(vocab, width, device="cuda", generator=g) * (2.0 * width ** -0.5)
+    t = torch.randint(0, vocab, (rows,), device="cuda", generator=g)
+    w, h = (common + own).bfloat16(), (5.0 * common + 5.0 * own[t]).bfloat16()
+    del own
+    _, dh, _ = lm.xent(h, w, t)
+    lm.sync()
+    hd, wd, at = h.double(), w.double(), torch.arange(rows, device="cuda")
+    x = hd @ wd.T
+    size = float((hd.abs() @ wd.abs().T).max())
+    d = torch.softmax(x, 1)
+    assert 1e-6 < float((1.0 - d[at, t]).median()) < 1e-2 and float(x[at, t].median()) > 55.0
+    d[at, t] -= 1.0
+    off = 2 * (64 + width / 1024 + 8) * ULP * size
+    bound = (np.expm1(off) + 2.0 ** -8 + 2.0 ** -8) * d.abs().sum(1) * float(torch.linalg.norm(wd, dim=1).max()) + 2.0 ** -20 * float(torch.linalg.norm(wd, dim=1).max())
+    assert bool((torch.linalg.norm(dh.double() - d @ wd, dim=1) <= bound).all())
+
+
+@pytest.mark.gpu
 def test_small_and_large_magnitudes_fp32(lm):
     """The split of fp32 matrices follows their largest element."""
     for a, b in ((1e-20, 1e20), (1e15, 1e-15), (1e-30, 1.0)):

@@ -175,7 +175,7 @@ struct SymmetricOp {
   typedef SymmetricParams Params;
   typedef TileForm<true, ONE> Form;
   static constexpr bool MIDDLE = KIND == MIDDLE_FACTOR;
-  static constexpr bool STORES = false, LONG = true;
+  static constexpr bool STORES = false, LONG = true, INFINITE = false;
   static constexpr int SUM = MUON_SUM;
   const SymmetricParams& p;
   int m_blocks, n_blocks, per;
@@ -285,7 +285,7 @@ template <bool LAST, bool ONE>
 struct NextOp {
   typedef NextParams Params;
   typedef TileForm<true, ONE> Form;
-  static constexpr bool STORES = false, LONG = true;
+  static constexpr bool STORES = false, LONG = true, INFINITE = false;
   static constexpr int SUM = MUON_SUM;
   const NextParams& p;
   int m_blocks, n_blocks;

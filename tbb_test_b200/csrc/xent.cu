@@ -302,7 +302,7 @@ struct LogitParams {
 template <class F>
 struct LogitTiles {
   typedef F Form;
-  static constexpr bool SPLIT = F::SPLIT;
+  static constexpr bool SPLIT = F::SPLIT, INFINITE = true;
   static constexpr int SUM = XENT_SUM, BN = F::BN, W = F::CHUNK;
   const LogitParams& p;
   int rows, m_blocks, n_blocks, band;
@@ -702,7 +702,7 @@ template <class F>
 struct HiddenOp {
   typedef ProductParams Params;
   typedef F Form;
-  static constexpr bool SPLIT = F::SPLIT, STORES = false;
+  static constexpr bool SPLIT = F::SPLIT, STORES = false, INFINITE = true;
   static constexpr bool LONG = SPLIT;
   static constexpr int SUM = XENT_SUM, BN = F::BN;
   const ProductParams& p;
@@ -775,7 +775,7 @@ template <class F>
 struct WeightOp {
   typedef ProductParams Params;
   typedef F Form;
-  static constexpr bool SPLIT = F::SPLIT, STORES = !SPLIT;
+  static constexpr bool SPLIT = F::SPLIT, STORES = !SPLIT, INFINITE = true;
   static constexpr bool LONG = SPLIT;
   static constexpr int SUM = XENT_SUM, BN = F::BN;
   const ProductParams& p;

@@ -14,7 +14,7 @@ template <bool SPLIT, bool ONE>
 struct LateOp {
   typedef LateParams Params;
   typedef TileForm<SPLIT, ONE> Form;
-  static constexpr bool STORES = false, LONG = SPLIT;
+  static constexpr bool STORES = false, LONG = SPLIT, INFINITE = false;
   static constexpr int SUM = 4, W = Form::CHUNK, COLS = 256 / Form::BN;
   const Params& p;
   __device__ explicit LateOp(const Params& q, const TileMaps&) : p(q) {}

@@ -408,7 +408,8 @@ int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dou
  * is padding have loss 0 and a zero row of dh, take no part in dw whatever they hold, and cost next to nothing. The
  * logits are computed in tiles; for gradients the workspace holds all of them in fp32 up to 64 MB (up to 512 MB where the width
  * makes computing them dearer), and larger ones are computed a second time in pieces of the vocabulary. Types: bf16 matrices
- * are multiplied as they are with fp32 sums, the logits' gradients rounded to bf16 once; fp32 matrices, and the
+ * are multiplied as they are with fp32 sums (the tensor core truncates at each addition, so long sums are cut and joined by rounded ones: one whose
+ * terms have one sign is at most about 2e-4 of itself too small), the logits' gradients rounded to bf16 once; fp32 matrices, and the
  * logits' gradients between them, at 22 bits of every element down to 2^-27 of the largest (1 for the latter) and to
  * 2^-50 of the largest below that; a logit with an infinite element of w or h in it is infinite or NaN by the definition, and one of
  * -inf a probability of 0, in either type. Equal inputs give equal bits. Limits: rows and vocab at most 2^24

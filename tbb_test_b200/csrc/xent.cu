@@ -640,6 +640,11 @@ __global__ void __launch_bounds__(1024) join_rows_kernel(const float2* __restric
 
 // ------------------------------------------------------------------ gradients
 
+// k-blocks of bf16 products after which sums are handed over and added up in fp32, where there are more than four times as many: the tensor core
+// truncates at each of its additions, which leaves long sums of one sign too small (dw of 8192 rows 2e-6, of 65536 4e-4, of 2^20 6.5e-3 of
+// its value, where a bf16 result is rounded by up to 4e-3).
+constexpr int LONG_SUM = 128;
+
 struct ProductParams {
   const Meta* meta;
   int v_begin, v_count;
@@ -698,13 +703,13 @@ struct HiddenSplit {
 };
 
 // dh (listed rows) += d w over a piece.
-template <class F>
+template <class F, bool LONG_>
 struct HiddenOp {
   typedef ProductParams Params;
   typedef F Form;
   static constexpr bool SPLIT = F::SPLIT, STORES = false, INFINITE = true;
-  static constexpr bool LONG = SPLIT;
-  static constexpr int SUM = XENT_SUM, BN = F::BN;
+  static constexpr bool LONG = SPLIT || LONG_;
+  static constexpr int SUM = SPLIT ? XENT_SUM : LONG_SUM, BN = F::BN;
   const ProductParams& p;
   HiddenSplit split;
   int kblocks;
@@ -751,7 +756,7 @@ struct HiddenOp {
       to = p.acc;
     }
   }
-  static constexpr int W = F::CHUNK;
+  static constexpr int W = LONG ? 16 : F::CHUNK;
   __device__ __forceinline__ void chunk(const Tile& t, int row0, int col0, float (&v)[W], uint8_t* stage, int lane) {
     if (t.z == -2 || col0 >= p.width) return;
     float4 old[W / 4];
@@ -771,13 +776,13 @@ struct HiddenOp {
 };
 
 // dw of a piece = d' h.
-template <class F>
+template <class F, bool LONG_>
 struct WeightOp {
   typedef ProductParams Params;
   typedef F Form;
   static constexpr bool SPLIT = F::SPLIT, STORES = !SPLIT, INFINITE = true;
-  static constexpr bool LONG = SPLIT;
-  static constexpr int SUM = XENT_SUM, BN = F::BN;
+  static constexpr bool LONG = SPLIT || LONG_;
+  static constexpr int SUM = SPLIT ? XENT_SUM : LONG_SUM, BN = F::BN;
   const ProductParams& p;
   const CUtensorMap* map;
   int m_blocks, n_blocks, kblocks;
@@ -801,13 +806,13 @@ struct WeightOp {
     return r;
   }
   __device__ __forceinline__ void begin(const Tile&, int, int, int) {}
-  static constexpr int W = F::CHUNK;
+  static constexpr int W = LONG ? 16 : F::CHUNK;
   __device__ __forceinline__ void chunk(const Tile&, int row0, int col0, float (&v)[W], uint8_t* stage, int lane) {
     if constexpr (!SPLIT) {
       if (p.by_tma) {  // pieces are whole 256-row tiles but for the last one, whose rows the map ends with
-        uint32_t w[16];
+        uint32_t w[W / 2];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) w[j] = pack_bf16(v[2 * j] * unit, v[2 * j + 1] * unit);
+        for (int j = 0; j < W / 2; ++j) w[j] = pack_bf16(v[2 * j] * unit, v[2 * j + 1] * unit);
         store_half_words(map, w, p.v_begin + row0, col0, stage, lane);
         return;
       }
@@ -1114,6 +1119,12 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
   };
   const bool h_one = single_ctas<SPLIT>(1, share_of(dh_one, 2 * pairs), 1, share_of(dh_pairs, pairs));
   pp.pairs = h_one ? 2 * pairs : pairs;
+  // long: the k range of a tile, or of a CTA's part where all tiles are cut. No part of such a range is empty, which the long form leaves out.
+  auto is_long = [](long long k) { return !SPLIT && k > 4 * LONG_SUM; };
+  const long long dh_tiles = h_one ? dh_one : dh_pairs;
+  const bool dh_long = is_long(dh_tiles >= pp.pairs ? dh_k : share_of(dh_tiles, pp.pairs));
+  auto hidden = h_one ? (dh_long ? tile_launch<HiddenOp<One, !SPLIT>> : tile_launch<HiddenOp<One, false>>)
+                      : (dh_long ? tile_launch<HiddenOp<Pairs, !SPLIT>> : tile_launch<HiddenOp<Pairs, false>>);
   pp.full_kblocks = (int)(z.piece / TILE_K);
   pp.ld_acc = pitch;
   pp.dw = c.dw;
@@ -1137,12 +1148,13 @@ int xent_run(const XentCall& c, const Sizes& z, const Space& s, int sms, cudaStr
     } else {
       rc = (sums ? tile_launch<GradOp<Pairs, !SPLIT>> : tile_launch<GradOp<Pairs, false>>)(who, h_k, w_k, SPLIT ? nullptr : &d_out, lp, !SPLIT, tiles_of<Pairs>(rows, count), sms, chain);
     }
-    if (rc == B2_OK && c.dh) rc = (h_one ? tile_launch<HiddenOp<One>> : tile_launch<HiddenOp<Pairs>>)(who, d_k, w_mn, nullptr, pp, !SPLIT, pp.pairs, sms, chain);
+    if (rc == B2_OK && c.dh) rc = hidden(who, d_k, w_mn, nullptr, pp, !SPLIT, pp.pairs, sms, chain);
     if (rc == B2_OK && c.dw) {
       const long long k = (rows + TILE_K - 1) / TILE_K;
       const bool one = single_ctas<SPLIT>((tiles_of<One>(count, width) + sms - 1) / sms, k, (tiles_of<Pairs>(count, width) + pairs - 1) / pairs, k);
-      rc = (one ? tile_launch<WeightOp<One>> : tile_launch<WeightOp<Pairs>>)(who, d_mn, h_mn, pp.by_tma ? &dw_out : nullptr, pp, !SPLIT,
-                                                                             one ? tiles_of<One>(count, width) : tiles_of<Pairs>(count, width), sms, chain);
+      auto weight = one ? (is_long(k) ? tile_launch<WeightOp<One, !SPLIT>> : tile_launch<WeightOp<One, false>>)
+                        : (is_long(k) ? tile_launch<WeightOp<Pairs, !SPLIT>> : tile_launch<WeightOp<Pairs, false>>);
+      rc = weight(who, d_mn, h_mn, pp.by_tma ? &dw_out : nullptr, pp, !SPLIT, one ? tiles_of<One>(count, width) : tiles_of<Pairs>(count, width), sms, chain);
     }
     if (rc != B2_OK) return rc;
   }

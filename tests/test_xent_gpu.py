@@ -290,6 +290,50 @@ def test_nearly_certain_targets(lm, rows, width, vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,width,vocab", [(300000, 64, 64), (300000, 200, 70), (300003, 63, 64), (1 << 20, 64, 64)])
+def test_sums_over_many_rows_have_no_bias(lm, rows, width, vocab):
+    """dw of words that are never the target: every term is positive. A sum of n truncating additions is too small by up to n 2^-24 of itself in the
+    mean; with sums of 512 k-blocks at most (2048 additions) that is 1.2e-4. The roundings to bf16, of d and of dw, have no sign: d's are spread
+    over all rows; dw's, of up to 2^-8 and 2^-8 / sqrt(3) in the mean square, over the n elements looked at, four times their mean for a bound."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    h = (torch.rand(rows, width, device="cuda", generator=g) + 0.5).bfloat16()
+    w = (torch.randn(vocab, width, device="cuda", generator=g) * 0.05).bfloat16()
+    t = torch.randint(0, 4, (rows,), device="cuda", generator=g)
+    _, _, dw = lm.xent(h, w, t, scale=1.0 / rows)
+    lm.sync()
+    want = torch.zeros(vocab, width, device="cuda", dtype=torch.float64)
+    for part, at in zip(h.split(1 << 18), t.split(1 << 18)):
+        d = torch.softmax(part.double() @ w.double().T, 1)
+        d[torch.arange(len(at), device="cuda"), at] -= 1.0
+        want += d.T @ part.double() / rows
+    off = ((dw.double() - want) / want)[4:]
+    # a word's probability is nearly the same in all rows, and with it the rounding of d: 2^-8 / sqrt(3) over the words
+    bound = 1.2e-4 + 4 * 2.0 ** -8 / 3 ** 0.5 * ((vocab - 4) ** -0.5 + off.numel() ** -0.5)
+    assert abs(float(off.mean())) <= bound
+
+
+@pytest.mark.gpu
+def test_sums_over_a_long_vocabulary_have_no_bias(lm):
+    """dh of rows with positive weights: the sum of p w is positive; as above, 2048 additions at most."""
+    rows, width, vocab = 2048, 1024, 1 << 17
+    g = torch.Generator(device="cuda").manual_seed(5)
+    h = (torch.randn(rows, width, device="cuda", generator=g) * 0.1).bfloat16()
+    w = (torch.rand(vocab, width, device="cuda", generator=g) + 0.5).bfloat16()
+    _, dh, _ = lm.xent(h, w, torch.zeros(rows, dtype=torch.int64, device="cuda"))
+    lm.sync()
+    total = torch.zeros(rows, device="cuda", dtype=torch.float64)
+    want = torch.zeros(rows, width, device="cuda", dtype=torch.float64)
+    for part in w.split(1 << 14):
+        p = torch.exp(h.double() @ part.double().T)
+        total += p.sum(1)
+        want += p @ part.double()
+    want /= total[:, None]
+    off = (dh.double() - want + w[0].double()) / want
+    # the roundings of d are spread over the vocabulary, those of dh over all its elements
+    assert abs(float(off.mean())) <= 1.2e-4 + 4 * 2.0 ** -8 / 3 ** 0.5 * (vocab ** -0.5 + off.numel() ** -0.5)
+
+
+@pytest.mark.gpu
 def test_small_and_large_magnitudes_fp32(lm):
     """The split of fp32 matrices follows their largest element."""
     for a, b in ((1e-20, 1e20), (1e15, 1e-15), (1e-30, 1.0)):

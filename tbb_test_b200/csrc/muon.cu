@@ -120,7 +120,9 @@ __global__ void __launch_bounds__(256) normalise_kernel(const __grid_constant__ 
   __syncthreads();
   sum = 0.0;
   for (int k = 0; k < 8; ++k) sum += part[k];
-  const float by = (float)(1.0 / (sqrt(sum) + (double)p.eps));
+  // A matrix of zeros stays one without an eps too; a norm whose reciprocal is no normal fp32 number takes a power of two first.
+  const double norm = sqrt(sum) + (double)p.eps;
+  const float first = norm < 0x1p-100 ? 0x1p100f : norm > 0x1p100 ? 0x1p-100f : 1.f, by = sum == 0.0 ? 0.f : (float)(1.0 / (norm * first));
   const float* m = p.list.m[blockIdx.y];
   const G* g = static_cast<const G*>(p.list.g[blockIdx.y]);
   const size_t base = (size_t)blockIdx.y * p.rows_up * p.cols_up;
@@ -148,7 +150,7 @@ __global__ void __launch_bounds__(256) normalise_kernel(const __grid_constant__ 
     }
     __half hi[4], lo[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) split_half(update_of(gv[e], mv[e], p) * by * X_UP, hi[e], lo[e]);
+    for (int e = 0; e < 4; ++e) split_half(update_of(gv[e], mv[e], p) * first * by * X_UP, hi[e], lo[e]);
     const size_t at = base + (size_t)r * p.cols_up + c;
     *reinterpret_cast<uint2*>(p.x_hi + at) = *reinterpret_cast<const uint2*>(hi);
     *reinterpret_cast<uint2*>(p.x_lo + at) = *reinterpret_cast<const uint2*>(lo);

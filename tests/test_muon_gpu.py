@@ -182,6 +182,28 @@ def test_zero_gradient_and_scales(lm):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols", [(70, 90), (33, 17)])
+def test_without_eps(lm, rows, cols, dtype, nesterov):
+    """A matrix of zeros beside others; gradients as small and as large as fp32 has them, whose norms' reciprocals it has not."""
+    g = torch.randn(5, rows, cols, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(dtype)
+    g[1] = 0.0
+    g[2] *= 2.0 ** -124
+    g[3] = 0.0
+    g[3, 5, 7] = 2.0 ** -133  # exact in either type, and |u| is this number alone
+    g[4] *= 2.0 ** 124
+    w, m = torch.randn(5, rows, cols, device="cuda"), torch.zeros(5, rows, cols, device="cuda")
+    before = w.clone()
+    o = dict(lr=0.5, weight_decay=0.25, eps=0.0, momentum=0.0, nesterov=nesterov)
+    lm.muon(w, m, g, **o)
+    assert torch.equal(w[1], before[1] * 0.875) and not m[1].any()
+    for i in (0, 2, 3, 4):
+        want, _, off = _exact(before[i].double(), 0.0, g[i].double(), 0.5, 0.0, nesterov, 0.25, 1.0, 0.0)
+        assert float(torch.linalg.norm(w[i].double() - want)) <= off + 2.0 ** -22 * (float(torch.linalg.norm(want)) + float(torch.linalg.norm(before[i])))
+
+
+@pytest.mark.gpu
 def test_not_a_number_stays_in_its_matrix(lm):
     w, m, g = _make(3, 130, 260, torch.float32)
     before = (w.clone(), m.clone(), g.clone())

@@ -189,6 +189,10 @@ def muon(w, momentum_buffer, grad, *, lr, momentum=0.95, nesterov=True, weight_d
 def sync(device=None):
     """Waits for the current stream of `device`; K.B2Error with code ERR_TIMEOUT if a bounded wait of a kernel on the device gave up
     since this stream last asked (see b2_lm_sync in include/b200mlp.h)."""
-    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise ValueError(f"device: {device}, wanted a CUDA device")
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
     with _on(device) as stream:
         _ck(K.lib().b2_lm_sync(stream))

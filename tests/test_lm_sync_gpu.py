@@ -78,3 +78,19 @@ def test_sync_on_several_streams(native):
             got = lm.xent(h, w, t)[0]
             lm.sync()
             assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_sync_takes_a_device_in_any_form(native):
+    torch = pytest.importorskip("torch")
+    from tbb_test_b200 import lm
+    for device in (None, "cuda", "cuda:0", 0, torch.device("cuda"), torch.device("cuda", 0)):
+        lm.sync(device)
+
+
+def test_sync_refuses_other_devices(native):
+    torch = pytest.importorskip("torch")
+    from tbb_test_b200 import lm
+    for device in ("cpu", torch.device("cpu")):
+        with pytest.raises(ValueError):
+            lm.sync(device)

@@ -385,7 +385,8 @@ int b2_launch_counts(const b2_handle* h, long long* total, long long* tensor_cor
  * may be captured. A workspace is caller-owned device memory of at least the size that the operator's *_workspace()
  * function gives, on a 256-byte boundary, whose contents nothing keeps between calls; calls that may overlap on the GPU
  * need one each. Errors are returned as everywhere, with the text in b2_last_error(NULL); a bad argument is
- * refused before anything is queued. Outputs may not overlap inputs, except where a matrix is said to be updated.
+ * refused before anything is queued. What a call writes (outputs, updated matrices, the workspace) may not overlap its other arguments,
+ * which is refused too; matrices that lie in the gaps of one another's rows do not overlap.
  * Tokens and targets are 32- or 64-bit integers (token_bytes 4 or 8) in device memory; one outside [0, vocab) is
  * padding: an embedding row of zeros, no gradient, no loss. */
 

@@ -654,6 +654,9 @@ int b2_embed(const void* tokens, int token_bytes, size_t n, const void* table, i
   const size_t e = dtype_bytes(dtype);
   if ((reinterpret_cast<size_t>(table) | reinterpret_cast<size_t>(out)) % e || reinterpret_cast<size_t>(tokens) % token_bytes)
     return call_error(B2_ERR_INVALID, "b2_embed: a pointer is not aligned to its elements");
+  Extent args[] = {extent("tokens", tokens, 1, n * token_bytes, n * token_bytes, false), extent("table", table, vocab, width * e, ld_table * e, false),
+                   extent("out", out, n, width * e, ld_out * e, true)};
+  if ((rc = refuse_overlap("b2_embed", args, 3)) != B2_OK) return rc;
   const int vb = vector_bytes(e, reinterpret_cast<size_t>(table) | reinterpret_cast<size_t>(out) | width * e | ld_table * e | ld_out * e);
   const int wide = token_bytes == 8;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -699,6 +702,9 @@ int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dou
   int sms;
   if ((rc = lm_device(&sms)) != B2_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  Extent args[] = {extent("tokens", tokens, 1, n * token_bytes, n * token_bytes, false), extent("dout", dout, n, width * e, ld_dout * e, false),
+                   extent("dtable", dtable, vocab, width * e, ld_dtable * e, true), extent("the workspace", workspace, 1, n ? need : 0, need, true)};
+  if ((rc = refuse_overlap("b2_embed_grad", args, 4)) != B2_OK) return rc;
   if (n == 0)
     return launch_error(cudaMemset2DAsync(dtable, ld_dtable * e, 0, width * e, vocab, s), "b2_embed_grad");
   const int wide = token_bytes == 8;

@@ -6,6 +6,7 @@
 
 #include "../../include/b200mlp.h"
 #include "common.cuh"
+#include "overlap.h"
 
 namespace b2 {
 
@@ -25,6 +26,12 @@ inline int launch_error(cudaError_t e, const char* what) {
 }
 inline size_t dtype_bytes(int dtype) { return dtype == B2_DTYPE_BF16 ? 2 : 4; }
 inline bool dtype_ok(int dtype) { return dtype == B2_DTYPE_F32 || dtype == B2_DTYPE_BF16; }
+
+// Refuses a call whose arguments x[0..n) overlap where one of them is written.
+inline int refuse_overlap(const char* who, Extent* x, int n) {
+  const Extent *a, *b;
+  return any_overlap(x, n, &a, &b) ? call_error(B2_ERR_INVALID, "%s: %s and %s overlap", who, a->name, b->name) : B2_OK;
+}
 
 // Pieces of a caller's workspace, each on a 256-byte boundary. With a null base it only adds up sizes.
 struct Carver {

@@ -18,6 +18,9 @@
 //
 // Matrices of a call have one shape and go side by side, so that small ones fill the GPU together. Sides are rounded up to
 // 64, a k-block, with zeros, which stay zeros.
+#include <memory>
+#include <new>
+
 #include "lm_tile.cuh"
 #include "wait_reports.h"
 
@@ -556,8 +559,31 @@ int muon_group(const MatrixList& list, int count, int rows, int cols, int grad_d
   return rc;
 }
 
+// The matrices of a call may lie in one another's gaps, but share nothing, gradients among themselves excepted.
+int check_overlap(const char* who, int count, int rows, int cols, int grad_dtype, float* const* w, size_t ld_w, void* const* copy, size_t ld_copy,
+                  float* const* momentum, size_t ld_m, const void* const* grad, size_t ld_g, void* workspace, size_t need) {
+  constexpr int FEW = 4 * MUON_GROUP + 1;
+  Extent few[FEW], *x = few;
+  std::unique_ptr<Extent[]> many;
+  if (4ll * count + 1 > FEW) {
+    many.reset(new (std::nothrow) Extent[4 * (size_t)count + 1]);
+    if (!many) return call_error(B2_ERR_STATE, "%s: no host memory for a list of %d matrices", who, count);
+    x = many.get();
+  }
+  const size_t n = rows, c = cols, g = dtype_bytes(grad_dtype);
+  int used = 0;
+  for (int i = 0; i < count; ++i) {
+    x[used++] = extent("w", w[i], n, c * 4, ld_w * 4, true);
+    x[used++] = extent("momentum", momentum[i], n, c * 4, ld_m * 4, true);
+    x[used++] = extent("grad", grad[i], n, c * g, ld_g * g, false);
+    if (copy) x[used++] = extent("copy", copy[i], n, c * 2, ld_copy * 2, true);
+  }
+  x[used++] = extent("the workspace", workspace, 1, need, need, true);
+  return refuse_overlap(who, x, used);
+}
+
 int check_muon(const char* who, int count, int rows, int cols) {
-  if (count < 0 || rows < 1 || cols < 1 || rows > 65536 || cols > 65536)
+  if (count < 0 || count > 1 << 24 || rows < 1 || cols < 1 || rows > 65536 || cols > 65536)
     return call_error(B2_ERR_INVALID, "%s: %d matrices of %d x %d (sides of 1 to 65536)", who, count, rows, cols);
   return B2_OK;
 }
@@ -611,6 +637,7 @@ int b2_muon(int count, int rows, int cols, int grad_dtype, float* const* w, size
   if (workspace_bytes < need) return call_error(B2_ERR_INVALID, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, need);
   int sms;
   if ((rc = lm_device(&sms)) != B2_OK) return rc;
+  rc = check_overlap(who, count, rows, cols, grad_dtype, w, ld_w, copy, ld_copy, momentum, ld_m, grad, ld_g, workspace, need);
   for (int i = 0; i < count && rc == B2_OK; i += z.group) {
     const int n = count - i < z.group ? count - i : z.group;
     MatrixList list{};

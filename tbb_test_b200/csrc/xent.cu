@@ -1218,14 +1218,20 @@ int b2_xent(size_t rows, size_t width, size_t vocab, int dtype, const void* h, s
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   Sizes z{};
   Space s;
+  size_t need = 0;
   if (rows) {
     z = sizes_of(rows, width, vocab, dtype, grads, w, ldw);
-    const size_t need = space_of(z, rows, vocab, grads, workspace, &s);
+    need = space_of(z, rows, vocab, grads, workspace, &s);
     if (workspace_bytes < need) return call_error(B2_ERR_INVALID, "b2_xent: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   }
   int sms;
   if ((rc = lm_device(&sms)) != B2_OK) return rc;
   if (sms > 2 * MOST_PAIRS) sms = 2 * MOST_PAIRS;  // what the workspace is made for
+  Extent args[] = {extent("h", h, rows, width * e, ldh * e, false), extent("w", w, vocab, width * e, ldw * e, false),
+                   extent("targets", targets, 1, rows * token_bytes, rows * token_bytes, false), extent("row_loss", row_loss, 1, rows * 4, rows * 4, true),
+                   extent("dh", dh, rows, width * e, ld_dh * e, true), extent("dw", dw, vocab, width * e, ld_dw * e, true),
+                   extent("the workspace", workspace, 1, need, need, true)};
+  if ((rc = refuse_overlap("b2_xent", args, 7)) != B2_OK) return rc;
   if (rows == 0) return dw ? launch_error(cudaMemset2DAsync(dw, ld_dw * e, 0, width * e, vocab, st), "b2_xent") : B2_OK;
   const XentCall c{rows, width, vocab, dtype, h, ldh, w, ldw, targets, token_bytes == 8, scale, row_loss, dh, ld_dh, dw, ld_dw};
   return z.split ? xent_run<true>(c, z, s, sms, st) : xent_run<false>(c, z, s, sms, st);

@@ -3,10 +3,12 @@
 // ctypes, with golden vectors produced by the reference's own functions.
 #include <chrono>
 #include <cstring>
+#include <string>
 #include <vector>
 
 #include "../csrc/bucket_plan.h"
 #include "../csrc/download_plan.h"
+#include "../csrc/overlap.h"
 #include "../csrc/row_pieces.h"
 #include "../csrc/simt_tile.h"
 #include "../csrc/step_choice.h"
@@ -165,6 +167,21 @@ void b2h_downloads(int n, const size_t* width, const size_t* rows, int cores, si
 
 // Tile of the CUDA-core GEMM for small fp32 grids (csrc/simt_tile.h), 0 where the general kernel serves.
 int b2h_f32_tile(int m, int n, int whole_pieces) { return b2::f32_tile(m, n, whole_pieces != 0, 148); }
+
+// Whether arguments of a call overlap (csrc/overlap.h): the places in the list of the pair found, 0 where there is none.
+int b2h_any_overlap(int n, const size_t* at, const size_t* rows, const size_t* row, const size_t* ld, const int* written, int* out2) {
+  std::vector<std::string> names(n);
+  std::vector<b2::Extent> x;
+  for (int i = 0; i < n; ++i) {
+    names[i] = std::to_string(i);
+    x.push_back(b2::extent(names[i].c_str(), reinterpret_cast<const void*>(at[i]), rows[i], row[i], ld[i], written[i] != 0));
+  }
+  const b2::Extent *a, *b;
+  if (!b2::any_overlap(x.data(), n, &a, &b)) return 0;
+  out2[0] = std::stoi(a->name);
+  out2[1] = std::stoi(b->name);
+  return 1;
+}
 
 // What streams that ask one after the other are told of waits that gave up (csrc/wait_reports.h): 0 or 1 each.
 void b2h_wait_reports(int n, const int* device, const unsigned long long* stream, const unsigned int* count, int* out) {

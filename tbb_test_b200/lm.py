@@ -9,6 +9,10 @@ Thin wrappers over the C ABI (include/b200mlp.h, "Operators around the layers of
 check shapes, types and devices, allocate what is returned, and queue the work on the current torch stream without waiting
 for it. Matrices are float32 or bfloat16, all of one call alike, with unit stride along rows and any distance between
 rows. Tokens are int32 or int64; one outside [0, vocab) is padding. There is no CPU path.
+
+Nothing here is recorded by autograd, whatever its arguments require: results require no gradient, and embed_grad and xent give the
+gradients themselves. What a call writes into a given tensor counts as an in-place change, so that autograd's own backward passes refuse
+to use a value that it saved before.
 """
 import ctypes as C
 import functools
@@ -77,6 +81,11 @@ def _workspace(device, entry, *sizes):
     return torch.empty(_workspace_bytes(entry, *sizes), dtype=torch.uint8, device=device)
 
 
+def _changed(tensors):
+    """Given tensors that a call has written to: counted as changed in place where autograd keeps count."""
+    torch.autograd.graph.increment_version([x for x in tensors if not x.is_inference()])
+
+
 class _on:
     """The device of a call made the current one, where it is not already; gives the address of its current stream."""
 
@@ -103,9 +112,12 @@ def embed(tokens, table, scale=1.0, out=None):
     device = table.device
     t, size = _tokens("tokens", tokens, device)
     n = t.numel()
+    given = [] if out is None else [out]
     out, po, ldo = _result("out", out, n, width, table.dtype, device)
     with _on(device) as stream:
         _ck(K.lib().b2_embed(t.data_ptr(), size, n, p, _DTYPES[table.dtype], vocab, width, ld, scale, po, ldo, stream))
+    if given:
+        _changed(given)
     return out
 
 
@@ -117,11 +129,14 @@ def embed_grad(tokens, dout, vocab, scale=1.0, out=None):
     t, size = _tokens("tokens", tokens, device)
     if t.numel() != n:
         raise ValueError(f"dout: {n} rows for {t.numel()} tokens")
+    given = [] if out is None else [out]
     out, po, ldo = _result("out", out, vocab, width, dout.dtype, device)
     with _on(device) as stream:
         ws = _workspace(device, "embed_grad", n, vocab, width)
         _ck(K.lib().b2_embed_grad(t.data_ptr(), size, n, p, _DTYPES[dout.dtype], ld, vocab, width, scale, po, ldo,
                                   ws.data_ptr(), ws.numel(), stream))
+    if given:
+        _changed(given)
     return out
 
 
@@ -139,6 +154,7 @@ def xent(h, w, targets, scale=1.0, grad=True, dh=None, dw=None):
         raise ValueError(f"targets: {t.numel()} for {rows} rows")
     if not grad and (dh is not None or dw is not None):
         raise ValueError("dh and dw go with grad=True")
+    given = [x for x in (dh, dw) if x is not None]
     loss = torch.empty(rows, dtype=torch.float32, device=device)
     pdh = pdw = None
     lddh = lddw = 0
@@ -150,12 +166,18 @@ def xent(h, w, targets, scale=1.0, grad=True, dh=None, dw=None):
         ws = _workspace(device, "xent", rows, width, vocab, _DTYPES[dtype], int(grad), pw % 256 or None, ldw)
         _ck(K.lib().b2_xent(rows, width, vocab, _DTYPES[dtype], ph, ldh, pw, ldw, t.data_ptr(), size, scale,
                             loss.data_ptr(), pdh, lddh, pdw, lddw, ws.data_ptr(), ws.numel(), stream))
+    if given:
+        _changed(given)
     return (loss, dh, dw) if grad else loss
 
 
-def _matrices(name, x, dtype, shape, device):
-    """(list of addresses, leading dimension) of equally shaped matrices: a three-dimensional tensor or a sequence of matrices."""
-    xs = list(x.unbind(0)) if isinstance(x, torch.Tensor) and x.dim() == 3 else list(x)
+def _listed(x):
+    """The matrices of a three-dimensional tensor, or of a sequence of them."""
+    return list(x.unbind(0)) if isinstance(x, torch.Tensor) and x.dim() == 3 else list(x)
+
+
+def _matrices(name, xs, dtype, shape, device):
+    """(list of addresses, leading dimension) of equally shaped matrices."""
     got = [_matrix(f"{name}[{i}]", y, dtype, shape, device) for i, y in enumerate(xs)]
     if len({ld for _, ld in got}) > 1:
         raise ValueError(f"{name}: the matrices' rows lie at different distances")
@@ -166,15 +188,15 @@ def muon(w, momentum_buffer, grad, *, lr, momentum=0.95, nesterov=True, weight_d
     """Updates the matrices `w` and their momenta in place (see b2_muon in include/b200mlp.h): sequences of matrices of one
     shape, or three-dimensional tensors of them. w and momentum_buffer are float32, grad float32 or bfloat16; `copy`, bfloat16,
     receives the new weights too."""
-    ws = list(w.unbind(0)) if isinstance(w, torch.Tensor) and w.dim() == 3 else list(w)
+    ws = _listed(w)
     if not ws:
         raise ValueError("w: no matrices")
     shape, device = ws[0].shape, ws[0].device
-    gs = list(grad.unbind(0)) if isinstance(grad, torch.Tensor) and grad.dim() == 3 else list(grad)
+    ms, gs, cs = _listed(momentum_buffer), _listed(grad), None if copy is None else _listed(copy)
     pw, ldw = _matrices("w", ws, torch.float32, shape, device)
-    pm, ldm = _matrices("momentum_buffer", momentum_buffer, torch.float32, shape, device)
+    pm, ldm = _matrices("momentum_buffer", ms, torch.float32, shape, device)
     pg, ldg = _matrices("grad", gs, gs[0].dtype if gs else None, shape, device)
-    pc, ldc = _matrices("copy", copy, torch.bfloat16, shape, device) if copy is not None else (None, 0)
+    pc, ldc = _matrices("copy", cs, torch.bfloat16, shape, device) if cs is not None else (None, 0)
     if not len(pw) == len(pm) == len(pg) == (len(pc) if pc is not None else len(pw)):
         raise ValueError("w, momentum_buffer, grad and copy list different numbers of matrices")
     n = len(pw)
@@ -184,6 +206,7 @@ def muon(w, momentum_buffer, grad, *, lr, momentum=0.95, nesterov=True, weight_d
         ws_ = _workspace(device, "muon", n, shape[0], shape[1])
         _ck(K.lib().b2_muon(n, shape[0], shape[1], _DTYPES[gs[0].dtype], arr(pw), ldw, arr(pc), ldc, arr(pm), ldm, arr(pg), ldg,
                             C.byref(o), ws_.data_ptr(), ws_.numel(), stream))
+    _changed(ws + ms + (cs or []))
 
 
 def sync(device=None):

@@ -103,6 +103,23 @@ def test_gradient_is_the_lookups_transpose(lm):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["padding", "zipf"])
+def test_gradient_is_the_lookups_transpose_in_large_products(lm, kind):
+    """The same with positive values, so that the products are large against what they may be off: one rounding per row of the lookup, and per
+    element of the gradient an addition for each of its terms and the scale."""
+    n, vocab = 5000, 800
+    t = _tokens(n, vocab, kind, 3)
+    x, dout = _rows(vocab, 96, "fp32", 1).abs(), _rows(n, 96, "fp32", 2).abs()
+    a = (dout.double() * lm.embed(t, x, scale=2.0).double()).sum()
+    b = (lm.embed_grad(t, dout, vocab, scale=2.0).double() * x.double()).sum()
+    ok = (t >= 0) & (t < vocab)
+    terms = int(torch.bincount(t[ok].cpu(), minlength=vocab).max())
+    size = float((dout[ok].double() * x[t[ok]].double() * 2.0).sum())
+    bound = (terms + 2) * 2.0 ** -24 * size
+    assert bound < size * 1e-3 and abs(float(a - b)) <= bound
+
+
+@pytest.mark.gpu
 def test_nan_and_inf_stay_in_their_rows(lm):
     t = torch.tensor([0, 1, -1, 1, 2], device="cuda")
     dout = torch.ones(5, 64, device="cuda")

@@ -408,11 +408,14 @@ int b2_embed_grad(const void* tokens, int token_bytes, size_t n, const void* dou
  * dh and dw are of `dtype` and are written, not added to; NULL leaves one (or both: losses only) out. Rows whose target
  * is padding have loss 0 and a zero row of dh, take no part in dw whatever they hold, and cost next to nothing. The
  * logits are computed in tiles; for gradients the workspace holds all of them in fp32 up to 64 MB (up to 512 MB where the width
- * makes computing them dearer), and larger ones are computed a second time in pieces of the vocabulary. Types: bf16 matrices
+ * makes computing them dearer), and larger ones are computed a second time in pieces of the vocabulary. Beside them it holds their
+ * gradients of a piece (up to 640 MB; pieces have 1024 columns at least, which are more from 327 680 rows in bf16 and 163 840 in fp32 on), a
+ * copy of h, dh in fp32, 8 bytes per row and 128 (bf16) or 32 (fp32) columns of the vocabulary, and a copy of w where one is said to be made. Types: bf16 matrices
  * are multiplied as they are with fp32 sums (the tensor core truncates at each addition, so long sums are cut and joined by rounded ones: one whose
  * terms have one sign is at most about 2e-4 of itself too small), the logits' gradients rounded to bf16 once; fp32 matrices, and the
  * logits' gradients between them, at 22 bits of every element down to 2^-27 of the largest (1 for the latter) and to
- * 2^-50 of the largest below that; a logit with an infinite element of w or h in it is infinite or NaN by the definition, and one of
+ * 2^-50 of the largest below that, where the largest is 2^-86 at least: the row of dw of a word whose probabilities are all about 1e-12 has 10 good
+ * bits; a logit with an infinite element of w or h in it is infinite or NaN by the definition, and one of
  * -inf a probability of 0, in either type. Equal inputs give equal bits. Limits: rows and vocab at most 2^24
  * each and 2^44 together, width at most 2^20. Fastest where w begins on a 16-byte boundary and ldw is a multiple of 8 (bf16); otherwise, and in fp32,
  * a copy of w goes to the workspace, which is why its size depends on `w` and `ldw`. `grads` is 1 where the call will

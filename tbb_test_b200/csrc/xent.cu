@@ -1,4 +1,5 @@
-// Softmax cross entropy behind a linear layer as wide as a vocabulary, with its gradients, without keeping more than 512 MB of logits:
+// Softmax cross entropy behind a linear layer as wide as a vocabulary, with its gradients, without keeping more than 512 MB of logits and 640 MB
+// of their gradients (from 327 680 rows in bf16 and 163 840 in fp32 on, 1024 columns of the latter):
 //
 //   x_iv = h_i . w_v      l_i = log sum_v exp(x_iv) - x_i,t_i      d_iv = exp(x_iv) / sum_u exp(x_iu) - [v = t_i]
 //   dh_i = scale sum_v d_iv w_v      dw_v = scale sum_i d_iv h_i
@@ -15,8 +16,8 @@
 //      piece = d' h.
 // A few rows with few tiles of long sums: the logits go out in parts of the k range, and 3 and d are one kernel with a block per row.
 //
-// Precision: bf16 matrices are multiplied as they are, with fp32 sums; d is rounded to bf16 once, as the
-// gradients are in the end. fp32 matrices are
+// Precision: bf16 matrices are multiplied as they are, with fp32 sums, which are handed over and joined where they would be long; d is rounded
+// to bf16 once, as the gradients are in the end: gradients are 1.9e-3 off in norm, 1.7e-3 of it by their own rounding. fp32 matrices are
 // split into fp16 pairs behind a power of two that brings the largest element to 2^14: 22 bits of an element down to 2^-27 of
 // the largest, and nothing finer than 2^-50 of it; d the same, with 1 for the largest. Infinite elements take no part in that: their
 // logits are infinite by the signs, or NaN, as in bf16. Maxima, sums and the losses are fp32.

@@ -6,7 +6,7 @@
   sync                waits for the current stream and raises if a kernel's bounded wait gave up
 
 Thin wrappers over the C ABI (include/b200mlp.h, "Operators around the layers of a language model"): they
-check shapes, types and devices, allocate what is returned, and queue the work on the current torch stream without waiting
+check shapes, types and devices (and the entries behind them overlaps), allocate what is returned, and queue the work on the current torch stream without waiting
 for it. Matrices are float32 or bfloat16, all of one call alike, with unit stride along rows and any distance between
 rows. Tokens are int32 or int64; one outside [0, vocab) is padding. There is no CPU path.
 
@@ -142,8 +142,9 @@ def embed_grad(tokens, dout, vocab, scale=1.0, out=None):
 
 def xent(h, w, targets, scale=1.0, grad=True, dh=None, dw=None):
     """Losses of `h @ w.T` against `targets`, one float32 per row (0 for padding); with `grad` also the gradients of
-    `scale * losses.sum()` with respect to h and w: (losses, dh, dw). `dh` and `dw` may be given to be written to. No more
-    than 512 MB of logits are held (see b2_xent in include/b200mlp.h)."""
+    `scale * losses.sum()` with respect to h and w: (losses, dh, dw). `dh` and `dw` may be given to be written to. The
+    workspace holds up to 512 MB of logits and 640 MB of their gradients beside copies of h and, in fp32, of w (see b2_xent in
+    include/b200mlp.h)."""
     ph, ldh = _matrix("h", h)
     rows, width = h.shape
     device, dtype = h.device, h.dtype

@@ -68,7 +68,7 @@ typedef enum {
                        third of the TF32 rate */
 } b2_precision;
 
-typedef enum { B2_DTYPE_F32 = 0, B2_DTYPE_BF16 = 1 } b2_dtype;
+typedef enum { B2_DTYPE_F32 = 0, B2_DTYPE_BF16 = 1, B2_DTYPE_E4M3 = 2 /* b2_norm's output only */ } b2_dtype;
 
 /* Replaces the compile-time model of mlp_bench_common.h:26-38 and the argv of
  * mlp_omp.cc:376-386. Fill with b2_config_default() first. */
@@ -448,6 +448,68 @@ int b2_muon_workspace(int count, int rows, int cols, size_t* bytes);
 int b2_muon(int count, int rows, int cols, int grad_dtype, float* const* w, size_t ld_w, void* const* copy,
             size_t ld_copy, float* const* momentum, size_t ld_m, const void* const* grad, size_t ld_g,
             const b2_muon_options* options, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Root-mean-square norm with the residual stream's addition:
+ *   t = x + residual, rounded to `dtype` (t = x where residual is NULL)
+ *   out = t / sqrt(mean of t's squares along the row + eps) * weight
+ * total (or NULL) receives t, which the next layer adds to and b2_norm_grad reads; out is the norm of exactly these values. weight (or NULL: ones)
+ * is of weight_dtype, which is `dtype` or B2_DTYPE_F32. out_dtype is `dtype`, or B2_DTYPE_E4M3: 8 bits with scales (fp32, ld_scales from row to row),
+ *   scale = max(largest |out| / 448, 2^-126)     q = out / scale, rounded once to e4m3
+ * one for each 128 columns (block = 128; the last one of a row may be shorter) or one per row (block = 0); then ld_out counts bytes. scales, ld_scales and
+ * block are ignored otherwise. Squares are summed in fp32 and fp64 over the whole range of fp32. Limits: rows below 2^31, width at most 2^20. */
+int b2_norm(size_t rows, size_t width, int dtype, const void* x, size_t ld_x, const void* residual, size_t ld_residual,
+            const void* weight, int weight_dtype, float eps, void* total, size_t ld_total, int out_dtype, void* out,
+            size_t ld_out, float* scales, size_t ld_scales, size_t block, void* stream);
+/* Its gradients, from t (`total`), the gradient dy of out and (or NULL) the gradient dtotal that arrives at t elsewhere:
+ *   n = t / sqrt(mean of squares + eps)    g = dy * weight    dx = (g - n * mean(g * n)) / sqrt(...) + dtotal
+ *   dweight = sum over rows of dy * n      (of weight_dtype; NULL: not wanted)
+ * dx is the gradient of x and of residual alike. An e4m3 output's gradient is taken as that of the values before they were rounded. Equal inputs give
+ * equal bits on equal devices. */
+int b2_norm_grad_workspace(size_t rows, size_t width, int dtype, size_t* bytes);
+int b2_norm_grad(size_t rows, size_t width, int dtype, const void* dy, size_t ld_dy, const void* total, size_t ld_total,
+                 const void* dtotal, size_t ld_dtotal, const void* weight, int weight_dtype, float eps, void* dx,
+                 size_t ld_dx, void* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The global norm of `count` tensors, and the tensors scaled down to a limit:
+ *   norm = sqrt(sum of the squares of all elements)     out = x * (norm > max_norm ? max_norm / norm : 1)
+ * norm (device memory) is always written; max_norm = INFINITY asks for nothing else, and outputs are then not allowed. out == x (with the same
+ * leading dimension) is in place, where nothing is written unless the norm is over the limit. A norm that is infinite or not a number leaves the
+ * values as they are: the caller sees it in `norm`. Types may be mixed; elements are squared, summed and scaled in fp32 and fp64 over the whole range
+ * of fp32 and rounded once. The list is a host array, read during the call. Equal inputs give equal bits on equal devices. Limits: 2^20 tensors,
+ * 2^42 elements together. */
+typedef struct {
+  const void* x;
+  void* out;
+  size_t rows, cols, ld_x, ld_out; /* a dense tensor of any shape is one row */
+  int dtype;
+} b2_clip_tensor;
+int b2_clip_workspace(size_t count, size_t* bytes);
+int b2_clip(size_t count, const b2_clip_tensor* tensors, float max_norm, float* norm, void* workspace,
+            size_t workspace_bytes, void* stream);
+
+/* One token per row of logits (rows x vocab) from given random numbers u (fp32, one per row, from [0, 1)):
+ *   w[v] = exp((x[v] - largest x) / temperature)
+ * Tokens in the order of falling logits, equal ones by number; kept are those that are among the first top_k, before which less than top_p of the
+ * weight of these top_k lies, and whose w is at least min_p; the first one always. The token is the first one by number up to which the kept ones'
+ * weight exceeds u times all the kept ones' weight. logprob (or NULL) receives log(its weight / all the kept ones' weight), fp32.
+ * temperature <= 0, top_k = 1, top_p <= 0 or min_p > 1 is the first token in that order, logprob 0. top_k <= 0, top_p >= 1 and min_p <= 0 are no limit. Each of the
+ * four may be given for each row (device memory: row_...), in place of the one for all. A logit of -inf or NaN is never taken; a row of nothing else
+ * gives token -1 and logprob 0. Logits of +inf share all the weight. u outside of [0, 1) counts as the nearer end, NaN as 1.
+ * Weights are computed and summed in fp64, so that the token is the one of the formula unless u or a border lies within about 1e-11 of a step of
+ * the running sum; weights below e^-40 of the largest count as none where a limit is looked for. Equal inputs give equal tokens. tokens are 32- or 64-bit integers
+ * (token_bytes). Limits: rows and vocab at most 2^24 each. */
+typedef struct {
+  float temperature;
+  int top_k;
+  float top_p, min_p;
+  const float* row_temperature; /* NULL: the one above for all rows */
+  const int* row_top_k;
+  const float *row_top_p, *row_min_p;
+} b2_sample_options;
+/* temperature 1, top_k 0, top_p 1, min_p 0, no row has its own */
+int b2_sample_options_default(b2_sample_options* options);
+int b2_sample(size_t rows, size_t vocab, int dtype, const void* logits, size_t ld, const float* u,
+              const b2_sample_options* options, void* tokens, int token_bytes, float* logprob, void* stream);
 
 /* Waits for `stream` and returns B2_ERR_TIMEOUT if a bounded wait inside one of this section's tensor-core kernels on
  * the current device gave up since the last b2_lm_sync of the same stream (at its first: since the library was loaded), B2_OK otherwise.

@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(HERE, "csrc", "libb200mlp.so")
 OK, ERR_INVALID, ERR_CUDA, ERR_NCCL, ERR_UNSUPPORTED, ERR_TIMEOUT, ERR_STATE = 0, -1, -2, -3, -4, -5, -6
 MODE_REF, MODE_BASELINE = 0, 1
 PREC_FP32, PREC_TF32, PREC_BF16, PREC_FP32_TC = 0, 1, 2, 3
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_E4M3 = 0, 1, 2
 EPI_NONE, EPI_RELU, EPI_MASK = 0, 1, 2
 T_FWD, T_WGT_GRAD, T_BWD, T_WGT_UPDATE, T_ALLREDUCE, T_ALLGATHER, T_NUM = 0, 1, 2, 3, 4, 5, 6
 NCCL_ID_BYTES = 128
@@ -37,6 +37,16 @@ class Config(C.Structure):
 class MuonOptions(C.Structure):
     _fields_ = [("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float), ("scale", C.c_float),
                 ("eps", C.c_float), ("nesterov", C.c_int), ("steps", C.c_int)]
+
+
+class ClipTensor(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("rows", C.c_size_t), ("cols", C.c_size_t), ("ld_x", C.c_size_t), ("ld_out", C.c_size_t),
+                ("dtype", C.c_int)]
+
+
+class SampleOptions(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int), ("top_p", C.c_float), ("min_p", C.c_float), ("row_temperature", C.c_void_p),
+                ("row_top_k", C.c_void_p), ("row_top_p", C.c_void_p), ("row_min_p", C.c_void_p)]
 
 
 # every symbol include/b200mlp.h declares: name -> (restype, argtypes)
@@ -106,6 +116,13 @@ SYMBOLS = {
     "b2_muon_workspace": (C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(_sz)]),
     "b2_muon": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(_vp), _sz, C.POINTER(_vp), _sz, C.POINTER(_vp), _sz,
                           C.POINTER(_vp), _sz, C.POINTER(MuonOptions), _vp, _sz, _vp]),
+    "b2_norm": (C.c_int, [_sz, _sz, C.c_int, _vp, _sz, _vp, _sz, _vp, C.c_int, C.c_float, _vp, _sz, C.c_int, _vp, _sz, _vp, _sz, _sz, _vp]),
+    "b2_norm_grad_workspace": (C.c_int, [_sz, _sz, C.c_int, C.POINTER(_sz)]),
+    "b2_norm_grad": (C.c_int, [_sz, _sz, C.c_int, _vp, _sz, _vp, _sz, _vp, _sz, _vp, C.c_int, C.c_float, _vp, _sz, _vp, _vp, _sz, _vp]),
+    "b2_clip_workspace": (C.c_int, [_sz, C.POINTER(_sz)]),
+    "b2_clip": (C.c_int, [_sz, _vp, C.c_float, _vp, _vp, _sz, _vp]),
+    "b2_sample_options_default": (C.c_int, [C.POINTER(SampleOptions)]),
+    "b2_sample": (C.c_int, [_sz, _sz, C.c_int, _vp, _sz, _vp, C.POINTER(SampleOptions), _vp, C.c_int, _vp, _vp]),
     "b2_lm_sync": (C.c_int, [_vp]),
 }
 

@@ -121,6 +121,22 @@ struct Elems {
   }
 };
 
+// Sums over the whole range of fp32: up to N terms are added in fp32 and such sums in fp64; where fp32 has no product, or not with all of its bits, products are
+// taken in fp64 as well.
+__device__ __forceinline__ bool safe_sum(float s) { return fabsf(s) > 1e-25f && fabsf(s) < 1e38f; }
+template <int N>
+__device__ __forceinline__ void add_squares(const float (&f)[N], double& sum) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) s = fmaf(f[i], f[i], s);
+  if (safe_sum(s)) {
+    sum += (double)s;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum = fma((double)f[i], (double)f[i], sum);
+  }
+}
+
 // Token number i of a list of 32- or 64-bit ones; anything outside [0, vocab) becomes vocab.
 __device__ __forceinline__ unsigned int token_at(const void* tokens, int wide, size_t i, unsigned int vocab) {
   const long long t = wide ? __ldg(static_cast<const long long*>(tokens) + i) : (long long)__ldg(static_cast<const int*>(tokens) + i);

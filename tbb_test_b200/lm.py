@@ -2,7 +2,11 @@
 
   embed, embed_grad   rows of a table by token number, and the table's gradient
   xent                softmax cross entropy behind a linear layer as wide as a vocabulary, with its gradients
+  norm, norm_e4m3     root-mean-square norm with the residual stream's addition, also with an output in 8 bits with scales
+  norm_grad           its gradients
+  clip                global norm of a list of gradients, and the gradients scaled down to a limit
   muon                momentum and an orthogonalised update of weight matrices
+  sample              a token per row of logits: temperature, top-k, top-p, min-p
   sync                waits for the current stream and raises if a kernel's bounded wait gave up
 
 Thin wrappers over the C ABI (include/b200mlp.h, "Operators around the layers of a language model"): they
@@ -10,12 +14,14 @@ check shapes, types and devices (and the entries behind them overlaps), allocate
 for it. Matrices are float32 or bfloat16, all of one call alike, with unit stride along rows and any distance between
 rows. Tokens are int32 or int64; one outside [0, vocab) is padding. There is no CPU path.
 
-Nothing here is recorded by autograd, whatever its arguments require: results require no gradient, and embed_grad and xent give the
-gradients themselves. What a call writes into a given tensor counts as an in-place change, so that autograd's own backward passes refuse
+Nothing here is recorded by autograd, whatever its arguments require: results require no gradient, and embed_grad, norm_grad and xent give
+the gradients themselves. What a call writes into a given tensor counts as an in-place change, so that autograd's own backward passes refuse
 to use a value that it saved before.
 """
+import array
 import ctypes as C
 import functools
+import math
 
 import torch
 
@@ -170,6 +176,191 @@ def xent(h, w, targets, scale=1.0, grad=True, dh=None, dw=None):
     if given:
         _changed(given)
     return (loss, dh, dw) if grad else loss
+
+
+def _weight(x, width, dtype, device):
+    """(address, DTYPE) of a norm's weight: of the matrices' type or float32; (None, the matrices' DTYPE) for none."""
+    if x is None:
+        return None, _DTYPES[dtype]
+    if not isinstance(x, torch.Tensor) or x.shape != (width,) or x.device != device:
+        raise ValueError(f"weight: a tensor of {width} elements on {device} is wanted")
+    if x.dtype not in (dtype, torch.float32):
+        raise ValueError(f"weight: {x.dtype}, wanted {dtype} or float32")
+    if width > 1 and x.stride(0) != 1:
+        raise ValueError("weight: unit stride is wanted")
+    return x.data_ptr(), _DTYPES[x.dtype]
+
+
+def _norm(x, weight, residual, eps, total, out, scales, block):
+    """The call of b2_norm. scales: None, or a list that receives the given or new scales (an e4m3 output)."""
+    px, ldx = _matrix("x", x)
+    rows, width = x.shape
+    device, dtype = x.device, x.dtype
+    pw, wt = _weight(weight, width, dtype, device)
+    pr = pt = ps = None
+    ldr = ldt = lds = 0
+    given = [y for y in (total, out) if y is not None]
+    if residual is not None:
+        pr, ldr = _matrix("residual", residual, dtype, (rows, width), device)
+        total, pt, ldt = _result("total", total, rows, width, dtype, device)
+    elif total is not None:
+        raise ValueError("total goes with residual")
+    if scales is None:
+        out, po, ldo = _result("out", out, rows, width, dtype, device)
+    else:
+        if block not in (0, 128):
+            raise ValueError(f"block: {block}, wanted 0 or 128")
+        out = torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=device)
+        lds = -(-width // block) if block else 1
+        scales.append(torch.empty(rows, lds, dtype=torch.float32, device=device))
+        po, ldo, ps = out.data_ptr(), width, scales[0].data_ptr()
+    with _on(device) as stream:
+        _ck(K.lib().b2_norm(rows, width, _DTYPES[dtype], px, ldx, pr, ldr, pw, wt, eps, pt, ldt, K.DTYPE_E4M3 if scales is not None else _DTYPES[dtype],
+                            po, ldo, ps, lds, block, stream))
+    if given:
+        _changed(given)
+    return out, total
+
+
+def norm(x, weight=None, residual=None, eps=1e-6, total=None, out=None):
+    """`t / sqrt(mean of t's squares + eps) * weight` for each row of t = x, or of t = x + residual rounded to their type: then
+    (norm, t), t to be added to by what comes next and for `norm_grad`. weight: one element per column, of the matrices' type or
+    float32. `total` (t) and `out` may be given to be written to."""
+    out, total = _norm(x, weight, residual, eps, total, out, None, 0)
+    return out if residual is None else (out, total)
+
+
+def norm_e4m3(x, weight=None, residual=None, eps=1e-6, block=128, total=None):
+    """The same with its result in 8 bits, to stand in front of a product of such operands: (q, scales), or (q, scales, t) with a
+    residual. q is float8_e4m3fn, and q * scale the norm: a float32 scale for each `block` = 128 columns, or for each row
+    (block = 0), rows x scales. Gradients are those of `norm` (norm_grad)."""
+    scales = []
+    out, total = _norm(x, weight, residual, eps, total, None, scales, block)
+    return (out, scales[0]) if residual is None else (out, scales[0], total)
+
+
+def norm_grad(dy, t, weight=None, dtotal=None, eps=1e-6, dx=None):
+    """Gradients of `norm` from the gradient dy of its result, at t (x, or x + residual as norm gave it): dx for x and residual
+    alike, or (dx, dweight) with a weight. `dtotal`: a gradient that arrives at t elsewhere, which dx includes."""
+    pd, ldd = _matrix("dy", dy)
+    rows, width = dy.shape
+    device, dtype = dy.device, dy.dtype
+    pt, ldt = _matrix("t", t, dtype, (rows, width), device)
+    pm, ldm = (None, 0) if dtotal is None else _matrix("dtotal", dtotal, dtype, (rows, width), device)
+    pw, wt = _weight(weight, width, dtype, device)
+    given = [] if dx is None else [dx]
+    dx, px, ldx = _result("dx", dx, rows, width, dtype, device)
+    dw = None if weight is None else torch.empty_like(weight, memory_format=torch.contiguous_format, requires_grad=False)
+    with _on(device) as stream:
+        ws = _workspace(device, "norm_grad", rows, width, _DTYPES[dtype])
+        _ck(K.lib().b2_norm_grad(rows, width, _DTYPES[dtype], pd, ldd, pt, ldt, pm, ldm, pw, wt, eps, px, ldx, None if dw is None else dw.data_ptr(),
+                                 ws.data_ptr(), ws.numel(), stream))
+    if given:
+        _changed(given)
+    return dx if dw is None else (dx, dw)
+
+
+def _rows_of(name, x, device):
+    """(rows, cols, distance of rows) of a tensor as b2_clip takes it: one row where it lies in memory without gaps, whatever its shape."""
+    if x.is_contiguous():
+        return 1, x.numel(), 0
+    if x.dim() == 2 and (x.shape[1] == 1 or x.stride(1) == 1) and x.stride(0) >= x.shape[1]:
+        return x.shape[0], x.shape[1], x.stride(0)
+    sides = sorted((s, n) for n, s in zip(x.shape, x.stride()) if n != 1)
+    at = 1
+    for s, n in sides:
+        if s != at:
+            raise ValueError(f"{name}: neither dense nor a matrix with unit stride along its rows")
+        at *= n
+    return 1, x.numel(), 0
+
+
+def clip(tensors, max_norm, out=None):
+    """The norm of all elements of `tensors` together, a float32 scalar on their device; where it is over `max_norm`, the tensors are multiplied
+    by max_norm / norm, in place or into the list `out` of tensors like them (which is always written). math.inf or None for max_norm: the
+    norm alone. A norm that is infinite or not a number leaves the values as they are. float32 and bfloat16 tensors of any sizes, each dense
+    or a matrix with unit stride along its rows, all on one device; none may overlap another (see b2_clip in include/b200mlp.h)."""
+    xs = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if not xs:
+        raise ValueError("tensors: none")
+    limited = max_norm is not None and max_norm != math.inf
+    ys = xs if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
+    if not limited and out is not None:
+        raise ValueError("out goes with a limit")
+    if limited and not max_norm >= 0:
+        raise ValueError(f"max_norm: {max_norm}")
+    if len(ys) != len(xs):
+        raise ValueError(f"out: {len(ys)} tensors for {len(xs)}")
+    device = xs[0].device if isinstance(xs[0], torch.Tensor) else None
+    for name, zs in (("tensors", xs), ("out", ys)) if out is not None else (("tensors", xs),):
+        for i, x in enumerate(zs):
+            if not isinstance(x, torch.Tensor) or not x.is_cuda or x.device != device:
+                raise ValueError(f"{name}[{i}]: on one CUDA device with the others is wanted")
+            if x.dtype not in _DTYPES or x.dtype != xs[i].dtype or x.shape != xs[i].shape:
+                raise ValueError(f"{name}[{i}]: {x.dtype} of shape {tuple(x.shape)}, wanted float32 or bfloat16, and out like tensors")
+    table = array.array("Q")
+    for i, (x, y) in enumerate(zip(xs, ys)):
+        rows, cols, ldx = _rows_of(f"tensors[{i}]", x, device)
+        ldy = ldx
+        if y is not x:
+            rows_y, cols_y, ldy = _rows_of(f"out[{i}]", y, device)
+            if x.stride() != y.stride():
+                if rows == 1 and not x.is_contiguous() or rows_y == 1 and not y.is_contiguous():
+                    raise ValueError(f"out[{i}]: elements lie in another order than in tensors[{i}]")
+                if rows != rows_y:  # one of them has gaps between its rows
+                    rows, cols = max(rows, rows_y), min(cols, cols_y)
+                    ldx, ldy = ldx or cols, ldy or cols
+        table.extend((x.data_ptr(), y.data_ptr(), rows, cols, ldx, ldy, _DTYPES[x.dtype]))
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    with _on(device) as stream:
+        ws = _workspace(device, "clip", len(xs))
+        _ck(K.lib().b2_clip(len(xs), table.buffer_info()[0], max_norm if limited else math.inf, norm.data_ptr(), ws.data_ptr(), ws.numel(), stream))
+    if limited:
+        _changed(ys)
+    return norm
+
+
+def _per_row(name, x, dtype, rows, device):
+    """(number for all rows, address of one for each row or None)"""
+    if not isinstance(x, torch.Tensor):
+        return x, None
+    if x.shape != (rows,) or x.dtype != dtype or x.device != device or (rows > 1 and x.stride(0) != 1):
+        raise ValueError(f"{name}: a number, or a contiguous {dtype} tensor of {rows} on {device}, is wanted")
+    return 1, x.data_ptr()
+
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprob=False, out=None):
+    """One token per row of `logits`, int64, by the uniform random numbers `u` (float32, one per row, from [0, 1)); with `logprob`
+    also the logarithm of its probability among the tokens that were kept, float32: (tokens, logprobs).
+
+    Kept are the top_k most probable tokens, of these the fewest whose probability reaches top_p, and of these the ones of at least
+    min_p times the largest probability; tokens of one logit count in the order of their numbers. Each of the four may be a tensor with one
+    for each row (float32; top_k int32). temperature 0 takes the most probable token. A logit of -inf or NaN is never taken; a row of nothing
+    else gives -1. `out`, int64 or int32, may be given to be written to. See b2_sample in include/b200mlp.h."""
+    p, ld = _matrix("logits", logits)
+    rows, vocab = logits.shape
+    device = logits.device
+    number, pu = _per_row("u", u, torch.float32, rows, device)
+    if pu is None:
+        raise ValueError("u: a tensor is wanted")
+    o = K.SampleOptions()
+    o.temperature, o.row_temperature = _per_row("temperature", temperature, torch.float32, rows, device)
+    o.top_k, o.row_top_k = _per_row("top_k", top_k, torch.int32, rows, device)
+    o.top_p, o.row_top_p = _per_row("top_p", top_p, torch.float32, rows, device)
+    o.min_p, o.row_min_p = _per_row("min_p", min_p, torch.float32, rows, device)
+    given = [] if out is None else [out]
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int64, device=device)
+    elif not isinstance(out, torch.Tensor) or out.shape != (rows,) or out.dtype not in (torch.int32, torch.int64) or out.device != device or (
+            rows > 1 and out.stride(0) != 1):
+        raise ValueError(f"out: a contiguous int64 or int32 tensor of {rows} on {device} is wanted")
+    lp = torch.empty(rows, dtype=torch.float32, device=device) if logprob else None
+    with _on(device) as stream:
+        _ck(K.lib().b2_sample(rows, vocab, _DTYPES[logits.dtype], p, ld, pu, C.byref(o), out.data_ptr(), out.element_size(),
+                              None if lp is None else lp.data_ptr(), stream))
+    if given:
+        _changed(given)
+    return (out, lp) if logprob else out
 
 
 def _listed(x):

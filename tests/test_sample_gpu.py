@@ -1,0 +1,263 @@
+"""Tokens drawn from logits (tbb_test_b200.lm.sample) against a plain implementation in 64 bits on the host.
+
+Tokens have to be equal: weights and sums are in fp64 on both sides, so that they could differ only where u or top_p falls within rounding (1e-12 of the whole)
+of a step of the running sum; the oracle says how near it came, and no row here may come that near unless both sums are exact. Log probabilities are fp64
+numbers rounded to fp32: half a step."""
+import ctypes as ct
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def lm(native):
+    from tbb_test_b200 import lm
+    return lm
+
+
+def oracle_row(x, u, t, k, p, m):
+    """(token, log probability, distance of u and top_p from the nearest step as a share of the whole) of one row, from the definition."""
+    x = np.where(np.isnan(x), -np.inf, x.astype(np.float64))
+    if not (x > -np.inf).any():
+        return -1, 0.0, 1.0
+    order = sorted(range(len(x)), key=lambda i: (-x[i], i)) if len(x) < 50 else list(np.lexsort((np.arange(len(x)), -x)))
+    top = x[order[0]]
+    if not t > 0 or k == 1 or p <= 0 or m > 1:
+        return order[0], 0.0, 1.0
+    t = min(t, float(np.finfo(np.float32).max))
+    with np.errstate(invalid="ignore", over="ignore", under="ignore"):
+        w = np.where(x == top, 1.0, np.exp((x - top) / t))
+    n = len(order) if k <= 0 else min(k, len(order))
+    sorted_w = w[order[:n]]
+    near = 1.0
+    if p < 1:
+        run = np.cumsum(sorted_w)
+        goal = p * run[-1]
+        n = max(1, int((run - sorted_w < goal).sum()))
+        near = float(np.abs(run - goal).min() / run[-1])
+    kept = [i for i in order[:n] if w[i] >= m or i == order[0]]
+    kept = np.sort(np.array([i for i in kept if w[i] > 0 and x[i] > -np.inf]))
+    run = np.cumsum(w[kept])
+    goal = u * run[-1] if u >= 0 else 0.0 if u < 0 else np.inf
+    at = min(int((run <= goal).sum()), len(kept) - 1)
+    if len(kept) > 1:
+        near = min(near, float(np.abs(run[:-1] - goal).min() / run[-1]))
+    with np.errstate(invalid="ignore"):
+        y = 0.0 if x[kept[at]] == top else (x[kept[at]] - top) / t
+    return kept[at], y - math.log(run[-1]), near
+
+
+def _check(lm, logits, u, t=1.0, k=0, p=1.0, m=0.0, out=None, exact=False):
+    rows = len(logits)
+    dev = lambda v, d: torch.tensor(v, dtype=d, device="cuda") if isinstance(v, list) else v  # noqa: E731
+    f = torch.float32
+    args = dict(temperature=dev(t, f), top_k=dev(k, torch.int32), top_p=dev(p, f), min_p=dev(m, f))
+    tokens, lp = lm.sample(logits, u, logprob=True, out=out, **args)
+    again, lp2 = lm.sample(logits, u, logprob=True, **args)
+    assert torch.equal(tokens.long(), again) and torch.equal(lp, lp2)
+    x, uu = logits.double().cpu().numpy(), u.double().cpu().numpy()
+    each = lambda v: np.float32(v if isinstance(v, list) else [v] * rows).astype(np.float64)  # noqa: E731
+    t, p, m, k = each(t), each(p), each(m), k if isinstance(k, list) else [k] * rows
+    for i in range(rows):
+        token, logprob, near = oracle_row(x[i], uu[i], t[i], k[i], p[i], m[i])
+        assert exact or near > 1e-12, "the inputs of a test have to be off the borders"
+        assert int(tokens[i]) == token, (i, int(tokens[i]), token, near)
+        assert abs(float(lp[i]) - logprob) <= 2.0 ** -24 * abs(logprob) + 1e-12, i
+    return tokens, lp
+
+
+def _logits(rows, vocab, dtype, seed, spread=2.5, ld=None, offset=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    ld = ld or vocab
+    buf = torch.full((rows * ld + offset + 8,), float("inf"), device="cuda", dtype=dtype)
+    view = buf[offset:offset + rows * ld].view(rows, ld)[:, :vocab]
+    view.copy_(torch.randn(rows, vocab, device="cuda", generator=g) * spread)
+    return view, torch.rand(rows, device="cuda", generator=g)
+
+
+SETTINGS = [dict(), dict(t=0.7), dict(k=5), dict(k=50, p=0.9), dict(p=0.8), dict(p=0.999), dict(m=0.05), dict(k=100, p=0.95, m=0.01, t=1.3), dict(t=0.0), dict(k=1), dict(p=1e-6),
+            dict(k=700), dict(k=700, p=0.97), dict(t=30.0, p=0.6), dict(t=30.0, k=900)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("rows,vocab,ld,offset", [(1, 1, 1, 0), (3, 2, 2, 0), (40, 100, 104, 0), (7, 1009, 1011, 1), (5, 4096, 4096, 0), (1, 50001, 50001, 0), (700, 300, 300, 0),
+                                                  (3, 33000, 33008, 8)])
+@pytest.mark.parametrize("setting", range(len(SETTINGS)))
+def test_sample(lm, dtype, rows, vocab, ld, offset, setting):
+    x, u = _logits(rows, vocab, dtype, 1, 2.5, ld, offset)
+    _check(lm, x, u, **SETTINGS[setting], out=torch.empty(rows, dtype=torch.int32, device="cuda") if setting % 2 else None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("setting", [0, 3, 4, 5, 11, 12, 13])
+@pytest.mark.parametrize("spread", [0.0, 1e-6, 0.01, 1.0, 8.0, 1e4])
+def test_spreads(lm, dtype, setting, spread):
+    """From rows of one value, where borders fall on steps and all sums are exact, to rows with one likely token."""
+    x, u = _logits(6, 9001, dtype, 2, spread)
+    _check(lm, x, u, **SETTINGS[setting], exact=spread == 0.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_large_vocabularies(lm, dtype):
+    x, u = _logits(2, 300007, dtype, 3, 1.0)
+    for s in (dict(), dict(p=0.9), dict(k=2000), dict(k=50, p=0.9)):
+        _check(lm, x, u, **s)
+
+
+@pytest.mark.gpu
+def test_rows_that_no_shared_memory_holds(lm):
+    """2^21 logits in fp32 are read from device memory again for each pass."""
+    x, u = _logits(1, (1 << 21) + 5, torch.float32, 3, 1.0)
+    for s in (dict(), dict(k=3000), dict(p=0.9)):
+        _check(lm, x, u, **s)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("vocab", [37, 5000])
+def test_a_row_has_its_own_numbers(lm, dtype, vocab):
+    n = 24
+    x, u = _logits(n, vocab, dtype, 4)
+    pick = lambda values: [values[i % len(values)] for i in range(n)]  # noqa: E731
+    _check(lm, x, u, t=pick([0.5, 1.0, 0.0, 2.0, math.nan, -1.0, 0.25]), k=pick([0, 3, 20, 1, -5, 10 ** 9]), p=pick([1.0, 0.9, 0.5, 2.0]), m=pick([0.0, 0.1, 0.0, -1.0, 1.0, 1.5]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("vocab", [50, 3001, 70001])
+def test_equal_logits_go_by_their_numbers(lm, dtype, vocab):
+    """Few different values: whole classes of thousands of tokens at the limit."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randint(-2, 3, (6, vocab), device="cuda", generator=g).to(dtype) * 0.5
+    u = torch.rand(6, device="cuda", generator=g)
+    for s in (dict(k=7), dict(k=vocab // 3), dict(p=0.3), dict(p=0.7), dict(k=vocab // 2, p=0.5), dict(m=0.4), dict(t=0.1, p=0.99)):
+        _check(lm, x, u, **s, exact=True)  # a few distinct weights: sums on both sides are within 1e-13, and so are steps of at least 1e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_masks(lm, dtype):
+    """Masked with -inf, NaN, the type's lowest value; rows of nothing, of one token, of +inf, of lowest values only, of both zeros."""
+    x, u = _logits(12, 4000, dtype, 6)
+    low = torch.finfo(dtype).min
+    x[0, 1::2] = -math.inf
+    x[1, ::3] = math.nan
+    x[2, 5:] = low
+    x[3] = -math.inf
+    x[4] = math.nan
+    x[5] = -math.inf
+    x[5, 3777] = -1e30
+    x[6, [5, 77, 3000]] = math.inf
+    x[7] = low
+    x[8] = 0.0
+    x[8, ::2] = -0.0
+    x[9, :3998] = -math.inf
+    x[10] = math.inf
+    x[11, 100:] = -math.inf
+    for s in (dict(), dict(k=40), dict(p=0.9), dict(k=3, p=0.7), dict(m=0.1), dict(t=0.0), dict(k=600, p=0.99), dict(t=1e-30), dict(t=3e38)):
+        tokens, _ = _check(lm, x, u, **s, exact=True)
+        assert int(tokens[3]) == int(tokens[4]) == -1 and int(tokens[5]) == 3777
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_ends_of_u(lm, dtype):
+    x, _ = _logits(6, 1000, dtype, 7)
+    u = torch.tensor([0.0, 1.0 - 2.0 ** -24, 1.0, 5.0, -3.0, math.nan], device="cuda")
+    for s in (dict(), dict(k=9), dict(p=0.5), dict(m=0.3)):
+        _check(lm, x, u, **s, exact=True)
+
+
+@pytest.mark.gpu
+def test_extreme_logits(lm):
+    """Differences that fp32 has not, temperatures as small and as large as it has them, one temperature per row."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x = torch.randn(8, 3000, device="cuda", generator=g)
+    x *= torch.tensor([1e-44, 1e-38, 1e-10, 1.0, 1e4, 1e20, 1e38, 3e38], device="cuda")[:, None] / 5
+    x = x.clamp(-3.4e38, 3.4e38)
+    u = torch.rand(8, device="cuda", generator=g)
+    for t in ([1e-44, 1e-38, 1e-10, 1.0, 1e4, 1e20, 1e38, 3e38], [1e-45] * 8, [3.4e38] * 8, [math.inf] * 8, [1e-3] * 8):
+        for s in (dict(), dict(k=30), dict(p=0.8), dict(k=1000, p=0.9)):
+            _check(lm, x, u, t=t, **s, exact=True)
+
+
+@pytest.mark.gpu
+def test_frequencies(lm):
+    """Each of 20 tokens comes as often as its probability says: 6 standard deviations of 200000 draws, which 20 tokens leave once in 2e7 runs."""
+    n = 200000
+    g = torch.Generator(device="cuda").manual_seed(9)
+    row = torch.randn(20, device="cuda", generator=g) * 1.5
+    u = torch.rand(n, device="cuda", generator=g)
+    tokens = lm.sample(row.expand(n, 20).contiguous(), u, temperature=0.8)
+    p = torch.softmax(row.double() / float(np.float32(0.8)), 0).cpu()
+    count = torch.bincount(tokens, minlength=20).double().cpu()
+    assert bool(((count - n * p).abs() <= 6 * (n * p * (1 - p)).sqrt() + 1).all())
+
+
+@pytest.mark.gpu
+def test_captured_and_on_another_stream(lm):
+    x, u = _logits(30, 20000, torch.bfloat16, 10)
+    want = lm.sample(x, u, top_p=0.9, logprob=True)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = lm.sample(x, u, top_p=0.9, logprob=True)
+    s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        third = lm.sample(x, u, top_p=0.9, logprob=True)
+    third[0].zero_()
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, b, c in zip(want, other, third):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    assert lm.sample(x[:0], u[:0]).shape == (0,)
+
+
+@pytest.mark.gpu
+def test_refusals(lm):
+    from tbb_test_b200._capi import B2Error
+    x, u = _logits(4, 64, torch.float32, 11)
+    f = torch.ones(4, device="cuda")
+    before = x.clone()
+    for call in (lambda: lm.sample(x[0], u), lambda: lm.sample(x.half(), u), lambda: lm.sample(x, u[:3]), lambda: lm.sample(x, u.double()), lambda: lm.sample(x, 0.5),
+                 lambda: lm.sample(x, u.cpu()), lambda: lm.sample(x, u, temperature=f[:2]), lambda: lm.sample(x, u, top_k=f), lambda: lm.sample(x, u, top_p=f.double()),
+                 lambda: lm.sample(x, u, out=f), lambda: lm.sample(x, u, min_p=torch.ones(8, device="cuda")[::2])):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: lm.sample(x, u, temperature=math.nan), lambda: lm.sample(x, u, top_p=math.nan), lambda: lm.sample(x, u, out=x.view(-1)[:8].view(torch.int64))):
+        with pytest.raises(B2Error):
+            call()
+    assert torch.equal(x, before)
+    out = torch.zeros(4, dtype=torch.int64, device="cuda")
+    version = out._version
+    assert lm.sample(x, u, out=out) is out and out._version > version
+
+
+def test_c_entry_refuses_before_any_device_work(native):
+    from tbb_test_b200 import _capi as K
+    lib = K.lib()
+    p = ct.c_void_p
+    o = K.SampleOptions()
+    assert lib.b2_sample_options_default(ct.byref(o)) == K.OK and o.temperature == 1.0 and o.top_k == 0 and o.top_p == 1.0 and o.min_p == 0.0 and not o.row_top_k
+    assert lib.b2_sample_options_default(None) == K.ERR_INVALID
+
+    def options(**kw):
+        y = K.SampleOptions()
+        lib.b2_sample_options_default(ct.byref(y))
+        for k, v in kw.items():
+            setattr(y, k, v)
+        return ct.byref(y)
+
+    good = dict(rows=2, vocab=8, dtype=0, x=p(256), ld=8, u=p(1024), o=options(), tokens=p(2048), size=8, lp=p(4096), stream=None)
+    for kw in (dict(dtype=2), dict(rows=(1 << 24) + 1), dict(vocab=0), dict(vocab=(1 << 24) + 1), dict(size=2), dict(o=None), dict(x=None), dict(u=None), dict(tokens=None), dict(ld=7),
+               dict(x=p(2)), dict(u=p(2)), dict(tokens=p(4)), dict(lp=p(2)), dict(o=options(temperature=math.nan)), dict(o=options(row_top_k=2)), dict(o=options(row_top_p=2))):
+        assert lib.b2_sample(*{**good, **kw}.values()) == K.ERR_INVALID, kw
+        assert lib.b2_last_error(None)

@@ -27,6 +27,7 @@ constexpr int BINS = 1024, BINS_PER_THREAD = BINS / SAMPLE_THREADS;
 constexpr float REACH = 40.f;  // of the first bins, in units of T: the last bin has all tokens of less than e^-40 of the largest weight
 constexpr int LIST = SAMPLE_THREADS;  // tokens that are put in order one by one
 constexpr int MOST_CLUSTER = 8;
+constexpr int STEPS = 16;  // 2^(n / 16) for n = 0 to 15 lie in different banks of shared memory
 
 struct SampleArgs {
   const char* logits;
@@ -51,23 +52,65 @@ struct SampleShared {
   double warp_sums[2][SAMPLE_WARPS];
   unsigned int warp_counts[SAMPLE_WARPS];
   unsigned int found[4];
-  unsigned int tie_counts[MOST_CLUSTER];
+  double powers[STEPS];
 };
 
-// Logits as unsigned numbers in the same order; +0 and -0 are one.
+// Logits as unsigned numbers in the same order; -0 is +0, so that no token has the key below +0's.
 __device__ __forceinline__ unsigned int key_of(float f) {
   const unsigned int b = __float_as_uint(f + 0.f);
   return b ^ (b >> 31 ? 0xFFFFFFFFu : 0x80000000u);
 }
 __device__ __forceinline__ float value_of(unsigned int key) { return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xFFFFFFFFu)); }
 
+// 2^(s / 16) - 1 for |s| <= 1/2, off by at most 5.1e-12, and exactly 0 at 0: s q(s), where q interpolates (2^(s / 16) - 1) / s at the four Chebyshev nodes of the range.
+__device__ __forceinline__ double small_power(double s) {
+  double q = fma(1.4676329855091502e-07, s, 1.3551125679403628e-05);
+  q = fma(q, s, 0.0009383847927372583);
+  q = fma(q, s, 0.043321698775062194);
+  return q * s;
+}
+
+// fp32 to fp64 by integer instructions, of which an SM has eight times as many per clock as conversions: exact for normal numbers; what is smaller comes out
+// as something below 2^-125, infinities as 2^128.
+__device__ __forceinline__ double widened(float f) {
+  const unsigned int b = __float_as_uint(f);
+  return __hiloint2double((b & 0x80000000u) | (((b & 0x7FFFFFFFu) >> 3) + 0x38000000u), b << 29);
+}
+
+// An upper edge: compared as a logit, -0 would let +0 in.
+__device__ __forceinline__ unsigned int without_minus_zero(unsigned int key) { return key == 0x7FFFFFFFu ? key - 1 : key; }
+
 // The row's largest logit and temperature.
 struct Weights {
   float top;
-  double inv_t;
-  float half_top, per_bin;  // per_bin: bins for each 2 of the logit
+  double wide_top, inv_t, steps;     // steps: 16 log2(e) / T
+  const double* powers;              // in shared memory
+  float least;                       // logits below it weigh nothing: less than 2^-1000, -inf
+  float half_top, per_bin;           // per_bin: bins for each 2 of the logit
+  bool plain;                        // what widened() makes of small numbers and infinities does not matter
+
+  __device__ __forceinline__ void set(float largest, float t) {
+    top = largest;
+    plain = (t > 1e-25f && t < 1e25f) || top == INFINITY;
+    wide_top = plain ? widened(top) : (double)top;
+    inv_t = 1.0 / (double)t;
+    steps = STEPS * 1.4426950408889634 * inv_t;
+    least = top == INFINITY ? top : (float)fmax((double)top - 693.0 * (double)t, -3.4028234663852886e38);
+    half_top = 0.5f * top;
+    per_bin = (float)fmin(2 * (BINS - 1) / REACH * inv_t, 1e38);
+  }
   __device__ __forceinline__ double exponent(float f) const { return f == top ? 0.0 : ((double)f - (double)top) * inv_t; }
-  __device__ __forceinline__ double of(float f) const { return exp(exponent(f)); }
+  // The weight: 2^((n + s) / 16), n an integer
+  __device__ __forceinline__ double of(float f) const {
+    const float g = fmaxf(f, least);
+    const double d = (plain ? widened(g) : (double)g) - wide_top;
+    const double t = fma(d, steps, 6755399441055744.0);  // 1.5 * 2^52: the sum's low bits are n
+    const double s = fma(d, steps, 6755399441055744.0 - t);
+    const int n = __double2loint(t);
+    const double base = powers[n & (STEPS - 1)], w = fma(base, small_power(s), base);
+    const unsigned int hi = __double2hiint(w) + ((n & ~(STEPS - 1)) << 16);
+    return __hiloint2double(f < least ? 0 : hi, f < least ? 0 : __double2loint(w));
+  }
   // 0 at the top; falls with f in steps, whatever fp32 rounds
   __device__ __forceinline__ unsigned int bin(float f) const {
     const unsigned int b = f == top ? 0u : __float2uint_rz(fmaf(-0.5f, f, half_top) * per_bin);
@@ -121,6 +164,31 @@ struct Sampler {
 #pragma unroll
       for (int j = 0; j < N; ++j) body(i + j, f[j]);
     }
+  }
+
+  // body(number of the first, logits) for the warp's tokens, N neighbours at a time.
+  template <class Body>
+  __device__ __forceinline__ void each_vector(Body body) const {
+    for (unsigned int i = w0 + lane * N; i < w1; i += TILE) {
+      float f[N];
+      fetch(i, f);
+      body(i, f);
+    }
+  }
+  // The sum of the weights that `counts` says, without a branch: the N computations go side by side.
+  template <class Counts>
+  __device__ __forceinline__ double weigh(const float (&f)[N], Counts counts) const {
+    double x[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      x[j] = w.of(f[j]);
+      x[j] = counts(f[j]) ? x[j] : 0.0;
+    }
+#pragma unroll
+    for (int o = 1; o < N; o *= 2)
+#pragma unroll
+      for (int j = 0; j + o < N; j += 2 * o) x[j] += x[j + o];
+    return x[0];
   }
 
   // Sums over the cluster of two values per thread, the same bits everywhere.
@@ -193,10 +261,11 @@ struct Sampler {
     return lo;
   }
 
-  // The cut at which `target` tokens (BY_COUNT) or `target` weight is reached; false: there is none before the tokens that weigh nothing.
-  // The first bins have been counted. search: 0 or 1, a list's counter of its own.
+  // The cut at which `target` tokens (BY_COUNT) or `target` weight is reached. The first bins have been counted. search: 0 or 1, a list's counter of its own.
+  // NONE: it is not reached before the tokens that weigh nothing. GATHERED: no cut, but a list of `gathered` tokens from the first one on in which it lies.
+  enum Found { NONE, CUT, GATHERED };
   template <bool BY_COUNT>
-  __device__ bool find(double target, int search, Cut& cut) {
+  __device__ Found find(double target, int search, Cut& cut, unsigned int& gathered) {
     unsigned int lo = 0, hi = key_of(w.top), shift = 0;  // the window's keys
     const unsigned int goal = BY_COUNT ? (unsigned int)target : 0;
     unsigned int above = 0;  // tokens above the window
@@ -239,7 +308,8 @@ struct Sampler {
         }
         __syncthreads();
         m = sh.found[0];
-        if (first && m >= BINS - 1) return false;
+        if (first && m >= BINS - 1) return NONE;
+        b2 = m;
       } else {
         // the running weight at the bins' ends, by the lightest, the heaviest and a middle token of each
         double low[BINS_PER_THREAD], mid[BINS_PER_THREAD], high[BINS_PER_THREAD];
@@ -279,17 +349,30 @@ struct Sampler {
           m += __syncthreads_count(upto == 0 || mass + before_mid + mid[k] < target);
           b2 += __syncthreads_count(upto == 0 || mass + before_low + low[k] < target);
         }
-        if (first && b1 >= BINS) return false;
+        if (first && b1 >= BINS) return NONE;
         const unsigned int last = sh.found[0];
         if (b2 > last) b2 = last;
         if (b1 > b2) b1 = b2;
         m = m < b1 ? b1 : m > b2 ? b2 : m;
 #pragma unroll
-        for (int k = 0; k < BINS_PER_THREAD; ++k)
+        for (int k = 0; k < BINS_PER_THREAD; ++k) {
           if (threadIdx.x * BINS_PER_THREAD + k == m) sh.found[2] = count[k];
+          if (threadIdx.x * BINS_PER_THREAD + k == b2) sh.found[3] = upto - (k + 1 < BINS_PER_THREAD ? count[BINS_PER_THREAD - 1] : 0);
+        }
         __syncthreads();
       }
-      const unsigned int n = sh.found[2], key_lo = edge_of(m, false), key_hi = edge_of(m, true);
+      if (first) {
+        const unsigned int all = BY_COUNT ? sh.found[1] + sh.found[2] : sh.found[3];
+        if (all <= LIST) {
+          each([&](unsigned int i, float f) {
+            if (w.bin(f) <= b2) append(search, f, i);
+          });
+          everyone();
+          gathered = all;
+          return GATHERED;
+        }
+      }
+      const unsigned int n = sh.found[2], key_lo = edge_of(m, false), key_hi = without_minus_zero(edge_of(m, true));
       if constexpr (BY_COUNT) above += sh.found[1];
       const bool one = key_lo == key_hi, listed = !one && n <= LIST;
       const unsigned int width = key_hi - key_lo;
@@ -298,23 +381,24 @@ struct Sampler {
       __syncthreads();  // the bins are zeroed, sh.found is read
       double s1 = 0.0, s2 = 0.0;
       if (!BY_COUNT || !one) {
-        each([&](unsigned int i, float f) {
-          const unsigned int key = key_of(f);
-          if (key < key_lo) return;
-          if constexpr (!BY_COUNT) {
-            const double x = w.of(f);
-            s2 += x;
-            if (key > key_hi) s1 += x;
-          }
-          if (key > key_hi || one) return;
-          if (listed) {
-            unsigned int* counter = ranks > 1 ? cluster.map_shared_rank(&sh.gathered_n[search], 0) : &sh.gathered_n[search];
-            unsigned long long* list = ranks > 1 ? cluster.map_shared_rank(sh.gathered, 0) : sh.gathered;
-            list[atomicAdd(counter, 1u) % LIST] = (unsigned long long)~key << 32 | i;
-          } else {
-            atomicAdd(&sh.bins[next][(key_hi - key) >> new_shift], 1u);
-          }
-        });
+        const float least_in = value_of(key_lo), most_in = value_of(key_hi);
+        if (!one)
+          each([&](unsigned int i, float f) {
+            if (!(f >= least_in && f <= most_in)) return;
+            if (listed) append(search, f, i);
+            else atomicAdd(&sh.bins[next][(key_hi - key_of(f)) >> new_shift], 1u);
+          });
+        if constexpr (!BY_COUNT)
+          each_vector([&](unsigned int, const float (&f)[N]) {
+            double x[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[j] = w.of(f[j]);
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+              s2 += f[j] >= least_in ? x[j] : 0.0;
+              s1 += f[j] > most_in ? x[j] : 0.0;
+            }
+          });
         if constexpr (!BY_COUNT) sum2(s1, s2);
         else everyone();
       }
@@ -324,7 +408,7 @@ struct Sampler {
           // the estimate was beside it: the bins between, counted anew
           const unsigned int old_lo = edge_of(b2, false), old_hi = edge_of(b1, true);
           lo = left ? key_hi + 1 : old_lo;
-          hi = left ? old_hi : key_lo - 1;
+          hi = without_minus_zero(left ? old_hi : key_lo - 1);
           mass = left ? 0.0 : s2;
           shift = 0;
           while ((hi - lo) >> shift >= BINS) ++shift;
@@ -334,10 +418,11 @@ struct Sampler {
           __syncthreads();
           each([&](unsigned int i, float f) {
             const unsigned int key = key_of(f);
-            if (key > hi && left) above_window += w.of(f);
             if (key >= lo && key <= hi) atomicAdd(&sh.bins[next][(hi - key) >> shift], 1u);
           });
           if (left) {
+            const float above_this = value_of(hi);
+            each_vector([&](unsigned int, const float (&f)[N]) { above_window += weigh(f, [&](float g) { return g > above_this; }); });
             sum2(above_window, none);
             mass = above_window;
           }
@@ -355,11 +440,11 @@ struct Sampler {
           const double more = ceil((target - s1) / w.of(cut.value));
           cut.ties = more < 1.0 ? 1u : more > (double)n ? n : (unsigned int)more;
         }
-        return true;
+        return CUT;
       }
       if (listed) {
         order_list(n, BY_COUNT ? (double)(goal - above) : target, s1, BY_COUNT, cut);
-        return true;
+        return CUT;
       }
       lo = key_lo;
       hi = key_hi;
@@ -370,8 +455,14 @@ struct Sampler {
     }
   }
 
-  // The cut among the n gathered tokens.
-  __device__ __forceinline__ void order_list(unsigned int n, double target, double before, bool by_count, Cut& cut) {
+  // A token into the first block's list.
+  __device__ __forceinline__ void append(int search, float f, unsigned int i) {
+    unsigned int* counter = ranks > 1 ? cluster.map_shared_rank(&sh.gathered_n[search], 0) : &sh.gathered_n[search];
+    unsigned long long* list = ranks > 1 ? cluster.map_shared_rank(sh.gathered, 0) : sh.gathered;
+    list[atomicAdd(counter, 1u) % LIST] = (unsigned long long)~key_of(f) << 32 | i;
+  }
+  // The n gathered tokens in `ordered`: by falling logit, equal ones by number.
+  __device__ __forceinline__ void order(unsigned int n) {
     const unsigned long long* list = ranks > 1 ? cluster.map_shared_rank(sh.gathered, 0) : sh.gathered;
     const unsigned int t = threadIdx.x;
     unsigned long long mine = ~0ull;
@@ -383,6 +474,48 @@ struct Sampler {
       sh.ordered[place] = mine;
     }
     __syncthreads();
+  }
+  // The token from n gathered ones that hold all that are kept, by the first block. mass: of all tokens that top_p counts, where it is not that of the first top_k.
+  __device__ __forceinline__ void choose(unsigned int r, unsigned int n, unsigned int top_k, bool by_k, double mass, bool by_p, double top_p, double least, double u) {
+    order(n);
+    const unsigned int t = threadIdx.x, number = t < n ? (unsigned int)sh.ordered[t] : 0xFFFFFFFFu;
+    const float logit = t < n ? value_of(~(unsigned int)(sh.ordered[t] >> 32)) : -INFINITY;
+    double x = t < n && (!by_k || t < top_k) ? w.of(logit) : 0.0;
+    if (by_p) {
+      const double upto = scan(x, sh.warp_sums[0]);
+      if (by_k) {
+        mass = 0.0;
+        for (int i = 0; i < SAMPLE_WARPS; ++i) mass += sh.warp_sums[0][i];
+      }
+      if (t > 0 && !(upto - x < top_p * mass)) x = 0.0;
+    }
+    if (t > 0 && !(x >= least)) x = 0.0;
+    // kept tokens by number
+    __syncthreads();
+    sh.own[t] = (unsigned long long)number << 32 | t;
+    const unsigned int kept = __syncthreads_count(x > 0.0);  // a prefix
+    double* sums = reinterpret_cast<double*>(sh.gathered);
+    if (t < kept) {
+      unsigned int place = 0;
+      for (unsigned int j = 0; j < kept; ++j) place += sh.own[j] < sh.own[t];
+      sums[place] = x;
+      sh.ordered[place] = (unsigned long long)__float_as_uint(logit) << 32 | number;
+    }
+    __syncthreads();
+    const double upto = scan(t < kept ? sums[t] : 0.0, sh.warp_sums[0]);
+    double total = 0.0;
+    for (int i = 0; i < SAMPLE_WARPS; ++i) total += sh.warp_sums[0][i];
+    const double target = target_of(u, total);
+    unsigned int at = __syncthreads_count(t < kept && !(upto > target));
+    if (at >= kept) at = kept - 1;
+    if (t == 0) write(r, (unsigned int)sh.ordered[at], (float)(w.exponent(__uint_as_float((unsigned int)(sh.ordered[at] >> 32))) - log(total)));
+  }
+  __device__ __forceinline__ static double target_of(double u, double total) { return u >= 0.0 ? u * total : u < 0.0 ? 0.0 : INFINITY; }  // NaN: the end
+
+  // The cut among the n gathered tokens.
+  __device__ __forceinline__ void order_list(unsigned int n, double target, double before, bool by_count, Cut& cut) {
+    order(n);
+    const unsigned int t = threadIdx.x;
     const unsigned int key = t < n ? ~(unsigned int)(sh.ordered[t] >> 32) : 0;
     unsigned int keep;
     if (by_count) {
@@ -429,6 +562,8 @@ struct Sampler {
     if (lane == 0) sh.warp_sums[0][warp] = top;
     for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) sh.bins[0][i] = 0;
     if (threadIdx.x < 2) sh.gathered_n[threadIdx.x] = 0;
+    if (threadIdx.x < STEPS) sh.powers[threadIdx.x] = exp2(threadIdx.x / (double)STEPS);
+    w.powers = sh.powers;
     __syncthreads();
     for (int i = 0; i < SAMPLE_WARPS; ++i) top = fmaxf(top, (float)sh.warp_sums[0][i]);
     give(top, 0.0);
@@ -452,34 +587,39 @@ struct Sampler {
       return;
     }
     t = fminf(t, 3.4028235e38f);
-    w.top = top;
-    w.inv_t = 1.0 / (double)t;
-    w.half_top = 0.5f * top;
-    w.per_bin = (float)fmin(2 * (BINS - 1) / REACH * w.inv_t, 1e38);
+    w.set(top, t);
     Cut cut{-INFINITY, 0, 0};
     const bool by_k = top_k > 0 && (unsigned int)top_k < a.vocab, by_p = top_p < 1.f;
     if (by_k || by_p) {
       double all = 0.0, none = 0.0;
-      each([&](unsigned int i, float f) {
+      each([&](unsigned int, float f) {
         const unsigned int b = w.bin(f);
         if (b < BINS - 1) atomicAdd(&sh.bins[0][b], 1u);
-        if (!by_k) all += w.of(f);
       });
+      if (!by_k)
+        each_vector([&](unsigned int, const float (&f)[N]) { all += weigh(f, [](float) { return true; }); });
       sum2(all, none);  // of all blocks: the bins are counted
+      unsigned int n = 0;
       if (by_k) {
-        find<true>(top_k, 0, cut);
+        if (find<true>(top_k, 0, cut, n) == GATHERED) {
+          if (rank == 0) choose(r, n, top_k, true, 0.0, by_p, top_p, min_p, u);
+          return;
+        }
         if (by_p) {
           all = none = 0.0;
-          each([&](unsigned int i, float f) {
-            if (f > cut.value) all += w.of(f);
-          });
+          each_vector([&](unsigned int, const float (&f)[N]) { all += weigh(f, [&](float g) { return g > cut.value; }); });
           sum2(all, none);
           if (cut.ties) all += cut.ties * w.of(cut.value);
         }
       }
       if (by_p) {
         Cut c;
-        if (find<false>((double)top_p * all, 1, c) && (c.value > cut.value || (c.value == cut.value && c.ties < cut.ties))) cut = c;
+        const Found found = find<false>((double)top_p * all, 1, c, n);
+        if (found == GATHERED) {
+          if (rank == 0) choose(r, n, 0, false, all, true, top_p, min_p, u);
+          return;
+        }
+        if (found == CUT && (c.value > cut.value || (c.value == cut.value && c.ties < cut.ties))) cut = c;
       }
     }
     // tokens at the cut: how many of them in blocks and warps before this one
@@ -530,14 +670,12 @@ struct Sampler {
         seen += tile;
       }
 #pragma unroll
+      for (int j = 0; j < N; ++j) x[j] = w.of(f[j]);
+#pragma unroll
       for (int j = 0; j < N; ++j) {
-        bool keep = f[j] > cut.value;
-        if (ties && f[j] == cut.value) keep = order++ < ties;
-        x[j] = 0.0;
-        if (keep) {
-          const double v = w.of(f[j]);
-          if (v >= least) x[j] = v;
-        }
+        const bool equal = f[j] == cut.value && ties, keep = (f[j] > cut.value || (equal && order < ties)) && x[j] >= least;
+        order += equal;
+        x[j] = keep ? x[j] : 0.0;
       }
     };
     double sum = 0.0;
@@ -559,7 +697,7 @@ struct Sampler {
     double total = 0.0;
     for (int i = 0; i < ranks; ++i) total += taken(i, 0);
     // which block, and which warp of it; the last one with any weight where rounding, or u, leaves none
-    const double target = u >= 0.0 ? u * total : u < 0.0 ? 0.0 : INFINITY;  // NaN: the end
+    const double target = target_of(u, total);
     int where = -1;
     double upto = 0.0, start = 0.0;
     bool crossed = false;
@@ -630,7 +768,7 @@ struct Sampler {
 };
 
 template <typename T, bool HELD>
-__global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleArgs a) {
   __shared__ SampleShared sh;
   extern __shared__ uint4 held[];
   cg::cluster_group cluster = cg::this_cluster();

@@ -495,8 +495,8 @@ int b2_clip(size_t count, const b2_clip_tensor* tensors, float max_norm, float* 
  * temperature <= 0, top_k = 1, top_p <= 0 or min_p > 1 is the first token in that order, logprob 0. top_k <= 0, top_p >= 1 and min_p <= 0 are no limit. Each of the
  * four may be given for each row (device memory: row_...), in place of the one for all. A logit of -inf or NaN is never taken; a row of nothing else
  * gives token -1 and logprob 0. Logits of +inf share all the weight. u outside of [0, 1) counts as the nearer end, NaN as 1.
- * Weights are computed and summed in fp64, so that the token is the one of the formula unless u or a border lies within about 1e-11 of a step of
- * the running sum; weights below e^-40 of the largest count as none where a limit is looked for. Equal inputs give equal tokens. tokens are 32- or 64-bit integers
+ * Where fp32 leaves the token open, weights are summed in fp64: it is the one of the formula unless u or a border lies within about 1e-11 of a step of
+ * the running sum. Weights below e^-40 of the largest count as none where a limit is looked for. logprob is off by 4e-7 at most, and half a step of fp32. Equal inputs give equal tokens. tokens are 32- or 64-bit integers
  * (token_bytes). Limits: rows and vocab at most 2^24 each. */
 typedef struct {
   float temperature;
@@ -508,8 +508,10 @@ typedef struct {
 } b2_sample_options;
 /* temperature 1, top_k 0, top_p 1, min_p 0, no row has its own */
 int b2_sample_options_default(b2_sample_options* options);
+int b2_sample_workspace(size_t rows, size_t vocab, size_t* bytes);
 int b2_sample(size_t rows, size_t vocab, int dtype, const void* logits, size_t ld, const float* u,
-              const b2_sample_options* options, void* tokens, int token_bytes, float* logprob, void* stream);
+              const b2_sample_options* options, void* tokens, int token_bytes, float* logprob, void* workspace,
+              size_t workspace_bytes, void* stream);
 
 /* Waits for `stream` and returns B2_ERR_TIMEOUT if a bounded wait inside one of this section's tensor-core kernels on
  * the current device gave up since the last b2_lm_sync of the same stream (at its first: since the library was loaded), B2_OK otherwise.

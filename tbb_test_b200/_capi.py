@@ -122,7 +122,8 @@ SYMBOLS = {
     "b2_clip_workspace": (C.c_int, [_sz, C.POINTER(_sz)]),
     "b2_clip": (C.c_int, [_sz, _vp, C.c_float, _vp, _vp, _sz, _vp]),
     "b2_sample_options_default": (C.c_int, [C.POINTER(SampleOptions)]),
-    "b2_sample": (C.c_int, [_sz, _sz, C.c_int, _vp, _sz, _vp, C.POINTER(SampleOptions), _vp, C.c_int, _vp, _vp]),
+    "b2_sample_workspace": (C.c_int, [_sz, _sz, C.POINTER(_sz)]),
+    "b2_sample": (C.c_int, [_sz, _sz, C.c_int, _vp, _sz, _vp, C.POINTER(SampleOptions), _vp, C.c_int, _vp, _vp, _sz, _vp]),
     "b2_lm_sync": (C.c_int, [_vp]),
 }
 

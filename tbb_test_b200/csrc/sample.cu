@@ -3,37 +3,48 @@
 //   w[v] = exp((x[v] - max) / T)      kept = a prefix of the tokens in falling order of x, equal ones by number
 //   token = first v by number with  sum of kept w up to v  >  u * sum of all kept w
 //
-// A cluster of 1, 2, 4 or 8 blocks takes a row, each block a part of it by number and each warp a part of that. Nothing is sorted: top-k and top-p
-// are a logit (the last one kept) and how many of the tokens that have exactly this one are kept, found by counting tokens in bins:
-// first bins of equal width in (max - x) / T, then of equal width in the logit's bits inside the bin in which the limit must lie, until a bin has few
-// enough tokens to put them in order one by one, or a single logit. For top-k counts say which bin. For top-p they only give an estimate, since a bin's
-// weights differ; the weight above and up to the bin is then summed exactly, so that a wrong estimate is found and the search goes on beside it.
-// Then every warp sums its kept weights, and the one in which the running sum crosses the target goes through its part once more.
+// Bound by reading the logits once. Two kernels:
 //
-// Sums are in fp64: with a vocabulary of 10^5 a step of the running sum may be 10^-5 of it, and what the sum is off, times the number of steps, is the
-// probability that another token comes out.
-#include <cooperative_groups.h>
+//   sample_tiles_kernel   a warp per tile of 1024 logits: their maximum, their weight relative to it, and for top-k each lane's maximum
+//   sample_kernel         a block per row. From the tiles' numbers come the row's maximum and weight. Without a limit the tile in which the running
+//                         weight crosses u's share is read once more. Otherwise a floor below which no token is kept comes from the lanes' maxima (top-k: as many
+//                         lanes as top_k reach it), the row's weight (top-p: tokens of less than (1 - p) / vocab of it are never needed) or the least
+//                         weight (min-p), and the tokens above it, mostly few, are gathered from the tiles that have any.
+//
+// Up to 512 gathered tokens are put in order one by one. With more nothing is sorted: top-k and top-p are a logit (the last one kept) and how many of the
+// tokens that have exactly this one are kept, found by counting tokens in bins: first bins of equal width in max - x, then of equal width in the logit's bits
+// inside the bin in which the limit must lie, until a bin has few enough tokens to put them in order, or a single logit. For top-k counts say which bin. For top-p
+// they only give an estimate, since a bin's weights differ; the weight above and up to the bin is then summed exactly, so that a wrong estimate is
+// found and the search goes on beside it.
+//
+// The token has to be the exact formula's. With a vocabulary of 10^5 a step of the running sum may be 10^-5 of it, and what the sum is off, times the number
+// of steps, is the probability that another token comes out: sums in fp32 would be wrong in some of a thousand rows. So a weight is computed to 5e-12 and summed in
+// fp64, some 30 instructions; but where all tokens of a row count (no limit, or top-p's whole weight), first in fp32, 8 instructions, with a bound of the
+// error: only where target and step are nearer than that, the row is summed once more in fp64.
 #include <math.h>
 
 #include "lm.cuh"
-
-namespace cg = cooperative_groups;
 
 namespace b2 {
 namespace {
 
 constexpr int SAMPLE_THREADS = 512, SAMPLE_WARPS = SAMPLE_THREADS / 32;
+constexpr int TILE_THREADS = 256, TILE = 1024, PER_LANE = TILE / 32;
 constexpr int BINS = 1024, BINS_PER_THREAD = BINS / SAMPLE_THREADS;
-constexpr float REACH = 40.f;  // of the first bins, in units of T: the last bin has all tokens of less than e^-40 of the largest weight
 constexpr int LIST = SAMPLE_THREADS;  // tokens that are put in order one by one
-constexpr int MOST_CLUSTER = 8;
-constexpr int STEPS = 16;  // 2^(n / 16) for n = 0 to 15 lie in different banks of shared memory
+constexpr int STORED = 8192;          // gathered tokens that shared memory holds; of more, those of the row are read again for each pass
+constexpr int STEPS = 16;             // 2^(n / 16) for n = 0 to 15 lie in different banks of shared memory
+constexpr double REACH = 40.0;        // in units of T: what weighs less than e^-40 of the largest weighs nothing where a limit is looked for
+
+struct TileStat {
+  double weight;  // of its tokens relative to 2^rint(largest * c), see FastWeights; negative: not to be had in fp32
+  float largest, none;
+};
 
 struct SampleArgs {
   const char* logits;
   size_t ld;  // bytes
-  unsigned int vocab, part;  // part: tokens per block, whole tiles for each warp
-  int vec;                   // rows begin on 16-byte boundaries
+  unsigned int vocab, tiles;
   const float* u;
   float temperature, top_p, min_p;
   int top_k;
@@ -42,17 +53,62 @@ struct SampleArgs {
   void* tokens;
   int wide;
   float* logprob;
+  TileStat* stats;    // rows x tiles
+  float* lane_most;   // rows x tiles x 32, or null where no row has a top_k
+  unsigned int* open;        // rows whose token fp32 leaves open
+  unsigned int* open_count;
 };
 
-struct SampleShared {
-  unsigned int bins[3][BINS];  // the first ones, and two that take turns
-  unsigned long long gathered[LIST], own[LIST], ordered[LIST];
-  unsigned int gathered_n[2];  // by search
-  double slots[2][MOST_CLUSTER][2];
-  double warp_sums[2][SAMPLE_WARPS];
-  unsigned int warp_counts[SAMPLE_WARPS];
-  unsigned int found[4];
-  double powers[STEPS];
+// What one row asks for.
+struct SampleRow {
+  float t, top_p, min_p;
+  int top_k;
+  bool by_k, by_p, by_m, greedy, whole;  // whole: the row's whole weight is needed
+  __device__ __forceinline__ SampleRow(const SampleArgs& a, size_t r) {
+    t = a.row_temperature ? a.row_temperature[r] : a.temperature;
+    top_p = a.row_top_p ? a.row_top_p[r] : a.top_p;
+    min_p = a.row_min_p ? a.row_min_p[r] : a.min_p;
+    top_k = a.row_top_k ? a.row_top_k[r] : a.top_k;
+    greedy = !(t > 0.f) || top_k == 1 || top_p <= 0.f || min_p > 1.f;
+    t = fminf(t, 3.4028235e38f);
+    by_k = top_k > 0 && (unsigned int)top_k < a.vocab;
+    by_p = top_p < 1.f;
+    by_m = min_p > 0.f;
+    whole = !greedy && !by_k && (by_p || !by_m);
+  }
+};
+
+// A row's tokens by place: place = number + shift, so that vectors of 16 bytes of the row begin at multiples of their length. What is not in the row, or not a
+// number, is -inf.
+template <typename T>
+struct RowView {
+  const T* row;
+  unsigned int shift, end;  // end: the place behind the last one
+  __device__ __forceinline__ RowView(const SampleArgs& a, size_t r) {
+    row = reinterpret_cast<const T*>(a.logits + r * a.ld);
+    shift = (unsigned int)(reinterpret_cast<size_t>(row) & 15) / sizeof(T);
+    end = a.vocab + shift;
+  }
+  // 16 bytes from place i on as they are, what is not in the row as -inf
+  __device__ __forceinline__ uint4 load_vector(unsigned int i) const {
+    constexpr int N = 16 / (int)sizeof(T);
+    if (i >= shift && i + N <= end) return __ldg(reinterpret_cast<const uint4*>(row + (i - shift)));
+    float f[N];
+    load(i, f);
+    return Elems<T, 16>::put(f);
+  }
+  // M neighbours from place i on, a multiple of M
+  template <int M>
+  __device__ __forceinline__ void load(unsigned int i, float (&f)[M]) const {
+    if (i >= shift && i + M <= end) {
+      Elems<T, M * (int)sizeof(T)>::get(__ldg(reinterpret_cast<const typename Raw<M * (int)sizeof(T)>::type*>(row + (i - shift))), f);
+#pragma unroll
+      for (int j = 0; j < M; ++j) f[j] = fmaxf(f[j], -INFINITY);
+    } else {
+#pragma unroll
+      for (int j = 0; j < M; ++j) f[j] = i + j >= shift && i + j < end ? fmaxf((float)row[i + j - shift], -INFINITY) : -INFINITY;
+    }
+  }
 };
 
 // Logits as unsigned numbers in the same order; -0 is +0, so that no token has the key below +0's.
@@ -97,9 +153,12 @@ struct Weights {
     steps = STEPS * 1.4426950408889634 * inv_t;
     least = top == INFINITY ? top : (float)fmax((double)top - 693.0 * (double)t, -3.4028234663852886e38);
     half_top = 0.5f * top;
-    per_bin = (float)fmin(2 * (BINS - 1) / REACH * inv_t, 1e38);
   }
+  // Bins that reach `span` below the top, in units of T; the last one has all that is lower.
+  __device__ __forceinline__ void set_bins(double span) { per_bin = (float)fmin(2 * (BINS - 1) / span * inv_t, 1e38); }
   __device__ __forceinline__ double exponent(float f) const { return f == top ? 0.0 : ((double)f - (double)top) * inv_t; }
+  // The weight of a logit `by` below the top.
+  __device__ __forceinline__ double below(double by) const { return exp2(-by * (steps / STEPS)); }
   // The weight: 2^((n + s) / 16), n an integer
   __device__ __forceinline__ double of(float f) const {
     const float g = fmaxf(f, least);
@@ -118,118 +177,252 @@ struct Weights {
   }
 };
 
+// Weights in fp32 up to a factor that all of them share: 2^(x c - N) with c = log2(e) / T and N = rint(largest c), by the nearest integer n of x c and 2^(x c - n).
+// A sum of eight is off by at most 3.5e-7 of itself: 1.5e-7 for ex2.approx (the most over all numbers in +-0.51), 2e-8 for its argument, 2^-24 for each of
+// three additions. Two such sums are compared: SLACK is twice that and a third more.
+constexpr double SLACK = 9.5367431640625e-7;  // 2^-20
+struct FastWeights {
+  float c, c_low, magic, least;
+  double n;     // N
+  bool usable;  // x c is exact enough and all of it in range
+  __device__ __forceinline__ void set(float largest, float t) {
+    const double exact = 1.4426950408889634 / (double)t;
+    n = rint((double)largest * exact);
+    c = (float)exact;
+    c_low = (float)(exact - (double)c);
+    magic = (float)(12582912.0 - n);  // 1.5 * 2^23: the sum's low bits are n of x c less N
+    least = (float)((double)largest - 80.0 * (double)t);
+    usable = t > 1e-25f && t < 1e25f && fabs(n) < 262144.0;
+  }
+  __device__ __forceinline__ float of(float f) const {
+    f = fmaxf(f, least);
+    const float m = fmaf(f, c, magic);
+    float r = fmaf(f, c, magic - m), y;
+    r = fmaf(f, c_low, r);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(r));
+    return __uint_as_float(__float_as_uint(y) + (__float_as_uint(m) << 23));
+  }
+  // What weights relative to another largest logit are to be multiplied by: a power of two.
+  __device__ __forceinline__ double unit(float other, float t) const {
+    const double by = rint((double)other * (1.4426950408889634 / (double)t)) - n;
+    return __hiloint2double((1023 + (int)fmax(by, -1000.0)) << 20, 0);
+  }
+  // To weights relative to the largest logit itself.
+  __device__ __forceinline__ double to_top(const Weights& w) const { return exp2(n - (double)w.top * 1.4426950408889634 * w.inv_t); }
+  template <int M>
+  __device__ __forceinline__ double sum(const float (&f)[M]) const {
+    float x[M];
+#pragma unroll
+    for (int j = 0; j < M; ++j) x[j] = of(f[j]);
+#pragma unroll
+    for (int o = 1; o < M; o *= 2)
+#pragma unroll
+      for (int j = 0; j + o < M; j += 2 * o) x[j] += x[j + o];
+    return (double)x[0];
+  }
+};
+
+// The largest of 16 bytes of logits; NaN is none.
+template <typename T>
+__device__ __forceinline__ float largest_of(const uint4& v) {
+  if constexpr (sizeof(T) == 2) {
+    const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const __nv_bfloat162 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+    return fmaxf(fmaxf(__low2float(m), __high2float(m)), -INFINITY);
+  } else {
+    const float* p = reinterpret_cast<const float*>(&v);
+    return fmaxf(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3])), -INFINITY);
+  }
+}
+
+// A warp per tile.
+template <typename T>
+__global__ void __launch_bounds__(TILE_THREADS) sample_tiles_kernel(const SampleArgs a, unsigned long long all) {
+  constexpr int N = 16 / (int)sizeof(T), VECS = PER_LANE / N;
+  let_next_start();
+  const unsigned long long tile = ((unsigned long long)blockIdx.x * TILE_THREADS + threadIdx.x) >> 5;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.open_count = 0;
+  if (tile >= all) return;
+  const size_t r = tile / a.tiles;
+  const unsigned int lane = threadIdx.x & 31, first = (unsigned int)(tile - r * a.tiles) * TILE + lane * N;
+  const RowView<T> row(a, r);
+  uint4 v[VECS];
+#pragma unroll
+  for (int k = 0; k < VECS; ++k) v[k] = row.load_vector(first + k * 32 * N);
+  float most = largest_of<T>(v[0]);
+#pragma unroll
+  for (int k = 1; k < VECS; ++k) most = fmaxf(most, largest_of<T>(v[k]));
+  if (a.lane_most) a.lane_most[tile * 32 + lane] = most;
+  for (int o = 16; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+  const SampleRow ask(a, r);
+  double sum = 0.0;
+  if (ask.whole && most > -INFINITY) {
+    FastWeights w;
+    w.set(most, ask.t);
+    if (w.usable) {
+#pragma unroll
+      for (int k = 0; k < VECS; ++k) {
+        float f[N];
+        Elems<T, 16>::get(v[k], f);
+        sum += w.sum(f);
+      }
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    } else {
+      sum = -1.0;
+    }
+  }
+  if (lane == 0) a.stats[tile] = TileStat{sum, most, 0.f};
+}
+
+struct SampleShared {
+  unsigned int bins[3][BINS];  // the first ones, and two that take turns
+  unsigned long long list[LIST], ordered[LIST], own[LIST];
+  double sums[2][SAMPLE_WARPS];
+  double powers[STEPS];
+  unsigned int counts[SAMPLE_WARPS], found[4], listed;
+  float stored[STORED];          // gathered tokens by number
+  unsigned int number[STORED];
+};
+
 // What is kept: logits above `value`, and the first `ties` of `equal` tokens that have it.
 struct Cut {
   float value;
   unsigned int ties, equal;
 };
 
-template <typename T, bool HELD>
+
+__device__ __forceinline__ double warp_sum(double s) {
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+  return s;
+}
+__device__ __forceinline__ float warp_max(float m) {
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  return m;
+}
+__device__ __forceinline__ double target_of(double u, double total) { return u >= 0.0 ? u * total : u < 0.0 ? 0.0 : INFINITY; }  // NaN: the end
+
+// One warp's: the number of the first token of a tile that has this logit.
+template <typename T>
+__device__ __forceinline__ unsigned int first_of(const RowView<T>& row, unsigned int tile, float logit, int lane) {
+  constexpr int N = 16 / (int)sizeof(T);
+  unsigned int at = 0xFFFFFFFFu;
+  for (unsigned int i = tile * TILE + lane * N; i < (tile + 1) * TILE; i += 32 * N) {
+    float f[N];
+    row.load(i, f);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (f[j] == logit) at = min(at, i + j);
+  }
+  return __reduce_min_sync(0xFFFFFFFFu, at) - row.shift;
+}
+
+// One warp's: the first token of places [from, to) with which `start` and the weight exceed the target, its weight, and in `start` what lies before it; without one the
+// last token with any weight. weights(i, f, x): a lane's K logits from place i on and their weights, 0 for what is not kept.
+template <int K, class V, class Of>
+__device__ __forceinline__ bool walk(int lane, unsigned int from, unsigned int to, double& start, double target, unsigned int& place, float& logit, double& weight, Of weights) {
+  for (unsigned int i = from + lane * K; i - lane * K < to; i += 32 * K) {
+    float f[K];
+    V x[K];
+    weights(i, f, x);
+    double mine = 0.0;
+#pragma unroll
+    for (int j = 0; j < K; ++j) mine += (double)x[j];
+    double run = mine;
+    for (int o = 1; o < 32; o <<= 1) {
+      const double below = __shfl_up_sync(0xFFFFFFFFu, run, o);
+      if (lane >= o) run += below;
+    }
+    const unsigned int past = __ballot_sync(0xFFFFFFFFu, mine > 0.0 && start + run > target);
+    const unsigned int any = __ballot_sync(0xFFFFFFFFu, mine > 0.0);
+    if (any) {
+      // in these vectors, or so far the last token with any weight
+      const int who = past ? __ffs(past) - 1 : 31 - __clz(any);
+      unsigned int at = 0;
+      float l = 0.f;
+      double s = start + (run - mine), before = s, own = 0.0;
+      bool done = false;
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        if (x[j] > (V)0 && !done) {
+          at = i + j;
+          l = f[j];
+          before = s;
+          own = (double)x[j];
+          s += own;
+          done = past && s > target;
+        }
+      }
+      place = __shfl_sync(0xFFFFFFFFu, at, who);
+      logit = __shfl_sync(0xFFFFFFFFu, l, who);
+      weight = __shfl_sync(0xFFFFFFFFu, own, who);
+      before = __shfl_sync(0xFFFFFFFFu, before, who);
+      if (past) {
+        start = before;
+        return true;
+      }
+    }
+    start += __shfl_sync(0xFFFFFFFFu, run, 31);
+  }
+  return false;
+}
+
+template <typename T>
 struct Sampler {
-  static constexpr int N = 16 / (int)sizeof(T), TILE = 32 * N;
+  static constexpr int M = 4;  // neighbours that a lane takes at a time, of the gathered tokens or of the row
   const SampleArgs& a;
   SampleShared& sh;
-  cg::cluster_group cluster;
-  const T* row;           // the whole row
-  const uint4* held;      // this block's part in shared memory
-  unsigned int part0, w0, w1;  // tokens: the block's first one, the warp's first one and the end of its tiles
-  int lane, warp, ranks, rank, turn;
+  size_t r;
+  RowView<T> row;
+  int lane, warp;
   Weights w;
+  bool stored;                // places are those of the gathered tokens, otherwise the row's
+  unsigned int begin, end;    // the warp's places
+  float floor;                // of those that count
 
-  __device__ __forceinline__ void everyone() {
-    if (ranks > 1) cluster.sync();
-    else __syncthreads();
-  }
-  // N tokens from number i on, NaN and what is behind the row as -inf.
-  __device__ __forceinline__ void load(unsigned int i, float (&f)[N]) const {
-    if (a.vec && i + N <= a.vocab) {
-      Elems<T, 16>::get(__ldg(reinterpret_cast<const uint4*>(row + i)), f);
-#pragma unroll
-      for (int j = 0; j < N; ++j) f[j] = fmaxf(f[j], -INFINITY);
+  // M tokens from place i on; what does not count as -inf.
+  __device__ __forceinline__ void fetch(unsigned int i, float (&f)[M]) const {
+    if (stored) {
+      Elems<float, 16>::get(*reinterpret_cast<const uint4*>(sh.stored + i), f);
     } else {
+      row.load(i, f);
 #pragma unroll
-      for (int j = 0; j < N; ++j) f[j] = i + j < a.vocab ? fmaxf((float)row[i + j], -INFINITY) : -INFINITY;
+      for (int j = 0; j < M; ++j) f[j] = f[j] >= floor ? f[j] : -INFINITY;
     }
   }
-  __device__ __forceinline__ void fetch(unsigned int i, float (&f)[N]) const {
-    if constexpr (HELD) Elems<T, 16>::get(held[(i - part0) / N], f);
-    else load(i, f);
-  }
-  // body(number, logit) for the warp's tokens, lane by lane N neighbours at a time.
+  __device__ __forceinline__ unsigned int number_of(unsigned int place) const { return stored ? sh.number[place] : place - row.shift; }
+  // body(place of the first, logits) for the warp's tokens.
   template <class Body>
   __device__ __forceinline__ void each(Body body) const {
-    for (unsigned int i = w0 + lane * N; i < w1; i += TILE) {
-      float f[N];
-      fetch(i, f);
-#pragma unroll
-      for (int j = 0; j < N; ++j) body(i + j, f[j]);
-    }
-  }
-
-  // body(number of the first, logits) for the warp's tokens, N neighbours at a time.
-  template <class Body>
-  __device__ __forceinline__ void each_vector(Body body) const {
-    for (unsigned int i = w0 + lane * N; i < w1; i += TILE) {
-      float f[N];
+    for (unsigned int i = begin + lane * M; i - lane * M < end; i += 32 * M) {
+      float f[M];
       fetch(i, f);
       body(i, f);
     }
   }
-  // The sum of the weights that `counts` says, without a branch: the N computations go side by side.
-  template <class Counts>
-  __device__ __forceinline__ double weigh(const float (&f)[N], Counts counts) const {
-    double x[N];
+  // The weight of those that `counts` says, without a branch: the computations go side by side.
+  template <int K, class Counts>
+  __device__ __forceinline__ double weigh(const float (&f)[K], Counts counts) const {
+    double x[K];
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
+    for (int j = 0; j < K; ++j) {
       x[j] = w.of(f[j]);
       x[j] = counts(f[j]) ? x[j] : 0.0;
     }
 #pragma unroll
-    for (int o = 1; o < N; o *= 2)
+    for (int o = 1; o < K; o *= 2)
 #pragma unroll
-      for (int j = 0; j + o < N; j += 2 * o) x[j] += x[j + o];
+      for (int j = 0; j + o < K; j += 2 * o) x[j] += x[j + o];
     return x[0];
   }
-
-  // Sums over the cluster of two values per thread, the same bits everywhere.
-  __device__ __forceinline__ void sum2(double& x, double& y) {
-    for (int o = 16; o; o >>= 1) {
-      x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
-      y += __shfl_xor_sync(0xFFFFFFFFu, y, o);
-    }
-    if (lane == 0) {
-      sh.warp_sums[0][warp] = x;
-      sh.warp_sums[1][warp] = y;
-    }
+  // Sums over the block of one value per thread, the same bits in all; the warps' own stay in sh.sums[k].
+  __device__ __forceinline__ double block_sum(double s, int k) {
+    s = warp_sum(s);
     __syncthreads();
-    x = y = 0.0;
-    for (int i = 0; i < SAMPLE_WARPS; ++i) {
-      x += sh.warp_sums[0][i];
-      y += sh.warp_sums[1][i];
-    }
-    exchange(x, y);
+    if (lane == 0) sh.sums[k][warp] = s;
+    __syncthreads();
+    return warps_sum(k);
   }
-  // x and y: the block's, in all of its threads; sums over the blocks in their order.
-  __device__ __forceinline__ void exchange(double& x, double& y) {
-    give(x, y);
-    x = y = 0.0;
-    for (int i = 0; i < ranks; ++i) {
-      x += taken(i, 0);
-      y += taken(i, 1);
-    }
-  }
-  // Every block's pair into every block's slots. The other set of slots is written next time: who gets there has seen that all blocks are past reading this one.
-  __device__ __forceinline__ void give(double x, double y) {
-    turn ^= 1;
-    if ((int)threadIdx.x < ranks) {
-      double* s = ranks > 1 ? cluster.map_shared_rank(&sh.slots[turn][rank][0], threadIdx.x) : &sh.slots[turn][0][0];
-      s[0] = x;
-      s[1] = y;
-    }
-    everyone();
-  }
-  __device__ __forceinline__ double taken(int r, int k) const { return sh.slots[turn][r][k]; }
-
+  __device__ __forceinline__ double warps_sum(int k) const { return warp_sum(lane < SAMPLE_WARPS ? sh.sums[k][lane] : 0.0); }
   // Inclusive scan over the block's threads.
   template <typename V>
   __device__ __forceinline__ V scan(V v, V* sums) {
@@ -240,8 +433,21 @@ struct Sampler {
     __syncthreads();
     if (lane == 31) sums[warp] = v;
     __syncthreads();
-    for (int i = 0; i < warp; ++i) v += sums[i];
-    return v;
+    V before = lane < SAMPLE_WARPS ? sums[lane] : (V)0;
+    for (int o = 1; o < SAMPLE_WARPS; o <<= 1) {
+      const V below = __shfl_up_sync(0xFFFFFFFFu, before, o);
+      if (lane >= o) before += below;
+    }
+    before = __shfl_sync(0xFFFFFFFFu, before, warp ? warp - 1 : 0);
+    return warp ? before + v : v;
+  }
+  __device__ __forceinline__ unsigned int lanes_before(unsigned int v) const {
+    unsigned int upto = v;
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned int below = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+      if (lane >= o) upto += below;
+    }
+    return upto - v;
   }
 
   // Largest key whose first bin is at least b, and smallest whose first bin is at most b.
@@ -261,68 +467,68 @@ struct Sampler {
     return lo;
   }
 
-  // The cut at which `target` tokens (BY_COUNT) or `target` weight is reached. The first bins have been counted. search: 0 or 1, a list's counter of its own.
-  // NONE: it is not reached before the tokens that weigh nothing. GATHERED: no cut, but a list of `gathered` tokens from the first one on in which it lies.
-  enum Found { NONE, CUT, GATHERED };
+  // The first bin up to which the bins hold `count` (BINS where none does), with what is below it and in it in sh.found[1] and [2].
+  __device__ __forceinline__ unsigned int reaches(int buffer, unsigned int count) {
+    unsigned int own[BINS_PER_THREAD], mine = 0;
+#pragma unroll
+    for (int k = 0; k < BINS_PER_THREAD; ++k) mine += own[k] = sh.bins[buffer][threadIdx.x * BINS_PER_THREAD + k];
+    unsigned int upto = scan(mine, sh.counts) - mine;
+    if (threadIdx.x == 0) sh.found[0] = BINS;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < BINS_PER_THREAD; ++k) {
+      if (upto < count && count <= upto + own[k]) {
+        sh.found[0] = threadIdx.x * BINS_PER_THREAD + k;
+        sh.found[1] = upto;
+        sh.found[2] = own[k];
+      }
+      upto += own[k];
+    }
+    __syncthreads();
+    return sh.found[0];
+  }
+
+  // The cut at which `target` tokens (BY_COUNT) or `target` weight is reached. The first bins have been counted.
+  // slack: the target may be off by this share of it. NONE: it is not reached before the tokens that weigh nothing. UNSURE: where depends on what the target is off.
+  enum Found { NONE, CUT, UNSURE };
   template <bool BY_COUNT>
-  __device__ Found find(double target, int search, Cut& cut, unsigned int& gathered) {
+  __device__ __noinline__ Found find(double target, double slack, Cut& cut) {
+    const double target_low = target * (1.0 - slack), target_high = target * (1.0 + slack);
     unsigned int lo = 0, hi = key_of(w.top), shift = 0;  // the window's keys
-    const unsigned int goal = BY_COUNT ? (unsigned int)target : 0;
-    unsigned int above = 0;  // tokens above the window
-    double mass = 0.0;       // weight above the window
+    unsigned int goal = BY_COUNT ? (unsigned int)target : 0;
+    double mass = 0.0;  // weight above the window
     bool first = true;
     int buffer = 0;
     for (;;) {
-      if (!first) everyone();  // all blocks have counted
-      unsigned int count[BINS_PER_THREAD];
-#pragma unroll
-      for (int k = 0; k < BINS_PER_THREAD; ++k) {
-        count[k] = 0;
-        for (int r = 0; r < ranks; ++r)
-          count[k] += *(ranks > 1 ? cluster.map_shared_rank(&sh.bins[buffer][threadIdx.x * BINS_PER_THREAD + k], r) : &sh.bins[buffer][threadIdx.x * BINS_PER_THREAD + k]);
-      }
+      __syncthreads();  // all have counted
       const unsigned int next = buffer == 1 ? 2 : 1;
-      for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) sh.bins[next][i] = 0;
       auto edge_of = [&](unsigned int b, bool upper) -> unsigned int {
         if (first) return edge(b, upper);
         if (upper) return hi - (b << shift);
         const unsigned int down = ((b + 1) << shift) - 1;
         return hi - lo > down ? hi - down : lo;
       };
-      unsigned int b1 = 0, b2 = 0, m = 0;
+      unsigned int b1 = 0, b2 = 0, m = 0, above = 0;
       if constexpr (BY_COUNT) {
-        unsigned int mine = 0;
-#pragma unroll
-        for (int k = 0; k < BINS_PER_THREAD; ++k) mine += count[k];
-        unsigned int upto = scan(mine, sh.warp_counts) - mine;
-        if (threadIdx.x == 0) sh.found[0] = BINS;
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < BINS_PER_THREAD; ++k) {
-          if (above + upto < goal && goal <= above + upto + count[k]) {
-            sh.found[0] = threadIdx.x * BINS_PER_THREAD + k;
-            sh.found[1] = upto;
-            sh.found[2] = count[k];
-          }
-          upto += count[k];
-        }
-        __syncthreads();
-        m = sh.found[0];
+        m = reaches(buffer, goal);
         if (first && m >= BINS - 1) return NONE;
-        b2 = m;
+        above = sh.found[1];
       } else {
         // the running weight at the bins' ends, by the lightest, the heaviest and a middle token of each
+        unsigned int count[BINS_PER_THREAD], mine = 0;
         double low[BINS_PER_THREAD], mid[BINS_PER_THREAD], high[BINS_PER_THREAD];
         double sum_low = 0.0, sum_mid = 0.0, sum_high = 0.0;
 #pragma unroll
         for (int k = 0; k < BINS_PER_THREAD; ++k) {
           const unsigned int b = threadIdx.x * BINS_PER_THREAD + k;
+          count[k] = sh.bins[buffer][b];
+          mine += count[k];
           double wl = 0.0, wh = 0.0;
           if (count[k]) {
             if (first) {
-              const double width = 2.0 * w.inv_t / (double)w.per_bin;  // rounded differences and products move a token by less than 1e-3 of a bin
-              wl = exp(-width * (b + 1.001));
-              wh = exp(-width * (b > 0 ? b - 0.001 : 0.0));
+              const double width = 2.0 / (double)w.per_bin;  // rounded differences and products move a token by less than 1e-3 of a bin
+              wl = w.below(width * (b + 1.001));
+              wh = w.below(width * (b > 0 ? b - 0.001 : 0.0));
             } else {
               wl = w.of(value_of(edge_of(b, false)));
               wh = w.of(value_of(edge_of(b, true)));
@@ -332,12 +538,9 @@ struct Sampler {
           high[k] = sum_high += wh * count[k];
           mid[k] = sum_mid += 0.5 * (wl + wh) * count[k];
         }
-        const double before_low = scan(sum_low, sh.warp_sums[0]) - sum_low, before_high = scan(sum_high, sh.warp_sums[0]) - sum_high,
-                     before_mid = scan(sum_mid, sh.warp_sums[0]) - sum_mid;
-        unsigned int mine = 0;
-#pragma unroll
-        for (int k = 0; k < BINS_PER_THREAD; ++k) mine += count[k];
-        unsigned int upto = scan(mine, sh.warp_counts) - mine;
+        const double before_low = scan(sum_low, sh.sums[0]) - sum_low, before_high = scan(sum_high, sh.sums[0]) - sum_high,
+                     before_mid = scan(sum_mid, sh.sums[0]) - sum_mid;
+        unsigned int upto = scan(mine, sh.counts) - mine;
         if (threadIdx.x == 0) sh.found[0] = 0;
         __syncthreads();
         // bins with tokens only: the first ones whose running weight reaches the target
@@ -345,87 +548,72 @@ struct Sampler {
         for (int k = 0; k < BINS_PER_THREAD; ++k) {
           upto += count[k];
           if (count[k]) atomicMax(&sh.found[0], (unsigned int)(threadIdx.x * BINS_PER_THREAD + k));
-          b1 += __syncthreads_count(upto == 0 || mass + before_high + high[k] < target);
+          b1 += __syncthreads_count(upto == 0 || mass + before_high + high[k] < target_low);
           m += __syncthreads_count(upto == 0 || mass + before_mid + mid[k] < target);
-          b2 += __syncthreads_count(upto == 0 || mass + before_low + low[k] < target);
+          b2 += __syncthreads_count(upto == 0 || mass + before_low + low[k] < target_high);
         }
         if (first && b1 >= BINS) return NONE;
         const unsigned int last = sh.found[0];
         if (b2 > last) b2 = last;
         if (b1 > b2) b1 = b2;
         m = m < b1 ? b1 : m > b2 ? b2 : m;
-#pragma unroll
-        for (int k = 0; k < BINS_PER_THREAD; ++k) {
-          if (threadIdx.x * BINS_PER_THREAD + k == m) sh.found[2] = count[k];
-          if (threadIdx.x * BINS_PER_THREAD + k == b2) sh.found[3] = upto - (k + 1 < BINS_PER_THREAD ? count[BINS_PER_THREAD - 1] : 0);
-        }
         __syncthreads();
+        if (threadIdx.x == 0) sh.found[2] = sh.bins[buffer][m];
       }
-      if (first) {
-        const unsigned int all = BY_COUNT ? sh.found[1] + sh.found[2] : sh.found[3];
-        if (all <= LIST) {
-          each([&](unsigned int i, float f) {
-            if (w.bin(f) <= b2) append(search, f, i);
-          });
-          everyone();
-          gathered = all;
-          return GATHERED;
-        }
-      }
+      for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) sh.bins[next][i] = 0;
+      if (threadIdx.x == 0) sh.listed = 0;
+      __syncthreads();
       const unsigned int n = sh.found[2], key_lo = edge_of(m, false), key_hi = without_minus_zero(edge_of(m, true));
-      if constexpr (BY_COUNT) above += sh.found[1];
+      if constexpr (BY_COUNT) goal -= above;  // of the bin's
       const bool one = key_lo == key_hi, listed = !one && n <= LIST;
-      const unsigned int width = key_hi - key_lo;
       unsigned int new_shift = 0;
-      while (width >> new_shift >= BINS) ++new_shift;
-      __syncthreads();  // the bins are zeroed, sh.found is read
-      double s1 = 0.0, s2 = 0.0;
-      if (!BY_COUNT || !one) {
-        const float least_in = value_of(key_lo), most_in = value_of(key_hi);
-        if (!one)
-          each([&](unsigned int i, float f) {
-            if (!(f >= least_in && f <= most_in)) return;
-            if (listed) append(search, f, i);
-            else atomicAdd(&sh.bins[next][(key_hi - key_of(f)) >> new_shift], 1u);
-          });
-        if constexpr (!BY_COUNT)
-          each_vector([&](unsigned int, const float (&f)[N]) {
-            double x[N];
+      while ((key_hi - key_lo) >> new_shift >= BINS) ++new_shift;
+      double s1 = 0.0, s2 = 0.0;  // the weight above the bin, and up to its end
+      const float least_in = value_of(key_lo), most_in = value_of(key_hi);
+      if (!BY_COUNT || !one)
+        each([&](unsigned int i, const float (&f)[M]) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) x[j] = w.of(f[j]);
+          for (int j = 0; j < M; ++j)
+            if (!one && f[j] >= least_in && f[j] <= most_in) {
+              if (listed) append(f[j], i + j);
+              else atomicAdd(&sh.bins[next][(key_hi - key_of(f[j])) >> new_shift], 1u);
+            }
+          if constexpr (!BY_COUNT) {
+            double x[M];
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
+            for (int j = 0; j < M; ++j) x[j] = w.of(f[j]);
+#pragma unroll
+            for (int j = 0; j < M; ++j) {
               s2 += f[j] >= least_in ? x[j] : 0.0;
               s1 += f[j] > most_in ? x[j] : 0.0;
             }
-          });
-        if constexpr (!BY_COUNT) sum2(s1, s2);
-        else everyone();
-      }
+          }
+        });
       if constexpr (!BY_COUNT) {
+        s1 = block_sum(s1, 0);
+        s2 = block_sum(s2, 1);
+        if ((s1 >= target_low && s1 < target_high) || (s2 >= target_low && s2 < target_high)) return UNSURE;
         const bool left = s1 >= target && m > b1, right = s2 < target && m < b2;
         if (left || right) {
           // the estimate was beside it: the bins between, counted anew
           const unsigned int old_lo = edge_of(b2, false), old_hi = edge_of(b1, true);
           lo = left ? key_hi + 1 : old_lo;
           hi = without_minus_zero(left ? old_hi : key_lo - 1);
-          mass = left ? 0.0 : s2;
           shift = 0;
           while ((hi - lo) >> shift >= BINS) ++shift;
-          if (listed && threadIdx.x == 0 && rank == 0) sh.gathered_n[search] = 0;
           for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) sh.bins[next][i] = 0;
-          double above_window = 0.0, none = 0.0;
           __syncthreads();
-          each([&](unsigned int i, float f) {
-            const unsigned int key = key_of(f);
-            if (key >= lo && key <= hi) atomicAdd(&sh.bins[next][(hi - key) >> shift], 1u);
+          const float above_this = value_of(hi);
+          double heavier = 0.0;
+          each([&](unsigned int, const float (&f)[M]) {
+            heavier += weigh(f, [&](float g) { return g > above_this; });
+#pragma unroll
+            for (int j = 0; j < M; ++j) {
+              const unsigned int key = key_of(f[j]);
+              if (key >= lo && key <= hi) atomicAdd(&sh.bins[next][(hi - key) >> shift], 1u);
+            }
           });
-          if (left) {
-            const float above_this = value_of(hi);
-            each_vector([&](unsigned int, const float (&f)[N]) { above_window += weigh(f, [&](float g) { return g > above_this; }); });
-            sum2(above_window, none);
-            mass = above_window;
-          }
+          mass = block_sum(heavier, 0);
           first = false;
           buffer = next;
           continue;
@@ -435,17 +623,15 @@ struct Sampler {
         cut.value = value_of(key_lo);
         cut.equal = n;
         if constexpr (BY_COUNT) {
-          cut.ties = goal - above;
+          cut.ties = goal;
         } else {
-          const double more = ceil((target - s1) / w.of(cut.value));
+          const double each_one = w.of(cut.value), more = ceil((target_low - s1) / each_one);
+          if (ceil((target_high - s1) / each_one) != more) return UNSURE;
           cut.ties = more < 1.0 ? 1u : more > (double)n ? n : (unsigned int)more;
         }
         return CUT;
       }
-      if (listed) {
-        order_list(n, BY_COUNT ? (double)(goal - above) : target, s1, BY_COUNT, cut);
-        return CUT;
-      }
+      if (listed) return order_list<BY_COUNT>(n, goal, target_low, target_high, s1, cut) ? CUT : UNSURE;
       lo = key_lo;
       hi = key_hi;
       shift = new_shift;
@@ -455,366 +641,605 @@ struct Sampler {
     }
   }
 
-  // A token into the first block's list.
-  __device__ __forceinline__ void append(int search, float f, unsigned int i) {
-    unsigned int* counter = ranks > 1 ? cluster.map_shared_rank(&sh.gathered_n[search], 0) : &sh.gathered_n[search];
-    unsigned long long* list = ranks > 1 ? cluster.map_shared_rank(sh.gathered, 0) : sh.gathered;
-    list[atomicAdd(counter, 1u) % LIST] = (unsigned long long)~key_of(f) << 32 | i;
+  // A token into the list.
+  __device__ __forceinline__ void append(float f, unsigned int place) {
+    sh.list[atomicAdd(&sh.listed, 1u) % LIST] = (unsigned long long)~key_of(f) << 32 | place;
   }
-  // The n gathered tokens in `ordered`: by falling logit, equal ones by number.
+  // The n listed tokens in `ordered`: by falling logit, equal ones by place.
   __device__ __forceinline__ void order(unsigned int n) {
-    const unsigned long long* list = ranks > 1 ? cluster.map_shared_rank(sh.gathered, 0) : sh.gathered;
-    const unsigned int t = threadIdx.x;
-    unsigned long long mine = ~0ull;
-    if (t < n) sh.own[t] = mine = list[t];
     __syncthreads();
+    const unsigned int t = threadIdx.x;
     if (t < n) {
+      const unsigned long long mine = sh.list[t];
       unsigned int place = 0;
-      for (unsigned int j = 0; j < n; ++j) place += sh.own[j] < mine;
+#pragma unroll 8
+      for (unsigned int j = 0; j < n; ++j) place += sh.list[j] < mine;
       sh.ordered[place] = mine;
     }
     __syncthreads();
   }
-  // The token from n gathered ones that hold all that are kept, by the first block. mass: of all tokens that top_p counts, where it is not that of the first top_k.
-  __device__ __forceinline__ void choose(unsigned int r, unsigned int n, unsigned int top_k, bool by_k, double mass, bool by_p, double top_p, double least, double u) {
-    order(n);
-    const unsigned int t = threadIdx.x, number = t < n ? (unsigned int)sh.ordered[t] : 0xFFFFFFFFu;
-    const float logit = t < n ? value_of(~(unsigned int)(sh.ordered[t] >> 32)) : -INFINITY;
-    double x = t < n && (!by_k || t < top_k) ? w.of(logit) : 0.0;
-    if (by_p) {
-      const double upto = scan(x, sh.warp_sums[0]);
-      if (by_k) {
-        mass = 0.0;
-        for (int i = 0; i < SAMPLE_WARPS; ++i) mass += sh.warp_sums[0][i];
-      }
-      if (t > 0 && !(upto - x < top_p * mass)) x = 0.0;
-    }
-    if (t > 0 && !(x >= least)) x = 0.0;
-    // kept tokens by number
-    __syncthreads();
-    sh.own[t] = (unsigned long long)number << 32 | t;
-    const unsigned int kept = __syncthreads_count(x > 0.0);  // a prefix
-    double* sums = reinterpret_cast<double*>(sh.gathered);
-    if (t < kept) {
-      unsigned int place = 0;
-      for (unsigned int j = 0; j < kept; ++j) place += sh.own[j] < sh.own[t];
-      sums[place] = x;
-      sh.ordered[place] = (unsigned long long)__float_as_uint(logit) << 32 | number;
-    }
-    __syncthreads();
-    const double upto = scan(t < kept ? sums[t] : 0.0, sh.warp_sums[0]);
-    double total = 0.0;
-    for (int i = 0; i < SAMPLE_WARPS; ++i) total += sh.warp_sums[0][i];
-    const double target = target_of(u, total);
-    unsigned int at = __syncthreads_count(t < kept && !(upto > target));
-    if (at >= kept) at = kept - 1;
-    if (t == 0) write(r, (unsigned int)sh.ordered[at], (float)(w.exponent(__uint_as_float((unsigned int)(sh.ordered[at] >> 32))) - log(total)));
-  }
-  __device__ __forceinline__ static double target_of(double u, double total) { return u >= 0.0 ? u * total : u < 0.0 ? 0.0 : INFINITY; }  // NaN: the end
-
-  // The cut among the n gathered tokens.
-  __device__ __forceinline__ void order_list(unsigned int n, double target, double before, bool by_count, Cut& cut) {
+  // The cut among the n listed tokens: after `count` of them, or where `before` and their weight reach the target; false where that is not sure.
+  template <bool BY_COUNT>
+  __device__ __forceinline__ bool order_list(unsigned int n, unsigned int count, double target_low, double target_high, double before, Cut& cut) {
     order(n);
     const unsigned int t = threadIdx.x;
     const unsigned int key = t < n ? ~(unsigned int)(sh.ordered[t] >> 32) : 0;
-    unsigned int keep;
-    if (by_count) {
-      keep = (unsigned int)target;
-    } else {
+    unsigned int keep = count;
+    if constexpr (!BY_COUNT) {
       const double x = t < n ? w.of(value_of(key)) : 0.0;
-      const double upto = scan(x, sh.warp_sums[0]);
-      keep = __syncthreads_count(t < n && before + (upto - x) < target);
+      const double at = before + (scan(x, sh.sums[0]) - x);
+      keep = __syncthreads_count(t < n && at < target_low);
+      if ((unsigned int)__syncthreads_count(t < n && at < target_high) != keep) return false;
       if (keep == 0) keep = 1;
     }
     const unsigned int last = ~(unsigned int)(sh.ordered[keep - 1] >> 32);
     cut.value = value_of(last);
     cut.ties = __syncthreads_count(t < keep && key == last);
     cut.equal = __syncthreads_count(t < n && key == last);
+    return true;
   }
 
-  __device__ __forceinline__ void write(unsigned int r, long long token, float lp) {
+  // One thread's.
+  __device__ __forceinline__ void write(long long token, float lp) {
     if (a.wide) static_cast<long long*>(a.tokens)[r] = token;
     else static_cast<int*>(a.tokens)[r] = (int)token;
     if (a.logprob) a.logprob[r] = lp;
   }
+  __device__ __forceinline__ void write(unsigned int token, float logit, double total) { write(token, (float)(w.exponent(logit) - log(total))); }
 
-  __device__ void run(unsigned int r) {
-    float t = a.row_temperature ? a.row_temperature[r] : a.temperature, top_p = a.row_top_p ? a.row_top_p[r] : a.top_p,
-          min_p = a.row_min_p ? a.row_min_p[r] : a.min_p;
-    const int top_k = a.row_top_k ? a.row_top_k[r] : a.top_k;
-    const double u = a.u[r];
-    // the part into shared memory, and the largest logit
-    float top = -INFINITY;
-    for (unsigned int i = w0 + lane * N; i < w1; i += TILE * 4) {
-      float f[4][N];
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (i + k * TILE < w1) load(i + k * TILE, f[k]);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (i + k * TILE >= w1) break;
-        if constexpr (HELD) const_cast<uint4*>(held)[(i + k * TILE - part0) / N] = Elems<T, 16>::put(f[k]);
-#pragma unroll
-        for (int j = 0; j < N; ++j) top = fmaxf(top, f[k][j]);
-      }
+  // The row's whole weight in fp64.
+  __device__ double whole_weight() {
+    double s = 0.0;
+    for (unsigned int i = threadIdx.x * M; i < row.end; i += SAMPLE_THREADS * M) {
+      float f[M];
+      row.load(i, f);
+      s += weigh(f, [](float) { return true; });
     }
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    if (lane == 0) sh.warp_sums[0][warp] = top;
-    for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) sh.bins[0][i] = 0;
-    if (threadIdx.x < 2) sh.gathered_n[threadIdx.x] = 0;
-    if (threadIdx.x < STEPS) sh.powers[threadIdx.x] = exp2(threadIdx.x / (double)STEPS);
-    w.powers = sh.powers;
+    return block_sum(s, 1);
+  }
+
+  // The token from the n listed ones, which hold all that are kept. mass: of all tokens that top_p counts, where it is not that of the first top_k; it may be
+  // off by SLACK.
+  __device__ __forceinline__ void choose(unsigned int n, const SampleRow& ask, double mass, double u) {
+    order(n);
+    const unsigned int t = threadIdx.x, number = t < n ? (unsigned int)sh.ordered[t] : 0xFFFFFFFFu;
+    const float logit = t < n ? value_of(~(unsigned int)(sh.ordered[t] >> 32)) : -INFINITY;
+    double x = t < n && (!ask.by_k || t < (unsigned int)ask.top_k) ? w.of(logit) : 0.0;
+    if (ask.by_p) {
+      const double before = scan(x, sh.sums[0]) - x, p = ask.top_p;
+      if (ask.by_k) mass = warps_sum(0);
+      else if (__syncthreads_or(t < n && before >= p * mass * (1.0 - SLACK) && before < p * mass * (1.0 + SLACK))) mass = whole_weight();
+      if (t > 0 && !(before < p * mass)) x = 0.0;
+    }
+    if (ask.by_m && t > 0 && !(x >= (double)ask.min_p)) x = 0.0;
+    // kept tokens by number
+    sh.own[t] = (unsigned long long)number << 32 | t;
+    const unsigned int kept = __syncthreads_count(x > 0.0);  // a prefix
+    double* sums = reinterpret_cast<double*>(sh.list);
+    if (t < kept) {
+      const unsigned long long mine = sh.own[t];
+      unsigned int place = 0;
+#pragma unroll 8
+      for (unsigned int j = 0; j < kept; ++j) place += sh.own[j] < mine;
+      sums[place] = x;
+      sh.ordered[place] = (unsigned long long)__float_as_uint(logit) << 32 | number;
+    }
     __syncthreads();
-    for (int i = 0; i < SAMPLE_WARPS; ++i) top = fmaxf(top, (float)sh.warp_sums[0][i]);
-    give(top, 0.0);
-    for (int i = 0; i < ranks; ++i) top = fmaxf(top, (float)taken(i, 0));
-    if (!(top > -INFINITY)) {
-      if (rank == 0 && threadIdx.x == 0) write(r, -1, 0.f);
-      return;
+    const double upto = scan(t < kept ? sums[t] : 0.0, sh.sums[0]), total = warps_sum(0);
+    const double target = target_of(u, total);
+    unsigned int at = __syncthreads_count(t < kept && !(upto > target));
+    if (at >= kept) at = kept - 1;
+    if (t == 0) write((unsigned int)sh.ordered[at], __uint_as_float((unsigned int)(sh.ordered[at] >> 32)), total);
+  }
+
+  // From the tiles' weights, relative to 2^n: their sum, and without a limit (choose) the token. False where fp32 leaves it open.
+  __device__ __forceinline__ bool from_tiles(const SampleRow& ask, bool token, double u, double& total) {
+    const TileStat* stats = a.stats + r * a.tiles;
+    FastWeights top;
+    top.set(w.top, ask.t);
+    // a thread's tiles are neighbours
+    const unsigned int each_has = (a.tiles + SAMPLE_THREADS - 1) / SAMPLE_THREADS, t0 = min(threadIdx.x * each_has, a.tiles), t1 = min(t0 + each_has, a.tiles);
+    double sum = 0.0;
+    bool usable = top.usable;
+    for (unsigned int k = t0; k < t1; ++k) {
+      const TileStat s = stats[k];
+      if (s.weight < 0.0) usable = false;
+      if (s.weight > 0.0) sum += s.weight * top.unit(s.largest, ask.t);
     }
-    if (!(t > 0.f) || top_k == 1 || top_p <= 0.f || min_p > 1.f) {
-      unsigned int at = 0xFFFFFFFFu;
-      each([&](unsigned int i, float f) {
-        if (f == top && i < at) at = i;
-      });
-      at = __reduce_min_sync(0xFFFFFFFFu, at);
-      if (lane == 0) sh.warp_counts[warp] = at;
-      __syncthreads();
-      for (int i = 0; i < SAMPLE_WARPS; ++i) at = min(at, sh.warp_counts[i]);
-      give(at, 0.0);
-      for (int i = 0; i < ranks; ++i) at = min(at, (unsigned int)taken(i, 0));
-      if (rank == 0 && threadIdx.x == 0) write(r, at, 0.f);
-      return;
+    if (!__syncthreads_and(usable)) return false;
+    const double upto = scan(sum, sh.sums[0]);
+    total = warps_sum(0);
+    const double to_top = top.to_top(w);
+    if (!token) {
+      total *= to_top;
+      return true;
     }
-    t = fminf(t, 3.4028235e38f);
-    w.set(top, t);
-    Cut cut{-INFINITY, 0, 0};
-    const bool by_k = top_k > 0 && (unsigned int)top_k < a.vocab, by_p = top_p < 1.f;
-    if (by_k || by_p) {
-      double all = 0.0, none = 0.0;
-      each([&](unsigned int, float f) {
-        const unsigned int b = w.bin(f);
-        if (b < BINS - 1) atomicAdd(&sh.bins[0][b], 1u);
-      });
-      if (!by_k)
-        each_vector([&](unsigned int, const float (&f)[N]) { all += weigh(f, [](float) { return true; }); });
-      sum2(all, none);  // of all blocks: the bins are counted
-      unsigned int n = 0;
-      if (by_k) {
-        if (find<true>(top_k, 0, cut, n) == GATHERED) {
-          if (rank == 0) choose(r, n, top_k, true, 0.0, by_p, top_p, min_p, u);
-          return;
+    const double target = target_of(u, total);
+    // the thread, the tile, and the warp of that thread goes through the tile
+    if (threadIdx.x == 0) sh.found[0] = 0, sh.found[1] = SAMPLE_THREADS;
+    __syncthreads();
+    if (sum > 0.0 && upto > target && upto - sum <= target) atomicMin(&sh.found[1], threadIdx.x);
+    __syncthreads();
+    const unsigned int owner = sh.found[1];
+    if (owner >> 5 == (unsigned int)warp && owner < SAMPLE_THREADS) {
+      const int from = owner & 31;
+      double start = __shfl_sync(0xFFFFFFFFu, upto - sum, from), weight = 0.0;
+      const unsigned int k0 = __shfl_sync(0xFFFFFFFFu, t0, from), k1 = __shfl_sync(0xFFFFFFFFu, t1, from);
+      for (unsigned int k = k0; k < k1; ++k) {
+        const TileStat s = stats[k];
+        if (!(s.weight > 0.0)) continue;
+        const double scale = top.unit(s.largest, ask.t);
+        if (k + 1 < k1 && start + s.weight * scale <= target) {
+          start += s.weight * scale;
+          continue;
         }
-        if (by_p) {
-          all = none = 0.0;
-          each_vector([&](unsigned int, const float (&f)[N]) { all += weigh(f, [&](float g) { return g > cut.value; }); });
-          sum2(all, none);
-          if (cut.ties) all += cut.ties * w.of(cut.value);
+        constexpr int N = 16 / (int)sizeof(T);
+        FastWeights tile;
+        tile.set(s.largest, ask.t);
+        unsigned int place = 0;
+        float logit = w.top;
+        double before = start / scale;  // an exact quotient by a power of two
+        const double goal = target / scale;
+        const bool found = walk<N, float>(lane, k * TILE, k * TILE + TILE, before, goal, place, logit, weight, [&](unsigned int i, float (&f)[N], float (&x)[N]) {
+          row.load(i, f);
+#pragma unroll
+          for (int j = 0; j < N; ++j) x[j] = tile.of(f[j]);
+        });
+        if (found && goal - before > SLACK * goal && before + weight - goal > SLACK * goal && lane == 0) {
+          write(place - row.shift, logit, total * to_top);
+          sh.found[0] = 1;
+        }
+        break;
+      }
+    }
+    __syncthreads();
+    return sh.found[0];
+  }
+
+  // The tokens of at least `floor`: how many there are, and in `own` how many of them the warp's tiles have, which are neighbours. Up to LIST of them are listed, with their
+  // numbers for places.
+  __device__ __forceinline__ unsigned int gather(unsigned int& own) {
+    constexpr int N = 16 / (int)sizeof(T);
+    const TileStat* stats = a.stats + r * a.tiles;
+    const float* most = a.lane_most ? a.lane_most + r * a.tiles * 32 : nullptr;
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+    own = 0;
+    const unsigned int t0 = a.tiles * warp / SAMPLE_WARPS, t1 = a.tiles * (warp + 1) / SAMPLE_WARPS;
+    for (unsigned int k = t0; k < t1; ++k) {
+      if (!(most ? most[k * 32 + lane] >= floor : stats[k].largest >= floor)) continue;
+      const bool room = *(volatile unsigned int*)&sh.listed < LIST;
+#pragma unroll
+      for (int v = 0; v < PER_LANE / N; ++v) {
+        const unsigned int i = k * TILE + (v * 32 + lane) * N;
+        float f[N];
+        row.load(i, f);
+#pragma unroll
+        for (int j = 0; j < N; ++j) own += f[j] >= floor;
+        if (room) {
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+            if (f[j] >= floor) {
+              const unsigned int at = atomicAdd(&sh.listed, 1u);
+              if (at < LIST) sh.list[at] = (unsigned long long)~key_of(f[j]) << 32 | (i + j - row.shift);
+            }
         }
       }
-      if (by_p) {
-        Cut c;
-        const Found found = find<false>((double)top_p * all, 1, c, n);
-        if (found == GATHERED) {
-          if (rank == 0) choose(r, n, 0, false, all, true, top_p, min_p, u);
-          return;
-        }
-        if (found == CUT && (c.value > cut.value || (c.value == cut.value && c.ties < cut.ties))) cut = c;
+    }
+    own = __reduce_add_sync(0xFFFFFFFFu, own);
+    if (lane == 0) sh.counts[warp] = own;
+    __syncthreads();
+    return __reduce_add_sync(0xFFFFFFFFu, lane < SAMPLE_WARPS ? sh.counts[lane] : 0u);
+  }
+  // All of them into shared memory by number.
+  __device__ __forceinline__ void store(unsigned int n, unsigned int own) {
+    constexpr int N = 16 / (int)sizeof(T);
+    const TileStat* stats = a.stats + r * a.tiles;
+    const unsigned int upto = scan(lane == 0 ? own : 0u, sh.counts);
+    unsigned int at = __shfl_sync(0xFFFFFFFFu, upto, 0) - own;
+    const unsigned int t0 = a.tiles * warp / SAMPLE_WARPS, t1 = a.tiles * (warp + 1) / SAMPLE_WARPS;
+    for (unsigned int k = t0; k < t1; ++k) {
+      if (!(stats[k].largest >= floor)) continue;
+#pragma unroll
+      for (int v = 0; v < PER_LANE / N; ++v) {
+        const unsigned int i = k * TILE + (v * 32 + lane) * N;
+        float f[N];
+        row.load(i, f);
+        unsigned int mine = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) mine += f[j] >= floor;
+        const unsigned int before = lanes_before(mine);
+        unsigned int to = at + before;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (f[j] >= floor) {
+            sh.stored[to] = f[j];
+            sh.number[to++] = i + j - row.shift;
+          }
+        at += __shfl_sync(0xFFFFFFFFu, before + mine, 31);
       }
     }
-    // tokens at the cut: how many of them in blocks and warps before this one
-    unsigned int ties = 0;  // of this warp's
-    const bool some = cut.ties < cut.equal;
+    __syncthreads();
+    for (unsigned int i = n + threadIdx.x; i < (n + 32 * M - 1) / (32 * M) * (32 * M); i += SAMPLE_THREADS) sh.stored[i] = -INFINITY;
+    __syncthreads();
+  }
+
+  // The token by sums over the kept ones in fp64, by places.
+  __device__ __forceinline__ void by_sums(const Cut& cut, double least, double u) {
+    unsigned int ties = 0;  // of this warp's at the cut
     if (cut.ties) {
       ties = 0xFFFFFFFFu;
-      if (some) {
+      if (cut.ties < cut.equal) {
         unsigned int mine = 0;
-        each([&](unsigned int i, float f) { mine += f == cut.value; });
+        each([&](unsigned int, const float (&f)[M]) {
+#pragma unroll
+          for (int j = 0; j < M; ++j) mine += f[j] == cut.value;
+        });
         mine = __reduce_add_sync(0xFFFFFFFFu, mine);
-        __syncthreads();
-        if (lane == 0) sh.warp_counts[warp] = mine;
-        __syncthreads();
-        unsigned int block = 0, before = 0;
-        for (int i = 0; i < SAMPLE_WARPS; ++i) {
-          if (i < warp) before += sh.warp_counts[i];
-          block += sh.warp_counts[i];
-        }
-        give(block, 0.0);
-        for (int i = 0; i < rank; ++i) before += (unsigned int)taken(i, 0);
+        const unsigned int before = __shfl_sync(0xFFFFFFFFu, scan(lane == 0 ? mine : 0u, sh.counts), 0) - mine;
         ties = before >= cut.ties ? 0 : cut.ties - before;
         if (ties >= mine) ties = 0xFFFFFFFFu;  // all of them
       }
     }
     const bool in_part = ties && ties != 0xFFFFFFFFu;
-    const double least = min_p > 0.f ? min_p : 0.0;
-    // weights of a lane's N tokens of the tile at i, 0 for what is not kept. seen: tokens at the cut in the warp's tiles before.
-    auto kept = [&](unsigned int i, unsigned int& seen, float (&f)[N], double (&x)[N]) {
+    unsigned int seen = 0;  // tokens at the cut in the warp's vectors before
+    auto kept = [&](unsigned int i, float (&f)[M], double (&x)[M]) {
       unsigned int order = 0;
-      if (i < w1) {
-        fetch(i, f);
-      } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) f[j] = -INFINITY;
-      }
+      fetch(i, f);
       if (in_part) {
         unsigned int mine = 0;
 #pragma unroll
-        for (int j = 0; j < N; ++j) mine += f[j] == cut.value;
-        order = mine;
-        for (int o = 1; o < 32; o <<= 1) {
-          const unsigned int below = __shfl_up_sync(0xFFFFFFFFu, order, o);
-          if (lane >= o) order += below;
-        }
-        const unsigned int tile = __shfl_sync(0xFFFFFFFFu, order, 31);
-        order += seen - mine;
-        seen += tile;
+        for (int j = 0; j < M; ++j) mine += f[j] == cut.value;
+        order = lanes_before(mine);
+        const unsigned int all = __shfl_sync(0xFFFFFFFFu, order + mine, 31);
+        order += seen;
+        seen += all;
       }
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[j] = w.of(f[j]);
+      for (int j = 0; j < M; ++j) x[j] = w.of(f[j]);
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
+      for (int j = 0; j < M; ++j) {
         const bool equal = f[j] == cut.value && ties, keep = (f[j] > cut.value || (equal && order < ties)) && x[j] >= least;
         order += equal;
         x[j] = keep ? x[j] : 0.0;
       }
     };
     double sum = 0.0;
-    unsigned int seen = 0;
-    for (unsigned int i = w0 + lane * N; i - lane * N < w1; i += TILE) {
-      float f[N];
-      double x[N];
-      kept(i, seen, f, x);
+    for (unsigned int i = begin + lane * M; i - lane * M < end; i += 32 * M) {
+      float f[M];
+      double x[M];
+      kept(i, f, x);
 #pragma unroll
-      for (int j = 0; j < N; ++j) sum += x[j];
+      for (int j = 0; j < M; ++j) sum += x[j];
     }
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-    __syncthreads();
-    if (lane == 0) sh.warp_sums[1][warp] = sum;
-    __syncthreads();
-    double block = 0.0;
-    for (int i = 0; i < SAMPLE_WARPS; ++i) block += sh.warp_sums[1][i];
-    give(block, 0.0);
-    double total = 0.0;
-    for (int i = 0; i < ranks; ++i) total += taken(i, 0);
-    // which block, and which warp of it; the last one with any weight where rounding, or u, leaves none
-    const double target = target_of(u, total);
-    int where = -1;
-    double upto = 0.0, start = 0.0;
-    bool crossed = false;
-    for (int i = 0; i < ranks && !crossed; ++i) {
-      const double s = taken(i, 0);
+    const double total = block_sum(sum, 1), target = target_of(u, total);
+    // the warp in which it is crossed, or the last one with any weight
+    double start = 0.0, upto = 0.0, weight;
+    int where = 0;
+    for (int i = 0; i < SAMPLE_WARPS; ++i) {
+      const double s = sh.sums[1][i];
       if (s > 0.0) {
         where = i;
         start = upto;
         upto += s;
-        crossed = upto > target;
+        if (upto > target) break;
       }
     }
-    if (where != rank) return;
-    int in_warp = -1;
-    upto = start;
-    bool here = false;
-    for (int i = 0; i < SAMPLE_WARPS && !here; ++i) {
-      const double s = sh.warp_sums[1][i];
-      if (s > 0.0) {
-        in_warp = i;
-        start = upto;
-        upto += s;
-        here = upto > target;
-      }
-    }
-    if (in_warp != warp) return;
-    unsigned int token = 0xFFFFFFFFu;
-    float logit = 0.f;
+    if (where != warp) return;
+    unsigned int place = 0;
+    float logit = w.top;
     seen = 0;
-    for (unsigned int i = w0 + lane * N; i - lane * N < w1; i += TILE) {
-      float f[N];
-      double x[N];
-      kept(i, seen, f, x);
-      double mine = 0.0;
-#pragma unroll
-      for (int j = 0; j < N; ++j) mine += x[j];
-      double run = mine;
-      for (int o = 1; o < 32; o <<= 1) {
-        const double below = __shfl_up_sync(0xFFFFFFFFu, run, o);
-        if (lane >= o) run += below;
-      }
-      const unsigned int past = __ballot_sync(0xFFFFFFFFu, mine > 0.0 && start + run > target);
-      const unsigned int any = __ballot_sync(0xFFFFFFFFu, mine > 0.0);
-      if (any) {
-        // in this tile, or so far the last token with any weight
-        const int who = past ? __ffs(past) - 1 : 31 - __clz(any);
-        unsigned int at = 0;
-        float l = 0.f;
-        double s = start + (run - mine);
-        bool done = false;
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          if (x[j] > 0.0 && !done) {
-            at = i + j;
-            l = f[j];
-            s += x[j];
-            done = past && s > target;
-          }
-        }
-        token = __shfl_sync(0xFFFFFFFFu, at, who);
-        logit = __shfl_sync(0xFFFFFFFFu, l, who);
-      }
-      if (past) break;
-      start += __shfl_sync(0xFFFFFFFFu, run, 31);
+    walk<M, double>(lane, begin, end, start, target, place, logit, weight, kept);
+    if (lane == 0) write(number_of(place), logit, total);
+  }
+
+  // The warps' shares of `all` places.
+  __device__ __forceinline__ void share(unsigned int all) {
+    constexpr unsigned int PIECE = 32 * M;
+    const unsigned int pieces = (all + PIECE - 1) / PIECE;
+    begin = pieces * warp / SAMPLE_WARPS * PIECE;
+    end = pieces * (warp + 1) / SAMPLE_WARPS * PIECE;
+  }
+
+  __device__ __forceinline__ void run() {
+    const SampleRow ask(a, r);
+    const TileStat* stats = a.stats + r * a.tiles;
+    const double u = a.u[r];
+    if (threadIdx.x < STEPS) sh.powers[threadIdx.x] = exp2(threadIdx.x / (double)STEPS);
+    w.powers = sh.powers;
+    float top = -INFINITY;
+    for (unsigned int k = threadIdx.x; k < a.tiles; k += SAMPLE_THREADS) top = fmaxf(top, stats[k].largest);
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    if (lane == 0) sh.sums[0][warp] = top;
+    __syncthreads();
+    for (int i = 0; i < SAMPLE_WARPS; ++i) top = fmaxf(top, (float)sh.sums[0][i]);
+    if (!(top > -INFINITY)) {
+      if (threadIdx.x == 0) write(-1, 0.f);
+      return;
     }
-    if (lane == 0) write(r, token, (float)(w.exponent(logit) - log(total)));
+    if (ask.greedy) {
+      // the first tile that has the largest, and in it the first place
+      unsigned int tile = 0xFFFFFFFFu, at;
+      for (unsigned int k = threadIdx.x; k < a.tiles; k += SAMPLE_THREADS)
+        if (stats[k].largest == top) {
+          tile = k;
+          break;
+        }
+      tile = __reduce_min_sync(0xFFFFFFFFu, tile);
+      if (lane == 0) sh.counts[warp] = tile;
+      __syncthreads();
+      for (int i = 0; i < SAMPLE_WARPS; ++i) tile = min(tile, sh.counts[i]);
+      if (warp) return;
+      at = first_of(row, tile, top, lane);
+      if (lane == 0) write(at, 0.f);
+      return;
+    }
+    w.set(top, ask.t);
+    stored = false;
+    floor = -3.4028234663852886e38f;
+    Cut cut{-INFINITY, 0, 0};
+    double all = 0.0, slack = SLACK;
+    if (!ask.by_k && !ask.by_p && !ask.by_m) {
+      if (from_tiles(ask, true, u, all)) return;
+      share(row.end);
+      by_sums(cut, 0.0, u);
+      return;
+    }
+    // what is certainly not kept
+    double lowest = -INFINITY;  // of logits, as a difference to the largest
+    if (ask.by_k) {
+      // as many lanes as top_k have a logit in the bins up to this one
+      for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) sh.bins[0][i] = 0;
+      __syncthreads();
+      w.set_bins(REACH);
+      const float* most = a.lane_most + r * a.tiles * 32;
+      for (unsigned int i = threadIdx.x; i < a.tiles * 32; i += SAMPLE_THREADS)
+        if (most[i] > -INFINITY) atomicAdd(&sh.bins[0][w.bin(most[i])], 1u);
+      __syncthreads();
+      const unsigned int bin = reaches(0, ask.top_k);
+      if (bin < BINS - 1) lowest = -(bin + 1.01) * 2.0 / (double)w.per_bin;
+    } else if (ask.by_p) {
+      if (!from_tiles(ask, false, u, all)) {
+        all = whole_weight();
+        slack = 0.0;
+      }
+      lowest = (log((1.0 - (double)ask.top_p) * all * (1.0 - SLACK) / a.vocab) - 1e-3) * (double)ask.t;
+    }
+    if (ask.by_m && !(ask.by_k && ask.by_p)) lowest = fmax(lowest, (log((double)ask.min_p) - 1e-3) * (double)ask.t);  // top_p counts all of the first top_k
+    // rounded to fp32 it is no more than any logit that it is no more than
+    floor = top == INFINITY ? top : (float)fmax((double)top + lowest, -3.4028234663852886e38);
+    unsigned int own;
+    const unsigned int n = gather(own);
+    if (n <= LIST) {
+      choose(n, ask, all, u);
+      return;
+    }
+    stored = n <= STORED;
+    if (stored) store(n, own);
+    share(stored ? n : row.end);
+    if (ask.by_k || ask.by_p) {
+      w.set_bins(fmin(REACH, -lowest * w.inv_t * 1.01 + 1e-6));
+      for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) sh.bins[0][i] = 0;
+      __syncthreads();
+      each([&](unsigned int, const float (&f)[M]) {
+#pragma unroll
+        for (int j = 0; j < M; ++j) {
+          const unsigned int b = w.bin(f[j]);
+          if (b < BINS - 1) atomicAdd(&sh.bins[0][b], 1u);
+        }
+      });
+      if (ask.by_k) {
+        find<true>(ask.top_k, 0.0, cut);
+        if (ask.by_p) {
+          double s = 0.0;
+          each([&](unsigned int, const float (&f)[M]) { s += weigh(f, [&](float g) { return g > cut.value; }); });
+          all = block_sum(s, 0);
+          if (cut.ties) all += cut.ties * w.of(cut.value);
+          slack = 0.0;
+        }
+      }
+      if (ask.by_p) {
+        Cut c;
+        Found found = find<false>((double)ask.top_p * all, slack, c);
+        if (found == UNSURE) found = find<false>((double)ask.top_p * whole_weight(), 0.0, c);
+        if (found == CUT && (c.value > cut.value || (c.value == cut.value && c.ties < cut.ties))) cut = c;
+      }
+    }
+    by_sums(cut, ask.by_m ? (double)ask.min_p : 0.0, u);
   }
 };
 
-template <typename T, bool HELD>
-__global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleArgs a) {
-  __shared__ SampleShared sh;
-  extern __shared__ uint4 held[];
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const unsigned int r = blockIdx.x / ranks;
-  const unsigned int part0 = rank * a.part, per_warp = a.part / SAMPLE_WARPS;
-  Sampler<T, HELD> s{a, sh, cluster, reinterpret_cast<const T*>(a.logits + r * a.ld), held, part0};
-  s.warp = threadIdx.x >> 5;
-  s.lane = threadIdx.x & 31;
-  s.w0 = part0 + s.warp * per_warp;
-  s.w1 = s.w0 + per_warp;
-  if (s.w1 > a.vocab) s.w1 = s.w0 >= a.vocab ? s.w0 : s.w0 + (a.vocab - s.w0 + s.TILE - 1) / s.TILE * s.TILE;
-  s.ranks = ranks;
-  s.rank = rank;
-  s.turn = 0;
-  s.run(r);
-  if (ranks > 1) cluster.sync();  // the others may still read this block's shared memory
+// ------------------------------------------------------------------ calls without a limit: a warp per row
+
+constexpr int WHOLE_THREADS = 128;
+
+// EXACT = false: every row, by its tiles' weights in fp32; rows that these leave open are listed. EXACT = true: the listed ones, by weights in fp64.
+template <typename T, bool EXACT>
+__global__ void __launch_bounds__(WHOLE_THREADS) sample_whole_kernel(const SampleArgs a, size_t rows) {
+  constexpr int N = 16 / (int)sizeof(T);
+  __shared__ double powers[STEPS];
+  let_next_start();
+  if (threadIdx.x < STEPS) powers[threadIdx.x] = exp2(threadIdx.x / (double)STEPS);
+  __syncthreads();
+  after_previous();
+  const int lane = threadIdx.x & 31;
+  const size_t count = EXACT ? *a.open_count : rows;
+  for (size_t at = ((size_t)blockIdx.x * WHOLE_THREADS + threadIdx.x) >> 5; at < count; at += (size_t)gridDim.x * WHOLE_THREADS / 32) {
+    const size_t r = EXACT ? a.open[at] : at;
+    const SampleRow ask(a, r);
+    const RowView<T> row(a, r);
+    const TileStat* stats = a.stats + r * a.tiles;
+    auto write = [&](long long token, float lp) {
+      if (lane) return;
+      if (a.wide) static_cast<long long*>(a.tokens)[r] = token;
+      else static_cast<int*>(a.tokens)[r] = (int)token;
+      if (a.logprob) a.logprob[r] = lp;
+    };
+    // a lane's tiles are neighbours
+    const unsigned int each_has = (a.tiles + 31) / 32, t0 = min(lane * each_has, a.tiles), t1 = min(t0 + each_has, a.tiles);
+    float top = -INFINITY;
+    unsigned int first = 0xFFFFFFFFu;
+    for (unsigned int k = t0; k < t1; ++k)
+      if (stats[k].largest > top) {
+        top = stats[k].largest;
+        first = k;
+      }
+    const float own = top;
+    top = warp_max(top);
+    if (!(top > -INFINITY)) {
+      write(-1, 0.f);
+      continue;
+    }
+    if (ask.greedy) {
+      first = __reduce_min_sync(0xFFFFFFFFu, own == top ? first : 0xFFFFFFFFu);
+      write(first_of(row, first, top, lane), 0.f);
+      continue;
+    }
+    Weights w;
+    w.powers = powers;
+    w.set(top, ask.t);
+    FastWeights fast;
+    fast.set(top, ask.t);
+    auto weight_of = [&](unsigned int k) {
+      const TileStat s = stats[k];
+      return EXACT ? s.weight : s.weight > 0.0 ? s.weight * fast.unit(s.largest, ask.t) : 0.0;
+    };
+    double sum = 0.0;
+    bool usable = EXACT || fast.usable;
+    for (unsigned int k = t0; k < t1; ++k) {
+      usable = usable && (EXACT || stats[k].weight >= 0.0);
+      sum += weight_of(k);
+    }
+    usable = __all_sync(0xFFFFFFFFu, usable);
+    double upto = sum;
+    for (int o = 1; o < 32; o <<= 1) {
+      const double below = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+      if (lane >= o) upto += below;
+    }
+    const double total = __shfl_sync(0xFFFFFFFFu, upto, 31), target = target_of(a.u[r], total);
+    // the lane's tiles, then the tile, in which it is crossed; the last one with any weight
+    const unsigned int any = __ballot_sync(0xFFFFFFFFu, sum > 0.0), past = __ballot_sync(0xFFFFFFFFu, sum > 0.0 && upto > target);
+    const int from = past ? __ffs(past) - 1 : 31 - __clz(any);
+    double start = __shfl_sync(0xFFFFFFFFu, upto - sum, from);
+    unsigned int tile = 0;
+    {
+      const unsigned int k0 = __shfl_sync(0xFFFFFFFFu, t0, from), k1 = __shfl_sync(0xFFFFFFFFu, t1, from);
+      double before = start;
+      for (unsigned int k = k0; k < k1; ++k) {
+        const double x = weight_of(k);
+        if (!(x > 0.0)) continue;
+        tile = k;
+        start = before;
+        before += x;
+        if (before > target) break;
+      }
+    }
+    unsigned int place = 0;
+    float logit = top;
+    double weight = 0.0;
+    if constexpr (EXACT) {
+      walk<N, double>(lane, tile * TILE, tile * TILE + TILE, start, target, place, logit, weight, [&](unsigned int i, float (&f)[N], double (&x)[N]) {
+        row.load(i, f);
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = w.of(f[j]);
+      });
+      write(place - row.shift, (float)(w.exponent(logit) - log(total)));
+    } else {
+      bool sure = false;
+      if (usable) {
+        FastWeights own_unit;
+        own_unit.set(stats[tile].largest, ask.t);
+        const double unit = fast.unit(stats[tile].largest, ask.t), goal = target / unit;  // exact quotients by a power of two
+        double before = start / unit;
+        const bool found = walk<N, float>(lane, tile * TILE, tile * TILE + TILE, before, goal, place, logit, weight, [&](unsigned int i, float (&f)[N], float (&x)[N]) {
+          row.load(i, f);
+#pragma unroll
+          for (int j = 0; j < N; ++j) x[j] = own_unit.of(f[j]);
+        });
+        sure = found && goal - before > SLACK * goal && before + weight - goal > SLACK * goal;
+      }
+      if (sure) write(place - row.shift, (float)(w.exponent(logit) - log(total * fast.to_top(w))));
+      else if (lane == 0) a.open[atomicAdd(a.open_count, 1u)] = (unsigned int)r;
+    }
+  }
 }
 
-constexpr size_t HELD_MOST = 200 * 1024;  // of a block's part in shared memory
-constexpr size_t SAMPLE_ROWS_MOST = 1 << 24, SAMPLE_VOCAB_MOST = 1 << 24;
-
-template <typename T, bool HELD>
-cudaError_t sample_launch(SampleArgs a, size_t rows, int ranks, cudaStream_t s) {
-  const size_t smem = HELD ? (size_t)a.part * sizeof(T) : 0;
-  cudaError_t e = cudaSuccess;
-  if (HELD) e = cudaFuncSetAttribute(sample_kernel<T, HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)HELD_MOST);
-  Chain chain(s);
-  chain.err = e;
-  chain.launch(sample_kernel<T, HELD>, dim3((unsigned int)(rows * ranks)), SAMPLE_THREADS, smem, ranks > 1 ? ranks : 0, a);
-  return chain.err;
+// Weights of the listed rows' tiles in fp64, relative to the row's largest logit: a warp per tile.
+template <typename T>
+__global__ void __launch_bounds__(TILE_THREADS) sample_exact_kernel(const SampleArgs a) {
+  constexpr int N = 16 / (int)sizeof(T);
+  __shared__ double powers[STEPS];
+  let_next_start();
+  if (threadIdx.x < STEPS) powers[threadIdx.x] = exp2(threadIdx.x / (double)STEPS);
+  __syncthreads();
+  after_previous();
+  const int lane = threadIdx.x & 31;
+  const unsigned long long all = (unsigned long long)*a.open_count * a.tiles;
+  for (unsigned long long at = ((unsigned long long)blockIdx.x * TILE_THREADS + threadIdx.x) >> 5; at < all; at += (unsigned long long)gridDim.x * TILE_THREADS / 32) {
+    const size_t r = a.open[at / a.tiles];
+    const unsigned int k = (unsigned int)(at % a.tiles);
+    TileStat* stats = a.stats + r * a.tiles;
+    float top = -INFINITY;
+    for (unsigned int i = lane; i < a.tiles; i += 32) top = fmaxf(top, stats[i].largest);
+    top = warp_max(top);
+    Weights w;
+    w.powers = powers;
+    w.set(top, SampleRow(a, r).t);
+    const RowView<T> row(a, r);
+    double sum = 0.0;
+    for (unsigned int i = k * TILE + lane * N; i < (k + 1) * TILE; i += 32 * N) {
+      float f[N];
+      row.load(i, f);
+      double x[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[j] = w.of(f[j]);
+#pragma unroll
+      for (int o = 1; o < N; o *= 2)
+#pragma unroll
+        for (int j = 0; j + o < N; j += 2 * o) x[j] += x[j + o];
+      sum += x[0];
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) stats[k].weight = sum;
+  }
 }
 
 template <typename T>
-cudaError_t sample_rows(SampleArgs a, size_t rows, int sms, cudaStream_t s) {
-  constexpr unsigned int WHOLE = SAMPLE_WARPS * 32 * (16 / (int)sizeof(T));  // tokens of one tile for each warp
-  auto part = [&](int ranks) {
-    const size_t share = (a.vocab + (size_t)ranks - 1) / ranks;
-    return (unsigned int)((share + WHOLE - 1) / WHOLE * WHOLE);
-  };
-  // more blocks per row while that takes less shared memory or more SMs, and each warp keeps a tile
-  int ranks = 1;
-  while (ranks < MOST_CLUSTER && part(ranks) > WHOLE && ((size_t)part(ranks) * sizeof(T) > 64 * 1024 || rows * ranks < (size_t)sms * 2)) ranks *= 2;
-  a.part = part(ranks);
-  if ((size_t)a.part * sizeof(T) <= HELD_MOST) return sample_launch<T, true>(a, rows, ranks, s);
-  return sample_launch<T, false>(a, rows, ranks, s);
+__global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleArgs a) {
+  extern __shared__ __align__(16) unsigned char shared[];
+  after_previous();
+  Sampler<T> s{a, *reinterpret_cast<SampleShared*>(shared), blockIdx.x, RowView<T>(a, blockIdx.x), (int)threadIdx.x & 31, (int)threadIdx.x >> 5};
+  s.run();
+}
+
+constexpr size_t SAMPLE_ROWS_MOST = 1 << 24, SAMPLE_VOCAB_MOST = 1 << 24;
+
+size_t sample_space(size_t rows, size_t vocab, void* base, SampleArgs* a) {
+  Carver c(base);
+  a->tiles = (unsigned int)((vocab + 7 + TILE - 1) / TILE);  // with up to 7 places before the first token
+  a->stats = c.take<TileStat>(rows * a->tiles);
+  a->lane_most = c.take<float>(rows * a->tiles * 32);
+  a->open_count = c.take<unsigned int>(1);
+  a->open = c.take<unsigned int>(rows);
+  return c.used;
+}
+
+template <typename T>
+cudaError_t sample_rows(const SampleArgs& a, size_t rows, bool limits, int sms, cudaStream_t s) {
+  const unsigned long long all = (unsigned long long)rows * a.tiles;
+  Chain chain(s);
+  if (!limits) {
+    const unsigned int per_block = WHOLE_THREADS / 32, blocks = (unsigned int)((rows + per_block - 1) / per_block), some = (unsigned int)sms * 4;
+    chain.launch(sample_tiles_kernel<T>, dim3((unsigned int)((all * 32 + TILE_THREADS - 1) / TILE_THREADS)), TILE_THREADS, 0, 0, a, all);
+    chain.launch(sample_whole_kernel<T, false>, dim3(blocks), WHOLE_THREADS, 0, 0, a, rows);
+    chain.launch(sample_exact_kernel<T>, dim3(all * 32 / TILE_THREADS + 1 < some ? (unsigned int)(all * 32 / TILE_THREADS + 1) : some), TILE_THREADS, 0, 0, a);
+    chain.launch(sample_whole_kernel<T, true>, dim3(blocks < some ? blocks : some), WHOLE_THREADS, 0, 0, a, rows);
+    return chain.err;
+  }
+  chain.err = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SampleShared));
+  chain.launch(sample_tiles_kernel<T>, dim3((unsigned int)((all * 32 + TILE_THREADS - 1) / TILE_THREADS)), TILE_THREADS, 0, 0, a, all);
+  chain.launch(sample_kernel<T>, dim3((unsigned int)rows), SAMPLE_THREADS, sizeof(SampleShared), 0, a);
+  return chain.err;
 }
 
 }  // namespace
@@ -830,14 +1255,23 @@ int b2_sample_options_default(b2_sample_options* o) {
   return B2_OK;
 }
 
+int b2_sample_workspace(size_t rows, size_t vocab, size_t* bytes) {
+  if (rows > SAMPLE_ROWS_MOST || vocab == 0 || vocab > SAMPLE_VOCAB_MOST)
+    return call_error(B2_ERR_INVALID, "b2_sample_workspace: %zu rows of %zu (2^24 at most, 1 to 2^24)", rows, vocab);
+  if (!bytes) return call_error(B2_ERR_INVALID, "b2_sample_workspace: null pointer");
+  SampleArgs a{};
+  *bytes = sample_space(rows, vocab, nullptr, &a);
+  return B2_OK;
+}
+
 int b2_sample(size_t rows, size_t vocab, int dtype, const void* logits, size_t ld, const float* u, const b2_sample_options* o, void* tokens,
-              int token_bytes, float* logprob, void* stream) {
+              int token_bytes, float* logprob, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "b2_sample";
   if (!dtype_ok(dtype)) return call_error(B2_ERR_INVALID, "%s: dtype %d", who, dtype);
   if (rows > SAMPLE_ROWS_MOST || vocab == 0 || vocab > SAMPLE_VOCAB_MOST)
     return call_error(B2_ERR_INVALID, "%s: %zu rows of %zu (2^24 at most, 1 to 2^24)", who, rows, vocab);
   if (token_bytes != 4 && token_bytes != 8) return call_error(B2_ERR_INVALID, "%s: tokens of %d bytes", who, token_bytes);
-  if (!o || (rows && (!logits || !u || !tokens))) return call_error(B2_ERR_INVALID, "%s: null pointer", who);
+  if (!o || (rows && (!logits || !u || !tokens || !workspace))) return call_error(B2_ERR_INVALID, "%s: null pointer", who);
   const size_t e = dtype_bytes(dtype);
   if (ld < vocab) return call_error(B2_ERR_INVALID, "%s: leading dimension smaller than the width", who);
   if (reinterpret_cast<size_t>(logits) % e || reinterpret_cast<size_t>(tokens) % token_bytes ||
@@ -845,19 +1279,22 @@ int b2_sample(size_t rows, size_t vocab, int dtype, const void* logits, size_t l
        reinterpret_cast<size_t>(o->row_top_p) | reinterpret_cast<size_t>(o->row_min_p)) % 4)
     return call_error(B2_ERR_INVALID, "%s: a pointer is not aligned to its elements", who);
   if (o->temperature != o->temperature || o->top_p != o->top_p || o->min_p != o->min_p) return call_error(B2_ERR_INVALID, "%s: an option is not a number", who);
+  if (reinterpret_cast<size_t>(workspace) % 256) return call_error(B2_ERR_INVALID, "%s: the workspace is not on a 256-byte boundary", who);
+  SampleArgs a{};
+  const size_t need = sample_space(rows, vocab, workspace, &a);
+  if (rows && workspace_bytes < need) return call_error(B2_ERR_INVALID, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, need);
   int sms, rc;
   if ((rc = lm_device(&sms)) != B2_OK) return rc;
   auto vector = [&](const char* name, const void* p, size_t bytes, bool written) { return extent(name, p, 1, rows * bytes, rows * bytes, written); };
   Extent args[] = {extent("logits", logits, rows, vocab * e, ld * e, false), vector("u", u, 4, false), vector("row_temperature", o->row_temperature, 4, false),
                    vector("row_top_k", o->row_top_k, 4, false), vector("row_top_p", o->row_top_p, 4, false), vector("row_min_p", o->row_min_p, 4, false),
-                   vector("tokens", tokens, token_bytes, true), vector("logprob", logprob, 4, true)};
-  if ((rc = refuse_overlap(who, args, 8)) != B2_OK) return rc;
+                   vector("tokens", tokens, token_bytes, true), vector("logprob", logprob, 4, true),
+                   extent("the workspace", workspace, 1, rows ? need : 0, need, true)};
+  if ((rc = refuse_overlap(who, args, 9)) != B2_OK) return rc;
   if (!rows) return B2_OK;
-  SampleArgs a{};
   a.logits = static_cast<const char*>(logits);
   a.ld = ld * e;
   a.vocab = (unsigned int)vocab;
-  a.vec = reinterpret_cast<size_t>(logits) % 16 == 0 && (ld * e % 16 == 0 || rows == 1);
   a.u = u;
   a.temperature = o->temperature;
   a.top_p = o->top_p;
@@ -870,8 +1307,10 @@ int b2_sample(size_t rows, size_t vocab, int dtype, const void* logits, size_t l
   a.tokens = tokens;
   a.wide = token_bytes == 8;
   a.logprob = logprob;
-  const cudaError_t err = dtype == B2_DTYPE_BF16 ? sample_rows<__nv_bfloat16>(a, rows, sms, static_cast<cudaStream_t>(stream))
-                                                 : sample_rows<float>(a, rows, sms, static_cast<cudaStream_t>(stream));
+  if (!o->row_top_k && !(o->top_k > 0 && (size_t)o->top_k < vocab)) a.lane_most = nullptr;
+  const bool limits = a.lane_most || o->row_top_p || o->top_p < 1.f || o->row_min_p || o->min_p > 0.f;
+  const cudaError_t err = dtype == B2_DTYPE_BF16 ? sample_rows<__nv_bfloat16>(a, rows, limits, sms, static_cast<cudaStream_t>(stream))
+                                                 : sample_rows<float>(a, rows, limits, sms, static_cast<cudaStream_t>(stream));
   return launch_error(err, who);
 }
 

@@ -356,8 +356,9 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprob=Fa
         raise ValueError(f"out: a contiguous int64 or int32 tensor of {rows} on {device} is wanted")
     lp = torch.empty(rows, dtype=torch.float32, device=device) if logprob else None
     with _on(device) as stream:
+        ws = _workspace(device, "sample", rows, vocab)
         _ck(K.lib().b2_sample(rows, vocab, _DTYPES[logits.dtype], p, ld, pu, C.byref(o), out.data_ptr(), out.element_size(),
-                              None if lp is None else lp.data_ptr(), stream))
+                              None if lp is None else lp.data_ptr(), ws.data_ptr(), ws.numel(), stream))
     if given:
         _changed(given)
     return (out, lp) if logprob else out

@@ -9,7 +9,8 @@
 //   sample_kernel         a block per row. From the tiles' numbers come the row's maximum and weight. Without a limit the tile in which the running
 //                         weight crosses u's share is read once more. Otherwise a floor below which no token is kept comes from the lanes' maxima (top-k: as many
 //                         lanes as top_k reach it), the row's weight (top-p: tokens of less than (1 - p) / vocab of it are never needed) or the least
-//                         weight (min-p), and the tokens above it, mostly few, are gathered from the tiles that have any.
+//                         weight (min-p), and the tokens above it, mostly few, are gathered in shared memory from the tiles that have any; where there is no room for
+//                         them, passes read the row again.
 //
 // Up to 512 gathered tokens are put in order one by one. With more nothing is sorted: top-k and top-p are a logit (the last one kept) and how many of the
 // tokens that have exactly this one are kept, found by counting tokens in bins: first bins of equal width in max - x, then of equal width in the logit's bits
@@ -32,7 +33,6 @@ constexpr int SAMPLE_THREADS = 512, SAMPLE_WARPS = SAMPLE_THREADS / 32;
 constexpr int TILE_THREADS = 256, TILE = 1024, PER_LANE = TILE / 32;
 constexpr int BINS = 1024, BINS_PER_THREAD = BINS / SAMPLE_THREADS;
 constexpr int LIST = SAMPLE_THREADS;  // tokens that are put in order one by one
-constexpr int STORED = 8192;          // gathered tokens that shared memory holds; of more, those of the row are read again for each pass
 constexpr int STEPS = 16;             // 2^(n / 16) for n = 0 to 15 lie in different banks of shared memory
 constexpr double REACH = 40.0;        // in units of T: what weighs less than e^-40 of the largest weighs nothing where a limit is looked for
 
@@ -140,6 +140,7 @@ __device__ __forceinline__ unsigned int without_minus_zero(unsigned int key) { r
 struct Weights {
   float top;
   double wide_top, inv_t, steps;     // steps: 16 log2(e) / T
+  double reach;                      // -693 T: weights of 2^-1000
   const double* powers;              // in shared memory
   float least;                       // logits below it weigh nothing: less than 2^-1000, -inf
   float half_top, per_bin;           // per_bin: bins for each 2 of the logit
@@ -150,31 +151,36 @@ struct Weights {
     plain = (t > 1e-25f && t < 1e25f) || top == INFINITY;
     wide_top = plain ? widened(top) : (double)top;
     inv_t = 1.0 / (double)t;
+    reach = -693.0 * (double)t;
     steps = STEPS * 1.4426950408889634 * inv_t;
-    least = top == INFINITY ? top : (float)fmax((double)top - 693.0 * (double)t, -3.4028234663852886e38);
+    least = top == INFINITY ? top : (float)fmax((double)top + reach, -3.4028234663852886e38);
     half_top = 0.5f * top;
   }
   // Bins that reach `span` below the top, in units of T; the last one has all that is lower.
   __device__ __forceinline__ void set_bins(double span) { per_bin = (float)fmin(2 * (BINS - 1) / span * inv_t, 1e38); }
   __device__ __forceinline__ double exponent(float f) const { return f == top ? 0.0 : ((double)f - (double)top) * inv_t; }
-  // The weight of a logit `by` below the top.
-  __device__ __forceinline__ double below(double by) const { return exp2(-by * (steps / STEPS)); }
-  // The weight: 2^((n + s) / 16), n an integer
-  __device__ __forceinline__ double of(float f) const {
-    const float g = fmaxf(f, least);
-    const double d = (plain ? widened(g) : (double)g) - wide_top;
+  // The weight of a logit d <= 0 above the top: 2^((n + s) / 16), n an integer, for d of -693 T at least
+  __device__ __forceinline__ double power(double d) const {
     const double t = fma(d, steps, 6755399441055744.0);  // 1.5 * 2^52: the sum's low bits are n
     const double s = fma(d, steps, 6755399441055744.0 - t);
     const int n = __double2loint(t);
-    const double base = powers[n & (STEPS - 1)], w = fma(base, small_power(s), base);
-    const unsigned int hi = __double2hiint(w) + ((n & ~(STEPS - 1)) << 16);
-    return __hiloint2double(f < least ? 0 : hi, f < least ? 0 : __double2loint(w));
+    const double base = powers[n & (STEPS - 1)], x = fma(base, small_power(s), base);
+    return __hiloint2double(__double2hiint(x) + ((n & ~(STEPS - 1)) << 16), __double2loint(x));
   }
-  // 0 at the top; falls with f in steps, whatever fp32 rounds
+  __device__ __forceinline__ double of(float f) const {
+    const float g = fmaxf(f, least);
+    const double x = power((plain ? widened(g) : (double)g) - wide_top);
+    return f < least ? 0.0 : x;
+  }
+  // The nearest whole number of bins below the top; falls with f in steps, whatever fp32 rounds.
   __device__ __forceinline__ unsigned int bin(float f) const {
-    const unsigned int b = f == top ? 0u : __float2uint_rz(fmaf(-0.5f, f, half_top) * per_bin);
-    return b < BINS ? b : BINS - 1;
+    const float b = f == top ? 0.f : fminf(fmaf(-0.5f, f, half_top) * per_bin, (float)(BINS - 1));
+    return __float_as_uint(b + 8388608.f) & (2 * BINS - 1);  // 2^23: the sum's low bits
   }
+  // Below the top, in units of the logit: where bins of numbers up to b end at the latest, and those from b on begin at the earliest. Rounded differences and products move a
+  // token by less than 1e-3 of a bin.
+  __device__ __forceinline__ double bin_end(unsigned int b) const { return (b + 0.501) * 2.0 / (double)per_bin; }
+  __device__ __forceinline__ double bin_begin(unsigned int b) const { return b ? (b - 0.501) * 2.0 / (double)per_bin : 0.0; }
 };
 
 // Weights in fp32 up to a factor that all of them share: 2^(x c - N) with c = log2(e) / T and N = rint(largest c), by the nearest integer n of x c and 2^(x c - n).
@@ -274,14 +280,19 @@ __global__ void __launch_bounds__(TILE_THREADS) sample_tiles_kernel(const Sample
   if (lane == 0) a.stats[tile] = TileStat{sum, most, 0.f};
 }
 
+// Tokens that the shared memory of a block holds of one warp's tiles, so that two blocks fit an SM.
+template <typename T> constexpr unsigned int SEGMENT = sizeof(T) == 2 ? 1280 : 896;
+constexpr unsigned int SEGMENT_TILES = 64;  // of one warp at most: offsets in 16 bits
+
+template <typename T>
 struct SampleShared {
   unsigned int bins[3][BINS];  // the first ones, and two that take turns
   unsigned long long list[LIST], ordered[LIST], own[LIST];
   double sums[2][SAMPLE_WARPS];
   double powers[STEPS];
   unsigned int counts[SAMPLE_WARPS], found[4], listed;
-  float stored[STORED];          // gathered tokens by number
-  unsigned int number[STORED];
+  alignas(16) T values[SAMPLE_WARPS * SEGMENT<T>];           // gathered tokens by warp, in their order
+  unsigned short offsets[SAMPLE_WARPS * SEGMENT<T>];         // of their places to the warp's first
 };
 
 // What is kept: logits above `value`, and the first `ties` of `equal` tokens that have it.
@@ -368,9 +379,9 @@ __device__ __forceinline__ bool walk(int lane, unsigned int from, unsigned int t
 
 template <typename T>
 struct Sampler {
-  static constexpr int M = 4;  // neighbours that a lane takes at a time, of the gathered tokens or of the row
+  static constexpr int M = 16 / (int)sizeof(T);  // neighbours that a lane takes at a time, of the gathered tokens or of the row
   const SampleArgs& a;
-  SampleShared& sh;
+  SampleShared<T>& sh;
   size_t r;
   RowView<T> row;
   int lane, warp;
@@ -382,14 +393,18 @@ struct Sampler {
   // M tokens from place i on; what does not count as -inf.
   __device__ __forceinline__ void fetch(unsigned int i, float (&f)[M]) const {
     if (stored) {
-      Elems<float, 16>::get(*reinterpret_cast<const uint4*>(sh.stored + i), f);
+      Elems<T, 16>::get(*reinterpret_cast<const uint4*>(sh.values + i), f);
     } else {
       row.load(i, f);
 #pragma unroll
       for (int j = 0; j < M; ++j) f[j] = f[j] >= floor ? f[j] : -INFINITY;
     }
   }
-  __device__ __forceinline__ unsigned int number_of(unsigned int place) const { return stored ? sh.number[place] : place - row.shift; }
+  __device__ __forceinline__ unsigned int number_of(unsigned int place) const {
+    return (stored ? first_tile(place / SEGMENT<T>) * TILE + sh.offsets[place] : place) - row.shift;
+  }
+  // Warps take neighbouring tiles.
+  __device__ __forceinline__ unsigned int first_tile(unsigned int of_warp) const { return (unsigned int)((unsigned long long)a.tiles * of_warp / SAMPLE_WARPS); }
   // body(place of the first, logits) for the warp's tokens.
   template <class Body>
   __device__ __forceinline__ void each(Body body) const {
@@ -488,6 +503,62 @@ struct Sampler {
     return sh.found[0];
   }
 
+  // Lowest and highest key of bin b of a window.
+  __device__ __forceinline__ unsigned int edge_of(bool first, unsigned int lo, unsigned int hi, unsigned int shift, unsigned int b, bool upper) const {
+    if (first) return edge(b, upper);
+    if (upper) return hi - (b << shift);
+    const unsigned int down = ((b + 1) << shift) - 1;
+    return hi - lo > down ? hi - down : lo;
+  }
+  // Bins of a window in which the running weight, `mass` above it, reaches the target: at the earliest, by estimate, at the latest; false where it does not before the
+  // tokens that weigh nothing. Weights of a bin's tokens are between those of its ends.
+  __device__ __forceinline__ bool bracket(int buffer, bool first, unsigned int lo, unsigned int hi, unsigned int shift, double mass, double target_low, double target,
+                                          double target_high, unsigned int& b1, unsigned int& m, unsigned int& b2) {
+    unsigned int count[BINS_PER_THREAD], mine = 0;
+    double low[BINS_PER_THREAD], mid[BINS_PER_THREAD], high[BINS_PER_THREAD];
+    double sum_low = 0.0, sum_mid = 0.0, sum_high = 0.0;
+#pragma unroll
+    for (int k = 0; k < BINS_PER_THREAD; ++k) {
+      const unsigned int b = threadIdx.x * BINS_PER_THREAD + k;
+      count[k] = first && b == BINS - 1 ? 0 : sh.bins[buffer][b];
+      mine += count[k];
+      double wl = 0.0, wh = 0.0;
+      if (count[k]) {
+        if (first) {
+          wl = -w.bin_end(b) >= w.reach ? w.power(-w.bin_end(b)) : 0.0;
+          wh = w.power(fmax(-w.bin_begin(b), w.reach));
+        } else {
+          wl = w.of(value_of(edge_of(false, lo, hi, shift, b, false)));
+          wh = w.of(value_of(edge_of(false, lo, hi, shift, b, true)));
+        }
+      }
+      low[k] = sum_low += wl * count[k];
+      high[k] = sum_high += wh * count[k];
+      mid[k] = sum_mid += 0.5 * (wl + wh) * count[k];
+    }
+    const double before_low = scan(sum_low, sh.sums[0]) - sum_low, before_high = scan(sum_high, sh.sums[0]) - sum_high,
+                 before_mid = scan(sum_mid, sh.sums[0]) - sum_mid;
+    unsigned int upto = scan(mine, sh.counts) - mine;
+    if (threadIdx.x == 0) sh.found[0] = 0;
+    __syncthreads();
+    // bins with tokens only: the first ones whose running weight reaches the target
+    b1 = m = b2 = 0;
+#pragma unroll
+    for (int k = 0; k < BINS_PER_THREAD; ++k) {
+      upto += count[k];
+      if (count[k]) atomicMax(&sh.found[0], (unsigned int)(threadIdx.x * BINS_PER_THREAD + k));
+      b1 += __syncthreads_count(upto == 0 || mass + before_high + high[k] < target_low);
+      m += __syncthreads_count(upto == 0 || mass + before_mid + mid[k] < target);
+      b2 += __syncthreads_count(upto == 0 || mass + before_low + low[k] < target_high);
+    }
+    if (first && b1 >= BINS) return false;
+    const unsigned int last = sh.found[0];
+    if (b2 > last) b2 = last;
+    if (b1 > b2) b1 = b2;
+    m = m < b1 ? b1 : m > b2 ? b2 : m;
+    return true;
+  }
+
   // The cut at which `target` tokens (BY_COUNT) or `target` weight is reached. The first bins have been counted.
   // slack: the target may be off by this share of it. NONE: it is not reached before the tokens that weigh nothing. UNSURE: where depends on what the target is off.
   enum Found { NONE, CUT, UNSURE };
@@ -502,61 +573,14 @@ struct Sampler {
     for (;;) {
       __syncthreads();  // all have counted
       const unsigned int next = buffer == 1 ? 2 : 1;
-      auto edge_of = [&](unsigned int b, bool upper) -> unsigned int {
-        if (first) return edge(b, upper);
-        if (upper) return hi - (b << shift);
-        const unsigned int down = ((b + 1) << shift) - 1;
-        return hi - lo > down ? hi - down : lo;
-      };
+      auto edge_of = [&](unsigned int b, bool upper) { return this->edge_of(first, lo, hi, shift, b, upper); };
       unsigned int b1 = 0, b2 = 0, m = 0, above = 0;
       if constexpr (BY_COUNT) {
         m = reaches(buffer, goal);
         if (first && m >= BINS - 1) return NONE;
         above = sh.found[1];
       } else {
-        // the running weight at the bins' ends, by the lightest, the heaviest and a middle token of each
-        unsigned int count[BINS_PER_THREAD], mine = 0;
-        double low[BINS_PER_THREAD], mid[BINS_PER_THREAD], high[BINS_PER_THREAD];
-        double sum_low = 0.0, sum_mid = 0.0, sum_high = 0.0;
-#pragma unroll
-        for (int k = 0; k < BINS_PER_THREAD; ++k) {
-          const unsigned int b = threadIdx.x * BINS_PER_THREAD + k;
-          count[k] = sh.bins[buffer][b];
-          mine += count[k];
-          double wl = 0.0, wh = 0.0;
-          if (count[k]) {
-            if (first) {
-              const double width = 2.0 / (double)w.per_bin;  // rounded differences and products move a token by less than 1e-3 of a bin
-              wl = w.below(width * (b + 1.001));
-              wh = w.below(width * (b > 0 ? b - 0.001 : 0.0));
-            } else {
-              wl = w.of(value_of(edge_of(b, false)));
-              wh = w.of(value_of(edge_of(b, true)));
-            }
-          }
-          low[k] = sum_low += wl * count[k];
-          high[k] = sum_high += wh * count[k];
-          mid[k] = sum_mid += 0.5 * (wl + wh) * count[k];
-        }
-        const double before_low = scan(sum_low, sh.sums[0]) - sum_low, before_high = scan(sum_high, sh.sums[0]) - sum_high,
-                     before_mid = scan(sum_mid, sh.sums[0]) - sum_mid;
-        unsigned int upto = scan(mine, sh.counts) - mine;
-        if (threadIdx.x == 0) sh.found[0] = 0;
-        __syncthreads();
-        // bins with tokens only: the first ones whose running weight reaches the target
-#pragma unroll
-        for (int k = 0; k < BINS_PER_THREAD; ++k) {
-          upto += count[k];
-          if (count[k]) atomicMax(&sh.found[0], (unsigned int)(threadIdx.x * BINS_PER_THREAD + k));
-          b1 += __syncthreads_count(upto == 0 || mass + before_high + high[k] < target_low);
-          m += __syncthreads_count(upto == 0 || mass + before_mid + mid[k] < target);
-          b2 += __syncthreads_count(upto == 0 || mass + before_low + low[k] < target_high);
-        }
-        if (first && b1 >= BINS) return NONE;
-        const unsigned int last = sh.found[0];
-        if (b2 > last) b2 = last;
-        if (b1 > b2) b1 = b2;
-        m = m < b1 ? b1 : m > b2 ? b2 : m;
+        if (!bracket(buffer, first, lo, hi, shift, mass, target_low, target, target_high, b1, m, b2)) return NONE;
         __syncthreads();
         if (threadIdx.x == 0) sh.found[2] = sh.bins[buffer][m];
       }
@@ -796,72 +820,114 @@ struct Sampler {
     return sh.found[0];
   }
 
-  // The tokens of at least `floor`: how many there are, and in `own` how many of them the warp's tiles have, which are neighbours. Up to LIST of them are listed, with their
-  // numbers for places.
-  __device__ __forceinline__ unsigned int gather(unsigned int& own) {
-    constexpr int N = 16 / (int)sizeof(T);
+  // top-p: the tokens from `lowest` on are counted in bins, which say how far down the limit can be at most.
+  __device__ __forceinline__ double narrowed(double lowest, double target) {
+    w.set_bins(fmin(REACH, -lowest * w.inv_t * 1.01 + 1e-6));
+    for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) sh.bins[0][i] = 0;
+    __syncthreads();
     const TileStat* stats = a.stats + r * a.tiles;
-    const float* most = a.lane_most ? a.lane_most + r * a.tiles * 32 : nullptr;
+    const float least = fmaxf((float)((double)w.top + lowest), -3.4028235e38f);
+    for (unsigned int k = warp; k < a.tiles; k += SAMPLE_WARPS) {
+      if (!(stats[k].largest >= least)) continue;
+      uint4 v[PER_LANE / M];
+#pragma unroll
+      for (int q = 0; q < PER_LANE / M; ++q) v[q] = row.load_vector(k * TILE + (q * 32 + lane) * M);
+#pragma unroll
+      for (int q = 0; q < PER_LANE / M; ++q) {
+        float f[M];
+        Elems<T, 16>::get(v[q], f);
+#pragma unroll
+        for (int j = 0; j < M; ++j)
+          if (f[j] >= least) atomicAdd(&sh.bins[0][w.bin(f[j])], 1u);
+      }
+    }
+    __syncthreads();
+    unsigned int b1, m, b2;
+    return bracket(0, true, 0, 0, 0, 0.0, target * (1.0 - SLACK), target, target * (1.0 + SLACK), b1, m, b2) ? fmax(lowest, -w.bin_end(b2)) : lowest;
+  }
+
+  // The tokens of at least `floor` where few are expected: how many there are, the first LIST that come listed with their numbers for places.
+  __device__ __forceinline__ unsigned int gather_few() {
+    const float* most = a.lane_most + r * a.tiles * 32;
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
-    own = 0;
-    const unsigned int t0 = a.tiles * warp / SAMPLE_WARPS, t1 = a.tiles * (warp + 1) / SAMPLE_WARPS;
+    for (unsigned int k = warp; k < a.tiles; k += SAMPLE_WARPS) {
+      if (!(most[k * 32 + lane] >= floor)) continue;
+      uint4 v[PER_LANE / M];
+#pragma unroll
+      for (int q = 0; q < PER_LANE / M; ++q) v[q] = row.load_vector(k * TILE + (q * 32 + lane) * M);
+#pragma unroll
+      for (int q = 0; q < PER_LANE / M; ++q) {
+        float f[M];
+        Elems<T, 16>::get(v[q], f);
+#pragma unroll
+        for (int j = 0; j < M; ++j)
+          if (f[j] >= floor) {
+            const unsigned int at = atomicAdd(&sh.listed, 1u);
+            if (at < LIST) sh.list[at] = (unsigned long long)~key_of(f[j]) << 32 | (k * TILE + (q * 32 + lane) * M + j - row.shift);
+          }
+      }
+    }
+    __syncthreads();
+    return sh.listed;
+  }
+
+  // The tokens of at least `floor`: how many there are. Each warp's go to its segment of shared memory, in their order and with -inf behind them, where there is room.
+  __device__ __forceinline__ unsigned int gather() {
+    const TileStat* stats = a.stats + r * a.tiles;
+    const float* most = a.lane_most ? a.lane_most + r * a.tiles * 32 : nullptr;
+    constexpr unsigned int SEG = SEGMENT<T>;
+    T* to = sh.values + warp * SEG;
+    unsigned short* offsets = sh.offsets + warp * SEG;
+    unsigned int own = 0;
+    const unsigned int t0 = first_tile(warp), t1 = first_tile(warp + 1);
     for (unsigned int k = t0; k < t1; ++k) {
-      if (!(most ? most[k * 32 + lane] >= floor : stats[k].largest >= floor)) continue;
-      const bool room = *(volatile unsigned int*)&sh.listed < LIST;
+      const bool some = most ? most[k * 32 + lane] >= floor : stats[k].largest >= floor;
+      if (!__any_sync(0xFFFFFFFFu, some)) continue;
+      uint4 v[PER_LANE / M];
 #pragma unroll
-      for (int v = 0; v < PER_LANE / N; ++v) {
-        const unsigned int i = k * TILE + (v * 32 + lane) * N;
-        float f[N];
-        row.load(i, f);
+      for (int q = 0; q < PER_LANE / M; ++q)
+        if (some) v[q] = row.load_vector(k * TILE + (q * 32 + lane) * M);
 #pragma unroll
-        for (int j = 0; j < N; ++j) own += f[j] >= floor;
-        if (room) {
+      for (int q = 0; q < PER_LANE / M; ++q) {
+        float f[M];
+        unsigned int mine = 0;
+        if (some) {
+          Elems<T, 16>::get(v[q], f);
 #pragma unroll
-          for (int j = 0; j < N; ++j)
+          for (int j = 0; j < M; ++j) mine += f[j] >= floor;
+        }
+        if (!__any_sync(0xFFFFFFFFu, mine)) continue;
+        const unsigned int before = lanes_before(mine);
+        unsigned int at = own + before;
+        const unsigned int offset = (k - t0) * TILE + (q * 32 + lane) * M;
+        if (mine) {
+#pragma unroll
+          for (int j = 0; j < M; ++j)
             if (f[j] >= floor) {
-              const unsigned int at = atomicAdd(&sh.listed, 1u);
-              if (at < LIST) sh.list[at] = (unsigned long long)~key_of(f[j]) << 32 | (i + j - row.shift);
+              if (at < SEG) {
+                to[at] = (T)f[j];
+                offsets[at] = (unsigned short)(offset + j);
+              }
+              ++at;
             }
         }
+        own += __shfl_sync(0xFFFFFFFFu, before + mine, 31);
       }
     }
-    own = __reduce_add_sync(0xFFFFFFFFu, own);
+    const unsigned int whole = min((own + 32 * M - 1) / (32 * M) * (32 * M), SEG);
+    for (unsigned int i = own + lane; i < whole; i += 32) to[i] = (T)-INFINITY;
     if (lane == 0) sh.counts[warp] = own;
-    __syncthreads();
+    begin = warp * SEG;
+    end = begin + whole;
+    stored = __syncthreads_and(own <= SEG && t1 - t0 <= SEGMENT_TILES);
     return __reduce_add_sync(0xFFFFFFFFu, lane < SAMPLE_WARPS ? sh.counts[lane] : 0u);
   }
-  // All of them into shared memory by number.
-  __device__ __forceinline__ void store(unsigned int n, unsigned int own) {
-    constexpr int N = 16 / (int)sizeof(T);
-    const TileStat* stats = a.stats + r * a.tiles;
-    const unsigned int upto = scan(lane == 0 ? own : 0u, sh.counts);
-    unsigned int at = __shfl_sync(0xFFFFFFFFu, upto, 0) - own;
-    const unsigned int t0 = a.tiles * warp / SAMPLE_WARPS, t1 = a.tiles * (warp + 1) / SAMPLE_WARPS;
-    for (unsigned int k = t0; k < t1; ++k) {
-      if (!(stats[k].largest >= floor)) continue;
-#pragma unroll
-      for (int v = 0; v < PER_LANE / N; ++v) {
-        const unsigned int i = k * TILE + (v * 32 + lane) * N;
-        float f[N];
-        row.load(i, f);
-        unsigned int mine = 0;
-#pragma unroll
-        for (int j = 0; j < N; ++j) mine += f[j] >= floor;
-        const unsigned int before = lanes_before(mine);
-        unsigned int to = at + before;
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (f[j] >= floor) {
-            sh.stored[to] = f[j];
-            sh.number[to++] = i + j - row.shift;
-          }
-        at += __shfl_sync(0xFFFFFFFFu, before + mine, 31);
-      }
-    }
-    __syncthreads();
-    for (unsigned int i = n + threadIdx.x; i < (n + 32 * M - 1) / (32 * M) * (32 * M); i += SAMPLE_THREADS) sh.stored[i] = -INFINITY;
-    __syncthreads();
+  // The gathered tokens as a list.
+  __device__ __forceinline__ void list_all() {
+    const unsigned int own = sh.counts[warp], before = __reduce_add_sync(0xFFFFFFFFu, lane < warp ? sh.counts[lane] : 0u);
+    for (unsigned int i = lane; i < own; i += 32)
+      sh.list[before + i] = (unsigned long long)~key_of((float)sh.values[begin + i]) << 32 | number_of(begin + i);
   }
 
   // The token by sums over the kept ones in fp64, by places.
@@ -997,36 +1063,41 @@ struct Sampler {
         if (most[i] > -INFINITY) atomicAdd(&sh.bins[0][w.bin(most[i])], 1u);
       __syncthreads();
       const unsigned int bin = reaches(0, ask.top_k);
-      if (bin < BINS - 1) lowest = -(bin + 1.01) * 2.0 / (double)w.per_bin;
+      if (bin < BINS - 1) lowest = -w.bin_end(bin);
     } else if (ask.by_p) {
       if (!from_tiles(ask, false, u, all)) {
         all = whole_weight();
         slack = 0.0;
       }
       lowest = (log((1.0 - (double)ask.top_p) * all * (1.0 - SLACK) / a.vocab) - 1e-3) * (double)ask.t;
+      lowest = narrowed(lowest, (double)ask.top_p * all);
     }
     if (ask.by_m && !(ask.by_k && ask.by_p)) lowest = fmax(lowest, (log((double)ask.min_p) - 1e-3) * (double)ask.t);  // top_p counts all of the first top_k
     // rounded to fp32 it is no more than any logit that it is no more than
     floor = top == INFINITY ? top : (float)fmax((double)top + lowest, -3.4028234663852886e38);
-    unsigned int own;
-    const unsigned int n = gather(own);
-    if (n <= LIST) {
+    if (ask.by_k && ask.top_k <= LIST) {
+      const unsigned int n = gather_few();
+      if (n <= LIST) {
+        choose(n, ask, all, u);
+        return;
+      }
+    }
+    const unsigned int n = gather();
+    if (stored && n <= LIST) {
+      list_all();
       choose(n, ask, all, u);
       return;
     }
-    stored = n <= STORED;
-    if (stored) store(n, own);
-    share(stored ? n : row.end);
+    if (!stored) share(row.end);
     if (ask.by_k || ask.by_p) {
       w.set_bins(fmin(REACH, -lowest * w.inv_t * 1.01 + 1e-6));
+      __syncthreads();
       for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) sh.bins[0][i] = 0;
       __syncthreads();
       each([&](unsigned int, const float (&f)[M]) {
 #pragma unroll
-        for (int j = 0; j < M; ++j) {
-          const unsigned int b = w.bin(f[j]);
-          if (b < BINS - 1) atomicAdd(&sh.bins[0][b], 1u);
-        }
+        for (int j = 0; j < M; ++j)
+          if (f[j] > -INFINITY) atomicAdd(&sh.bins[0][w.bin(f[j])], 1u);
       });
       if (ask.by_k) {
         find<true>(ask.top_k, 0.0, cut);
@@ -1208,7 +1279,7 @@ template <typename T>
 __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) unsigned char shared[];
   after_previous();
-  Sampler<T> s{a, *reinterpret_cast<SampleShared*>(shared), blockIdx.x, RowView<T>(a, blockIdx.x), (int)threadIdx.x & 31, (int)threadIdx.x >> 5};
+  Sampler<T> s{a, *reinterpret_cast<SampleShared<T>*>(shared), blockIdx.x, RowView<T>(a, blockIdx.x), (int)threadIdx.x & 31, (int)threadIdx.x >> 5};
   s.run();
 }
 
@@ -1236,9 +1307,9 @@ cudaError_t sample_rows(const SampleArgs& a, size_t rows, bool limits, int sms, 
     chain.launch(sample_whole_kernel<T, true>, dim3(blocks < some ? blocks : some), WHOLE_THREADS, 0, 0, a, rows);
     return chain.err;
   }
-  chain.err = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SampleShared));
+  chain.err = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SampleShared<T>));
   chain.launch(sample_tiles_kernel<T>, dim3((unsigned int)((all * 32 + TILE_THREADS - 1) / TILE_THREADS)), TILE_THREADS, 0, 0, a, all);
-  chain.launch(sample_kernel<T>, dim3((unsigned int)rows), SAMPLE_THREADS, sizeof(SampleShared), 0, a);
+  chain.launch(sample_kernel<T>, dim3((unsigned int)rows), SAMPLE_THREADS, sizeof(SampleShared<T>), 0, a);
   return chain.err;
 }
 

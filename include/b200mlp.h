@@ -472,19 +472,15 @@ int b2_norm_grad(size_t rows, size_t width, int dtype, const void* dy, size_t ld
 
 /* The global norm of `count` tensors, and the tensors scaled down to a limit:
  *   norm = sqrt(sum of the squares of all elements)     out = x * (norm > max_norm ? max_norm / norm : 1)
- * norm (device memory) is always written; max_norm = INFINITY asks for nothing else, and outputs are then not allowed. out == x (with the same
- * leading dimension) is in place, where nothing is written unless the norm is over the limit. A norm that is infinite or not a number leaves the
- * values as they are: the caller sees it in `norm`. Types may be mixed; elements are squared, summed and scaled in fp32 and fp64 over the whole range
- * of fp32 and rounded once. The list is a host array, read during the call. Equal inputs give equal bits on equal devices. Limits: 2^20 tensors,
- * 2^42 elements together. */
-typedef struct {
-  const void* x;
-  void* out;
-  size_t rows, cols, ld_x, ld_out; /* a dense tensor of any shape is one row */
-  int dtype;
-} b2_clip_tensor;
+ * x[i] and out[i] have elements[i] elements of dtypes[i] (types may be mixed), one behind the other: tensors of any shape without gaps. Where widths is
+ * not NULL, x[i] and out[i] are matrices of rows of widths[i] elements (a divisor of elements[i]), ld_x[i] and ld_out[i] elements apart. out = NULL, or an
+ * out[i] that is x[i] with the same leading dimension, is in place, where nothing is written unless the norm is over the limit. norm (device memory) is
+ * always written; max_norm = INFINITY asks for nothing else, and out has to be NULL then. A norm that is infinite or not a number leaves the
+ * values as they are: the caller sees it in `norm`. Elements are squared, summed and scaled in fp32 and fp64 over the whole range of fp32 and rounded
+ * once. The lists are host arrays, read during the call. Equal inputs give equal bits on equal devices. Limits: 2^20 tensors, 2^42 elements together. */
 int b2_clip_workspace(size_t count, size_t* bytes);
-int b2_clip(size_t count, const b2_clip_tensor* tensors, float max_norm, float* norm, void* workspace,
+int b2_clip(size_t count, const void* const* x, void* const* out, const size_t* elements, const int* dtypes,
+            const size_t* widths, const size_t* ld_x, const size_t* ld_out, float max_norm, float* norm, void* workspace,
             size_t workspace_bytes, void* stream);
 
 /* One token per row of logits (rows x vocab) from given random numbers u (fp32, one per row, from [0, 1)):

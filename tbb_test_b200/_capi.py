@@ -39,11 +39,6 @@ class MuonOptions(C.Structure):
                 ("eps", C.c_float), ("nesterov", C.c_int), ("steps", C.c_int)]
 
 
-class ClipTensor(C.Structure):
-    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("rows", C.c_size_t), ("cols", C.c_size_t), ("ld_x", C.c_size_t), ("ld_out", C.c_size_t),
-                ("dtype", C.c_int)]
-
-
 class SampleOptions(C.Structure):
     _fields_ = [("temperature", C.c_float), ("top_k", C.c_int), ("top_p", C.c_float), ("min_p", C.c_float), ("row_temperature", C.c_void_p),
                 ("row_top_k", C.c_void_p), ("row_top_p", C.c_void_p), ("row_min_p", C.c_void_p)]
@@ -120,7 +115,7 @@ SYMBOLS = {
     "b2_norm_grad_workspace": (C.c_int, [_sz, _sz, C.c_int, C.POINTER(_sz)]),
     "b2_norm_grad": (C.c_int, [_sz, _sz, C.c_int, _vp, _sz, _vp, _sz, _vp, _sz, _vp, C.c_int, C.c_float, _vp, _sz, _vp, _vp, _sz, _vp]),
     "b2_clip_workspace": (C.c_int, [_sz, C.POINTER(_sz)]),
-    "b2_clip": (C.c_int, [_sz, _vp, C.c_float, _vp, _vp, _sz, _vp]),
+    "b2_clip": (C.c_int, [_sz, _vp, _vp, _vp, _vp, _vp, _vp, _vp, C.c_float, _vp, _vp, _sz, _vp]),
     "b2_sample_options_default": (C.c_int, [C.POINTER(SampleOptions)]),
     "b2_sample_workspace": (C.c_int, [_sz, _sz, C.POINTER(_sz)]),
     "b2_sample": (C.c_int, [_sz, _sz, C.c_int, _vp, _sz, _vp, C.POINTER(SampleOptions), _vp, C.c_int, _vp, _vp, _sz, _vp]),

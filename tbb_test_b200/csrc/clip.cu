@@ -278,8 +278,18 @@ cudaError_t clip_launch(const std::vector<ClipTensor>& tensors, bool in_place, f
   return chain.err;
 }
 
-int clip_tensors(const char* who, size_t count, const b2_clip_tensor* x, float max_norm, float* norm, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+struct ClipCall {
+  size_t count;
+  const void* const* x;
+  void* const* out;
+  const size_t* elements;
+  const int* dtypes;
+  const size_t *widths, *ld_x, *ld_out;
+};
+
+int clip_tensors(const char* who, const ClipCall& c, float max_norm, float* norm, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
   const bool limited = max_norm < INFINITY;
+  const size_t count = c.count;
   bool in_place = true;
   std::vector<Extent> args;
   std::vector<ClipTensor> tensors;
@@ -287,28 +297,34 @@ int clip_tensors(const char* who, size_t count, const b2_clip_tensor* x, float m
   tensors.reserve(count);
   unsigned long long all = 0;
   for (size_t i = 0; i < count; ++i) {
-    const b2_clip_tensor& t = x[i];
-    if (!dtype_ok(t.dtype)) return call_error(B2_ERR_INVALID, "%s: dtype %d of tensor %zu", who, t.dtype, i);
-    const size_t e = dtype_bytes(t.dtype);
-    if (t.rows == 0 || t.cols == 0) continue;
-    if (!t.x || !t.out) return call_error(B2_ERR_INVALID, "%s: null pointer of tensor %zu", who, i);
-    if (t.cols > ELEMENTS_MOST || t.rows > ELEMENTS_MOST / t.cols || (all += (unsigned long long)t.rows * t.cols) > ELEMENTS_MOST)
-      return call_error(B2_ERR_INVALID, "%s: more than 2^42 elements up to tensor %zu", who, i);
-    if (t.rows > 1 && (t.ld_x < t.cols || t.ld_out < t.cols))
-      return call_error(B2_ERR_INVALID, "%s: leading dimension of tensor %zu smaller than its width", who, i);
-    if ((reinterpret_cast<size_t>(t.x) | reinterpret_cast<size_t>(t.out)) % e)
+    const int dtype = c.dtypes[i];
+    if (!dtype_ok(dtype)) return call_error(B2_ERR_INVALID, "%s: dtype %d of tensor %zu", who, dtype, i);
+    const size_t e = dtype_bytes(dtype), size = c.elements[i];
+    if (size == 0) continue;
+    const void* x = c.x[i];
+    void* out = c.out ? c.out[i] : const_cast<void*>(x);
+    if (!x || !out) return call_error(B2_ERR_INVALID, "%s: null pointer of tensor %zu", who, i);
+    if (size > ELEMENTS_MOST || (all += size) > ELEMENTS_MOST) return call_error(B2_ERR_INVALID, "%s: more than 2^42 elements up to tensor %zu", who, i);
+    size_t width = size, ld_x = size, ld_out = size;
+    if (c.widths && c.widths[i] != size) {
+      width = c.widths[i];
+      ld_x = c.ld_x[i];
+      ld_out = c.out ? c.ld_out[i] : ld_x;
+      if (width == 0 || size % width) return call_error(B2_ERR_INVALID, "%s: %zu elements of tensor %zu are not whole rows of %zu", who, size, i, width);
+      if (ld_x < width || ld_out < width) return call_error(B2_ERR_INVALID, "%s: leading dimension of tensor %zu smaller than its width", who, i);
+    }
+    if ((reinterpret_cast<size_t>(x) | reinterpret_cast<size_t>(out)) % e)
       return call_error(B2_ERR_INVALID, "%s: a pointer of tensor %zu is not aligned to its elements", who, i);
-    const bool here = t.out == t.x && (t.rows == 1 || t.ld_out == t.ld_x);
-    args.push_back(extent("a tensor", t.x, t.rows, t.cols * e, t.ld_x * e, limited && here));
+    const bool here = out == x && ld_out == ld_x;
+    args.push_back(extent("a tensor", x, size / width, width * e, ld_x * e, limited && here));
     if (!here) {
-      args.push_back(extent("an output", t.out, t.rows, t.cols * e, t.ld_out * e, true));
+      args.push_back(extent("an output", out, size / width, width * e, ld_out * e, true));
       in_place = false;
     }
-    const bool gaps = t.rows > 1 && (t.ld_x != t.cols || t.ld_out != t.cols);
-    tensors.push_back(ClipTensor{static_cast<const char*>(t.x), static_cast<char*>(t.out), (unsigned long long)t.rows * t.cols, t.cols, t.ld_x, t.ld_out,
-                                 t.dtype == B2_DTYPE_F32, gaps});
+    tensors.push_back(ClipTensor{static_cast<const char*>(x), static_cast<char*>(out), size, width, ld_x, ld_out, dtype == B2_DTYPE_F32,
+                                 ld_x != width || ld_out != width});
   }
-  if (!limited && !in_place) return call_error(B2_ERR_INVALID, "%s: outputs without a limit", who);
+  if (!limited && c.out) return call_error(B2_ERR_INVALID, "%s: outputs without a limit", who);
   const int most = count <= LIST_SHORT ? LIST_SHORT : LIST_MOST;
   double* partial;
   const size_t need = clip_space(count ? count : 1, most, workspace, &partial);
@@ -338,15 +354,17 @@ int b2_clip_workspace(size_t count, size_t* bytes) {
   return B2_OK;
 }
 
-int b2_clip(size_t count, const b2_clip_tensor* tensors, float max_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
+int b2_clip(size_t count, const void* const* x, void* const* out, const size_t* elements, const int* dtypes, const size_t* widths, const size_t* ld_x,
+            const size_t* ld_out, float max_norm, float* norm, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "b2_clip";
   if (count > TENSORS_MOST) return call_error(B2_ERR_INVALID, "%s: %zu tensors (2^20 at most)", who, count);
   if (!(max_norm >= 0.f)) return call_error(B2_ERR_INVALID, "%s: max_norm is negative or not a number", who);
-  if ((count && !tensors) || !norm || !workspace) return call_error(B2_ERR_INVALID, "%s: null pointer", who);
+  if ((count && (!x || !elements || !dtypes || (widths && (!ld_x || (out && !ld_out))))) || !norm || !workspace) return call_error(B2_ERR_INVALID, "%s: null pointer", who);
   if (reinterpret_cast<size_t>(norm) % 4) return call_error(B2_ERR_INVALID, "%s: norm is not aligned", who);
   if (reinterpret_cast<size_t>(workspace) % 256) return call_error(B2_ERR_INVALID, "%s: the workspace is not on a 256-byte boundary", who);
   try {
-    return clip_tensors(who, count, tensors, max_norm, norm, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+    return clip_tensors(who, ClipCall{count, x, out, elements, dtypes, widths, ld_x, ld_out}, max_norm, norm, workspace, workspace_bytes,
+                        static_cast<cudaStream_t>(stream));
   } catch (const std::exception&) {
     return call_error(B2_ERR_INVALID, "%s: no host memory for the list", who);
   }

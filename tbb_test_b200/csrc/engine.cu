@@ -1246,12 +1246,16 @@ int b2::call_error(int code, const char* fmt, ...) {
 }
 
 int b2::lm_device(int* sms) {
+  // asked for once per device: what it says does not change, and each question costs a caller of small operators some of its time
+  static std::atomic<int> known[64];
   int dev = 0, major = 0;
   cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && dev < 64 && (*sms = known[dev].load(std::memory_order_relaxed)) > 0) return B2_OK;
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return call_error(B2_ERR_CUDA, "no usable CUDA device: %s (there is no CPU path)", cudaGetErrorString(e));
   if (major != 10) return call_error(B2_ERR_UNSUPPORTED, "device %d has compute capability %d.x; the kernels are built for sm_100a", dev, major);
+  if (dev < 64) known[dev].store(*sms, std::memory_order_relaxed);
   return B2_OK;
 }
 

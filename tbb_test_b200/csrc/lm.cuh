@@ -4,6 +4,8 @@
 
 #include <stddef.h>
 
+#include <atomic>
+
 #include "../../include/b200mlp.h"
 #include "common.cuh"
 #include "overlap.h"
@@ -89,6 +91,19 @@ struct Chain {
   }
 };
 
+// Lets blocks of a kernel have `bytes` of dynamic shared memory on the current device; a caller asks for the most that any launch of the kernel needs. Once per device:
+// it takes as long as a launch.
+template <auto kernel>
+cudaError_t with_shared(int bytes) {
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && (done.load(std::memory_order_relaxed) >> dev & 1))) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return e;
+}
+
 // The widest vector (16, 8 or 4 bytes, or one element) that divides every one of the given addresses and byte counts.
 inline int vector_bytes(size_t elem, size_t bits) {
   for (int v = 16; v > (int)elem; v >>= 1)
@@ -108,15 +123,30 @@ struct Elems {
   static constexpr int N = BYTES / (int)sizeof(T);
   typedef typename Raw<BYTES>::type raw;
   static __device__ __forceinline__ void get(const raw& r, float (&f)[N]) {
-    const T* t = reinterpret_cast<const T*>(&r);
+    if constexpr (sizeof(T) == 2 && N > 1) {  // a bf16 is the upper half of its fp32: one instruction each
+      const unsigned int* t = reinterpret_cast<const unsigned int*>(&r);
 #pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = (float)t[i];
+      for (int i = 0; i < N; i += 2) {
+        f[i] = __uint_as_float(t[i / 2] << 16);
+        f[i + 1] = __uint_as_float(t[i / 2] & 0xFFFF0000u);
+      }
+    } else {
+      const T* t = reinterpret_cast<const T*>(&r);
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = (float)t[i];
+    }
   }
   static __device__ __forceinline__ raw put(const float (&f)[N]) {
     raw r;
-    T* t = reinterpret_cast<T*>(&r);
+    if constexpr (sizeof(T) == 2 && N > 1) {  // rounded two at a time
+      __nv_bfloat162* t = reinterpret_cast<__nv_bfloat162*>(&r);
 #pragma unroll
-    for (int i = 0; i < N; ++i) t[i] = (T)f[i];
+      for (int i = 0; i < N; i += 2) t[i / 2] = __floats2bfloat162_rn(f[i], f[i + 1]);
+    } else {
+      T* t = reinterpret_cast<T*>(&r);
+#pragma unroll
+      for (int i = 0; i < N; ++i) t[i] = (T)f[i];
+    }
     return r;
   }
 };

@@ -92,15 +92,24 @@ __device__ __forceinline__ float lanes_max(float m, int lanes) {
 
 __device__ __forceinline__ float scale_of(float largest) { return fmaxf(largest / E4M3_MAX, LEAST_SCALE); }
 
-// y / scale as e4m3: fp32's quotient rounded once more, which is off by more than half a step of e4m3 only within 2^-24 of a tie.
+// y / scale as e4m3: fp32's quotient rounded once more, which is off by more than half a step of e4m3 only within 2^-24 of a tie. The quotient is the product with
+// the reciprocal, mended by one step of Newton's, which a scale of infinity would make NaN of 0.
+struct Scaled {
+  float scale, inverse;
+  __device__ __forceinline__ explicit Scaled(float s) : scale(s < INFINITY ? s : 0.f), inverse(1.f / s) {}
+  __device__ __forceinline__ float of(float y) const {
+    const float q = y * inverse;
+    return fmaf(fmaf(-q, scale, y), inverse, q);
+  }
+};
 template <int N>
-__device__ __forceinline__ void store_e4m3(char* at, const float (&y)[N], float scale) {
-  unsigned char b[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) b[i] = __nv_cvt_float_to_fp8(y[i] / scale, __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ void store_e4m3(char* at, const float (&y)[N], const Scaled& s) {
   if constexpr (N == 1) {
-    *reinterpret_cast<unsigned char*>(at) = b[0];
+    *reinterpret_cast<unsigned char*>(at) = __nv_cvt_float_to_fp8(s.of(y[0]), __NV_SATFINITE, __NV_E4M3);
   } else {
+    unsigned short b[N / 2];
+#pragma unroll
+    for (int i = 0; i < N; i += 2) b[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(s.of(y[i]), s.of(y[i + 1])), __NV_SATFINITE, __NV_E4M3);
     typename Raw<N>::type r;
     memcpy(&r, b, N);
     *reinterpret_cast<typename Raw<N>::type*>(at) = r;
@@ -237,7 +246,7 @@ __global__ void __launch_bounds__(ROW_MOST_THREADS) norm_kernel(const NormArgs a
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = in_row + (k << g_log2);
-      if (c < vecs) store_e4m3(a.out + row * a.ld_out + (size_t)c * N, y[k], scale_of(largest[k]));
+      if (c < vecs) store_e4m3(a.out + row * a.ld_out + (size_t)c * N, y[k], Scaled(scale_of(largest[k])));
     }
   }
 }
@@ -309,11 +318,12 @@ __global__ void __launch_bounds__(ROW_MOST_THREADS) norm_long_kernel(const NormA
       }
       largest = a.block ? lanes_max(largest, 32) : whole;
       if (a.block && lane == 0) scales[b] = scale_of(largest);
+      const Scaled scaled(scale_of(largest));
 #pragma unroll
       for (int i = 0; i < PER_LANE; ++i) {
         const int c = b * (int)SCALE_BLOCK + i * 32 + lane;
         const float f[1] = {y[i]};
-        if (c < a.width) store_e4m3(out + c, f, scale_of(largest));
+        if (c < a.width) store_e4m3(out + c, f, scaled);
       }
     }
   }
@@ -358,72 +368,102 @@ struct GradRow {
   __device__ __forceinline__ float dx(float g, float n, float more) const { return rms.times(g - n * c) + more; }
 };
 
+// A block's groups take rows at distances of the grid, the next one's loads on their way while one is worked on; weights and the sums for the weight's gradient
+// stay in registers. K as small as a block of 256 threads allows: 8 elements per thread have room for three blocks per SM, 16 for two, and 32 for two without loads ahead.
+template <int K, int N, int MOST>
+constexpr int GRAD_PER_SM = MOST > NORM_THREADS ? 1 : K * N <= 8 ? 3 : 2;
+
 template <typename T, int VB, int K, int MOST>
-__global__ void __launch_bounds__(MOST, MOST > NORM_THREADS ? 1 : 2) norm_grad_kernel(const NormGradArgs a, int g_log2) {
+__global__ void __launch_bounds__(MOST, (GRAD_PER_SM<K, VB / (int)sizeof(T), MOST>)) norm_grad_kernel(const NormGradArgs a, int g_log2) {
   typedef Elems<T, VB> E;
   typedef typename E::raw raw;
   constexpr int N = E::N;
+  constexpr bool AHEAD = MOST <= NORM_THREADS && K * N <= 16;
   __shared__ double slots[2][2 * MOST / 32];
   extern __shared__ float sums[];  // a row of partial sums
   let_next_start();
   const int g = 1 << g_log2, in_row = threadIdx.x & (g - 1), sub = threadIdx.x >> g_log2, rows_here = blockDim.x >> g_log2;
   const int vecs = a.width / N;
-  float dw[K][N];
+  float dw[K][N], w[K][N];
 #pragma unroll
-  for (int k = 0; k < K; ++k)
+  for (int k = 0; k < K; ++k) {
+    const int c = in_row + (k << g_log2);
 #pragma unroll
-    for (int i = 0; i < N; ++i) dw[k][i] = 0.f;
-  int turn = 0;
-  for (size_t row0 = (size_t)blockIdx.x * rows_here; row0 < a.rows; row0 += (size_t)gridDim.x * rows_here, turn ^= 1) {
-    const size_t row = row0 + sub;
-    const bool active = row < a.rows;
+    for (int i = 0; i < N; ++i) dw[k][i] = w[k][i] = 0.f;
+    if (AHEAD && c < vecs) load_weight(a.weight, a.weight_f32, c * N, w[k]);
+  }
+  struct Row {
     raw t[K], d[K], m[K];
+  };
+  auto load = [&](Row& v, size_t row) {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = in_row + (k << g_log2);
-      memset(&t[k], 0, sizeof(raw));
-      memset(&d[k], 0, sizeof(raw));
-      memset(&m[k], 0, sizeof(raw));
-      if (active && c < vecs) {
-        t[k] = __ldg(reinterpret_cast<const raw*>(a.total + row * a.ld_total) + c);
-        d[k] = __ldg(reinterpret_cast<const raw*>(a.dy + row * a.ld_dy) + c);
-        if (a.dtotal) m[k] = __ldg(reinterpret_cast<const raw*>(a.dtotal + row * a.ld_dtotal) + c);
+      memset(&v.t[k], 0, sizeof(raw));
+      memset(&v.d[k], 0, sizeof(raw));
+      memset(&v.m[k], 0, sizeof(raw));
+      if (row < a.rows && c < vecs) {
+        v.t[k] = __ldg(reinterpret_cast<const raw*>(a.total + row * a.ld_total) + c);
+        v.d[k] = __ldg(reinterpret_cast<const raw*>(a.dy + row * a.ld_dy) + c);
+        if (a.dtotal) v.m[k] = __ldg(reinterpret_cast<const raw*>(a.dtotal + row * a.ld_dtotal) + c);
       }
     }
+  };
+  int turn = 0;
+  const size_t step = (size_t)gridDim.x * rows_here;
+  Row now, next;
+  if (AHEAD) load(now, (size_t)blockIdx.x * rows_here + sub);
+  for (size_t row0 = (size_t)blockIdx.x * rows_here; row0 < a.rows; row0 += step, turn ^= 1) {
+    const size_t row = row0 + sub;
+    if (AHEAD) load(next, row + step);
+    else load(now, row);
     double s[2] = {0.0, 0.0};
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = in_row + (k << g_log2);
-      float f[N], h[N], w[N];
-      E::get(t[k], f);
-      E::get(d[k], h);
+      float f[N], h[N];
+      E::get(now.t[k], f);
+      E::get(now.d[k], h);
       if (c < vecs) {
-        load_weight(a.weight, a.weight_f32, c * N, w);
+        if (!AHEAD) load_weight(a.weight, a.weight_f32, c * N, w[k]);
 #pragma unroll
-        for (int i = 0; i < N; ++i) h[i] *= w[i];
+        for (int i = 0; i < N; ++i) h[i] *= w[k][i];
         add_squares(f, s[0]);
         add_products(h, f, s[1]);
       }
     }
     row_sums(s, g_log2, slots[turn]);
     const GradRow r(s, a.width, a.eps);
+    if (row < a.rows) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = in_row + (k << g_log2);
-      if (!active || c >= vecs) break;
-      float f[N], h[N], w[N], o[N];
-      E::get(t[k], f);
-      E::get(d[k], h);
-      E::get(m[k], o);
-      load_weight(a.weight, a.weight_f32, c * N, w);
+      for (int k = 0; k < K; ++k) {
+        const int c = in_row + (k << g_log2);
+        if (c >= vecs) break;
+        float f[N], h[N], o[N];
+        E::get(now.t[k], f);
+        E::get(now.d[k], h);
+        E::get(now.m[k], o);
+        if (!AHEAD) load_weight(a.weight, a.weight_f32, c * N, w[k]);
+        if (!r.rms.far) {
+          const float rr = (float)r.rms.r;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float n = r.rms.times(f[i]);
-        dw[k][i] = fmaf(h[i], n, dw[k][i]);
-        o[i] = r.dx(h[i] * w[i], n, o[i]);
+          for (int i = 0; i < N; ++i) {
+            const float n = f[i] * rr;
+            dw[k][i] = fmaf(h[i], n, dw[k][i]);
+            o[i] = fmaf(rr, h[i] * w[k][i] - n * r.c, o[i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const float n = r.rms.times(f[i]);
+            dw[k][i] = fmaf(h[i], n, dw[k][i]);
+            o[i] = r.dx(h[i] * w[k][i], n, o[i]);
+          }
+        }
+        reinterpret_cast<raw*>(a.dx + row * a.ld_dx)[c] = E::put(o);
       }
-      reinterpret_cast<raw*>(a.dx + row * a.ld_dx)[c] = E::put(o);
     }
+    if (AHEAD) now = next;
   }
   after_previous();
   if (!a.partial) return;
@@ -442,22 +482,26 @@ __global__ void __launch_bounds__(MOST, MOST > NORM_THREADS ? 1 : 2) norm_grad_k
   for (int c = threadIdx.x; c < a.width; c += blockDim.x) a.partial[(size_t)blockIdx.x * a.width + c] = sums[c];
 }
 
-// dweight[c] = sum of `count` partial sums, in order: 32 columns per block, a warp for every 8th partial sum.
-constexpr int JOIN_WARPS = 8;
+// dweight[c] = sum of `count` partial sums: 32 columns per block, a warp for every 32nd partial sum, and the warps' sums in order.
+constexpr int JOIN_WARPS = 32;
 __global__ void __launch_bounds__(JOIN_WARPS * 32) norm_join_kernel(const float* __restrict__ partial, int count, int width, void* dweight, int f32) {
-  __shared__ float part[JOIN_WARPS][32];
+  __shared__ float part[JOIN_WARPS][33];
   after_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float s = 0.f;
-  if (c < width)
+  if (c < width) {
+#pragma unroll 8
     for (int i = warp; i < count; i += JOIN_WARPS) s += partial[(size_t)i * width + c];
+  }
   part[warp][lane] = s;
   __syncthreads();
-  if (warp || c >= width) return;
-#pragma unroll
-  for (int i = 1; i < JOIN_WARPS; ++i) s += part[i][lane];
-  if (f32) static_cast<float*>(dweight)[c] = s;
-  else static_cast<__nv_bfloat16*>(dweight)[c] = (__nv_bfloat16)s;
+  // a warp per column of the first
+  s = part[lane][warp];
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+  const int mine = blockIdx.x * 32 + warp;
+  if (lane || mine >= width) return;
+  if (f32) static_cast<float*>(dweight)[mine] = s;
+  else static_cast<__nv_bfloat16*>(dweight)[mine] = (__nv_bfloat16)s;
 }
 
 // Long rows: dx by a block per row, which leaves r; then sums by columns over slices of rows.
@@ -556,47 +600,48 @@ void norm_by_vector(const NormArgs& a, int vb, int sms, Chain& chain) {
   else if constexpr (sizeof(T) == 2) norm_launch<T, 2, E4M3>(a, sms, chain);
 }
 
-// Blocks of the gradient's kernels, as for 148 SMs at most, so that the workspace does not depend on the device: two per SM of up to 256 threads, one
-// of more, and slices of rows where a row takes more than a block's registers (from 4097 columns on, by alignment).
-constexpr int GRAD_BLOCKS = 296, GRAD_WIDE_BLOCKS = 148, COLUMN_SLICES = 64;
-constexpr size_t GRAD_WIDTH = (size_t)NORM_THREADS * 32, GRAD_WIDE_WIDTH = (size_t)ROW_MOST_THREADS * 16, GRAD_LEAST_LONG = 4097;
+// Blocks of the gradient's kernels, as for 148 SMs at most, so that the workspace does not depend on the device, and slices of rows where a row takes more than a
+// block's registers (from 4097 columns on, by alignment).
+constexpr int SMS_MOST = 148, COLUMN_SLICES = 64;
+constexpr size_t GRAD_LEAST_LONG = 4097, GRAD_WIDTH_MOST = (size_t)ROW_MOST_THREADS * 16;
 constexpr size_t ROWS_MOST = (size_t)1 << 31, WIDTH_MOST = (size_t)1 << 20;
 
 size_t grad_space(size_t rows, size_t width, void* base, float** partial, double** rms_of) {
   Carver c(base);
-  *partial = c.take<float>((width <= GRAD_WIDTH ? GRAD_BLOCKS : width <= GRAD_WIDE_WIDTH ? GRAD_WIDE_BLOCKS : COLUMN_SLICES) * width);
+  const size_t per_sm = width <= NORM_THREADS * 8 ? 3 : 2;
+  const size_t blocks = width <= NORM_THREADS * 32 ? SMS_MOST * per_sm : width <= GRAD_WIDTH_MOST ? SMS_MOST : COLUMN_SLICES;
+  *partial = c.take<float>((blocks > COLUMN_SLICES ? blocks : COLUMN_SLICES) * width);
   *rms_of = c.take<double>(width >= GRAD_LEAST_LONG ? rows : 0);
   return c.used;
+}
+
+template <typename T, int VB, int K, int MOST>
+int grad_rows(const NormGradArgs& a, const RowForm& f, int sms, Chain& chain) {
+  constexpr int PER_SM = GRAD_PER_SM<K, VB / (int)sizeof(T), MOST>;
+  const size_t here = f.threads >> f.g_log2, blocks = (a.rows + here - 1) / here, most = (size_t)(sms < SMS_MOST ? sms : SMS_MOST) * PER_SM;
+  const int parts = (int)(blocks < most ? blocks : most);
+  const size_t smem = a.partial ? (size_t)a.width * 4 : 0;
+  if (smem > 40 * 1024) chain.err = with_shared<norm_grad_kernel<T, VB, K, MOST>>((int)GRAD_WIDTH_MOST * 4);
+  chain.launch(norm_grad_kernel<T, VB, K, MOST>, dim3(parts), f.threads, smem, 0, a, f.g_log2);
+  return parts;
 }
 
 template <typename T, int VB>
 void norm_grad_launch(const NormGradArgs& a, double* rms_of, void* dweight, int sms, Chain& chain) {
   constexpr int N = VB / (int)sizeof(T), MOST_K = N >= 8 ? 4 : 8;
   // 1024 threads have 64 registers each: half as many elements
-  RowForm f = row_form(a.rows, a.width / N, MOST_K, 1, NORM_THREADS, (size_t)sms * 1024);
-  if (!f.k) f = row_form(a.rows, a.width / N, MOST_K / 2, 1, ROW_MOST_THREADS, 0);
-  int parts;
-  if (f.k) {
-    const size_t here = f.threads >> f.g_log2, blocks = (a.rows + here - 1) / here;
-    size_t most = (size_t)sms * (f.threads > NORM_THREADS ? 1 : 2);
-    const size_t room = f.threads > NORM_THREADS ? GRAD_WIDE_BLOCKS : GRAD_BLOCKS;
-    if (most > room) most = room;
-    parts = (int)(blocks < most ? blocks : most);
-    const size_t smem = a.partial ? (size_t)a.width * 4 : 0;
-    auto go = [&](auto kernel) {
-      if (chain.err == cudaSuccess && smem > 40 * 1024) chain.err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-      chain.launch(kernel, dim3(parts), f.threads, smem, 0, a, f.g_log2);
-    };
-    if (f.threads > NORM_THREADS) {
-      if (f.k == 1) go(norm_grad_kernel<T, VB, 1, ROW_MOST_THREADS>);
-      else if (f.k == 2) go(norm_grad_kernel<T, VB, 2, ROW_MOST_THREADS>);
-      else if constexpr (MOST_K == 8) go(norm_grad_kernel<T, VB, 4, ROW_MOST_THREADS>);
-    } else {
-      if (f.k == 1) go(norm_grad_kernel<T, VB, 1, NORM_THREADS>);
-      else if (f.k == 2) go(norm_grad_kernel<T, VB, 2, NORM_THREADS>);
-      else if (f.k == 4) go(norm_grad_kernel<T, VB, 4, NORM_THREADS>);
-      else if constexpr (MOST_K == 8) go(norm_grad_kernel<T, VB, 8, NORM_THREADS>);
-    }
+  RowForm f = row_form(1, a.width / N, MOST_K, 1, NORM_THREADS, NORM_THREADS);
+  if (!f.k) f = row_form(1, a.width / N, MOST_K / 2, 1, ROW_MOST_THREADS, 0);
+  int parts = 0;
+  if (f.k && f.threads > NORM_THREADS) {
+    if (f.k == 1) parts = grad_rows<T, VB, 1, ROW_MOST_THREADS>(a, f, sms, chain);
+    else if (f.k == 2) parts = grad_rows<T, VB, 2, ROW_MOST_THREADS>(a, f, sms, chain);
+    else if constexpr (MOST_K == 8) parts = grad_rows<T, VB, 4, ROW_MOST_THREADS>(a, f, sms, chain);
+  } else if (f.k) {
+    if (f.k == 1) parts = grad_rows<T, VB, 1, NORM_THREADS>(a, f, sms, chain);
+    else if (f.k == 2) parts = grad_rows<T, VB, 2, NORM_THREADS>(a, f, sms, chain);
+    else if (f.k == 4) parts = grad_rows<T, VB, 4, NORM_THREADS>(a, f, sms, chain);
+    else if constexpr (MOST_K == 8) parts = grad_rows<T, VB, 8, NORM_THREADS>(a, f, sms, chain);
   } else {
     parts = a.rows < COLUMN_SLICES ? (int)a.rows : COLUMN_SLICES;
     chain.launch(norm_grad_long_kernel<T>, dim3((unsigned int)a.rows), ROW_MOST_THREADS, 0, 0, a, rms_of);

@@ -1307,7 +1307,7 @@ cudaError_t sample_rows(const SampleArgs& a, size_t rows, bool limits, int sms, 
     chain.launch(sample_whole_kernel<T, true>, dim3(blocks < some ? blocks : some), WHOLE_THREADS, 0, 0, a, rows);
     return chain.err;
   }
-  chain.err = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SampleShared<T>));
+  chain.err = with_shared<sample_kernel<T>>((int)sizeof(SampleShared<T>));
   chain.launch(sample_tiles_kernel<T>, dim3((unsigned int)((all * 32 + TILE_THREADS - 1) / TILE_THREADS)), TILE_THREADS, 0, 0, a, all);
   chain.launch(sample_kernel<T>, dim3((unsigned int)rows), SAMPLE_THREADS, sizeof(SampleShared<T>), 0, a);
   return chain.err;

@@ -59,7 +59,7 @@ def _matrix(name, x, dtype=None, shape=None, device=None):
 def _result(name, x, rows, cols, dtype, device):
     """(tensor, address, leading dimension) of a result: the given one, checked, or a new one."""
     if x is None:
-        x = torch.empty(rows, cols, dtype=dtype, device=device)
+        x = torch.empty((rows, cols), dtype=dtype, device=device)
         return x, x.data_ptr(), cols
     return (x, *_matrix(name, x, dtype, (rows, cols), device))
 
@@ -89,7 +89,10 @@ def _workspace(device, entry, *sizes):
 
 def _changed(tensors):
     """Given tensors that a call has written to: counted as changed in place where autograd keeps count."""
-    torch.autograd.graph.increment_version([x for x in tensors if not x.is_inference()])
+    try:
+        torch.autograd.graph.increment_version(tensors)
+    except RuntimeError:  # some were made in inference mode, which keeps no count; counting the others twice does no harm
+        torch.autograd.graph.increment_version([x for x in tensors if not x.is_inference()])
 
 
 class _on:
@@ -260,19 +263,27 @@ def norm_grad(dy, t, weight=None, dtotal=None, eps=1e-6, dx=None):
     return dx if dw is None else (dx, dw)
 
 
-def _rows_of(name, x, device):
-    """(rows, cols, distance of rows) of a tensor as b2_clip takes it: one row where it lies in memory without gaps, whatever its shape."""
-    if x.is_contiguous():
-        return 1, x.numel(), 0
+def _rows_of(name, x):
+    """(width, distance of rows) of a tensor that is not contiguous, as b2_clip takes it: a matrix with gaps, or (elements, elements) where it lies in memory without gaps
+    in another order."""
+    n = x.numel()
     if x.dim() == 2 and (x.shape[1] == 1 or x.stride(1) == 1) and x.stride(0) >= x.shape[1]:
-        return x.shape[0], x.shape[1], x.stride(0)
-    sides = sorted((s, n) for n, s in zip(x.shape, x.stride()) if n != 1)
+        return x.shape[1], x.stride(0)
     at = 1
-    for s, n in sides:
-        if s != at:
+    for stride, size in sorted((s, k) for k, s in zip(x.shape, x.stride()) if k != 1):
+        if stride != at:
             raise ValueError(f"{name}: neither dense nor a matrix with unit stride along its rows")
-        at *= n
-    return 1, x.numel(), 0
+        at *= size
+    return n, n
+
+
+def _same(name, xs, device):
+    """Whether all are contiguous; refuses what is not a float32 or bfloat16 tensor of the device."""
+    if not all(isinstance(x, torch.Tensor) for x in xs) or {x.get_device() for x in xs} != {device.index} or not device.type == "cuda":
+        raise ValueError(f"{name}: tensors on one CUDA device are wanted")
+    if not {x.dtype for x in xs} <= _DTYPES.keys():
+        raise ValueError(f"{name}: float32 or bfloat16 is wanted")
+    return all([x.is_contiguous() for x in xs])
 
 
 def clip(tensors, max_norm, out=None):
@@ -281,42 +292,44 @@ def clip(tensors, max_norm, out=None):
     norm alone. A norm that is infinite or not a number leaves the values as they are. float32 and bfloat16 tensors of any sizes, each dense
     or a matrix with unit stride along its rows, all on one device; none may overlap another (see b2_clip in include/b200mlp.h)."""
     xs = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    if not xs:
-        raise ValueError("tensors: none")
+    if not xs or not isinstance(xs[0], torch.Tensor):
+        raise ValueError("tensors: none" if not xs else "tensors: tensors are wanted")
     limited = max_norm is not None and max_norm != math.inf
-    ys = xs if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
-    if not limited and out is not None:
-        raise ValueError("out goes with a limit")
     if limited and not max_norm >= 0:
         raise ValueError(f"max_norm: {max_norm}")
-    if len(ys) != len(xs):
-        raise ValueError(f"out: {len(ys)} tensors for {len(xs)}")
-    device = xs[0].device if isinstance(xs[0], torch.Tensor) else None
-    for name, zs in (("tensors", xs), ("out", ys)) if out is not None else (("tensors", xs),):
-        for i, x in enumerate(zs):
-            if not isinstance(x, torch.Tensor) or not x.is_cuda or x.device != device:
-                raise ValueError(f"{name}[{i}]: on one CUDA device with the others is wanted")
-            if x.dtype not in _DTYPES or x.dtype != xs[i].dtype or x.shape != xs[i].shape:
-                raise ValueError(f"{name}[{i}]: {x.dtype} of shape {tuple(x.shape)}, wanted float32 or bfloat16, and out like tensors")
-    table = array.array("Q")
-    for i, (x, y) in enumerate(zip(xs, ys)):
-        rows, cols, ldx = _rows_of(f"tensors[{i}]", x, device)
-        ldy = ldx
-        if y is not x:
-            rows_y, cols_y, ldy = _rows_of(f"out[{i}]", y, device)
-            if x.stride() != y.stride():
-                if rows == 1 and not x.is_contiguous() or rows_y == 1 and not y.is_contiguous():
-                    raise ValueError(f"out[{i}]: elements lie in another order than in tensors[{i}]")
-                if rows != rows_y:  # one of them has gaps between its rows
-                    rows, cols = max(rows, rows_y), min(cols, cols_y)
-                    ldx, ldy = ldx or cols, ldy or cols
-        table.extend((x.data_ptr(), y.data_ptr(), rows, cols, ldx, ldy, _DTYPES[x.dtype]))
+    device = xs[0].device
+    dense = _same("tensors", xs, device)
+    elements = [x.numel() for x in xs]
+    ys = None
+    if out is not None:
+        ys = [out] if isinstance(out, torch.Tensor) else list(out)
+        if not limited:
+            raise ValueError("out goes with a limit")
+        if len(ys) != len(xs):
+            raise ValueError(f"out: {len(ys)} tensors for {len(xs)}")
+        dense = _same("out", ys, device) and dense
+        if any(x.shape != y.shape or x.dtype != y.dtype for x, y in zip(xs, ys)):
+            raise ValueError("out: shapes and types like those of tensors are wanted")
+    q = lambda v: array.array("Q", v)  # noqa: E731
+    widths = ld_x = ld_y = None
+    if not dense:
+        rows = [(n, n) if x.is_contiguous() else _rows_of(f"tensors[{i}]", x) for i, (x, n) in enumerate(zip(xs, elements))]
+        rows_y = rows if ys is None else [(n, n) if y.is_contiguous() else _rows_of(f"out[{i}]", y) for i, (y, n) in enumerate(zip(ys, elements))]
+        for i, (n, (a, _), (b, _)) in enumerate(zip(elements, rows, rows_y)):
+            if ys is not None and xs[i].stride() != ys[i].stride() and (a == n and not xs[i].is_contiguous() or b == n and not ys[i].is_contiguous()) and n > 1:
+                raise ValueError(f"out[{i}]: elements lie in another order than in tensors[{i}]")
+        width = [min(a, b) for (a, _), (b, _) in zip(rows, rows_y)]
+        widths, ld_x, ld_y = q(width), q([ld if a == k else k for k, (a, ld) in zip(width, rows)]), q([ld if b == k else k for k, (b, ld) in zip(width, rows_y)])
+    px, py, sizes = q([x.data_ptr() for x in xs]), None if ys is None else q([y.data_ptr() for y in ys]), q(elements)
+    types = array.array("i", [_DTYPES[x.dtype] for x in xs])
+    at = lambda v: None if v is None else v.buffer_info()[0]  # noqa: E731
     norm = torch.empty((), dtype=torch.float32, device=device)
     with _on(device) as stream:
         ws = _workspace(device, "clip", len(xs))
-        _ck(K.lib().b2_clip(len(xs), table.buffer_info()[0], max_norm if limited else math.inf, norm.data_ptr(), ws.data_ptr(), ws.numel(), stream))
+        _ck(K.lib().b2_clip(len(xs), at(px), at(py), at(sizes), at(types), at(widths), at(ld_x), at(ld_y), max_norm if limited else math.inf, norm.data_ptr(),
+                            ws.data_ptr(), ws.numel(), stream))
     if limited:
-        _changed(ys)
+        _changed(xs if ys is None else ys)
     return norm
 
 

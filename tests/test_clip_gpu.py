@@ -201,16 +201,14 @@ def test_c_entry_refuses_before_any_device_work(native):
     from tbb_test_b200 import _capi as K
     lib = K.lib()
     p = ct.c_void_p
-
-    def tensors(**kw):
-        good = dict(x=256, out=256, rows=2, cols=8, ld_x=8, ld_out=8, dtype=0)
-        return (K.ClipTensor * 2)(K.ClipTensor(*good.values()), K.ClipTensor(*{**good, "x": 4096, "out": 4096, **kw}.values()))
-
-    good = dict(count=2, tensors=tensors(), max_norm=1.0, norm=p(1 << 16), ws=p(1 << 20), ws_bytes=1 << 20, stream=None)
-    for kw in (dict(count=(1 << 20) + 1), dict(tensors=None), dict(max_norm=-1.0), dict(max_norm=math.nan), dict(norm=None), dict(norm=p(2)), dict(ws=None), dict(ws=p(64)),
-               dict(ws_bytes=16), dict(tensors=tensors(dtype=2)), dict(tensors=tensors(x=None)), dict(tensors=tensors(out=None)), dict(tensors=tensors(x=4098)),
-               dict(tensors=tensors(out=4098)), dict(tensors=tensors(ld_x=7)), dict(tensors=tensors(ld_out=7)), dict(tensors=tensors(cols=(1 << 42) + 1)),
-               dict(tensors=tensors(rows=1 << 60, cols=1 << 60)), dict(tensors=tensors(out=1 << 30), max_norm=math.inf)):
+    ptr = lambda *v: (ct.c_void_p * 2)(*v)  # noqa: E731
+    num = lambda *v: (ct.c_size_t * 2)(*v)  # noqa: E731
+    good = dict(count=2, x=ptr(256, 4096), out=ptr(256, 4096), elements=num(16, 16), dtypes=(ct.c_int * 2)(0, 0), widths=num(8, 8), ld_x=num(8, 8), ld_out=num(8, 8),
+                max_norm=1.0, norm=p(1 << 16), ws=p(1 << 20), ws_bytes=1 << 20, stream=None)
+    for kw in (dict(count=(1 << 20) + 1), dict(x=None), dict(elements=None), dict(dtypes=None), dict(ld_x=None), dict(ld_out=None), dict(max_norm=-1.0), dict(max_norm=math.nan),
+               dict(norm=None), dict(norm=p(2)), dict(ws=None), dict(ws=p(64)), dict(ws_bytes=16), dict(dtypes=(ct.c_int * 2)(0, 2)), dict(x=ptr(256, None)),
+               dict(out=ptr(256, None)), dict(x=ptr(256, 4098)), dict(out=ptr(256, 4098)), dict(ld_x=num(8, 7)), dict(ld_out=num(8, 7)), dict(widths=num(8, 5)),
+               dict(widths=num(8, 0)), dict(elements=num(16, (1 << 42) + 1)), dict(elements=num(1 << 41, (1 << 41) + 8)), dict(max_norm=math.inf)):
         assert lib.b2_clip(*{**good, **kw}.values()) == K.ERR_INVALID, kw
         assert lib.b2_last_error(None)
     need = ct.c_size_t()

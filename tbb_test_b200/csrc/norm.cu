@@ -26,18 +26,24 @@ struct NormArgs {
   size_t rows;
   int width, weight_f32, block;
   float eps;
+  double inverse_width;
 };
 
-// 1 / sqrt(mean + eps), and whether products with it have to be taken in fp64: outside this range r or t r leaves fp32's.
+// 1 / sqrt(mean + eps), and whether products with it have to be taken in fp64: outside this range r or t r leaves fp32's. The approximate root's reciprocal and a step of
+// Newton's are as near as a rounded root and a rounded quotient, in a quarter of the instructions.
 struct Rms {
-  double r;
+  double wide;
+  float r;
   bool far;
-  __device__ __forceinline__ Rms(double squares, int width, float eps) {
-    const double m = squares / width + (double)eps;
+  __device__ __forceinline__ Rms(double mean, float eps) {
+    const double m = mean + (double)eps;
     far = !(m > 1e-36 && m < 1e36);
-    r = far ? 1.0 / sqrt(m) : (double)(1.f / sqrtf((float)m));
+    const float f = (float)m, x = rsqrtf(f);
+    r = fmaf(0.5f * x, fmaf(-f * x, x, 1.f), x);
+    wide = 0.0;
+    if (far) wide = 1.0 / sqrt(m);
   }
-  __device__ __forceinline__ float times(float t) const { return far ? (float)(t * r) : t * (float)r; }
+  __device__ __forceinline__ float times(float t) const { return far ? (float)(t * wide) : t * r; }
 };
 
 // N consecutive weights from column `col`.
@@ -90,13 +96,17 @@ __device__ __forceinline__ float lanes_max(float m, int lanes) {
   return m;
 }
 
-__device__ __forceinline__ float scale_of(float largest) { return fmaxf(largest / E4M3_MAX, LEAST_SCALE); }
+// largest / 448: the product with 1 / 448, mended by a step of Newton's (which would make NaN of infinity)
+__device__ __forceinline__ float scale_of(float largest) {
+  const float q = largest * (1.f / E4M3_MAX), s = fmaf(fmaf(-q, E4M3_MAX, largest), 1.f / E4M3_MAX, q);
+  return fmaxf(largest < INFINITY ? s : largest, LEAST_SCALE);
+}
 
 // y / scale as e4m3: fp32's quotient rounded once more, which is off by more than half a step of e4m3 only within 2^-24 of a tie. The quotient is the product with
 // the reciprocal, mended by one step of Newton's, which a scale of infinity would make NaN of 0.
 struct Scaled {
   float scale, inverse;
-  __device__ __forceinline__ explicit Scaled(float s) : scale(s < INFINITY ? s : 0.f), inverse(1.f / s) {}
+  __device__ __forceinline__ explicit Scaled(float s) : scale(s < INFINITY ? s : 0.f) { asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(s)); }
   __device__ __forceinline__ float of(float y) const {
     const float q = y * inverse;
     return fmaf(fmaf(-q, scale, y), inverse, q);
@@ -168,7 +178,7 @@ __global__ void __launch_bounds__(ROW_MOST_THREADS) norm_kernel(const NormArgs a
     add_squares(f, s[0]);
   }
   row_sums(s, g_log2, slots);
-  const Rms rms(s[0], a.width, a.eps);
+  const Rms rms(s[0] * a.inverse_width, a.eps);
   if constexpr (!E4M3) {
     if (!active) return;
     raw* out = reinterpret_cast<raw*>(a.out + row * a.ld_out);
@@ -179,8 +189,13 @@ __global__ void __launch_bounds__(ROW_MOST_THREADS) norm_kernel(const NormArgs a
       float f[N], w[N];
       E::get(v[k], f);
       load_weight(a.weight, a.weight_f32, c * N, w);
+      if (!rms.far) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = rms.times(f[i]) * w[i];
+        for (int i = 0; i < N; ++i) f[i] = f[i] * rms.r * w[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = rms.times(f[i]) * w[i];
+      }
       out[c] = E::put(f);
     }
   } else {
@@ -195,11 +210,15 @@ __global__ void __launch_bounds__(ROW_MOST_THREADS) norm_kernel(const NormArgs a
       largest[k] = 0.f;
       if (c < vecs) {
         load_weight(a.weight, a.weight_f32, c * N, w);
+        if (!rms.far) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          y[k][i] = rms.times(y[k][i]) * w[i];
-          largest[k] = fmaxf(largest[k], fabsf(y[k][i]));
+          for (int i = 0; i < N; ++i) y[k][i] = y[k][i] * rms.r * w[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) y[k][i] = rms.times(y[k][i]) * w[i];
         }
+#pragma unroll
+        for (int i = 0; i < N; ++i) largest[k] = fmaxf(largest[k], fabsf(y[k][i]));
       }
       whole = fmaxf(whole, largest[k]);
     }
@@ -293,7 +312,7 @@ __global__ void __launch_bounds__(ROW_MOST_THREADS) norm_long_kernel(const NormA
     add_squares(f, s[0]);
   }
   row_sums(s, 10, slots);
-  const Rms rms(s[0], a.width, a.eps);
+  const Rms rms(s[0] * a.inverse_width, a.eps);
   if constexpr (!E4M3) {
     T* out = reinterpret_cast<T*>(a.out + row * a.ld_out);
     for (int c = threadIdx.x; c < a.width; c += blockDim.x) out[c] = (T)(rms.times(in.sum(c)) * in.scale(c));
@@ -339,6 +358,7 @@ struct NormGradArgs {
   size_t rows;
   int width, weight_f32;
   float eps;
+  double inverse_width;
 };
 
 // sum += f * h, as add_squares() does.
@@ -364,7 +384,8 @@ __device__ __forceinline__ void add_products(const float (&f)[N], const float (&
 struct GradRow {
   Rms rms;
   float c;
-  __device__ __forceinline__ GradRow(const double (&s)[2], int width, float eps) : rms(s[0], width, eps), c((float)(rms.r * (s[1] / width))) {}
+  __device__ __forceinline__ GradRow(const double (&s)[2], double inverse_width, float eps)
+      : rms(s[0] * inverse_width, eps), c((float)((rms.far ? rms.wide : (double)rms.r) * (s[1] * inverse_width))) {}
   __device__ __forceinline__ float dx(float g, float n, float more) const { return rms.times(g - n * c) + more; }
 };
 
@@ -433,7 +454,7 @@ __global__ void __launch_bounds__(MOST, (GRAD_PER_SM<K, VB / (int)sizeof(T), MOS
       }
     }
     row_sums(s, g_log2, slots[turn]);
-    const GradRow r(s, a.width, a.eps);
+    const GradRow r(s, a.inverse_width, a.eps);
     if (row < a.rows) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
@@ -445,7 +466,7 @@ __global__ void __launch_bounds__(MOST, (GRAD_PER_SM<K, VB / (int)sizeof(T), MOS
         E::get(now.m[k], o);
         if (!AHEAD) load_weight(a.weight, a.weight_f32, c * N, w[k]);
         if (!r.rms.far) {
-          const float rr = (float)r.rms.r;
+          const float rr = r.rms.r;
 #pragma unroll
           for (int i = 0; i < N; ++i) {
             const float n = f[i] * rr;
@@ -521,8 +542,8 @@ __global__ void __launch_bounds__(ROW_MOST_THREADS) norm_grad_long_kernel(const 
     add_products(h, f, s[1]);
   }
   row_sums(s, 10, slots);
-  const GradRow r(s, a.width, a.eps);
-  if (threadIdx.x == 0 && rms_of) rms_of[row] = r.rms.far ? -r.rms.r : r.rms.r;
+  const GradRow r(s, a.inverse_width, a.eps);
+  if (threadIdx.x == 0 && rms_of) rms_of[row] = r.rms.far ? -r.rms.wide : (double)r.rms.r;
   for (int c = threadIdx.x; c < a.width; c += blockDim.x)
     dx[c] = (T)r.dx((float)dy[c] * in.scale(c), r.rms.times(in.sum(c)), more ? (float)more[c] : 0.f);
   after_previous();
@@ -630,7 +651,8 @@ template <typename T, int VB>
 void norm_grad_launch(const NormGradArgs& a, double* rms_of, void* dweight, int sms, Chain& chain) {
   constexpr int N = VB / (int)sizeof(T), MOST_K = N >= 8 ? 4 : 8;
   // 1024 threads have 64 registers each: half as many elements
-  RowForm f = row_form(1, a.width / N, MOST_K, 1, NORM_THREADS, NORM_THREADS);
+  RowForm f = row_form(1, a.width / N, 2, 1, NORM_THREADS, 0);
+  if (!f.k) f = row_form(1, a.width / N, MOST_K, 1, NORM_THREADS, 0);
   if (!f.k) f = row_form(1, a.width / N, MOST_K / 2, 1, ROW_MOST_THREADS, 0);
   int parts = 0;
   if (f.k && f.threads > NORM_THREADS) {
@@ -710,6 +732,7 @@ int b2_norm(size_t rows, size_t width, int dtype, const void* x, size_t ld_x, co
   a.weight_f32 = weight_dtype == B2_DTYPE_F32;
   a.block = (int)block;
   a.eps = eps;
+  a.inverse_width = 1.0 / (double)width;
   size_t bits = address(x) | a.ld_x | width * e;
   if (residual) bits |= address(residual) | a.ld_residual;
   if (total) bits |= address(total) | a.ld_total;
@@ -778,6 +801,7 @@ int b2_norm_grad(size_t rows, size_t width, int dtype, const void* dy, size_t ld
   a.width = (int)width;
   a.weight_f32 = weight_dtype == B2_DTYPE_F32;
   a.eps = eps;
+  a.inverse_width = 1.0 / (double)width;
   size_t bits = address(dy) | a.ld_dy | address(total) | a.ld_total | address(dx) | a.ld_dx | width * e;
   if (dtotal) bits |= address(dtotal) | a.ld_dtotal;
   const int vb = norm_vector(e, bits, weight, we);

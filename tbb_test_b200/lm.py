@@ -37,6 +37,9 @@ def _ck(rc):
 
 def _matrix(name, x, dtype=None, shape=None, device=None):
     """(address, leading dimension) of a two-dimensional CUDA tensor with unit stride along its rows."""
+    if isinstance(x, torch.Tensor) and x.dim() == 2 and x.is_contiguous() and (x.is_cuda if device is None else x.device == device) and (
+            x.dtype in _DTYPES if dtype is None else x.dtype == dtype) and (shape is None or x.shape == shape):
+        return x.data_ptr(), x.shape[1]  # what most callers give
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         raise ValueError(f"{name}: a two-dimensional tensor is wanted")
     if not x.is_cuda or (device is not None and x.device != device):
@@ -56,12 +59,22 @@ def _matrix(name, x, dtype=None, shape=None, device=None):
     return x.data_ptr(), between
 
 
-def _result(name, x, rows, cols, dtype, device):
-    """(tensor, address, leading dimension) of a result: the given one, checked, or a new one."""
+def _result(name, x, rows, cols, dtype, device, like=None):
+    """(tensor, address, leading dimension) of a result: the given one, checked, or a new one. like: a matrix of its shape and type, if there is one."""
     if x is None:
-        x = torch.empty((rows, cols), dtype=dtype, device=device)
+        x = _new(device, dtype, rows, cols) if like is None or not like.is_contiguous() else torch.empty_like(like)
         return x, x.data_ptr(), cols
     return (x, *_matrix(name, x, dtype, (rows, cols), device))
+
+
+@functools.lru_cache(maxsize=256)
+def _template(device, dtype):
+    """A tensor without elements: new ones made from it take half the time of torch.empty's with a type and a device."""
+    return torch.empty(0, dtype=dtype, device=device)
+
+
+def _new(device, dtype, *shape):
+    return _template(device, dtype).new_empty(shape)
 
 
 def _tokens(name, t, device):
@@ -84,7 +97,7 @@ def _workspace_bytes(entry, *sizes):
 
 def _workspace(device, entry, *sizes):
     """Device memory from torch's allocator, which hands it out again only behind this stream's work."""
-    return torch.empty(_workspace_bytes(entry, *sizes), dtype=torch.uint8, device=device)
+    return _new(device, torch.uint8, _workspace_bytes(entry, *sizes))
 
 
 def _changed(tensors):
@@ -104,7 +117,7 @@ class _on:
         self.index = device.index
 
     def __enter__(self):
-        self.before = torch.cuda.current_device()
+        self.before = torch._C._cuda_getDevice()
         if self.index != self.before:
             torch.cuda.set_device(self.index)
         return torch._C._cuda_getCurrentRawStream(self.index)
@@ -169,8 +182,8 @@ def xent(h, w, targets, scale=1.0, grad=True, dh=None, dw=None):
     pdh = pdw = None
     lddh = lddw = 0
     if grad:
-        dh, pdh, lddh = _result("dh", dh, rows, width, dtype, device)
-        dw, pdw, lddw = _result("dw", dw, vocab, width, dtype, device)
+        dh, pdh, lddh = _result("dh", dh, rows, width, dtype, device, h)
+        dw, pdw, lddw = _result("dw", dw, vocab, width, dtype, device, w)
     with _on(device) as stream:
         # the size goes by the alignment of w and its rows
         ws = _workspace(device, "xent", rows, width, vocab, _DTYPES[dtype], int(grad), pw % 256 or None, ldw)
@@ -204,18 +217,18 @@ def _norm(x, weight, residual, eps, total, out, scales, block):
     ldr = ldt = lds = 0
     given = [y for y in (total, out) if y is not None]
     if residual is not None:
-        pr, ldr = _matrix("residual", residual, dtype, (rows, width), device)
-        total, pt, ldt = _result("total", total, rows, width, dtype, device)
+        pr, ldr = _matrix("residual", residual, dtype, x.shape, device)
+        total, pt, ldt = _result("total", total, rows, width, dtype, device, x)
     elif total is not None:
         raise ValueError("total goes with residual")
     if scales is None:
-        out, po, ldo = _result("out", out, rows, width, dtype, device)
+        out, po, ldo = _result("out", out, rows, width, dtype, device, x)
     else:
         if block not in (0, 128):
             raise ValueError(f"block: {block}, wanted 0 or 128")
-        out = torch.empty(rows, width, dtype=torch.float8_e4m3fn, device=device)
+        out = _new(device, torch.float8_e4m3fn, rows, width)
         lds = -(-width // block) if block else 1
-        scales.append(torch.empty(rows, lds, dtype=torch.float32, device=device))
+        scales.append(_new(device, torch.float32, rows, lds))
         po, ldo, ps = out.data_ptr(), width, scales[0].data_ptr()
     with _on(device) as stream:
         _ck(K.lib().b2_norm(rows, width, _DTYPES[dtype], px, ldx, pr, ldr, pw, wt, eps, pt, ldt, K.DTYPE_E4M3 if scales is not None else _DTYPES[dtype],
@@ -248,12 +261,12 @@ def norm_grad(dy, t, weight=None, dtotal=None, eps=1e-6, dx=None):
     pd, ldd = _matrix("dy", dy)
     rows, width = dy.shape
     device, dtype = dy.device, dy.dtype
-    pt, ldt = _matrix("t", t, dtype, (rows, width), device)
-    pm, ldm = (None, 0) if dtotal is None else _matrix("dtotal", dtotal, dtype, (rows, width), device)
+    pt, ldt = _matrix("t", t, dtype, dy.shape, device)
+    pm, ldm = (None, 0) if dtotal is None else _matrix("dtotal", dtotal, dtype, dy.shape, device)
     pw, wt = _weight(weight, width, dtype, device)
     given = [] if dx is None else [dx]
-    dx, px, ldx = _result("dx", dx, rows, width, dtype, device)
-    dw = None if weight is None else torch.empty_like(weight, memory_format=torch.contiguous_format, requires_grad=False)
+    dx, px, ldx = _result("dx", dx, rows, width, dtype, device, dy)
+    dw = None if weight is None else torch.empty_like(weight)
     with _on(device) as stream:
         ws = _workspace(device, "norm_grad", rows, width, _DTYPES[dtype])
         _ck(K.lib().b2_norm_grad(rows, width, _DTYPES[dtype], pd, ldd, pt, ldt, pm, ldm, pw, wt, eps, px, ldx, None if dw is None else dw.data_ptr(),
@@ -277,13 +290,16 @@ def _rows_of(name, x):
     return n, n
 
 
-def _same(name, xs, device):
-    """Whether all are contiguous; refuses what is not a float32 or bfloat16 tensor of the device."""
-    if not all(isinstance(x, torch.Tensor) for x in xs) or {x.get_device() for x in xs} != {device.index} or not device.type == "cuda":
+def _columns(name, xs, device):
+    """(whether all are contiguous, numbers of elements, types) of a list; refuses what is not a tensor of the device. One thing of all tensors at a time: with hundreds of
+    them that takes half as long as tensor by tensor."""
+    try:
+        devices = {x.get_device() for x in xs}
+    except AttributeError:
+        devices = None
+    if devices != {device.index} or device.type != "cuda":
         raise ValueError(f"{name}: tensors on one CUDA device are wanted")
-    if not {x.dtype for x in xs} <= _DTYPES.keys():
-        raise ValueError(f"{name}: float32 or bfloat16 is wanted")
-    return all([x.is_contiguous() for x in xs])
+    return all([x.is_contiguous() for x in xs]), [x.numel() for x in xs], [x.dtype for x in xs]
 
 
 def clip(tensors, max_norm, out=None):
@@ -298,8 +314,7 @@ def clip(tensors, max_norm, out=None):
     if limited and not max_norm >= 0:
         raise ValueError(f"max_norm: {max_norm}")
     device = xs[0].device
-    dense = _same("tensors", xs, device)
-    elements = [x.numel() for x in xs]
+    dense, elements, types = _columns("tensors", xs, device)
     ys = None
     if out is not None:
         ys = [out] if isinstance(out, torch.Tensor) else list(out)
@@ -307,9 +322,14 @@ def clip(tensors, max_norm, out=None):
             raise ValueError("out goes with a limit")
         if len(ys) != len(xs):
             raise ValueError(f"out: {len(ys)} tensors for {len(xs)}")
-        dense = _same("out", ys, device) and dense
-        if any(x.shape != y.shape or x.dtype != y.dtype for x, y in zip(xs, ys)):
+        dense_y, elements_y, types_y = _columns("out", ys, device)
+        dense = dense and dense_y
+        if elements_y != elements or types_y != types or (not dense and [y.shape for y in ys] != [x.shape for x in xs]):
             raise ValueError("out: shapes and types like those of tensors are wanted")
+    try:
+        types = array.array("i", [_DTYPES[t] for t in types])
+    except KeyError:
+        raise ValueError("tensors: float32 or bfloat16 is wanted") from None
     q = lambda v: array.array("Q", v)  # noqa: E731
     widths = ld_x = ld_y = None
     if not dense:
@@ -321,9 +341,8 @@ def clip(tensors, max_norm, out=None):
         width = [min(a, b) for (a, _), (b, _) in zip(rows, rows_y)]
         widths, ld_x, ld_y = q(width), q([ld if a == k else k for k, (a, ld) in zip(width, rows)]), q([ld if b == k else k for k, (b, ld) in zip(width, rows_y)])
     px, py, sizes = q([x.data_ptr() for x in xs]), None if ys is None else q([y.data_ptr() for y in ys]), q(elements)
-    types = array.array("i", [_DTYPES[x.dtype] for x in xs])
     at = lambda v: None if v is None else v.buffer_info()[0]  # noqa: E731
-    norm = torch.empty((), dtype=torch.float32, device=device)
+    norm = _new(device, torch.float32)
     with _on(device) as stream:
         ws = _workspace(device, "clip", len(xs))
         _ck(K.lib().b2_clip(len(xs), at(px), at(py), at(sizes), at(types), at(widths), at(ld_x), at(ld_y), max_norm if limited else math.inf, norm.data_ptr(),
@@ -363,11 +382,11 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprob=Fa
     o.min_p, o.row_min_p = _per_row("min_p", min_p, torch.float32, rows, device)
     given = [] if out is None else [out]
     if out is None:
-        out = torch.empty(rows, dtype=torch.int64, device=device)
+        out = _new(device, torch.int64, rows)
     elif not isinstance(out, torch.Tensor) or out.shape != (rows,) or out.dtype not in (torch.int32, torch.int64) or out.device != device or (
             rows > 1 and out.stride(0) != 1):
         raise ValueError(f"out: a contiguous int64 or int32 tensor of {rows} on {device} is wanted")
-    lp = torch.empty(rows, dtype=torch.float32, device=device) if logprob else None
+    lp = _new(device, torch.float32, rows) if logprob else None
     with _on(device) as stream:
         ws = _workspace(device, "sample", rows, vocab)
         _ck(K.lib().b2_sample(rows, vocab, _DTYPES[logits.dtype], p, ld, pu, C.byref(o), out.data_ptr(), out.element_size(),

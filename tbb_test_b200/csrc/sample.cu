@@ -41,6 +41,21 @@ struct TileStat {
   float largest, none;
 };
 
+// What weights in fp32 need of a temperature: c = log2(e) / T in two parts, 80 T.
+struct TemperatureScale {
+  float c, c_low, reach;
+  bool usable;
+};
+__host__ __device__ inline TemperatureScale scale_of_temperature(float t) {
+  const double exact = 1.4426950408889634 / (double)t;
+  TemperatureScale s;
+  s.usable = t > 1e-25f && t < 1e25f;
+  s.c = s.usable ? (float)exact : 0.f;
+  s.c_low = s.usable ? (float)(exact - (double)s.c) : 0.f;
+  s.reach = 80.f * t;
+  return s;
+}
+
 struct SampleArgs {
   const char* logits;
   size_t ld;  // bytes
@@ -48,6 +63,7 @@ struct SampleArgs {
   const float* u;
   float temperature, top_p, min_p;
   int top_k;
+  TemperatureScale scale;  // of the temperature for all rows
   const float *row_temperature, *row_top_p, *row_min_p;
   const int* row_top_k;
   void* tokens;
@@ -63,6 +79,7 @@ struct SampleArgs {
 struct SampleRow {
   float t, top_p, min_p;
   int top_k;
+  TemperatureScale scale;
   bool by_k, by_p, by_m, greedy, whole;  // whole: the row's whole weight is needed
   __device__ __forceinline__ SampleRow(const SampleArgs& a, size_t r) {
     t = a.row_temperature ? a.row_temperature[r] : a.temperature;
@@ -71,6 +88,7 @@ struct SampleRow {
     top_k = a.row_top_k ? a.row_top_k[r] : a.top_k;
     greedy = !(t > 0.f) || top_k == 1 || top_p <= 0.f || min_p > 1.f;
     t = fminf(t, 3.4028235e38f);
+    scale = a.row_temperature ? scale_of_temperature(t) : a.scale;
     by_k = top_k > 0 && (unsigned int)top_k < a.vocab;
     by_p = top_p < 1.f;
     by_m = min_p > 0.f;
@@ -187,44 +205,62 @@ struct Weights {
 // A sum of eight is off by at most 3.5e-7 of itself: 1.5e-7 for ex2.approx (the most over all numbers in +-0.51), 2e-8 for its argument, 2^-24 for each of
 // three additions. Two such sums are compared: SLACK is twice that and a third more.
 constexpr double SLACK = 9.5367431640625e-7;  // 2^-20
+__device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)), "l"(reinterpret_cast<const unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<const unsigned long long&>(a)), "l"(reinterpret_cast<const unsigned long long&>(b)));
+  return d;
+}
+
 struct FastWeights {
-  float c, c_low, magic, least;
-  double n;     // N
-  bool usable;  // x c is exact enough and all of it in range
-  __device__ __forceinline__ void set(float largest, float t) {
-    const double exact = 1.4426950408889634 / (double)t;
-    n = rint((double)largest * exact);
-    c = (float)exact;
-    c_low = (float)(exact - (double)c);
-    magic = (float)(12582912.0 - n);  // 1.5 * 2^23: the sum's low bits are n of x c less N
-    least = (float)((double)largest - 80.0 * (double)t);
-    usable = t > 1e-25f && t < 1e25f && fabs(n) < 262144.0;
+  TemperatureScale t;
+  float n, magic, least;  // n: N
+  bool usable;            // x c is exact enough and all of it in range
+  __device__ __forceinline__ void set(float largest, const TemperatureScale& scale) {
+    t = scale;
+    n = rintf(largest * t.c);
+    magic = 12582912.f - n;  // 1.5 * 2^23: the sum's low bits are n of x c less N
+    least = largest - t.reach;
+    usable = t.usable && fabsf(n) < 262144.f;
   }
   __device__ __forceinline__ float of(float f) const {
     f = fmaxf(f, least);
-    const float m = fmaf(f, c, magic);
-    float r = fmaf(f, c, magic - m), y;
-    r = fmaf(f, c_low, r);
+    const float m = fmaf(f, t.c, magic);
+    return finish(fmaf(f, t.c_low, fmaf(f, t.c, magic - m)), m);
+  }
+  static __device__ __forceinline__ float finish(float r, float m) {
+    float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(r));
     return __uint_as_float(__float_as_uint(y) + (__float_as_uint(m) << 23));
   }
-  // What weights relative to another largest logit are to be multiplied by: a power of two.
-  __device__ __forceinline__ double unit(float other, float t) const {
-    const double by = rint((double)other * (1.4426950408889634 / (double)t)) - n;
-    return __hiloint2double((1023 + (int)fmax(by, -1000.0)) << 20, 0);
+  // The same two at a time, the same bits.
+  __device__ __forceinline__ float2 of_pair(float f, float g) const {
+    const float2 x = make_float2(fmaxf(f, least), fmaxf(g, least)), c = make_float2(t.c, t.c), low = make_float2(t.c_low, t.c_low), base = make_float2(magic, magic);
+    const float2 m = fma_pair(x, c, base), r = fma_pair(x, low, fma_pair(x, c, fma_pair(m, make_float2(-1.f, -1.f), base)));
+    return make_float2(finish(r.x, m.x), finish(r.y, m.y));
   }
+  // What weights relative to another largest logit are to be multiplied by: a power of two.
+  __device__ __forceinline__ double unit(float other) const { return __hiloint2double((1023 + (int)fmaxf(rintf(other * t.c) - n, -1000.f)) << 20, 0); }
   // To weights relative to the largest logit itself.
-  __device__ __forceinline__ double to_top(const Weights& w) const { return exp2(n - (double)w.top * 1.4426950408889634 * w.inv_t); }
+  __device__ __forceinline__ double to_top(const Weights& w) const { return exp2((double)n - (double)w.top * 1.4426950408889634 * w.inv_t); }
   template <int M>
   __device__ __forceinline__ double sum(const float (&f)[M]) const {
-    float x[M];
+    float2 x[M / 2];
 #pragma unroll
-    for (int j = 0; j < M; ++j) x[j] = of(f[j]);
+    for (int j = 0; j < M / 2; ++j) x[j] = of_pair(f[2 * j], f[2 * j + 1]);
 #pragma unroll
-    for (int o = 1; o < M; o *= 2)
+    for (int o = 1; o < M / 2; o *= 2)
 #pragma unroll
-      for (int j = 0; j + o < M; j += 2 * o) x[j] += x[j + o];
-    return (double)x[0];
+      for (int j = 0; j + o < M / 2; j += 2 * o) x[j] = add_pair(x[j], x[j + o]);
+    return (double)(x[0].x + x[0].y);
   }
 };
 
@@ -249,7 +285,7 @@ __global__ void __launch_bounds__(TILE_THREADS) sample_tiles_kernel(const Sample
   const unsigned long long tile = ((unsigned long long)blockIdx.x * TILE_THREADS + threadIdx.x) >> 5;
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.open_count = 0;
   if (tile >= all) return;
-  const size_t r = tile / a.tiles;
+  const size_t r = all >> 32 ? tile / a.tiles : (unsigned int)tile / a.tiles;
   const unsigned int lane = threadIdx.x & 31, first = (unsigned int)(tile - r * a.tiles) * TILE + lane * N;
   const RowView<T> row(a, r);
   uint4 v[VECS];
@@ -264,7 +300,7 @@ __global__ void __launch_bounds__(TILE_THREADS) sample_tiles_kernel(const Sample
   double sum = 0.0;
   if (ask.whole && most > -INFINITY) {
     FastWeights w;
-    w.set(most, ask.t);
+    w.set(most, ask.scale);
     if (w.usable) {
 #pragma unroll
       for (int k = 0; k < VECS; ++k) {
@@ -760,7 +796,7 @@ struct Sampler {
   __device__ __forceinline__ bool from_tiles(const SampleRow& ask, bool token, double u, double& total) {
     const TileStat* stats = a.stats + r * a.tiles;
     FastWeights top;
-    top.set(w.top, ask.t);
+    top.set(w.top, ask.scale);
     // a thread's tiles are neighbours
     const unsigned int each_has = (a.tiles + SAMPLE_THREADS - 1) / SAMPLE_THREADS, t0 = min(threadIdx.x * each_has, a.tiles), t1 = min(t0 + each_has, a.tiles);
     double sum = 0.0;
@@ -768,7 +804,7 @@ struct Sampler {
     for (unsigned int k = t0; k < t1; ++k) {
       const TileStat s = stats[k];
       if (s.weight < 0.0) usable = false;
-      if (s.weight > 0.0) sum += s.weight * top.unit(s.largest, ask.t);
+      if (s.weight > 0.0) sum += s.weight * top.unit(s.largest);
     }
     if (!__syncthreads_and(usable)) return false;
     const double upto = scan(sum, sh.sums[0]);
@@ -792,14 +828,14 @@ struct Sampler {
       for (unsigned int k = k0; k < k1; ++k) {
         const TileStat s = stats[k];
         if (!(s.weight > 0.0)) continue;
-        const double scale = top.unit(s.largest, ask.t);
+        const double scale = top.unit(s.largest);
         if (k + 1 < k1 && start + s.weight * scale <= target) {
           start += s.weight * scale;
           continue;
         }
         constexpr int N = 16 / (int)sizeof(T);
         FastWeights tile;
-        tile.set(s.largest, ask.t);
+        tile.set(s.largest, ask.scale);
         unsigned int place = 0;
         float logit = w.top;
         double before = start / scale;  // an exact quotient by a power of two
@@ -1170,10 +1206,10 @@ __global__ void __launch_bounds__(WHOLE_THREADS) sample_whole_kernel(const Sampl
     w.powers = powers;
     w.set(top, ask.t);
     FastWeights fast;
-    fast.set(top, ask.t);
+    fast.set(top, ask.scale);
     auto weight_of = [&](unsigned int k) {
       const TileStat s = stats[k];
-      return EXACT ? s.weight : s.weight > 0.0 ? s.weight * fast.unit(s.largest, ask.t) : 0.0;
+      return EXACT ? s.weight : s.weight > 0.0 ? s.weight * fast.unit(s.largest) : 0.0;
     };
     double sum = 0.0;
     bool usable = EXACT || fast.usable;
@@ -1208,9 +1244,19 @@ __global__ void __launch_bounds__(WHOLE_THREADS) sample_whole_kernel(const Sampl
     unsigned int place = 0;
     float logit = top;
     double weight = 0.0;
+    uint4 v[PER_LANE / N];  // the tile, its loads side by side
+#pragma unroll
+    for (int k = 0; k < PER_LANE / N; ++k) v[k] = row.load_vector(tile * TILE + (k * 32 + lane) * N);
+    auto logits = [&](unsigned int i, float (&f)[N]) {
+#pragma unroll
+      for (int k = 0; k < PER_LANE / N; ++k)
+        if ((i - tile * TILE) / (32 * N) == k) Elems<T, 16>::get(v[k], f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) f[j] = fmaxf(f[j], -INFINITY);
+    };
     if constexpr (EXACT) {
       walk<N, double>(lane, tile * TILE, tile * TILE + TILE, start, target, place, logit, weight, [&](unsigned int i, float (&f)[N], double (&x)[N]) {
-        row.load(i, f);
+        logits(i, f);
 #pragma unroll
         for (int j = 0; j < N; ++j) x[j] = w.of(f[j]);
       });
@@ -1219,11 +1265,11 @@ __global__ void __launch_bounds__(WHOLE_THREADS) sample_whole_kernel(const Sampl
       bool sure = false;
       if (usable) {
         FastWeights own_unit;
-        own_unit.set(stats[tile].largest, ask.t);
-        const double unit = fast.unit(stats[tile].largest, ask.t), goal = target / unit;  // exact quotients by a power of two
+        own_unit.set(stats[tile].largest, ask.scale);
+        const double unit = fast.unit(stats[tile].largest), goal = target / unit;  // exact quotients by a power of two
         double before = start / unit;
         const bool found = walk<N, float>(lane, tile * TILE, tile * TILE + TILE, before, goal, place, logit, weight, [&](unsigned int i, float (&f)[N], float (&x)[N]) {
-          row.load(i, f);
+          logits(i, f);
 #pragma unroll
           for (int j = 0; j < N; ++j) x[j] = own_unit.of(f[j]);
         });
@@ -1368,6 +1414,7 @@ int b2_sample(size_t rows, size_t vocab, int dtype, const void* logits, size_t l
   a.vocab = (unsigned int)vocab;
   a.u = u;
   a.temperature = o->temperature;
+  a.scale = scale_of_temperature(o->temperature < 3.4028235e38f ? o->temperature : 3.4028235e38f);
   a.top_p = o->top_p;
   a.min_p = o->min_p;
   a.top_k = o->top_k;

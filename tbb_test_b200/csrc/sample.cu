@@ -177,14 +177,16 @@ struct Weights {
   // Bins that reach `span` below the top, in units of T; the last one has all that is lower.
   __device__ __forceinline__ void set_bins(double span) { per_bin = (float)fmin(2 * (BINS - 1) / span * inv_t, 1e38); }
   __device__ __forceinline__ double exponent(float f) const { return f == top ? 0.0 : ((double)f - (double)top) * inv_t; }
-  // The weight of a logit d <= 0 above the top: 2^((n + s) / 16), n an integer, for d of -693 T at least
-  __device__ __forceinline__ double power(double d) const {
-    const double t = fma(d, steps, 6755399441055744.0);  // 1.5 * 2^52: the sum's low bits are n
-    const double s = fma(d, steps, 6755399441055744.0 - t);
+  // 2^(x / 16) = 2^((n + s) / 16), n an integer, for x = d * by of -16000 at least
+  __device__ __forceinline__ double sixteenths(double d, double by) const {
+    const double t = fma(d, by, 6755399441055744.0);  // 1.5 * 2^52: the sum's low bits are n
+    const double s = fma(d, by, 6755399441055744.0 - t);
     const int n = __double2loint(t);
     const double base = powers[n & (STEPS - 1)], x = fma(base, small_power(s), base);
     return __hiloint2double(__double2hiint(x) + ((n & ~(STEPS - 1)) << 16), __double2loint(x));
   }
+  // The weight of a logit d <= 0 above the top, for d of -693 T at least
+  __device__ __forceinline__ double power(double d) const { return sixteenths(d, steps); }
   __device__ __forceinline__ double of(float f) const {
     const float g = fmaxf(f, least);
     const double x = power((plain ? widened(g) : (double)g) - wide_top);
@@ -204,7 +206,8 @@ struct Weights {
 // Weights in fp32 up to a factor that all of them share: 2^(x c - N) with c = log2(e) / T and N = rint(largest c), by the nearest integer n of x c and 2^(x c - n).
 // A sum of eight is off by at most 3.5e-7 of itself: 1.5e-7 for ex2.approx (the most over all numbers in +-0.51), 2e-8 for its argument, 2^-24 for each of
 // three additions. Two such sums are compared: SLACK is twice that and a third more.
-constexpr double SLACK = 9.5367431640625e-7;  // 2^-20
+constexpr double SLACK = 9.5367431640625e-7;          // 2^-20
+constexpr double SLACK_OF_ONE = 4.76837158203125e-7;  // 2^-21: such a sum against an exact one
 __device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
   float2 d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;"
@@ -250,7 +253,7 @@ struct FastWeights {
   // What weights relative to another largest logit are to be multiplied by: a power of two.
   __device__ __forceinline__ double unit(float other) const { return __hiloint2double((1023 + (int)fmaxf(rintf(other * t.c) - n, -1000.f)) << 20, 0); }
   // To weights relative to the largest logit itself.
-  __device__ __forceinline__ double to_top(const Weights& w) const { return exp2((double)n - (double)w.top * 1.4426950408889634 * w.inv_t); }
+  __device__ __forceinline__ double to_top(const Weights& w) const { return w.sixteenths((double)n - (double)w.top * 1.4426950408889634 * w.inv_t, STEPS); }
   template <int M>
   __device__ __forceinline__ double sum(const float (&f)[M]) const {
     float2 x[M / 2];
@@ -316,7 +319,7 @@ __global__ void __launch_bounds__(TILE_THREADS) sample_tiles_kernel(const Sample
   if (lane == 0) a.stats[tile] = TileStat{sum, most, 0.f};
 }
 
-// Tokens that the shared memory of a block holds of one warp's tiles, so that two blocks fit an SM.
+// Tokens that the shared memory of a block holds of one warp's tiles.
 template <typename T> constexpr unsigned int SEGMENT = sizeof(T) == 2 ? 1280 : 896;
 constexpr unsigned int SEGMENT_TILES = 64;  // of one warp at most: offsets in 16 bits
 
@@ -324,7 +327,7 @@ template <typename T>
 struct SampleShared {
   unsigned int bins[3][BINS];  // the first ones, and two that take turns
   unsigned long long list[LIST], ordered[LIST], own[LIST];
-  double sums[2][SAMPLE_WARPS];
+  double sums[4][SAMPLE_WARPS];
   double powers[STEPS];
   unsigned int counts[SAMPLE_WARPS], found[4], listed;
   alignas(16) T values[SAMPLE_WARPS * SEGMENT<T>];           // gathered tokens by warp, in their order
@@ -492,6 +495,26 @@ struct Sampler {
     before = __shfl_sync(0xFFFFFFFFu, before, warp ? warp - 1 : 0);
     return warp ? before + v : v;
   }
+  // Four of them at a time.
+  __device__ __forceinline__ void scan4(double (&v)[4]) {
+    for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const double below = __shfl_up_sync(0xFFFFFFFFu, v[k], o);
+        if (lane >= o) v[k] += below;
+      }
+    __syncthreads();
+    if (lane == 31)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sh.sums[k][warp] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      double before = lane < warp ? sh.sums[k][lane] : 0.0;
+      for (int o = SAMPLE_WARPS / 2; o; o >>= 1) before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
+      v[k] += __shfl_sync(0xFFFFFFFFu, before, 0);
+    }
+  }
   __device__ __forceinline__ unsigned int lanes_before(unsigned int v) const {
     unsigned int upto = v;
     for (int o = 1; o < 32; o <<= 1) {
@@ -572,9 +595,10 @@ struct Sampler {
       high[k] = sum_high += wh * count[k];
       mid[k] = sum_mid += 0.5 * (wl + wh) * count[k];
     }
-    const double before_low = scan(sum_low, sh.sums[0]) - sum_low, before_high = scan(sum_high, sh.sums[0]) - sum_high,
-                 before_mid = scan(sum_mid, sh.sums[0]) - sum_mid;
-    unsigned int upto = scan(mine, sh.counts) - mine;
+    double upto4[4] = {sum_low, sum_mid, sum_high, (double)mine};
+    scan4(upto4);
+    const double before_low = upto4[0] - sum_low, before_mid = upto4[1] - sum_mid, before_high = upto4[2] - sum_high;
+    unsigned int upto = (unsigned int)upto4[3] - mine;
     if (threadIdx.x == 0) sh.found[0] = 0;
     __syncthreads();
     // bins with tokens only: the first ones whose running weight reaches the target
@@ -592,6 +616,11 @@ struct Sampler {
     if (b2 > last) b2 = last;
     if (b1 > b2) b1 = b2;
     m = m < b1 ? b1 : m > b2 ? b2 : m;
+#pragma unroll
+    for (int k = BINS_PER_THREAD - 1; k >= 0; --k) {
+      if (threadIdx.x * BINS_PER_THREAD + k == b2) sh.found[3] = upto;  // tokens up to this bin's end
+      upto -= count[k];
+    }
     return true;
   }
 
@@ -750,11 +779,7 @@ struct Sampler {
   // The row's whole weight in fp64.
   __device__ double whole_weight() {
     double s = 0.0;
-    for (unsigned int i = threadIdx.x * M; i < row.end; i += SAMPLE_THREADS * M) {
-      float f[M];
-      row.load(i, f);
-      s += weigh(f, [](float) { return true; });
-    }
+    each_of_row(-INFINITY, [&](unsigned int, const float (&f)[M]) { s += weigh(f, [](float g) { return g >= -INFINITY; }); });  // not NaN
     return block_sum(s, 1);
   }
 
@@ -768,7 +793,7 @@ struct Sampler {
     if (ask.by_p) {
       const double before = scan(x, sh.sums[0]) - x, p = ask.top_p;
       if (ask.by_k) mass = warps_sum(0);
-      else if (__syncthreads_or(t < n && before >= p * mass * (1.0 - SLACK) && before < p * mass * (1.0 + SLACK))) mass = whole_weight();
+      else if (__syncthreads_or(t < n && before >= p * mass * (1.0 - SLACK_OF_ONE) && before < p * mass * (1.0 + SLACK_OF_ONE))) mass = whole_weight();
       if (t > 0 && !(before < p * mass)) x = 0.0;
     }
     if (ask.by_m && t > 0 && !(x >= (double)ask.min_p)) x = 0.0;
@@ -856,54 +881,62 @@ struct Sampler {
     return sh.found[0];
   }
 
-  // top-p: the tokens from `lowest` on are counted in bins, which say how far down the limit can be at most.
-  __device__ __forceinline__ double narrowed(double lowest, double target) {
+  // body(place of the first, logits) for the row's tokens, M neighbours per lane and four such vectors at a time, by all warps. Vectors of tiles that have nothing of at
+  // least `least` are left out.
+  template <class Body>
+  __device__ __forceinline__ void each_of_row(float least, Body body) const {
+    constexpr unsigned int PER_TILE = PER_LANE / M;
+    const TileStat* stats = a.stats + r * a.tiles;
+    for (unsigned int q = warp; q < a.tiles * PER_TILE; q += 4 * SAMPLE_WARPS) {
+      uint4 v[4];
+      bool some[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const unsigned int at = q + k * SAMPLE_WARPS;
+        some[k] = at < a.tiles * PER_TILE && stats[at / PER_TILE].largest >= least;
+        if (some[k]) v[k] = row.load_vector(at * (32 * M) + lane * M);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (some[k]) {
+          float f[M];
+          Elems<T, 16>::get(v[k], f);
+          body((q + k * SAMPLE_WARPS) * (32 * M) + lane * M, f);
+        }
+    }
+  }
+
+  // top-p: the tokens from `lowest` on are counted in bins, which say how far down the limit can be at most, and how many tokens there are up to there.
+  __device__ __forceinline__ double narrowed(double lowest, double target, unsigned int& expected) {
     w.set_bins(fmin(REACH, -lowest * w.inv_t * 1.01 + 1e-6));
     for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) sh.bins[0][i] = 0;
     __syncthreads();
-    const TileStat* stats = a.stats + r * a.tiles;
     const float least = fmaxf((float)((double)w.top + lowest), -3.4028235e38f);
-    for (unsigned int k = warp; k < a.tiles; k += SAMPLE_WARPS) {
-      if (!(stats[k].largest >= least)) continue;
-      uint4 v[PER_LANE / M];
+    each_of_row(least, [&](unsigned int, const float (&f)[M]) {
 #pragma unroll
-      for (int q = 0; q < PER_LANE / M; ++q) v[q] = row.load_vector(k * TILE + (q * 32 + lane) * M);
-#pragma unroll
-      for (int q = 0; q < PER_LANE / M; ++q) {
-        float f[M];
-        Elems<T, 16>::get(v[q], f);
-#pragma unroll
-        for (int j = 0; j < M; ++j)
-          if (f[j] >= least) atomicAdd(&sh.bins[0][w.bin(f[j])], 1u);
-      }
-    }
+      for (int j = 0; j < M; ++j)
+        if (f[j] >= least) atomicAdd(&sh.bins[0][w.bin(f[j])], 1u);
+    });
     __syncthreads();
     unsigned int b1, m, b2;
-    return bracket(0, true, 0, 0, 0, 0.0, target * (1.0 - SLACK), target, target * (1.0 + SLACK), b1, m, b2) ? fmax(lowest, -w.bin_end(b2)) : lowest;
+    if (!bracket(0, true, 0, 0, 0, 0.0, target * (1.0 - SLACK), target, target * (1.0 + SLACK), b1, m, b2)) return lowest;
+    __syncthreads();
+    expected = sh.found[3];
+    return fmax(lowest, -w.bin_end(b2));
   }
 
   // The tokens of at least `floor` where few are expected: how many there are, the first LIST that come listed with their numbers for places.
   __device__ __forceinline__ unsigned int gather_few() {
-    const float* most = a.lane_most + r * a.tiles * 32;
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
-    for (unsigned int k = warp; k < a.tiles; k += SAMPLE_WARPS) {
-      if (!(most[k * 32 + lane] >= floor)) continue;
-      uint4 v[PER_LANE / M];
+    each_of_row(floor, [&](unsigned int i, const float (&f)[M]) {
 #pragma unroll
-      for (int q = 0; q < PER_LANE / M; ++q) v[q] = row.load_vector(k * TILE + (q * 32 + lane) * M);
-#pragma unroll
-      for (int q = 0; q < PER_LANE / M; ++q) {
-        float f[M];
-        Elems<T, 16>::get(v[q], f);
-#pragma unroll
-        for (int j = 0; j < M; ++j)
-          if (f[j] >= floor) {
-            const unsigned int at = atomicAdd(&sh.listed, 1u);
-            if (at < LIST) sh.list[at] = (unsigned long long)~key_of(f[j]) << 32 | (k * TILE + (q * 32 + lane) * M + j - row.shift);
-          }
-      }
-    }
+      for (int j = 0; j < M; ++j)
+        if (f[j] >= floor) {
+          const unsigned int at = atomicAdd(&sh.listed, 1u);
+          if (at < LIST) sh.list[at] = (unsigned long long)~key_of(f[j]) << 32 | (i + j - row.shift);
+        }
+    });
     __syncthreads();
     return sh.listed;
   }
@@ -911,44 +944,57 @@ struct Sampler {
   // The tokens of at least `floor`: how many there are. Each warp's go to its segment of shared memory, in their order and with -inf behind them, where there is room.
   __device__ __forceinline__ unsigned int gather() {
     const TileStat* stats = a.stats + r * a.tiles;
-    const float* most = a.lane_most ? a.lane_most + r * a.tiles * 32 : nullptr;
     constexpr unsigned int SEG = SEGMENT<T>;
     T* to = sh.values + warp * SEG;
     unsigned short* offsets = sh.offsets + warp * SEG;
     unsigned int own = 0;
-    const unsigned int t0 = first_tile(warp), t1 = first_tile(warp + 1);
-    for (unsigned int k = t0; k < t1; ++k) {
-      const bool some = most ? most[k * 32 + lane] >= floor : stats[k].largest >= floor;
-      if (!__any_sync(0xFFFFFFFFu, some)) continue;
-      uint4 v[PER_LANE / M];
+    const unsigned int t0 = first_tile(warp), t1 = first_tile(warp + 1), lower = (1u << lane) - 1;
+    uint4 v[PER_LANE / M], next[PER_LANE / M];
+    auto load = [&](unsigned int k) {
+      return k < t1 && stats[k].largest >= floor;
+    };
+    auto vectors = [&](unsigned int k) {
 #pragma unroll
-      for (int q = 0; q < PER_LANE / M; ++q)
-        if (some) v[q] = row.load_vector(k * TILE + (q * 32 + lane) * M);
+      for (int q = 0; q < PER_LANE / M; ++q) next[q] = row.load_vector(k * TILE + (q * 32 + lane) * M);
+    };
+    bool some = load(t0);
+    if (some) vectors(t0);
+    for (unsigned int k = t0; k < t1; ++k) {
+      const bool now = some;
+#pragma unroll
+      for (int q = 0; q < PER_LANE / M; ++q) v[q] = next[q];
+      some = load(k + 1);
+      if (some) vectors(k + 1);
+      if (!now) continue;
 #pragma unroll
       for (int q = 0; q < PER_LANE / M; ++q) {
         float f[M];
         unsigned int mine = 0;
-        if (some) {
-          Elems<T, 16>::get(v[q], f);
+        Elems<T, 16>::get(v[q], f);
 #pragma unroll
-          for (int j = 0; j < M; ++j) mine += f[j] >= floor;
+        for (int j = 0; j < M; ++j) mine += f[j] >= floor;
+        // how many the lanes before have, by the bits of their numbers
+        unsigned int before = 0, all = 0;
+#pragma unroll
+        for (int b = 0; (1 << b) <= M; ++b) {
+          const unsigned int have = __ballot_sync(0xFFFFFFFFu, mine >> b & 1);
+          before += __popc(have & lower) << b;
+          all += __popc(have) << b;
         }
-        if (!__any_sync(0xFFFFFFFFu, mine)) continue;
-        const unsigned int before = lanes_before(mine);
-        unsigned int at = own + before;
-        const unsigned int offset = (k - t0) * TILE + (q * 32 + lane) * M;
         if (mine) {
+          unsigned int at = own + before;
+          const unsigned int offset = (k - t0) * TILE + (q * 32 + lane) * M;
 #pragma unroll
-          for (int j = 0; j < M; ++j)
-            if (f[j] >= floor) {
-              if (at < SEG) {
-                to[at] = (T)f[j];
-                offsets[at] = (unsigned short)(offset + j);
-              }
-              ++at;
+          for (int j = 0; j < M; ++j) {
+            const bool keep = f[j] >= floor;
+            if (keep && at < SEG) {
+              to[at] = (T)f[j];
+              offsets[at] = (unsigned short)(offset + j);
             }
+            at += keep;
+          }
         }
-        own += __shfl_sync(0xFFFFFFFFu, before + mine, 31);
+        own += all;
       }
     }
     const unsigned int whole = min((own + 32 * M - 1) / (32 * M) * (32 * M), SEG);
@@ -1047,7 +1093,6 @@ struct Sampler {
     const SampleRow ask(a, r);
     const TileStat* stats = a.stats + r * a.tiles;
     const double u = a.u[r];
-    if (threadIdx.x < STEPS) sh.powers[threadIdx.x] = exp2(threadIdx.x / (double)STEPS);
     w.powers = sh.powers;
     float top = -INFINITY;
     for (unsigned int k = threadIdx.x; k < a.tiles; k += SAMPLE_THREADS) top = fmaxf(top, stats[k].largest);
@@ -1080,7 +1125,7 @@ struct Sampler {
     stored = false;
     floor = -3.4028234663852886e38f;
     Cut cut{-INFINITY, 0, 0};
-    double all = 0.0, slack = SLACK;
+    double all = 0.0, slack = SLACK_OF_ONE;
     if (!ask.by_k && !ask.by_p && !ask.by_m) {
       if (from_tiles(ask, true, u, all)) return;
       share(row.end);
@@ -1089,6 +1134,7 @@ struct Sampler {
     }
     // what is certainly not kept
     double lowest = -INFINITY;  // of logits, as a difference to the largest
+    unsigned int expected = 0xFFFFFFFFu;  // tokens that will be gathered
     if (ask.by_k) {
       // as many lanes as top_k have a logit in the bins up to this one
       for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) sh.bins[0][i] = 0;
@@ -1099,19 +1145,23 @@ struct Sampler {
         if (most[i] > -INFINITY) atomicAdd(&sh.bins[0][w.bin(most[i])], 1u);
       __syncthreads();
       const unsigned int bin = reaches(0, ask.top_k);
-      if (bin < BINS - 1) lowest = -w.bin_end(bin);
+      if (bin < BINS - 1) {
+        lowest = -w.bin_end(bin);
+        expected = ask.top_k;  // and some
+      }
     } else if (ask.by_p) {
       if (!from_tiles(ask, false, u, all)) {
         all = whole_weight();
         slack = 0.0;
       }
-      lowest = (log((1.0 - (double)ask.top_p) * all * (1.0 - SLACK) / a.vocab) - 1e-3) * (double)ask.t;
-      lowest = narrowed(lowest, (double)ask.top_p * all);
+      // logf is off by 1e-5 at most here, and the sum by less
+      lowest = (double)(logf((float)((1.0 - (double)ask.top_p) * all) / (float)a.vocab) - 1e-3f) * (double)ask.t;
+      lowest = narrowed(lowest, (double)ask.top_p * all, expected);
     }
-    if (ask.by_m && !(ask.by_k && ask.by_p)) lowest = fmax(lowest, (log((double)ask.min_p) - 1e-3) * (double)ask.t);  // top_p counts all of the first top_k
+    if (ask.by_m && !(ask.by_k && ask.by_p)) lowest = fmax(lowest, (double)(logf(ask.min_p) - 1e-3f) * (double)ask.t);  // top_p counts all of the first top_k
     // rounded to fp32 it is no more than any logit that it is no more than
     floor = top == INFINITY ? top : (float)fmax((double)top + lowest, -3.4028234663852886e38);
-    if (ask.by_k && ask.top_k <= LIST) {
+    if (expected <= LIST) {
       const unsigned int n = gather_few();
       if (n <= LIST) {
         choose(n, ask, all, u);
@@ -1322,10 +1372,12 @@ __global__ void __launch_bounds__(TILE_THREADS) sample_exact_kernel(const Sample
 }
 
 template <typename T>
-__global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs a) {
   extern __shared__ __align__(16) unsigned char shared[];
+  SampleShared<T>& sh = *reinterpret_cast<SampleShared<T>*>(shared);
+  if (threadIdx.x < STEPS) sh.powers[threadIdx.x] = exp2(threadIdx.x / (double)STEPS);
   after_previous();
-  Sampler<T> s{a, *reinterpret_cast<SampleShared<T>*>(shared), blockIdx.x, RowView<T>(a, blockIdx.x), (int)threadIdx.x & 31, (int)threadIdx.x >> 5};
+  Sampler<T> s{a, sh, blockIdx.x, RowView<T>(a, blockIdx.x), (int)threadIdx.x & 31, (int)threadIdx.x >> 5};
   s.run();
 }
 
@@ -1426,7 +1478,8 @@ int b2_sample(size_t rows, size_t vocab, int dtype, const void* logits, size_t l
   a.wide = token_bytes == 8;
   a.logprob = logprob;
   if (!o->row_top_k && !(o->top_k > 0 && (size_t)o->top_k < vocab)) a.lane_most = nullptr;
-  const bool limits = a.lane_most || o->row_top_p || o->top_p < 1.f || o->row_min_p || o->min_p > 0.f;
+  const bool greedy = (!o->row_temperature && !(o->temperature > 0.f)) || (!o->row_top_k && o->top_k == 1) || (!o->row_top_p && o->top_p <= 0.f) || (!o->row_min_p && o->min_p > 1.f);
+  const bool limits = !greedy && (a.lane_most || o->row_top_p || o->top_p < 1.f || o->row_min_p || o->min_p > 0.f);
   const cudaError_t err = dtype == B2_DTYPE_BF16 ? sample_rows<__nv_bfloat16>(a, rows, limits, sms, static_cast<cudaStream_t>(stream))
                                                  : sample_rows<float>(a, rows, limits, sms, static_cast<cudaStream_t>(stream));
   return launch_error(err, who);

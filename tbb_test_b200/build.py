@@ -8,11 +8,15 @@ Outputs (git-ignored, next to their sources):
     tbb_test_b200/host/libb2host.so     C++ host mirror of the reference's
                                         Partition / TwistedHyperCube / driver code
     tbb_test_b200/host/mlp_cuda         driver binary (counterpart of mlp_omp)
+    tbb_test_b200/native/_lm_native.so  calls of the operators in lm.py on torch tensors
+                                        (built where torch is installed)
 """
 import glob
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -22,6 +26,7 @@ HOST = os.path.join(PKG, "host")
 LIB = os.path.join(CSRC, "libb200mlp.so")
 HOST_LIB = os.path.join(HOST, "libb2host.so")
 DRIVER = os.path.join(HOST, "mlp_cuda")
+NATIVE = os.path.join(PKG, "native", "_lm_native.so")
 
 NVCC = os.environ.get("B2_NVCC", "/usr/local/cuda/bin/nvcc")
 CXX = os.environ.get("B2_CXX", "/usr/bin/g++")
@@ -79,9 +84,27 @@ def build_host(force=False, verbose=False):
     return HOST_LIB
 
 
+def build_native(force=False, verbose=False):
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        return None
+    src = os.path.join(PKG, "native", "lm_native.cc")
+    # against the headers of the torch that will load it
+    if not force and not _stale(NATIVE, [src, os.path.join(ROOT, "include", "b200mlp.h"), spec.origin]):
+        return NATIVE
+    torch_dir = os.path.dirname(spec.origin)
+    lib, inc = os.path.join(torch_dir, "lib"), os.path.join(torch_dir, "include")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")
+    _run([CXX, "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-I", inc, "-I", os.path.join(inc, "torch", "csrc", "api", "include"), "-I", cuda,
+          "-I", sysconfig.get_paths()["include"], "-D_GLIBCXX_USE_CXX11_ABI=1", "-o", NATIVE, src, "-L", lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
+          "-ltorch_python", "-Wl,-rpath," + lib], verbose)
+    return NATIVE
+
+
 def build_all(force=False, verbose=False):
     build_cuda(force, verbose)
     build_host(force, verbose)
+    build_native(force, verbose)
 
 
 if __name__ == "__main__":

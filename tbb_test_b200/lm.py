@@ -9,7 +9,7 @@
   sample              a token per row of logits: temperature, top-k, top-p, min-p
   sync                waits for the current stream and raises if a kernel's bounded wait gave up
 
-Thin wrappers over the C ABI (include/b200mlp.h, "Operators around the layers of a language model"): they
+Thin wrappers over the C ABI (include/b200mlp.h, "Operators around the layers of a language model"), those of norm, clip and sample in C++ (native/lm_native.cc): they
 check shapes, types and devices (and the entries behind them overlaps), allocate what is returned, and queue the work on the current torch stream without waiting
 for it. Matrices are float32 or bfloat16, all of one call alike, with unit stride along rows and any distance between
 rows. Tokens are int32 or int64; one outside [0, vocab) is padding. There is no CPU path.
@@ -18,10 +18,8 @@ Nothing here is recorded by autograd, whatever its arguments require: results re
 the gradients themselves. What a call writes into a given tensor counts as an in-place change, so that autograd's own backward passes refuse
 to use a value that it saved before.
 """
-import array
 import ctypes as C
 import functools
-import math
 
 import torch
 
@@ -194,112 +192,36 @@ def xent(h, w, targets, scale=1.0, grad=True, dh=None, dw=None):
     return (loss, dh, dw) if grad else loss
 
 
-def _weight(x, width, dtype, device):
-    """(address, DTYPE) of a norm's weight: of the matrices' type or float32; (None, the matrices' DTYPE) for none."""
-    if x is None:
-        return None, _DTYPES[dtype]
-    if not isinstance(x, torch.Tensor) or x.shape != (width,) or x.device != device:
-        raise ValueError(f"weight: a tensor of {width} elements on {device} is wanted")
-    if x.dtype not in (dtype, torch.float32):
-        raise ValueError(f"weight: {x.dtype}, wanted {dtype} or float32")
-    if width > 1 and x.stride(0) != 1:
-        raise ValueError("weight: unit stride is wanted")
-    return x.data_ptr(), _DTYPES[x.dtype]
-
-
-def _norm(x, weight, residual, eps, total, out, scales, block):
-    """The call of b2_norm. scales: None, or a list that receives the given or new scales (an e4m3 output)."""
-    px, ldx = _matrix("x", x)
-    rows, width = x.shape
-    device, dtype = x.device, x.dtype
-    pw, wt = _weight(weight, width, dtype, device)
-    pr = pt = ps = None
-    ldr = ldt = lds = 0
-    given = [y for y in (total, out) if y is not None]
-    if residual is not None:
-        pr, ldr = _matrix("residual", residual, dtype, x.shape, device)
-        total, pt, ldt = _result("total", total, rows, width, dtype, device, x)
-    elif total is not None:
-        raise ValueError("total goes with residual")
-    if scales is None:
-        out, po, ldo = _result("out", out, rows, width, dtype, device, x)
-    else:
-        if block not in (0, 128):
-            raise ValueError(f"block: {block}, wanted 0 or 128")
-        out = _new(device, torch.float8_e4m3fn, rows, width)
-        lds = -(-width // block) if block else 1
-        scales.append(_new(device, torch.float32, rows, lds))
-        po, ldo, ps = out.data_ptr(), width, scales[0].data_ptr()
-    with _on(device) as stream:
-        _ck(K.lib().b2_norm(rows, width, _DTYPES[dtype], px, ldx, pr, ldr, pw, wt, eps, pt, ldt, K.DTYPE_E4M3 if scales is not None else _DTYPES[dtype],
-                            po, ldo, ps, lds, block, stream))
-    if given:
-        _changed(given)
-    return out, total
+@functools.lru_cache(maxsize=None)
+def _native():
+    """The C++ side of the calls below, with the entries of the library that this process uses."""
+    try:
+        from .native import _lm_native
+    except ImportError as e:
+        raise ImportError(f"{e}: build it with `python -m tbb_test_b200.build` (there is no CPU or PyTorch fallback)") from None
+    entries = ("b2_norm", "b2_norm_grad_workspace", "b2_norm_grad", "b2_clip_workspace", "b2_clip", "b2_sample_workspace", "b2_sample", "b2_last_error")
+    _lm_native.use(*[C.cast(getattr(K.lib(), name), C.c_void_p).value for name in entries], K.B2Error)
+    return _lm_native
 
 
 def norm(x, weight=None, residual=None, eps=1e-6, total=None, out=None):
     """`t / sqrt(mean of t's squares + eps) * weight` for each row of t = x, or of t = x + residual rounded to their type: then
     (norm, t), t to be added to by what comes next and for `norm_grad`. weight: one element per column, of the matrices' type or
     float32. `total` (t) and `out` may be given to be written to."""
-    out, total = _norm(x, weight, residual, eps, total, out, None, 0)
-    return out if residual is None else (out, total)
+    return _native().norm(x, weight, residual, eps, total, out, None)
 
 
 def norm_e4m3(x, weight=None, residual=None, eps=1e-6, block=128, total=None):
     """The same with its result in 8 bits, to stand in front of a product of such operands: (q, scales), or (q, scales, t) with a
     residual. q is float8_e4m3fn, and q * scale the norm: a float32 scale for each `block` = 128 columns, or for each row
     (block = 0), rows x scales. Gradients are those of `norm` (norm_grad)."""
-    scales = []
-    out, total = _norm(x, weight, residual, eps, total, None, scales, block)
-    return (out, scales[0]) if residual is None else (out, scales[0], total)
+    return _native().norm(x, weight, residual, eps, total, None, block)
 
 
 def norm_grad(dy, t, weight=None, dtotal=None, eps=1e-6, dx=None):
     """Gradients of `norm` from the gradient dy of its result, at t (x, or x + residual as norm gave it): dx for x and residual
     alike, or (dx, dweight) with a weight. `dtotal`: a gradient that arrives at t elsewhere, which dx includes."""
-    pd, ldd = _matrix("dy", dy)
-    rows, width = dy.shape
-    device, dtype = dy.device, dy.dtype
-    pt, ldt = _matrix("t", t, dtype, dy.shape, device)
-    pm, ldm = (None, 0) if dtotal is None else _matrix("dtotal", dtotal, dtype, dy.shape, device)
-    pw, wt = _weight(weight, width, dtype, device)
-    given = [] if dx is None else [dx]
-    dx, px, ldx = _result("dx", dx, rows, width, dtype, device, dy)
-    dw = None if weight is None else torch.empty_like(weight)
-    with _on(device) as stream:
-        ws = _workspace(device, "norm_grad", rows, width, _DTYPES[dtype])
-        _ck(K.lib().b2_norm_grad(rows, width, _DTYPES[dtype], pd, ldd, pt, ldt, pm, ldm, pw, wt, eps, px, ldx, None if dw is None else dw.data_ptr(),
-                                 ws.data_ptr(), ws.numel(), stream))
-    if given:
-        _changed(given)
-    return dx if dw is None else (dx, dw)
-
-
-def _rows_of(name, x):
-    """(width, distance of rows) of a tensor that is not contiguous, as b2_clip takes it: a matrix with gaps, or (elements, elements) where it lies in memory without gaps
-    in another order."""
-    n = x.numel()
-    if x.dim() == 2 and (x.shape[1] == 1 or x.stride(1) == 1) and x.stride(0) >= x.shape[1]:
-        return x.shape[1], x.stride(0)
-    at = 1
-    for stride, size in sorted((s, k) for k, s in zip(x.shape, x.stride()) if k != 1):
-        if stride != at:
-            raise ValueError(f"{name}: neither dense nor a matrix with unit stride along its rows")
-        at *= size
-    return n, n
-
-
-def _columns(name, xs, device):
-    """(whether all are contiguous, numbers of elements, types) of a list; refuses what is not a tensor of the device. One thing of all tensors at a time: with hundreds of
-    them that takes half as long as tensor by tensor."""
-    try:
-        devices = {x.get_device() for x in xs}
-    except AttributeError:
-        devices = None
-    if devices != {device.index} or device.type != "cuda":
-        raise ValueError(f"{name}: tensors on one CUDA device are wanted")
-    return all([x.is_contiguous() for x in xs]), [x.numel() for x in xs], [x.dtype for x in xs]
+    return _native().norm_grad(dy, t, weight, dtotal, eps, dx)
 
 
 def clip(tensors, max_norm, out=None):
@@ -307,58 +229,7 @@ def clip(tensors, max_norm, out=None):
     by max_norm / norm, in place or into the list `out` of tensors like them (which is always written). math.inf or None for max_norm: the
     norm alone. A norm that is infinite or not a number leaves the values as they are. float32 and bfloat16 tensors of any sizes, each dense
     or a matrix with unit stride along its rows, all on one device; none may overlap another (see b2_clip in include/b200mlp.h)."""
-    xs = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    if not xs or not isinstance(xs[0], torch.Tensor):
-        raise ValueError("tensors: none" if not xs else "tensors: tensors are wanted")
-    limited = max_norm is not None and max_norm != math.inf
-    if limited and not max_norm >= 0:
-        raise ValueError(f"max_norm: {max_norm}")
-    device = xs[0].device
-    dense, elements, types = _columns("tensors", xs, device)
-    ys = None
-    if out is not None:
-        ys = [out] if isinstance(out, torch.Tensor) else list(out)
-        if not limited:
-            raise ValueError("out goes with a limit")
-        if len(ys) != len(xs):
-            raise ValueError(f"out: {len(ys)} tensors for {len(xs)}")
-        dense_y, elements_y, types_y = _columns("out", ys, device)
-        dense = dense and dense_y
-        if elements_y != elements or types_y != types or (not dense and [y.shape for y in ys] != [x.shape for x in xs]):
-            raise ValueError("out: shapes and types like those of tensors are wanted")
-    try:
-        types = array.array("i", [_DTYPES[t] for t in types])
-    except KeyError:
-        raise ValueError("tensors: float32 or bfloat16 is wanted") from None
-    q = lambda v: array.array("Q", v)  # noqa: E731
-    widths = ld_x = ld_y = None
-    if not dense:
-        rows = [(n, n) if x.is_contiguous() else _rows_of(f"tensors[{i}]", x) for i, (x, n) in enumerate(zip(xs, elements))]
-        rows_y = rows if ys is None else [(n, n) if y.is_contiguous() else _rows_of(f"out[{i}]", y) for i, (y, n) in enumerate(zip(ys, elements))]
-        for i, (n, (a, _), (b, _)) in enumerate(zip(elements, rows, rows_y)):
-            if ys is not None and xs[i].stride() != ys[i].stride() and (a == n and not xs[i].is_contiguous() or b == n and not ys[i].is_contiguous()) and n > 1:
-                raise ValueError(f"out[{i}]: elements lie in another order than in tensors[{i}]")
-        width = [min(a, b) for (a, _), (b, _) in zip(rows, rows_y)]
-        widths, ld_x, ld_y = q(width), q([ld if a == k else k for k, (a, ld) in zip(width, rows)]), q([ld if b == k else k for k, (b, ld) in zip(width, rows_y)])
-    px, py, sizes = q([x.data_ptr() for x in xs]), None if ys is None else q([y.data_ptr() for y in ys]), q(elements)
-    at = lambda v: None if v is None else v.buffer_info()[0]  # noqa: E731
-    norm = _new(device, torch.float32)
-    with _on(device) as stream:
-        ws = _workspace(device, "clip", len(xs))
-        _ck(K.lib().b2_clip(len(xs), at(px), at(py), at(sizes), at(types), at(widths), at(ld_x), at(ld_y), max_norm if limited else math.inf, norm.data_ptr(),
-                            ws.data_ptr(), ws.numel(), stream))
-    if limited:
-        _changed(xs if ys is None else ys)
-    return norm
-
-
-def _per_row(name, x, dtype, rows, device):
-    """(number for all rows, address of one for each row or None)"""
-    if not isinstance(x, torch.Tensor):
-        return x, None
-    if x.shape != (rows,) or x.dtype != dtype or x.device != device or (rows > 1 and x.stride(0) != 1):
-        raise ValueError(f"{name}: a number, or a contiguous {dtype} tensor of {rows} on {device}, is wanted")
-    return 1, x.data_ptr()
+    return _native().clip(tensors, max_norm, out)
 
 
 def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprob=False, out=None):
@@ -369,31 +240,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprob=Fa
     min_p times the largest probability; tokens of one logit count in the order of their numbers. Each of the four may be a tensor with one
     for each row (float32; top_k int32). temperature 0 takes the most probable token. A logit of -inf or NaN is never taken; a row of nothing
     else gives -1. `out`, int64 or int32, may be given to be written to. See b2_sample in include/b200mlp.h."""
-    p, ld = _matrix("logits", logits)
-    rows, vocab = logits.shape
-    device = logits.device
-    number, pu = _per_row("u", u, torch.float32, rows, device)
-    if pu is None:
-        raise ValueError("u: a tensor is wanted")
-    o = K.SampleOptions()
-    o.temperature, o.row_temperature = _per_row("temperature", temperature, torch.float32, rows, device)
-    o.top_k, o.row_top_k = _per_row("top_k", top_k, torch.int32, rows, device)
-    o.top_p, o.row_top_p = _per_row("top_p", top_p, torch.float32, rows, device)
-    o.min_p, o.row_min_p = _per_row("min_p", min_p, torch.float32, rows, device)
-    given = [] if out is None else [out]
-    if out is None:
-        out = _new(device, torch.int64, rows)
-    elif not isinstance(out, torch.Tensor) or out.shape != (rows,) or out.dtype not in (torch.int32, torch.int64) or out.device != device or (
-            rows > 1 and out.stride(0) != 1):
-        raise ValueError(f"out: a contiguous int64 or int32 tensor of {rows} on {device} is wanted")
-    lp = _new(device, torch.float32, rows) if logprob else None
-    with _on(device) as stream:
-        ws = _workspace(device, "sample", rows, vocab)
-        _ck(K.lib().b2_sample(rows, vocab, _DTYPES[logits.dtype], p, ld, pu, C.byref(o), out.data_ptr(), out.element_size(),
-                              None if lp is None else lp.data_ptr(), ws.data_ptr(), ws.numel(), stream))
-    if given:
-        _changed(given)
-    return (out, lp) if logprob else out
+    return _native().sample(logits, u, temperature, top_k, top_p, min_p, logprob, out)
 
 
 def _listed(x):

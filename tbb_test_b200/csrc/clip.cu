@@ -10,6 +10,7 @@
 // kernel adds all blocks' sums in the same order, so that equal inputs give equal bits.
 #include <math.h>
 
+#include <algorithm>
 #include <exception>
 
 #include "lm.cuh"
@@ -291,9 +292,10 @@ int clip_tensors(const char* who, const ClipCall& c, float max_norm, float* norm
   const bool limited = max_norm < INFINITY;
   const size_t count = c.count;
   bool in_place = true;
-  std::vector<Extent> args;
+  std::vector<Extent> args, outputs;
   std::vector<ClipTensor> tensors;
   args.reserve(2 * count + 2);
+  outputs.reserve(c.out ? count + 2 : 2);
   tensors.reserve(count);
   unsigned long long all = 0;
   for (size_t i = 0; i < count; ++i) {
@@ -318,7 +320,7 @@ int clip_tensors(const char* who, const ClipCall& c, float max_norm, float* norm
     const bool here = out == x && ld_out == ld_x;
     args.push_back(extent("a tensor", x, size / width, width * e, ld_x * e, limited && here));
     if (!here) {
-      args.push_back(extent("an output", out, size / width, width * e, ld_out * e, true));
+      outputs.push_back(extent("an output", out, size / width, width * e, ld_out * e, true));
       in_place = false;
     }
     tensors.push_back(ClipTensor{static_cast<const char*>(x), static_cast<char*>(out), size, width, ld_x, ld_out, dtype == B2_DTYPE_F32,
@@ -331,9 +333,16 @@ int clip_tensors(const char* who, const ClipCall& c, float max_norm, float* norm
   if (workspace_bytes < need) return call_error(B2_ERR_INVALID, "%s: workspace of %zu bytes, %zu needed", who, workspace_bytes, need);
   int sms, rc;
   if ((rc = lm_device(&sms)) != B2_OK) return rc;
-  args.push_back(extent("norm", norm, 1, 4, 4, true));
-  args.push_back(extent("the workspace", workspace, 1, need, need, true));
-  if ((rc = refuse_overlap(who, args.data(), (int)args.size())) != B2_OK) return rc;
+  // tensors and outputs mostly come in the order in which they lie in memory: hundreds are sorted in no time then
+  const size_t inputs = args.size();
+  for (std::vector<Extent>* v : {&args, &outputs})
+    if (!std::is_sorted(v->begin(), v->end(), begins_before)) std::sort(v->begin(), v->end(), begins_before);
+  Extent more[] = {extent("norm", norm, 1, 4, 4, true), extent("the workspace", workspace, 1, need, need, true)};
+  for (const Extent& x : more) outputs.insert(std::upper_bound(outputs.begin(), outputs.end(), x, begins_before), x);
+  args.insert(args.end(), outputs.begin(), outputs.end());
+  std::inplace_merge(args.begin(), args.begin() + inputs, args.end(), begins_before);
+  const Extent *one, *other;
+  if (first_overlap(args.data(), (int)args.size(), &one, &other)) return call_error(B2_ERR_INVALID, "%s: %s and %s overlap", who, one->name, other->name);
   const cudaError_t e = most == LIST_SHORT ? clip_launch<LIST_SHORT>(tensors, in_place, max_norm, norm, partial, sms, stream)
                                            : clip_launch<LIST_MOST>(tensors, in_place, max_norm, norm, partial, sms, stream);
   return launch_error(e, who);

@@ -45,9 +45,10 @@ inline bool overlap(Extent a, Extent b) {
   return false;
 }
 
-// The first pair among n extents that overlap, at least one of them written, in *a and *b. Sorts them.
-inline bool any_overlap(Extent* x, int n, const Extent** a, const Extent** b) {
-  std::sort(x, x + n, [](const Extent& p, const Extent& q) { return p.at < q.at; });
+inline bool begins_before(const Extent& p, const Extent& q) { return p.at < q.at; }
+
+// The first pair among n extents, sorted by where they begin, that overlap, at least one of them written, in *a and *b.
+inline bool first_overlap(const Extent* x, int n, const Extent** a, const Extent** b) {
   for (int i = 0; i < n; ++i)
     for (int j = i + 1; j < n && x[j].at < x[i].end(); ++j)
       if ((x[i].written || x[j].written) && overlap(x[i], x[j])) {
@@ -56,6 +57,12 @@ inline bool any_overlap(Extent* x, int n, const Extent** a, const Extent** b) {
         return true;
       }
   return false;
+}
+
+// The same of extents in any order. Sorts them.
+inline bool any_overlap(Extent* x, int n, const Extent** a, const Extent** b) {
+  std::sort(x, x + n, begins_before);
+  return first_overlap(x, n, a, b);
 }
 
 }  // namespace b2

@@ -12,6 +12,7 @@
 
 #include <algorithm>
 #include <exception>
+#include <memory>
 
 #include "lm.cuh"
 
@@ -252,7 +253,7 @@ template <int MOST>
 cudaError_t clip_launch(const std::vector<ClipTensor>& tensors, bool in_place, float max_norm, float* norm, double* partial, int sms, cudaStream_t stream) {
   typedef ClipList<MOST> List;
   const size_t launches = tensors.empty() ? 1 : (tensors.size() + MOST - 1) / MOST;
-  std::vector<List> lists(launches);
+  const std::unique_ptr<List[]> lists(new List[launches]);
   std::vector<int> blocks(launches);
   int partials = 0;
   Chain chain(stream);
@@ -269,13 +270,17 @@ cudaError_t clip_launch(const std::vector<ClipTensor>& tensors, bool in_place, f
     l.first[l.count] = units;
     const int most = sms * 2 < CLIP_BLOCKS ? sms * 2 : CLIP_BLOCKS;
     blocks[i] = units == 0 ? 1 : units < (unsigned int)most ? (int)units : most;
-    chain.launch(clip_norm_kernel<List>, dim3(blocks[i]), CLIP_THREADS, 0, 0, l, partial + partials);
+    double* sums = partial + partials;
+    chain.launch_at(clip_norm_kernel<List>, dim3(blocks[i]), CLIP_THREADS, &l, &sums);
     partials += blocks[i];
   }
   const bool limited = max_norm < INFINITY;
-  for (size_t i = 0; i < (limited ? launches : 1); ++i)
-    chain.launch(clip_scale_kernel<List>, dim3(limited ? blocks[i] : 1), CLIP_THREADS, 0, 0, lists[i], partial, partials, max_norm, (int)in_place,
-                 i == 0 ? norm : nullptr);
+  int place = in_place;
+  for (size_t i = 0; i < (limited ? launches : 1); ++i) {
+    float* to = i == 0 ? norm : nullptr;
+    const double* sums = partial;
+    chain.launch_at(clip_scale_kernel<List>, dim3(limited ? blocks[i] : 1), CLIP_THREADS, &lists[i], &sums, &partials, &max_norm, &place, &to);
+  }
   return chain.err;
 }
 

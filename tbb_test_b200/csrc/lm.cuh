@@ -5,6 +5,7 @@
 #include <stddef.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "../../include/b200mlp.h"
 #include "common.cuh"
@@ -64,31 +65,45 @@ struct Chain {
   // cluster: CTAs per cluster, 0 for none
   template <typename... P, typename... A>
   void launch(void (*kernel)(P...), dim3 grid, unsigned int threads, size_t smem, int cluster, A&&... args) {
-    if (err != cudaSuccess) return;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    int n = 0;
-    if (cluster) {
-      attr[n].id = cudaLaunchAttributeClusterDimension;
-      attr[n].val.clusterDim.x = cluster;
-      attr[n].val.clusterDim.y = 1;
-      attr[n].val.clusterDim.z = 1;
-      ++n;
-    }
-    if (!first) {
-      attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-      attr[n].val.programmaticStreamSerializationAllowed = 1;
-      ++n;
-    }
-    cfg.attrs = attr;
-    cfg.numAttrs = n;
-    err = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    Config c(grid, threads, smem, stream, cluster, !first);
+    if (err == cudaSuccess) err = cudaLaunchKernelEx(&c.cfg, kernel, static_cast<P>(args)...);
     first = false;
   }
+  // Arguments where they lie: large ones are copied once only, by the launch.
+  template <typename... P>
+  void launch_at(void (*kernel)(P...), dim3 grid, unsigned int threads, typename std::remove_const<P>::type*... args) {
+    Config c(grid, threads, 0, stream, 0, !first);
+    void* p[] = {args...};
+    if (err == cudaSuccess) err = cudaLaunchKernelExC(&c.cfg, reinterpret_cast<const void*>(kernel), p);
+    first = false;
+  }
+
+ private:
+  struct Config {
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[2];
+    Config(dim3 grid, unsigned int threads, size_t smem, cudaStream_t stream, int cluster, bool behind) : cfg() {
+      cfg.gridDim = grid;
+      cfg.blockDim = dim3(threads);
+      cfg.dynamicSmemBytes = smem;
+      cfg.stream = stream;
+      int n = 0;
+      if (cluster) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = cluster;
+        attr[n].val.clusterDim.y = 1;
+        attr[n].val.clusterDim.z = 1;
+        ++n;
+      }
+      if (behind) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+      }
+      cfg.attrs = attr;
+      cfg.numAttrs = n;
+    }
+  };
 };
 
 // Lets blocks of a kernel have `bytes` of dynamic shared memory on the current device; a caller asks for the most that any launch of the kernel needs. Once per device:

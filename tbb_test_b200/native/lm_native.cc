@@ -268,20 +268,20 @@ PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t) {
     bool dense = true;
     for (size_t i = 0; i < n; ++i) {
       const at::Tensor& x = xs[i];
-      const std::string at_i = "[" + std::to_string(i) + "]";
-      if (!x.is_cuda() || x.device() != device) refuse("tensors" + at_i + ": on one CUDA device with the others is wanted");
-      if ((types[i] = type_code(x.scalar_type())) < 0) refuse("tensors" + at_i + ": float32 or bfloat16 is wanted");
+      const auto at = [&](const char* list, const char* what) { refuse(std::string(list) + "[" + std::to_string(i) + "]: " + what); };
+      if (!x.is_cuda() || x.device() != device) at("tensors", "on one CUDA device with the others is wanted");
+      if ((types[i] = type_code(x.scalar_type())) < 0) at("tensors", "float32 or bfloat16 is wanted");
       px[i] = x.data_ptr();
       elements[i] = x.numel();
       const auto [wx, lx] = rows_of("tensors", i, x);
       size_t wy = wx, ly = lx;
       if (apart) {
         const at::Tensor& y = ys[i];
-        if (y.device() != device || y.scalar_type() != x.scalar_type() || y.sizes() != x.sizes()) refuse("out" + at_i + ": device, type and shape of tensors" + at_i + " are wanted");
+        if (y.device() != device || y.scalar_type() != x.scalar_type() || y.sizes() != x.sizes()) at("out", "device, type and shape like those of its tensor are wanted");
         std::tie(wy, ly) = rows_of("out", i, y);
         // a whole piece in another order than the other side's
         if (elements[i] > 1 && x.strides() != y.strides() && ((wx == elements[i] && !x.is_contiguous()) || (wy == elements[i] && !y.is_contiguous())))
-          refuse("out" + at_i + ": elements lie in another order than in tensors" + at_i);
+          at("out", "elements lie in another order than in its tensor");
         py[i] = y.data_ptr();
       }
       widths[i] = wx < wy ? wx : wy;

@@ -36,7 +36,7 @@ def _ck(rc):
 def _matrix(name, x, dtype=None, shape=None, device=None):
     """(address, leading dimension) of a two-dimensional CUDA tensor with unit stride along its rows."""
     if isinstance(x, torch.Tensor) and x.dim() == 2 and x.is_contiguous() and (x.is_cuda if device is None else x.device == device) and (
-            x.dtype in _DTYPES if dtype is None else x.dtype == dtype) and (shape is None or x.shape == shape):
+            x.dtype in _DTYPES and dtype in (None, x.dtype)) and (shape is None or x.shape == shape):
         return x.data_ptr(), x.shape[1]  # what most callers give
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         raise ValueError(f"{name}: a two-dimensional tensor is wanted")

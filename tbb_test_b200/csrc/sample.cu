@@ -909,14 +909,17 @@ struct Sampler {
   // top-p: the tokens from `lowest` on are counted in bins, which say how far down the limit can be at most, and how many tokens there are up to there.
   __device__ __forceinline__ double narrowed(double lowest, double target, unsigned int& expected) {
     w.set_bins(fmin(REACH, -lowest * w.inv_t * 1.01 + 1e-6));
-    for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) sh.bins[0][i] = 0;
+    for (int i = threadIdx.x; i < 3 * BINS; i += SAMPLE_THREADS) sh.bins[0][i] = 0;
     __syncthreads();
     const float least = fmaxf((float)((double)w.top + lowest), -3.4028235e38f);
+    unsigned int* bins = sh.bins[warp % 3];  // three sets: fewer warps meet at one bin
     each_of_row(least, [&](unsigned int, const float (&f)[M]) {
 #pragma unroll
       for (int j = 0; j < M; ++j)
-        if (f[j] >= least) atomicAdd(&sh.bins[0][w.bin(f[j])], 1u);
+        if (f[j] >= least) atomicAdd(bins + w.bin(f[j]), 1u);
     });
+    __syncthreads();
+    for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) sh.bins[0][i] += sh.bins[1][i] + sh.bins[2][i];
     __syncthreads();
     unsigned int b1, m, b2;
     if (!bracket(0, true, 0, 0, 0, 0.0, target * (1.0 - SLACK), target, target * (1.0 + SLACK), b1, m, b2)) return lowest;

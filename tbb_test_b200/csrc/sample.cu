@@ -571,10 +571,12 @@ struct Sampler {
   }
   // Bins of a window in which the running weight, `mass` above it, reaches the target: at the earliest, by estimate, at the latest; false where it does not before the
   // tokens that weigh nothing. Weights of a bin's tokens are between those of its ends.
+  // In mid and count: the estimates up to the ends of the thread's bins, and their tokens.
   __device__ __forceinline__ bool bracket(int buffer, bool first, unsigned int lo, unsigned int hi, unsigned int shift, double mass, double target_low, double target,
-                                          double target_high, unsigned int& b1, unsigned int& m, unsigned int& b2) {
-    unsigned int count[BINS_PER_THREAD], mine = 0;
-    double low[BINS_PER_THREAD], mid[BINS_PER_THREAD], high[BINS_PER_THREAD];
+                                          double target_high, unsigned int& b1, unsigned int& m, unsigned int& b2, double (&mid)[BINS_PER_THREAD],
+                                          unsigned int (&count)[BINS_PER_THREAD]) {
+    unsigned int mine = 0;
+    double low[BINS_PER_THREAD], high[BINS_PER_THREAD];
     double sum_low = 0.0, sum_mid = 0.0, sum_high = 0.0;
 #pragma unroll
     for (int k = 0; k < BINS_PER_THREAD; ++k) {
@@ -608,7 +610,8 @@ struct Sampler {
       upto += count[k];
       if (count[k]) atomicMax(&sh.found[0], (unsigned int)(threadIdx.x * BINS_PER_THREAD + k));
       b1 += __syncthreads_count(upto == 0 || mass + before_high + high[k] < target_low);
-      m += __syncthreads_count(upto == 0 || mass + before_mid + mid[k] < target);
+      mid[k] += mass + before_mid;
+      m += __syncthreads_count(upto == 0 || mid[k] < target);
       b2 += __syncthreads_count(upto == 0 || mass + before_low + low[k] < target_high);
     }
     if (first && b1 >= BINS) return false;
@@ -627,6 +630,67 @@ struct Sampler {
   // The cut at which `target` tokens (BY_COUNT) or `target` weight is reached. The first bins have been counted.
   // slack: the target may be off by this share of it. NONE: it is not reached before the tokens that weigh nothing. UNSURE: where depends on what the target is off.
   enum Found { NONE, CUT, UNSURE };
+  // The first bins' part of it for weights, while bins have few tokens: exact sums up to the estimated bin's ends say whether the limit is in it, and what all estimates are
+  // off by there, so that the next one is hardly ever wrong. Not done: bin m has too many tokens.
+  __device__ __forceinline__ Found by_bins(double target_low, double target, double target_high, unsigned int b1, unsigned int& m, unsigned int b2,
+                                           const double (&mid)[BINS_PER_THREAD], const unsigned int (&count)[BINS_PER_THREAD], Cut& cut, bool& done) {
+    done = true;
+    for (;;) {
+      __syncthreads();
+      if (threadIdx.x == 0) sh.listed = 0;
+#pragma unroll
+      for (int k = 0; k < BINS_PER_THREAD; ++k)
+        if (threadIdx.x * BINS_PER_THREAD + k == m) {
+          sh.found[2] = count[k];
+          sh.sums[3][0] = mid[k];
+        }
+      __syncthreads();
+      const unsigned int n = sh.found[2];
+      const double estimate = sh.sums[3][0];
+      if (n > LIST) {
+        done = false;
+        return NONE;
+      }
+      double s1 = 0.0, s2 = 0.0;  // the weight above the bin, and up to its end
+      each([&](unsigned int i, const float (&f)[M]) {
+        double x[M];
+#pragma unroll
+        for (int j = 0; j < M; ++j) x[j] = w.of(f[j]);
+#pragma unroll
+        for (int j = 0; j < M; ++j) {
+          const unsigned int b = w.bin(f[j]);
+          s2 += b <= m ? x[j] : 0.0;
+          s1 += b < m ? x[j] : 0.0;
+          if (b == m) append(f[j], i + j);
+        }
+      });
+      s1 = block_sum(s1, 0);
+      s2 = block_sum(s2, 1);
+      if ((s1 >= target_low && s1 < target_high) || (s2 >= target_low && s2 < target_high)) return UNSURE;
+      const bool left = s1 >= target && m > b1, right = s2 < target && m < b2;
+      if (!left && !right) return order_list<false>(n, 0, target_low, target_high, s1, cut) ? CUT : UNSURE;
+      if (left) b2 = m - 1;
+      else b1 = m + 1;
+      // the first bin with tokens from b1 on that reaches the target, or the last one with tokens up to b2
+      const double off = s2 - estimate;
+      if (threadIdx.x == 0) {
+        sh.found[0] = BINS;
+        sh.found[1] = 0;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < BINS_PER_THREAD; ++k) {
+        const unsigned int b = threadIdx.x * BINS_PER_THREAD + k;
+        if (count[k] && b >= b1 && b <= b2) {
+          if (mid[k] + off >= target) atomicMin(&sh.found[0], b);
+          atomicMax(&sh.found[1], b);
+        }
+      }
+      __syncthreads();
+      m = sh.found[0] < BINS ? sh.found[0] : sh.found[1];
+    }
+  }
+
   template <bool BY_COUNT>
   __device__ __noinline__ Found find(double target, double slack, Cut& cut) {
     const double target_low = target * (1.0 - slack), target_high = target * (1.0 + slack);
@@ -644,8 +708,26 @@ struct Sampler {
         m = reaches(buffer, goal);
         if (first && m >= BINS - 1) return NONE;
         above = sh.found[1];
+        if (first && sh.found[2] <= LIST) {
+          const unsigned int n = sh.found[2];
+          if (threadIdx.x == 0) sh.listed = 0;
+          __syncthreads();
+          each([&](unsigned int i, const float (&f)[M]) {
+#pragma unroll
+            for (int j = 0; j < M; ++j)
+              if (w.bin(f[j]) == m) append(f[j], i + j);
+          });
+          return order_list<true>(n, goal - above, 0.0, 0.0, 0.0, cut) ? CUT : UNSURE;
+        }
       } else {
-        if (!bracket(buffer, first, lo, hi, shift, mass, target_low, target, target_high, b1, m, b2)) return NONE;
+        double mid[BINS_PER_THREAD];
+        unsigned int count[BINS_PER_THREAD];
+        if (!bracket(buffer, first, lo, hi, shift, mass, target_low, target, target_high, b1, m, b2, mid, count)) return NONE;
+        if (first) {
+          bool done;
+          const Found found = by_bins(target_low, target, target_high, b1, m, b2, mid, count, cut, done);
+          if (done) return found;
+        }
         __syncthreads();
         if (threadIdx.x == 0) sh.found[2] = sh.bins[buffer][m];
       }
@@ -921,8 +1003,9 @@ struct Sampler {
     __syncthreads();
     for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) sh.bins[0][i] += sh.bins[1][i] + sh.bins[2][i];
     __syncthreads();
-    unsigned int b1, m, b2;
-    if (!bracket(0, true, 0, 0, 0, 0.0, target * (1.0 - SLACK), target, target * (1.0 + SLACK), b1, m, b2)) return lowest;
+    unsigned int b1, m, b2, count[BINS_PER_THREAD];
+    double mid[BINS_PER_THREAD];
+    if (!bracket(0, true, 0, 0, 0, 0.0, target * (1.0 - SLACK), target, target * (1.0 + SLACK), b1, m, b2, mid, count)) return lowest;
     __syncthreads();
     expected = sh.found[3];
     return fmax(lowest, -w.bin_end(b2));

@@ -8,6 +8,10 @@
 // Elements of all tensors are cut into units of UNIT_BYTES, and every block takes an equal share of neighbouring units, whichever tensors they
 // lie in (a binary search over the first units of the tensors, which are kernel parameters), and leaves one fp64 sum; each block of the second
 // kernel adds all blocks' sums in the same order, so that equal inputs give equal bits.
+//
+// Measured on one B200 (a copy reaches 6.56 TB/s): 8 x 4096 x 4096 bf16 within the limit 46 us, 5.8 TB/s; scaled into other tensors 138 us for three passes of 268 MB (5.8
+// TB/s, some of the second from the L2 cache; forwards instead of backwards 141, and 55 for 49.5 us with three matrices). 5 x 1024 x 1024 fp32 scaled 18 us: two
+// kernels of 7 and 8 us, of which each is 3 us of launch, reduction and end.
 #include <math.h>
 
 #include <algorithm>
@@ -30,7 +34,8 @@ struct ClipTensor {
   unsigned long long size, cols, ld_x, ld_out;  // elements
   unsigned int f32, gaps;                       // gaps: rows with gaps between them; otherwise one piece of `size` elements
 };
-// Kernel parameters: up to MOST tensors. Two sizes, because a launch takes longer with more of them (28 KB of the 32 KB that there are).
+// Kernel parameters: up to MOST tensors. Two sizes, because a launch takes longer with more of them (28 KB of the 32 KB that there are): 5 tensors take 7.1 us of the
+// caller's time for 8.5.
 template <int MOST>
 struct ClipList {
   ClipTensor t[MOST];

@@ -6,6 +6,10 @@
 // Both are bound by HBM: every matrix is read or written once. A row is held in registers by a group of threads, from 1 to a block of
 // 1024, each with K vectors at distances of the group, so that the row's sum of squares is one reduction between the load and the store.
 // The gradient needs no statistics of the forward pass: mean(t^2) and mean(g t) are reduced together.
+//
+// Measured on one B200 (a copy reaches 6.56 TB/s): 65536 x 1024 bf16 with residual and fp32 weight 85 us, 6.3 TB/s; its gradients 101 us, 5.3 TB/s (63 % of issue slots;
+// two kernels); 8192 x 4096 bf16 with residual to e4m3 47 us, 5.0 TB/s (73 % of issue slots: the largest magnitude, the quotient mended and rounded per element); one row of
+// 4096 2.5 us.
 #include <cuda_fp8.h>
 
 #include "lm.cuh"
@@ -571,7 +575,9 @@ struct RowForm {
   int g_log2, k, threads;
   int g() const { return 1 << g_log2; }
 };
-// most_k: vectors that a thread may hold. few: rows times threads below this leave the GPU partly idle, so that more threads share a row.
+// most_k: vectors that a thread may hold; the fewest threads that hold a row leave the most loads in flight and the fewest threads to reduce over (65536 x 1024 bf16 with 4, 2
+// and 1 vectors 85, 86 and 94 us; 8192 x 4096 to e4m3 47, 52 and 57). few: rows times threads below this leave the GPU partly idle, so that more threads share a row (1 x
+// 4096 bf16 2.5 us for 3.3, 600 x 1024 2.9 for 3.7).
 RowForm row_form(size_t rows, int vecs, int most_k, int least_g, int most_g, size_t few) {
   RowForm f{0, 0, 0};
   while (f.g() < least_g || (f.g() < most_g && (size_t)f.g() * most_k < (size_t)vecs)) ++f.g_log2;
@@ -650,6 +656,7 @@ int grad_rows(const NormGradArgs& a, const RowForm& f, int sms, Chain& chain) {
 template <typename T, int VB>
 void norm_grad_launch(const NormGradArgs& a, double* rms_of, void* dweight, int sms, Chain& chain) {
   constexpr int N = VB / (int)sizeof(T), MOST_K = N >= 8 ? 4 : 8;
+  // two vectors per thread share the row's reduction and leave registers for the next row's loads (65536 x 1024 bf16 101 us, with one 118, with four and no loads ahead 217);
   // 1024 threads have 64 registers each: half as many elements
   RowForm f = row_form(1, a.width / N, 2, 1, NORM_THREADS, 0);
   if (!f.k) f = row_form(1, a.width / N, MOST_K, 1, NORM_THREADS, 0);

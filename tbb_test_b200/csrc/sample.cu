@@ -236,7 +236,7 @@ struct FastWeights {
     n = rintf(largest * t.c);
     magic = 12582912.f - n;  // 1.5 * 2^23: the sum's low bits are n of x c less N
     least = largest - t.reach;
-    usable = t.usable && fabsf(n) < 262144.f;
+    usable = t.usable && fabsf(n) < 131072.f;  // x c_low is below 2^-7: r stays in +-0.51
   }
   __device__ __forceinline__ float of(float f) const {
     f = fmaxf(f, least);
@@ -343,7 +343,6 @@ struct Cut {
   float value;
   unsigned int ties, equal;
 };
-
 
 __device__ __forceinline__ double warp_sum(double s) {
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
@@ -870,7 +869,7 @@ struct Sampler {
   }
 
   // The token from the n listed ones, which hold all that are kept. mass: of all tokens that top_p counts, where it is not that of the first top_k; it may be
-  // off by SLACK.
+  // off by SLACK_OF_ONE.
   __device__ __forceinline__ void choose(unsigned int n, const SampleRow& ask, double mass, double u) {
     order(n);
     const unsigned int t = threadIdx.x, number = t < n ? (unsigned int)sh.ordered[t] : 0xFFFFFFFFu;
@@ -1015,11 +1014,12 @@ struct Sampler {
     return fmax(lowest, -w.bin_end(b2));
   }
 
-  // The tokens of at least `floor` where few are expected: how many there are, the first LIST that come listed with their numbers for places.
+  // The tokens of at least `floor` where few are expected, listed with their numbers for places: how many there are, or some number above LIST where there are more.
   __device__ __forceinline__ unsigned int gather_few() {
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
     each_of_row(floor, [&](unsigned int i, const float (&f)[M]) {
+      if (*(volatile unsigned int*)&sh.listed > LIST) return;
 #pragma unroll
       for (int j = 0; j < M; ++j)
         if (f[j] >= floor) {

@@ -131,8 +131,12 @@ std::pair<void*, int> weight_of(PyObject* w, const at::Tensor& x) {
 }
 
 template <class Body>
-PyObject* guarded(Body body) {
+PyObject* guarded(Py_ssize_t given_args, Py_ssize_t wanted, Body body) {
   try {
+    if (given_args != wanted) {
+      PyErr_Format(PyExc_TypeError, "%zd arguments, %zd wanted", given_args, wanted);
+      throw Raised();
+    }
     return body();
   } catch (const Raised&) {
   } catch (const std::exception& e) {
@@ -142,8 +146,8 @@ PyObject* guarded(Body body) {
 }
 
 // x, weight, residual, eps, total, out, block (None: an output of x's type)
-PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t) {
-  return guarded([&]() -> PyObject* {
+PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded(n_args, 7, [&]() -> PyObject* {
     const at::Tensor& x = tensor("x", a[0]);
     const Matrix mx = matrix("x", x);
     const auto [pw, wt] = weight_of(a[1], x);
@@ -184,8 +188,8 @@ PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t) {
 }
 
 // dy, t, weight, dtotal, eps, dx
-PyObject* norm_grad(PyObject*, PyObject* const* a, Py_ssize_t) {
-  return guarded([&]() -> PyObject* {
+PyObject* norm_grad(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded(n_args, 6, [&]() -> PyObject* {
     const at::Tensor& dy = tensor("dy", a[0]);
     const Matrix md = matrix("dy", dy), mt = matrix("t", tensor("t", a[1]), &dy);
     const auto [pw, wt] = weight_of(a[2], dy);
@@ -245,8 +249,8 @@ std::vector<at::Tensor> listed(const char* name, PyObject* x) {
 }
 
 // tensors, max_norm, out
-PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t) {
-  return guarded([&]() -> PyObject* {
+PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded(n_args, 3, [&]() -> PyObject* {
     const std::vector<at::Tensor> xs = listed("tensors", a[0]);
     if (xs.empty()) refuse("tensors: none");
     const double limit = given(a[1]) ? number(a[1]) : std::numeric_limits<double>::infinity();
@@ -315,8 +319,8 @@ const V* per_row(const char* name, PyObject* x, at::ScalarType type, const char*
 }
 
 // logits, u, temperature, top_k, top_p, min_p, logprob, out
-PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t) {
-  return guarded([&]() -> PyObject* {
+PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded(n_args, 8, [&]() -> PyObject* {
     const at::Tensor& logits = tensor("logits", a[0]);
     const Matrix m = matrix("logits", logits);
     const auto floats = [&](const char* name, PyObject* x) { return per_row<float>(name, x, at::kFloat, "float32", logits); };

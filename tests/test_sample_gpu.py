@@ -112,6 +112,29 @@ def test_large_vocabularies(lm, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("kind", ["flat", "peaked", "part_light", "part_light_peaked", "part_heavy", "equal", "masked", "lowest"])
+def test_top_p_over_long_rows(lm, dtype, kind):
+    """Where a part of the row (every eighth warp's vectors) says how far down top-p reaches: rows that it tells well, and rows whose part is unlike the rest."""
+    x, u = _logits(5, 70001, dtype, 5, 0.0 if kind == "equal" else 6.0 if "peaked" in kind else 2.0, 70008)
+    part = torch.arange(70001, device="cuda") // (32 * 16 // x.element_size()) % 8 == 0
+    if "part" in kind:
+        x[:, part if "light" in kind else ~part] -= 30.0
+    if kind in ("masked", "lowest"):
+        x[:, torch.rand(70001, device="cuda", generator=torch.Generator(device="cuda").manual_seed(6)) < 0.4] = -math.inf if kind == "masked" else torch.finfo(dtype).min
+    for s in (dict(p=0.3), dict(p=0.9), dict(p=0.999), dict(p=0.9, m=0.03), dict(p=0.97, m=1e-4, t=1.5), dict(p=[0.2, 0.5, 0.8, 0.99, 1.0], t=[0.3, 0.7, 1.0, 2.0, 5.0])):
+        _check(lm, x, u, **s, exact=kind == "equal")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_top_p_of_many_flat_rows(lm, dtype):
+    """With tokens this light the row's weight in fp32 leaves some rows open."""
+    x, u = _logits(200, 33001, dtype, 7, 1.5)
+    _check(lm, x, u, p=0.9)
+
+
+@pytest.mark.gpu
 def test_rows_that_no_shared_memory_holds(lm):
     """2^21 logits in fp32 are read from device memory again for each pass."""
     x, u = _logits(1, (1 << 21) + 5, torch.float32, 3, 1.0)

@@ -1339,7 +1339,7 @@ struct Sampler {
     Cut cut{-INFINITY, 0, 0};
     double all = 0.0, slack = SLACK_OF_ONE;
     if (!ask.by_k && !ask.by_p && !ask.by_m) {
-      if (from_tiles(ask, true, u, all)) return;
+      if (!a.logprob && from_tiles(ask, true, u, all)) return;  // a logarithm near 0 needs more than fp32 sums
       share(row.end);
       by_sums(cut, 0.0, u);
       return;
@@ -1547,7 +1547,22 @@ __global__ void __launch_bounds__(WHOLE_THREADS) sample_whole_kernel(const Sampl
         });
         sure = found && goal - before > SLACK * goal && before + weight - goal > SLACK * goal;
       }
-      if (sure) write(place - row.shift, (float)(w.exponent(logit) - log(total * fast.to_top(w))));
+      double all = total * fast.to_top(w);
+      if (a.logprob && usable) {
+        // the largest token's tile in fp64: where it has most of the weight the logarithm is near 0, and what fp32 is off would be much of it
+        const unsigned int most = __reduce_min_sync(0xFFFFFFFFu, own == top ? first : 0xFFFFFFFFu);
+        double exact = 0.0;
+#pragma unroll
+        for (int k = 0; k < PER_LANE / N; ++k) {
+          float f[N];
+          Elems<T, 16>::get(row.load_vector(most * TILE + (k * 32 + lane) * N), f);
+#pragma unroll
+          for (int j = 0; j < N; ++j) exact += w.of(fmaxf(f[j], -INFINITY));
+        }
+        for (int o = 16; o; o >>= 1) exact += __shfl_xor_sync(0xFFFFFFFFu, exact, o);
+        all += exact - stats[most].weight * fast.unit(stats[most].largest) * fast.to_top(w);
+      }
+      if (sure) write(place - row.shift, (float)(w.exponent(logit) - log(all)));
       else if (lane == 0) a.open[atomicAdd(a.open_count, 1u)] = (unsigned int)r;
     }
   }
@@ -1615,7 +1630,8 @@ size_t sample_space(size_t rows, size_t vocab, void* base, SampleArgs* a) {
   return c.used;
 }
 
-// Rows of at least so many tiles are estimated from a part: 256 rows of 32768 with a spread of 4 and top-p 0.99 104 -> 99 us, of 16384 with a spread of 2 and top-p 0.5 65 -> 72.
+// Rows of at least so many tiles are estimated from a part: 256 rows with top-p 0.99, 32768 with a spread of 4 104 -> 82 us, 24576 92 -> 78; but 16384 with a spread of 2
+// and top-p 0.9 76 -> 87, 8192 66 -> 71.
 constexpr unsigned int PART_TILES = 32;
 
 template <typename T>

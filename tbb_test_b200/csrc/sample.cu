@@ -165,7 +165,7 @@ struct Weights {
   double wide_top, inv_t, steps;     // steps: 16 log2(e) / T
   double reach;                      // -693 T: weights of 2^-1000
   const double* powers;              // in shared memory
-  float least;                       // logits below it weigh nothing: less than 2^-1000, -inf
+  float least;                       // logits below it weigh nothing: less than 2^-1000, -inf. Rounded up: one below top + reach is outside of sixteenths()'s range
   float half_top, per_bin;           // per_bin: bins for each 2 of the logit
   bool plain;                        // what widened() makes of small numbers and infinities does not matter
 
@@ -176,7 +176,7 @@ struct Weights {
     inv_t = 1.0 / (double)t;
     reach = -693.0 * (double)t;
     steps = STEPS * 1.4426950408889634 * inv_t;
-    least = top == INFINITY ? top : (float)fmax((double)top + reach, -3.4028234663852886e38);
+    least = top == INFINITY ? top : __double2float_ru(fmax((double)top + reach, -3.4028234663852886e38));
     half_top = 0.5f * top;
   }
   // Bins that reach `span` below the top, in units of T; the last one has all that is lower.

@@ -288,3 +288,33 @@ def test_c_entry_refuses_before_any_device_work(native):
     need = ct.c_size_t()
     assert lib.b2_sample_workspace(2, 8, ct.byref(need)) == K.OK and need.value > 0
     assert lib.b2_sample_workspace(2, 8, None) == lib.b2_sample_workspace(2, 0, ct.byref(need)) == K.ERR_INVALID
+
+
+def _check_both(lm, logits, u, **settings):
+    """_check, and the same tokens by the calls without log probabilities, which go another way for rows without a limit."""
+    tokens, _ = _check(lm, logits, u, **settings)
+    dev = lambda v, d: torch.tensor(v, dtype=d, device="cuda") if isinstance(v, list) else v  # noqa: E731
+    f = torch.float32
+    again = lm.sample(logits, u, dev(settings.get("t", 1.0), f), dev(settings.get("k", 0), torch.int32), dev(settings.get("p", 1.0), f), dev(settings.get("m", 0.0), f))
+    assert torch.equal(again, tokens)
+    return tokens
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab,ld,offset", [(300, 300, 0), (9001, 9003, 1), (70001, 70002, 3)])
+def test_logits_a_few_steps_of_fp32_below_the_largest_at_a_tiny_temperature(lm, vocab, ld, offset):
+    """Differences of 1 to 24 steps of fp32 with temperatures of a 1400th to a 30th of a step: most weights are below the smallest number of any type."""
+    g = torch.Generator(device="cuda").manual_seed(12)
+    tops, shares = [1.0, 12.0, 100.0, 1000.0, -1.0, -700.0], [1400.0, 700.0, 350.0, 100.0, 30.0, 1000.0]
+    step = [2.0 ** (math.frexp(abs(v) * (1 - 2.0 ** -30))[1] - 24) for v in tops]  # of the numbers next to it that are smaller in size: finer at powers of two
+    x, u = _logits(6, vocab, torch.float32, 12, 0.0, ld, offset)
+    below = torch.randint(1, 25, (6, vocab), device="cuda", generator=g).double() * 2  # even: numbers larger in size than a power of two lie twice as far apart
+    exact = torch.tensor(tops, device="cuda", dtype=torch.float64)[:, None] - below * torch.tensor(step, device="cuda", dtype=torch.float64)[:, None]
+    assert torch.equal(exact.float().double(), exact)
+    x.copy_(exact)
+    x[:, torch.randint(0, vocab, (3,), device="cuda", generator=g)] = torch.tensor(tops, device="cuda")[:, None]
+    for turn in range(6):
+        t = [step[i] / shares[(i + turn) % 6] for i in range(6)]
+        for s in (dict(), dict(k=2), dict(k=600), dict(p=0.9), dict(k=700, p=0.97), dict(m=1e-30)):
+            tokens = _check_both(lm, x, u, t=t, **s, exact=True)
+            assert bool(((tokens >= 0) & (tokens < vocab)).all())

@@ -213,6 +213,12 @@ struct Weights {
 // three additions. Two such sums are compared: SLACK is twice that and a third more.
 constexpr double SLACK = 9.5367431640625e-7;          // 2^-20
 constexpr double SLACK_OF_ONE = 4.76837158203125e-7;  // 2^-21: such a sum against an exact one
+// Whether the token whose own weight lies between `before` and `before + weight` is the one at `goal` for sure, all relative to its tile's unit. Logits of less than 80 T below a
+// tile's largest, -inf among them, and places that are not in the row weigh some 2^-115 each in fp32 instead of less or nothing, below 2^-104 per tile: goals above
+// 2^-80 have a slack of more than that (2^-100), and the smaller ones, which take a u of less than 1e-23, are left open.
+__device__ __forceinline__ bool for_sure(double before, double weight, double goal) {
+  return goal > 8.271806125530277e-25 && goal - before > SLACK * goal && before + weight - goal > SLACK * goal;
+}
 __device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
   float2 d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;"
@@ -1020,7 +1026,7 @@ struct Sampler {
 #pragma unroll
           for (int j = 0; j < N; ++j) x[j] = tile.of(f[j]);
         });
-        if (found && goal - before > SLACK * goal && before + weight - goal > SLACK * goal && lane == 0) {
+        if (found && for_sure(before, weight, goal) && lane == 0) {
           write(place - row.shift, logit, total * to_top);
           sh.found[0] = 1;
         }
@@ -1545,7 +1551,7 @@ __global__ void __launch_bounds__(WHOLE_THREADS) sample_whole_kernel(const Sampl
 #pragma unroll
           for (int j = 0; j < N; ++j) x[j] = own_unit.of(f[j]);
         });
-        sure = found && goal - before > SLACK * goal && before + weight - goal > SLACK * goal;
+        sure = found && for_sure(before, weight, goal);
       }
       double all = total * fast.to_top(w);
       if (a.logprob && usable) {

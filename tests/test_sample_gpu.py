@@ -318,3 +318,20 @@ def test_logits_a_few_steps_of_fp32_below_the_largest_at_a_tiny_temperature(lm, 
         for s in (dict(), dict(k=2), dict(k=600), dict(p=0.9), dict(k=700, p=0.97), dict(m=1e-30)):
             tokens = _check_both(lm, x, u, t=t, **s, exact=True)
             assert bool(((tokens >= 0) & (tokens < vocab)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("vocab,ld,offset", [(40, 41, 1), (3000, 3007, 3), (70001, 70003, 5)])
+def test_tiny_numbers_never_take_a_masked_token(lm, dtype, vocab, ld, offset):
+    """u down to fp32's smallest number, with masks and unaligned beginnings ahead of the first token that may be taken; rows with a limit beside ones without."""
+    x, _ = _logits(8, vocab, dtype, 13, 2.5, ld, offset)
+    x[0, 0] = x[1, :17] = x[2, :vocab - 3] = -math.inf
+    x[3, :9] = math.nan
+    x[4, :20] = torch.finfo(dtype).min
+    x[5, :30] = -90.0  # weighs something, but less than fp32 weights tell
+    x[6, 0] = x[0].max() - 79.0
+    for value in (0.0, 1e-45, 1e-40, 1e-38, 1e-36, 2.3e-35, 1e-34, 1e-32, 1e-30, 1e-26, 1e-22, 1e-17, 2.0 ** -24):
+        u = torch.full((8,), value, device="cuda")
+        for s in (dict(), dict(t=0.5), dict(k=[0] * 7 + [3]), dict(p=[1.0] * 7 + [0.9], m=[0.0, 1e-20] * 4)):
+            _check_both(lm, x, u, **s, exact=True)

@@ -39,7 +39,7 @@ constexpr int TILE_THREADS = 256, TILE = 1024, PER_LANE = TILE / 32;
 constexpr int BINS = 1024, BINS_PER_THREAD = BINS / SAMPLE_THREADS;
 constexpr int LIST = SAMPLE_THREADS;  // tokens that are put in order one by one
 constexpr int STEPS = 16;             // 2^(n / 16) for n = 0 to 15 lie in different banks of shared memory
-constexpr double REACH = 40.0;        // in units of T: what weighs less than e^-40 of the largest weighs nothing where a limit is looked for
+constexpr double REACH = 40.0;        // in units of T: what weighs less than e^-40 of the largest weighs nothing where top-p's limit is looked for
 
 struct TileStat {
   double weight;  // of its tokens relative to 2^rint(largest * c), see FastWeights; negative: not to be had in fp32
@@ -671,9 +671,7 @@ struct Sampler {
     return true;
   }
 
-  // The cut at which `target` tokens (BY_COUNT) or `target` weight is reached. The first bins have been counted.
-  // False: it is not reached before the tokens that weigh nothing.
-  // The first bins' part of it for weights, while bins have few tokens: exact sums up to the ends of some bins around the estimated one say whether the limit is in them,
+  // find()'s part in the first bins for weights, while bins have few tokens: exact sums up to the ends of some bins around the estimated one say whether the limit is in them,
   // and what all estimates are off by there, so that the next ones are hardly ever wrong. Where the weight of all counted tokens is known, the first one is
   // corrected, too: what it is off comes from the heavy tokens. Without it half of the rows needed a second pass. False: bin m has too many tokens.
   static constexpr unsigned int BESIDE = 48;
@@ -764,6 +762,8 @@ struct Sampler {
     }
   }
 
+  // The cut at which `target` tokens (BY_COUNT) or `target` weight is reached. The first bins have been counted.
+  // False: there are not so many tokens; the weight is not reached before the tokens that weigh nothing.
   template <bool BY_COUNT>
   __device__ __noinline__ bool find(Target target, Cut& cut) {
     unsigned int lo = 0, hi = key_of(w.top), shift = 0;  // the window's keys
@@ -778,7 +778,7 @@ struct Sampler {
       unsigned int b1 = 0, b2 = 0, m = 0, above = 0;
       if constexpr (BY_COUNT) {
         m = reaches(buffer, goal);
-        if (first && m >= BINS - 1) return false;
+        if (m >= BINS) return false;  // no more tokens than that
         above = sh.found[1];
         if (first && sh.found[2] <= LIST) {
           const unsigned int n = sh.found[2];
@@ -787,7 +787,7 @@ struct Sampler {
           each([&](unsigned int i, const float (&f)[M]) {
 #pragma unroll
             for (int j = 0; j < M; ++j)
-              if (w.bin(f[j]) == m) append(f[j], i + j);
+              if (f[j] > -INFINITY && w.bin(f[j]) == m) append(f[j], i + j);
           });
           order_list<true>(n, goal - above, target, 0.0, cut);
           return true;
@@ -803,7 +803,8 @@ struct Sampler {
       for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) sh.bins[next][i] = 0;
       if (threadIdx.x == 0) sh.listed = 0;
       __syncthreads();
-      const unsigned int n = sh.found[2], key_lo = edge_of(m, false), key_hi = without_minus_zero(edge_of(m, true));
+      // the last one of the first bins has no lower end
+      const unsigned int n = sh.found[2], key_lo = max(edge_of(m, false), key_of(-3.4028234663852886e38f)), key_hi = without_minus_zero(edge_of(m, true));
       if constexpr (BY_COUNT) goal -= above;  // of the bin's
       const bool one = key_lo == key_hi, listed = !one && n <= LIST;
       unsigned int new_shift = 0;

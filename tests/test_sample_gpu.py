@@ -335,3 +335,21 @@ def test_tiny_numbers_never_take_a_masked_token(lm, dtype, vocab, ld, offset):
         u = torch.full((8,), value, device="cuda")
         for s in (dict(), dict(t=0.5), dict(k=[0] * 7 + [3]), dict(p=[1.0] * 7 + [0.9], m=[0.0, 1e-20] * 4)):
             _check_both(lm, x, u, **s, exact=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("vocab,ld,offset", [(9001, 9003, 1), (40000, 40000, 0)])
+@pytest.mark.parametrize("k", [5, 50, 511, 700, 3000])
+def test_top_k_among_tokens_of_hardly_any_weight(lm, dtype, vocab, ld, offset, k):
+    """Temperatures at which the k-th token weighs e^-40 to e^-690 of the first one: with u = 0 the token is the first kept one by number, whatever it weighs. Other rows have fewer
+    tokens than k that are not masked, or thousands of equal ones at the limit."""
+    x, _ = _logits(6, vocab, dtype, 14, 0.5, ld, offset)
+    x[4, k // 2:] = -math.inf
+    x[5].copy_((x[5].float() * 8).round() / 8)
+    x[:, vocab // 2] = x.nan_to_num(neginf=-9.0).amax(1) + torch.tensor([0.0, 0.5, 1.0, 1.5, 0.5, 1.0], device="cuda").to(dtype)
+    x[4, 0] = x[4, vocab // 2] - 3.0
+    for value in (0.0, -1.0, 0.3):
+        u = torch.full((6,), value, device="cuda")
+        for s in (dict(t=0.01), dict(t=0.005), dict(t=0.01, p=0.9), dict(t=0.01, m=1e-30), dict(t=[0.01, 0.008, 0.02, 0.01, 0.01, 0.04])):
+            _check_both(lm, x, u, k=k, **s, exact=True)

@@ -475,7 +475,7 @@ int b2_norm_grad(size_t rows, size_t width, int dtype, const void* dy, size_t ld
  * x[i] and out[i] have elements[i] elements of dtypes[i] (types may be mixed), one behind the other: tensors of any shape without gaps. Where widths is
  * not NULL, x[i] and out[i] are matrices of rows of widths[i] elements (a divisor of elements[i]), ld_x[i] and ld_out[i] elements apart. out = NULL, or an
  * out[i] that is x[i] with the same leading dimension, is in place, where nothing is written unless the norm is over the limit. norm (device memory) is
- * always written; max_norm = INFINITY asks for nothing else, and out has to be NULL then. A norm that is infinite or not a number leaves the
+ * always written; max_norm = INFINITY asks for nothing else, and out has to be NULL then. A norm that is infinite in fp32 or not a number leaves the
  * values as they are: the caller sees it in `norm`. Elements are squared, summed and scaled in fp32 and fp64 over the whole range of fp32 and rounded
  * once. The lists are host arrays, read during the call. Equal inputs give equal bits on equal devices. Limits: 2^20 tensors, 2^42 elements together. */
 int b2_clip_workspace(size_t count, size_t* bytes);

@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(CLIP_THREADS, 2) clip_scale_kernel(const __gri
   for (int i = threadIdx.x; i < partials; i += CLIP_THREADS) sum += partial[i];
   const double norm = sqrt(block_sum(sum, slots));
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
-  const bool over = norm > (double)max_norm && norm <= 1.7976931348623157e308;  // an infinite norm, or none, leaves the tensors as they are
+  const bool over = norm > (double)max_norm && (float)norm < INFINITY;  // a norm that is reported as infinite, or none, leaves the tensors as they are
   if (in_place && !over) return;
   const float factor = over ? (float)((double)max_norm / norm) : 1.f;
   unsigned int begin, u;

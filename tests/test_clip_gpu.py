@@ -214,3 +214,15 @@ def test_c_entry_refuses_before_any_device_work(native):
     need = ct.c_size_t()
     assert lib.b2_clip_workspace(700, ct.byref(need)) == K.OK and need.value > 0
     assert lib.b2_clip_workspace(1, None) == lib.b2_clip_workspace((1 << 20) + 1, ct.byref(need)) == K.ERR_INVALID
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_a_norm_beyond_fp32_is_infinite_and_changes_nothing(lm, dtype):
+    """Two elements of 3e38: each is finite, their norm is not in fp32. One of 3e38 beside it is clipped as ever."""
+    xs = [torch.tensor([3e38, 1.0], device="cuda").to(dtype), torch.tensor([-2.0, 3e38, 5.0], device="cuda").to(dtype)]
+    before, outs = [x.clone() for x in xs], [torch.zeros_like(x) for x in xs]
+    for norm in (lm.clip(xs, 1.0), lm.clip(xs, 1.0, out=outs), lm.clip(xs, None)):
+        assert math.isinf(float(norm))
+    assert all(torch.equal(x, b) and torch.equal(o, b) for x, o, b in zip(xs, outs, before))
+    _check(xs[:1], before[:1], lm.clip(xs[:1], 1e38), 1e38)

@@ -476,8 +476,8 @@ int b2_norm_grad(size_t rows, size_t width, int dtype, const void* dy, size_t ld
  * not NULL, x[i] and out[i] are matrices of rows of widths[i] elements (a divisor of elements[i]), ld_x[i] and ld_out[i] elements apart. out = NULL, or an
  * out[i] that is x[i] with the same leading dimension, is in place, where nothing is written unless the norm is over the limit. norm (device memory) is
  * always written; max_norm = INFINITY asks for nothing else, and out has to be NULL then. A norm that is infinite in fp32 or not a number leaves the
- * values as they are: the caller sees it in `norm`. Elements are squared, summed and scaled in fp32 and fp64 over the whole range of fp32 and rounded
- * once. The lists are host arrays, read during the call. Equal inputs give equal bits on equal devices. Limits: 2^20 tensors, 2^42 elements together. */
+ * values as they are: the caller sees it in `norm`. Elements are squared and summed in fp32 and fp64 over the whole range of fp32. The factor is rounded
+ * to fp32 (below 2^-126 it stays in fp64), the product once more. The lists are host arrays, read during the call. Equal inputs give equal bits on equal devices. Limits: 2^20 tensors, 2^42 elements together. */
 int b2_clip_workspace(size_t count, size_t* bytes);
 int b2_clip(size_t count, const void* const* x, void* const* out, const size_t* elements, const int* dtypes,
             const size_t* widths, const size_t* ld_x, const size_t* ld_out, float max_norm, float* norm, void* workspace,

@@ -202,12 +202,18 @@ __device__ __forceinline__ void scale_dense(const T* x, T* out, int n, float fac
   else scale_from<T, sizeof(T)>(x, out, n, 0, factor);
 }
 
-template <typename T>
-__device__ __forceinline__ void scale_rows(const ClipTensor& t, unsigned long long from, int n, float factor) {
+// Of a matrix with gaps between its rows; with a factor in fp64 of any tensor.
+template <typename T, typename F>
+__device__ __forceinline__ void scale_rows(const ClipTensor& t, unsigned long long from, int n, F factor) {
   for (int i = threadIdx.x; i < n; i += CLIP_THREADS) {
     const unsigned long long at = from + i, row = at / t.cols, col = at - row * t.cols;
-    reinterpret_cast<T*>(t.out)[row * t.ld_out + col] = (T)((float)reinterpret_cast<const T*>(t.x)[row * t.ld_x + col] * factor);
+    reinterpret_cast<T*>(t.out)[row * t.ld_out + col] = (T)(float)((F)(float)reinterpret_cast<const T*>(t.x)[row * t.ld_x + col] * factor);
   }
+}
+
+__device__ __noinline__ void scale_far(const ClipTensor& t, unsigned long long from, int n, double factor) {
+  if (t.f32) scale_rows<float>(t, from, n, factor);
+  else scale_rows<__nv_bfloat16>(t, from, n, factor);
 }
 
 // in_place: nothing is written where nothing is over the limit. norm: of the first launch of a call only.
@@ -223,7 +229,9 @@ __global__ void __launch_bounds__(CLIP_THREADS, 2) clip_scale_kernel(const __gri
   if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
   const bool over = norm > (double)max_norm && (float)norm < INFINITY;  // a norm that is reported as infinite, or none, leaves the tensors as they are
   if (in_place && !over) return;
-  const float factor = over ? (float)((double)max_norm / norm) : 1.f;
+  const double exact = over ? (double)max_norm / norm : 1.0;
+  const float factor = (float)exact;
+  const bool far = exact > 0.0 && exact < 1.1754943508222875e-38;  // fp32 has no such factor, or not with all of its bits; limits so far below the norm are rare: one element at a time
   unsigned int begin, u;
   share(list, begin, u);
   while (u > begin) {
@@ -233,7 +241,9 @@ __global__ void __launch_bounds__(CLIP_THREADS, 2) clip_scale_kernel(const __gri
     const ClipTensor& t = list.t[k];
     const ClipPart p = part_of(list, k, from, u);
     const int n = (int)p.n;
-    if (t.gaps) {
+    if (far) {
+      scale_far(t, p.from, n, exact);
+    } else if (t.gaps) {
       if (t.f32) scale_rows<float>(t, p.from, n, factor);
       else scale_rows<__nv_bfloat16>(t, p.from, n, factor);
     } else if (t.f32) {

@@ -226,3 +226,25 @@ def test_a_norm_beyond_fp32_is_infinite_and_changes_nothing(lm, dtype):
         assert math.isinf(float(norm))
     assert all(torch.equal(x, b) and torch.equal(o, b) for x, o, b in zip(xs, outs, before))
     _check(xs[:1], before[:1], lm.clip(xs[:1], 1e38), 1e38)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("scale,limit", [(1e30, 1e-12), (1e30, 1e-16), (1e36, 1e-6), (3e30, 1e-35), (1e-3, 1e-44), (1e20, 1e-17), (1.0, 1e-38)])
+def test_limits_far_below_the_norm(lm, dtype, scale, limit):
+    """Factors that fp32 has not, or not with all of its bits, among dense tensors and matrices with gaps, in place and not. Results below the type's normal numbers are off by
+    up to half of its smallest step; through fp32, bf16 by half of fp32's more."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    buf = (torch.randn(70, 50, device="cuda", generator=g).clamp(-3, 3) * scale).to(dtype)
+    xs = [buf[:, :33], (torch.randn(5003, device="cuda", generator=g).clamp(-3, 3) * scale).to(dtype)[1:], buf[3:4, 40:41]]
+    before, rest = [x.clone() for x in xs], buf[:, 41:].clone()
+    limit = float(torch.tensor(limit))
+    outs = [torch.full_like(x, 7) for x in xs]
+    norm = lm.clip(xs, limit, out=outs)
+    assert torch.equal(lm.clip(xs, limit), norm) and all(torch.equal(x, o) for x, o in zip(xs, outs)) and torch.equal(buf[:, 41:], rest)
+    want = _norm(before)
+    assert abs(float(norm) - want) <= 5 * U * want
+    least = 2.0 ** -150 if dtype == torch.float32 else 2.0 ** -134 + 2.0 ** -150
+    for o, b in zip(outs, before):
+        exact = b.double() * (limit / want)
+        assert bool(((o.double() - exact).abs() <= exact.abs() * (6 * U + torch.finfo(dtype).eps / 2) + least).all())

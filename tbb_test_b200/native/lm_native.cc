@@ -256,6 +256,8 @@ PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const double limit = given(a[1]) ? number(a[1]) : std::numeric_limits<double>::infinity();
     if (!(limit >= 0.0)) refuse("max_norm: negative or not a number");
     const bool limited = limit <= std::numeric_limits<double>::max();
+    // the same as any limit that fp32 has not: norms beyond it leave the values as they are
+    const float most = std::numeric_limits<float>::max(), max_norm = !limited ? std::numeric_limits<float>::infinity() : limit < most ? (float)limit : most;
     const bool apart = given(a[2]);
     std::vector<at::Tensor> ys;
     if (apart) {
@@ -300,7 +302,7 @@ PyObject* clip(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const at::Tensor ws = workspace(need, device);
     check(without_gil([&] {
       return p_clip(n, px.data(), apart ? py.data() : nullptr, elements.data(), types.data(), dense ? nullptr : widths.data(), ldx.data(), ldy.data(),
-                    limited ? (float)limit : std::numeric_limits<float>::infinity(), static_cast<float*>(norm.data_ptr()), ws.data_ptr(), ws.numel(), on.stream);
+                    max_norm, static_cast<float*>(norm.data_ptr()), ws.data_ptr(), ws.numel(), on.stream);
     }));
     if (limited)
       for (const at::Tensor& t : apart ? ys : xs) changed(t);

@@ -248,3 +248,11 @@ def test_limits_far_below_the_norm(lm, dtype, scale, limit):
     for o, b in zip(outs, before):
         exact = b.double() * (limit / want)
         assert bool(((o.double() - exact).abs() <= exact.abs() * (6 * U + torch.finfo(dtype).eps / 2) + least).all())
+
+
+@pytest.mark.gpu
+def test_limits_beyond_fp32(lm):
+    """Finite in a Python number: outputs are written, and nothing is over such a limit."""
+    x, out = torch.full((9,), 1e38, device="cuda"), torch.zeros(9, device="cuda")
+    assert abs(float(lm.clip([x], 1e39, out=[out])) - 3e38) <= 3e38 * 5 * U and torch.equal(out, x)
+    assert float(lm.clip([x], 3.5e38)) < math.inf and bool((x == 1e38).all())

@@ -208,14 +208,14 @@ def norm(x, weight=None, residual=None, eps=1e-6, total=None, out=None):
     """`t / sqrt(mean of t's squares + eps) * weight` for each row of t = x, or of t = x + residual rounded to their type: then
     (norm, t), t to be added to by what comes next and for `norm_grad`. weight: one element per column, of the matrices' type or
     float32. `total` (t) and `out` may be given to be written to."""
-    return _native().norm(x, weight, residual, eps, total, out, None)
+    return _native().norm(x, weight, residual, eps, total, out, False, 0)
 
 
 def norm_e4m3(x, weight=None, residual=None, eps=1e-6, block=128, total=None):
     """The same with its result in 8 bits, to stand in front of a product of such operands: (q, scales), or (q, scales, t) with a
     residual. q is float8_e4m3fn, and q * scale the norm: a float32 scale for each `block` = 128 columns, or for each row
     (block = 0), rows x scales. Gradients are those of `norm` (norm_grad)."""
-    return _native().norm(x, weight, residual, eps, total, None, block)
+    return _native().norm(x, weight, residual, eps, total, None, True, block)
 
 
 def norm_grad(dy, t, weight=None, dtotal=None, eps=1e-6, dx=None):

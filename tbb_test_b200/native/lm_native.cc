@@ -145,15 +145,15 @@ PyObject* guarded(Py_ssize_t given_args, Py_ssize_t wanted, Body body) {
   return nullptr;
 }
 
-// x, weight, residual, eps, total, out, block (None: an output of x's type)
+// x, weight, residual, eps, total, out, e4m3 (False: an output of x's type), block (of e4m3 only)
 PyObject* norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-  return guarded(n_args, 7, [&]() -> PyObject* {
+  return guarded(n_args, 8, [&]() -> PyObject* {
+    const bool e4m3 = a[6] == Py_True;
+    const long block = e4m3 ? integer(a[7]) : 0;
     const at::Tensor& x = tensor("x", a[0]);
     const Matrix mx = matrix("x", x);
     const auto [pw, wt] = weight_of(a[1], x);
     const double eps = number(a[3]);
-    const bool e4m3 = given(a[6]);
-    const long block = e4m3 ? integer(a[6]) : 0;
     if (block != 0 && block != 128) refuse("block: " + std::to_string(block) + ", wanted 0 or 128");
     Matrix mr, mt, mo;
     at::Tensor total, out, scales;

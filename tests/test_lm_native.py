@@ -31,3 +31,11 @@ def test_numbers_have_to_be_numbers(lm):
     for call in (lambda: lm._native().norm(x), lambda: lm._native().clip(x, 1.0, None, None), lambda: lm.clip([x], "much")):
         with pytest.raises(TypeError):
             call()
+
+
+def test_an_8_bit_norm_without_a_block_is_refused(lm):
+    """None is no number of columns, nor a norm in the type of x."""
+    x = torch.zeros(4, 8)
+    for block in (None, "128", 128.0):
+        with pytest.raises(TypeError):
+            lm.norm_e4m3(x, block=block)

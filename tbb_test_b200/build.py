@@ -9,7 +9,8 @@ Outputs (git-ignored, next to their sources):
                                         Partition / TwistedHyperCube / driver code
     tbb_test_b200/host/mlp_cuda         driver binary (counterpart of mlp_omp)
     tbb_test_b200/native/_lm_native.so  calls of the operators in lm.py on torch tensors
-                                        (built where torch is installed)
+                                        (built where torch for CUDA and the headers that it
+                                        takes are installed; nothing else needs it)
 """
 import glob
 import importlib.util
@@ -94,10 +95,17 @@ def build_native(force=False, verbose=False):
         return NATIVE
     torch_dir = os.path.dirname(spec.origin)
     lib, inc = os.path.join(torch_dir, "lib"), os.path.join(torch_dir, "include")
-    cuda = os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")
+    cuda, py = os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include"), sysconfig.get_paths()["include"]
+    libs = ["c10", "c10_cuda", "torch_cpu", "torch_cuda", "torch_python"]
+    wanted = [os.path.join(lib, f"lib{x}.so") for x in libs] + [os.path.join(inc, "torch", "csrc", "autograd", "python_variable.h"),
+                                                               os.path.join(py, "Python.h"), os.path.join(cuda, "cuda_runtime_api.h")]
+    lacking = [x for x in wanted if not os.path.exists(x)]
+    if lacking:
+        print(f"{NATIVE} is not built, and norm, clip and sample of tbb_test_b200.lm cannot be called: there is no " + ", no ".join(lacking), file=sys.stderr, flush=True)
+        return None
+    import torch
     _run([CXX, "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-I", inc, "-I", os.path.join(inc, "torch", "csrc", "api", "include"), "-I", cuda,
-          "-I", sysconfig.get_paths()["include"], "-D_GLIBCXX_USE_CXX11_ABI=1", "-o", NATIVE, src, "-L", lib, "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
-          "-ltorch_python", "-Wl,-rpath," + lib], verbose)
+          "-I", py, f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-o", NATIVE, src, "-L", lib, *["-l" + x for x in libs], "-Wl,-rpath," + lib], verbose)
     return NATIVE
 
 

@@ -657,20 +657,17 @@ template <typename T, int VB>
 void norm_grad_launch(const NormGradArgs& a, double* rms_of, void* dweight, int sms, Chain& chain) {
   constexpr int N = VB / (int)sizeof(T), MOST_K = N >= 8 ? 4 : 8;
   // two vectors per thread share the row's reduction and leave registers for the next row's loads (65536 x 1024 bf16 101 us, with one 118, with four and no loads ahead 217);
-  // 1024 threads have 64 registers each: half as many elements
+  // 1024 threads have 64 registers each: half as many elements. 256 threads with more than two vectors have MOST_K, and 1024 threads half of that: rows that fewer hold go to fewer threads
   RowForm f = row_form(1, a.width / N, 2, 1, NORM_THREADS, 0);
   if (!f.k) f = row_form(1, a.width / N, MOST_K, 1, NORM_THREADS, 0);
   if (!f.k) f = row_form(1, a.width / N, MOST_K / 2, 1, ROW_MOST_THREADS, 0);
   int parts = 0;
   if (f.k && f.threads > NORM_THREADS) {
-    if (f.k == 1) parts = grad_rows<T, VB, 1, ROW_MOST_THREADS>(a, f, sms, chain);
-    else if (f.k == 2) parts = grad_rows<T, VB, 2, ROW_MOST_THREADS>(a, f, sms, chain);
-    else if constexpr (MOST_K == 8) parts = grad_rows<T, VB, 4, ROW_MOST_THREADS>(a, f, sms, chain);
+    parts = grad_rows<T, VB, MOST_K / 2, ROW_MOST_THREADS>(a, f, sms, chain);
   } else if (f.k) {
     if (f.k == 1) parts = grad_rows<T, VB, 1, NORM_THREADS>(a, f, sms, chain);
     else if (f.k == 2) parts = grad_rows<T, VB, 2, NORM_THREADS>(a, f, sms, chain);
-    else if (f.k == 4) parts = grad_rows<T, VB, 4, NORM_THREADS>(a, f, sms, chain);
-    else if constexpr (MOST_K == 8) parts = grad_rows<T, VB, 8, NORM_THREADS>(a, f, sms, chain);
+    else parts = grad_rows<T, VB, MOST_K, NORM_THREADS>(a, f, sms, chain);
   } else {
     parts = a.rows < COLUMN_SLICES ? (int)a.rows : COLUMN_SLICES;
     chain.launch(norm_grad_long_kernel<T>, dim3((unsigned int)a.rows), ROW_MOST_THREADS, 0, 0, a, rms_of);

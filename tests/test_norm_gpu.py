@@ -294,3 +294,39 @@ def test_c_entries_refuse_before_any_device_work(native):
     for kw in (dict(dtype=2), dict(wt=1), dict(width=0), dict(eps=-1.0), dict(w=None), dict(dy=None), dict(t=None), dict(dx=None), dict(ws=None), dict(ldy=7), dict(ldt=7),
                dict(ldm=7), dict(ldx=7), dict(dy=p(1)), dict(dw=p(2)), dict(ws=p(64)), dict(ws_bytes=100)):
         assert lib.b2_norm_grad(*{**good, **kw}.values()) == K.ERR_INVALID, kw
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("width", [v * n for n in (1, 2, 4, 8) for v in (1, 512, 513, 2048, 2049, 4095, 4097)])
+def test_gradients_at_the_ends_of_their_forms(lm, dtype, width):
+    """Rows of so many vectors of 1, 2, 4 or 8 elements: as many as 256 threads hold with two each or with all that they may, 1024 threads, and one more."""
+    test_gradients(lm, dtype, 3, width, width, 0, "fp32", True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("width", [203, 1024, 40000])
+@pytest.mark.parametrize("block", [0, 128])
+def test_e4m3_of_infinite_elements_and_over_the_whole_range(lm, dtype, width, block):
+    """Norms of 1e-38 to 1e38 by their weights. A block with an infinite norm has an infinite scale, behind which the finite ones are 0; NaN stays where it is and scales nothing."""
+    x = _rows(4, width, dtype, 1).contiguous()
+    w = torch.ones(width, device="cuda")
+    for factor in (1e-38, 1e-30, 1e30, 2e36):
+        q, scales = lm.norm_e4m3(x, w * factor, block=block)
+        y = _exact(x, w * factor, float(torch.tensor(1e-6)))[0]
+        s = scales.double().repeat_interleave(block or width, 1)[:, :width]
+        assert bool(torch.isfinite(scales).all())
+        # three bits behind the leading one, or half of 2^-9 scales below 2^-6 of them; y's own 9 u and the scale's 10 u
+        assert bool(((q.double() * s - y).abs() <= y.abs() * (2.0 ** -4 + 20 * U) + 2.0 ** -10 * s * (1 + 20 * U)).all())
+    clean_q, clean_s = lm.norm_e4m3(x, w, block=block)
+    bad = w.clone()
+    bad[3], bad[7] = math.inf, math.nan
+    q, scales = lm.norm_e4m3(x, bad, block=block)
+    here = block or width
+    assert bool(torch.isinf(scales[:, 0]).all()) and torch.equal(scales[:, 1:], clean_s[:, 1:]) and torch.equal(q[:, here:].float(), clean_q[:, here:].float())
+    first = q[:, :min(here, width)].float()
+    assert bool(torch.isnan(first[:, [3, 7]]).all()) and not first[:, :3].any() and not first[:, 8:].any()
+    bad[3] = 1.0
+    q, scales = lm.norm_e4m3(x, bad, block=block)
+    assert bool(torch.isfinite(scales).all()) and bool(torch.isnan(q.float()[:, 7]).all()) and int(torch.isnan(q.float()).sum()) == 4

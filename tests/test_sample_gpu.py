@@ -353,3 +353,38 @@ def test_top_k_among_tokens_of_hardly_any_weight(lm, dtype, vocab, ld, offset, k
         u = torch.full((6,), value, device="cuda")
         for s in (dict(t=0.01), dict(t=0.005), dict(t=0.01, p=0.9), dict(t=0.01, m=1e-30), dict(t=[0.01, 0.008, 0.02, 0.01, 0.01, 0.04])):
             _check_both(lm, x, u, k=k, **s, exact=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("vocab,ld,offset,spread", [(1, 1, 0, 2.5), (700, 701, 1, 2.5), (9001, 9004, 3, 0.3), (9001, 9004, 3, 9.0), (70001, 70003, 1, 2.5), (70001, 70008, 0, 9.0), (600011, 600011, 0, 0.3)])
+def test_rows_without_a_limit_beside_others(lm, dtype, vocab, ld, offset, spread):
+    """Settings by row, where some rows have no limit: with log probabilities and without, over tiles that are masked by -inf or by the type's lowest value, and with more tiles than
+    threads."""
+    n = 12
+    x, u = _logits(n, vocab, dtype, 15, spread, ld, offset)
+    tile = torch.arange(vocab, device="cuda") // 1024
+    if vocab > 5000:
+        x[1, tile % 3 != 1] = -math.inf
+        x[2, tile % 2 == 0] = torch.finfo(dtype).min
+        x[3, :vocab - 5] = -math.inf
+        x[5, tile < tile[-1] // 2] = -30.0 - spread * 10
+    pick = lambda values: [values[i % len(values)] for i in range(n)]  # noqa: E731
+    k, p, m = [0] * 9 + [20, 0, 0], [1.0] * 10 + [0.9, 1.0], [0.0] * 11 + [0.05]
+    _check_both(lm, x, u, t=pick([1.0, 0.5, 1.0, 2.0, 0.25]), k=k, p=p, m=m)
+    _check_both(lm, x, u, t=pick([1.0, 0.0, math.nan, 1e30, 1e-30]), p=p, exact=True)
+    _check_both(lm, x, u, m=m)
+    many = torch.rand(n, device="cuda", generator=torch.Generator(device="cuda").manual_seed(16))
+    _check_both(lm, x, many, k=k, p=p)
+
+
+@pytest.mark.gpu
+def test_log_probabilities_over_the_whole_range_of_fp32_powers(lm):
+    """The bound of fp32 weights: two tokens in different tiles, the second of them as a power of two with a fraction anywhere in +-1/2, against the logarithm in 64 bits."""
+    n = 1 << 14
+    x = torch.full((n, 1100), -math.inf, device="cuda")
+    x[:, 0] = 0.0
+    x[:, 1050] = -torch.linspace(1e-4, 2.1, n, device="cuda")
+    tokens, lp = lm.sample(x, torch.zeros(n, device="cuda"), logprob=True)
+    want = -torch.log1p(torch.exp(x[:, 1050].double()))
+    assert not tokens.any() and bool(((lp.double() - want).abs() <= 2.0 ** -24 * want.abs() + 3.5e-7).all())

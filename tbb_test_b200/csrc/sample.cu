@@ -24,9 +24,10 @@
 // fp64, some 30 instructions; but where all tokens of a row count (no limit, or top-p's whole weight), first in fp32, 8 instructions, with a bound of the
 // error: only where target and step are nearer than that, the row is summed once more in fp64.
 //
-// Measured on one B200 (a copy reaches 6.56 TB/s): 1024 rows of 65536 bf16 without a limit 60 us, of which the tiles take 40 (75 % of issue slots: 14 instructions per
-// logit; 3.4 TB/s) and the rows that fp32 leaves open, some 4 %, 20; 256 rows of 65536 with top-p 0.94 over a flat distribution (11 000 of the tokens kept) 125 us: a
-// block per row and 16 warps per SM, two rounds of 85 000 clocks, of which 26 000 gather tokens, 25 000 find the limit, 10 000 sum up and 17 000 estimate and confirm; one row of 32768 with top-k 50 16 us: latency of one block.
+// Measured on one B200 (a copy reaches 6.56 TB/s): 1024 rows of 65536 bf16 without a limit and with log probabilities 66 us, of which the tiles take 40 (75 % of issue slots: 14
+// instructions per logit; 3.4 TB/s), the rows that fp32 leaves open, some 4 %, 20, and the largest tokens' tiles in fp64 4; 256 rows of 65536 with top-p 0.94 over a flat distribution
+// (11 000 of the tokens kept) 122 to 132 us on several machines: a block per row and 16 warps per SM, two rounds of 85 000 clocks, of which 26 000 gather tokens, 25 000 find the limit,
+// 10 000 sum up and 17 000 estimate and confirm; one row of 32768 with top-k 50 16 to 18 us: latency of one block.
 #include <math.h>
 
 #include "lm.cuh"
@@ -210,7 +211,7 @@ struct Weights {
 
 // Weights in fp32 up to a factor that all of them share: 2^(x c - N) with c = log2(e) / T and N = rint(largest c), by the nearest integer n of x c and 2^(x c - n).
 // A sum of eight is off by at most 3.5e-7 of itself: 1.5e-7 for ex2.approx (the most over all numbers in +-0.51), 2e-8 for its argument, 2^-24 for each of
-// three additions. Two such sums are compared: SLACK is twice that and a third more.
+// three additions. Two such sums are compared: SLACK is twice that and a third more. (tests/test_sample_gpu.py compares log probabilities with this bound over powers in +-1/2.)
 constexpr double SLACK = 9.5367431640625e-7;          // 2^-20
 constexpr double SLACK_OF_ONE = 4.76837158203125e-7;  // 2^-21: such a sum against an exact one
 // Whether the token whose own weight lies between `before` and `before + weight` is the one at `goal` for sure, all relative to its tile's unit. Logits of less than 80 T below a
@@ -1435,7 +1436,7 @@ struct Sampler {
   }
 };
 
-// ------------------------------------------------------------------ calls without a limit: a warp per row (1024 rows of 65536 60 us, by a block per row 130)
+// ------------------------------------------------------------------ calls without a limit: a warp per row (1024 rows of 65536 62 us, by a block per row 130)
 
 constexpr int WHOLE_THREADS = 128;
 

@@ -227,7 +227,7 @@ def norm_grad(dy, t, weight=None, dtotal=None, eps=1e-6, dx=None):
 def clip(tensors, max_norm, out=None):
     """The norm of all elements of `tensors` together, a float32 scalar on their device; where it is over `max_norm`, the tensors are multiplied
     by max_norm / norm, in place or into the list `out` of tensors like them (which is always written). math.inf or None for max_norm: the
-    norm alone. A norm that is infinite or not a number leaves the values as they are. float32 and bfloat16 tensors of any sizes, each dense
+    norm alone. A norm that is infinite (in float32) or not a number leaves the values as they are. float32 and bfloat16 tensors of any sizes, each dense
     or a matrix with unit stride along its rows, all on one device; none may overlap another (see b2_clip in include/b200mlp.h)."""
     return _native().clip(tensors, max_norm, out)
 

@@ -492,7 +492,8 @@ int b2_clip(size_t count, const void* const* x, void* const* out, const size_t* 
  * four may be given for each row (device memory: row_...), in place of the one for all. A logit of -inf or NaN is never taken; a row of nothing else
  * gives token -1 and logprob 0. Logits of +inf share all the weight. u outside of [0, 1) counts as the nearer end, NaN as 1.
  * Where fp32 leaves the token open, weights are summed in fp64: it is the one of the formula unless u or a border lies within about 1e-11 of a step of
- * the running sum. Weights below e^-40 of the largest count as none where top_p's limit is looked for. Weights below 2^-1000 of the largest are none: such a token is not taken, not by a u of 0 or 1 either. logprob is off by 4e-7 at most, and half a step of fp32. Equal inputs give equal tokens. tokens are 32- or 64-bit integers
+ * the running sum. Weights below e^-40 of the largest count as none where top_p's limit is looked for. A token of less than 2^-1000 of the largest weight
+ * is never taken, not by a u of 0 or 1 either. logprob is off by 4e-7 at most, and half a step of fp32. Equal inputs give equal tokens. tokens are 32- or 64-bit integers
  * (token_bytes). Limits: rows and vocab at most 2^24 each. */
 typedef struct {
   float temperature;
